@@ -173,7 +173,7 @@ def _layer(heads, latent, rope, nope, value, bs, dtype):
 def _run_own(s):
     case = s["case"]
     op = _layer(*(case[k] for k in ("heads", "latent", "rope", "nope", "value", "bs", "dtype")))
-    inputs = {k: s[k] for k in ("cache", "past_lens", "subsequence_begins", "block_indices", "block_indices_begins", "max_context_len")}
+    inputs = {k: s[k] for k in ("cache", "past_lens", "subsequence_begins", "block_indices", "block_indices_begins")}
     Dn = case["nope"]
     if case["kind"] == "append":
         inputs.update(latent=s["latent"], norm_weight=s["norm_weight"], norm_eps=EPS, query_rope=s["query"][..., Dn:],
