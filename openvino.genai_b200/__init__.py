@@ -1,5 +1,5 @@
-"""B200-native per-step compute of a continuous-batching pipeline: the PagedAttention operator
-and the Sampler, as hand-written sm_100a CUDA behind a C ABI (include/*.h).
+"""B200-native per-step compute of a continuous-batching pipeline: the PagedAttention operator,
+latent attention and the Sampler, as hand-written sm_100a CUDA behind a C ABI (include/*.h).
 
 This Python layer is a thin host-side mirror of the operator / sampler interface used by tests
 and the benchmark.  It never computes anything itself: if the CUDA library is missing the
@@ -13,7 +13,7 @@ from pathlib import Path
 from . import _abi
 from .build import LIB_PATH, build_all
 
-__all__ = ["load_library", "library_path", "build_all", "PagedAttentionExtension", "GenaiB200Error"]
+__all__ = ["load_library", "library_path", "build_all", "PagedAttentionExtension", "LatentAttention", "GenaiB200Error"]
 
 _lib = None
 
@@ -44,8 +44,11 @@ def load_library(build_if_missing: bool = False) -> ctypes.CDLL:
     _abi.bind(lib, _exchange_abi.EXCHANGE_SYMBOLS)
     from . import _eviction_abi
     _abi.bind(lib, _eviction_abi.EVICTION_SYMBOLS)
+    from . import _latent_abi
+    _abi.bind(lib, _latent_abi.LATENT_SYMBOLS)
     _lib = lib
     return lib
 
 
 from .paged_attention import PagedAttentionExtension  # noqa: E402
+from .latent_attention import LatentAttention  # noqa: E402

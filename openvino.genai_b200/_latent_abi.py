@@ -1,0 +1,82 @@
+"""ctypes mirror of include/latent_b200.h (struct layouts and prototypes)."""
+from __future__ import annotations
+
+import ctypes as C
+
+PA_LATENT_AUTO = 0
+PA_LATENT_ABSORBED = 1
+PA_LATENT_EXPANDED = 2
+
+
+class pa_latent_desc(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32)] + [(n, C.c_int32) for n in (
+        "num_heads", "latent_size", "rope_size", "nope_size", "value_size", "block_size", "dtype")]
+
+
+class pa_latent_append_args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("latent", C.c_void_p),
+        ("latent_stride", C.c_int64),
+        ("norm_weight", C.c_void_p),
+        ("norm_eps", C.c_float),
+        ("query_rope", C.c_void_p),
+        ("query_rope_token_stride", C.c_int64),
+        ("query_rope_head_stride", C.c_int64),
+        ("query_rope_out", C.c_void_p),
+        ("query_rope_out_token_stride", C.c_int64),
+        ("query_rope_out_head_stride", C.c_int64),
+        ("rope_table", C.c_void_p),
+        ("rope_table_rows", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("positions", C.c_void_p),
+        ("num_tokens", C.c_int32),
+        ("cache", C.c_void_p),
+        ("num_blocks", C.c_int32),
+        ("past_lens", C.c_void_p),
+        ("subsequence_begins", C.c_void_p),
+        ("block_indices", C.c_void_p),
+        ("block_indices_begins", C.c_void_p),
+        ("num_sequences", C.c_int32),
+        ("num_block_indices", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class pa_latent_attention_args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("query_nope", C.c_void_p),
+        ("query_nope_token_stride", C.c_int64),
+        ("query_nope_head_stride", C.c_int64),
+        ("query_rope", C.c_void_p),
+        ("query_rope_token_stride", C.c_int64),
+        ("query_rope_head_stride", C.c_int64),
+        ("key_up", C.c_void_p),
+        ("key_up_head_stride", C.c_int64),
+        ("value_up", C.c_void_p),
+        ("value_up_head_stride", C.c_int64),
+        ("output", C.c_void_p),
+        ("num_tokens", C.c_int32),
+        ("cache", C.c_void_p),
+        ("num_blocks", C.c_int32),
+        ("past_lens", C.c_void_p),
+        ("subsequence_begins", C.c_void_p),
+        ("block_indices", C.c_void_p),
+        ("block_indices_begins", C.c_void_p),
+        ("num_sequences", C.c_int32),
+        ("num_block_indices", C.c_int32),
+        ("scale", C.c_float),
+        ("form", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+LATENT_SYMBOLS = {
+    "pa_b200_latent_create": (C.c_int, [C.POINTER(pa_latent_desc), C.c_int, C.POINTER(C.c_void_p)]),
+    "pa_b200_latent_destroy": (C.c_int, [C.c_void_p]),
+    "pa_b200_latent_append": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_append_args)]),
+    "pa_b200_latent_attention": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_attention_args)]),
+    "pa_b200_latent_last_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
+    "pa_b200_latent_launch_count": (C.c_int64, [C.c_void_p]),
+}

@@ -1,0 +1,106 @@
+// Internal launch interface of latent attention, between the C ABI (latent_api.cu) and the kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/latent_b200.h"
+#include "pa_common.cuh"
+
+namespace latent {
+
+// The step's paged metadata and the layer's sizes, passed by value.  All pointers are device memory.
+struct Step {
+    int H, R, P, Dn, Dv, bs;
+    int num_tokens, num_sequences, num_block_indices, num_blocks;
+    const int32_t* past_lens;
+    const int32_t* subsequence_begins;
+    const int32_t* block_indices;
+    const int32_t* block_indices_begins;
+    uint32_t* status;
+};
+
+struct AppendArgs {
+    Step m;
+    const void* latent;
+    long long latent_stride;
+    const void* norm_weight;
+    float norm_eps;
+    const void* q_in;
+    long long q_in_token, q_in_head;
+    void* q_out;
+    long long q_out_token, q_out_head;
+    const float* rope_table;
+    int rope_rows;
+    int interleaved;
+    const int32_t* positions;
+    void* cache;
+};
+
+struct AttentionArgs {
+    Step m;
+    const void* q_nope;
+    long long qn_token, qn_head;
+    const void* q_rope;
+    long long qr_token, qr_head;
+    const void* key_up;
+    long long key_up_head;
+    const void* value_up;
+    long long value_up_head;
+    void* output;
+    const void* cache;
+    float scale;
+};
+
+cudaError_t launch_append(const AppendArgs& a, int dtype, cudaStream_t stream, int* launches);
+cudaError_t launch_attention_simple(const AttentionArgs& a, int dtype, cudaStream_t stream, int* launches);
+
+#ifdef __CUDACC__
+// One sequence's slice of the metadata, checked before anything is indexed with it: begins monotone and inside the arrays they
+// index, past_len >= 0, and a block table long enough for past_len + new tokens.  A sequence that fails sets its status bit
+// and gets no work.
+struct SeqView {
+    int t0, n;      // its new tokens
+    int past;
+    int tb;         // its block table inside block_indices
+};
+__device__ __forceinline__ bool seq_view(const Step& m, int s, SeqView& v) {
+    const int t0 = m.subsequence_begins[s], t1 = m.subsequence_begins[s + 1];
+    const int tb = m.block_indices_begins[s], te = m.block_indices_begins[s + 1];
+    const int past = m.past_lens[s];
+    v = SeqView{0, 0, 0, 0};
+    if (t0 < 0 || t1 < t0 || t1 > m.num_tokens || tb < 0 || te < tb || te > m.num_block_indices) {
+        atomicOr(m.status, PA_DEV_BAD_BEGINS);
+        return false;
+    }
+    if (past < 0 || (long long)(te - tb) * m.bs < (long long)past + (t1 - t0)) {
+        atomicOr(m.status, PA_DEV_BAD_PAST_LEN);
+        return false;
+    }
+    v = SeqView{t0, t1 - t0, past, tb};
+    return true;
+}
+
+// The sequence that owns token t.  In a step of one token each that is sequence t, which two loads show; else a binary search.
+__device__ __forceinline__ int find_sequence(const Step& m, int t) {
+    if (t < m.num_sequences && m.subsequence_begins[t] == t && m.subsequence_begins[t + 1] == t + 1) return t;
+    int lo = 0, hi = m.num_sequences;   // begins[lo] <= t < begins[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (m.subsequence_begins[mid] <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Sequence and checked view of token t; false (with the status bit set) where the prefix sums leave it out.
+__device__ __forceinline__ bool token_view(const Step& m, int t, SeqView& v) {
+    if (!seq_view(m, find_sequence(m, t), v)) return false;
+    if (t < v.t0 || t >= v.t0 + v.n) {
+        atomicOr(m.status, PA_DEV_BAD_BEGINS);
+        return false;
+    }
+    return true;
+}
+#endif
+
+}  // namespace latent
