@@ -26,6 +26,9 @@
 extern "C" {
 #endif
 
+/* Device status bit, beside those of pa_b200.h: a bounded wait of an attention kernel ran out; the step's output is incomplete. */
+#define PA_DEV_WAIT_TIMEOUT_LATENT 0x10000000u
+
 /* Static attributes of one layer. */
 typedef struct pa_latent_desc {
     uint32_t struct_size; /* sizeof(pa_latent_desc)                                               */
@@ -110,6 +113,10 @@ int pa_b200_latent_create(const pa_latent_desc* desc, int device, pa_latent_hand
 int pa_b200_latent_destroy(pa_latent_handle* h);
 int pa_b200_latent_append(pa_latent_handle* h, const pa_latent_append_args* args);
 int pa_b200_latent_attention(pa_latent_handle* h, const pa_latent_attention_args* args);
+
+/* The handle's scratch grows when a call needs more (cudaMalloc, never inside a stream capture).  After reserve, attention calls of no more
+ * tokens, sequences and block indices, in the same or a narrower form, do not allocate. */
+int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices, int32_t form);
 
 /* Reads (and clears) the device status word; synchronises the device's work on it. */
 int pa_b200_latent_last_device_status(pa_latent_handle* h, uint32_t* status_bits);

@@ -77,6 +77,7 @@ LATENT_SYMBOLS = {
     "pa_b200_latent_destroy": (C.c_int, [C.c_void_p]),
     "pa_b200_latent_append": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_append_args)]),
     "pa_b200_latent_attention": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_attention_args)]),
+    "pa_b200_latent_reserve": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "pa_b200_latent_last_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
     "pa_b200_latent_launch_count": (C.c_int64, [C.c_void_p]),
 }

@@ -1,0 +1,678 @@
+// Latent attention in its absorbed form, on the 5th-generation tensor cores (tcgen05 + TMEM): query rows are moved into the latent space
+// (q~ = key_up^T q), attend over the paged latents as they lie in the cache, and the sums of latents go through value_up.
+//   project_query   q~ per head, and the plan of the attention (first CTA)
+//   attend          split over the context: every CTA an equal slice of all (row tile, context tile) units
+//   combine         joins the partial results of a row
+//   project_value   output per head
+#include <algorithm>
+
+#include "latent_tc.cuh"
+
+namespace latent {
+
+namespace {
+
+// ---- the plan --------------------------------------------------------------------------------------------------------
+struct SeqPlan {
+    int blocks;          // row blocks
+    long long tiles;     // context tiles of each
+};
+__device__ __forceinline__ SeqPlan seq_plan(const AbsorbedArgs& a, int s) {
+    SeqView v;
+    if (!seq_view(a.m, s, v) || v.n == 0 || v.n > a.max_new) return SeqPlan{0, 0};
+    const int rows = kTile * a.row_tiles;
+    return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTile - 1) / kTile};
+}
+
+// Exclusive prefix sums over the sequences, by one block of 128 threads.
+__device__ void build_plan(const AbsorbedArgs& a) {
+    __shared__ long long sh_u[4], run_u;
+    __shared__ int sh_b[4], run_b;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = a.m.num_sequences;
+    if (tid == 0) { run_u = 0; run_b = 0; }
+    __syncthreads();
+    for (int base = 0; base < B; base += 128) {
+        const int s = base + tid;
+        const SeqPlan p = s < B ? seq_plan(a, s) : SeqPlan{0, 0};
+        long long u = p.blocks * p.tiles;
+        int b = p.blocks;
+        const long long mine_u = u;
+        const int mine_b = b;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long pu = __shfl_up_sync(0xffffffffu, u, o);
+            const int pb = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) { u += pu; b += pb; }
+        }
+        if (lane == 31) { sh_u[wid] = u; sh_b[wid] = b; }
+        __syncthreads();
+        long long off_u = run_u;
+        int off_b = run_b;
+        for (int w = 0; w < wid; ++w) { off_u += sh_u[w]; off_b += sh_b[w]; }
+        if (s < B) { a.unit_prefix[s] = off_u + u - mine_u; a.block_prefix[s] = off_b + b - mine_b; }
+        __syncthreads();
+        if (tid == 127) { run_u = off_u + u; run_b = off_b + b; }
+        __syncthreads();
+    }
+    if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; }
+}
+
+// Units of a group's slice.
+__device__ __forceinline__ long long slice_size(const AbsorbedArgs& a) {
+    const long long total = a.unit_prefix[a.m.num_sequences];
+    return total > 0 ? (total + a.groups - 1) / a.groups : 1;
+}
+
+// Which of the tile's tokens belong to sequences of this form; false (for the whole block) if none does.
+__device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&live)[kTile]) {
+    bool mine = false;
+    if (threadIdx.x < kTile) {
+        SeqView v;
+        mine = t0 + (int)threadIdx.x < a.m.num_tokens && token_view(a.m, t0 + threadIdx.x, v) && v.n <= a.max_new;
+        live[threadIdx.x] = mine;
+    }
+    return __syncthreads_or(mine) != 0;
+}
+
+// ---- q~ = key_up^T q ----------------------------------------------------------------------------------------------------
+// A CTA computes 128 latent elements of 64 tokens of one head: D[latent][token] with the weight's rows (d, latent contiguous) as an
+// MN-major operand, one tile of each operand, so the CTAs of an SM overlap one another's loads, products and stores.
+template <bool BF>
+__global__ void __launch_bounds__(128) project_query_kernel(const __grid_constant__ AbsorbedArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full, done;
+    __shared__ bool live[kTile];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag;
+    const Step& m = a.m;
+    if (blockIdx.x == 0) {
+        build_plan(a);
+        return;
+    }
+    const int parts = m.R / 128, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int i = blockIdx.x - 1, part = i % parts, h = i / parts % m.H, t0 = i / parts / m.H * kTile;
+    if (!tile_rows(a, t0, live)) return;
+    uint8_t* const sw = smem;                        // two atoms of [Dn][64 latent elements]
+    uint8_t* const sq = smem + 2 * m.Dn * 128;       // Dn / 64 atoms of [64 tokens][64 elements]
+    if (tid == 0) {
+        pa::mbar_init(&full, 1);
+        pa::mbar_init(&done, 1);
+        pa::mbar_fence_init();
+        abort_flag = 0;
+        pa::mbar_expect_tx(&full, 2 * m.Dn * 128 + m.Dn / 64 * 8192);
+        for (int c = 0; c < 2; ++c) tma_3d(sw + c * m.Dn * 128, &a.map_key_up, part * 128 + c * 64, 0, h, &full);
+        for (int c = 0; c < m.Dn / 64; ++c) tma_3d(sq + c * 8192, &a.map_qn, c * 64, h, t0, &full);
+    }
+    if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    tc05::fence_after_thread_sync();
+    const Waiter wt{&abort_flag, m.status};
+    const uint32_t tmem = tmem_base;
+    bool ok = wt.wait(&full, 0);
+    if (warp == 0 && __all_sync(0xffffffffu, ok)) {
+        constexpr uint32_t idesc = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
+        const uint64_t da = tc05::smem_desc_sw128(pa::smem_u32(sw), 1024, m.Dn * 128), db = tc05::smem_desc_sw128(pa::smem_u32(sq), 1024);
+        if (tc05::elect_one()) {
+            for (int kk = 0; kk < m.Dn / 16; ++kk)
+                tc05::mma_ss(tmem, da + 128 * kk, db + ((kk >> 2) * 8192 + (kk & 3) * 32 >> 4), idesc, kk > 0);
+            tc05::commit(&done);
+        }
+    }
+    if (part == 0) {   // the rotated part goes along as it is
+        const int pieces = m.P / 8;
+        for (int u = tid; u < kTile * pieces; u += 128) {
+            const int t = t0 + u / pieces, c = u % pieces;
+            if (t < m.num_tokens)
+                *reinterpret_cast<uint4*>((uint16_t*)a.q_abs + ((long long)t * m.H + h) * (m.R + m.P) + m.R + 8 * c) =
+                    *reinterpret_cast<const uint4*>((const uint16_t*)a.q_rope + t * a.qr_token + h * a.qr_head + 8 * c);
+        }
+    }
+    ok = ok && wt.wait(&done, 0);
+    tc05::fence_after_thread_sync();
+    if (__all_sync(0xffffffffu, ok)) {
+        uint16_t* dst = (uint16_t*)a.q_abs + ((long long)t0 * m.H + h) * (m.R + m.P) + part * 128 + tid;
+#pragma unroll
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+            uint32_t r[32];
+            tc05::ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
+            tc05::wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (live[c0 + c]) dst[(long long)(c0 + c) * m.H * (m.R + m.P)] = pack1<BF>(__uint_as_float(r[c]));
+        }
+    }
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    if (warp == 0) tc05::tmem_dealloc(tmem, 64);
+    (void)lane;
+}
+
+// ---- attention over the latents ------------------------------------------------------------------------------------------
+// Roles meet through mbarriers only: a loader warp walks the slice and has the TMA engine bring query rows and 64-token tiles of the cache,
+// one warp issues the products, four warps (64 rows, 16 a warp) do the softmax and write the partial results.
+//   S[row][token]     = Q~ K^T          M 64, N 64, K R + P; two buffers, so that S of the next tile is computed beside a softmax
+//   O^T[latent][row] += K^T P^T         M 128 (R / 128 times), N 64, K 64: the tile is read MN-major from the same image, and the
+//                                       rows (heads) are columns, so few heads leave no tensor-memory lane idle
+constexpr int kSlots = 4;               // depth of the queue of runs
+constexpr int kThreads = 192;           // warps 0 - 3: softmax, 4: loader, 5: products
+constexpr float kLazy = 4.f;            // log2 of the growth of a row maximum that rescales O
+
+// A stretch of context tiles of one row tile.
+struct Run {
+    int rows;            // rows of the tile, 0: no more runs
+    int row0;            // its first row among the sequence's (token, head) rows
+    long long grow0;     // and among the step's
+    int past;
+    int first, tiles;    // context tiles
+    int end;             // context the tile's last row sees
+    int tb;
+    long long slot;
+};
+
+template <int R>
+struct AttendSmem {
+    static constexpr int NC = R / 64 + 1;           // 64-element chunks of a row, the last one the rotated part
+    static constexpr int NST = R == 512 ? 2 : 4;    // context tiles in flight
+    alignas(1024) uint8_t q[NC][kTile * 128];
+    alignas(1024) uint8_t k[NST][NC][kTile * 128];
+    alignas(1024) uint8_t p[kTile * 128];           // [row][token]
+    float alpha[2][kTile];
+    volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
+    uint64_t k_full[NST], k_free[NST];              // loader -> products (bytes), products -> loader
+    uint64_t q_full, q_free;
+    uint64_t vote;                                  // softmax warps among themselves
+    uint64_t s_full[2], p_full, o_done;             // products -> softmax, softmax -> products, products -> softmax
+    uint64_t run_full[kSlots], run_free[kSlots];
+    Run run[kSlots];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int R, bool BF>
+__global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AbsorbedArgs a) {
+    using Smem = AttendSmem<R>;
+    constexpr int NC = Smem::NC, NST = Smem::NST, MT = R / 128;
+    constexpr uint32_t kTmemS = MT * kTile;         // O^T: MT x 64 columns, then S twice
+    extern __shared__ uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const Step& m = a.m;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < NST; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
+        pa::mbar_init(&sm.q_full, 1);
+        pa::mbar_init(&sm.q_free, 1);
+        pa::mbar_init(&sm.s_full[0], 1);
+        pa::mbar_init(&sm.s_full[1], 1);
+        pa::mbar_init(&sm.vote, 4);
+        pa::mbar_init(&sm.p_full, 4);
+        pa::mbar_init(&sm.o_done, 1);
+        for (int i = 0; i < kSlots; ++i) { pa::mbar_init(&sm.run_full[i], 1); pa::mbar_init(&sm.run_free[i], 5); }
+        pa::mbar_fence_init();
+        sm.grew[0] = sm.grew[1] = 0;
+        sm.abort_flag = 0;
+    }
+    if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    tc05::fence_after_thread_sync();
+    const uint32_t tmem = sm.tmem_base;
+    const Waiter wt{&sm.abort_flag, m.status};
+    // The next run of the queue; false: a wait ran out.
+    auto fetch = [&](uint32_t n, Run& r) -> bool {
+        const int slot = n % kSlots;
+        if (!wt.wait_warp(&sm.run_full[slot], (n / kSlots) & 1)) return false;
+        r = sm.run[slot];
+        warp_arrive(&sm.run_free[slot]);
+        return true;
+    };
+
+    if (warp == 4) {
+        // ======================= loader =================================================================
+        const int group = blockIdx.x / a.row_tiles, member = blockIdx.x % a.row_tiles, B = m.num_sequences;
+        const long long per = slice_size(a), total = a.unit_prefix[B];
+        long long u = group * per;
+        const long long u_end = min(total, u + per);
+        uint32_t n = 0, nr = 0, nq = 0;      // tiles, queue entries, query tiles so far
+        bool ok = true, bad_index = false;
+        if (lane == 0) { prefetch_map(&a.map_cache); prefetch_map(&a.map_q_abs); }
+        int s = 0;
+        if (u < u_end) {
+            int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.unit_prefix[mid] <= u) lo = mid; else hi = mid;
+            }
+            s = lo;
+        }
+        auto publish = [&](const Run& r) -> bool {
+            const int slot = nr % kSlots;
+            if (nr >= kSlots && !wt.wait_warp(&sm.run_free[slot], (nr / kSlots - 1) & 1)) return false;
+            if (lane == 0) sm.run[slot] = r;
+            warp_arrive(&sm.run_full[slot]);
+            ++nr;
+            return true;
+        };
+        while (ok && u < u_end) {
+            SeqView v;
+            seq_view(m, s, v);
+            const long long rel = u - a.unit_prefix[s];
+            const int tiles = (int)(((long long)v.past + v.n + kTile - 1) / kTile);
+            const int block = (int)(rel / tiles), first = (int)(rel % tiles);
+            const int len = (int)min((long long)(tiles - first), u_end - u);
+            Run r;
+            r.row0 = (block * a.row_tiles + member) * kTile;
+            r.rows = (int)min((long long)kTile, (long long)v.n * m.H - r.row0);
+            if (r.rows > 0) {
+                r.grow0 = (long long)v.t0 * m.H + r.row0;
+                r.past = v.past;
+                r.end = v.past + (r.row0 + r.rows - 1) / m.H + 1;
+                r.first = first;
+                r.tiles = max(0, min(first + len, (r.end + kTile - 1) / kTile) - first);
+                r.tb = v.tb;
+                r.slot = ((long long)a.block_prefix[s] + block + group) * a.row_tiles + member;
+                ok = publish(r);
+                if (ok && r.tiles > 0) {
+                    if (nq > 0) ok = wt.wait_warp(&sm.q_free, (nq - 1) & 1);
+                    if (ok && lane == 0) {
+                        const int pieces = (r.rows + 15) / 16;   // of 16 rows
+                        pa::mbar_expect_tx(&sm.q_full, pieces * 16 * 128 * NC);
+                        for (int c = 0; c < NC; ++c)
+                            for (int i = 0; i < pieces; ++i) tma_2d(sm.q[c] + i * 2048, &a.map_q_abs, 64 * c, (int)r.grow0 + 16 * i, &sm.q_full);
+                    }
+                    ++nq;
+                    const int per_tile = kTile / m.bs, last_block = (r.end - 1) / m.bs;
+                    int page = 0, base = -1;     // this lane's block of the 32 from `base`
+                    for (int j = 0; ok && j < r.tiles; ++j, ++n) {
+                        const int b0 = (r.first + j) * per_tile, blocks = min(per_tile, last_block - b0 + 1);
+                        if (base < 0 || b0 + per_tile > base + 32) {
+                            base = b0;
+                            page = 0;
+                            if (base + lane <= last_block) {
+                                page = m.block_indices[r.tb + base + lane];
+                                if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
+                            }
+                        }
+                        const int st = n % NST;
+                        if (n >= NST) ok = wt.wait_warp(&sm.k_free[st], (n / NST - 1) & 1);
+                        if (ok && lane == 0) pa::mbar_expect_tx(&sm.k_full[st], blocks * m.bs * 128 * NC);
+                        for (int i = 0; i < blocks; ++i) {
+                            const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * m.bs;
+                            if (ok && lane == 0)
+                                for (int c = 0; c < NC; ++c) tma_2d(sm.k[st][c] + i * m.bs * 128, &a.map_cache, 64 * c, at, &sm.k_full[st]);
+                        }
+                    }
+                }
+            }
+            u += len;
+            while (s < B && u >= a.unit_prefix[s + 1]) ++s;
+        }
+        if (ok) {
+            Run r{};
+            publish(r);
+        }
+        if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
+        // what was issued has to have arrived before the CTA's memory is given back
+        if (sm.abort_flag) {
+            for (uint32_t k = 0; nq > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.q_full, (nq - 1) & 1); ++k) {}
+            for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i)
+                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.k_full[i % NST], (i / NST) & 1); ++k) {}
+        }
+    } else if (warp == 5) {
+        // ======================= products ================================================================
+        constexpr uint32_t idesc_s = tc05::instr_desc_f16(kTile, kTile, BF ? 1 : 0, 0, 0);
+        constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
+        const uint64_t dq = tc05::smem_desc_sw128(pa::smem_u32(sm.q), 1024), dk = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024);
+        const uint64_t dv = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024, kTile * 128), dp = tc05::smem_desc_sw128(pa::smem_u32(sm.p), 1024);
+        constexpr uint32_t kStage = NC * kTile * 128 >> 4;
+        const int last_steps = m.P / 16;
+        uint32_t n = 0;
+        bool ok = true;
+        Run r;
+        for (uint32_t nr = 0, nq = 0; ok; ++nr) {
+            if (!fetch(nr, r) || r.rows == 0) break;
+            if (r.tiles == 0) continue;
+            ok = wt.wait_warp(&sm.q_full, nq & 1);
+            ++nq;
+            const uint32_t end = n + r.tiles;
+            uint32_t next_s = n, next_o = n;
+            uint32_t idle = 0;
+            // S of a tile as soon as the tile is there, but no more than one ahead of O; O as soon as its P is
+            while (ok && next_o < end) {
+                if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, pa::mbar_try_wait(&sm.k_full[next_s % NST], (next_s / NST) & 1))) {
+                    const uint64_t db = dk + (next_s % NST) * kStage;
+                    const uint32_t d = tmem + kTmemS + (next_s & 1) * kTile;
+                    tc05::fence_after_thread_sync();
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < R / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2;
+                            if (kk == 0) tc05::mma_ss<0>(d, dq + off, db + off, idesc_s);
+                            else tc05::mma_ss<1>(d, dq + off, db + off, idesc_s);
+                        }
+                        for (int kk = 0; kk < last_steps; ++kk) {
+                            const uint32_t off = (R / 64) * (kTile * 128 >> 4) + kk * 2;
+                            tc05::mma_ss<1>(d, dq + off, db + off, idesc_s);
+                        }
+                        tc05::commit(&sm.s_full[next_s & 1]);
+                        if (next_s + 1 == end) tc05::commit(&sm.q_free);
+                    }
+                    __syncwarp();
+                    ++next_s;
+                    idle = 0;
+                } else if (next_o < next_s && __all_sync(0xffffffffu, pa::mbar_try_wait(&sm.p_full, next_o & 1))) {
+                    const uint64_t da = dv + (next_o % NST) * kStage;
+                    const uint32_t acc = next_o > n ? 1u : 0u;
+                    tc05::fence_after_thread_sync();
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int kk = 0; kk < kTile / 16; ++kk)
+                                tc05::mma_ss(tmem + mt * kTile, da + mt * 2 * (kTile * 128 >> 4) + kk * 128, dp + kk * 2, idesc_o, kk > 0 ? 1u : acc);
+                        tc05::commit(&sm.k_free[next_o % NST]);
+                        tc05::commit(&sm.o_done);
+                    }
+                    __syncwarp();
+                    ++next_o;
+                    idle = 0;
+                } else if (++idle > (1u << 21)) {
+                    wt.give_up();
+                    ok = false;
+                } else if ((idle & 255u) == 255u && __any_sync(0xffffffffu, sm.abort_flag)) {
+                    ok = false;
+                }
+            }
+            n = end;
+        }
+    } else {
+        // ======================= softmax and partial results ==============================================
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int rl[2] = {16 * warp + lane / 4, 16 * warp + lane / 4 + 8};
+        const float c2 = a.scale_log2;
+        uint32_t n = 0;
+        Run r;
+        for (uint32_t nr = 0;; ++nr) {
+            if (!fetch(nr, r) || r.rows == 0) break;
+            int limit[2];          // context each of the thread's two rows sees
+            float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) limit[x] = rl[x] < r.rows ? r.past + (r.row0 + rl[x]) / m.H + 1 : 0;
+            bool ok = true;
+            for (int j = 0; j < r.tiles; ++j, ++n) {
+                if (!wt.wait_warp(&sm.s_full[n & 1], (n >> 1) & 1)) { ok = false; break; }
+                tc05::fence_after_thread_sync();
+                uint32_t raw[32];
+                ld_16x256b_x8(tmem + kTmemS + (n & 1) * kTile + lanes, raw);
+                tc05::wait_ld();
+                float sv[2][16];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sv[e >> 1][2 * i + (e & 1)] = __uint_as_float(raw[4 * i + e]) * c2;
+                const int col0 = (r.first + j) * kTile;
+                float alpha[2] = {1.f, 1.f};
+                bool grew = false;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (col0 + kTile > limit[x]) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (col0 + 8 * (c >> 1) + 2 * (lane & 3) + (c & 1) >= limit[x]) sv[x][c] = -INFINITY;
+                    }
+                    float t = sv[x][0];
+#pragma unroll
+                    for (int c = 1; c < 16; ++c) t = fmaxf(t, sv[x][c]);
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    // (a row that has seen nothing yet takes its first maximum without a rescale: its O is zero)
+                    if (mx[x] == -INFINITY) mx[x] = t;
+                    else if (t > mx[x] + kLazy) { alpha[x] = ex2(mx[x] - t); mx[x] = t; grew = true; }
+                    if ((lane & 3) == 0) sm.alpha[n & 1][rl[x]] = alpha[x];
+                    const float ref = mx[x] == -INFINITY ? 0.f : mx[x];
+                    float sum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) { sv[x][c] = ex2(sv[x][c] - ref); sum += sv[x][c]; }
+                    l[x] = l[x] * alpha[x] + sum;
+                }
+                // the warps agree on a rescale (a barrier of the hardware could not be left when a wait runs out)
+                if (grew) sm.grew[n & 1] = n + 1;
+                warp_arrive(&sm.vote);
+                if (!wt.wait_warp(&sm.vote, n & 1)) { ok = false; break; }
+                const bool rescale = sm.grew[n & 1] == n + 1;
+                if (n > 0 && !wt.wait_warp(&sm.o_done, (n - 1) & 1)) { ok = false; break; }
+                tc05::fence_after_thread_sync();
+                if (rescale) {
+#pragma unroll 1
+                    for (int q = 0; q < MT * 2; ++q) {
+                        uint32_t o[32];
+                        tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
+                        tc05::wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * sm.alpha[n & 1][(q & 1) * 32 + c]);
+                        tc05::st_32x32b_x32(tmem + 32 * q + lanes, o);
+                    }
+                    tc05::wait_st();
+                }
+                // P: a row's 64 tokens are 128 bytes, 16-byte pieces swizzled by the row
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint32_t*>(sm.p + rl[x] * 128 + ((i ^ (rl[x] & 7)) << 4) + (lane & 3) * 4) = pack2<BF>(sv[x][2 * i], sv[x][2 * i + 1]);
+                if (col0 + kTile > r.end) {
+                    // tokens behind the context: whatever lies there (stale bytes, not-a-number) meets probabilities of zero, which does not
+                    // make it zero, so the latents are cleared
+                    const int st = n % NST, valid = r.end - col0;
+                    if (!wt.wait_warp(&sm.k_full[st], (n / NST) & 1)) { ok = false; break; }
+                    for (int i = tid; i < (kTile - valid) * 8; i += 128) {
+                        const int row = valid + i / 8;
+#pragma unroll
+                        for (int c = 0; c < R / 64; ++c) *reinterpret_cast<uint4*>(sm.k[st][c] + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                tc05::fence_proxy_async_smem();
+                tc05::fence_before_thread_sync();
+                warp_arrive(&sm.p_full);
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+                l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+                if ((lane & 3) == 0 && rl[x] < r.rows) a.part_ml[r.slot * kTile + rl[x]] = make_float2(mx[x], l[x]);
+            }
+            if (r.tiles == 0) continue;
+            if (!wt.wait_warp(&sm.o_done, (n - 1) & 1)) break;
+            tc05::fence_after_thread_sync();
+            float* dst = a.part_o + r.slot * kTile * R + 32 * warp + lane;
+#pragma unroll 1
+            for (int q = 0; q < MT * 2; ++q) {
+                const int c0 = (q & 1) * 32;
+                if (c0 >= r.rows) continue;
+                uint32_t o[32];
+                tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
+                tc05::wait_ld();
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (c0 + c < r.rows) dst[(long long)(c0 + c) * R + (q >> 1) * 128] = __uint_as_float(o[c]);
+            }
+            tc05::fence_before_thread_sync();
+        }
+    }
+    __syncthreads();
+    if (warp == 5) tc05::tmem_dealloc(tmem, 512);
+}
+
+// ---- joining the partial results of a row ----------------------------------------------------------------------------------
+// One CTA per row (new token, head): thread (piece group, four latent elements).  Leaves sum / denominator as two 16-bit pieces, so that the
+// product with value_up does not see another rounding.
+template <int R, bool BF>
+__global__ void __launch_bounds__(R) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
+    constexpr int kPer = R / 4, kGroups = 4;       // threads of a piece group
+    __shared__ float4 sh[kGroups - 1][kPer];
+    const Step& m = a.m;
+    const int t = blockIdx.x / m.H, h = blockIdx.x % m.H, tid = threadIdx.x, g = tid / kPer, e = tid % kPer;
+    SeqView v;
+    const int s = find_sequence(m, t);
+    if (!seq_view(m, s, v) || t < v.t0 || t >= v.t0 + v.n || v.n > a.max_new) return;
+    const int row = (t - v.t0) * m.H + h, rt = row / kTile, block = rt / a.row_tiles;
+    const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, per = slice_size(a);
+    const long long u0 = a.unit_prefix[s] + block * tiles, w0 = u0 / per, w1 = (u0 + tiles - 1) / per;
+    const long long slot0 = ((long long)a.block_prefix[s] + block) * a.row_tiles + rt % a.row_tiles;
+    float top = -INFINITY, sum = 0.f;
+    for (long long w = w0; w <= w1; ++w) top = fmaxf(top, a.part_ml[(slot0 + w * a.row_tiles) * kTile + row % kTile].x);
+    for (long long w = w0; w <= w1; ++w) {
+        const float2 ml = a.part_ml[(slot0 + w * a.row_tiles) * kTile + row % kTile];
+        if (ml.y > 0.f) sum += ml.y * ex2(ml.x - top);
+    }
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (long long w = w0 + g; w <= w1; w += kGroups) {
+        const long long at = (slot0 + w * a.row_tiles) * kTile + row % kTile;
+        const float2 ml = a.part_ml[at];
+        if (ml.y > 0.f) {     // (a piece whose tiles the row does not see has no sums)
+            const float k = ex2(ml.x - top);
+            const float4 p = *reinterpret_cast<const float4*>(a.part_o + at * R + 4 * e);
+            x.x += k * p.x; x.y += k * p.y; x.z += k * p.z; x.w += k * p.w;
+        }
+    }
+    if (g > 0) sh[g - 1][e] = x;
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int i = 0; i < kGroups - 1; ++i) { const float4 p = sh[i][e]; x.x += p.x; x.y += p.y; x.z += p.z; x.w += p.w; }
+    const float inv = 1.f / sum;
+    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
+        lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
+    }
+    uint16_t* dst = (uint16_t*)a.o_lat + ((long long)t * m.H + h) * (2 * R) + 4 * e;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo[0], lo[1]);
+}
+
+// ---- output = value_up o~ ---------------------------------------------------------------------------------------------------
+// A CTA computes one head's output of 64 tokens: D[value][token], K = R twice (high and low pieces against the same weights).
+constexpr int kValueStages = 4;
+template <bool BF>
+__global__ void __launch_bounds__(160) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full[kValueStages], free_[kValueStages], done;
+    __shared__ bool live[kTile];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag;
+    const Step& m = a.m;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * kTile, chunks = m.R / 64;
+    if (!tile_rows(a, t0, live)) return;
+    const int w_bytes = m.Dv * 128, stage = w_bytes + 2 * 8192;
+    if (tid == 0) {
+        for (int i = 0; i < kValueStages; ++i) { pa::mbar_init(&full[i], 1); pa::mbar_init(&free_[i], 1); }
+        pa::mbar_init(&done, 1);
+        pa::mbar_fence_init();
+        abort_flag = 0;
+    }
+    if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    tc05::fence_after_thread_sync();
+    const uint32_t tmem = tmem_base;
+    const Waiter wt{&abort_flag, m.status};
+    if (warp == 4) {
+        bool ok = true;
+        const uint32_t idesc = tc05::instr_desc_f16(m.Dv, kTile, BF ? 1 : 0, 0, 0);
+        auto load = [&](int c) {
+            const int st = c % kValueStages;
+            uint8_t* p = smem + st * stage;
+            if (lane == 0) {
+                pa::mbar_expect_tx(&full[st], stage);
+                tma_3d(p, &a.map_value_up, c * 64, 0, h, &full[st]);
+                tma_3d(p + w_bytes, &a.map_o_lat, c * 64, h, t0, &full[st]);
+                tma_3d(p + w_bytes + 8192, &a.map_o_lat, m.R + c * 64, h, t0, &full[st]);
+            }
+            __syncwarp();
+        };
+        for (int c = 0; c < kValueStages && c < chunks; ++c) load(c);
+        for (int c = 0; ok && c < chunks; ++c) {
+            const int st = c % kValueStages;
+            ok = wt.wait_warp(&full[st], (c / kValueStages) & 1);
+            if (!ok) break;
+            tc05::fence_after_thread_sync();
+            const uint32_t base = pa::smem_u32(smem + st * stage);
+            const uint64_t da = tc05::smem_desc_sw128(base, 1024), db = tc05::smem_desc_sw128(base + w_bytes, 1024);
+            if (tc05::elect_one()) {
+                for (int part = 0; part < 2; ++part)
+                    for (int kk = 0; kk < 4; ++kk) tc05::mma_ss(tmem, da + 2 * kk, db + part * 512 + 2 * kk, idesc, c + part + kk > 0);
+                tc05::commit(&free_[st]);
+                if (c + 1 == chunks) tc05::commit(&done);
+            }
+            __syncwarp();
+            if (c + kValueStages < chunks) {
+                ok = wt.wait_warp(&free_[st], (c / kValueStages) & 1);
+                if (ok) load(c + kValueStages);
+            }
+        }
+    } else {
+        const bool ok = wt.wait_warp(&done, 0);
+        tc05::fence_after_thread_sync();
+        // 128 rows: a warp has 32 of them; 64 rows: 16, in the first half of its lanes
+        const int d = m.Dv == 128 ? 32 * warp + lane : 16 * warp + lane;
+        if (ok) {
+            uint16_t* dst = (uint16_t*)a.output + ((long long)t0 * m.H + h) * m.Dv + d;
+#pragma unroll
+            for (int c0 = 0; c0 < kTile; c0 += 32) {
+                uint32_t r[32];
+                tc05::ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
+                tc05::wait_ld();
+                if (m.Dv == 128 || lane < 16) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (live[c0 + c]) dst[(long long)(c0 + c) * m.H * m.Dv] = pack1<BF>(__uint_as_float(r[c]));
+                }
+            }
+        }
+    }
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    if (warp == 0) tc05::tmem_dealloc(tmem, 64);
+}
+
+template <int R, bool BF>
+cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
+    const Step& m = a.m;
+    const int token_tiles = (m.num_tokens + kTile - 1) / kTile;
+    const int smem_q = 2 * m.Dn * 128 + m.Dn / 64 * 8192 + 1024, smem_v = kValueStages * (m.Dv * 128 + 2 * 8192) + 1024;
+    const int smem_a = sizeof(AttendSmem<R>) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_a);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
+    if (e != cudaSuccess) return e;
+    project_query_kernel<BF><<<1 + token_tiles * m.H * (R / 128), 128, smem_q, stream>>>(a);
+    attend_kernel<R, BF><<<a.groups * a.row_tiles, kThreads, smem_a, stream>>>(a);
+    combine_kernel<R, BF><<<m.num_tokens * m.H, R, 0, stream>>>(a);
+    project_value_kernel<BF><<<token_tiles * m.H, 160, smem_v, stream>>>(a);
+    *launches += 4;
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles) {
+    // a sequence of n tokens has ceil(n * heads / rows) blocks; that is at most n * ceil(heads / rows), and n * heads / rows + 1
+    const long long rows = (long long)kTile * row_tiles;
+    const long long blocks = std::min(tokens * ((heads + rows - 1) / rows), (long long)tokens * heads / rows + sequences);
+    return (blocks + groups) * row_tiles;
+}
+
+cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t stream, int* launches) {
+    if (dtype == PA_DTYPE_BF16) return a.m.R == 512 ? launch<512, true>(a, stream, launches) : launch<256, true>(a, stream, launches);
+    return a.m.R == 512 ? launch<512, false>(a, stream, launches) : launch<256, false>(a, stream, launches);
+}
+
+}  // namespace latent

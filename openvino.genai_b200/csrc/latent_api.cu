@@ -1,7 +1,10 @@
 // C ABI of latent attention (include/latent_b200.h): argument checking, scratch and launch sequencing.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <new>
 #include <string>
 
@@ -17,6 +20,8 @@ struct pa_latent_handle {
     int sm_count = 148;
     cudaStream_t stream = nullptr;
     uint32_t* status = nullptr;   // device status word
+    uint8_t* ws = nullptr;        // kernel scratch
+    size_t ws_bytes = 0;
     int64_t launches = 0;
 };
 
@@ -74,8 +79,83 @@ int validate_desc(const pa_latent_desc* d) {
     return PA_OK;
 }
 
+const char kBadStride[] = "a stride is not positive or not a multiple of 8 elements";
+
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool strided(int64_t s) { return s >= 0 && (s & 7) == 0; }
+bool strided(int64_t s) { return s > 0 && (s & 7) == 0; }
+// A stride that is never stepped along may be anything: it is replaced.
+int64_t used_stride(int64_t s, int64_t extent, int64_t instead) { return extent > 1 ? s : instead; }
+
+size_t align_up(size_t x) { return (x + 1023) / 1024 * 1024; }
+
+// ---- tensor maps ------------------------------------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+                   ? (EncodeTiled)p : (EncodeTiled) nullptr;
+    }();
+    return fn;
+}
+
+// A map of 16-bit elements whose boxes are 64 elements wide and land 128-byte-swizzled; elements outside the tensor read as zero.
+// sizes and box in elements, innermost first; strides in elements, of dimensions 1 and 2.
+bool make_map(CUtensorMap* map, int dtype, const void* base, int rank, const long long* sizes, const long long* strides, const int* box) {
+    cuuint64_t dims[3], pitch[2];
+    cuuint32_t b[3], one[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) { dims[i] = (cuuint64_t)sizes[i]; b[i] = (cuuint32_t)box[i]; }
+    for (int i = 0; i + 1 < rank; ++i) pitch[i] = (cuuint64_t)strides[i] * 2;
+    const EncodeTiled encode = encode_tiled();
+    return encode && encode(map, dtype == PA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
+                            dims, pitch, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ---- scratch ------------------------------------------------------------------------------------------------------------
+// New tokens up to which a sequence of an AUTO step takes the absorbed form.
+constexpr int kAutoMaxNew = 64;
+
+struct Scratch {
+    int row_tiles, groups;
+    size_t unit_prefix, block_prefix, q_abs, part_o, part_ml, o_lat, total;
+};
+
+Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int form) {
+    const pa_latent_desc& d = h->desc;
+    Scratch s{};
+    // Two row tiles of a sequence read the same context: two CTAs walk it side by side, so that one of them finds it in the L2 cache
+    s.row_tiles = d.num_heads > latent::kTile ? 2 : 1;
+    s.groups = h->sm_count / s.row_tiles;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += align_up(bytes); return at; };
+    if (form != PA_LATENT_EXPANDED) {
+        const size_t rows = (size_t)tokens * d.num_heads;
+        // in an AUTO step only the short sequences' rows have partial results
+        const int most = form == PA_LATENT_AUTO ? (int)std::min<long long>(tokens, (long long)sequences * kAutoMaxNew) : tokens;
+        const size_t slots = (size_t)latent::absorbed_slots(most, sequences, d.num_heads, s.groups, s.row_tiles);
+        s.unit_prefix = take(((size_t)sequences + 1) * sizeof(long long));
+        s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
+        s.q_abs = take(rows * (d.latent_size + d.rope_size) * 2);
+        s.o_lat = take(rows * 2 * d.latent_size * 2);
+        s.part_ml = take(slots * latent::kTile * sizeof(float2));
+        s.part_o = take(slots * latent::kTile * d.latent_size * sizeof(float));
+    }
+    s.total = off;
+    return s;
+}
+
+int ensure_ws(pa_latent_handle* h, size_t bytes) {
+    if (bytes <= h->ws_bytes) return PA_OK;
+    if (h->ws) LATENT_CUDA(cudaFree(h->ws));   // (waits for the work that uses it)
+    h->ws = nullptr; h->ws_bytes = 0;
+    const size_t want = (bytes + bytes / 4 + (1 << 20) - 1) >> 20 << 20;
+    LATENT_CUDA(cudaMalloc((void**)&h->ws, want));
+    h->ws_bytes = want;
+    return PA_OK;
+}
 
 // What both calls share.
 template <class Args>
@@ -85,6 +165,7 @@ int validate_step(const Args* a) {
     if (a->num_tokens == 0 || a->num_sequences == 0) return PA_OK;
     if (!a->past_lens || !a->subsequence_begins || !a->block_indices_begins || !a->cache) return fail(PA_ERR_INVALID_ARG, "NULL metadata or cache pointer");
     if (a->num_block_indices > 0 && !a->block_indices) return fail(PA_ERR_INVALID_ARG, "NULL block_indices");
+    if (a->num_blocks == 0) return fail(PA_ERR_INVALID_ARG, "the cache has no blocks");
     if (!aligned(a->cache)) return fail(PA_ERR_UNSUPPORTED, "cache is not 16-byte aligned");
     return PA_OK;
 }
@@ -108,15 +189,16 @@ int append(pa_latent_handle* h, const pa_latent_append_args* a) {
     if ((a->query_rope != nullptr) != (a->query_rope_out != nullptr)) return fail(PA_ERR_INVALID_ARG, "query_rope and query_rope_out must be given together");
     if (!aligned(a->latent) || !aligned(a->norm_weight) || !aligned(a->query_rope) || !aligned(a->query_rope_out) || !aligned(a->rope_table))
         return fail(PA_ERR_UNSUPPORTED, "a tensor is not 16-byte aligned");
-    if (!strided(a->latent_stride) || !strided(a->query_rope_token_stride) || !strided(a->query_rope_head_stride) ||
-        !strided(a->query_rope_out_token_stride) || !strided(a->query_rope_out_head_stride))
-        return fail(PA_ERR_UNSUPPORTED, "a stride is negative or not a multiple of 8 elements");
+    const int T = a->num_tokens, H = h->desc.num_heads, P = h->desc.rope_size;
+    const int64_t ls = used_stride(a->latent_stride, T, h->desc.latent_size + P);
+    const int64_t qt = used_stride(a->query_rope_token_stride, T, H * P), qh = used_stride(a->query_rope_head_stride, H, P);
+    const int64_t ot = used_stride(a->query_rope_out_token_stride, T, H * P), oh = used_stride(a->query_rope_out_head_stride, H, P);
+    if (!strided(ls) || (a->query_rope && (!strided(qt) || !strided(qh) || !strided(ot) || !strided(oh))))
+        return fail(PA_ERR_UNSUPPORTED, kBadStride);
     DeviceScope scope(h->device);
     LATENT_CUDA(scope.error);
-    latent::AppendArgs k{make_step(h, a), a->latent, a->latent_stride, a->norm_weight, a->norm_eps,
-                         a->query_rope, a->query_rope_token_stride, a->query_rope_head_stride,
-                         a->query_rope_out, a->query_rope_out_token_stride, a->query_rope_out_head_stride,
-                         a->rope_table, a->rope_table_rows, a->interleaved, a->positions, a->cache};
+    latent::AppendArgs k{make_step(h, a), a->latent, ls, a->norm_weight, a->norm_eps, a->query_rope, qt, qh, a->query_rope_out, ot, oh, a->rope_table,
+                         a->rope_table_rows, a->interleaved, a->positions, a->cache};
     int launches = 0;
     LATENT_CUDA(latent::launch_append(k, h->desc.dtype, a->stream ? (cudaStream_t)a->stream : h->stream, &launches));
     h->launches += launches;
@@ -127,24 +209,61 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
     if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
     if (!a || a->struct_size != sizeof(pa_latent_attention_args)) return fail(PA_ERR_INVALID_ARG, "pa_latent_attention_args: NULL or struct_size mismatch");
     if (a->form != PA_LATENT_AUTO && a->form != PA_LATENT_ABSORBED && a->form != PA_LATENT_EXPANDED) return fail(PA_ERR_INVALID_ARG, "unknown form");
-    const int rc = validate_step(a);
+    int rc = validate_step(a);
     if (rc != PA_OK) return rc;
     if (a->num_tokens == 0 || a->num_sequences == 0) return PA_OK;
     if (!a->query_nope || !a->query_rope || !a->key_up || !a->value_up || !a->output) return fail(PA_ERR_INVALID_ARG, "NULL query, weight or output pointer");
     if (!aligned(a->query_nope) || !aligned(a->query_rope) || !aligned(a->key_up) || !aligned(a->value_up) || !aligned(a->output))
         return fail(PA_ERR_UNSUPPORTED, "a tensor is not 16-byte aligned");
-    if (!strided(a->query_nope_token_stride) || !strided(a->query_nope_head_stride) || !strided(a->query_rope_token_stride) ||
-        !strided(a->query_rope_head_stride) || !strided(a->key_up_head_stride) || !strided(a->value_up_head_stride))
-        return fail(PA_ERR_UNSUPPORTED, "a stride is negative or not a multiple of 8 elements");
-    if ((long long)a->num_tokens * h->desc.num_heads > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
+    const pa_latent_desc& d = h->desc;
+    const int T = a->num_tokens, H = d.num_heads, R = d.latent_size, P = d.rope_size;
+    const int64_t nt = used_stride(a->query_nope_token_stride, T, H * d.nope_size), nh = used_stride(a->query_nope_head_stride, H, d.nope_size);
+    const int64_t rt = used_stride(a->query_rope_token_stride, T, H * P), rh = used_stride(a->query_rope_head_stride, H, P);
+    const int64_t kh = used_stride(a->key_up_head_stride, H, (int64_t)d.nope_size * R), vh = used_stride(a->value_up_head_stride, H, (int64_t)d.value_size * R);
+    if (!strided(nt) || !strided(nh) || !strided(rt) || !strided(rh) || !strided(kh) || !strided(vh)) return fail(PA_ERR_UNSUPPORTED, kBadStride);
+    if ((long long)T * H > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
+    if ((long long)a->num_blocks * d.block_size > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of cache");
     DeviceScope scope(h->device);
     LATENT_CUDA(scope.error);
-    const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf((float)(h->desc.nope_size + h->desc.rope_size));
-    latent::AttentionArgs k{make_step(h, a), a->query_nope, a->query_nope_token_stride, a->query_nope_head_stride,
-                            a->query_rope, a->query_rope_token_stride, a->query_rope_head_stride, a->key_up, a->key_up_head_stride,
-                            a->value_up, a->value_up_head_stride, a->output, a->cache, scale};
+    const cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
+    const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf((float)(d.nope_size + P));
+    const Scratch s = plan_scratch(h, T, a->num_sequences, a->form);
+    rc = ensure_ws(h, s.total);
+    if (rc != PA_OK) return rc;
+    const int max_new = a->form == PA_LATENT_ABSORBED ? INT_MAX : kAutoMaxNew;
     int launches = 0;
-    LATENT_CUDA(latent::launch_attention_simple(k, h->desc.dtype, a->stream ? (cudaStream_t)a->stream : h->stream, &launches));
+    if (a->form != PA_LATENT_EXPANDED) {
+        latent::AbsorbedArgs k{};
+        k.m = make_step(h, a);
+        k.max_new = max_new;
+        k.groups = s.groups; k.row_tiles = s.row_tiles;
+        k.unit_prefix = (long long*)(h->ws + s.unit_prefix);
+        k.block_prefix = (int*)(h->ws + s.block_prefix);
+        k.q_rope = a->query_rope; k.qr_token = rt; k.qr_head = rh;
+        k.q_abs = h->ws + s.q_abs;
+        k.part_o = (float*)(h->ws + s.part_o);
+        k.part_ml = (float2*)(h->ws + s.part_ml);
+        k.o_lat = h->ws + s.o_lat;
+        k.output = a->output;
+        k.scale_log2 = scale * 1.4426950408889634f;
+        const int W = R + P;
+        const long long qn_size[3] = {d.nope_size, H, T}, qn_stride[2] = {nh, nt};
+        const long long ku_size[3] = {R, d.nope_size, H}, ku_stride[2] = {R, kh};
+        const long long vu_size[3] = {R, d.value_size, H}, vu_stride[2] = {R, vh};
+        const long long qa_size[2] = {W, (long long)T * H}, ca_size[2] = {W, (long long)a->num_blocks * d.block_size}, row_stride[1] = {W};
+        const long long ol_size[3] = {2 * R, H, T}, ol_stride[2] = {2 * R, 2ll * R * H};
+        const int box_tokens[3] = {64, 1, latent::kTile}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1}, box_q[2] = {64, 16}, box_c[2] = {64, d.block_size};
+        if (!make_map(&k.map_qn, d.dtype, a->query_nope, 3, qn_size, qn_stride, box_tokens) || !make_map(&k.map_key_up, d.dtype, a->key_up, 3, ku_size, ku_stride, box_ku) ||
+            !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_q_abs, d.dtype, k.q_abs, 2, qa_size, row_stride, box_q) ||
+            !make_map(&k.map_cache, d.dtype, a->cache, 2, ca_size, row_stride, box_c) || !make_map(&k.map_o_lat, d.dtype, k.o_lat, 3, ol_size, ol_stride, box_tokens))
+            return fail(PA_ERR_CUDA, "a tensor map could not be made");
+        LATENT_CUDA(latent::launch_absorbed(k, d.dtype, stream, &launches));
+    }
+    if (a->form != PA_LATENT_ABSORBED && (a->form == PA_LATENT_EXPANDED || T > max_new)) {
+        latent::AttentionArgs k{make_step(h, a), a->query_nope, nt, nh, a->query_rope, rt, rh, a->key_up, kh, a->value_up, vh, a->output, a->cache, scale,
+                                a->form == PA_LATENT_EXPANDED ? 1 : max_new + 1};
+        LATENT_CUDA(latent::launch_attention_simple(k, d.dtype, stream, &launches));
+    }
     h->launches += launches;
     return PA_OK;
 }
@@ -187,6 +306,7 @@ int pa_b200_latent_destroy(pa_latent_handle* h) {
     if (!h) return PA_OK;
     DeviceScope scope(h->device);
     if (h->stream) cudaStreamSynchronize(h->stream);
+    if (h->ws) cudaFree(h->ws);   // (waits for the work that uses it)
     if (h->status) cudaFree(h->status);
     if (h->stream) cudaStreamDestroy(h->stream);
     delete h;
@@ -199,6 +319,17 @@ int pa_b200_latent_append(pa_latent_handle* h, const pa_latent_append_args* a) {
 
 int pa_b200_latent_attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
     return guarded([&] { return attention(h, a); });
+}
+
+int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices, int32_t form) {
+    return guarded([&] {
+        if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
+        if (num_tokens < 0 || num_sequences < 0 || num_block_indices < 0) return fail(PA_ERR_INVALID_ARG, "negative size");
+        if (form != PA_LATENT_AUTO && form != PA_LATENT_ABSORBED && form != PA_LATENT_EXPANDED) return fail(PA_ERR_INVALID_ARG, "unknown form");
+        DeviceScope scope(h->device);
+        LATENT_CUDA(scope.error);
+        return ensure_ws(h, plan_scratch(h, num_tokens, num_sequences, form).total);
+    });
 }
 
 int pa_b200_latent_last_device_status(pa_latent_handle* h, uint32_t* status_bits) {

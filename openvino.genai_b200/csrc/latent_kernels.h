@@ -1,6 +1,7 @@
 // Internal launch interface of latent attention, between the C ABI (latent_api.cu) and the kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -50,7 +51,34 @@ struct AttentionArgs {
     void* output;
     const void* cache;
     float scale;
+    int min_new;                // sequences with fewer new tokens are not served
 };
+
+// The absorbed form.  Its unit of work is a tile of 64 context tokens for a block of `row_tiles` tiles of 64 query rows (new token, head) of one
+// sequence; sequence s has block_prefix[s + 1] - block_prefix[s] such blocks, every one of the same number of tiles.  Units are
+// numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut, or
+// not, leaves one partial result per group in slot (block + group) * row_tiles + row tile.
+constexpr int kTile = 64;      // context tokens of a tile, query rows of a row tile, tokens of a projection's tile
+
+struct AbsorbedArgs {
+    Step m;
+    int max_new;                // sequences with more new tokens are left to the expanded form
+    int groups, row_tiles;
+    long long* unit_prefix;     // [num_sequences + 1]
+    int* block_prefix;          // [num_sequences + 1]
+    const void* q_rope;
+    long long qr_token, qr_head;
+    void* q_abs;                // [num_tokens * H][R + P] absorbed query rows
+    float* part_o;              // [slot][64][R]
+    float2* part_ml;            // [slot][64] maximum (base 2, scaled) and sum
+    void* o_lat;                // [num_tokens * H][2 R] sums of latents, high and low pieces
+    void* output;
+    float scale_log2;           // softmax scale * log2(e)
+    CUtensorMap map_qn, map_key_up, map_q_abs, map_cache, map_value_up, map_o_lat;
+};
+// Largest number of slots a step can need.
+long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);
+cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t stream, int* launches);
 
 cudaError_t launch_append(const AppendArgs& a, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_attention_simple(const AttentionArgs& a, int dtype, cudaStream_t stream, int* launches);

@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(kWarps * 32) simple_kernel(AttentionArgs a) {
     const Step& m = a.m;
     const int t = blockIdx.x / m.H, h = blockIdx.x % m.H, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     SeqView v;
-    if (!token_view(m, t, v)) return;
+    if (!token_view(m, t, v) || v.n < a.min_new) return;
     const T* qn = (const T*)a.q_nope + t * a.qn_token + h * a.qn_head;
     const T* qr = (const T*)a.q_rope + t * a.qr_token + h * a.qr_head;
     const T* up = (const T*)a.key_up + h * a.key_up_head;

@@ -1,0 +1,90 @@
+// Device helpers of the tensor-core kernels of latent attention: tensor-map copies, bounded waits, tensor-memory accesses
+// for 64-row accumulators.
+#pragma once
+
+#include <cuda.h>
+#include <stdint.h>
+
+#include "latent_kernels.h"
+#include "tc05.cuh"
+
+namespace latent {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(pa::smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(pa::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     pa::smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(pa::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pa::smem_u32(bar)) : "memory");
+}
+// One arrival for the whole warp, after every lane's preceding writes.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Waits of a CTA's roles on one another are bounded: one that runs out raises `abort`, which all others poll, and sets the status bit.
+struct Waiter {
+    volatile int* abort;
+    uint32_t* status;
+    __device__ __forceinline__ bool give_up() const {
+        *abort = 1;
+        atomicOr(status, PA_DEV_WAIT_TIMEOUT_LATENT);
+        return false;
+    }
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
+        for (uint32_t i = 0; i < (1u << 22); ++i) {
+            if (pa::mbar_try_wait(bar, parity)) return true;
+            if ((i & 255u) == 255u && *abort) return false;
+        }
+        return give_up();
+    }
+    __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) const { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return BF ? pa::pack_bf2(a, b) : pa::pack_h2(a, b);
+}
+template <bool BF>
+__device__ __forceinline__ uint16_t pack1(float a) {
+    return (uint16_t)(pack2<BF>(a, 0.f) & 0xffffu);
+}
+template <bool BF>
+__device__ __forceinline__ float unpack1(uint16_t b) {
+    return BF ? __bfloat162float(__ushort_as_bfloat16(b)) : __half2float(__ushort_as_half(b));
+}
+
+// 16 lanes x 64 columns of a 64-row accumulator: a warp's 16 rows lie in the first 16 of its lanes.  Thread t gets, for every
+// group i of eight columns, row t / 4: r[4 i], r[4 i + 1] and row t / 4 + 8: r[4 i + 2], r[4 i + 3], at columns 8 i + 2 (t % 4) and the next.
+__device__ __forceinline__ void ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+}  // namespace latent

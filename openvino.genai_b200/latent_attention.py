@@ -129,6 +129,10 @@ class LatentAttention:
         self._metadata(a, inputs)
         self._check(self.lib.pa_b200_latent_attention(self._h, C.byref(a)))
 
+    def reserve(self, num_tokens: int, num_sequences: int, num_block_indices: int, form: str = "auto") -> None:
+        """Grows the scratch for steps of up to this size, so that `attend` does not allocate (stream captures need that)."""
+        self._check(self.lib.pa_b200_latent_reserve(self._h, num_tokens, num_sequences, num_block_indices, _FORMS[form]))
+
     def device_status(self) -> int:
         """Reads and clears the device status word (PA_DEV_* bits)."""
         bits = C.c_uint32(0)
