@@ -118,12 +118,19 @@ bool make_map(CUtensorMap* map, int dtype, const void* base, int rank, const lon
 // New tokens up to which a sequence of an AUTO step takes the absorbed form.
 constexpr int kAutoMaxNew = 64;
 
+// Expanded keys and values of as many heads as fit this are made at a time.
+constexpr size_t kExpandBytes = (size_t)1 << 30;
+
 struct Scratch {
     int row_tiles, groups;
-    size_t unit_prefix, block_prefix, q_abs, part_o, part_ml, o_lat, total;
+    size_t unit_prefix, block_prefix, q_abs, part_o, part_ml, o_lat;
+    int heads, passes;       // expanded: heads of a pass
+    long long rows;
+    size_t tile_prefix, query_prefix, order, counter, k, v, k_rope;
+    size_t total;
 };
 
-Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int form) {
+Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int block_indices, int form) {
     const pa_latent_desc& d = h->desc;
     Scratch s{};
     // Two row tiles of a sequence read the same context: two CTAs walk it side by side, so that one of them finds it in the L2 cache
@@ -142,6 +149,20 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int f
         s.o_lat = take(rows * 2 * d.latent_size * 2);
         s.part_ml = take(slots * latent::kTile * sizeof(float2));
         s.part_o = take(slots * latent::kTile * d.latent_size * sizeof(float));
+    }
+    if (form == PA_LATENT_EXPANDED || (form == PA_LATENT_AUTO && tokens > kAutoMaxNew)) {
+        const int served = form == PA_LATENT_AUTO ? std::min(sequences, tokens / (kAutoMaxNew + 1)) : sequences;
+        s.rows = ((long long)block_indices * d.block_size / latent::kExpandTile + served) * latent::kExpandTile;
+        const size_t head = (size_t)s.rows * (d.nope_size + d.value_size) * 2;
+        s.heads = (int)std::max<size_t>(1, std::min<size_t>(d.num_heads, kExpandBytes / std::max<size_t>(1, head)));
+        s.passes = (d.num_heads + s.heads - 1) / s.heads;
+        s.tile_prefix = take(((size_t)sequences + 1) * sizeof(int));
+        s.query_prefix = take(((size_t)sequences + 1) * sizeof(int));
+        s.order = take(((size_t)tokens / latent::kQueryTile + served) * sizeof(int2));
+        s.counter = take((size_t)s.passes * sizeof(int));
+        s.k_rope = take((size_t)s.rows * 64 * 2);
+        s.k = take((size_t)s.heads * s.rows * d.nope_size * 2);
+        s.v = take((size_t)s.heads * s.rows * d.value_size * 2);
     }
     s.total = off;
     return s;
@@ -221,13 +242,14 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
     const int64_t rt = used_stride(a->query_rope_token_stride, T, H * P), rh = used_stride(a->query_rope_head_stride, H, P);
     const int64_t kh = used_stride(a->key_up_head_stride, H, (int64_t)d.nope_size * R), vh = used_stride(a->value_up_head_stride, H, (int64_t)d.value_size * R);
     if (!strided(nt) || !strided(nh) || !strided(rt) || !strided(rh) || !strided(kh) || !strided(vh)) return fail(PA_ERR_UNSUPPORTED, kBadStride);
+    if (!(a->scale >= 0.f) || std::isinf(a->scale)) return fail(PA_ERR_INVALID_ARG, "scale is negative or not finite");
     if ((long long)T * H > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
     if ((long long)a->num_blocks * d.block_size > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of cache");
     DeviceScope scope(h->device);
     LATENT_CUDA(scope.error);
     const cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
     const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf((float)(d.nope_size + P));
-    const Scratch s = plan_scratch(h, T, a->num_sequences, a->form);
+    const Scratch s = plan_scratch(h, T, a->num_sequences, a->num_block_indices, a->form);
     rc = ensure_ws(h, s.total);
     if (rc != PA_OK) return rc;
     const int max_new = a->form == PA_LATENT_ABSORBED ? INT_MAX : kAutoMaxNew;
@@ -259,10 +281,41 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
             return fail(PA_ERR_CUDA, "a tensor map could not be made");
         LATENT_CUDA(latent::launch_absorbed(k, d.dtype, stream, &launches));
     }
-    if (a->form != PA_LATENT_ABSORBED && (a->form == PA_LATENT_EXPANDED || T > max_new)) {
-        latent::AttentionArgs k{make_step(h, a), a->query_nope, nt, nh, a->query_rope, rt, rh, a->key_up, kh, a->value_up, vh, a->output, a->cache, scale,
-                                a->form == PA_LATENT_EXPANDED ? 1 : max_new + 1};
-        LATENT_CUDA(latent::launch_attention_simple(k, d.dtype, stream, &launches));
+    if (s.passes > 0) {
+        if (s.heads * s.rows > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 rows of expanded keys");
+        latent::ExpandedArgs k{};
+        k.m = make_step(h, a);
+        k.min_new = a->form == PA_LATENT_EXPANDED ? 1 : kAutoMaxNew + 1;
+        k.rows = s.rows;
+        k.tile_prefix = (int*)(h->ws + s.tile_prefix);
+        k.query_prefix = (int*)(h->ws + s.query_prefix);
+        k.order = (int2*)(h->ws + s.order);
+        k.counter = (int*)(h->ws + s.counter);
+        k.passes = s.passes;
+        k.cache = a->cache;
+        k.k_rope = h->ws + s.k_rope;
+        k.output = a->output;
+        k.scale_log2 = scale * 1.4426950408889634f;
+        const int W = R + P;
+        const long long ca_size[2] = {W, (long long)a->num_blocks * d.block_size}, ca_stride[1] = {W};
+        const long long ku_size[3] = {R, d.nope_size, H}, ku_stride[2] = {R, kh}, vu_size[3] = {R, d.value_size, H}, vu_stride[2] = {R, vh};
+        const long long qn_size[3] = {d.nope_size, H, T}, qn_stride[2] = {nh, nt}, qr_size[3] = {P, H, T}, qr_stride[2] = {rh, rt};
+        const long long k_size[2] = {d.nope_size, s.heads * s.rows}, k_stride[1] = {d.nope_size}, v_size[2] = {d.value_size, s.heads * s.rows}, v_stride[1] = {d.value_size};
+        const long long r_size[2] = {64, s.rows}, r_stride[1] = {64};
+        const int box_c[2] = {64, d.block_size}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1}, box_q[3] = {64, 1, 128};
+        const int box_out[2] = {64, 32}, box_k[2] = {64, latent::kExpandTile}, box_v[2] = {64, 64};
+        if (!make_map(&k.map_cache, d.dtype, a->cache, 2, ca_size, ca_stride, box_c) || !make_map(&k.map_key_up, d.dtype, a->key_up, 3, ku_size, ku_stride, box_ku) ||
+            !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_k_out, d.dtype, h->ws + s.k, 2, k_size, k_stride, box_out) ||
+            !make_map(&k.map_v_out, d.dtype, h->ws + s.v, 2, v_size, v_stride, box_out) || !make_map(&k.map_k, d.dtype, h->ws + s.k, 2, k_size, k_stride, box_k) ||
+            !make_map(&k.map_v, d.dtype, h->ws + s.v, 2, v_size, v_stride, box_v) || !make_map(&k.map_k_rope, d.dtype, k.k_rope, 2, r_size, r_stride, box_k) ||
+            !make_map(&k.map_qn, d.dtype, a->query_nope, 3, qn_size, qn_stride, box_q) || !make_map(&k.map_qr, d.dtype, a->query_rope, 3, qr_size, qr_stride, box_q))
+            return fail(PA_ERR_CUDA, "a tensor map could not be made");
+        LATENT_CUDA(latent::launch_expanded_plan(k, stream, &launches));
+        for (k.pass = 0; k.pass < s.passes; ++k.pass) {
+            k.h0 = k.pass * s.heads;
+            k.heads = std::min(s.heads, H - k.h0);
+            LATENT_CUDA(latent::launch_expanded(k, d.dtype, h->sm_count, stream, &launches));
+        }
     }
     h->launches += launches;
     return PA_OK;
@@ -328,7 +381,7 @@ int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_
         if (form != PA_LATENT_AUTO && form != PA_LATENT_ABSORBED && form != PA_LATENT_EXPANDED) return fail(PA_ERR_INVALID_ARG, "unknown form");
         DeviceScope scope(h->device);
         LATENT_CUDA(scope.error);
-        return ensure_ws(h, plan_scratch(h, num_tokens, num_sequences, form).total);
+        return ensure_ws(h, plan_scratch(h, num_tokens, num_sequences, num_block_indices, form).total);
     });
 }
 

@@ -1,0 +1,676 @@
+// Latent attention in its expanded form, on the 5th-generation tensor cores (tcgen05 + TMEM): keys and values of the served contexts are
+// made per head (k = key_up c, v = value_up c), then attention over them.
+//   plan     context tiles and query tiles of the sequences, query tiles longest context first
+//   expand   k, v of every (128 context tokens, head), and the rotated key part gathered from its pages
+//   attend   256 new tokens of one head at a time
+#include <algorithm>
+
+#include "latent_tc.cuh"
+
+namespace latent {
+
+namespace {
+
+// ---- plan ------------------------------------------------------------------------------------------------------------------
+constexpr int kBuckets = 1024;
+__global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constant__ ExpandedArgs a) {
+    __shared__ int sh_c[8], sh_q[8], run_c, run_q;
+    __shared__ int bucket[kBuckets];
+    const Step& m = a.m;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = m.num_sequences;
+    if (tid == 0) { run_c = 0; run_q = 0; }
+    for (int i = tid; i < a.passes; i += 256) a.counter[i] = 0;
+    for (int i = tid; i < kBuckets; i += 256) bucket[i] = 0;
+    __syncthreads();
+    for (int base = 0; base < B; base += 256) {
+        const int s = base + tid;
+        int c = 0, q = 0;
+        if (s < B) {
+            SeqView v;
+            if (seq_view(m, s, v) && v.n > 0 && v.n >= a.min_new) {
+                c = (int)(((long long)v.past + v.n + kExpandTile - 1) / kExpandTile);
+                q = (v.n + kQueryTile - 1) / kQueryTile;
+            }
+        }
+        const int mine_c = c, mine_q = q;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int pc = __shfl_up_sync(0xffffffffu, c, o), pq = __shfl_up_sync(0xffffffffu, q, o);
+            if (lane >= o) { c += pc; q += pq; }
+        }
+        if (lane == 31) { sh_c[wid] = c; sh_q[wid] = q; }
+        __syncthreads();
+        int off_c = run_c, off_q = run_q;
+        for (int w = 0; w < wid; ++w) { off_c += sh_c[w]; off_q += sh_q[w]; }
+        if (s < B) { a.tile_prefix[s] = off_c + c - mine_c; a.query_prefix[s] = off_q + q - mine_q; }
+        __syncthreads();
+        if (tid == 255) { run_c = off_c + c; run_q = off_q + q; }
+        __syncthreads();
+    }
+    if (tid == 0) { a.tile_prefix[B] = run_c; a.query_prefix[B] = run_q; }
+    __syncthreads();
+    // counting sort of the query tiles by the context they see, the longest first, so that the last items to be drawn are short
+    const int total = run_q;
+    auto place = [&](int i, int& s, int& qt) {
+        int lo = 0, hi = B;   // query_prefix[lo] <= i < query_prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.query_prefix[mid] <= i) lo = mid; else hi = mid;
+        }
+        s = lo;
+        qt = i - a.query_prefix[lo];
+        const int n = m.subsequence_begins[lo + 1] - m.subsequence_begins[lo];
+        const int tiles = (m.past_lens[lo] + min(n, (qt + 1) * kQueryTile) + kExpandTile - 1) / kExpandTile;
+        return kBuckets - 1 - min(tiles, kBuckets - 1);
+    };
+    for (int i = tid; i < total; i += 256) {
+        int s, qt;
+        atomicAdd(&bucket[place(i, s, qt)], 1);
+    }
+    __syncthreads();
+    if (tid < 32) {          // exclusive prefix sum over the buckets
+        int run = 0;
+        for (int base = 0; base < kBuckets; base += 32) {
+            const int mine = bucket[base + lane];
+            int v = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int p = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += p;
+            }
+            bucket[base + lane] = run + v - mine;
+            run += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < total; i += 256) {
+        int s, qt;
+        const int b = place(i, s, qt);
+        a.order[atomicAdd(&bucket[b], 1)] = make_int2(s, qt);
+    }
+}
+
+// ---- k = key_up c, v = value_up c ---------------------------------------------------------------------------------------------
+// A CTA keeps a tile of 128 context rows in shared memory and walks over heads: D[token][element] of the head's keys, then of its values, with
+// the weights streamed in chunks of 64 latent elements.  Two accumulators, so that one head is written out while the next is computed.
+constexpr int kExpandThreads = 192;    // warps 0 - 3: output, 4: loader, 5: products
+constexpr int kWeightStages = 4;
+
+template <int R>
+struct ExpandSmem {
+    alignas(1024) uint8_t a[R / 64][kExpandTile * 128];
+    alignas(1024) uint8_t w[kWeightStages][128 * 128];
+    alignas(1024) uint8_t out[2][kExpandTile * 128];        // 128 elements of every row on their way to global memory
+    uint64_t a_full, a_free, w_full[kWeightStages], w_free[kWeightStages], d_full[2], d_free[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+struct ExpandItem {
+    int s, tile, h_first, h_end;    // sequence, its context tile, heads (of this pass)
+    int valid;                      // rows of the tile inside the context
+    int row;                        // first row in the scratch
+    int block0, blocks;             // its blocks inside block_indices
+};
+
+__device__ __forceinline__ int expand_heads_per_item(const ExpandedArgs& a) {
+    // enough items for every CTA to have a few, else as many heads as pay for bringing the context tile in
+    const long long all = (long long)a.tile_prefix[a.m.num_sequences] * a.heads;
+    return (int)min(8ll, max(1ll, all / (gridDim.x * 3ll)));
+}
+
+__device__ __forceinline__ ExpandItem expand_item(const ExpandedArgs& a, int i, int per) {
+    const int head_groups = (a.heads + per - 1) / per, tile = i / head_groups;
+    ExpandItem it;
+    it.h_first = i % head_groups * per;
+    it.h_end = min(a.heads, it.h_first + per);
+    int lo = 0, hi = a.m.num_sequences;   // tile_prefix[lo] <= tile < tile_prefix[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.tile_prefix[mid] <= tile) lo = mid; else hi = mid;
+    }
+    it.s = lo;
+    it.tile = tile - a.tile_prefix[lo];
+    SeqView v;
+    seq_view(a.m, lo, v);
+    const int from = it.tile * kExpandTile;
+    it.valid = min(kExpandTile, v.past + v.n - from);
+    it.row = tile * kExpandTile;
+    it.block0 = v.tb + from / a.m.bs;
+    it.blocks = (it.valid + a.m.bs - 1) / a.m.bs;
+    return it;
+}
+
+template <int R, bool BF>
+__global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_constant__ ExpandedArgs a) {
+    using Smem = ExpandSmem<R>;
+    constexpr int NC = R / 64;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const Step& m = a.m;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        pa::mbar_init(&sm.a_full, 1);
+        pa::mbar_init(&sm.a_free, 1);
+        for (int i = 0; i < kWeightStages; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
+        for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.d_full[i], 1); pa::mbar_init(&sm.d_free[i], 4); }
+        pa::mbar_fence_init();
+        sm.abort_flag = 0;
+    }
+    if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    tc05::fence_after_thread_sync();
+    const uint32_t tmem = sm.tmem_base;
+    const Waiter wt{&sm.abort_flag, m.status};
+    const int per = expand_heads_per_item(a), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
+    const int buffer = m.Dn + m.Dv;      // tensor-memory columns of one head
+
+    if (warp == 4) {
+        uint32_t n = 0, na = 0;
+        bool ok = true, bad_index = false;
+        for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
+            const ExpandItem it = expand_item(a, i, per);
+            int page = 0;
+            if (lane < it.blocks) {
+                page = m.block_indices[it.block0 + lane];
+                if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
+            }
+            if (na > 0) ok = wt.wait_warp(&sm.a_free, (na - 1) & 1);
+            if (!ok) break;
+            if (lane == 0) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
+            for (int b = 0; b < it.blocks; ++b) {
+                const int at = __shfl_sync(0xffffffffu, page, b) * m.bs;
+                if (lane == 0)
+                    for (int c = 0; c < NC; ++c) tma_2d(sm.a[c] + b * m.bs * 128, &a.map_cache, 64 * c, at, &sm.a_full);
+            }
+            for (int h = it.h_first; ok && h < it.h_end; ++h)
+                for (int x = 0; ok && x < 2 * NC; ++x, ++n) {
+                    const int st = n % kWeightStages;
+                    if (n >= kWeightStages) ok = wt.wait_warp(&sm.w_free[st], (n / kWeightStages - 1) & 1);
+                    if (ok && lane == 0) {
+                        pa::mbar_expect_tx(&sm.w_full[st], (x < NC ? m.Dn : m.Dv) * 128);
+                        tma_3d(sm.w[st], x < NC ? &a.map_key_up : &a.map_value_up, 64 * (x % NC), 0, a.h0 + h, &sm.w_full[st]);
+                    }
+                    __syncwarp();
+                }
+        }
+        if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
+        if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
+            for (uint32_t k = 0; na > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.a_full, (na - 1) & 1); ++k) {}
+            for (uint32_t i = n > kWeightStages ? n - kWeightStages : 0; i < n; ++i)
+                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % kWeightStages], (i / kWeightStages) & 1); ++k) {}
+        }
+    } else if (warp == 5) {
+        const uint32_t idesc_k = tc05::instr_desc_f16(128, m.Dn, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, m.Dv, BF ? 1 : 0, 0, 0);
+        const uint64_t da = tc05::smem_desc_sw128(pa::smem_u32(sm.a), 1024), dw = tc05::smem_desc_sw128(pa::smem_u32(sm.w), 1024);
+        uint32_t n = 0, na = 0, nd = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
+            const ExpandItem it = expand_item(a, i, per);
+            ok = wt.wait_warp(&sm.a_full, na & 1);
+            for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
+                if (nd >= 2) ok = wt.wait_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
+                for (int x = 0; ok && x < 2 * NC; ++x, ++n) {
+                    const int st = n % kWeightStages;
+                    ok = wt.wait_warp(&sm.w_full[st], (n / kWeightStages) & 1);
+                    if (!ok) break;
+                    tc05::fence_after_thread_sync();
+                    const uint32_t d = tmem + (nd & 1) * buffer + (x < NC ? 0 : m.Dn);
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc05::mma_ss(d, da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, dw + st * (128 * 128 >> 4) + 2 * kk, x < NC ? idesc_k : idesc_v,
+                                         (x % NC) + kk > 0 ? 1u : 0u);
+                        tc05::commit(&sm.w_free[st]);
+                        if (x == 2 * NC - 1) {
+                            tc05::commit(&sm.d_full[nd & 1]);
+                            if (h + 1 == it.h_end) tc05::commit(&sm.a_free);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        uint32_t nd = 0;
+        const int row = tid;       // of the tile
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        bool ok = true;
+        for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+            const ExpandItem it = expand_item(a, i, per);
+            const bool live = row < it.valid;
+            if (it.h_first == 0 && a.h0 == 0) {      // the rotated part of the keys, once
+                uint4* dst = reinterpret_cast<uint4*>((uint16_t*)a.k_rope + ((long long)it.row + row) * 64);
+                const uint4* src = nullptr;
+                if (live) {
+                    const int page = m.block_indices[it.block0 + row / m.bs];
+                    if (page >= 0 && page < m.num_blocks)
+                        src = reinterpret_cast<const uint4*>((const uint16_t*)a.cache + ((long long)page * m.bs + row % m.bs) * (m.R + m.P) + m.R);
+                }
+                for (int c = 0; c < m.P / 8; ++c) dst[c] = src ? src[c] : make_uint4(0, 0, 0, 0);
+            }
+            for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
+                ok = wt.wait_warp(&sm.d_full[nd & 1], (nd / 2) & 1);
+                if (!ok) break;
+                tc05::fence_after_thread_sync();
+                for (int part = 0; part < 2; ++part) {
+                    const int D = part ? m.Dv : m.Dn;
+                    const uint32_t src = tmem + (nd & 1) * buffer + (part ? m.Dn : 0) + lanes;
+                    // the copies out of the staging rows that this warp wrote before have read them (a warp stages and sends its own 32 rows)
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        uint32_t r[32];
+                        tc05::ld_32x32b_x32(src + c0, r);
+                        tc05::wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8) {
+                            uint4 w = make_uint4(0, 0, 0, 0);     // rows behind the context: zeros, whatever the cache holds there
+                            if (live)
+                                w = make_uint4(pack2<BF>(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), pack2<BF>(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])),
+                                               pack2<BF>(__uint_as_float(r[c + 4]), __uint_as_float(r[c + 5])), pack2<BF>(__uint_as_float(r[c + 6]), __uint_as_float(r[c + 7])));
+                            const int chunk = (c0 + c) / 8;
+                            *reinterpret_cast<uint4*>(sm.out[chunk >> 3] + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = w;
+                        }
+                    }
+                    if (part == 1) {
+                        tc05::fence_before_thread_sync();
+                        warp_arrive(&sm.d_free[nd & 1]);
+                    }
+                    tc05::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int y = (int)(h * a.rows + it.row + warp * 32);
+                        for (int c = 0; c < D / 64; ++c)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(part ? &a.map_v_out : &a.map_k_out),
+                                         "r"(64 * c), "r"(y), "r"(pa::smem_u32(sm.out[c] + warp * 32 * 128)) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == 5) tc05::tmem_dealloc(tmem, 512);
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------------------
+// A work item is 256 new tokens of one head in two halves A and B of 128 rows.  S_X = Q_X K^T (M 128, N 128) into TMEM, P_X over S_X, O_X += P_X V
+// with P read from TMEM; the tensor core computes P V and the next S of one half beside the softmax of the other.
+// Warps 0 - 3 and 4 - 7: softmax of A and B, a thread per row; 8: loader, 9: products; 10, 11 fill the warpgroup whose registers go to the softmax.
+constexpr int kAttendThreads = 384;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 and 128 threads of the 384 x 168 that the CTA is launched with
+constexpr int kItemSlots = 4;
+constexpr float kGrow = 4.f;       // log2 of the growth of a row maximum that rescales O
+
+struct QueryItem {
+    int h;               // head of this pass, -1: no more items
+    int t0;              // first new token of the item
+    int rows;            // its new tokens
+    int past;            // context its first row sees, less one
+    int row;             // first row of the sequence's context in the scratch
+    int tiles[2];        // context tiles of each half
+};
+
+template <int DN, int DV>
+struct ExpandedSmem {
+    static constexpr int NQ = DN / 64 + 1, NV = DV / 64;
+    static constexpr int KS = DN == 128 ? 2 : 3, VS = DN == 128 && DV == 128 ? 2 : 4;    // tiles of keys (128 tokens), of values (64 tokens)
+    alignas(1024) uint8_t q[2][NQ][128 * 128];
+    alignas(1024) uint8_t k[KS][NQ][kExpandTile * 128];
+    alignas(1024) uint8_t v[VS][NV][64 * 128];
+    uint64_t q_full[2], q_free[2], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2], o_done[2];
+    uint64_t item_full[kItemSlots], item_free[kItemSlots];
+    QueryItem item[kItemSlots];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+template <int DN, int DV, bool BF>
+__global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(const __grid_constant__ ExpandedArgs a) {
+    using Smem = ExpandedSmem<DN, DV>;
+    constexpr int NQ = Smem::NQ, NV = Smem::NV, KS = Smem::KS, VS = Smem::VS;
+    constexpr uint32_t kO = 256;       // S_A, S_B: 128 columns each (P in the first 64), then O_A, O_B
+    extern __shared__ uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const Step& m = a.m;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int x = 0; x < 2; ++x) {
+            pa::mbar_init(&sm.q_full[x], 1);
+            pa::mbar_init(&sm.q_free[x], 1);
+            pa::mbar_init(&sm.s_full[x], 1);
+            pa::mbar_init(&sm.p_full[x], 4);
+            pa::mbar_init(&sm.o_done[x], 1);
+        }
+        for (int i = 0; i < KS; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
+        for (int i = 0; i < VS; ++i) { pa::mbar_init(&sm.v_full[i], 1); pa::mbar_init(&sm.v_free[i], 1); }
+        for (int i = 0; i < kItemSlots; ++i) { pa::mbar_init(&sm.item_full[i], 1); pa::mbar_init(&sm.item_free[i], 9); }
+        pa::mbar_fence_init();
+        sm.abort_flag = 0;
+    }
+    if (warp == 9) tc05::tmem_alloc(&sm.tmem_base, 512);
+    tc05::fence_before_thread_sync();
+    __syncthreads();
+    tc05::fence_after_thread_sync();
+    const uint32_t tmem = sm.tmem_base;
+    const Waiter wt{&sm.abort_flag, m.status};
+    auto fetch = [&](uint32_t n, QueryItem& it) -> bool {
+        const int slot = n % kItemSlots;
+        if (!wt.wait_warp(&sm.item_full[slot], (n / kItemSlots) & 1)) return false;
+        it = sm.item[slot];
+        warp_arrive(&sm.item_free[slot]);
+        return true;
+    };
+
+    if (warp >= 8) {
+        reg_dec<kOtherRegs>();
+        if (warp == 8) {
+            // ======================= loader =============================================================
+            const int items = a.query_prefix[m.num_sequences] * a.heads;
+            uint32_t ni = 0, nk = 0, nv = 0, nq[2] = {0, 0};
+            bool ok = true;
+            while (ok) {
+                int i = 0;
+                if (lane == 0) i = atomicAdd(a.counter + a.pass, 1);
+                i = __shfl_sync(0xffffffffu, i, 0);
+                QueryItem it;
+                it.h = -1;
+                if (i < items) {
+                    const int2 at = a.order[i / a.heads];
+                    SeqView v;
+                    seq_view(m, at.x, v);
+                    it.h = i % a.heads;
+                    it.t0 = v.t0 + at.y * kQueryTile;
+                    it.rows = min(kQueryTile, v.n - at.y * kQueryTile);
+                    it.past = v.past + at.y * kQueryTile;
+                    it.row = a.tile_prefix[at.x] * kExpandTile;
+                    for (int x = 0; x < 2; ++x) {
+                        const int last = min(it.rows, 128 * (x + 1));     // rows up to the half's end
+                        it.tiles[x] = last > 128 * x ? (it.past + last + kExpandTile - 1) / kExpandTile : 0;
+                    }
+                }
+                const int slot = ni % kItemSlots;
+                if (ni >= kItemSlots) ok = wt.wait_warp(&sm.item_free[slot], (ni / kItemSlots - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) sm.item[slot] = it;
+                warp_arrive(&sm.item_full[slot]);
+                ++ni;
+                if (it.h < 0) break;
+                const int tiles = max(it.tiles[0], it.tiles[1]);
+                for (int x = 0; ok && x < 2; ++x) {
+                    if (it.tiles[x] == 0) continue;
+                    if (nq[x] > 0) ok = wt.wait_warp(&sm.q_free[x], (nq[x] - 1) & 1);
+                    if (ok && lane == 0) {
+                        pa::mbar_expect_tx(&sm.q_full[x], NQ * 128 * 128);
+                        for (int c = 0; c < NQ - 1; ++c) tma_3d(sm.q[x][c], &a.map_qn, 64 * c, a.h0 + it.h, it.t0 + 128 * x, &sm.q_full[x]);
+                        tma_3d(sm.q[x][NQ - 1], &a.map_qr, 0, a.h0 + it.h, it.t0 + 128 * x, &sm.q_full[x]);
+                    }
+                    __syncwarp();
+                    ++nq[x];
+                }
+                const int y0 = (int)(it.h * a.rows) + it.row;
+                auto load_k = [&](int j) {
+                    const int st = nk % KS;
+                    if (nk >= KS) ok = wt.wait_warp(&sm.k_free[st], (nk / KS - 1) & 1);
+                    if (!ok) return;
+                    if (lane == 0) {
+                        pa::mbar_expect_tx(&sm.k_full[st], NQ * kExpandTile * 128);
+                        for (int c = 0; c < NQ - 1; ++c) tma_2d(sm.k[st][c], &a.map_k, 64 * c, y0 + j * kExpandTile, &sm.k_full[st]);
+                        tma_2d(sm.k[st][NQ - 1], &a.map_k_rope, 0, it.row + j * kExpandTile, &sm.k_full[st]);
+                    }
+                    __syncwarp();
+                    ++nk;
+                };
+                for (int j = 0; ok && j < tiles; ++j) {
+                    if (j == 0) load_k(0);
+                    if (ok && j + 1 < tiles) load_k(j + 1);
+                    for (int u = 0; ok && u < 2; ++u) {
+                        const int st = nv % VS;
+                        if (nv >= VS) ok = wt.wait_warp(&sm.v_free[st], (nv / VS - 1) & 1);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            pa::mbar_expect_tx(&sm.v_full[st], NV * 64 * 128);
+                            for (int c = 0; c < NV; ++c) tma_2d(sm.v[st][c], &a.map_v, 64 * c, y0 + j * kExpandTile + 64 * u, &sm.v_full[st]);
+                        }
+                        __syncwarp();
+                        ++nv;
+                    }
+                }
+            }
+            if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
+                auto drain = [&](uint64_t* bar, uint32_t parity) {
+                    for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(bar, parity); ++k) {}
+                };
+                for (int x = 0; x < 2; ++x)
+                    if (nq[x] > 0) drain(&sm.q_full[x], (nq[x] - 1) & 1);
+                for (uint32_t i = nk > KS ? nk - KS : 0; i < nk; ++i) drain(&sm.k_full[i % KS], (i / KS) & 1);
+                for (uint32_t i = nv > VS ? nv - VS : 0; i < nv; ++i) drain(&sm.v_full[i % VS], (i / VS) & 1);
+            }
+        } else if (warp == 9) {
+            // ======================= products ============================================================
+            constexpr uint32_t idesc_s = tc05::instr_desc_f16(128, kExpandTile, BF ? 1 : 0, 0, 0);
+            constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 1);
+            const uint64_t dq = tc05::smem_desc_sw128(pa::smem_u32(sm.q), 1024), dk = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024);
+            const uint64_t dv = tc05::smem_desc_sw128(pa::smem_u32(sm.v), 1024, 64 * 128);
+            constexpr uint32_t kAtom = 128 * 128 >> 4;
+            const int rope_steps = m.P / 16;
+            uint32_t ni = 0, nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0};   // tiles of keys, units of values, before this item; query tiles, P tiles so far
+            bool ok = true;
+            QueryItem it;
+            for (; ok; ++ni) {
+                if (!fetch(ni, it) || it.h < 0) break;
+                const int tiles = max(it.tiles[0], it.tiles[1]);
+                const int last_half = it.tiles[1] > 0 ? 1 : 0;      // B sees no fewer tiles than A, where it has rows
+                auto issue_s = [&](int X, int j) {
+                    const int st = (nk + j) % KS;
+                    ok = wt.wait_warp(&sm.k_full[st], ((nk + j) / KS) & 1);
+                    if (!ok) return;
+                    tc05::fence_after_thread_sync();
+                    const uint64_t da = dq + X * NQ * kAtom, db = dk + st * NQ * kAtom;
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < DN / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 2;
+                            if (kk == 0) tc05::mma_ss<0>(tmem + X * 128, da + off, db + off, idesc_s);
+                            else tc05::mma_ss<1>(tmem + X * 128, da + off, db + off, idesc_s);
+                        }
+                        for (int kk = 0; kk < rope_steps; ++kk) tc05::mma_ss<1>(tmem + X * 128, da + (NQ - 1) * kAtom + 2 * kk, db + (NQ - 1) * kAtom + 2 * kk, idesc_s);
+                        tc05::commit(&sm.s_full[X]);
+                        if (X == last_half) tc05::commit(&sm.k_free[st]);
+                        if (j + 1 == it.tiles[X]) tc05::commit(&sm.q_free[X]);
+                    }
+                    __syncwarp();
+                };
+                auto issue_o = [&](int X, int j) {
+                    ok = wt.wait_warp(&sm.p_full[X], np[X] & 1);
+                    ++np[X];
+                    for (int u = 0; ok && u < 2; ++u) {
+                        const int st = (nv + 2 * j + u) % VS;
+                        ok = wt.wait_warp(&sm.v_full[st], ((nv + 2 * j + u) / VS) & 1);
+                        if (!ok) return;
+                        tc05::fence_after_thread_sync();
+                        if (tc05::elect_one()) {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const uint32_t p = tmem + X * 128 + u * 32 + kk * 8;
+                                const uint64_t db = dv + st * (NV * 64 * 128 >> 4) + kk * 128;
+                                if (kk == 0 && u == 0 && j == 0) tc05::mma_ts<0>(tmem + kO + X * DV, p, db, idesc_o);
+                                else tc05::mma_ts<1>(tmem + kO + X * DV, p, db, idesc_o);
+                            }
+                            if (X == last_half) tc05::commit(&sm.v_free[st]);
+                            if (u == 1 && j + 1 == it.tiles[X]) tc05::commit(&sm.o_done[X]);
+                        }
+                        __syncwarp();
+                    }
+                };
+                for (int X = 0; ok && X < 2; ++X)
+                    if (it.tiles[X] > 0) {
+                        ok = wt.wait_warp(&sm.q_full[X], nq[X] & 1);
+                        ++nq[X];
+                        if (ok) issue_s(X, 0);
+                    }
+                for (int j = 0; ok && j < tiles; ++j)
+                    for (int X = 0; ok && X < 2; ++X)
+                        if (j < it.tiles[X]) {
+                            issue_o(X, j);
+                            if (ok && j + 1 < it.tiles[X]) issue_s(X, j + 1);
+                        }
+                nk += tiles;
+                nv += 2 * tiles;
+            }
+        }
+    } else {
+        // ======================= softmax and output of half X ============================================
+        reg_inc<kSoftmaxRegs>();
+        const int X = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem + X * 128 + lanes, tmem_o = tmem + kO + X * DV + lanes;
+        const float c2 = a.scale_log2;
+        uint32_t n = 0, no = 0;
+        QueryItem it;
+        for (uint32_t ni = 0;; ++ni) {
+            if (!fetch(ni, it) || it.h < 0) break;
+            const int tiles = it.tiles[X];
+            if (tiles == 0) continue;
+            const int i = 128 * X + r;                      // row of the item
+            const int limit = i < it.rows ? it.past + i + 1 : 0;
+            float top = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int j = 0; j < tiles; ++j, ++n) {
+                if (!wt.wait_warp(&sm.s_full[X], n & 1)) { ok = false; break; }
+                tc05::fence_after_thread_sync();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tc05::ld_32x32b_x32(tmem_s + 32 * q, s[q]);
+                tc05::wait_ld();
+                const int seen = limit - j * kExpandTile;
+                if (__any_sync(0xffffffffu, seen < kExpandTile)) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (32 * q + c >= seen) s[q][c] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    mx[q] = __uint_as_float(s[q][0]);
+#pragma unroll
+                    for (int c = 1; c < 31; c += 2) mx[q] = max3(mx[q], __uint_as_float(s[q][c]), __uint_as_float(s[q][c + 1]));
+                    mx[q] = fmaxf(mx[q], __uint_as_float(s[q][31]));
+                }
+                const float t = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+                float alpha = 1.f;
+                bool grew = false;
+                if (top == -INFINITY) top = t;
+                else if (t > top + kGrow) { alpha = ex2(top - t); top = t; grew = true; }
+                if (__any_sync(0xffffffffu, grew)) {     // (the products of the tile before are complete: they precede this tile's S)
+#pragma unroll 1
+                    for (int q = 0; q < DV / 32; ++q) {
+                        uint32_t o[32];
+                        tc05::ld_32x32b_x32(tmem_o + 32 * q, o);
+                        tc05::wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                        tc05::st_32x32b_x32(tmem_o + 32 * q, o);
+                    }
+                    l *= alpha;
+                }
+                const float ref = top == -INFINITY ? 0.f : -top;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2) {
+                        const float x = ex2(fmaf(__uint_as_float(s[q + (c >> 5)][c & 31]), c2, ref)), y = ex2(fmaf(__uint_as_float(s[q + (c >> 5)][(c & 31) + 1]), c2, ref));
+                        sum[c & 2] += x;
+                        sum[(c & 2) + 1] += y;
+                        p[c >> 1] = pack2<BF>(x, y);
+                    }
+                    tc05::st_32x32b_x32(tmem_s + 16 * q, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc05::wait_st();
+                tc05::fence_before_thread_sync();
+                warp_arrive(&sm.p_full[X]);
+            }
+            if (!ok || !wt.wait_warp(&sm.o_done[X], no & 1)) break;
+            ++no;
+            tc05::fence_after_thread_sync();
+            const float inv = 1.f / l;
+            uint4* dst = reinterpret_cast<uint4*>((uint16_t*)a.output + ((long long)(it.t0 + i) * m.H + a.h0 + it.h) * DV);
+#pragma unroll 1
+            for (int q = 0; q < DV / 32; ++q) {
+                uint32_t o[32];
+                tc05::ld_32x32b_x32(tmem_o + 32 * q, o);
+                tc05::wait_ld();
+                if (limit > 0) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack2<BF>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+                        dst[4 * q + c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            tc05::fence_before_thread_sync();
+        }
+    }
+    __syncthreads();
+    if (warp == 9) tc05::tmem_dealloc(tmem, 512);
+}
+
+template <int DN, int DV, bool BF>
+cudaError_t attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream) {
+    const int smem = sizeof(ExpandedSmem<DN, DV>) + 1024;
+    // the warpgroups re-divide the registers that the CTA was launched with: fewer than this would leave one of them waiting
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, expanded_attend_kernel<DN, DV, BF>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs * kAttendThreads < 256 * kSoftmaxRegs + 128 * kOtherRegs) return cudaErrorInvalidConfiguration;
+    const cudaError_t e = cudaFuncSetAttribute(expanded_attend_kernel<DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    expanded_attend_kernel<DN, DV, BF><<<sm_count, kAttendThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+template <int R, bool BF>
+cudaError_t launch(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
+    const int smem = sizeof(ExpandSmem<R>) + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(expand_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    expand_kernel<R, BF><<<sm_count, kExpandThreads, smem, stream>>>(a);
+    *launches += 2;
+    if (a.m.Dn == 128) return a.m.Dv == 128 ? attend<128, 128, BF>(a, sm_count, stream) : attend<128, 64, BF>(a, sm_count, stream);
+    return a.m.Dv == 128 ? attend<64, 128, BF>(a, sm_count, stream) : attend<64, 64, BF>(a, sm_count, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_expanded_plan(const ExpandedArgs& a, cudaStream_t stream, int* launches) {
+    expanded_plan_kernel<<<1, 256, 0, stream>>>(a);
+    ++*launches;
+    return cudaGetLastError();
+}
+
+cudaError_t launch_expanded(const ExpandedArgs& a, int dtype, int sm_count, cudaStream_t stream, int* launches) {
+    if (dtype == PA_DTYPE_BF16) return a.m.R == 512 ? launch<512, true>(a, sm_count, stream, launches) : launch<256, true>(a, sm_count, stream, launches);
+    return a.m.R == 512 ? launch<512, false>(a, sm_count, stream, launches) : launch<256, false>(a, sm_count, stream, launches);
+}
+
+}  // namespace latent

@@ -38,22 +38,6 @@ struct AppendArgs {
     void* cache;
 };
 
-struct AttentionArgs {
-    Step m;
-    const void* q_nope;
-    long long qn_token, qn_head;
-    const void* q_rope;
-    long long qr_token, qr_head;
-    const void* key_up;
-    long long key_up_head;
-    const void* value_up;
-    long long value_up_head;
-    void* output;
-    const void* cache;
-    float scale;
-    int min_new;                // sequences with fewer new tokens are not served
-};
-
 // The absorbed form.  Its unit of work is a tile of 64 context tokens for a block of `row_tiles` tiles of 64 query rows (new token, head) of one
 // sequence; sequence s has block_prefix[s + 1] - block_prefix[s] such blocks, every one of the same number of tiles.  Units are
 // numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut, or
@@ -80,8 +64,32 @@ struct AbsorbedArgs {
 long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);
 cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t stream, int* launches);
 
+// The expanded form.  Keys and values of the context are made per head in scratch, whose rows are the contexts of the served sequences one
+// after another, each in whole tiles of 128 tokens (rows behind a context are zero); then every (256 new tokens, head) attends over them.
+constexpr int kExpandTile = 128;   // context tokens of a tile
+constexpr int kQueryTile = 256;    // new tokens of a work item, in two halves
+
+struct ExpandedArgs {
+    Step m;
+    int min_new;                // sequences with fewer new tokens are left to the absorbed form
+    int h0, heads;              // heads of this pass
+    long long rows;             // rows of a head's scratch
+    int* tile_prefix;           // [num_sequences + 1] context tiles
+    int* query_prefix;          // [num_sequences + 1] query tiles
+    int2* order;                // (sequence, query tile), longest context first
+    int* counter;               // [passes] work counters
+    int pass, passes;
+    const void* cache;
+    void* k_rope;               // [rows][64] rotated key part (the same for every head)
+    void* output;
+    float scale_log2;           // softmax scale * log2(e)
+    // k, v: the scratch [heads * rows][Dn] and [heads * rows][Dv], written 32 rows and read 128 (k) or 64 (v) rows at a time
+    CUtensorMap map_cache, map_key_up, map_value_up, map_k_out, map_v_out, map_k, map_v, map_k_rope, map_qn, map_qr;
+};
+cudaError_t launch_expanded_plan(const ExpandedArgs& a, cudaStream_t stream, int* launches);
+cudaError_t launch_expanded(const ExpandedArgs& a, int dtype, int sm_count, cudaStream_t stream, int* launches);
+
 cudaError_t launch_append(const AppendArgs& a, int dtype, cudaStream_t stream, int* launches);
-cudaError_t launch_attention_simple(const AttentionArgs& a, int dtype, cudaStream_t stream, int* launches);
 
 #ifdef __CUDACC__
 // One sequence's slice of the metadata, checked before anything is indexed with it: begins monotone and inside the arrays they
