@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
         build_plan(a);
         return;
     }
-    const int parts = m.R / 128, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int parts = m.R / 128, tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     const int i = blockIdx.x - 1, part = i % parts, h = i / parts % m.H, t0 = i / parts / m.H * kTile;
     if (!tile_rows(a, t0, live)) return;
     uint8_t* const sw = smem;                        // two atoms of [Dn][64 latent elements]
@@ -113,10 +113,14 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
     bool ok = wt.wait(&full, 0);
     if (warp == 0 && __all_sync(0xffffffffu, ok)) {
         constexpr uint32_t idesc = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
-        const uint64_t da = tc05::smem_desc_sw128(pa::smem_u32(sw), 1024, m.Dn * 128), db = tc05::smem_desc_sw128(pa::smem_u32(sq), 1024);
+        const uint32_t da = desc_low(sw, m.Dn * 128), db = desc_low(sq);
         if (tc05::elect_one()) {
-            for (int kk = 0; kk < m.Dn / 16; ++kk)
-                tc05::mma_ss(tmem, da + 128 * kk, db + ((kk >> 2) * 8192 + (kk & 3) * 32 >> 4), idesc, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+                const uint32_t pa = da + 128 * kk, pb = db + (kk >> 2) * 512 + (kk & 3) * 2;
+                if (kk == 0) mma_ss<0>(tmem, pa, pb, idesc);
+                else if (kk < 4 || m.Dn == 128) mma_ss<1>(tmem, pa, pb, idesc);
+            }
             tc05::commit(&done);
         }
     }
@@ -151,13 +155,15 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
 
 // ---- attention over the latents ------------------------------------------------------------------------------------------
 // Roles meet through mbarriers only: a loader warp walks the slice and has the TMA engine bring query rows and 64-token tiles of the cache,
-// one warp issues the products, four warps (64 rows, 16 a warp) do the softmax and write the partial results.
+// one warp issues the products, four warps (64 rows, 16 a warp) do the softmax, four more rescale O and write results.
 //   S[row][token]     = Q~ K^T          M 64, N 64, K R + P; two buffers, so that S of the next tile is computed beside a softmax
 //   O^T[latent][row] += K^T P^T         M 128 (R / 128 times), N 64, K 64: the tile is read MN-major from the same image, and the
 //                                       rows (heads) are columns, so few heads leave no tensor-memory lane idle
+// A tile lies in shared memory in groups of eight tokens, [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view
+// of the cache, so a block is two copies (the rotated part is the other) whatever the block size; issuing nine took 900 cycles.
 constexpr int kSlots = 4;               // depth of the queue of runs
-constexpr int kThreads = 192;           // warps 0 - 3: softmax, 4: loader, 5: products
-constexpr float kLazy = 4.f;            // log2 of the growth of a row maximum that rescales O
+constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: products, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)
+constexpr float kLazy = 8.f;            // log2 of the growth of a row maximum that rescales O
 
 // A stretch of context tiles of one row tile.
 struct Run {
@@ -168,22 +174,32 @@ struct Run {
     int first, tiles;    // context tiles
     int end;             // context the tile's last row sees
     int tb;
+    bool whole;          // all of the row tile's context: no other CTA has a part of it
     long long slot;
 };
 
 template <int R>
 struct AttendSmem {
-    static constexpr int NC = R / 64 + 1;           // 64-element chunks of a row, the last one the rotated part
     static constexpr int NST = R == 512 ? 2 : 4;    // context tiles in flight
-    alignas(1024) uint8_t q[NC][kTile * 128];
-    alignas(1024) uint8_t k[NST][NC][kTile * 128];
+    alignas(1024) uint8_t q[kTile * R * 2];
+    alignas(1024) uint8_t q_rope[kTile * 128];
+    struct Tile {
+        uint8_t c[kTile * R * 2];
+        uint8_t rope[kTile * 128];
+    };
+    alignas(1024) Tile k[NST];
     alignas(1024) uint8_t p[kTile * 128];           // [row][token]
     float alpha[2][kTile];
+    float2 stat[2][kTile];                          // maximum and sum of the rows of a run
     volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
+    volatile int event;                             // what the results warps are asked for: rescale after tile `event` - 1, or results (0)
     uint64_t k_full[NST], k_free[NST];              // loader -> products (bytes), products -> loader
     uint64_t q_full, q_free;
-    uint64_t vote;                                  // softmax warps among themselves
-    uint64_t s_full[2], p_full, o_done;             // products -> softmax, softmax -> products, products -> softmax
+    uint64_t s_full[2], p_full, o_done;             // products -> softmax, softmax -> products, products -> softmax and results
+    uint64_t asked, answered;                       // products -> results, results -> products
+    // softmax -> results, runs in turn: the softmax can be a run ahead of the results, and no more, because the first P of a run waits for the last
+    // product of the run before, whose first product waits for the results before that
+    uint64_t stat_full[2];
     uint64_t run_full[kSlots], run_free[kSlots];
     Run run[kSlots];
     uint32_t tmem_base;
@@ -193,22 +209,26 @@ struct AttendSmem {
 template <int R, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AbsorbedArgs a) {
     using Smem = AttendSmem<R>;
-    constexpr int NC = Smem::NC, NST = Smem::NST, MT = R / 128;
+    constexpr int NC = R / 64, NST = Smem::NST, MT = R / 128;
+    constexpr uint32_t kGroup = NC * 1024;          // bytes from one group of eight rows to the next
     constexpr uint32_t kTmemS = MT * kTile;         // O^T: MT x 64 columns, then S twice
     extern __shared__ uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const Step& m = a.m;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
         pa::mbar_init(&sm.q_full, 1);
         pa::mbar_init(&sm.q_free, 1);
         pa::mbar_init(&sm.s_full[0], 1);
         pa::mbar_init(&sm.s_full[1], 1);
-        pa::mbar_init(&sm.vote, 4);
         pa::mbar_init(&sm.p_full, 4);
         pa::mbar_init(&sm.o_done, 1);
-        for (int i = 0; i < kSlots; ++i) { pa::mbar_init(&sm.run_full[i], 1); pa::mbar_init(&sm.run_free[i], 5); }
+        pa::mbar_init(&sm.asked, 1);
+        pa::mbar_init(&sm.answered, 4);
+        pa::mbar_init(&sm.stat_full[0], 4);
+        pa::mbar_init(&sm.stat_full[1], 4);
+        for (int i = 0; i < kSlots; ++i) { pa::mbar_init(&sm.run_full[i], 1); pa::mbar_init(&sm.run_free[i], 9); }
         pa::mbar_fence_init();
         sm.grew[0] = sm.grew[1] = 0;
         sm.abort_flag = 0;
@@ -236,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         const long long u_end = min(total, u + per);
         uint32_t n = 0, nr = 0, nq = 0;      // tiles, queue entries, query tiles so far
         bool ok = true, bad_index = false;
-        if (lane == 0) { prefetch_map(&a.map_cache); prefetch_map(&a.map_q_abs); }
         int s = 0;
         if (u < u_end) {
             int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
@@ -271,16 +290,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 r.first = first;
                 r.tiles = max(0, min(first + len, (r.end + kTile - 1) / kTile) - first);
                 r.tb = v.tb;
+                r.whole = len == tiles;
                 r.slot = ((long long)a.block_prefix[s] + block + group) * a.row_tiles + member;
                 ok = publish(r);
                 if (ok && r.tiles > 0) {
                     if (nq > 0) ok = wt.wait_warp(&sm.q_free, (nq - 1) & 1);
-                    if (ok && lane == 0) {
-                        const int pieces = (r.rows + 15) / 16;   // of 16 rows
-                        pa::mbar_expect_tx(&sm.q_full, pieces * 16 * 128 * NC);
-                        for (int c = 0; c < NC; ++c)
-                            for (int i = 0; i < pieces; ++i) tma_2d(sm.q[c] + i * 2048, &a.map_q_abs, 64 * c, (int)r.grow0 + 16 * i, &sm.q_full);
+                    if (ok && tc05::elect_one()) {
+                        pa::mbar_expect_tx(&sm.q_full, kTile * (R * 2 + 128));     // (rows behind the tile's are other rows' or zeros)
+                        tma_3d(sm.q, &a.map_q_abs, 0, (int)r.grow0, 0, &sm.q_full);
+                        tma_2d(sm.q_rope, &a.map_q_abs_rope, 0, (int)r.grow0, &sm.q_full);
                     }
+                    __syncwarp();
                     ++nq;
                     const int per_tile = kTile / m.bs, last_block = (r.end - 1) / m.bs;
                     int page = 0, base = -1;     // this lane's block of the 32 from `base`
@@ -296,11 +316,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                         }
                         const int st = n % NST;
                         if (n >= NST) ok = wt.wait_warp(&sm.k_free[st], (n / NST - 1) & 1);
-                        if (ok && lane == 0) pa::mbar_expect_tx(&sm.k_full[st], blocks * m.bs * 128 * NC);
+                        if (!ok) break;
+                        if (tc05::elect_one()) pa::mbar_expect_tx(&sm.k_full[st], blocks * m.bs * (R * 2 + 128));
+                        __syncwarp();
                         for (int i = 0; i < blocks; ++i) {
-                            const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * m.bs;
-                            if (ok && lane == 0)
-                                for (int c = 0; c < NC; ++c) tma_2d(sm.k[st][c] + i * m.bs * 128, &a.map_cache, 64 * c, at, &sm.k_full[st]);
+                            const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * (m.bs / 8);
+                            if (tc05::elect_one()) {
+                                tma_4d(sm.k[st].c + i * (m.bs / 8) * kGroup, &a.map_cache, 0, 0, 0, at, &sm.k_full[st]);
+                                tma_3d(sm.k[st].rope + i * m.bs * 128, &a.map_cache_rope, 0, 0, at, &sm.k_full[st]);
+                            }
+                            __syncwarp();
                         }
                     }
                 }
@@ -321,15 +346,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         }
     } else if (warp == 5) {
         // ======================= products ================================================================
+        // (the whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took twice as long to issue)
         constexpr uint32_t idesc_s = tc05::instr_desc_f16(kTile, kTile, BF ? 1 : 0, 0, 0);
         constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
-        const uint64_t dq = tc05::smem_desc_sw128(pa::smem_u32(sm.q), 1024), dk = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024);
-        const uint64_t dv = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024, kTile * 128), dp = tc05::smem_desc_sw128(pa::smem_u32(sm.p), 1024);
-        constexpr uint32_t kStage = NC * kTile * 128 >> 4;
-        const int last_steps = m.P / 16;
-        uint32_t n = 0;
+        const uint32_t dq = desc_low(sm.q), dqr = desc_low(sm.q_rope), dk = desc_low(sm.k[0].c), dkr = desc_low(sm.k[0].rope);
+        const uint32_t dv = desc_low(sm.k[0].c, 1024), dp = desc_low(sm.p);
+        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4;
+        const bool wide = m.P == 64;
+        uint32_t n = 0, asked = 0;
         bool ok = true;
         Run r;
+        auto ask = [&](int event) {
+            if (lane == 0) sm.event = event;
+            warp_arrive(&sm.asked);
+            ++asked;
+        };
         for (uint32_t nr = 0, nq = 0; ok; ++nr) {
             if (!fetch(nr, r) || r.rows == 0) break;
             if (r.tiles == 0) continue;
@@ -338,22 +369,49 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             const uint32_t end = n + r.tiles;
             uint32_t next_s = n, next_o = n;
             uint32_t idle = 0;
-            // S of a tile as soon as the tile is there, but no more than one ahead of O; O as soon as its P is
+            // O as soon as its P is there; S of a tile as soon as the tile is, but no more than one ahead of O
             while (ok && next_o < end) {
-                if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, pa::mbar_try_wait(&sm.k_full[next_s % NST], (next_s / NST) & 1))) {
-                    const uint64_t db = dk + (next_s % NST) * kStage;
-                    const uint32_t d = tmem + kTmemS + (next_s & 1) * kTile;
+                if (next_o < next_s && __all_sync(0xffffffffu, mbar_test(&sm.p_full, next_o & 1))) {
+                    if (next_o == n) {
+                        // the first product overwrites O: the results of the run before have been read
+                        if (asked > 0) ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
+                    } else if (sm.grew[next_o & 1] == next_o + 1) {
+                        ask((int)next_o);
+                        ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
+                    }
+                    if (!ok) break;
+                    tc05::fence_after_thread_sync();
+                    const uint32_t da = dv + next_o % NST * kStage;
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            const uint32_t d = tmem + mt * kTile, pa = da + mt * (2048 >> 4);
+                            if (next_o > n) mma_ss<1, kGroup>(d, pa, dp, idesc_o);
+                            else mma_ss<0, kGroup>(d, pa, dp, idesc_o);
+#pragma unroll
+                            for (int kk = 1; kk < kTile / 16; ++kk) mma_ss<1, kGroup>(d, pa + kk * (2 * kGroup >> 4), dp + kk * 2, idesc_o);
+                        }
+                        tc05::commit(&sm.k_free[next_o % NST]);
+                        tc05::commit(&sm.o_done);
+                    }
+                    __syncwarp();
+                    ++next_o;
+                    idle = 0;
+                } else if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, mbar_test(&sm.k_full[next_s % NST], (next_s / NST) & 1))) {
+                    const uint32_t db = dk + next_s % NST * kStage, dbr = dkr + next_s % NST * kStage, d = tmem + kTmemS + (next_s & 1) * kTile;
                     tc05::fence_after_thread_sync();
                     if (tc05::elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < R / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2;
-                            if (kk == 0) tc05::mma_ss<0>(d, dq + off, db + off, idesc_s);
-                            else tc05::mma_ss<1>(d, dq + off, db + off, idesc_s);
+                            const uint32_t qa = dq + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, kb = db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2;
+                            if (kk == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
+                            else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
                         }
-                        for (int kk = 0; kk < last_steps; ++kk) {
-                            const uint32_t off = (R / 64) * (kTile * 128 >> 4) + kk * 2;
-                            tc05::mma_ss<1>(d, dq + off, db + off, idesc_s);
+                        mma_ss<1>(d, dqr, dbr, idesc_s);
+                        mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
+                        if (wide) {
+                            mma_ss<1>(d, dqr + 4, dbr + 4, idesc_s);
+                            mma_ss<1>(d, dqr + 6, dbr + 6, idesc_s);
                         }
                         tc05::commit(&sm.s_full[next_s & 1]);
                         if (next_s + 1 == end) tc05::commit(&sm.q_free);
@@ -361,37 +419,89 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     __syncwarp();
                     ++next_s;
                     idle = 0;
-                } else if (next_o < next_s && __all_sync(0xffffffffu, pa::mbar_try_wait(&sm.p_full, next_o & 1))) {
-                    const uint64_t da = dv + (next_o % NST) * kStage;
-                    const uint32_t acc = next_o > n ? 1u : 0u;
-                    tc05::fence_after_thread_sync();
-                    if (tc05::elect_one()) {
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int kk = 0; kk < kTile / 16; ++kk)
-                                tc05::mma_ss(tmem + mt * kTile, da + mt * 2 * (kTile * 128 >> 4) + kk * 128, dp + kk * 2, idesc_o, kk > 0 ? 1u : acc);
-                        tc05::commit(&sm.k_free[next_o % NST]);
-                        tc05::commit(&sm.o_done);
-                    }
-                    __syncwarp();
-                    ++next_o;
-                    idle = 0;
-                } else if (++idle > (1u << 21)) {
-                    wt.give_up();
-                    ok = false;
-                } else if ((idle & 255u) == 255u && __any_sync(0xffffffffu, sm.abort_flag)) {
+                } else if (++idle > (1u << 26)) {
+                    ok = wt.give_up();
+                } else if ((idle & 1023u) == 1023u && __any_sync(0xffffffffu, *wt.abort)) {
                     ok = false;
                 }
             }
             n = end;
+            if (ok) ask(-1);
         }
-    } else {
-        // ======================= softmax and partial results ==============================================
+    } else if (warp >= 8) {
+        // ======================= rescaling and results ====================================================
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int e = 32 * (warp & 3) + lane;           // latent element, of every 128
+        uint32_t n = 0, asked = 0;                      // tiles before this run, requests so far
+        Run r;
+        bool ok = true;
+        for (uint32_t nr = 0, ns = 0; ok; ++nr) {
+            if (!fetch(nr, r) || r.rows == 0) break;
+            for (; r.tiles > 0; ++asked) {
+                if (!wt.wait_warp(&sm.asked, asked & 1)) { ok = false; break; }
+                const int event = sm.event;
+                const uint32_t done = event >= 0 ? (uint32_t)event - 1 : n + r.tiles - 1;    // the products that have to be complete
+                if (!wt.wait_warp(&sm.o_done, done & 1)) { ok = false; break; }
+                tc05::fence_after_thread_sync();
+                if (event < 0) break;
+                const float* alpha = sm.alpha[event & 1];
+#pragma unroll 1
+                for (int q = 0; q < MT * 2; ++q) {
+                    uint32_t o[32];
+                    tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
+                    tc05::wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[(q & 1) * 32 + c]);
+                    tc05::st_32x32b_x32(tmem + 32 * q + lanes, o);
+                }
+                tc05::wait_st();
+                tc05::fence_before_thread_sync();
+                warp_arrive(&sm.answered);
+            }
+            if (!ok) break;
+            n += r.tiles;
+            if (r.tiles == 0) {
+                if (e < r.rows) a.part_ml[r.slot * kTile + e] = make_float2(-INFINITY, 0.f);
+                continue;
+            }
+            if (!wt.wait_warp(&sm.stat_full[ns & 1], (ns >> 1) & 1)) break;
+            const float2* stat = sm.stat[ns & 1];
+            ++ns;
+            if (!r.whole && e < r.rows) a.part_ml[r.slot * kTile + e] = stat[e];
+#pragma unroll 1
+            for (int q = 0; q < MT * 2; ++q) {
+                const int c0 = (q & 1) * 32;
+                if (c0 >= r.rows) continue;
+                uint32_t o[32];
+                tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
+                tc05::wait_ld();
+                if (r.whole) {
+                    uint16_t* dst = (uint16_t*)a.o_lat + (r.grow0 + c0) * (2 * R) + (q >> 1) * 128 + e;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (c0 + c < r.rows) {
+                            const float x = __uint_as_float(o[c]) * __frcp_rn(stat[c0 + c].y);
+                            const uint16_t hi = pack1<BF>(x);
+                            dst[c * (2 * R)] = hi;
+                            dst[c * (2 * R) + R] = pack1<BF>(x - unpack1<BF>(hi));
+                        }
+                } else {
+                    float* dst = a.part_o + (r.slot * kTile + c0) * R + (q >> 1) * 128 + e;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (c0 + c < r.rows) dst[c * R] = __uint_as_float(o[c]);
+                }
+            }
+            tc05::fence_before_thread_sync();
+            warp_arrive(&sm.answered);
+            ++asked;
+        }
+    } else if (warp < 4) {
+        // ======================= softmax ==================================================================
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const int rl[2] = {16 * warp + lane / 4, 16 * warp + lane / 4 + 8};
+        const int rl[2] = {16 * warp + lane / 4, 16 * warp + lane / 4 + 8};     // this thread's rows of S
         const float c2 = a.scale_log2;
-        uint32_t n = 0;
+        uint32_t n = 0, nst = 0;
         Run r;
         for (uint32_t nr = 0;; ++nr) {
             if (!fetch(nr, r) || r.rows == 0) break;
@@ -399,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < 2; ++x) limit[x] = rl[x] < r.rows ? r.past + (r.row0 + rl[x]) / m.H + 1 : 0;
+            const int least = __reduce_min_sync(0xffffffffu, min(limit[0], limit[1]));
             bool ok = true;
             for (int j = 0; j < r.tiles; ++j, ++n) {
                 if (!wt.wait_warp(&sm.s_full[n & 1], (n >> 1) & 1)) { ok = false; break; }
@@ -410,51 +521,40 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sv[e >> 1][2 * i + (e & 1)] = __uint_as_float(raw[4 * i + e]) * c2;
+                    for (int e = 0; e < 4; ++e) sv[e >> 1][2 * i + (e & 1)] = __uint_as_float(raw[4 * i + e]);
                 const int col0 = (r.first + j) * kTile;
-                float alpha[2] = {1.f, 1.f};
-                bool grew = false;
+                if (col0 + kTile > least) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (col0 + kTile > limit[x]) {
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
                             if (col0 + 8 * (c >> 1) + 2 * (lane & 3) + (c & 1) >= limit[x]) sv[x][c] = -INFINITY;
-                    }
-                    float t = sv[x][0];
+                }
+                bool grew = false;
 #pragma unroll
-                    for (int c = 1; c < 16; ++c) t = fmaxf(t, sv[x][c]);
+                for (int x = 0; x < 2; ++x) {
+                    float t = fmaxf(sv[x][0], sv[x][1]);
+#pragma unroll
+                    for (int c = 2; c < 16; c += 2) t = max3(t, sv[x][c], sv[x][c + 1]);
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2)) * c2;
+                    float alpha = 1.f;
                     // (a row that has seen nothing yet takes its first maximum without a rescale: its O is zero)
                     if (mx[x] == -INFINITY) mx[x] = t;
-                    else if (t > mx[x] + kLazy) { alpha[x] = ex2(mx[x] - t); mx[x] = t; grew = true; }
-                    if ((lane & 3) == 0) sm.alpha[n & 1][rl[x]] = alpha[x];
-                    const float ref = mx[x] == -INFINITY ? 0.f : mx[x];
-                    float sum = 0.f;
+                    else if (t > mx[x] + kLazy) { alpha = ex2(mx[x] - t); mx[x] = t; grew = true; }
+                    if ((lane & 3) == 0) sm.alpha[n & 1][rl[x]] = alpha;
+                    l[x] *= alpha;
+                    const float ref = mx[x] == -INFINITY ? 0.f : -mx[x];
+                    float sum[2] = {0.f, 0.f};
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) { sv[x][c] = ex2(sv[x][c] - ref); sum += sv[x][c]; }
-                    l[x] = l[x] * alpha[x] + sum;
-                }
-                // the warps agree on a rescale (a barrier of the hardware could not be left when a wait runs out)
-                if (grew) sm.grew[n & 1] = n + 1;
-                warp_arrive(&sm.vote);
-                if (!wt.wait_warp(&sm.vote, n & 1)) { ok = false; break; }
-                const bool rescale = sm.grew[n & 1] == n + 1;
-                if (n > 0 && !wt.wait_warp(&sm.o_done, (n - 1) & 1)) { ok = false; break; }
-                tc05::fence_after_thread_sync();
-                if (rescale) {
-#pragma unroll 1
-                    for (int q = 0; q < MT * 2; ++q) {
-                        uint32_t o[32];
-                        tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
-                        tc05::wait_ld();
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * sm.alpha[n & 1][(q & 1) * 32 + c]);
-                        tc05::st_32x32b_x32(tmem + 32 * q + lanes, o);
+                    for (int c = 0; c < 16; ++c) {
+                        sv[x][c] = ex2(fmaf(sv[x][c], c2, ref));
+                        sum[c & 1] += sv[x][c];
                     }
-                    tc05::wait_st();
+                    l[x] += sum[0] + sum[1];
                 }
+                if (grew) sm.grew[n & 1] = n + 1;
+                if (n > 0 && !wt.wait_warp(&sm.o_done, (n - 1) & 1)) { ok = false; break; }     // P of the tile before has been read
                 // P: a row's 64 tokens are 128 bytes, 16-byte pieces swizzled by the row
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
@@ -469,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     for (int i = tid; i < (kTile - valid) * 8; i += 128) {
                         const int row = valid + i / 8;
 #pragma unroll
-                        for (int c = 0; c < R / 64; ++c) *reinterpret_cast<uint4*>(sm.k[st][c] + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int c = 0; c < NC; ++c)
+                            *reinterpret_cast<uint4*>(sm.k[st].c + (row >> 3) * kGroup + c * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 tc05::fence_proxy_async_smem();
@@ -477,28 +578,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 warp_arrive(&sm.p_full);
             }
             if (!ok) break;
+            if (r.tiles == 0) continue;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-                if ((lane & 3) == 0 && rl[x] < r.rows) a.part_ml[r.slot * kTile + rl[x]] = make_float2(mx[x], l[x]);
+                if ((lane & 3) == 0) sm.stat[nst & 1][rl[x]] = make_float2(mx[x], l[x]);
             }
-            if (r.tiles == 0) continue;
-            if (!wt.wait_warp(&sm.o_done, (n - 1) & 1)) break;
-            tc05::fence_after_thread_sync();
-            float* dst = a.part_o + r.slot * kTile * R + 32 * warp + lane;
-#pragma unroll 1
-            for (int q = 0; q < MT * 2; ++q) {
-                const int c0 = (q & 1) * 32;
-                if (c0 >= r.rows) continue;
-                uint32_t o[32];
-                tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
-                tc05::wait_ld();
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    if (c0 + c < r.rows) dst[(long long)(c0 + c) * R + (q >> 1) * 128] = __uint_as_float(o[c]);
-            }
-            tc05::fence_before_thread_sync();
+            warp_arrive(&sm.stat_full[nst & 1]);
+            ++nst;
         }
     }
     __syncthreads();
@@ -506,54 +594,71 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 }
 
 // ---- joining the partial results of a row ----------------------------------------------------------------------------------
-// One CTA per row (new token, head): thread (piece group, four latent elements).  Leaves sum / denominator as two 16-bit pieces, so that the
-// product with value_up does not see another rounding.
+// A block of rows is cut where a slice begins inside it, so there are fewer cut blocks than slices: one CTA per (slice, row tile, four rows)
+// joins the block that its slice cuts first.  Leaves sum / denominator as two 16-bit pieces, so that the product with value_up does not
+// see another rounding.
+constexpr int kCombineRows = 4;
 template <int R, bool BF>
 __global__ void __launch_bounds__(R) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
-    constexpr int kPer = R / 4, kGroups = 4;       // threads of a piece group
-    __shared__ float4 sh[kGroups - 1][kPer];
+    constexpr int kPer = R / 4;                    // threads of a row, four latent elements each
+    extern __shared__ float weight[];              // [kCombineRows][pieces]
     const Step& m = a.m;
-    const int t = blockIdx.x / m.H, h = blockIdx.x % m.H, tid = threadIdx.x, g = tid / kPer, e = tid % kPer;
+    const int part = blockIdx.x % (kTile / kCombineRows), member = blockIdx.x / (kTile / kCombineRows) % a.row_tiles;
+    const long long w = blockIdx.x / (kTile / kCombineRows) / a.row_tiles + 1, total = a.unit_prefix[m.num_sequences], per = slice_size(a);
+    if (w * per >= total) return;
+    int lo = 0, hi = m.num_sequences;              // unit_prefix[lo] <= w * per < unit_prefix[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.unit_prefix[mid] <= w * per) lo = mid; else hi = mid;
+    }
     SeqView v;
-    const int s = find_sequence(m, t);
-    if (!seq_view(m, s, v) || t < v.t0 || t >= v.t0 + v.n || v.n > a.max_new) return;
-    const int row = (t - v.t0) * m.H + h, rt = row / kTile, block = rt / a.row_tiles;
-    const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, per = slice_size(a);
-    const long long u0 = a.unit_prefix[s] + block * tiles, w0 = u0 / per, w1 = (u0 + tiles - 1) / per;
-    const long long slot0 = ((long long)a.block_prefix[s] + block) * a.row_tiles + rt % a.row_tiles;
-    float top = -INFINITY, sum = 0.f;
-    for (long long w = w0; w <= w1; ++w) top = fmaxf(top, a.part_ml[(slot0 + w * a.row_tiles) * kTile + row % kTile].x);
-    for (long long w = w0; w <= w1; ++w) {
-        const float2 ml = a.part_ml[(slot0 + w * a.row_tiles) * kTile + row % kTile];
-        if (ml.y > 0.f) sum += ml.y * ex2(ml.x - top);
-    }
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (long long w = w0 + g; w <= w1; w += kGroups) {
-        const long long at = (slot0 + w * a.row_tiles) * kTile + row % kTile;
-        const float2 ml = a.part_ml[at];
-        if (ml.y > 0.f) {     // (a piece whose tiles the row does not see has no sums)
-            const float k = ex2(ml.x - top);
-            const float4 p = *reinterpret_cast<const float4*>(a.part_o + at * R + 4 * e);
-            x.x += k * p.x; x.y += k * p.y; x.z += k * p.z; x.w += k * p.w;
+    seq_view(m, lo, v);
+    const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, block = (w * per - a.unit_prefix[lo]) / tiles;
+    const long long u0 = a.unit_prefix[lo] + block * tiles, w0 = u0 / per, w1 = (u0 + tiles - 1) / per;
+    if (u0 == w * per || w0 + 1 != w) return;      // not cut here, or cut by an earlier slice
+    const int row0 = (int)(block * a.row_tiles + member) * kTile;
+    const int rows = (int)min((long long)kTile, (long long)v.n * m.H - row0) - part * kCombineRows;
+    if (rows <= 0) return;
+    const int pieces = (int)(w1 - w0) + 1, tid = threadIdx.x;
+    const long long slot0 = ((long long)a.block_prefix[lo] + block + w0) * a.row_tiles + member;
+    auto at = [&](int i, int row) { return (slot0 + (long long)i * a.row_tiles) * kTile + part * kCombineRows + row; };
+    // weights of the pieces: a warp per row
+    const int warp = tid >> 5, lane = tid & 31;
+    if (warp < kCombineRows && warp < rows) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < pieces; i += 32) {
+            const float2 ml = a.part_ml[at(i, warp)];
+            if (ml.y > 0.f) top = fmaxf(top, ml.x);
         }
+        top = pa::warp_max(top);
+        for (int i = lane; i < pieces; i += 32) {
+            const float2 ml = a.part_ml[at(i, warp)];
+            const float k = ml.y > 0.f ? ex2(ml.x - top) : 0.f;      // (a piece whose tiles the row does not see has no sums)
+            weight[warp * pieces + i] = k;
+            sum += k * ml.y;
+        }
+        sum = pa::warp_sum(sum);
+        for (int i = lane; i < pieces; i += 32) weight[warp * pieces + i] *= __frcp_rn(sum);
     }
-    if (g > 0) sh[g - 1][e] = x;
     __syncthreads();
-    if (g > 0) return;
-#pragma unroll
-    for (int i = 0; i < kGroups - 1; ++i) { const float4 p = sh[i][e]; x.x += p.x; x.y += p.y; x.z += p.z; x.w += p.w; }
-    const float inv = 1.f / sum;
-    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-    uint32_t hi[2], lo[2];
+    const int row = tid / kPer, e = tid % kPer;
+    if (row >= rows) return;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int i = 0; i < pieces; ++i) {
+        const float k = weight[row * pieces + i];
+        const float4 p = k != 0.f ? *reinterpret_cast<const float4*>(a.part_o + at(i, row) * R + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w;
+    }
+    uint32_t hi2[2], lo2[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
-        lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
+        hi2[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
+        lo2[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi2[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi2[i] >> 16)));
     }
-    uint16_t* dst = (uint16_t*)a.o_lat + ((long long)t * m.H + h) * (2 * R) + 4 * e;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo[0], lo[1]);
+    uint16_t* dst = (uint16_t*)a.o_lat + ((long long)v.t0 * m.H + row0 + part * kCombineRows + row) * (2 * R) + 4 * e;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(hi2[0], hi2[1]);
+    *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo2[0], lo2[1]);
 }
 
 // ---- output = value_up o~ ---------------------------------------------------------------------------------------------------
@@ -568,7 +673,7 @@ __global__ void __launch_bounds__(160) project_value_kernel(const __grid_constan
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
     const Step& m = a.m;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * kTile, chunks = m.R / 64;
     if (!tile_rows(a, t0, live)) return;
     const int w_bytes = m.Dv * 128, stage = w_bytes + 2 * 8192;
@@ -604,11 +709,12 @@ __global__ void __launch_bounds__(160) project_value_kernel(const __grid_constan
             ok = wt.wait_warp(&full[st], (c / kValueStages) & 1);
             if (!ok) break;
             tc05::fence_after_thread_sync();
-            const uint32_t base = pa::smem_u32(smem + st * stage);
-            const uint64_t da = tc05::smem_desc_sw128(base, 1024), db = tc05::smem_desc_sw128(base + w_bytes, 1024);
+            const uint32_t da = desc_low(smem + st * stage), db = da + (w_bytes >> 4);
             if (tc05::elect_one()) {
-                for (int part = 0; part < 2; ++part)
-                    for (int kk = 0; kk < 4; ++kk) tc05::mma_ss(tmem, da + 2 * kk, db + part * 512 + 2 * kk, idesc, c + part + kk > 0);
+                if (c == 0) mma_ss<0>(tmem, da, db, idesc);
+                else mma_ss<1>(tmem, da, db, idesc);
+#pragma unroll
+                for (int kk = 1; kk < 8; ++kk) mma_ss<1>(tmem, da + 2 * (kk & 3), db + (kk >> 2) * 512 + 2 * (kk & 3), idesc);
                 tc05::commit(&free_[st]);
                 if (c + 1 == chunks) tc05::commit(&done);
             }
@@ -655,7 +761,7 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     if (e != cudaSuccess) return e;
     project_query_kernel<BF><<<1 + token_tiles * m.H * (R / 128), 128, smem_q, stream>>>(a);
     attend_kernel<R, BF><<<a.groups * a.row_tiles, kThreads, smem_a, stream>>>(a);
-    combine_kernel<R, BF><<<m.num_tokens * m.H, R, 0, stream>>>(a);
+    combine_kernel<R, BF><<<(a.groups - 1) * a.row_tiles * (kTile / kCombineRows), R, kCombineRows * a.groups * sizeof(float), stream>>>(a);
     project_value_kernel<BF><<<token_tiles * m.H, 160, smem_v, stream>>>(a);
     *launches += 4;
     return cudaGetLastError();

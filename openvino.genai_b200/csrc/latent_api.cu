@@ -102,10 +102,10 @@ EncodeTiled encode_tiled() {
 }
 
 // A map of 16-bit elements whose boxes are 64 elements wide and land 128-byte-swizzled; elements outside the tensor read as zero.
-// sizes and box in elements, innermost first; strides in elements, of dimensions 1 and 2.
+// sizes and box in elements, innermost first; strides in elements, of the dimensions behind the first.
 bool make_map(CUtensorMap* map, int dtype, const void* base, int rank, const long long* sizes, const long long* strides, const int* box) {
-    cuuint64_t dims[3], pitch[2];
-    cuuint32_t b[3], one[3] = {1, 1, 1};
+    cuuint64_t dims[4], pitch[3];
+    cuuint32_t b[4], one[4] = {1, 1, 1, 1};
     for (int i = 0; i < rank; ++i) { dims[i] = (cuuint64_t)sizes[i]; b[i] = (cuuint32_t)box[i]; }
     for (int i = 0; i + 1 < rank; ++i) pitch[i] = (cuuint64_t)strides[i] * 2;
     const EncodeTiled encode = encode_tiled();
@@ -272,12 +272,17 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         const long long qn_size[3] = {d.nope_size, H, T}, qn_stride[2] = {nh, nt};
         const long long ku_size[3] = {R, d.nope_size, H}, ku_stride[2] = {R, kh};
         const long long vu_size[3] = {R, d.value_size, H}, vu_stride[2] = {R, vh};
-        const long long qa_size[2] = {W, (long long)T * H}, ca_size[2] = {W, (long long)a->num_blocks * d.block_size}, row_stride[1] = {W};
+        // rows of latents in groups of eight, every 64-element chunk of a group 1024 bytes in shared memory; the rotated part by itself
+        const long long groups = (long long)a->num_blocks * d.block_size / 8;
+        const long long ca_size[4] = {64, 8, R / 64, groups}, ca_stride[3] = {W, 64, 8 * W}, cr_size[3] = {P, 8, groups}, cr_stride[2] = {W, 8 * W};
+        const long long qa_size[3] = {64, (long long)T * H, R / 64}, qa_stride[2] = {W, 64}, qr_size[2] = {P, (long long)T * H}, qr_stride[1] = {W};
         const long long ol_size[3] = {2 * R, H, T}, ol_stride[2] = {2 * R, 2ll * R * H};
-        const int box_tokens[3] = {64, 1, latent::kTile}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1}, box_q[2] = {64, 16}, box_c[2] = {64, d.block_size};
+        const int box_tokens[3] = {64, 1, latent::kTile}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1};
+        const int box_q[3] = {64, latent::kTile, R / 64}, box_qr[2] = {64, latent::kTile}, box_c[4] = {64, 8, R / 64, d.block_size / 8}, box_cr[3] = {64, 8, d.block_size / 8};
         if (!make_map(&k.map_qn, d.dtype, a->query_nope, 3, qn_size, qn_stride, box_tokens) || !make_map(&k.map_key_up, d.dtype, a->key_up, 3, ku_size, ku_stride, box_ku) ||
-            !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_q_abs, d.dtype, k.q_abs, 2, qa_size, row_stride, box_q) ||
-            !make_map(&k.map_cache, d.dtype, a->cache, 2, ca_size, row_stride, box_c) || !make_map(&k.map_o_lat, d.dtype, k.o_lat, 3, ol_size, ol_stride, box_tokens))
+            !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_q_abs, d.dtype, k.q_abs, 3, qa_size, qa_stride, box_q) ||
+            !make_map(&k.map_q_abs_rope, d.dtype, (const uint16_t*)k.q_abs + R, 2, qr_size, qr_stride, box_qr) ||
+            !make_map(&k.map_cache, d.dtype, a->cache, 4, ca_size, ca_stride, box_c) || !make_map(&k.map_cache_rope, d.dtype, (const uint16_t*)a->cache + R, 3, cr_size, cr_stride, box_cr) || !make_map(&k.map_o_lat, d.dtype, k.o_lat, 3, ol_size, ol_stride, box_tokens))
             return fail(PA_ERR_CUDA, "a tensor map could not be made");
         LATENT_CUDA(latent::launch_absorbed(k, d.dtype, stream, &launches));
     }

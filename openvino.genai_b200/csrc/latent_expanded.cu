@@ -141,14 +141,14 @@ __device__ __forceinline__ ExpandItem expand_item(const ExpandedArgs& a, int i, 
     return it;
 }
 
-template <int R, bool BF>
+template <int R, int DN, int DV, bool BF>
 __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_constant__ ExpandedArgs a) {
     using Smem = ExpandSmem<R>;
     constexpr int NC = R / 64;
     extern __shared__ uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const Step& m = a.m;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
         pa::mbar_init(&sm.a_full, 1);
         pa::mbar_init(&sm.a_free, 1);
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     const uint32_t tmem = sm.tmem_base;
     const Waiter wt{&sm.abort_flag, m.status};
     const int per = expand_heads_per_item(a), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
-    const int buffer = m.Dn + m.Dv;      // tensor-memory columns of one head
+    constexpr int kBuffer = DN + DV;     // tensor-memory columns of one head
 
     if (warp == 4) {
         uint32_t n = 0, na = 0;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                     const int st = n % kWeightStages;
                     if (n >= kWeightStages) ok = wt.wait_warp(&sm.w_free[st], (n / kWeightStages - 1) & 1);
                     if (ok && lane == 0) {
-                        pa::mbar_expect_tx(&sm.w_full[st], (x < NC ? m.Dn : m.Dv) * 128);
+                        pa::mbar_expect_tx(&sm.w_full[st], (x < NC ? DN : DV) * 128);
                         tma_3d(sm.w[st], x < NC ? &a.map_key_up : &a.map_value_up, 64 * (x % NC), 0, a.h0 + h, &sm.w_full[st]);
                     }
                     __syncwarp();
@@ -202,26 +202,31 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                 for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % kWeightStages], (i / kWeightStages) & 1); ++k) {}
         }
     } else if (warp == 5) {
-        const uint32_t idesc_k = tc05::instr_desc_f16(128, m.Dn, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, m.Dv, BF ? 1 : 0, 0, 0);
-        const uint64_t da = tc05::smem_desc_sw128(pa::smem_u32(sm.a), 1024), dw = tc05::smem_desc_sw128(pa::smem_u32(sm.w), 1024);
-        uint32_t n = 0, na = 0, nd = 0;
+        constexpr uint32_t idesc_k = tc05::instr_desc_f16(128, DN, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 0);
+        static_assert(2 * NC % kWeightStages == 0, "a head begins with the first stage");
+        const uint32_t da = desc_low(sm.a), dw = desc_low(sm.w);
+        uint32_t na = 0, nd = 0;
         bool ok = true;
         for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
             const ExpandItem it = expand_item(a, i, per);
             ok = wt.wait_warp(&sm.a_full, na & 1);
             for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
                 if (nd >= 2) ok = wt.wait_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
-                for (int x = 0; ok && x < 2 * NC; ++x, ++n) {
-                    const int st = n % kWeightStages;
-                    ok = wt.wait_warp(&sm.w_full[st], (n / kWeightStages) & 1);
+#pragma unroll
+                for (int x = 0; x < 2 * NC; ++x) {
+                    constexpr int kRound = 2 * NC / kWeightStages;     // (a stage's phase: its round in the head, and the heads before)
+                    const int st = x % kWeightStages;
+                    if (ok) ok = wt.wait_warp(&sm.w_full[st], (nd * kRound + x / kWeightStages) & 1);
                     if (!ok) break;
                     tc05::fence_after_thread_sync();
-                    const uint32_t d = tmem + (nd & 1) * buffer + (x < NC ? 0 : m.Dn);
+                    const uint32_t d = tmem + (nd & 1) * kBuffer + (x < NC ? 0 : DN);
                     if (tc05::elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc05::mma_ss(d, da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, dw + st * (128 * 128 >> 4) + 2 * kk, x < NC ? idesc_k : idesc_v,
-                                         (x % NC) + kk > 0 ? 1u : 0u);
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint32_t pa = da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, pw = dw + st * (128 * 128 >> 4) + 2 * kk;
+                            if (x % NC + kk == 0) mma_ss<0>(d, pa, pw, x < NC ? idesc_k : idesc_v);
+                            else mma_ss<1>(d, pa, pw, x < NC ? idesc_k : idesc_v);
+                        }
                         tc05::commit(&sm.w_free[st]);
                         if (x == 2 * NC - 1) {
                             tc05::commit(&sm.d_full[nd & 1]);
@@ -254,12 +259,14 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                 ok = wt.wait_warp(&sm.d_full[nd & 1], (nd / 2) & 1);
                 if (!ok) break;
                 tc05::fence_after_thread_sync();
+#pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    const int D = part ? m.Dv : m.Dn;
-                    const uint32_t src = tmem + (nd & 1) * buffer + (part ? m.Dn : 0) + lanes;
+                    const int D = part ? DV : DN;
+                    const uint32_t src = tmem + (nd & 1) * kBuffer + (part ? DN : 0) + lanes;
                     // the copies out of the staging rows that this warp wrote before have read them (a warp stages and sends its own 32 rows)
                     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
+#pragma unroll
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t r[32];
                         tc05::ld_32x32b_x32(src + c0, r);
@@ -300,7 +307,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
 // ---- attention ------------------------------------------------------------------------------------------------------------------
 // A work item is 256 new tokens of one head in two halves A and B of 128 rows.  S_X = Q_X K^T (M 128, N 128) into TMEM, P_X over S_X, O_X += P_X V
 // with P read from TMEM; the tensor core computes P V and the next S of one half beside the softmax of the other.
-// Warps 0 - 3 and 4 - 7: softmax of A and B, a thread per row; 8: loader, 9: products; 10, 11 fill the warpgroup whose registers go to the softmax.
+// Warps 0 - 3 and 4 - 7: softmax of A and B, a thread per row; 8: queries and keys, 9: products, 10: values;
+// 11 fills the warpgroup whose registers go to the softmax.
 constexpr int kAttendThreads = 384;
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 and 128 threads of the 384 x 168 that the CTA is launched with
 constexpr int kItemSlots = 4;
@@ -318,25 +326,30 @@ struct QueryItem {
 template <int DN, int DV>
 struct ExpandedSmem {
     static constexpr int NQ = DN / 64 + 1, NV = DV / 64;
-    static constexpr int KS = DN == 128 ? 2 : 3, VS = DN == 128 && DV == 128 ? 2 : 4;    // tiles of keys (128 tokens), of values (64 tokens)
+    // Rings of key atoms (128 tokens x 64 elements, NQ of them a tile) and of value units (64 tokens): each is freed by itself, so that a
+    // tile and a part of the next fit beside the queries
+    static constexpr int KS = DN == 128 ? 5 : 4, VS = DN == 128 && DV == 128 ? 3 : DV == 128 ? 4 : 6;
     alignas(1024) uint8_t q[2][NQ][128 * 128];
-    alignas(1024) uint8_t k[KS][NQ][kExpandTile * 128];
+    alignas(1024) uint8_t k[KS][kExpandTile * 128];
     alignas(1024) uint8_t v[VS][NV][64 * 128];
-    uint64_t q_full[2], q_free[2], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2], o_done[2];
+    uint64_t q_full[2], q_free[2], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2][2], o_done[2];
     uint64_t item_full[kItemSlots], item_free[kItemSlots];
     QueryItem item[kItemSlots];
     uint32_t tmem_base;
     int abort_flag;
 };
 
+// A place in a ring of N barriers and the phase that it waits for.
+template <int N>
+struct Ring {
+    uint32_t at = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) { at = 0; phase ^= 1u; }
+    }
+};
+
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
 template <int DN, int DV, bool BF>
 __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(const __grid_constant__ ExpandedArgs a) {
     using Smem = ExpandedSmem<DN, DV>;
@@ -345,18 +358,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
     extern __shared__ uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const Step& m = a.m;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
             pa::mbar_init(&sm.q_full[x], 1);
             pa::mbar_init(&sm.q_free[x], 1);
             pa::mbar_init(&sm.s_full[x], 1);
-            pa::mbar_init(&sm.p_full[x], 4);
+            pa::mbar_init(&sm.p_full[x][0], 4);
+            pa::mbar_init(&sm.p_full[x][1], 4);
             pa::mbar_init(&sm.o_done[x], 1);
         }
         for (int i = 0; i < KS; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
         for (int i = 0; i < VS; ++i) { pa::mbar_init(&sm.v_full[i], 1); pa::mbar_init(&sm.v_free[i], 1); }
-        for (int i = 0; i < kItemSlots; ++i) { pa::mbar_init(&sm.item_full[i], 1); pa::mbar_init(&sm.item_free[i], 9); }
+        for (int i = 0; i < kItemSlots; ++i) { pa::mbar_init(&sm.item_full[i], 1); pa::mbar_init(&sm.item_free[i], 10); }
         pa::mbar_fence_init();
         sm.abort_flag = 0;
     }
@@ -379,7 +393,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
         if (warp == 8) {
             // ======================= loader =============================================================
             const int items = a.query_prefix[m.num_sequences] * a.heads;
-            uint32_t ni = 0, nk = 0, nv = 0, nq[2] = {0, 0};
+            uint32_t ni = 0, nk = 0, nq[2] = {0, 0};
             bool ok = true;
             while (ok) {
                 int i = 0;
@@ -422,32 +436,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 }
                 const int y0 = (int)(it.h * a.rows) + it.row;
                 auto load_k = [&](int j) {
-                    const int st = nk % KS;
-                    if (nk >= KS) ok = wt.wait_warp(&sm.k_free[st], (nk / KS - 1) & 1);
-                    if (!ok) return;
-                    if (lane == 0) {
-                        pa::mbar_expect_tx(&sm.k_full[st], NQ * kExpandTile * 128);
-                        for (int c = 0; c < NQ - 1; ++c) tma_2d(sm.k[st][c], &a.map_k, 64 * c, y0 + j * kExpandTile, &sm.k_full[st]);
-                        tma_2d(sm.k[st][NQ - 1], &a.map_k_rope, 0, it.row + j * kExpandTile, &sm.k_full[st]);
-                    }
-                    __syncwarp();
-                    ++nk;
-                };
-                for (int j = 0; ok && j < tiles; ++j) {
-                    if (j == 0) load_k(0);
-                    if (ok && j + 1 < tiles) load_k(j + 1);
-                    for (int u = 0; ok && u < 2; ++u) {
-                        const int st = nv % VS;
-                        if (nv >= VS) ok = wt.wait_warp(&sm.v_free[st], (nv / VS - 1) & 1);
-                        if (!ok) break;
+                    for (int c = 0; ok && c < NQ; ++c, ++nk) {
+                        const int st = nk % KS;
+                        if (nk >= KS) ok = wt.wait_warp(&sm.k_free[st], (nk / KS - 1) & 1);
+                        if (!ok) return;
                         if (lane == 0) {
-                            pa::mbar_expect_tx(&sm.v_full[st], NV * 64 * 128);
-                            for (int c = 0; c < NV; ++c) tma_2d(sm.v[st][c], &a.map_v, 64 * c, y0 + j * kExpandTile + 64 * u, &sm.v_full[st]);
+                            pa::mbar_expect_tx(&sm.k_full[st], kExpandTile * 128);
+                            if (c + 1 < NQ) tma_2d(sm.k[st], &a.map_k, 64 * c, y0 + j * kExpandTile, &sm.k_full[st]);
+                            else tma_2d(sm.k[st], &a.map_k_rope, 0, it.row + j * kExpandTile, &sm.k_full[st]);
                         }
                         __syncwarp();
-                        ++nv;
                     }
-                }
+                };
+                for (int j = 0; ok && j < tiles; ++j) load_k(j);
             }
             if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
                 auto drain = [&](uint64_t* bar, uint32_t parity) {
@@ -456,79 +457,125 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 for (int x = 0; x < 2; ++x)
                     if (nq[x] > 0) drain(&sm.q_full[x], (nq[x] - 1) & 1);
                 for (uint32_t i = nk > KS ? nk - KS : 0; i < nk; ++i) drain(&sm.k_full[i % KS], (i / KS) & 1);
-                for (uint32_t i = nv > VS ? nv - VS : 0; i < nv; ++i) drain(&sm.v_full[i % VS], (i / VS) & 1);
             }
-        } else if (warp == 9) {
-            // ======================= products ============================================================
-            constexpr uint32_t idesc_s = tc05::instr_desc_f16(128, kExpandTile, BF ? 1 : 0, 0, 0);
-            constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 1);
-            const uint64_t dq = tc05::smem_desc_sw128(pa::smem_u32(sm.q), 1024), dk = tc05::smem_desc_sw128(pa::smem_u32(sm.k), 1024);
-            const uint64_t dv = tc05::smem_desc_sw128(pa::smem_u32(sm.v), 1024, 64 * 128);
-            constexpr uint32_t kAtom = 128 * 128 >> 4;
-            const int rope_steps = m.P / 16;
-            uint32_t ni = 0, nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0};   // tiles of keys, units of values, before this item; query tiles, P tiles so far
+        } else if (warp == 10) {
+            // ======================= loader of the values ====================================================
+            uint32_t nv = 0;
             bool ok = true;
             QueryItem it;
-            for (; ok; ++ni) {
+            for (uint32_t ni = 0; ok; ++ni) {
                 if (!fetch(ni, it) || it.h < 0) break;
-                const int tiles = max(it.tiles[0], it.tiles[1]);
-                const int last_half = it.tiles[1] > 0 ? 1 : 0;      // B sees no fewer tiles than A, where it has rows
-                auto issue_s = [&](int X, int j) {
-                    const int st = (nk + j) % KS;
-                    ok = wt.wait_warp(&sm.k_full[st], ((nk + j) / KS) & 1);
-                    if (!ok) return;
-                    tc05::fence_after_thread_sync();
-                    const uint64_t da = dq + X * NQ * kAtom, db = dk + st * NQ * kAtom;
-                    if (tc05::elect_one()) {
-#pragma unroll
-                        for (int kk = 0; kk < DN / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 2;
-                            if (kk == 0) tc05::mma_ss<0>(tmem + X * 128, da + off, db + off, idesc_s);
-                            else tc05::mma_ss<1>(tmem + X * 128, da + off, db + off, idesc_s);
-                        }
-                        for (int kk = 0; kk < rope_steps; ++kk) tc05::mma_ss<1>(tmem + X * 128, da + (NQ - 1) * kAtom + 2 * kk, db + (NQ - 1) * kAtom + 2 * kk, idesc_s);
-                        tc05::commit(&sm.s_full[X]);
-                        if (X == last_half) tc05::commit(&sm.k_free[st]);
-                        if (j + 1 == it.tiles[X]) tc05::commit(&sm.q_free[X]);
+                const int units = 2 * max(it.tiles[0], it.tiles[1]), y0 = (int)(it.h * a.rows) + it.row;
+                for (int u = 0; ok && u < units; ++u, ++nv) {
+                    const int st = nv % VS;
+                    if (nv >= VS) ok = wt.wait_warp(&sm.v_free[st], (nv / VS - 1) & 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        pa::mbar_expect_tx(&sm.v_full[st], NV * 64 * 128);
+                        for (int c = 0; c < NV; ++c) tma_2d(sm.v[st][c], &a.map_v, 64 * c, y0 + 64 * u, &sm.v_full[st]);
                     }
                     __syncwarp();
-                };
-                auto issue_o = [&](int X, int j) {
-                    ok = wt.wait_warp(&sm.p_full[X], np[X] & 1);
-                    ++np[X];
-                    for (int u = 0; ok && u < 2; ++u) {
-                        const int st = (nv + 2 * j + u) % VS;
-                        ok = wt.wait_warp(&sm.v_full[st], ((nv + 2 * j + u) / VS) & 1);
-                        if (!ok) return;
-                        tc05::fence_after_thread_sync();
-                        if (tc05::elect_one()) {
+                }
+            }
+            if (sm.abort_flag)
+                for (uint32_t i = nv > VS ? nv - VS : 0; i < nv; ++i)
+                    for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.v_full[i % VS], (i / VS) & 1); ++k) {}
+        } else if (warp == 9) {
+            // ======================= products ============================================================
+            // The whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took 110 cycles to issue in
+            // place of 50.
+            {
+                constexpr uint32_t idesc_s = tc05::instr_desc_f16(128, kExpandTile, BF ? 1 : 0, 0, 0);
+                constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 1);
+                const uint32_t dq = desc_low(sm.q), dk = desc_low(sm.k), dv = desc_low(sm.v, 64 * 128);
+                constexpr uint32_t kAtom = 128 * 128 >> 4, kUnit = NV * 64 * 128 >> 4;
+                const bool wide = m.P == 64;
+                Ring<KS> k[2];           // where each half is in the rings
+                Ring<VS> v[2];
+                uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+                bool ok = true;
+                for (uint32_t ni = 0; ok; ++ni) {
+                    const int slot = ni % kItemSlots;
+                    if (!wt.wait_warp(&sm.item_full[slot], (ni / kItemSlots) & 1)) break;
+                    const QueryItem it = sm.item[slot];
+                    warp_arrive(&sm.item_free[slot]);
+                    if (it.h < 0) break;
+                    const int tiles = max(it.tiles[0], it.tiles[1]);
+                    const int last_half = it.tiles[1] > 0 ? 1 : 0;      // B sees no fewer tiles than A, where it has rows
+                    auto issue_s = [&](int X, int j) {
+                        const bool fresh = X == 0 || j >= it.tiles[0];  // (else A has waited for these keys)
+                        const uint32_t d = tmem + X * 128;
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk) {
-                                const uint32_t p = tmem + X * 128 + u * 32 + kk * 8;
-                                const uint64_t db = dv + st * (NV * 64 * 128 >> 4) + kk * 128;
-                                if (kk == 0 && u == 0 && j == 0) tc05::mma_ts<0>(tmem + kO + X * DV, p, db, idesc_o);
-                                else tc05::mma_ts<1>(tmem + kO + X * DV, p, db, idesc_o);
+                        for (int c = 0; c < NQ; ++c) {
+                            if (fresh) ok = ok && wt.wait_warp(&sm.k_full[k[X].at], k[X].phase);
+                            if (!ok) return;
+                            tc05::fence_after_thread_sync();
+                            const uint32_t da = dq + (X * NQ + c) * kAtom, db = dk + k[X].at * kAtom;
+                            if (tc05::elect_one()) {
+                            if (c == 0) mma_ss<0>(d, da, db, idesc_s);
+                            else mma_ss<1>(d, da, db, idesc_s);
+                            mma_ss<1>(d, da + 2, db + 2, idesc_s);
+                            if (c + 1 < NQ || wide) {
+                                mma_ss<1>(d, da + 4, db + 4, idesc_s);
+                                mma_ss<1>(d, da + 6, db + 6, idesc_s);
                             }
-                            if (X == last_half) tc05::commit(&sm.v_free[st]);
+                            if (X == last_half) tc05::commit(&sm.k_free[k[X].at]);
+                            if (c + 1 == NQ) {
+                                tc05::commit(&sm.s_full[X]);
+                                if (j + 1 == it.tiles[X]) tc05::commit(&sm.q_free[X]);
+                            }
+                            }
+                            __syncwarp();
+                            k[X].next();
+                        }
+                    };
+                    auto issue_o = [&](int X, int j) {
+                        const bool fresh = X == 0 || j >= it.tiles[0];
+                        const uint32_t d = tmem + kO + X * DV;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            if (fresh) ok = ok && wt.wait_warp(&sm.v_full[v[X].at], v[X].phase);
+                            ok = ok && wt.wait_warp(&sm.p_full[X][u], np[X] & 1);
+                            if (!ok) return;
+                            tc05::fence_after_thread_sync();
+                            const uint32_t p = tmem + X * 128 + u * 32, db = dv + v[X].at * kUnit;
+                            if (tc05::elect_one()) {
+                            if (u == 0 && j == 0) mma_ts<0>(d, p, db, idesc_o);
+                            else mma_ts<1>(d, p, db, idesc_o);
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) mma_ts<1>(d, p + kk * 8, db + kk * 128, idesc_o);
+                            if (X == last_half) tc05::commit(&sm.v_free[v[X].at]);
                             if (u == 1 && j + 1 == it.tiles[X]) tc05::commit(&sm.o_done[X]);
+                            }
+                            __syncwarp();
+                            v[X].next();
                         }
-                        __syncwarp();
-                    }
-                };
-                for (int X = 0; ok && X < 2; ++X)
-                    if (it.tiles[X] > 0) {
-                        ok = wt.wait_warp(&sm.q_full[X], nq[X] & 1);
-                        ++nq[X];
-                        if (ok) issue_s(X, 0);
-                    }
-                for (int j = 0; ok && j < tiles; ++j)
-                    for (int X = 0; ok && X < 2; ++X)
-                        if (j < it.tiles[X]) {
-                            issue_o(X, j);
-                            if (ok && j + 1 < it.tiles[X]) issue_s(X, j + 1);
+                        ++np[X];
+                    };
+#pragma unroll
+                    for (int X = 0; X < 2; ++X)
+                        if (ok && it.tiles[X] > 0) {
+                            ok = wt.wait_warp(&sm.q_full[X], nq[X] & 1);
+                            ++nq[X];
+                            if (ok) issue_s(X, 0);
                         }
-                nk += tiles;
-                nv += 2 * tiles;
+                    for (int j = 0; ok && j < tiles; ++j) {
+#pragma unroll
+                        for (int X = 0; X < 2; ++X)
+                            if (ok && j < it.tiles[X]) {
+                                issue_o(X, j);
+                                if (ok && j + 1 < it.tiles[X]) issue_s(X, j + 1);
+                            }
+                    }
+#pragma unroll
+                    for (int X = 0; X < 2; ++X)      // past the tiles that only the other half sees
+                        for (int j = it.tiles[X]; j < tiles; ++j) {
+#pragma unroll
+                            for (int c = 0; c < NQ; ++c) k[X].next();
+                            v[X].next();
+                            v[X].next();
+                        }
+                }
             }
         }
     } else {
@@ -601,11 +648,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         p[c >> 1] = pack2<BF>(x, y);
                     }
                     tc05::st_32x32b_x32(tmem_s + 16 * q, p);
+                    tc05::wait_st();
+                    tc05::fence_before_thread_sync();
+                    warp_arrive(&sm.p_full[X][q / 2]);      // the products of these 64 tokens run beside the exponentials of the others
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc05::wait_st();
-                tc05::fence_before_thread_sync();
-                warp_arrive(&sm.p_full[X]);
             }
             if (!ok || !wt.wait_warp(&sm.o_done[X], no & 1)) break;
             ++no;
@@ -649,15 +696,21 @@ cudaError_t attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+template <int R, int DN, int DV, bool BF>
+cudaError_t expand_and_attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
+    const int smem = sizeof(ExpandSmem<R>) + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(expand_kernel<R, DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    expand_kernel<R, DN, DV, BF><<<sm_count, kExpandThreads, smem, stream>>>(a);
+    *launches += 2;
+    return attend<DN, DV, BF>(a, sm_count, stream);
+}
+
 template <int R, bool BF>
 cudaError_t launch(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
-    const int smem = sizeof(ExpandSmem<R>) + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(expand_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    expand_kernel<R, BF><<<sm_count, kExpandThreads, smem, stream>>>(a);
-    *launches += 2;
-    if (a.m.Dn == 128) return a.m.Dv == 128 ? attend<128, 128, BF>(a, sm_count, stream) : attend<128, 64, BF>(a, sm_count, stream);
-    return a.m.Dv == 128 ? attend<64, 128, BF>(a, sm_count, stream) : attend<64, 64, BF>(a, sm_count, stream);
+    if (a.m.Dn == 128)
+        return a.m.Dv == 128 ? expand_and_attend<R, 128, 128, BF>(a, sm_count, stream, launches) : expand_and_attend<R, 128, 64, BF>(a, sm_count, stream, launches);
+    return a.m.Dv == 128 ? expand_and_attend<R, 64, 128, BF>(a, sm_count, stream, launches) : expand_and_attend<R, 64, 64, BF>(a, sm_count, stream, launches);
 }
 
 }  // namespace

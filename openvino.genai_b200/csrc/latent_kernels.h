@@ -40,8 +40,8 @@ struct AppendArgs {
 
 // The absorbed form.  Its unit of work is a tile of 64 context tokens for a block of `row_tiles` tiles of 64 query rows (new token, head) of one
 // sequence; sequence s has block_prefix[s + 1] - block_prefix[s] such blocks, every one of the same number of tiles.  Units are
-// numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut, or
-// not, leaves one partial result per group in slot (block + group) * row_tiles + row tile.
+// numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut leaves
+// one partial result per group in slot (block + group) * row_tiles + row tile.
 constexpr int kTile = 64;      // context tokens of a tile, query rows of a row tile, tokens of a projection's tile
 
 struct AbsorbedArgs {
@@ -58,7 +58,7 @@ struct AbsorbedArgs {
     void* o_lat;                // [num_tokens * H][2 R] sums of latents, high and low pieces
     void* output;
     float scale_log2;           // softmax scale * log2(e)
-    CUtensorMap map_qn, map_key_up, map_q_abs, map_cache, map_value_up, map_o_lat;
+    CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_rope, map_value_up, map_o_lat;
 };
 // Largest number of slots a step can need.
 long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);

@@ -23,6 +23,12 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(pa::smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                     pa::smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(pa::smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -32,6 +38,14 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Whether the barrier's phase is complete, without the suspension that try_wait may take: for a warp that watches two barriers.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(pa::smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
 }
 
 // Waits of a CTA's roles on one another are bounded: one that runs out raises `abort`, which all others poll, and sets the status bit.
@@ -53,9 +67,42 @@ struct Waiter {
     __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) const { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; }
 };
 
+// Operand descriptors of 128-byte-swizzled tiles whose 8-row groups are GROUP bytes apart.  Their high words are constants, so only the low
+// word (address and, for operands whose rows run along M or N, the distance of 64-element atoms) is carried along; a step is an addition.
+__host__ __device__ constexpr uint32_t desc_high(uint32_t group_bytes) { return (group_bytes >> 4) | (1u << 14) | (2u << 29); }
+__device__ __forceinline__ uint32_t desc_low(const void* smem, uint32_t atom_bytes = 16) {
+    return ((pa::smem_u32(smem) >> 4) & 0x3fffu) | ((atom_bytes >> 4) & 0x3fffu) << 16;
+}
+// D[tmem] (+)= A[smem] * B[smem], issued by one thread; ACC == 0 overwrites D.
+template <int ACC, uint32_t AGROUP = 1024, uint32_t BGROUP = 1024>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %6};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(ACC), "n"(desc_high(AGROUP)), "n"(desc_high(BGROUP))
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem].
+template <int ACC>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a_tmem), "r"(b), "r"(idesc), "n"(ACC), "n"(desc_high(1024))
+        : "memory");
+}
+// The warp's number as a value that is the same for the whole warp.
+__device__ __forceinline__ int warp_id() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
 
