@@ -159,8 +159,10 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
 //   S[row][token]     = Q~ K^T          M 64, N 64, K R + P; two buffers, so that S of the next tile is computed beside a softmax
 //   O^T[latent][row] += K^T P^T         M 128 (R / 128 times), N 64, K 64: the tile is read MN-major from the same image, and the
 //                                       rows (heads) are columns, so few heads leave no tensor-memory lane idle
-// A tile lies in shared memory in groups of eight tokens, [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view
-// of the cache, so a block is two copies (the rotated part is the other) whatever the block size; issuing nine took 900 cycles.
+// A tile lies in shared memory in two halves of its latent elements (the second with the rotated part), each in groups of eight tokens,
+// [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view of the cache, so a block is three copies; issuing one for
+// every chunk took 900 cycles.  Halves come and are freed by themselves: S begins with the first, and the products of the first half of O free
+// it while the second is at work.
 constexpr int kSlots = 4;               // depth of the queue of runs
 constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: products, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)
 constexpr float kLazy = 8.f;            // log2 of the growth of a row maximum that rescales O
@@ -184,7 +186,7 @@ struct AttendSmem {
     alignas(1024) uint8_t q[kTile * R * 2];
     alignas(1024) uint8_t q_rope[kTile * 128];
     struct Tile {
-        uint8_t c[kTile * R * 2];
+        uint8_t c[2][kTile * R];
         uint8_t rope[kTile * 128];
     };
     alignas(1024) Tile k[NST];
@@ -193,7 +195,7 @@ struct AttendSmem {
     float2 stat[2][kTile];                          // maximum and sum of the rows of a run
     volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
     volatile int event;                             // what the results warps are asked for: rescale after tile `event` - 1, or results (0)
-    uint64_t k_full[NST], k_free[NST];              // loader -> products (bytes), products -> loader
+    uint64_t k_full[NST][2], k_free[NST][2];        // loader -> products (bytes), products -> loader
     uint64_t q_full, q_free;
     uint64_t s_full[2], p_full, o_done;             // products -> softmax, softmax -> products, products -> softmax and results
     uint64_t asked, answered;                       // products -> results, results -> products
@@ -210,14 +212,14 @@ template <int R, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AbsorbedArgs a) {
     using Smem = AttendSmem<R>;
     constexpr int NC = R / 64, NST = Smem::NST, MT = R / 128;
-    constexpr uint32_t kGroup = NC * 1024;          // bytes from one group of eight rows to the next
+    constexpr uint32_t kGroup = NC / 2 * 1024;      // bytes from one group of eight rows to the next, in a half of a tile
     constexpr uint32_t kTmemS = MT * kTile;         // O^T: MT x 64 columns, then S twice
     extern __shared__ uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < NST; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
+        for (int i = 0; i < 2 * NST; ++i) { pa::mbar_init(&sm.k_full[0][i], 1); pa::mbar_init(&sm.k_free[0][i], 1); }
         pa::mbar_init(&sm.q_full, 1);
         pa::mbar_init(&sm.q_free, 1);
         pa::mbar_init(&sm.s_full[0], 1);
@@ -273,6 +275,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ++nr;
             return true;
         };
+        Cut cut{0, 0, 0, 0};
+        if (u < u_end) {
+            // where this slice is the first to begin inside a block of rows, its partial results are joined afterwards
+            SeqView v;
+            seq_view(m, s, v);
+            const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, block = (u - a.unit_prefix[s]) / tiles, u0 = a.unit_prefix[s] + block * tiles;
+            if (u0 < u && u0 / per + 1 == group) {
+                const int row0 = (int)(block * a.row_tiles + member) * kTile;
+                cut.rows = (int)min((long long)kTile, (long long)v.n * m.H - row0);
+                cut.grow0 = (int)((long long)v.t0 * m.H + row0);
+                cut.slot = (int)(((long long)a.block_prefix[s] + block + u0 / per) * a.row_tiles + member);
+                cut.pieces = (int)((u0 + tiles - 1) / per - u0 / per) + 1;
+            }
+        }
+        if (lane == 0) a.cuts[blockIdx.x] = cut;
         while (ok && u < u_end) {
             SeqView v;
             seq_view(m, s, v);
@@ -315,17 +332,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                             }
                         }
                         const int st = n % NST;
-                        if (n >= NST) ok = wt.wait_warp(&sm.k_free[st], (n / NST - 1) & 1);
-                        if (!ok) break;
-                        if (tc05::elect_one()) pa::mbar_expect_tx(&sm.k_full[st], blocks * m.bs * (R * 2 + 128));
-                        __syncwarp();
-                        for (int i = 0; i < blocks; ++i) {
-                            const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * (m.bs / 8);
-                            if (tc05::elect_one()) {
-                                tma_4d(sm.k[st].c + i * (m.bs / 8) * kGroup, &a.map_cache, 0, 0, 0, at, &sm.k_full[st]);
-                                tma_3d(sm.k[st].rope + i * m.bs * 128, &a.map_cache_rope, 0, 0, at, &sm.k_full[st]);
-                            }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (ok && n >= NST) ok = wt.wait_warp(&sm.k_free[st][half], (n / NST - 1) & 1);
+                            if (!ok) break;
+                            if (tc05::elect_one()) pa::mbar_expect_tx(&sm.k_full[st][half], blocks * m.bs * (R + half * 128));
                             __syncwarp();
+                            for (int i = 0; i < blocks; ++i) {
+                                const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * (m.bs / 8);
+                                if (tc05::elect_one()) {
+                                    tma_4d(sm.k[st].c[half] + i * (m.bs / 8) * kGroup, &a.map_cache, 0, 0, half * (NC / 2), at, &sm.k_full[st][half]);
+                                    if (half == 1) tma_3d(sm.k[st].rope + i * m.bs * 128, &a.map_cache_rope, 0, 0, at, &sm.k_full[st][half]);
+                                }
+                                __syncwarp();
+                            }
                         }
                     }
                 }
@@ -342,16 +362,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         if (sm.abort_flag) {
             for (uint32_t k = 0; nq > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.q_full, (nq - 1) & 1); ++k) {}
             for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i)
-                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.k_full[i % NST], (i / NST) & 1); ++k) {}
+                for (uint32_t k = 0; k < (1u << 20) && !(pa::mbar_try_wait(&sm.k_full[i % NST][0], (i / NST) & 1) && pa::mbar_try_wait(&sm.k_full[i % NST][1], (i / NST) & 1)); ++k) {}
         }
     } else if (warp == 5) {
         // ======================= products ================================================================
         // (the whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took twice as long to issue)
         constexpr uint32_t idesc_s = tc05::instr_desc_f16(kTile, kTile, BF ? 1 : 0, 0, 0);
         constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
-        const uint32_t dq = desc_low(sm.q), dqr = desc_low(sm.q_rope), dk = desc_low(sm.k[0].c), dkr = desc_low(sm.k[0].rope);
-        const uint32_t dv = desc_low(sm.k[0].c, 1024), dp = desc_low(sm.p);
-        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4;
+        const uint32_t dq = desc_low(sm.q), dqr = desc_low(sm.q_rope), dk = desc_low(sm.k[0].c[0]), dkr = desc_low(sm.k[0].rope);
+        const uint32_t dv = desc_low(sm.k[0].c[0], 1024), dp = desc_low(sm.p);
+        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4, kHalf = kTile * R >> 4;
         const bool wide = m.P == 64;
         uint32_t n = 0, asked = 0;
         bool ok = true;
@@ -367,9 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ok = wt.wait_warp(&sm.q_full, nq & 1);
             ++nq;
             const uint32_t end = n + r.tiles;
-            uint32_t next_s = n, next_o = n;
+            uint32_t next_s = n, half = 0, next_o = n;
             uint32_t idle = 0;
-            // O as soon as its P is there; S of a tile as soon as the tile is, but no more than one ahead of O
+            // O as soon as its P is there; each half of S as soon as that of the tile is, but no more than a tile ahead of O
             while (ok && next_o < end) {
                 if (next_o < next_s && __all_sync(0xffffffffu, mbar_test(&sm.p_full, next_o & 1))) {
                     if (next_o == n) {
@@ -385,39 +405,42 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     if (tc05::elect_one()) {
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            const uint32_t d = tmem + mt * kTile, pa = da + mt * (2048 >> 4);
+                            const uint32_t d = tmem + mt * kTile, pa = da + mt / (MT / 2) * kHalf + mt % (MT / 2) * (2048 >> 4);
                             if (next_o > n) mma_ss<1, kGroup>(d, pa, dp, idesc_o);
                             else mma_ss<0, kGroup>(d, pa, dp, idesc_o);
 #pragma unroll
                             for (int kk = 1; kk < kTile / 16; ++kk) mma_ss<1, kGroup>(d, pa + kk * (2 * kGroup >> 4), dp + kk * 2, idesc_o);
+                            if (mt % (MT / 2) == MT / 2 - 1) tc05::commit(&sm.k_free[next_o % NST][mt / (MT / 2)]);
                         }
-                        tc05::commit(&sm.k_free[next_o % NST]);
                         tc05::commit(&sm.o_done);
                     }
                     __syncwarp();
                     ++next_o;
                     idle = 0;
-                } else if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, mbar_test(&sm.k_full[next_s % NST], (next_s / NST) & 1))) {
-                    const uint32_t db = dk + next_s % NST * kStage, dbr = dkr + next_s % NST * kStage, d = tmem + kTmemS + (next_s & 1) * kTile;
+                } else if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, mbar_test(&sm.k_full[next_s % NST][half], (next_s / NST) & 1))) {
+                    const uint32_t db = dk + next_s % NST * kStage + half * kHalf, dbr = dkr + next_s % NST * kStage, d = tmem + kTmemS + (next_s & 1) * kTile;
+                    const uint32_t dqh = dq + half * kHalf;
                     tc05::fence_after_thread_sync();
                     if (tc05::elect_one()) {
+                        if (half == 0) mma_ss<0, 1024, kGroup>(d, dqh, db, idesc_s);
+                        else mma_ss<1, 1024, kGroup>(d, dqh, db, idesc_s);
 #pragma unroll
-                        for (int kk = 0; kk < R / 16; ++kk) {
-                            const uint32_t qa = dq + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, kb = db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2;
-                            if (kk == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
-                            else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
+                        for (int kk = 1; kk < R / 32; ++kk)
+                            mma_ss<1, 1024, kGroup>(d, dqh + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2, idesc_s);
+                        if (half == 1) {
+                            mma_ss<1>(d, dqr, dbr, idesc_s);
+                            mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
+                            if (wide) {
+                                mma_ss<1>(d, dqr + 4, dbr + 4, idesc_s);
+                                mma_ss<1>(d, dqr + 6, dbr + 6, idesc_s);
+                            }
+                            tc05::commit(&sm.s_full[next_s & 1]);
+                            if (next_s + 1 == end) tc05::commit(&sm.q_free);
                         }
-                        mma_ss<1>(d, dqr, dbr, idesc_s);
-                        mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
-                        if (wide) {
-                            mma_ss<1>(d, dqr + 4, dbr + 4, idesc_s);
-                            mma_ss<1>(d, dqr + 6, dbr + 6, idesc_s);
-                        }
-                        tc05::commit(&sm.s_full[next_s & 1]);
-                        if (next_s + 1 == end) tc05::commit(&sm.q_free);
                     }
                     __syncwarp();
-                    ++next_s;
+                    next_s += half;
+                    half ^= 1u;
                     idle = 0;
                 } else if (++idle > (1u << 26)) {
                     ok = wt.give_up();
@@ -514,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             for (int j = 0; j < r.tiles; ++j, ++n) {
                 if (!wt.wait_warp(&sm.s_full[n & 1], (n >> 1) & 1)) { ok = false; break; }
                 tc05::fence_after_thread_sync();
+                const bool free_p = n == 0 || mbar_test(&sm.o_done, (n - 1) & 1);      // P of the tile before has been read (looked at early: the answer takes its time)
                 uint32_t raw[32];
                 ld_16x256b_x8(tmem + kTmemS + (n & 1) * kTile + lanes, raw);
                 tc05::wait_ld();
@@ -554,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     l[x] += sum[0] + sum[1];
                 }
                 if (grew) sm.grew[n & 1] = n + 1;
-                if (n > 0 && !wt.wait_warp(&sm.o_done, (n - 1) & 1)) { ok = false; break; }     // P of the tile before has been read
+                if (!__all_sync(0xffffffffu, free_p) && !wt.wait_warp(&sm.o_done, (n - 1) & 1)) { ok = false; break; }
                 // P: a row's 64 tokens are 128 bytes, 16-byte pieces swizzled by the row
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
@@ -565,12 +589,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     // tokens behind the context: whatever lies there (stale bytes, not-a-number) meets probabilities of zero, which does not
                     // make it zero, so the latents are cleared
                     const int st = n % NST, valid = r.end - col0;
-                    if (!wt.wait_warp(&sm.k_full[st], (n / NST) & 1)) { ok = false; break; }
+                    if (!wt.wait_warp(&sm.k_full[st][0], (n / NST) & 1) || !wt.wait_warp(&sm.k_full[st][1], (n / NST) & 1)) { ok = false; break; }
                     for (int i = tid; i < (kTile - valid) * 8; i += 128) {
                         const int row = valid + i / 8;
 #pragma unroll
                         for (int c = 0; c < NC; ++c)
-                            *reinterpret_cast<uint4*>(sm.k[st].c + (row >> 3) * kGroup + c * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sm.k[st].c[c / (NC / 2)] + (row >> 3) * kGroup + c % (NC / 2) * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 tc05::fence_proxy_async_smem();
@@ -594,71 +618,56 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 }
 
 // ---- joining the partial results of a row ----------------------------------------------------------------------------------
-// A block of rows is cut where a slice begins inside it, so there are fewer cut blocks than slices: one CTA per (slice, row tile, four rows)
-// joins the block that its slice cuts first.  Leaves sum / denominator as two 16-bit pieces, so that the product with value_up does not
-// see another rounding.
-constexpr int kCombineRows = 4;
+// A block of rows is cut where a slice begins inside it, so there are fewer cut blocks than slices: eight CTAs per slice, eight rows each, join the
+// block that the slice cuts first.  Leaves sum / denominator as two 16-bit pieces, so that the product with value_up does not see another
+// rounding.
+constexpr int kCombineRows = 8, kCombineThreads = 512;
 template <int R, bool BF>
-__global__ void __launch_bounds__(R) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
     constexpr int kPer = R / 4;                    // threads of a row, four latent elements each
     extern __shared__ float weight[];              // [kCombineRows][pieces]
-    const Step& m = a.m;
-    const int part = blockIdx.x % (kTile / kCombineRows), member = blockIdx.x / (kTile / kCombineRows) % a.row_tiles;
-    const long long w = blockIdx.x / (kTile / kCombineRows) / a.row_tiles + 1, total = a.unit_prefix[m.num_sequences], per = slice_size(a);
-    if (w * per >= total) return;
-    int lo = 0, hi = m.num_sequences;              // unit_prefix[lo] <= w * per < unit_prefix[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.unit_prefix[mid] <= w * per) lo = mid; else hi = mid;
-    }
-    SeqView v;
-    seq_view(m, lo, v);
-    const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, block = (w * per - a.unit_prefix[lo]) / tiles;
-    const long long u0 = a.unit_prefix[lo] + block * tiles, w0 = u0 / per, w1 = (u0 + tiles - 1) / per;
-    if (u0 == w * per || w0 + 1 != w) return;      // not cut here, or cut by an earlier slice
-    const int row0 = (int)(block * a.row_tiles + member) * kTile;
-    const int rows = (int)min((long long)kTile, (long long)v.n * m.H - row0) - part * kCombineRows;
+    const int part = blockIdx.x % (kTile / kCombineRows);
+    const Cut cut = a.cuts[blockIdx.x / (kTile / kCombineRows)];
+    const int rows = min(kCombineRows, cut.rows - part * kCombineRows);
     if (rows <= 0) return;
-    const int pieces = (int)(w1 - w0) + 1, tid = threadIdx.x;
-    const long long slot0 = ((long long)a.block_prefix[lo] + block + w0) * a.row_tiles + member;
-    auto at = [&](int i, int row) { return (slot0 + (long long)i * a.row_tiles) * kTile + part * kCombineRows + row; };
-    // weights of the pieces: a warp per row
-    const int warp = tid >> 5, lane = tid & 31;
-    if (warp < kCombineRows && warp < rows) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto at = [&](int i, int row) { return ((long long)cut.slot + (long long)i * a.row_tiles) * kTile + part * kCombineRows + row; };
+    if (warp < rows) {                             // weights of the pieces: a warp per row
         float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < pieces; i += 32) {
+        for (int i = lane; i < cut.pieces; i += 32) {
             const float2 ml = a.part_ml[at(i, warp)];
             if (ml.y > 0.f) top = fmaxf(top, ml.x);
         }
         top = pa::warp_max(top);
-        for (int i = lane; i < pieces; i += 32) {
+        for (int i = lane; i < cut.pieces; i += 32) {
             const float2 ml = a.part_ml[at(i, warp)];
             const float k = ml.y > 0.f ? ex2(ml.x - top) : 0.f;      // (a piece whose tiles the row does not see has no sums)
-            weight[warp * pieces + i] = k;
+            weight[warp * cut.pieces + i] = k;
             sum += k * ml.y;
         }
         sum = pa::warp_sum(sum);
-        for (int i = lane; i < pieces; i += 32) weight[warp * pieces + i] *= __frcp_rn(sum);
+        for (int i = lane; i < cut.pieces; i += 32) weight[warp * cut.pieces + i] *= __frcp_rn(sum);
     }
     __syncthreads();
-    const int row = tid / kPer, e = tid % kPer;
-    if (row >= rows) return;
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int row = tid / kPer; row < rows; row += kCombineThreads / kPer) {
+        const int e = tid % kPer;
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int i = 0; i < pieces; ++i) {
-        const float k = weight[row * pieces + i];
-        const float4 p = k != 0.f ? *reinterpret_cast<const float4*>(a.part_o + at(i, row) * R + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
-        y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w;
-    }
-    uint32_t hi2[2], lo2[2];
+        for (int i = 0; i < cut.pieces; ++i) {
+            const float k = weight[row * cut.pieces + i];
+            const float4 p = k != 0.f ? *reinterpret_cast<const float4*>(a.part_o + at(i, row) * R + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w;
+        }
+        uint32_t hi[2], lo[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        hi2[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
-        lo2[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi2[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi2[i] >> 16)));
+        for (int i = 0; i < 2; ++i) {
+            hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
+            lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
+        }
+        uint16_t* dst = (uint16_t*)a.o_lat + ((long long)cut.grow0 + part * kCombineRows + row) * (2 * R) + 4 * e;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo[0], lo[1]);
     }
-    uint16_t* dst = (uint16_t*)a.o_lat + ((long long)v.t0 * m.H + row0 + part * kCombineRows + row) * (2 * R) + 4 * e;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(hi2[0], hi2[1]);
-    *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo2[0], lo2[1]);
 }
 
 // ---- output = value_up o~ ---------------------------------------------------------------------------------------------------
@@ -761,7 +770,7 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     if (e != cudaSuccess) return e;
     project_query_kernel<BF><<<1 + token_tiles * m.H * (R / 128), 128, smem_q, stream>>>(a);
     attend_kernel<R, BF><<<a.groups * a.row_tiles, kThreads, smem_a, stream>>>(a);
-    combine_kernel<R, BF><<<(a.groups - 1) * a.row_tiles * (kTile / kCombineRows), R, kCombineRows * a.groups * sizeof(float), stream>>>(a);
+    combine_kernel<R, BF><<<a.groups * a.row_tiles * (kTile / kCombineRows), kCombineThreads, kCombineRows * a.groups * sizeof(float), stream>>>(a);
     project_value_kernel<BF><<<token_tiles * m.H, 160, smem_v, stream>>>(a);
     *launches += 4;
     return cudaGetLastError();

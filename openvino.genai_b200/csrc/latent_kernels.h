@@ -44,6 +44,14 @@ struct AppendArgs {
 // one partial result per group in slot (block + group) * row_tiles + row tile.
 constexpr int kTile = 64;      // context tokens of a tile, query rows of a row tile, tokens of a projection's tile
 
+// A row tile whose block the CTA's slice is the first to cut: where its partial results are and where the joined rows go.
+struct __align__(16) Cut {
+    int rows;       // 0: none
+    int grow0;      // first row among the step's (token, head) rows
+    int slot;       // of the first piece; the next ones follow `row_tiles` slots apart
+    int pieces;
+};
+
 struct AbsorbedArgs {
     Step m;
     int max_new;                // sequences with more new tokens are left to the expanded form
@@ -55,6 +63,7 @@ struct AbsorbedArgs {
     void* q_abs;                // [num_tokens * H][R + P] absorbed query rows
     float* part_o;              // [slot][64][R]
     float2* part_ml;            // [slot][64] maximum (base 2, scaled) and sum
+    Cut* cuts;                  // [groups * row_tiles]
     void* o_lat;                // [num_tokens * H][2 R] sums of latents, high and low pieces
     void* output;
     float scale_log2;           // softmax scale * log2(e)
