@@ -21,7 +21,7 @@ __device__ __forceinline__ SeqPlan seq_plan(const AbsorbedArgs& a, int s) {
     SeqView v;
     if (!seq_view(a.m, s, v) || v.n == 0 || v.n > a.max_new) return SeqPlan{0, 0};
     const int rows = kTile * a.row_tiles;
-    return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTile - 1) / kTile};
+    return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTokens - 1) / kTokens};
 }
 
 // Exclusive prefix sums over the sequences, by one block of 128 threads.
@@ -55,12 +55,27 @@ __device__ void build_plan(const AbsorbedArgs& a) {
         __syncthreads();
     }
     if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; }
-}
-
-// Units of a group's slice.
-__device__ __forceinline__ long long slice_size(const AbsorbedArgs& a) {
-    const long long total = a.unit_prefix[a.m.num_sequences];
-    return total > 0 ? (total + a.groups - 1) / a.groups : 1;
+    __syncthreads();
+    // where every slice begins, so that a CTA of the attention has one record to read instead of a search
+    const long long total = run_u, per = total > 0 ? (total + a.groups - 1) / a.groups : 1;
+    for (int w = tid; w < a.groups; w += 128) {
+        const long long u = w * per;
+        SliceStart st{-1, 0, 0, 0};
+        if (u < total) {
+            int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.unit_prefix[mid] <= u) lo = mid; else hi = mid;
+            }
+            const long long rel = u - a.unit_prefix[lo], tiles = seq_plan(a, lo).tiles;
+            st.s = lo;
+            st.block = (int)(rel / tiles);
+            st.first = (int)(rel % tiles);
+            st.units = (int)min(per, total - u);
+        }
+        a.starts[w] = st;
+    }
+    if (tid == 0) *a.per = per;
 }
 
 // Which of the tile's tokens belong to sequences of this form; false (for the whole block) if none does.
@@ -79,8 +94,7 @@ __device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&
 // MN-major operand, one tile of each operand, so the CTAs of an SM overlap one another's loads, products and stores.
 template <bool BF>
 __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constant__ AbsorbedArgs a) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full, done;
     __shared__ bool live[kTile];
     __shared__ uint32_t tmem_base;
@@ -155,16 +169,17 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
 
 // ---- attention over the latents ------------------------------------------------------------------------------------------
 // Roles meet through mbarriers only: a loader warp walks the slice and has the TMA engine bring query rows and 64-token tiles of the cache,
-// one warp issues the products, four warps (64 rows, 16 a warp) do the softmax, four more rescale O and write results.
+// two warps issue the products, four warps (64 rows, 16 a warp) do the softmax, four more rescale O and write results.
 //   S[row][token]     = Q~ K^T          M 64, N 64, K R + P; two buffers, so that S of the next tile is computed beside a softmax
 //   O^T[latent][row] += K^T P^T         M 128 (R / 128 times), N 64, K 64: the tile is read MN-major from the same image, and the
 //                                       rows (heads) are columns, so few heads leave no tensor-memory lane idle
-// A tile lies in shared memory in two halves of its latent elements (the second with the rotated part), each in groups of eight tokens,
-// [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view of the cache, so a block is three copies; issuing one for
-// every chunk took 900 cycles.  Halves come and are freed by themselves: S begins with the first, and the products of the first half of O free
-// it while the second is at work.
+// A tile lies in shared memory in groups of eight tokens, [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view of
+// the cache, so a block is two copies (the rotated part is the other); issuing one for every chunk took 900 cycles.  Its halves of 32 tokens come
+// and are freed by themselves.
+// S and O are issued by a warp each: one warp for both had to look at two barriers in turn, and a look, with what follows it, is 200 cycles.
+// Tiles of 32 tokens, four in flight, were no faster: an M 64, N 32 step takes 26 cycles, one of N 64 33.
 constexpr int kSlots = 4;               // depth of the queue of runs
-constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: products, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)
+constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: S, 6: O, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)
 constexpr float kLazy = 8.f;            // log2 of the growth of a row maximum that rescales O
 
 // A stretch of context tiles of one row tile.
@@ -186,21 +201,22 @@ struct AttendSmem {
     alignas(1024) uint8_t q[kTile * R * 2];
     alignas(1024) uint8_t q_rope[kTile * 128];
     struct Tile {
-        uint8_t c[2][kTile * R];
-        uint8_t rope[kTile * 128];
+        uint8_t c[kTokens * R * 2];
+        uint8_t rope[kTokens * 128];
     };
     alignas(1024) Tile k[NST];
     alignas(1024) uint8_t p[kTile * 128];           // [row][token]
     float alpha[2][kTile];
-    float2 stat[2][kTile];                          // maximum and sum of the rows of a run
+    float stat[2][kTile][3];                        // maximum, sum and its reciprocal of the rows of a run
     volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
     volatile int event;                             // what the results warps are asked for: rescale after tile `event` - 1, or results (0)
-    uint64_t k_full[NST][2], k_free[NST][2];        // loader -> products (bytes), products -> loader
+    uint64_t k_full[NST][2], k_free[NST][2];        // halves of tiles: loader -> products (bytes), products -> loader
     uint64_t q_full, q_free;
-    uint64_t s_full[2], p_full, o_done;             // products -> softmax, softmax -> products, products -> softmax and results
+    uint64_t s_full[2], s_free[2];                  // products -> softmax, softmax -> products
+    uint64_t p_full, o_done;                        // softmax -> products, products -> softmax and results
     uint64_t asked, answered;                       // products -> results, results -> products
-    // softmax -> results, runs in turn: the softmax can be a run ahead of the results, and no more, because the first P of a run waits for the last
-    // product of the run before, whose first product waits for the results before that
+    // softmax -> results, runs in turn.  The softmax gets at most a run ahead of the results: a tile's P waits for the products of the tile
+    // before, and a run's first products wait for the results of the run before
     uint64_t stat_full[2];
     uint64_t run_full[kSlots], run_free[kSlots];
     Run run[kSlots];
@@ -212,25 +228,22 @@ template <int R, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AbsorbedArgs a) {
     using Smem = AttendSmem<R>;
     constexpr int NC = R / 64, NST = Smem::NST, MT = R / 128;
-    constexpr uint32_t kGroup = NC / 2 * 1024;      // bytes from one group of eight rows to the next, in a half of a tile
+    constexpr uint32_t kGroup = NC * 1024;          // bytes from one group of eight tokens to the next
     constexpr uint32_t kTmemS = MT * kTile;         // O^T: MT x 64 columns, then S twice
-    extern __shared__ uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2 * NST; ++i) { pa::mbar_init(&sm.k_full[0][i], 1); pa::mbar_init(&sm.k_free[0][i], 1); }
         pa::mbar_init(&sm.q_full, 1);
         pa::mbar_init(&sm.q_free, 1);
-        pa::mbar_init(&sm.s_full[0], 1);
-        pa::mbar_init(&sm.s_full[1], 1);
+        for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.s_full[i], 1); pa::mbar_init(&sm.s_free[i], 4); pa::mbar_init(&sm.stat_full[i], 4); }
         pa::mbar_init(&sm.p_full, 4);
         pa::mbar_init(&sm.o_done, 1);
         pa::mbar_init(&sm.asked, 1);
         pa::mbar_init(&sm.answered, 4);
-        pa::mbar_init(&sm.stat_full[0], 4);
-        pa::mbar_init(&sm.stat_full[1], 4);
-        for (int i = 0; i < kSlots; ++i) { pa::mbar_init(&sm.run_full[i], 1); pa::mbar_init(&sm.run_free[i], 9); }
+        for (int i = 0; i < kSlots; ++i) { pa::mbar_init(&sm.run_full[i], 1); pa::mbar_init(&sm.run_free[i], 10); }
         pa::mbar_fence_init();
         sm.grew[0] = sm.grew[1] = 0;
         sm.abort_flag = 0;
@@ -252,21 +265,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 
     if (warp == 4) {
         // ======================= loader =================================================================
-        const int group = blockIdx.x / a.row_tiles, member = blockIdx.x % a.row_tiles, B = m.num_sequences;
-        const long long per = slice_size(a), total = a.unit_prefix[B];
-        long long u = group * per;
-        const long long u_end = min(total, u + per);
+        const int group = blockIdx.x / a.row_tiles, member = blockIdx.x % a.row_tiles;
+        const SliceStart start = a.starts[group];
+        int s = start.s, block = start.block, first = start.first, left = start.units;     // left: units of the slice
         uint32_t n = 0, nr = 0, nq = 0;      // tiles, queue entries, query tiles so far
         bool ok = true, bad_index = false;
-        int s = 0;
-        if (u < u_end) {
-            int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.unit_prefix[mid] <= u) lo = mid; else hi = mid;
-            }
-            s = lo;
-        }
         auto publish = [&](const Run& r) -> bool {
             const int slot = nr % kSlots;
             if (nr >= kSlots && !wt.wait_warp(&sm.run_free[slot], (nr / kSlots - 1) & 1)) return false;
@@ -275,28 +278,34 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ++nr;
             return true;
         };
-        Cut cut{0, 0, 0, 0};
-        if (u < u_end) {
-            // where this slice is the first to begin inside a block of rows, its partial results are joined afterwards
-            SeqView v;
-            seq_view(m, s, v);
-            const long long tiles = ((long long)v.past + v.n + kTile - 1) / kTile, block = (u - a.unit_prefix[s]) / tiles, u0 = a.unit_prefix[s] + block * tiles;
-            if (u0 < u && u0 / per + 1 == group) {
-                const int row0 = (int)(block * a.row_tiles + member) * kTile;
-                cut.rows = (int)min((long long)kTile, (long long)v.n * m.H - row0);
-                cut.grow0 = (int)((long long)v.t0 * m.H + row0);
-                cut.slot = (int)(((long long)a.block_prefix[s] + block + u0 / per) * a.row_tiles + member);
-                cut.pieces = (int)((u0 + tiles - 1) / per - u0 / per) + 1;
+        // Where this slice is the first to begin inside a block of rows, its partial results are joined afterwards.
+        if (lane == 0) {
+            Cut cut{0, 0, 0, 0};
+            if (s >= 0 && first > 0) {
+                SeqView v;
+                seq_view(m, s, v);
+                const long long per = *a.per, tiles = ((long long)v.past + v.n + kTokens - 1) / kTokens, u0 = group * per - first;
+                if (u0 / per + 1 == group) {
+                    const int row0 = (block * a.row_tiles + member) * kTile;
+                    cut.rows = (int)min((long long)kTile, (long long)v.n * m.H - row0);
+                    cut.grow0 = (int)((long long)v.t0 * m.H + row0);
+                    cut.slot = (int)(((long long)a.block_prefix[s] + block + u0 / per) * a.row_tiles + member);
+                    cut.pieces = (int)((u0 + tiles - 1) / per - u0 / per) + 1;
+                }
             }
+            a.cuts[blockIdx.x] = cut;
         }
-        if (lane == 0) a.cuts[blockIdx.x] = cut;
-        while (ok && u < u_end) {
+        __syncwarp();
+        while (ok && s >= 0 && left > 0) {
             SeqView v;
             seq_view(m, s, v);
-            const long long rel = u - a.unit_prefix[s];
-            const int tiles = (int)(((long long)v.past + v.n + kTile - 1) / kTile);
-            const int block = (int)(rel / tiles), first = (int)(rel % tiles);
-            const int len = (int)min((long long)(tiles - first), u_end - u);
+            const SeqPlan plan = seq_plan(a, s);
+            if (block >= plan.blocks) {      // the next sequence with work
+                ++s;
+                block = first = 0;
+                continue;
+            }
+            const int tiles = (int)plan.tiles, len = min(tiles - first, left);
             Run r;
             r.row0 = (block * a.row_tiles + member) * kTile;
             r.rows = (int)min((long long)kTile, (long long)v.n * m.H - r.row0);
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 r.past = v.past;
                 r.end = v.past + (r.row0 + r.rows - 1) / m.H + 1;
                 r.first = first;
-                r.tiles = max(0, min(first + len, (r.end + kTile - 1) / kTile) - first);
+                r.tiles = max(0, min(first + len, (r.end + kTokens - 1) / kTokens) - first);
                 r.tb = v.tb;
                 r.whole = len == tiles;
                 r.slot = ((long long)a.block_prefix[s] + block + group) * a.row_tiles + member;
@@ -319,39 +328,48 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     }
                     __syncwarp();
                     ++nq;
-                    const int per_tile = kTile / m.bs, last_block = (r.end - 1) / m.bs;
+                    // pieces of a half tile: 32 tokens of a block, or two blocks of 16 (all powers of two)
+                    const int bs_log2 = 31 - __clz(m.bs), piece_log2 = min(bs_log2, 5), piece = 1 << piece_log2, pieces = 32 >> piece_log2;
+                    const int sub_log2 = bs_log2 - piece_log2, last_piece = (r.end - 1) >> piece_log2;
                     int page = 0, base = -1;     // this lane's block of the 32 from `base`
                     for (int j = 0; ok && j < r.tiles; ++j, ++n) {
-                        const int b0 = (r.first + j) * per_tile, blocks = min(per_tile, last_block - b0 + 1);
-                        if (base < 0 || b0 + per_tile > base + 32) {
+                        const int p0 = (r.first + j) * 2 * pieces, b0 = p0 >> sub_log2;
+                        if (base < 0 || b0 + 2 * pieces > base + 32) {
                             base = b0;
                             page = 0;
-                            if (base + lane <= last_block) {
+                            if (base + lane <= last_piece >> sub_log2) {
                                 page = m.block_indices[r.tb + base + lane];
                                 if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
                             }
                         }
                         const int st = n % NST;
+                        int group[4];            // of eight tokens of the cache, of every piece of the tile
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = p0 + min(i, 2 * pieces - 1);
+                            group[i] = (__shfl_sync(0xffffffffu, page, (at >> sub_log2) - base) << (bs_log2 - 3)) + ((at & ((1 << sub_log2) - 1)) << (piece_log2 - 3));
+                        }
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
+                            const int count = max(0, min(pieces, last_piece - (p0 + half * pieces) + 1));
                             if (ok && n >= NST) ok = wt.wait_warp(&sm.k_free[st][half], (n / NST - 1) & 1);
                             if (!ok) break;
-                            if (tc05::elect_one()) pa::mbar_expect_tx(&sm.k_full[st][half], blocks * m.bs * (R + half * 128));
-                            __syncwarp();
-                            for (int i = 0; i < blocks; ++i) {
-                                const int at = __shfl_sync(0xffffffffu, page, b0 + i - base) * (m.bs / 8);
-                                if (tc05::elect_one()) {
-                                    tma_4d(sm.k[st].c[half] + i * (m.bs / 8) * kGroup, &a.map_cache, 0, 0, half * (NC / 2), at, &sm.k_full[st][half]);
-                                    if (half == 1) tma_3d(sm.k[st].rope + i * m.bs * 128, &a.map_cache_rope, 0, 0, at, &sm.k_full[st][half]);
+                            if (tc05::elect_one()) {
+                                pa::mbar_expect_tx(&sm.k_full[st][half], count * piece * (R * 2 + 128));
+                                for (int i = 0; i < count; ++i) {
+                                    const int row = half * 32 + i * piece, g = pieces == 1 ? group[half] : i == 0 ? group[2 * half] : group[2 * half + 1];
+                                    tma_4d(sm.k[st].c + (row >> 3) * kGroup, &a.map_cache, 0, 0, 0, g, &sm.k_full[st][half]);
+                                    tma_3d(sm.k[st].rope + row * 128, &a.map_cache_rope, 0, 0, g, &sm.k_full[st][half]);
                                 }
-                                __syncwarp();
                             }
+                            __syncwarp();
                         }
                     }
                 }
             }
-            u += len;
-            while (s < B && u >= a.unit_prefix[s + 1]) ++s;
+            left -= len;
+            first += len;
+            if (first == tiles) { first = 0; ++block; }
         }
         if (ok) {
             Run r{};
@@ -365,14 +383,51 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 for (uint32_t k = 0; k < (1u << 20) && !(pa::mbar_try_wait(&sm.k_full[i % NST][0], (i / NST) & 1) && pa::mbar_try_wait(&sm.k_full[i % NST][1], (i / NST) & 1)); ++k) {}
         }
     } else if (warp == 5) {
-        // ======================= products ================================================================
+        // ======================= S ========================================================================
         // (the whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took twice as long to issue)
-        constexpr uint32_t idesc_s = tc05::instr_desc_f16(kTile, kTile, BF ? 1 : 0, 0, 0);
-        constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
-        const uint32_t dq = desc_low(sm.q), dqr = desc_low(sm.q_rope), dk = desc_low(sm.k[0].c[0]), dkr = desc_low(sm.k[0].rope);
-        const uint32_t dv = desc_low(sm.k[0].c[0], 1024), dp = desc_low(sm.p);
-        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4, kHalf = kTile * R >> 4;
+        constexpr uint32_t idesc_s = tc05::instr_desc_f16(kTile, kTokens, BF ? 1 : 0, 0, 0);
+        const uint32_t dq = desc_low(sm.q), dqr = desc_low(sm.q_rope), dk = desc_low(sm.k[0].c), dkr = desc_low(sm.k[0].rope);
+        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4;
         const bool wide = m.P == 64;
+        uint32_t n = 0;
+        bool ok = true;
+        Run r;
+        for (uint32_t nr = 0, nq = 0; ok; ++nr) {
+            if (!fetch(nr, r) || r.rows == 0) break;
+            if (r.tiles == 0) continue;
+            ok = wt.wait_warp(&sm.q_full, nq & 1);
+            ++nq;
+            for (int j = 0; ok && j < r.tiles; ++j, ++n) {
+                const int st = n % NST;
+                ok = (n < 2 || wt.wait_warp(&sm.s_free[n & 1], ((n >> 1) - 1) & 1)) && wt.wait_warp(&sm.k_full[st][0], (n / NST) & 1) &&
+                     wt.wait_warp(&sm.k_full[st][1], (n / NST) & 1);
+                if (!ok) break;
+                const uint32_t db = dk + st * kStage, dbr = dkr + st * kStage, d = tmem + kTmemS + (n & 1) * kTokens;
+                tc05::fence_after_thread_sync();
+                if (tc05::elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < R / 16; ++kk) {
+                        const uint32_t qa = dq + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, kb = db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2;
+                        if (kk == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
+                        else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
+                    }
+                    mma_ss<1>(d, dqr, dbr, idesc_s);
+                    mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
+                    if (wide) {
+                        mma_ss<1>(d, dqr + 4, dbr + 4, idesc_s);
+                        mma_ss<1>(d, dqr + 6, dbr + 6, idesc_s);
+                    }
+                    tc05::commit(&sm.s_full[n & 1]);
+                    if (j + 1 == r.tiles) tc05::commit(&sm.q_free);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 6) {
+        // ======================= O ========================================================================
+        constexpr uint32_t idesc_o = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
+        const uint32_t dv = desc_low(sm.k[0].c, 1024), dp = desc_low(sm.p);
+        constexpr uint32_t kStage = sizeof(typename Smem::Tile) >> 4;
         uint32_t n = 0, asked = 0;
         bool ok = true;
         Run r;
@@ -381,74 +436,33 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             warp_arrive(&sm.asked);
             ++asked;
         };
-        for (uint32_t nr = 0, nq = 0; ok; ++nr) {
+        for (uint32_t nr = 0; ok; ++nr) {
             if (!fetch(nr, r) || r.rows == 0) break;
             if (r.tiles == 0) continue;
-            ok = wt.wait_warp(&sm.q_full, nq & 1);
-            ++nq;
-            const uint32_t end = n + r.tiles;
-            uint32_t next_s = n, half = 0, next_o = n;
-            uint32_t idle = 0;
-            // O as soon as its P is there; each half of S as soon as that of the tile is, but no more than a tile ahead of O
-            while (ok && next_o < end) {
-                if (next_o < next_s && __all_sync(0xffffffffu, mbar_test(&sm.p_full, next_o & 1))) {
-                    if (next_o == n) {
-                        // the first product overwrites O: the results of the run before have been read
-                        if (asked > 0) ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
-                    } else if (sm.grew[next_o & 1] == next_o + 1) {
-                        ask((int)next_o);
-                        ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
-                    }
-                    if (!ok) break;
-                    tc05::fence_after_thread_sync();
-                    const uint32_t da = dv + next_o % NST * kStage;
-                    if (tc05::elect_one()) {
+            for (int j = 0; ok && j < r.tiles; ++j, ++n) {
+                ok = wt.wait_warp(&sm.p_full, n & 1);
+                if (ok && j > 0 && sm.grew[n & 1] == n + 1) ask((int)n);
+                // (the first product overwrites O: the results of the run before have been read)
+                if (ok && asked > 0 && (j == 0 || sm.grew[n & 1] == n + 1)) ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
+                if (!ok) break;
+                tc05::fence_after_thread_sync();
+                const uint32_t da = dv + n % NST * kStage;
+                if (tc05::elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < kTokens / 16; ++kk) {
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            const uint32_t d = tmem + mt * kTile, pa = da + mt / (MT / 2) * kHalf + mt % (MT / 2) * (2048 >> 4);
-                            if (next_o > n) mma_ss<1, kGroup>(d, pa, dp, idesc_o);
-                            else mma_ss<0, kGroup>(d, pa, dp, idesc_o);
-#pragma unroll
-                            for (int kk = 1; kk < kTile / 16; ++kk) mma_ss<1, kGroup>(d, pa + kk * (2 * kGroup >> 4), dp + kk * 2, idesc_o);
-                            if (mt % (MT / 2) == MT / 2 - 1) tc05::commit(&sm.k_free[next_o % NST][mt / (MT / 2)]);
+                            const uint32_t d = tmem + mt * kTile, pa = da + mt * (2048 >> 4) + kk * (2 * kGroup >> 4);
+                            if (kk == 0 && j == 0) mma_ss<0, kGroup>(d, pa, dp, idesc_o);
+                            else mma_ss<1, kGroup>(d, pa, dp + kk * 2, idesc_o);
                         }
-                        tc05::commit(&sm.o_done);
+                        if (kk == kTokens / 32 - 1) tc05::commit(&sm.k_free[n % NST][0]);
                     }
-                    __syncwarp();
-                    ++next_o;
-                    idle = 0;
-                } else if (next_s < end && next_s <= next_o + 1 && __all_sync(0xffffffffu, mbar_test(&sm.k_full[next_s % NST][half], (next_s / NST) & 1))) {
-                    const uint32_t db = dk + next_s % NST * kStage + half * kHalf, dbr = dkr + next_s % NST * kStage, d = tmem + kTmemS + (next_s & 1) * kTile;
-                    const uint32_t dqh = dq + half * kHalf;
-                    tc05::fence_after_thread_sync();
-                    if (tc05::elect_one()) {
-                        if (half == 0) mma_ss<0, 1024, kGroup>(d, dqh, db, idesc_s);
-                        else mma_ss<1, 1024, kGroup>(d, dqh, db, idesc_s);
-#pragma unroll
-                        for (int kk = 1; kk < R / 32; ++kk)
-                            mma_ss<1, 1024, kGroup>(d, dqh + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2, idesc_s);
-                        if (half == 1) {
-                            mma_ss<1>(d, dqr, dbr, idesc_s);
-                            mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
-                            if (wide) {
-                                mma_ss<1>(d, dqr + 4, dbr + 4, idesc_s);
-                                mma_ss<1>(d, dqr + 6, dbr + 6, idesc_s);
-                            }
-                            tc05::commit(&sm.s_full[next_s & 1]);
-                            if (next_s + 1 == end) tc05::commit(&sm.q_free);
-                        }
-                    }
-                    __syncwarp();
-                    next_s += half;
-                    half ^= 1u;
-                    idle = 0;
-                } else if (++idle > (1u << 26)) {
-                    ok = wt.give_up();
-                } else if ((idle & 1023u) == 1023u && __any_sync(0xffffffffu, *wt.abort)) {
-                    ok = false;
+                    tc05::commit(&sm.k_free[n % NST][1]);
+                    tc05::commit(&sm.o_done);
                 }
+                __syncwarp();
             }
-            n = end;
             if (ok) ask(-1);
         }
     } else if (warp >= 8) {
@@ -488,9 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 continue;
             }
             if (!wt.wait_warp(&sm.stat_full[ns & 1], (ns >> 1) & 1)) break;
-            const float2* stat = sm.stat[ns & 1];
+            const float (*stat)[3] = sm.stat[ns & 1];
             ++ns;
-            if (!r.whole && e < r.rows) a.part_ml[r.slot * kTile + e] = stat[e];
+            if (!r.whole && e < r.rows) a.part_ml[r.slot * kTile + e] = make_float2(stat[e][0], stat[e][1]);
 #pragma unroll 1
             for (int q = 0; q < MT * 2; ++q) {
                 const int c0 = (q & 1) * 32;
@@ -503,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 #pragma unroll
                     for (int c = 0; c < 32; ++c)
                         if (c0 + c < r.rows) {
-                            const float x = __uint_as_float(o[c]) * __frcp_rn(stat[c0 + c].y);
+                            const float x = __uint_as_float(o[c]) * stat[c0 + c][2];
                             const uint16_t hi = pack1<BF>(x);
                             dst[c * (2 * R)] = hi;
                             dst[c * (2 * R) + R] = pack1<BF>(x - unpack1<BF>(hi));
@@ -539,15 +553,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 tc05::fence_after_thread_sync();
                 const bool free_p = n == 0 || mbar_test(&sm.o_done, (n - 1) & 1);      // P of the tile before has been read (looked at early: the answer takes its time)
                 uint32_t raw[32];
-                ld_16x256b_x8(tmem + kTmemS + (n & 1) * kTile + lanes, raw);
+                ld_16x256b_x8(tmem + kTmemS + (n & 1) * kTokens + lanes, raw);
                 tc05::wait_ld();
+                tc05::fence_before_thread_sync();
+                warp_arrive(&sm.s_free[n & 1]);
                 float sv[2][16];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sv[e >> 1][2 * i + (e & 1)] = __uint_as_float(raw[4 * i + e]);
-                const int col0 = (r.first + j) * kTile;
-                if (col0 + kTile > least) {
+                const int col0 = (r.first + j) * kTokens;
+                if (col0 + kTokens > least) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -585,16 +601,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<uint32_t*>(sm.p + rl[x] * 128 + ((i ^ (rl[x] & 7)) << 4) + (lane & 3) * 4) = pack2<BF>(sv[x][2 * i], sv[x][2 * i + 1]);
-                if (col0 + kTile > r.end) {
+                if (col0 + kTokens > r.end) {
                     // tokens behind the context: whatever lies there (stale bytes, not-a-number) meets probabilities of zero, which does not
                     // make it zero, so the latents are cleared
                     const int st = n % NST, valid = r.end - col0;
                     if (!wt.wait_warp(&sm.k_full[st][0], (n / NST) & 1) || !wt.wait_warp(&sm.k_full[st][1], (n / NST) & 1)) { ok = false; break; }
-                    for (int i = tid; i < (kTile - valid) * 8; i += 128) {
+                    for (int i = tid; i < (kTokens - valid) * 8; i += 128) {
                         const int row = valid + i / 8;
 #pragma unroll
                         for (int c = 0; c < NC; ++c)
-                            *reinterpret_cast<uint4*>(sm.k[st].c[c / (NC / 2)] + (row >> 3) * kGroup + c % (NC / 2) * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sm.k[st].c + (row >> 3) * kGroup + c * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 tc05::fence_proxy_async_smem();
@@ -607,7 +623,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             for (int x = 0; x < 2; ++x) {
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-                if ((lane & 3) == 0) sm.stat[nst & 1][rl[x]] = make_float2(mx[x], l[x]);
+                if ((lane & 3) == 0) {
+                    float* stat = sm.stat[nst & 1][rl[x]];
+                    stat[0] = mx[x]; stat[1] = l[x]; stat[2] = 1.f / l[x];
+                }
             }
             warp_arrive(&sm.stat_full[nst & 1]);
             ++nst;
@@ -675,8 +694,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
 constexpr int kValueStages = 4;
 template <bool BF>
 __global__ void __launch_bounds__(160) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full[kValueStages], free_[kValueStages], done;
     __shared__ bool live[kTile];
     __shared__ uint32_t tmem_base;
@@ -762,8 +780,8 @@ template <int R, bool BF>
 cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     const Step& m = a.m;
     const int token_tiles = (m.num_tokens + kTile - 1) / kTile;
-    const int smem_q = 2 * m.Dn * 128 + m.Dn / 64 * 8192 + 1024, smem_v = kValueStages * (m.Dv * 128 + 2 * 8192) + 1024;
-    const int smem_a = sizeof(AttendSmem<R>) + 1024;
+    const int smem_q = 2 * m.Dn * 128 + m.Dn / 64 * 8192, smem_v = kValueStages * (m.Dv * 128 + 2 * 8192);
+    const int smem_a = sizeof(AttendSmem<R>);
     cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_a);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);

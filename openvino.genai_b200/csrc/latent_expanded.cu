@@ -145,8 +145,8 @@ template <int R, int DN, int DV, bool BF>
 __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_constant__ ExpandedArgs a) {
     using Smem = ExpandSmem<R>;
     constexpr int NC = R / 64;
-    extern __shared__ uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
     using Smem = ExpandedSmem<DN, DV>;
     constexpr int NQ = Smem::NQ, NV = Smem::NV, KS = Smem::KS, VS = Smem::VS;
     constexpr uint32_t kO = 256;       // S_A, S_B: 128 columns each (P in the first 64), then O_A, O_B
-    extern __shared__ uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
 
 template <int DN, int DV, bool BF>
 cudaError_t attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream) {
-    const int smem = sizeof(ExpandedSmem<DN, DV>) + 1024;
+    const int smem = sizeof(ExpandedSmem<DN, DV>);
     // the warpgroups re-divide the registers that the CTA was launched with: fewer than this would leave one of them waiting
     static const int regs = [] {
         cudaFuncAttributes f;
@@ -698,7 +698,7 @@ cudaError_t attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream) {
 
 template <int R, int DN, int DV, bool BF>
 cudaError_t expand_and_attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
-    const int smem = sizeof(ExpandSmem<R>) + 1024;
+    const int smem = sizeof(ExpandSmem<R>);
     const cudaError_t e = cudaFuncSetAttribute(expand_kernel<R, DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     expand_kernel<R, DN, DV, BF><<<sm_count, kExpandThreads, smem, stream>>>(a);

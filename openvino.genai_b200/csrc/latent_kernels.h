@@ -42,7 +42,8 @@ struct AppendArgs {
 // sequence; sequence s has block_prefix[s + 1] - block_prefix[s] such blocks, every one of the same number of tiles.  Units are
 // numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut leaves
 // one partial result per group in slot (block + group) * row_tiles + row tile.
-constexpr int kTile = 64;      // context tokens of a tile, query rows of a row tile, tokens of a projection's tile
+constexpr int kTile = 64;      // query rows of a row tile, new tokens of a projection's tile
+constexpr int kTokens = 64;    // context tokens of a tile
 
 // A row tile whose block the CTA's slice is the first to cut: where its partial results are and where the joined rows go.
 struct __align__(16) Cut {
@@ -52,12 +53,19 @@ struct __align__(16) Cut {
     int pieces;
 };
 
+// Where a group's slice begins: sequence (-1: no units), row block of the sequence, context tile of the block, and its units.
+struct __align__(16) SliceStart {
+    int s, block, first, units;
+};
+
 struct AbsorbedArgs {
     Step m;
     int max_new;                // sequences with more new tokens are left to the expanded form
     int groups, row_tiles;
     long long* unit_prefix;     // [num_sequences + 1]
     int* block_prefix;          // [num_sequences + 1]
+    SliceStart* starts;         // [groups]
+    long long* per;             // units of a slice
     const void* q_rope;
     long long qr_token, qr_head;
     void* q_abs;                // [num_tokens * H][R + P] absorbed query rows
