@@ -56,26 +56,41 @@ __device__ void build_plan(const AbsorbedArgs& a) {
     }
     if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; }
     __syncthreads();
-    // where every slice begins, so that a CTA of the attention has one record to read instead of a search
+    // where every slice begins, so that a CTA of the attention has one record to read instead of a search, and what it cuts
     const long long total = run_u, per = total > 0 ? (total + a.groups - 1) / a.groups : 1;
     for (int w = tid; w < a.groups; w += 128) {
         const long long u = w * per;
-        SliceStart st{-1, 0, 0, 0};
+        SliceStart st{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        Cut cut{0, 0, 0, 0};
         if (u < total) {
             int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (a.unit_prefix[mid] <= u) lo = mid; else hi = mid;
             }
-            const long long rel = u - a.unit_prefix[lo], tiles = seq_plan(a, lo).tiles;
-            st.s = lo;
-            st.block = (int)(rel / tiles);
-            st.first = (int)(rel % tiles);
-            st.units = (int)min(per, total - u);
+            SeqView v;
+            seq_view(a.m, lo, v);
+            const SeqPlan p = seq_plan(a, lo);
+            const long long rel = u - a.unit_prefix[lo];
+            st = SliceStart{lo, (int)(rel / p.tiles), (int)(rel % p.tiles), (int)min(per, total - u), v.t0, v.n, v.past, v.tb, p.blocks, (int)p.tiles, a.block_prefix[lo], 0};
+            const long long u0 = u - st.first;
+            if (st.first > 0 && u0 / per + 1 == w) {      // the first slice to begin inside this block: its partial results are joined afterwards
+                const int row0 = st.block * a.row_tiles * kTile;
+                cut.rows = (int)min((long long)kTile * a.row_tiles, (long long)v.n * a.m.H - row0);
+                cut.grow0 = (int)((long long)v.t0 * a.m.H + row0);
+                cut.slot = (int)(((long long)st.block0 + st.block + u0 / per) * a.row_tiles);
+                cut.pieces = (int)((u0 + p.tiles - 1) / per - u0 / per) + 1;
+            }
         }
         a.starts[w] = st;
+        for (int member = 0; member < a.row_tiles; ++member) {
+            Cut c = cut;
+            c.rows = max(0, min(kTile, cut.rows - member * kTile));
+            c.grow0 += member * kTile;
+            c.slot += member;
+            a.cuts[w * a.row_tiles + member] = c;
+        }
     }
-    if (tid == 0) *a.per = per;
 }
 
 // Which of the tile's tokens belong to sequences of this form; false (for the whole block) if none does.
@@ -180,6 +195,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
 // Tiles of 32 tokens, four in flight, were no faster: an M 64, N 32 step takes 26 cycles, one of N 64 33.
 constexpr int kSlots = 4;               // depth of the queue of runs
 constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: S, 6: O, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)
+template <int R> constexpr int kAheadOf = R == 512 ? 4 : 6;     // tiles ahead of the loads that are brought into the L2 cache
 constexpr float kLazy = 8.f;            // log2 of the growth of a row maximum that rescales O
 
 // A stretch of context tiles of one row tile.
@@ -268,7 +284,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         const int group = blockIdx.x / a.row_tiles, member = blockIdx.x % a.row_tiles;
         const SliceStart start = a.starts[group];
         int s = start.s, block = start.block, first = start.first, left = start.units;     // left: units of the slice
+        SeqView v{start.t0, start.n, start.past, start.tb};
+        int blocks = start.blocks, tiles = start.tiles, block0 = start.block0;
         uint32_t n = 0, nr = 0, nq = 0;      // tiles, queue entries, query tiles so far
+        const uint64_t policy = evict_first();
         bool ok = true, bad_index = false;
         auto publish = [&](const Run& r) -> bool {
             const int slot = nr % kSlots;
@@ -278,34 +297,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ++nr;
             return true;
         };
-        // Where this slice is the first to begin inside a block of rows, its partial results are joined afterwards.
-        if (lane == 0) {
-            Cut cut{0, 0, 0, 0};
-            if (s >= 0 && first > 0) {
-                SeqView v;
-                seq_view(m, s, v);
-                const long long per = *a.per, tiles = ((long long)v.past + v.n + kTokens - 1) / kTokens, u0 = group * per - first;
-                if (u0 / per + 1 == group) {
-                    const int row0 = (block * a.row_tiles + member) * kTile;
-                    cut.rows = (int)min((long long)kTile, (long long)v.n * m.H - row0);
-                    cut.grow0 = (int)((long long)v.t0 * m.H + row0);
-                    cut.slot = (int)(((long long)a.block_prefix[s] + block + u0 / per) * a.row_tiles + member);
-                    cut.pieces = (int)((u0 + tiles - 1) / per - u0 / per) + 1;
-                }
-            }
-            a.cuts[blockIdx.x] = cut;
-        }
-        __syncwarp();
         while (ok && s >= 0 && left > 0) {
-            SeqView v;
-            seq_view(m, s, v);
-            const SeqPlan plan = seq_plan(a, s);
-            if (block >= plan.blocks) {      // the next sequence with work
+            if (block >= blocks) {      // the next sequence with work
                 ++s;
                 block = first = 0;
+                seq_view(m, s, v);
+                const SeqPlan plan = seq_plan(a, s);
+                blocks = plan.blocks;
+                tiles = (int)plan.tiles;
+                block0 = a.block_prefix[s];
                 continue;
             }
-            const int tiles = (int)plan.tiles, len = min(tiles - first, left);
+            const int len = min(tiles - first, left);
             Run r;
             r.row0 = (block * a.row_tiles + member) * kTile;
             r.rows = (int)min((long long)kTile, (long long)v.n * m.H - r.row0);
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 r.tiles = max(0, min(first + len, (r.end + kTokens - 1) / kTokens) - first);
                 r.tb = v.tb;
                 r.whole = len == tiles;
-                r.slot = ((long long)a.block_prefix[s] + block + group) * a.row_tiles + member;
+                r.slot = ((long long)block0 + block + group) * a.row_tiles + member;
                 ok = publish(r);
                 if (ok && r.tiles > 0) {
                     if (nq > 0) ok = wt.wait_warp(&sm.q_free, (nq - 1) & 1);
@@ -332,9 +335,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     const int bs_log2 = 31 - __clz(m.bs), piece_log2 = min(bs_log2, 5), piece = 1 << piece_log2, pieces = 32 >> piece_log2;
                     const int sub_log2 = bs_log2 - piece_log2, last_piece = (r.end - 1) >> piece_log2;
                     int page = 0, base = -1;     // this lane's block of the 32 from `base`
+                    // group of eight tokens of the cache at which piece `at` of the sequence lies
+                    auto group_of = [&](int at) {
+                        return (__shfl_sync(0xffffffffu, page, (at >> sub_log2) - base) << (bs_log2 - 3)) + ((at & ((1 << sub_log2) - 1)) << (piece_log2 - 3));
+                    };
                     for (int j = 0; ok && j < r.tiles; ++j, ++n) {
                         const int p0 = (r.first + j) * 2 * pieces, b0 = p0 >> sub_log2;
-                        if (base < 0 || b0 + 2 * pieces > base + 32) {
+                        if (base < 0 || b0 + (kAheadOf<R> + 1) * 2 * pieces > base + 32) {
                             base = b0;
                             page = 0;
                             if (base + lane <= last_piece >> sub_log2) {
@@ -343,12 +350,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                             }
                         }
                         const int st = n % NST;
-                        int group[4];            // of eight tokens of the cache, of every piece of the tile
+                        int group[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int at = p0 + min(i, 2 * pieces - 1);
-                            group[i] = (__shfl_sync(0xffffffffu, page, (at >> sub_log2) - base) << (bs_log2 - 3)) + ((at & ((1 << sub_log2) - 1)) << (piece_log2 - 3));
-                        }
+                        for (int i = 0; i < 4; ++i) group[i] = group_of(p0 + min(i, 2 * pieces - 1));
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const int count = max(0, min(pieces, last_piece - (p0 + half * pieces) + 1));
@@ -358,12 +362,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                                 pa::mbar_expect_tx(&sm.k_full[st][half], count * piece * (R * 2 + 128));
                                 for (int i = 0; i < count; ++i) {
                                     const int row = half * 32 + i * piece, g = pieces == 1 ? group[half] : i == 0 ? group[2 * half] : group[2 * half + 1];
-                                    tma_4d(sm.k[st].c + (row >> 3) * kGroup, &a.map_cache, 0, 0, 0, g, &sm.k_full[st][half]);
-                                    tma_3d(sm.k[st].rope + row * 128, &a.map_cache_rope, 0, 0, g, &sm.k_full[st][half]);
+                                    tma_4d(sm.k[st].c + (row >> 3) * kGroup, &a.map_cache, 0, 0, 0, g, &sm.k_full[st][half], policy);
+                                    tma_3d(sm.k[st].rope + row * 128, &a.map_cache_rope, 0, 0, g, &sm.k_full[st][half], policy);
                                 }
                             }
                             __syncwarp();
                         }
+                        // tiles to come go to the L2 cache meanwhile (the CTAs of a group take turns): two tiles in flight do not cover the memory's latency
+                        for (int ahead = j == 0 ? NST : kAheadOf<R>; ahead <= kAheadOf<R>; ++ahead)
+                            if ((j + ahead) % a.row_tiles == member)
+                                for (int i = 0; i < 2 * pieces; ++i) {
+                                    const int at = p0 + ahead * 2 * pieces + i, g = group_of(min(at, last_piece));
+                                    if (at <= last_piece && tc05::elect_one()) {
+                                        prefetch_4d(&a.map_cache, 0, 0, 0, g, policy);
+                                        prefetch_3d(&a.map_cache_rope, 0, 0, g, policy);
+                                    }
+                                    __syncwarp();
+                                }
                     }
                 }
             }
@@ -399,17 +414,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ++nq;
             for (int j = 0; ok && j < r.tiles; ++j, ++n) {
                 const int st = n % NST;
-                ok = (n < 2 || wt.wait_warp(&sm.s_free[n & 1], ((n >> 1) - 1) & 1)) && wt.wait_warp(&sm.k_full[st][0], (n / NST) & 1) &&
-                     wt.wait_warp(&sm.k_full[st][1], (n / NST) & 1);
+                ok = (n < 2 || wt.spin_warp(&sm.s_free[n & 1], ((n >> 1) - 1) & 1)) && wt.spin_warp(&sm.k_full[st][0], (n / NST) & 1) &&
+                     wt.spin_warp(&sm.k_full[st][1], (n / NST) & 1);
                 if (!ok) break;
                 const uint32_t db = dk + st * kStage, dbr = dkr + st * kStage, d = tmem + kTmemS + (n & 1) * kTokens;
                 tc05::fence_after_thread_sync();
                 if (tc05::elect_one()) {
-#pragma unroll
-                    for (int kk = 0; kk < R / 16; ++kk) {
-                        const uint32_t qa = dq + (kk >> 2) * (kTile * 128 >> 4) + (kk & 3) * 2, kb = db + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2;
-                        if (kk == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
+#pragma unroll 4
+                    for (int c = 0; c < NC; ++c) {
+                        const uint32_t qa = dq + c * (kTile * 128 >> 4), kb = db + c * (1024 >> 4);
+                        if (c == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
                         else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
+#pragma unroll
+                        for (int kk = 1; kk < 4; ++kk) mma_ss<1, 1024, kGroup>(d, qa + kk * 2, kb + kk * 2, idesc_s);
                     }
                     mma_ss<1>(d, dqr, dbr, idesc_s);
                     mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
@@ -440,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             if (!fetch(nr, r) || r.rows == 0) break;
             if (r.tiles == 0) continue;
             for (int j = 0; ok && j < r.tiles; ++j, ++n) {
-                ok = wt.wait_warp(&sm.p_full, n & 1);
+                ok = wt.spin_warp(&sm.p_full, n & 1);
                 if (ok && j > 0 && sm.grew[n & 1] == n + 1) ask((int)n);
                 // (the first product overwrites O: the results of the run before have been read)
                 if (ok && asked > 0 && (j == 0 || sm.grew[n & 1] == n + 1)) ok = wt.wait_warp(&sm.answered, (asked - 1) & 1);
@@ -513,15 +530,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
                 tc05::wait_ld();
                 if (r.whole) {
-                    uint16_t* dst = (uint16_t*)a.o_lat + (r.grow0 + c0) * (2 * R) + (q >> 1) * 128 + e;
+                    // two lanes (neighbouring elements) share two rows: each stores both elements of one
+                    uint16_t* dst = (uint16_t*)a.o_lat + (r.grow0 + c0 + (lane & 1)) * (2 * R) + (q >> 1) * 128 + (e & ~1);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (c0 + c < r.rows) {
-                            const float x = __uint_as_float(o[c]) * stat[c0 + c][2];
-                            const uint16_t hi = pack1<BF>(x);
-                            dst[c * (2 * R)] = hi;
-                            dst[c * (2 * R) + R] = pack1<BF>(x - unpack1<BF>(hi));
+                    for (int c = 0; c < 32; c += 2) {
+                        const float x0 = __uint_as_float(o[c]) * stat[c0 + c][2], x1 = __uint_as_float(o[c + 1]) * stat[c0 + c + 1][2];
+                        const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x0 : x1, 1);
+                        const float lo = lane & 1 ? other : x0, up = lane & 1 ? x1 : other;
+                        const uint32_t hi = pack2<BF>(lo, up);
+                        if (c0 + c + (lane & 1) < r.rows) {
+                            *reinterpret_cast<uint32_t*>(dst + c * (2 * R)) = hi;
+                            *reinterpret_cast<uint32_t*>(dst + c * (2 * R) + R) = pack2<BF>(lo - unpack1<BF>((uint16_t)hi), up - unpack1<BF>((uint16_t)(hi >> 16)));
                         }
+                    }
                 } else {
                     float* dst = a.part_o + (r.slot * kTile + c0) * R + (q >> 1) * 128 + e;
 #pragma unroll

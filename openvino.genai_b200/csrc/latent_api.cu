@@ -123,7 +123,7 @@ constexpr size_t kExpandBytes = (size_t)1 << 30;
 
 struct Scratch {
     int row_tiles, groups;
-    size_t unit_prefix, block_prefix, starts, per, q_abs, part_o, part_ml, cuts, o_lat;
+    size_t unit_prefix, block_prefix, starts, q_abs, part_o, part_ml, cuts, o_lat;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
     size_t tile_prefix, query_prefix, order, counter, k, v, k_rope;
@@ -146,7 +146,6 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.unit_prefix = take(((size_t)sequences + 1) * sizeof(long long));
         s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.starts = take(s.groups * sizeof(latent::SliceStart));
-        s.per = take(sizeof(long long));
         s.q_abs = take(rows * (d.latent_size + d.rope_size) * 2);
         s.o_lat = take(rows * 2 * d.latent_size * 2);
         s.cuts = take((size_t)s.groups * s.row_tiles * sizeof(latent::Cut));
@@ -265,7 +264,6 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         k.unit_prefix = (long long*)(h->ws + s.unit_prefix);
         k.block_prefix = (int*)(h->ws + s.block_prefix);
         k.starts = (latent::SliceStart*)(h->ws + s.starts);
-        k.per = (long long*)(h->ws + s.per);
         k.q_rope = a->query_rope; k.qr_token = rt; k.qr_head = rh;
         k.q_abs = h->ws + s.q_abs;
         k.part_o = (float*)(h->ws + s.part_o);

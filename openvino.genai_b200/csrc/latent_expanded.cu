@@ -211,12 +211,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
             const ExpandItem it = expand_item(a, i, per);
             ok = wt.wait_warp(&sm.a_full, na & 1);
             for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
-                if (nd >= 2) ok = wt.wait_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
+                if (nd >= 2) ok = wt.spin_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
 #pragma unroll
                 for (int x = 0; x < 2 * NC; ++x) {
                     constexpr int kRound = 2 * NC / kWeightStages;     // (a stage's phase: its round in the head, and the heads before)
                     const int st = x % kWeightStages;
-                    if (ok) ok = wt.wait_warp(&sm.w_full[st], (nd * kRound + x / kWeightStages) & 1);
+                    if (ok) ok = wt.spin_warp(&sm.w_full[st], (nd * kRound + x / kWeightStages) & 1);
                     if (!ok) break;
                     tc05::fence_after_thread_sync();
                     const uint32_t d = tmem + (nd & 1) * kBuffer + (x < NC ? 0 : DN);
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 bool ok = true;
                 for (uint32_t ni = 0; ok; ++ni) {
                     const int slot = ni % kItemSlots;
-                    if (!wt.wait_warp(&sm.item_full[slot], (ni / kItemSlots) & 1)) break;
+                    if (!wt.spin_warp(&sm.item_full[slot], (ni / kItemSlots) & 1)) break;
                     const QueryItem it = sm.item[slot];
                     warp_arrive(&sm.item_free[slot]);
                     if (it.h < 0) break;
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         const uint32_t d = tmem + X * 128;
 #pragma unroll
                         for (int c = 0; c < NQ; ++c) {
-                            if (fresh) ok = ok && wt.wait_warp(&sm.k_full[k[X].at], k[X].phase);
+                            if (fresh) ok = ok && wt.spin_warp(&sm.k_full[k[X].at], k[X].phase);
                             if (!ok) return;
                             tc05::fence_after_thread_sync();
                             const uint32_t da = dq + (X * NQ + c) * kAtom, db = dk + k[X].at * kAtom;
@@ -534,8 +534,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         const uint32_t d = tmem + kO + X * DV;
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            if (fresh) ok = ok && wt.wait_warp(&sm.v_full[v[X].at], v[X].phase);
-                            ok = ok && wt.wait_warp(&sm.p_full[X][u], np[X] & 1);
+                            if (fresh) ok = ok && wt.spin_warp(&sm.v_full[v[X].at], v[X].phase);
+                            ok = ok && wt.spin_warp(&sm.p_full[X][u], np[X] & 1);
                             if (!ok) return;
                             tc05::fence_after_thread_sync();
                             const uint32_t p = tmem + X * 128 + u * 32, db = dv + v[X].at * kUnit;
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
 #pragma unroll
                     for (int X = 0; X < 2; ++X)
                         if (ok && it.tiles[X] > 0) {
-                            ok = wt.wait_warp(&sm.q_full[X], nq[X] & 1);
+                            ok = wt.spin_warp(&sm.q_full[X], nq[X] & 1);
                             ++nq[X];
                             if (ok) issue_s(X, 0);
                         }
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             float top = -INFINITY, l = 0.f;
             bool ok = true;
             for (int j = 0; j < tiles; ++j, ++n) {
-                if (!wt.wait_warp(&sm.s_full[X], n & 1)) { ok = false; break; }
+                if (!wt.spin_warp(&sm.s_full[X], n & 1)) { ok = false; break; }
                 tc05::fence_after_thread_sync();
                 uint32_t s[4][32];
 #pragma unroll

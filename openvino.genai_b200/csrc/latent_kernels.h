@@ -53,9 +53,14 @@ struct __align__(16) Cut {
     int pieces;
 };
 
-// Where a group's slice begins: sequence (-1: no units), row block of the sequence, context tile of the block, and its units.
+// Where a group's slice begins: sequence (-1: no units) and what there is to know of it, row block of the sequence, context tile of the block; and
+// the slice's units.
 struct __align__(16) SliceStart {
     int s, block, first, units;
+    int t0, n, past, tb;            // of the sequence (SeqView)
+    int blocks, tiles;              // its row blocks, and context tiles of each
+    int block0;                     // row blocks of the sequences before
+    int unused;
 };
 
 struct AbsorbedArgs {
@@ -65,7 +70,6 @@ struct AbsorbedArgs {
     long long* unit_prefix;     // [num_sequences + 1]
     int* block_prefix;          // [num_sequences + 1]
     SliceStart* starts;         // [groups]
-    long long* per;             // units of a slice
     const void* q_rope;
     long long qr_token, qr_head;
     void* q_abs;                // [num_tokens * H][R + P] absorbed query rows

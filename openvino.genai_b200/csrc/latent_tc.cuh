@@ -23,13 +23,32 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(pa::smem_u32(bar))
                  : "memory");
 }
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+// Loads of what is read once or twice in short order: its lines are the first to leave the L2 cache, so that a long cache that streams through
+// does not take weights, scratch and the kernels' own code with it.
+__device__ __forceinline__ uint64_t evict_first() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(
                      pa::smem_u32(dst)),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(pa::smem_u32(bar))
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(pa::smem_u32(bar)), "l"(policy)
                  : "memory");
 }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(
+                     pa::smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(pa::smem_u32(bar)), "l"(policy)
+                 : "memory");
+}
+// The same boxes into the L2 cache only.
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int x, int y, int z, uint64_t policy) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile.L2::cache_hint [%0, {%1, %2, %3}], %4;" ::"l"(map), "r"(x), "r"(y), "r"(z), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void prefetch_4d(const CUtensorMap* map, int x, int y, int z, int w, uint64_t policy) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile.L2::cache_hint [%0, {%1, %2, %3, %4}], %5;" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy) : "memory");
+}
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pa::smem_u32(bar)) : "memory");
@@ -65,6 +84,17 @@ struct Waiter {
         return give_up();
     }
     __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) const { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; }
+    // The same without the suspension: for the warps that hand the tensor core its work, whose every wait is on everybody's way (the attention of
+    // 1100 - 2048 new tokens by 32 heads 431 -> 357 us).
+    __device__ __forceinline__ bool spin_warp(uint64_t* bar, uint32_t parity) const {
+        bool ok = false;
+        for (uint32_t i = 0; i < (1u << 26); ++i) {
+            if (mbar_test(bar, parity)) { ok = true; break; }
+            if ((i & 1023u) == 1023u && *abort) break;
+        }
+        if (__all_sync(0xffffffffu, ok)) return true;
+        return give_up();
+    }
 };
 
 // Operand descriptors of 128-byte-swizzled tiles whose 8-row groups are GROUP bytes apart.  Their high words are constants, so only the low
