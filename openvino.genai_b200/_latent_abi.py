@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 PA_LATENT_AUTO = 0
 PA_LATENT_ABSORBED = 1
@@ -72,11 +73,24 @@ class pa_latent_attention_args(C.Structure):
     ]
 
 
+_FORMAT = {C.c_uint32: "I", C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "P"}
+
+
+def packer(args) -> struct.Struct:
+    """Writes all fields of an argument struct at once: filling a ctypes structure costs several times as much, which single rows notice."""
+    p = struct.Struct("@" + "".join(_FORMAT[kind] for _, kind in args._fields_))
+    assert p.size == C.sizeof(args)
+    return p
+
+
+APPEND_ARGS = packer(pa_latent_append_args)
+ATTENTION_ARGS = packer(pa_latent_attention_args)
+
 LATENT_SYMBOLS = {
     "pa_b200_latent_create": (C.c_int, [C.POINTER(pa_latent_desc), C.c_int, C.POINTER(C.c_void_p)]),
     "pa_b200_latent_destroy": (C.c_int, [C.c_void_p]),
-    "pa_b200_latent_append": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_append_args)]),
-    "pa_b200_latent_attention": (C.c_int, [C.c_void_p, C.POINTER(pa_latent_attention_args)]),
+    "pa_b200_latent_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "pa_b200_latent_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
     "pa_b200_latent_reserve": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "pa_b200_latent_last_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
     "pa_b200_latent_launch_count": (C.c_int64, [C.c_void_p]),

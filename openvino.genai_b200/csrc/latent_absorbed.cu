@@ -116,12 +116,13 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
     __shared__ int abort_flag;
     const Step& m = a.m;
     if (blockIdx.x == 0) {
+        pa::grid_wait();
+        pa::grid_release();
         build_plan(a);
         return;
     }
     const int parts = m.R / 128, tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     const int i = blockIdx.x - 1, part = i % parts, h = i / parts % m.H, t0 = i / parts / m.H * kTile;
-    if (!tile_rows(a, t0, live)) return;
     uint8_t* const sw = smem;                        // two atoms of [Dn][64 latent elements]
     uint8_t* const sq = smem + 2 * m.Dn * 128;       // Dn / 64 atoms of [64 tokens][64 elements]
     if (tid == 0) {
@@ -129,18 +130,23 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
         pa::mbar_init(&done, 1);
         pa::mbar_fence_init();
         abort_flag = 0;
+        for (int c = 0; c < 2; ++c) prefetch_3d(&a.map_key_up, part * 128 + c * 64, 0, h);
+    }
+    if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
+    pa::grid_wait();
+    pa::grid_release();
+    if (tid == 0) {
         pa::mbar_expect_tx(&full, 2 * m.Dn * 128 + m.Dn / 64 * 8192);
         for (int c = 0; c < 2; ++c) tma_3d(sw + c * m.Dn * 128, &a.map_key_up, part * 128 + c * 64, 0, h, &full);
         for (int c = 0; c < m.Dn / 64; ++c) tma_3d(sq + c * 8192, &a.map_qn, c * 64, h, t0, &full);
     }
-    if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
     tc05::fence_before_thread_sync();
-    __syncthreads();
+    const bool any = tile_rows(a, t0, live);
     tc05::fence_after_thread_sync();
     const Waiter wt{&abort_flag, m.status};
     const uint32_t tmem = tmem_base;
     bool ok = wt.wait(&full, 0);
-    if (warp == 0 && __all_sync(0xffffffffu, ok)) {
+    if (any && warp == 0 && __all_sync(0xffffffffu, ok)) {
         constexpr uint32_t idesc = tc05::instr_desc_f16(128, kTile, BF ? 1 : 0, 1, 0);
         const uint32_t da = desc_low(sw, m.Dn * 128), db = desc_low(sq);
         if (tc05::elect_one()) {
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
             tc05::commit(&done);
         }
     }
-    if (part == 0) {   // the rotated part goes along as it is
+    if (any && part == 0) {   // the rotated part goes along as it is
         const int pieces = m.P / 8;
         for (int u = tid; u < kTile * pieces; u += 128) {
             const int t = t0 + u / pieces, c = u % pieces;
@@ -162,7 +168,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
                     *reinterpret_cast<const uint4*>((const uint16_t*)a.q_rope + t * a.qr_token + h * a.qr_head + 8 * c);
         }
     }
-    ok = ok && wt.wait(&done, 0);
+    ok = any && ok && wt.wait(&done, 0);
     tc05::fence_after_thread_sync();
     if (__all_sync(0xffffffffu, ok)) {
         uint16_t* dst = (uint16_t*)a.q_abs + ((long long)t0 * m.H + h) * (m.R + m.P) + part * 128 + tid;
@@ -265,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         sm.abort_flag = 0;
     }
     if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
+    pa::grid_wait();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -665,6 +672,8 @@ constexpr int kCombineRows = 8, kCombineThreads = 512;
 template <int R, bool BF>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
     constexpr int kPer = R / 4;                    // threads of a row, four latent elements each
+    pa::grid_wait();
+    pa::grid_release();
     extern __shared__ float weight[];              // [kCombineRows][pieces]
     const int part = blockIdx.x % (kTile / kCombineRows);
     const Cut cut = a.cuts[blockIdx.x / (kTile / kCombineRows)];
@@ -723,21 +732,24 @@ __global__ void __launch_bounds__(160) project_value_kernel(const __grid_constan
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * kTile, chunks = m.R / 64;
-    if (!tile_rows(a, t0, live)) return;
     const int w_bytes = m.Dv * 128, stage = w_bytes + 2 * 8192;
     if (tid == 0) {
         for (int i = 0; i < kValueStages; ++i) { pa::mbar_init(&full[i], 1); pa::mbar_init(&free_[i], 1); }
         pa::mbar_init(&done, 1);
         pa::mbar_fence_init();
         abort_flag = 0;
+        for (int c = 0; c < chunks; ++c) prefetch_3d(&a.map_value_up, c * 64, 0, h);
     }
     if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
+    pa::grid_wait();
     tc05::fence_before_thread_sync();
-    __syncthreads();
+    const bool any = tile_rows(a, t0, live);
     tc05::fence_after_thread_sync();
     const uint32_t tmem = tmem_base;
     const Waiter wt{&abort_flag, m.status};
-    if (warp == 4) {
+    if (!any) {
+        // (nothing to do for these tokens)
+    } else if (warp == 4) {
         bool ok = true;
         const uint32_t idesc = tc05::instr_desc_f16(m.Dv, kTile, BF ? 1 : 0, 0, 0);
         auto load = [&](int c) {
@@ -797,22 +809,28 @@ __global__ void __launch_bounds__(160) project_value_kernel(const __grid_constan
     if (warp == 0) tc05::tmem_dealloc(tmem, 64);
 }
 
+int query_smem(const Step& m) { return 2 * m.Dn * 128 + m.Dn / 64 * 8192; }
+int value_smem(const Step& m) { return kValueStages * (m.Dv * 128 + 2 * 8192); }
+
 template <int R, bool BF>
 cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     const Step& m = a.m;
     const int token_tiles = (m.num_tokens + kTile - 1) / kTile;
-    const int smem_q = 2 * m.Dn * 128 + m.Dn / 64 * 8192, smem_v = kValueStages * (m.Dv * 128 + 2 * 8192);
-    const int smem_a = sizeof(AttendSmem<R>);
-    cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_a);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
-    if (e != cudaSuccess) return e;
-    project_query_kernel<BF><<<1 + token_tiles * m.H * (R / 128), 128, smem_q, stream>>>(a);
-    attend_kernel<R, BF><<<a.groups * a.row_tiles, kThreads, smem_a, stream>>>(a);
-    combine_kernel<R, BF><<<a.groups * a.row_tiles * (kTile / kCombineRows), kCombineThreads, kCombineRows * a.groups * sizeof(float), stream>>>(a);
-    project_value_kernel<BF><<<token_tiles * m.H, 160, smem_v, stream>>>(a);
+    cudaError_t e = pa::launch_dependent(project_query_kernel<BF>, 1 + token_tiles * m.H * (R / 128), 128, query_smem(m), stream, a);
+    if (e == cudaSuccess) e = pa::launch_dependent(attend_kernel<R, BF>, a.groups * a.row_tiles, kThreads, sizeof(AttendSmem<R>), stream, a);
+    if (e == cudaSuccess)
+        e = pa::launch_dependent(combine_kernel<R, BF>, a.groups * a.row_tiles * (kTile / kCombineRows), kCombineThreads, kCombineRows * a.groups * sizeof(float), stream, a);
+    if (e == cudaSuccess) e = pa::launch_dependent(project_value_kernel<BF>, token_tiles * m.H, 160, value_smem(m), stream, a);
     *launches += 4;
-    return cudaGetLastError();
+    return e;
+}
+
+template <int R, bool BF>
+cudaError_t prepare(const Step& m) {
+    cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, query_smem(m));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(AttendSmem<R>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, value_smem(m));
+    return e;
 }
 
 }  // namespace
@@ -827,6 +845,11 @@ long long absorbed_slots(int tokens, int sequences, int heads, int groups, int r
 cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t stream, int* launches) {
     if (dtype == PA_DTYPE_BF16) return a.m.R == 512 ? launch<512, true>(a, stream, launches) : launch<256, true>(a, stream, launches);
     return a.m.R == 512 ? launch<512, false>(a, stream, launches) : launch<256, false>(a, stream, launches);
+}
+
+cudaError_t prepare_absorbed(const Step& m, int dtype) {
+    if (dtype == PA_DTYPE_BF16) return m.R == 512 ? prepare<512, true>(m) : prepare<256, true>(m);
+    return m.R == 512 ? prepare<512, false>(m) : prepare<256, false>(m);
 }
 
 }  // namespace latent

@@ -355,6 +355,10 @@ int pa_b200_latent_create(const pa_latent_desc* desc, int device, pa_latent_hand
         cudaError_t e = cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking);
         if (e == cudaSuccess) e = cudaMalloc((void**)&h->status, 256);
         if (e == cudaSuccess) e = cudaMemset(h->status, 0, 256);
+        latent::Step sizes{};
+        sizes.H = desc->num_heads; sizes.R = desc->latent_size; sizes.P = desc->rope_size; sizes.Dn = desc->nope_size; sizes.Dv = desc->value_size;
+        if (e == cudaSuccess) e = latent::prepare_absorbed(sizes, desc->dtype);
+        if (e == cudaSuccess) e = latent::prepare_expanded(sizes, desc->dtype);
         if (e != cudaSuccess) {
             pa_b200_latent_destroy(h);
             return fail_cuda("pa_b200_latent_create", e);

@@ -66,6 +66,8 @@ __device__ __forceinline__ void rotate16(const uint16_t* src, uint16_t* dst, con
 // A warp takes a token's latent row, or 32 pieces (sixteen elements each) of its heads' query rows.
 template <bool BF>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+    pa::grid_wait();
+    pa::grid_release();
     const Step& m = a.m;
     const int lane = threadIdx.x & 31;
     const int pieces = m.P / 16;                                            // lanes of one row's rotation
@@ -131,10 +133,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
 cudaError_t launch_append(const AppendArgs& a, int dtype, cudaStream_t stream, int* launches) {
     const long long warps = (long long)a.m.num_tokens * (1 + (a.q_in ? (a.m.H * (a.m.P / 16) + 31) / 32 : 0));
     const unsigned blocks = (unsigned)((warps + 7) / 8);
-    if (dtype == PA_DTYPE_BF16) append_kernel<true><<<blocks, 256, 0, stream>>>(a);
-    else append_kernel<false><<<blocks, 256, 0, stream>>>(a);
     ++*launches;
-    return cudaGetLastError();
+    return pa::launch_dependent(dtype == PA_DTYPE_BF16 ? append_kernel<true> : append_kernel<false>, blocks, 256, 0, stream, a);
 }
 
 }  // namespace latent

@@ -18,6 +18,8 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
     __shared__ int bucket[kBuckets];
     const Step& m = a.m;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = m.num_sequences;
+    pa::grid_wait();
+    pa::grid_release();
     if (tid == 0) { run_c = 0; run_q = 0; }
     for (int i = tid; i < a.passes; i += 256) a.counter[i] = 0;
     for (int i = tid; i < kBuckets; i += 256) bucket[i] = 0;
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
         sm.abort_flag = 0;
     }
     if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
+    pa::grid_wait();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -375,6 +378,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
         sm.abort_flag = 0;
     }
     if (warp == 9) tc05::tmem_alloc(&sm.tmem_base, 512);
+    pa::grid_wait();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -681,29 +685,23 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
     if (warp == 9) tc05::tmem_dealloc(tmem, 512);
 }
 
-template <int DN, int DV, bool BF>
-cudaError_t attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream) {
-    const int smem = sizeof(ExpandedSmem<DN, DV>);
-    // the warpgroups re-divide the registers that the CTA was launched with: fewer than this would leave one of them waiting
-    static const int regs = [] {
-        cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, expanded_attend_kernel<DN, DV, BF>) == cudaSuccess ? f.numRegs : 0;
-    }();
-    if (regs * kAttendThreads < 256 * kSoftmaxRegs + 128 * kOtherRegs) return cudaErrorInvalidConfiguration;
-    const cudaError_t e = cudaFuncSetAttribute(expanded_attend_kernel<DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    expanded_attend_kernel<DN, DV, BF><<<sm_count, kAttendThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+template <int R, int DN, int DV, bool BF>
+cudaError_t expand_and_attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
+    cudaError_t e = pa::launch_dependent(expand_kernel<R, DN, DV, BF>, sm_count, kExpandThreads, sizeof(ExpandSmem<R>), stream, a);
+    if (e == cudaSuccess) e = pa::launch_dependent(expanded_attend_kernel<DN, DV, BF>, sm_count, kAttendThreads, sizeof(ExpandedSmem<DN, DV>), stream, a);
+    *launches += 2;
+    return e;
 }
 
 template <int R, int DN, int DV, bool BF>
-cudaError_t expand_and_attend(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int* launches) {
-    const int smem = sizeof(ExpandSmem<R>);
-    const cudaError_t e = cudaFuncSetAttribute(expand_kernel<R, DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    expand_kernel<R, DN, DV, BF><<<sm_count, kExpandThreads, smem, stream>>>(a);
-    *launches += 2;
-    return attend<DN, DV, BF>(a, sm_count, stream);
+cudaError_t prepare() {
+    // the warpgroups re-divide the registers that the CTA was launched with: fewer than this would leave one of them waiting
+    cudaFuncAttributes f;
+    cudaError_t e = cudaFuncGetAttributes(&f, expanded_attend_kernel<DN, DV, BF>);
+    if (e == cudaSuccess && f.numRegs * kAttendThreads < 256 * kSoftmaxRegs + 128 * kOtherRegs) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(expand_kernel<R, DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ExpandSmem<R>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(expanded_attend_kernel<DN, DV, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ExpandedSmem<DN, DV>));
+    return e;
 }
 
 template <int R, bool BF>
@@ -713,17 +711,27 @@ cudaError_t launch(const ExpandedArgs& a, int sm_count, cudaStream_t stream, int
     return a.m.Dv == 128 ? expand_and_attend<R, 64, 128, BF>(a, sm_count, stream, launches) : expand_and_attend<R, 64, 64, BF>(a, sm_count, stream, launches);
 }
 
+template <int R, bool BF>
+cudaError_t prepare(const Step& m) {
+    if (m.Dn == 128) return m.Dv == 128 ? prepare<R, 128, 128, BF>() : prepare<R, 128, 64, BF>();
+    return m.Dv == 128 ? prepare<R, 64, 128, BF>() : prepare<R, 64, 64, BF>();
+}
+
 }  // namespace
 
 cudaError_t launch_expanded_plan(const ExpandedArgs& a, cudaStream_t stream, int* launches) {
-    expanded_plan_kernel<<<1, 256, 0, stream>>>(a);
     ++*launches;
-    return cudaGetLastError();
+    return pa::launch_dependent(expanded_plan_kernel, 1, 256, 0, stream, a);
 }
 
 cudaError_t launch_expanded(const ExpandedArgs& a, int dtype, int sm_count, cudaStream_t stream, int* launches) {
     if (dtype == PA_DTYPE_BF16) return a.m.R == 512 ? launch<512, true>(a, sm_count, stream, launches) : launch<256, true>(a, sm_count, stream, launches);
     return a.m.R == 512 ? launch<512, false>(a, sm_count, stream, launches) : launch<256, false>(a, sm_count, stream, launches);
+}
+
+cudaError_t prepare_expanded(const Step& m, int dtype) {
+    if (dtype == PA_DTYPE_BF16) return m.R == 512 ? prepare<512, true>(m) : prepare<256, true>(m);
+    return m.R == 512 ? prepare<512, false>(m) : prepare<256, false>(m);
 }
 
 }  // namespace latent

@@ -110,6 +110,10 @@ struct ExpandedArgs {
 cudaError_t launch_expanded_plan(const ExpandedArgs& a, cudaStream_t stream, int* launches);
 cudaError_t launch_expanded(const ExpandedArgs& a, int dtype, int sm_count, cudaStream_t stream, int* launches);
 
+// What a kernel's launches need once on every device.
+cudaError_t prepare_absorbed(const Step& m, int dtype);
+cudaError_t prepare_expanded(const Step& m, int dtype);
+
 cudaError_t launch_append(const AppendArgs& a, int dtype, cudaStream_t stream, int* launches);
 
 #ifdef __CUDACC__

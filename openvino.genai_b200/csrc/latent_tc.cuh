@@ -43,6 +43,9 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
                  : "memory");
 }
 // The same boxes into the L2 cache only.
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
+}
 __device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int x, int y, int z, uint64_t policy) {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile.L2::cache_hint [%0, {%1, %2, %3}], %4;" ::"l"(map), "r"(x), "r"(y), "r"(z), "l"(policy) : "memory");
 }

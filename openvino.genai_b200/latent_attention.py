@@ -17,7 +17,6 @@ from . import _abi, _latent_abi as A
 
 _DTYPES = {torch.float16: _abi.PA_DTYPE_F16, torch.bfloat16: _abi.PA_DTYPE_BF16}
 _FORMS = {"auto": A.PA_LATENT_AUTO, "absorbed": A.PA_LATENT_ABSORBED, "expanded": A.PA_LATENT_EXPANDED}
-_METADATA = ("past_lens", "subsequence_begins", "block_indices", "block_indices_begins")
 
 
 class LatentAttention:
@@ -34,6 +33,13 @@ class LatentAttention:
         self.num_heads, self.latent_size, self.rope_size = num_heads, latent_size, rope_size
         self.nope_size, self.value_size, self.block_size = nope_size, value_size, block_size
         self.dtype, self.device = dtype, torch.device("cuda", device)
+        row = latent_size + rope_size
+        self._ordinal = device
+        self._row_shape, self._block_shape, self._output_shape = (row,), (block_size, row), (num_heads * value_size,)
+        self._nope_shape, self._rope_shape = (num_heads, nope_size), (num_heads, rope_size)
+        self._key_shape, self._value_shape = (nope_size, latent_size), (value_size, latent_size)
+        self._args = C.create_string_buffer(max(A.APPEND_ARGS.size, A.ATTENTION_ARGS.size))
+        self._append, self._attend = self.lib.pa_b200_latent_append, self.lib.pa_b200_latent_attention
         desc = A.pa_latent_desc(C.sizeof(A.pa_latent_desc), num_heads, latent_size, rope_size, nope_size, value_size, block_size, _DTYPES[dtype])
         self._check(self.lib.pa_b200_latent_create(C.byref(desc), device, C.byref(self._h)))
 
@@ -52,55 +58,75 @@ class LatentAttention:
         return torch.zeros((num_blocks, self.block_size, self.latent_size + self.rope_size), dtype=self.dtype, device=self.device)
 
     # ---- checks --------------------------------------------------------------------------------
-    def _tensor(self, name: str, t, dtype: torch.dtype, shape: tuple, contiguous: bool = False) -> torch.Tensor:
-        """`t` if it is a device tensor of this type and shape (None: any size) whose last dimension, or all of it, is contiguous."""
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self.device or t.dim() != len(shape) or \
-                any(want is not None and want != have for want, have in zip(shape, t.shape)):
-            what = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-            raise self._err(f"{name}: expected {dtype} {shape} on {self.device}, got {what}")
-        if not (t.is_contiguous() if contiguous else t.stride(-1) == 1 or t.shape[-1] == 1):
-            raise self._err(f"{name}: strides {t.stride()} are not supported")
-        return t
+    # (they run before every launch: a small step's time is the host's)
+    def _refuse(self, name: str, t, expected: str):
+        what = f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise self._err(f"{name}: expected {expected} on {self.device}, got {what}")
 
-    def _metadata(self, a, inputs: dict) -> None:
-        past, begins, blocks, block_begins = (self._tensor(n, inputs[n], torch.int32, (None,), True) for n in _METADATA)
-        a.num_sequences, a.num_block_indices = past.shape[0], blocks.shape[0]
-        if begins.shape[0] != a.num_sequences + 1 or block_begins.shape[0] != a.num_sequences + 1:
+    def _rows(self, name: str, t, shape: tuple):
+        """The strides of a device tensor of the operator's type whose dimensions behind the first are `shape` and whose last is contiguous."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not self.dtype or t.device != self.device or t.shape[1:] != shape:
+            self._refuse(name, t, f"{self.dtype} [rows, {', '.join(map(str, shape))}]")
+        strides = t.stride()
+        if strides[-1] != 1:
+            self._refuse(name, t, "a contiguous last dimension")
+        return strides
+
+    def _whole(self, name: str, t, dtype: torch.dtype, shape: tuple) -> int:
+        """The address of a contiguous device tensor of this type whose dimensions behind the first are `shape`."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != self.device or t.dim() == 0 or t.shape[1:] != shape or not t.is_contiguous():
+            self._refuse(name, t, f"contiguous {dtype} [rows{''.join(', ' + str(n) for n in shape)}]")
+        return t.data_ptr()
+
+    def _step(self, inputs: dict) -> tuple:
+        """cache, num_blocks, the paged metadata and its sizes, in the order of the argument structs."""
+        past, begins, blocks, block_begins, cache = inputs["past_lens"], inputs["subsequence_begins"], inputs["block_indices"], \
+            inputs["block_indices_begins"], inputs["cache"]
+        whole, i32 = self._whole, torch.int32
+        addresses = (whole("past_lens", past, i32, ()), whole("subsequence_begins", begins, i32, ()), whole("block_indices", blocks, i32, ()),
+                     whole("block_indices_begins", block_begins, i32, ()))
+        sequences = past.shape[0]
+        if begins.shape[0] != sequences + 1 or block_begins.shape[0] != sequences + 1:
             raise self._err("subsequence_begins and block_indices_begins need num_sequences + 1 entries")
-        a.past_lens, a.subsequence_begins, a.block_indices, a.block_indices_begins = (t.data_ptr() for t in (past, begins, blocks, block_begins))
-        cache = self._tensor("cache", inputs["cache"], self.dtype, (None, self.block_size, self.latent_size + self.rope_size), True)
-        a.cache, a.num_blocks = cache.data_ptr(), cache.shape[0]
+        return (whole("cache", cache, self.dtype, self._block_shape), cache.shape[0], *addresses, sequences, blocks.shape[0])
+
+    def _stream(self, inputs: dict) -> int:
         # 1 = cudaStreamLegacy: a null handle would select the operator's own stream
-        a.stream = inputs.get("stream") or torch.cuda.current_stream(self.device).cuda_stream or 1
+        return inputs.get("stream") or torch._C._cuda_getCurrentRawStream(self._ordinal) or 1
 
     # ---- the operators -------------------------------------------------------------------------
     def append(self, inputs: dict, outputs: Optional[dict] = None) -> None:
         """inputs: latent [T, latent + rope], norm_weight [latent] (optional) with norm_eps, rope_table f32 [rows, rope] (cos | sin),
         interleaved (default False), positions i32 [T] (optional), query_rope [T, heads, rope] (optional), cache and the paged
         metadata.  outputs: query_rope, which may be the input itself; the cache is written in place."""
-        a = A.pa_latent_append_args()
-        a.struct_size = C.sizeof(A.pa_latent_append_args)
-        latent = self._tensor("latent", inputs["latent"], self.dtype, (None, self.latent_size + self.rope_size))
+        latent, weight, query, table = inputs["latent"], inputs.get("norm_weight"), inputs.get("query_rope"), inputs["rope_table"]
+        latent_stride = self._rows("latent", latent, self._row_shape)[0]
         tokens = latent.shape[0]
-        a.latent, a.latent_stride, a.num_tokens = latent.data_ptr(), latent.stride(0), tokens
-        weight = inputs.get("norm_weight")
+        norm = eps = 0
         if weight is not None:
-            a.norm_weight = self._tensor("norm_weight", weight, self.dtype, (self.latent_size,)).data_ptr()
-            a.norm_eps = inputs["norm_eps"]
-        query = inputs.get("query_rope")
+            norm, eps = self._whole("norm_weight", weight, self.dtype, ()), inputs["norm_eps"]
+            if weight.shape[0] != self.latent_size:
+                self._refuse("norm_weight", weight, f"[{self.latent_size}]")
+        query_address = out_address = 0
+        q = o = (0, 0)
         if query is not None:
-            query = self._tensor("query_rope", query, self.dtype, (tokens, self.num_heads, self.rope_size))
-            out = self._tensor("output query_rope", (outputs or {}).get("query_rope"), self.dtype, (tokens, self.num_heads, self.rope_size))
-            a.query_rope, a.query_rope_out = query.data_ptr(), out.data_ptr()
-            a.query_rope_token_stride, a.query_rope_head_stride, _ = query.stride()
-            a.query_rope_out_token_stride, a.query_rope_out_head_stride, _ = out.stride()
-        table = self._tensor("rope_table", inputs["rope_table"], torch.float32, (None, self.rope_size), True)
-        a.rope_table, a.rope_table_rows = table.data_ptr(), table.shape[0]
-        a.interleaved = 1 if inputs.get("interleaved") else 0
-        if inputs.get("positions") is not None:
-            a.positions = self._tensor("positions", inputs["positions"], torch.int32, (tokens,), True).data_ptr()
-        self._metadata(a, inputs)
-        self._check(self.lib.pa_b200_latent_append(self._h, C.byref(a)))
+            out = (outputs or {}).get("query_rope")
+            q, o = self._rows("query_rope", query, self._rope_shape), self._rows("output query_rope", out, self._rope_shape)
+            if query.shape[0] != tokens or out.shape[0] != tokens:
+                raise self._err("latent, query_rope and output query_rope need the same number of tokens")
+            query_address, out_address = query.data_ptr(), out.data_ptr()
+        table_address = self._whole("rope_table", table, torch.float32, (self.rope_size,))
+        positions = inputs.get("positions")
+        if positions is not None:
+            if positions.shape != (tokens,):
+                self._refuse("positions", positions, f"[{tokens}]")
+            positions = self._whole("positions", positions, torch.int32, ())
+        A.APPEND_ARGS.pack_into(self._args, 0, A.APPEND_ARGS.size, latent.data_ptr(), latent_stride, norm, eps, query_address, q[0], q[1],
+                                out_address, o[0], o[1], table_address, table.shape[0], 1 if inputs.get("interleaved") else 0, positions or 0, tokens,
+                                *self._step(inputs), self._stream(inputs))
+        rc = self._append(self._h, self._args)
+        if rc:
+            self._check(rc)
 
     def attend(self, inputs: dict, outputs: dict, form: str = "auto") -> None:
         """inputs: query_nope [T, heads, nope], query_rope [T, heads, rope] (rotated), key_up [heads, nope, latent],
@@ -108,26 +134,22 @@ class LatentAttention:
         outputs: output [T, heads * value].  form: "absorbed", "expanded", or "auto" (each sequence in the one that suits it)."""
         if form not in _FORMS:
             raise self._err(f"unknown form {form!r}: one of {', '.join(_FORMS)}")
-        a = A.pa_latent_attention_args()
-        a.struct_size = C.sizeof(A.pa_latent_attention_args)
-        a.form = _FORMS[form]
-        nope = self._tensor("query_nope", inputs["query_nope"], self.dtype, (None, self.num_heads, self.nope_size))
+        nope, rope, key_up, value_up, output = inputs["query_nope"], inputs["query_rope"], inputs["key_up"], inputs["value_up"], outputs["output"]
+        n, r = self._rows("query_nope", nope, self._nope_shape), self._rows("query_rope", rope, self._rope_shape)
+        k, v = self._rows("key_up", key_up, self._key_shape), self._rows("value_up", value_up, self._value_shape)
+        out = self._whole("output", output, self.dtype, self._output_shape)
         tokens = nope.shape[0]
-        rope = self._tensor("query_rope", inputs["query_rope"], self.dtype, (tokens, self.num_heads, self.rope_size))
-        key_up = self._tensor("key_up", inputs["key_up"], self.dtype, (self.num_heads, self.nope_size, self.latent_size))
-        value_up = self._tensor("value_up", inputs["value_up"], self.dtype, (self.num_heads, self.value_size, self.latent_size))
-        for name, t in (("key_up", key_up), ("value_up", value_up)):
-            if t.stride(1) != self.latent_size:
-                raise self._err(f"{name}: a head's rows have to be contiguous")
-        out = self._tensor("output", outputs["output"], self.dtype, (tokens, self.num_heads * self.value_size), True)
-        a.num_tokens, a.output = tokens, out.data_ptr()
-        a.query_nope, a.query_rope, a.key_up, a.value_up = nope.data_ptr(), rope.data_ptr(), key_up.data_ptr(), value_up.data_ptr()
-        a.query_nope_token_stride, a.query_nope_head_stride, _ = nope.stride()
-        a.query_rope_token_stride, a.query_rope_head_stride, _ = rope.stride()
-        a.key_up_head_stride, a.value_up_head_stride = key_up.stride(0), value_up.stride(0)
-        a.scale = inputs.get("scale") or 0.0
-        self._metadata(a, inputs)
-        self._check(self.lib.pa_b200_latent_attention(self._h, C.byref(a)))
+        if rope.shape[0] != tokens or output.shape[0] != tokens:
+            raise self._err("query_nope, query_rope and output need the same number of tokens")
+        if key_up.shape[0] != self.num_heads or value_up.shape[0] != self.num_heads:
+            raise self._err(f"key_up and value_up need {self.num_heads} heads")
+        if k[1] != self.latent_size or v[1] != self.latent_size:
+            raise self._err("key_up and value_up: a head's rows have to be contiguous")
+        A.ATTENTION_ARGS.pack_into(self._args, 0, A.ATTENTION_ARGS.size, nope.data_ptr(), n[0], n[1], rope.data_ptr(), r[0], r[1], key_up.data_ptr(), k[0],
+                                   value_up.data_ptr(), v[0], out, tokens, *self._step(inputs), inputs.get("scale") or 0.0, _FORMS[form], self._stream(inputs))
+        rc = self._attend(self._h, self._args)
+        if rc:
+            self._check(rc)
 
     def reserve(self, num_tokens: int, num_sequences: int, num_block_indices: int, form: str = "auto") -> None:
         """Grows the scratch for steps of up to this size, so that `attend` does not allocate (stream captures need that)."""
