@@ -2,8 +2,7 @@
 // (q~ = key_up^T q), attend over the paged latents as they lie in the cache, and the sums of latents go through value_up.
 //   project_query   q~ per head, and the plan of the attention (first CTA)
 //   attend          split over the context: every CTA an equal slice of all (row tile, context tile) units
-//   combine         joins the partial results of a row
-//   project_value   output per head
+//   project_value   joins the partial results of the rows, output per head
 #include <algorithm>
 
 #include "latent_tc.cuh"
@@ -56,12 +55,11 @@ __device__ void build_plan(const AbsorbedArgs& a) {
     }
     if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; }
     __syncthreads();
-    // where every slice begins, so that a CTA of the attention has one record to read instead of a search, and what it cuts
+    // where every slice begins, so that a CTA of the attention has one record to read instead of a search
     const long long total = run_u, per = total > 0 ? (total + a.groups - 1) / a.groups : 1;
     for (int w = tid; w < a.groups; w += 128) {
         const long long u = w * per;
         SliceStart st{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        Cut cut{0, 0, 0, 0};
         if (u < total) {
             int lo = 0, hi = B;              // unit_prefix[lo] <= u < unit_prefix[hi]
             while (hi - lo > 1) {
@@ -72,31 +70,18 @@ __device__ void build_plan(const AbsorbedArgs& a) {
             seq_view(a.m, lo, v);
             const SeqPlan p = seq_plan(a, lo);
             const long long rel = u - a.unit_prefix[lo];
-            st = SliceStart{lo, (int)(rel / p.tiles), (int)(rel % p.tiles), (int)min(per, total - u), v.t0, v.n, v.past, v.tb, p.blocks, (int)p.tiles, a.block_prefix[lo], 0};
-            const long long u0 = u - st.first;
-            if (st.first > 0 && u0 / per + 1 == w) {      // the first slice to begin inside this block: its partial results are joined afterwards
-                const int row0 = st.block * a.row_tiles * kTile;
-                cut.rows = (int)min((long long)kTile * a.row_tiles, (long long)v.n * a.m.H - row0);
-                cut.grow0 = (int)((long long)v.t0 * a.m.H + row0);
-                cut.slot = (int)(((long long)st.block0 + st.block + u0 / per) * a.row_tiles);
-                cut.pieces = (int)((u0 + p.tiles - 1) / per - u0 / per) + 1;
-            }
+            st = SliceStart{lo, (int)(rel / p.tiles), (int)(rel % p.tiles), (int)min(per, total - u), v.t0, v.n, v.past, v.tb, p.blocks, (int)p.tiles, a.block_prefix[lo],
+                            (int)per};
         }
         a.starts[w] = st;
-        for (int member = 0; member < a.row_tiles; ++member) {
-            Cut c = cut;
-            c.rows = max(0, min(kTile, cut.rows - member * kTile));
-            c.grow0 += member * kTile;
-            c.slot += member;
-            a.cuts[w * a.row_tiles + member] = c;
-        }
     }
 }
 
 // Which of the tile's tokens belong to sequences of this form; false (for the whole block) if none does.
-__device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&live)[kTile]) {
+template <int NT>
+__device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&live)[NT]) {
     bool mine = false;
-    if (threadIdx.x < kTile) {
+    if (threadIdx.x < NT) {
         SeqView v;
         mine = t0 + (int)threadIdx.x < a.m.num_tokens && token_view(a.m, t0 + threadIdx.x, v) && v.n <= a.max_new;
         live[threadIdx.x] = mine;
@@ -213,8 +198,8 @@ struct Run {
     int first, tiles;    // context tiles
     int end;             // context the tile's last row sees
     int tb;
-    bool whole;          // all of the row tile's context: no other CTA has a part of it
-    long long slot;
+    int slot;            // of the partial result
+    int pieces;          // partial results of the row tile, if this is the first, else 0
 };
 
 template <int R>
@@ -229,7 +214,7 @@ struct AttendSmem {
     alignas(1024) Tile k[NST];
     alignas(1024) uint8_t p[kTile * 128];           // [row][token]
     float alpha[2][kTile];
-    float stat[2][kTile][3];                        // maximum, sum and its reciprocal of the rows of a run
+    float2 stat[2][kTile];                          // maximum and sum of the rows of a run
     volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
     volatile int event;                             // what the results warps are asked for: rescale after tile `event` - 1, or results (0)
     uint64_t k_full[NST][2], k_free[NST][2];        // halves of tiles: loader -> products (bytes), products -> loader
@@ -326,8 +311,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 r.first = first;
                 r.tiles = max(0, min(first + len, (r.end + kTokens - 1) / kTokens) - first);
                 r.tb = v.tb;
-                r.whole = len == tiles;
-                r.slot = ((long long)block0 + block + group) * a.row_tiles + member;
+                r.slot = (block0 + block + group) * a.row_tiles + member;
+                // the block's units run on through the slices behind this one
+                r.pieces = first > 0 ? 0 : 1 + max(0, tiles - left + start.per - 1) / start.per;
                 ok = publish(r);
                 if (ok && r.tiles > 0) {
                     if (nq > 0) ok = wt.wait_warp(&sm.q_free, (nq - 1) & 1);
@@ -521,14 +507,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             }
             if (!ok) break;
             n += r.tiles;
+            if (r.pieces > 0 && e < r.rows) a.row_part[r.grow0 + e] = make_int2(r.slot * kTile + e, r.pieces);
             if (r.tiles == 0) {
-                if (e < r.rows) a.part_ml[r.slot * kTile + e] = make_float2(-INFINITY, 0.f);
+                if (e < r.rows) a.part_ml[(long long)r.slot * kTile + e] = make_float2(-INFINITY, 0.f);
                 continue;
             }
             if (!wt.wait_warp(&sm.stat_full[ns & 1], (ns >> 1) & 1)) break;
-            const float (*stat)[3] = sm.stat[ns & 1];
+            const float2* stat = sm.stat[ns & 1];
             ++ns;
-            if (!r.whole && e < r.rows) a.part_ml[r.slot * kTile + e] = make_float2(stat[e][0], stat[e][1]);
+            if (e < r.rows) a.part_ml[(long long)r.slot * kTile + e] = stat[e];
 #pragma unroll 1
             for (int q = 0; q < MT * 2; ++q) {
                 const int c0 = (q & 1) * 32;
@@ -536,26 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 uint32_t o[32];
                 tc05::ld_32x32b_x32(tmem + 32 * q + lanes, o);
                 tc05::wait_ld();
-                if (r.whole) {
-                    // two lanes (neighbouring elements) share two rows: each stores both elements of one
-                    uint16_t* dst = (uint16_t*)a.o_lat + (r.grow0 + c0 + (lane & 1)) * (2 * R) + (q >> 1) * 128 + (e & ~1);
+                float* dst = a.part_o + ((long long)r.slot * kTile + c0) * R + (q >> 1) * 128 + e;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float x0 = __uint_as_float(o[c]) * stat[c0 + c][2], x1 = __uint_as_float(o[c + 1]) * stat[c0 + c + 1][2];
-                        const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x0 : x1, 1);
-                        const float lo = lane & 1 ? other : x0, up = lane & 1 ? x1 : other;
-                        const uint32_t hi = pack2<BF>(lo, up);
-                        if (c0 + c + (lane & 1) < r.rows) {
-                            *reinterpret_cast<uint32_t*>(dst + c * (2 * R)) = hi;
-                            *reinterpret_cast<uint32_t*>(dst + c * (2 * R) + R) = pack2<BF>(lo - unpack1<BF>((uint16_t)hi), up - unpack1<BF>((uint16_t)(hi >> 16)));
-                        }
-                    }
-                } else {
-                    float* dst = a.part_o + (r.slot * kTile + c0) * R + (q >> 1) * 128 + e;
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (c0 + c < r.rows) dst[c * R] = __uint_as_float(o[c]);
-                }
+                for (int c = 0; c < 32; ++c)
+                    if (c0 + c < r.rows) dst[c * R] = __uint_as_float(o[c]);
             }
             tc05::fence_before_thread_sync();
             warp_arrive(&sm.answered);
@@ -651,10 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             for (int x = 0; x < 2; ++x) {
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
                 l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-                if ((lane & 3) == 0) {
-                    float* stat = sm.stat[nst & 1][rl[x]];
-                    stat[0] = mx[x]; stat[1] = l[x]; stat[2] = 1.f / l[x];
-                }
+                if ((lane & 3) == 0) sm.stat[nst & 1][rl[x]] = make_float2(mx[x], l[x]);
             }
             warp_arrive(&sm.stat_full[nst & 1]);
             ++nst;
@@ -664,153 +632,219 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
     if (warp == 5) tc05::tmem_dealloc(tmem, 512);
 }
 
-// ---- joining the partial results of a row ----------------------------------------------------------------------------------
-// A block of rows is cut where a slice begins inside it, so there are fewer cut blocks than slices: eight CTAs per slice, eight rows each, join the
-// block that the slice cuts first.  Leaves sum / denominator as two 16-bit pieces, so that the product with value_up does not see another
-// rounding.
-constexpr int kCombineRows = 8, kCombineThreads = 512;
-template <int R, bool BF>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ AbsorbedArgs a) {
-    constexpr int kPer = R / 4;                    // threads of a row, four latent elements each
-    pa::grid_wait();
-    pa::grid_release();
-    extern __shared__ float weight[];              // [kCombineRows][pieces]
-    const int part = blockIdx.x % (kTile / kCombineRows);
-    const Cut cut = a.cuts[blockIdx.x / (kTile / kCombineRows)];
-    const int rows = min(kCombineRows, cut.rows - part * kCombineRows);
-    if (rows <= 0) return;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    auto at = [&](int i, int row) { return ((long long)cut.slot + (long long)i * a.row_tiles) * kTile + part * kCombineRows + row; };
-    if (warp < rows) {                             // weights of the pieces: a warp per row
-        float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < cut.pieces; i += 32) {
-            const float2 ml = a.part_ml[at(i, warp)];
-            if (ml.y > 0.f) top = fmaxf(top, ml.x);
-        }
-        top = pa::warp_max(top);
-        for (int i = lane; i < cut.pieces; i += 32) {
-            const float2 ml = a.part_ml[at(i, warp)];
-            const float k = ml.y > 0.f ? ex2(ml.x - top) : 0.f;      // (a piece whose tiles the row does not see has no sums)
-            weight[warp * cut.pieces + i] = k;
-            sum += k * ml.y;
-        }
-        sum = pa::warp_sum(sum);
-        for (int i = lane; i < cut.pieces; i += 32) weight[warp * cut.pieces + i] *= __frcp_rn(sum);
-    }
-    __syncthreads();
-    for (int row = tid / kPer; row < rows; row += kCombineThreads / kPer) {
-        const int e = tid % kPer;
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int i = 0; i < cut.pieces; ++i) {
-            const float k = weight[row * cut.pieces + i];
-            const float4 p = k != 0.f ? *reinterpret_cast<const float4*>(a.part_o + at(i, row) * R + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
-            y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w;
-        }
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
-            lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
-        }
-        uint16_t* dst = (uint16_t*)a.o_lat + ((long long)cut.grow0 + part * kCombineRows + row) * (2 * R) + 4 * e;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(dst + R) = make_uint2(lo[0], lo[1]);
-    }
-}
-
 // ---- output = value_up o~ ---------------------------------------------------------------------------------------------------
-// A CTA computes one head's output of 64 tokens: D[value][token], K = R twice (high and low pieces against the same weights).
-constexpr int kValueStages = 4;
-template <bool BF>
-__global__ void __launch_bounds__(160) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
+// A CTA joins the partial results of one head's rows of NT tokens and computes their output: D[value][token], K = R twice, because the joined sums
+// go in as two 16-bit pieces (high and low), so that the product does not see another rounding.  Few tokens take tiles of 16, so
+// that there are CTAs enough to join their rows.
+// Bound by the chain record -> statistics -> partial results -> product -> output for few tokens (one row 8 us behind its predecessor; joining in a
+// kernel of its own took 7 us more, and 38 where 74 CTAs had a part of one row), by the partial results' bytes for many.
+constexpr int kJoinWarps = 16, kJoinThreads = 32 * kJoinWarps;
+constexpr int kValueThreads = kJoinThreads + 32;     // warps 0 - 15: joining, then (0 - 3) output; 16: weights and products
+
+template <int R, int NT>
+struct ValueSmem {
+    static constexpr int NC = R / 64, NW = 4;                    // chunks of 64 latent elements, of which weights are in flight
+    alignas(1024) uint8_t o[2][NC][NT * 128];                    // joined rows, high and low pieces
+    alignas(1024) uint8_t w[NW][128 * 128];
+    uint64_t w_full[NW], w_free[NW], o_full, done;
+    struct Row { int first, pieces; float top, inv, k0, k1; } row[NT];   // first partial row, how many, their maximum, 1 / denominator, weights of the first two
+    bool live[NT];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int R, int NT, bool BF>
+__global__ void __launch_bounds__(kValueThreads) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
+    using Smem = ValueSmem<R, NT>;
+    constexpr int NC = Smem::NC, NW = Smem::NW;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full[kValueStages], free_[kValueStages], done;
-    __shared__ bool live[kTile];
-    __shared__ uint32_t tmem_base;
-    __shared__ int abort_flag;
+    Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
-    const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * kTile, chunks = m.R / 64;
-    const int w_bytes = m.Dv * 128, stage = w_bytes + 2 * 8192;
-    if (tid == 0) {
-        for (int i = 0; i < kValueStages; ++i) { pa::mbar_init(&full[i], 1); pa::mbar_init(&free_[i], 1); }
-        pa::mbar_init(&done, 1);
+    const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * NT;
+    if (tid == kJoinThreads) {
+        for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
+        pa::mbar_init(&sm.o_full, kJoinWarps);
+        pa::mbar_init(&sm.done, 1);
         pa::mbar_fence_init();
-        abort_flag = 0;
-        for (int c = 0; c < chunks; ++c) prefetch_3d(&a.map_value_up, c * 64, 0, h);
+        sm.abort_flag = 0;
+        for (int c = 0; c < NC; ++c) prefetch_3d(&a.map_value_up, c * 64, 0, h);
     }
-    if (warp == 0) tc05::tmem_alloc(&tmem_base, 64);
+    if (warp == kJoinWarps) tc05::tmem_alloc(&sm.tmem_base, 64);
     pa::grid_wait();
     tc05::fence_before_thread_sync();
-    const bool any = tile_rows(a, t0, live);
+    const bool any = tile_rows(a, t0, sm.live);
     tc05::fence_after_thread_sync();
-    const uint32_t tmem = tmem_base;
-    const Waiter wt{&abort_flag, m.status};
+    const uint32_t tmem = sm.tmem_base;
+    const Waiter wt{&sm.abort_flag, m.status};
     if (!any) {
         // (nothing to do for these tokens)
-    } else if (warp == 4) {
+    } else if (warp == kJoinWarps) {
         bool ok = true;
-        const uint32_t idesc = tc05::instr_desc_f16(m.Dv, kTile, BF ? 1 : 0, 0, 0);
+        const uint32_t idesc = tc05::instr_desc_f16(m.Dv, NT, BF ? 1 : 0, 0, 0), dw = desc_low(sm.w), doh = desc_low(sm.o[0]), dol = desc_low(sm.o[1]);
         auto load = [&](int c) {
-            const int st = c % kValueStages;
-            uint8_t* p = smem + st * stage;
-            if (lane == 0) {
-                pa::mbar_expect_tx(&full[st], stage);
-                tma_3d(p, &a.map_value_up, c * 64, 0, h, &full[st]);
-                tma_3d(p + w_bytes, &a.map_o_lat, c * 64, h, t0, &full[st]);
-                tma_3d(p + w_bytes + 8192, &a.map_o_lat, m.R + c * 64, h, t0, &full[st]);
+            if (tc05::elect_one()) {
+                pa::mbar_expect_tx(&sm.w_full[c % NW], m.Dv * 128);
+                tma_3d(sm.w[c % NW], &a.map_value_up, c * 64, 0, h, &sm.w_full[c % NW]);
             }
             __syncwarp();
         };
-        for (int c = 0; c < kValueStages && c < chunks; ++c) load(c);
-        for (int c = 0; ok && c < chunks; ++c) {
-            const int st = c % kValueStages;
-            ok = wt.wait_warp(&full[st], (c / kValueStages) & 1);
+        for (int c = 0; c < NW; ++c) load(c);
+        ok = wt.wait_warp(&sm.o_full, 0);
+        for (int c = 0; ok && c < NC; ++c) {
+            ok = wt.wait_warp(&sm.w_full[c % NW], (c / NW) & 1);
             if (!ok) break;
             tc05::fence_after_thread_sync();
-            const uint32_t da = desc_low(smem + st * stage), db = da + (w_bytes >> 4);
+            const uint32_t da = dw + c % NW * (128 * 128 >> 4), dh = doh + c * (NT * 128 >> 4), dl = dol + c * (NT * 128 >> 4);
             if (tc05::elect_one()) {
-                if (c == 0) mma_ss<0>(tmem, da, db, idesc);
-                else mma_ss<1>(tmem, da, db, idesc);
+                if (c == 0) mma_ss<0>(tmem, da, dh, idesc);
+                else mma_ss<1>(tmem, da, dh, idesc);
 #pragma unroll
-                for (int kk = 1; kk < 8; ++kk) mma_ss<1>(tmem, da + 2 * (kk & 3), db + (kk >> 2) * 512 + 2 * (kk & 3), idesc);
-                tc05::commit(&free_[st]);
-                if (c + 1 == chunks) tc05::commit(&done);
+                for (int kk = 1; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dh + 2 * kk, idesc);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dl + 2 * kk, idesc);
+                tc05::commit(&sm.w_free[c % NW]);
+                if (c + 1 == NC) tc05::commit(&sm.done);
             }
             __syncwarp();
-            if (c + kValueStages < chunks) {
-                ok = wt.wait_warp(&free_[st], (c / kValueStages) & 1);
-                if (ok) load(c + kValueStages);
+            if (c + NW < NC) {
+                ok = wt.wait_warp(&sm.w_free[c % NW], (c / NW) & 1);
+                if (ok) load(c + NW);
             }
         }
     } else {
-        const bool ok = wt.wait_warp(&done, 0);
-        tc05::fence_after_thread_sync();
-        // 128 rows: a warp has 32 of them; 64 rows: 16, in the first half of its lanes
-        const int d = m.Dv == 128 ? 32 * warp + lane : 16 * warp + lane;
-        if (ok) {
-            uint16_t* dst = (uint16_t*)a.output + ((long long)t0 * m.H + h) * m.Dv + d;
+        const int step = a.row_tiles * kTile;        // from a row's partial result to the next
+        // a warp per row: the pieces' common maximum, and the denominator
+        for (int r = warp; r < NT; r += kJoinWarps) {
+            typename Smem::Row row{0, 0, 0.f, 0.f, 0.f, 0.f};
+            if (sm.live[r]) {
+                const int2 part = a.row_part[(long long)(t0 + r) * m.H + h];
+                row.first = part.x;
+                row.pieces = part.y;
+                float2 mine = make_float2(-INFINITY, 0.f);
+                float top = -INFINITY, sum = 0.f;
+                for (int i = lane; i < part.y; i += 32) {
+                    const float2 ml = a.part_ml[part.x + (long long)i * step];
+                    if (i == lane) mine = ml;
+                    if (ml.y > 0.f) {                // (a piece whose tiles the row does not see has no sums)
+                        const float t = fmaxf(top, ml.x);
+                        sum = sum * ex2(top - t) + ml.y * ex2(ml.x - t);
+                        top = t;
+                    }
+                }
+                row.top = pa::warp_max(top);
+                row.inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - row.top));
+                const float k = mine.y > 0.f ? ex2(mine.x - row.top) * row.inv : 0.f;
+                row.k0 = __shfl_sync(0xffffffffu, k, 0);
+                row.k1 = __shfl_sync(0xffffffffu, k, 1);
+            }
+            if (lane == 0) sm.row[r] = row;
+        }
+        auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kJoinThreads) : "memory"); };   // (the joining warps; none of them can have left)
+        meet();
+        constexpr int kPer = R / 4, kAtOnce = kJoinThreads / kPer;   // threads of a row, four latent elements each; rows at a time
+        const int e = tid % kPer;
+        auto load = [&](const typename Smem::Row& row, int i) { return *reinterpret_cast<const float4*>(a.part_o + (row.first + (long long)i * step) * R + 4 * e); };
+        auto add = [](float (&y)[4], float k, const float4& p) { y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w; };
+        auto weight = [&](const typename Smem::Row& row, int i) {
+            const float2 ml = a.part_ml[row.first + (long long)i * step];
+            return ml.y > 0.f ? ex2(ml.x - row.top) * row.inv : 0.f;
+        };
+        auto store = [&](int r, const float (&y)[4]) {
+            uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int c0 = 0; c0 < kTile; c0 += 32) {
-                uint32_t r[32];
-                tc05::ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
-                tc05::wait_ld();
-                if (m.Dv == 128 || lane < 16) {
+            for (int i = 0; i < 2; ++i) {
+                hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
+                lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
+            }
+            const uint32_t at = r * 128 + (((e % 16 >> 1) ^ (r & 7)) << 4) + (e & 1) * 8;      // swizzled by the row
+            *reinterpret_cast<uint2*>(sm.o[0][e / 16] + at) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(sm.o[1][e / 16] + at) = make_uint2(lo[0], lo[1]);
+        };
+        if (NT == 16 && sm.row[0].pieces > 8) {
+            // few rows of many pieces: all threads on a row, its pieces dealt out
+            __shared__ float4 sh[kAtOnce][kPer];
+            for (int r = 0; r < NT; ++r) {
+                const typename Smem::Row row = sm.row[r];
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                if (row.pieces > 0) {
+#pragma unroll 8
+                    for (int i = tid / kPer; i < row.pieces; i += kAtOnce) {
+                        const float k = weight(row, i);
+                        const float4 p = load(row, i);
+                        if (k != 0.f) add(y, k, p);
+                    }
+                    sh[tid / kPer][e] = make_float4(y[0], y[1], y[2], y[3]);
+                    meet();
+                    if (tid < kPer) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (live[c0 + c]) dst[(long long)(c0 + c) * m.H * m.Dv] = pack1<BF>(__uint_as_float(r[c]));
+                        for (int d = 1; d < kAtOnce; ++d) add(y, 1.f, sh[d][e]);
+                    }
+                    meet();
+                }
+                if (tid < kPer) store(r, y);
+            }
+        } else {
+            // four rows a thread, two pieces of each under way together (most rows have no more)
+            for (int r0 = tid / kPer; r0 < NT; r0 += 4 * kAtOnce) {
+                float y[4][4] = {};
+                int most = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (r0 + u * kAtOnce < NT) most = max(most, sm.row[r0 + u * kAtOnce].pieces);
+                for (int i = 0; i < most; i += 2) {
+                    float4 p[4][2];
+                    float k[4][2];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = r0 + u * kAtOnce;
+                        const int left = r < NT ? sm.row[r].pieces - i : 0;
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            p[u][v] = left > v ? load(sm.row[r], i + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            k[u][v] = left > v ? (i == 0 ? (v ? sm.row[r].k1 : sm.row[r].k0) : weight(sm.row[r], i + v)) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int v = 0; v < 2; ++v)
+                            if (k[u][v] != 0.f) add(y[u], k[u][v], p[u][v]);      // (a piece without sums has no results either)
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (r0 + u * kAtOnce < NT) store(r0 + u * kAtOnce, y[u]);
+            }
+        }
+        tc05::fence_proxy_async_smem();
+        warp_arrive(&sm.o_full);
+        if (warp < 4) {
+            const bool ok = wt.wait_warp(&sm.done, 0);
+            tc05::fence_after_thread_sync();
+            // 128 rows: a warp has 32 of them; 64 rows: 16, in the first half of its lanes
+            const int d = m.Dv == 128 ? 32 * warp + lane : 16 * warp + lane;
+            if (ok) {
+                uint16_t* dst = (uint16_t*)a.output + ((long long)t0 * m.H + h) * m.Dv + d;
+#pragma unroll
+                for (int c0 = 0; c0 < NT; c0 += 16) {
+                    uint32_t r[16];
+                    tc05::ld_32x32b_x16(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
+                    tc05::wait_ld();
+                    if (m.Dv == 128 || lane < 16) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (sm.live[c0 + c]) dst[(long long)(c0 + c) * m.H * m.Dv] = pack1<BF>(__uint_as_float(r[c]));
+                    }
                 }
             }
         }
     }
     tc05::fence_before_thread_sync();
     __syncthreads();
-    if (warp == 0) tc05::tmem_dealloc(tmem, 64);
+    if (warp == kJoinWarps) tc05::tmem_dealloc(tmem, 64);
 }
 
 int query_smem(const Step& m) { return 2 * m.Dn * 128 + m.Dn / 64 * 8192; }
-int value_smem(const Step& m) { return kValueStages * (m.Dv * 128 + 2 * 8192); }
 
 template <int R, bool BF>
 cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
@@ -818,10 +852,13 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     const int token_tiles = (m.num_tokens + kTile - 1) / kTile;
     cudaError_t e = pa::launch_dependent(project_query_kernel<BF>, 1 + token_tiles * m.H * (R / 128), 128, query_smem(m), stream, a);
     if (e == cudaSuccess) e = pa::launch_dependent(attend_kernel<R, BF>, a.groups * a.row_tiles, kThreads, sizeof(AttendSmem<R>), stream, a);
-    if (e == cudaSuccess)
-        e = pa::launch_dependent(combine_kernel<R, BF>, a.groups * a.row_tiles * (kTile / kCombineRows), kCombineThreads, kCombineRows * a.groups * sizeof(float), stream, a);
-    if (e == cudaSuccess) e = pa::launch_dependent(project_value_kernel<BF>, token_tiles * m.H, 160, value_smem(m), stream, a);
-    *launches += 4;
+    if (e == cudaSuccess) {
+        // tiles of 16 tokens where those of 64 would leave SMs without one; in an AUTO step most tokens may be the expanded form's
+        const int rows = a.max_new < m.num_tokens ? std::min(m.num_tokens, m.num_sequences) : m.num_tokens;
+        if (rows <= 16 || (long long)(rows + kTile - 1) / kTile * m.H < a.groups * a.row_tiles * 2 / 3) e = pa::launch_dependent(project_value_kernel<R, 16, BF>, (m.num_tokens + 15) / 16 * m.H, kValueThreads, sizeof(ValueSmem<R, 16>), stream, a);
+        else e = pa::launch_dependent(project_value_kernel<R, 64, BF>, token_tiles * m.H, kValueThreads, sizeof(ValueSmem<R, 64>), stream, a);
+    }
+    *launches += 3;
     return e;
 }
 
@@ -829,7 +866,8 @@ template <int R, bool BF>
 cudaError_t prepare(const Step& m) {
     cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, query_smem(m));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(AttendSmem<R>));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, value_smem(m));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<R, 16, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ValueSmem<R, 16>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<R, 64, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ValueSmem<R, 64>));
     return e;
 }
 

@@ -123,7 +123,7 @@ constexpr size_t kExpandBytes = (size_t)1 << 30;
 
 struct Scratch {
     int row_tiles, groups;
-    size_t unit_prefix, block_prefix, starts, q_abs, part_o, part_ml, cuts, o_lat;
+    size_t unit_prefix, block_prefix, starts, q_abs, part_o, part_ml, row_part;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
     size_t tile_prefix, query_prefix, order, counter, k, v, k_rope;
@@ -147,8 +147,7 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.starts = take(s.groups * sizeof(latent::SliceStart));
         s.q_abs = take(rows * (d.latent_size + d.rope_size) * 2);
-        s.o_lat = take(rows * 2 * d.latent_size * 2);
-        s.cuts = take((size_t)s.groups * s.row_tiles * sizeof(latent::Cut));
+        s.row_part = take(rows * sizeof(int2));
         s.part_ml = take(slots * latent::kTile * sizeof(float2));
         s.part_o = take(slots * latent::kTile * d.latent_size * sizeof(float));
     }
@@ -268,8 +267,7 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         k.q_abs = h->ws + s.q_abs;
         k.part_o = (float*)(h->ws + s.part_o);
         k.part_ml = (float2*)(h->ws + s.part_ml);
-        k.cuts = (latent::Cut*)(h->ws + s.cuts);
-        k.o_lat = h->ws + s.o_lat;
+        k.row_part = (int2*)(h->ws + s.row_part);
         k.output = a->output;
         k.scale_log2 = scale * 1.4426950408889634f;
         const int W = R + P;
@@ -280,13 +278,12 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         const long long groups = (long long)a->num_blocks * d.block_size / 8;
         const long long ca_size[4] = {64, 8, R / 64, groups}, ca_stride[3] = {W, 64, 8 * W}, cr_size[3] = {P, 8, groups}, cr_stride[2] = {W, 8 * W};
         const long long qa_size[3] = {64, (long long)T * H, R / 64}, qa_stride[2] = {W, 64}, qr_size[2] = {P, (long long)T * H}, qr_stride[1] = {W};
-        const long long ol_size[3] = {2 * R, H, T}, ol_stride[2] = {2 * R, 2ll * R * H};
         const int box_tokens[3] = {64, 1, latent::kTile}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1};
         const int box_q[3] = {64, latent::kTile, R / 64}, box_qr[2] = {64, latent::kTile}, box_c[4] = {64, 8, R / 64, std::min(d.block_size, latent::kTokens / 2) / 8}, box_cr[3] = {64, 8, box_c[3]};
         if (!make_map(&k.map_qn, d.dtype, a->query_nope, 3, qn_size, qn_stride, box_tokens) || !make_map(&k.map_key_up, d.dtype, a->key_up, 3, ku_size, ku_stride, box_ku) ||
             !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_q_abs, d.dtype, k.q_abs, 3, qa_size, qa_stride, box_q) ||
             !make_map(&k.map_q_abs_rope, d.dtype, (const uint16_t*)k.q_abs + R, 2, qr_size, qr_stride, box_qr) ||
-            !make_map(&k.map_cache, d.dtype, a->cache, 4, ca_size, ca_stride, box_c) || !make_map(&k.map_cache_rope, d.dtype, (const uint16_t*)a->cache + R, 3, cr_size, cr_stride, box_cr) || !make_map(&k.map_o_lat, d.dtype, k.o_lat, 3, ol_size, ol_stride, box_tokens))
+            !make_map(&k.map_cache, d.dtype, a->cache, 4, ca_size, ca_stride, box_c) || !make_map(&k.map_cache_rope, d.dtype, (const uint16_t*)a->cache + R, 3, cr_size, cr_stride, box_cr))
             return fail(PA_ERR_CUDA, "a tensor map could not be made");
         LATENT_CUDA(latent::launch_absorbed(k, d.dtype, stream, &launches));
     }

@@ -40,18 +40,10 @@ struct AppendArgs {
 
 // The absorbed form.  Its unit of work is a tile of 64 context tokens for a block of `row_tiles` tiles of 64 query rows (new token, head) of one
 // sequence; sequence s has block_prefix[s + 1] - block_prefix[s] such blocks, every one of the same number of tiles.  Units are
-// numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block that is cut leaves
-// one partial result per group in slot (block + group) * row_tiles + row tile.
+// numbered by sequence, block and tile, and group w of `row_tiles` CTAs takes the w-th of equal slices; a block leaves one partial result
+// for every group that has a part of it, in slot (block + group) * row_tiles + row tile.
 constexpr int kTile = 64;      // query rows of a row tile, new tokens of a projection's tile
 constexpr int kTokens = 64;    // context tokens of a tile
-
-// A row tile whose block the CTA's slice is the first to cut: where its partial results are and where the joined rows go.
-struct __align__(16) Cut {
-    int rows;       // 0: none
-    int grow0;      // first row among the step's (token, head) rows
-    int slot;       // of the first piece; the next ones follow `row_tiles` slots apart
-    int pieces;
-};
 
 // Where a group's slice begins: sequence (-1: no units) and what there is to know of it, row block of the sequence, context tile of the block; and
 // the slice's units.
@@ -60,7 +52,7 @@ struct __align__(16) SliceStart {
     int t0, n, past, tb;            // of the sequence (SeqView)
     int blocks, tiles;              // its row blocks, and context tiles of each
     int block0;                     // row blocks of the sequences before
-    int unused;
+    int per;                        // units of a whole slice
 };
 
 struct AbsorbedArgs {
@@ -75,11 +67,10 @@ struct AbsorbedArgs {
     void* q_abs;                // [num_tokens * H][R + P] absorbed query rows
     float* part_o;              // [slot][64][R]
     float2* part_ml;            // [slot][64] maximum (base 2, scaled) and sum
-    Cut* cuts;                  // [groups * row_tiles]
-    void* o_lat;                // [num_tokens * H][2 R] sums of latents, high and low pieces
+    int2* row_part;             // [num_tokens * H] a row's first partial result (slot * 64 + row of the tile) and how many it has
     void* output;
     float scale_log2;           // softmax scale * log2(e)
-    CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_rope, map_value_up, map_o_lat;
+    CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_rope, map_value_up;
 };
 // Largest number of slots a step can need.
 long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);
