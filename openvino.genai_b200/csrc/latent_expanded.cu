@@ -96,14 +96,23 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
 // A CTA keeps a tile of 128 context rows in shared memory and walks over heads: D[token][element] of the head's keys, then of its values, with
 // the weights streamed in chunks of 64 latent elements.  Two accumulators, so that one head is written out while the next is computed.
 constexpr int kExpandThreads = 192;    // warps 0 - 3: output, 4: loader, 5: products
-constexpr int kWeightStages = 4;
+
+// A place in a ring of N barriers and the phase that it waits for.
+template <int N>
+struct Ring {
+    uint32_t at = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) { at = 0; phase ^= 1u; }
+    }
+};
 
 template <int R>
 struct ExpandSmem {
+    static constexpr int NW = R == 512 ? 5 : 8;              // chunks of weights under way: what the context tile leaves room for
     alignas(1024) uint8_t a[R / 64][kExpandTile * 128];
-    alignas(1024) uint8_t w[kWeightStages][128 * 128];
-    alignas(1024) uint8_t out[2][kExpandTile * 128];        // 128 elements of every row on their way to global memory
-    uint64_t a_full, a_free, w_full[kWeightStages], w_free[kWeightStages], d_full[2], d_free[2];
+    alignas(1024) uint8_t w[NW][128 * 128];
+    alignas(1024) uint8_t out[kExpandTile * 128];            // 64 elements of every row on their way to global memory
+    uint64_t a_full, a_free, w_full[NW], w_free[NW], d_full[2], d_free[2];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -146,7 +155,7 @@ __device__ __forceinline__ ExpandItem expand_item(const ExpandedArgs& a, int i, 
 template <int R, int DN, int DV, bool BF>
 __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_constant__ ExpandedArgs a) {
     using Smem = ExpandSmem<R>;
-    constexpr int NC = R / 64;
+    constexpr int NC = R / 64, NW = Smem::NW;
     extern __shared__ __align__(1024) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
@@ -154,7 +163,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     if (tid == 0) {
         pa::mbar_init(&sm.a_full, 1);
         pa::mbar_init(&sm.a_free, 1);
-        for (int i = 0; i < kWeightStages; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
+        for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
         for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.d_full[i], 1); pa::mbar_init(&sm.d_free[i], 4); }
         pa::mbar_fence_init();
         sm.abort_flag = 0;
@@ -181,17 +190,19 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
             }
             if (na > 0) ok = wt.wait_warp(&sm.a_free, (na - 1) & 1);
             if (!ok) break;
-            if (lane == 0) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
+            if (tc05::elect_one()) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
+            __syncwarp();
             for (int b = 0; b < it.blocks; ++b) {
                 const int at = __shfl_sync(0xffffffffu, page, b) * m.bs;
-                if (lane == 0)
+                if (tc05::elect_one())
                     for (int c = 0; c < NC; ++c) tma_2d(sm.a[c] + b * m.bs * 128, &a.map_cache, 64 * c, at, &sm.a_full);
+                __syncwarp();
             }
             for (int h = it.h_first; ok && h < it.h_end; ++h)
                 for (int x = 0; ok && x < 2 * NC; ++x, ++n) {
-                    const int st = n % kWeightStages;
-                    if (n >= kWeightStages) ok = wt.wait_warp(&sm.w_free[st], (n / kWeightStages - 1) & 1);
-                    if (ok && lane == 0) {
+                    const int st = n % NW;
+                    if (n >= NW) ok = wt.spin_warp(&sm.w_free[st], (n / NW - 1) & 1);
+                    if (ok && tc05::elect_one()) {
                         pa::mbar_expect_tx(&sm.w_full[st], (x < NC ? DN : DV) * 128);
                         tma_3d(sm.w[st], x < NC ? &a.map_key_up : &a.map_value_up, 64 * (x % NC), 0, a.h0 + h, &sm.w_full[st]);
                     }
@@ -201,12 +212,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
         if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
         if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
             for (uint32_t k = 0; na > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.a_full, (na - 1) & 1); ++k) {}
-            for (uint32_t i = n > kWeightStages ? n - kWeightStages : 0; i < n; ++i)
-                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % kWeightStages], (i / kWeightStages) & 1); ++k) {}
+            for (uint32_t i = n > NW ? n - NW : 0; i < n; ++i)
+                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % NW], (i / NW) & 1); ++k) {}
         }
     } else if (warp == 5) {
         constexpr uint32_t idesc_k = tc05::instr_desc_f16(128, DN, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 0);
-        static_assert(2 * NC % kWeightStages == 0, "a head begins with the first stage");
+        Ring<NW> w;
         const uint32_t da = desc_low(sm.a), dw = desc_low(sm.w);
         uint32_t na = 0, nd = 0;
         bool ok = true;
@@ -217,32 +228,32 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                 if (nd >= 2) ok = wt.spin_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
 #pragma unroll
                 for (int x = 0; x < 2 * NC; ++x) {
-                    constexpr int kRound = 2 * NC / kWeightStages;     // (a stage's phase: its round in the head, and the heads before)
-                    const int st = x % kWeightStages;
-                    if (ok) ok = wt.spin_warp(&sm.w_full[st], (nd * kRound + x / kWeightStages) & 1);
+                    if (ok) ok = wt.spin_warp(&sm.w_full[w.at], w.phase);
                     if (!ok) break;
                     tc05::fence_after_thread_sync();
                     const uint32_t d = tmem + (nd & 1) * kBuffer + (x < NC ? 0 : DN);
                     if (tc05::elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
-                            const uint32_t pa = da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, pw = dw + st * (128 * 128 >> 4) + 2 * kk;
+                            const uint32_t pa = da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, pw = dw + w.at * (128 * 128 >> 4) + 2 * kk;
                             if (x % NC + kk == 0) mma_ss<0>(d, pa, pw, x < NC ? idesc_k : idesc_v);
                             else mma_ss<1>(d, pa, pw, x < NC ? idesc_k : idesc_v);
                         }
-                        tc05::commit(&sm.w_free[st]);
+                        tc05::commit(&sm.w_free[w.at]);
                         if (x == 2 * NC - 1) {
                             tc05::commit(&sm.d_full[nd & 1]);
                             if (h + 1 == it.h_end) tc05::commit(&sm.a_free);
                         }
                     }
                     __syncwarp();
+                    w.next();
                 }
             }
         }
     } else {
         uint32_t nd = 0;
         const int row = tid;       // of the tile
+        const bool leader = tc05::elect_one();     // the lane whose copies and waits for them are the warp's
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         bool ok = true;
         for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
@@ -262,45 +273,43 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                 ok = wt.wait_warp(&sm.d_full[nd & 1], (nd / 2) & 1);
                 if (!ok) break;
                 tc05::fence_after_thread_sync();
+                // 64 elements of the warp's 32 rows at a time
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    const int D = part ? DV : DN;
-                    const uint32_t src = tmem + (nd & 1) * kBuffer + (part ? DN : 0) + lanes;
-                    // the copies out of the staging rows that this warp wrote before have read them (a warp stages and sends its own 32 rows)
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    __syncwarp();
-#pragma unroll
-                    for (int c0 = 0; c0 < D; c0 += 32) {
-                        uint32_t r[32];
-                        tc05::ld_32x32b_x32(src + c0, r);
-                        tc05::wait_ld();
-#pragma unroll
-                        for (int c = 0; c < 32; c += 8) {
-                            uint4 w = make_uint4(0, 0, 0, 0);     // rows behind the context: zeros, whatever the cache holds there
-                            if (live)
-                                w = make_uint4(pack2<BF>(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), pack2<BF>(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])),
-                                               pack2<BF>(__uint_as_float(r[c + 4]), __uint_as_float(r[c + 5])), pack2<BF>(__uint_as_float(r[c + 6]), __uint_as_float(r[c + 7])));
-                            const int chunk = (c0 + c) / 8;
-                            *reinterpret_cast<uint4*>(sm.out[chunk >> 3] + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = w;
-                        }
-                    }
-                    if (part == 1) {
+                for (int c0 = 0; c0 < kBuffer; c0 += 64) {
+                    const uint32_t src = tmem + (nd & 1) * kBuffer + c0 + lanes;
+                    uint32_t r[2][32];
+                    tc05::ld_32x32b_x32(src, r[0]);
+                    tc05::ld_32x32b_x32(src + 32, r[1]);
+                    tc05::wait_ld();
+                    if (c0 + 64 == kBuffer) {
                         tc05::fence_before_thread_sync();
                         warp_arrive(&sm.d_free[nd & 1]);
                     }
+                    // the copy out of the warp's staging rows before has read them
+                    if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const uint32_t* v = &r[q >> 2][8 * (q & 3)];
+                        uint4 w = make_uint4(0, 0, 0, 0);     // rows behind the context: zeros, whatever the cache holds there
+                        if (live)
+                            w = make_uint4(pack2<BF>(__uint_as_float(v[0]), __uint_as_float(v[1])), pack2<BF>(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                                           pack2<BF>(__uint_as_float(v[4]), __uint_as_float(v[5])), pack2<BF>(__uint_as_float(v[6]), __uint_as_float(v[7])));
+                        *reinterpret_cast<uint4*>(sm.out + row * 128 + ((q ^ (row & 7)) << 4)) = w;
+                    }
                     tc05::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
-                        const int y = (int)(h * a.rows + it.row + warp * 32);
-                        for (int c = 0; c < D / 64; ++c)
-                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(part ? &a.map_v_out : &a.map_k_out),
-                                         "r"(64 * c), "r"(y), "r"(pa::smem_u32(sm.out[c] + warp * 32 * 128)) : "memory");
+                    if (leader) {
+                        const bool value = c0 >= DN;
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(value ? &a.map_v_out : &a.map_k_out),
+                                     "r"(value ? c0 - DN : c0), "r"((int)(h * a.rows + it.row + warp * 32)), "r"(pa::smem_u32(sm.out + warp * 32 * 128)) : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
+                    __syncwarp();
                 }
             }
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
     }
     __syncthreads();
@@ -340,15 +349,6 @@ struct ExpandedSmem {
     QueryItem item[kItemSlots];
     uint32_t tmem_base;
     int abort_flag;
-};
-
-// A place in a ring of N barriers and the phase that it waits for.
-template <int N>
-struct Ring {
-    uint32_t at = 0, phase = 0;
-    __device__ __forceinline__ void next() {
-        if (++at == N) { at = 0; phase ^= 1u; }
-    }
 };
 
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
