@@ -93,9 +93,12 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
 }
 
 // ---- k = key_up c, v = value_up c ---------------------------------------------------------------------------------------------
-// A CTA keeps a tile of 128 context rows in shared memory and walks over heads: D[token][element] of the head's keys, then of its values, with
-// the weights streamed in chunks of 64 latent elements.  Two accumulators, so that one head is written out while the next is computed.
-constexpr int kExpandThreads = 192;    // warps 0 - 3: output, 4: loader, 5: products
+// A CTA keeps a tile of 128 context rows in tensor memory and walks over heads: D[token][element] of the head's keys, then of its values, with the
+// weights streamed in chunks of 64 latent elements.  Keys and values have an accumulator each, so that one is written out while the other is
+// computed.  The rows go from the cache to shared memory (the next tile's beside this one's products) and from there to tensor memory, because an
+// M 128, N 128 step with both operands in shared memory takes all of that memory's bandwidth and leaves none for the weights to come in:
+// 129 us for 10 k rows by 32 heads of 512 -> 128 + 128.
+constexpr int kExpandThreads = 224;    // warps 0 - 3: output, 4: rows and even chunks of weights, 5: products, 6: odd chunks (one warp takes 450 cycles a chunk, the products 256)
 
 // A place in a ring of N barriers and the phase that it waits for.
 template <int N>
@@ -112,7 +115,8 @@ struct ExpandSmem {
     alignas(1024) uint8_t a[R / 64][kExpandTile * 128];
     alignas(1024) uint8_t w[NW][128 * 128];
     alignas(1024) uint8_t out[kExpandTile * 128];            // 64 elements of every row on their way to global memory
-    uint64_t a_full, a_free, w_full[NW], w_free[NW], d_full[2], d_free[2];
+    uint64_t a_full, a_free, a_ready;                        // rows in shared memory, read, in tensor memory
+    uint64_t w_full[NW], w_free[NW], d_full[2], d_free[2];   // weights; accumulators of keys and values
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -162,7 +166,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
         pa::mbar_init(&sm.a_full, 1);
-        pa::mbar_init(&sm.a_free, 1);
+        pa::mbar_init(&sm.a_free, 4);
+        pa::mbar_init(&sm.a_ready, 4);
         for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
         for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.d_full[i], 1); pa::mbar_init(&sm.d_free[i], 4); }
         pa::mbar_fence_init();
@@ -176,30 +181,34 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     const uint32_t tmem = sm.tmem_base;
     const Waiter wt{&sm.abort_flag, m.status};
     const int per = expand_heads_per_item(a), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
-    constexpr int kBuffer = DN + DV;     // tensor-memory columns of one head
+    constexpr uint32_t kD = R / 2;       // tensor memory: the rows (two elements a column), then 128 columns each for keys and values
 
-    if (warp == 4) {
+    if (warp == 4 || warp == 6) {
+        const bool even = warp == 4;
         uint32_t n = 0, na = 0;
         bool ok = true, bad_index = false;
         for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
             const ExpandItem it = expand_item(a, i, per);
-            int page = 0;
-            if (lane < it.blocks) {
-                page = m.block_indices[it.block0 + lane];
-                if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
-            }
-            if (na > 0) ok = wt.wait_warp(&sm.a_free, (na - 1) & 1);
-            if (!ok) break;
-            if (tc05::elect_one()) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
-            __syncwarp();
-            for (int b = 0; b < it.blocks; ++b) {
-                const int at = __shfl_sync(0xffffffffu, page, b) * m.bs;
-                if (tc05::elect_one())
-                    for (int c = 0; c < NC; ++c) tma_2d(sm.a[c] + b * m.bs * 128, &a.map_cache, 64 * c, at, &sm.a_full);
+            if (even) {
+                int page = 0;
+                if (lane < it.blocks) {
+                    page = m.block_indices[it.block0 + lane];
+                    if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
+                }
+                if (na > 0) ok = wt.wait_warp(&sm.a_free, (na - 1) & 1);
+                if (!ok) break;
+                if (tc05::elect_one()) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
                 __syncwarp();
+                for (int b = 0; b < it.blocks; ++b) {
+                    const int at = __shfl_sync(0xffffffffu, page, b) * m.bs;
+                    if (tc05::elect_one())
+                        for (int c = 0; c < NC; ++c) tma_2d(sm.a[c] + b * m.bs * 128, &a.map_cache, 64 * c, at, &sm.a_full);
+                    __syncwarp();
+                }
             }
             for (int h = it.h_first; ok && h < it.h_end; ++h)
                 for (int x = 0; ok && x < 2 * NC; ++x, ++n) {
+                    if ((n & 1) == (even ? 1u : 0u)) continue;
                     const int st = n % NW;
                     if (n >= NW) ok = wt.spin_warp(&sm.w_free[st], (n / NW - 1) & 1);
                     if (ok && tc05::elect_one()) {
@@ -211,51 +220,69 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
         }
         if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
         if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
-            for (uint32_t k = 0; na > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.a_full, (na - 1) & 1); ++k) {}
+            for (uint32_t k = 0; even && na > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.a_full, (na - 1) & 1); ++k) {}
             for (uint32_t i = n > NW ? n - NW : 0; i < n; ++i)
-                for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % NW], (i / NW) & 1); ++k) {}
+                for (uint32_t k = 0; (i & 1) != (even ? 1u : 0u) && k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % NW], (i / NW) & 1); ++k) {}
         }
     } else if (warp == 5) {
         constexpr uint32_t idesc_k = tc05::instr_desc_f16(128, DN, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 0);
         Ring<NW> w;
-        const uint32_t da = desc_low(sm.a), dw = desc_low(sm.w);
+        const uint32_t dw = desc_low(sm.w);
         uint32_t na = 0, nd = 0;
         bool ok = true;
         for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
             const ExpandItem it = expand_item(a, i, per);
-            ok = wt.wait_warp(&sm.a_full, na & 1);
-            for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
-                if (nd >= 2) ok = wt.spin_warp(&sm.d_free[nd & 1], (nd / 2 - 1) & 1);
+            ok = wt.spin_warp(&sm.a_ready, na & 1);
+            for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd)
 #pragma unroll
-                for (int x = 0; x < 2 * NC; ++x) {
-                    if (ok) ok = wt.spin_warp(&sm.w_full[w.at], w.phase);
-                    if (!ok) break;
-                    tc05::fence_after_thread_sync();
-                    const uint32_t d = tmem + (nd & 1) * kBuffer + (x < NC ? 0 : DN);
-                    if (tc05::elect_one()) {
+                for (int part = 0; part < 2; ++part) {
+                    if (ok && nd > 0) ok = wt.spin_warp(&sm.d_free[part], (nd - 1) & 1);
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            const uint32_t pa = da + (x % NC) * (kExpandTile * 128 >> 4) + 2 * kk, pw = dw + w.at * (128 * 128 >> 4) + 2 * kk;
-                            if (x % NC + kk == 0) mma_ss<0>(d, pa, pw, x < NC ? idesc_k : idesc_v);
-                            else mma_ss<1>(d, pa, pw, x < NC ? idesc_k : idesc_v);
+                    for (int c = 0; c < NC; ++c) {
+                        if (ok) ok = wt.spin_warp(&sm.w_full[w.at], w.phase);
+                        if (!ok) break;
+                        tc05::fence_after_thread_sync();
+                        const uint32_t d = tmem + kD + part * 128, rows = tmem + c * 32, pw = dw + w.at * (128 * 128 >> 4), idesc = part ? idesc_v : idesc_k;
+                        if (tc05::elect_one()) {
+                            if (c == 0) mma_ts<0>(d, rows, pw, idesc);
+                            else mma_ts<1>(d, rows, pw, idesc);
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) mma_ts<1>(d, rows + 8 * kk, pw + 2 * kk, idesc);
+                            tc05::commit(&sm.w_free[w.at]);
+                            if (c + 1 == NC) tc05::commit(&sm.d_full[part]);
                         }
-                        tc05::commit(&sm.w_free[w.at]);
-                        if (x == 2 * NC - 1) {
-                            tc05::commit(&sm.d_full[nd & 1]);
-                            if (h + 1 == it.h_end) tc05::commit(&sm.a_free);
-                        }
+                        __syncwarp();
+                        w.next();
                     }
-                    __syncwarp();
-                    w.next();
                 }
-            }
         }
     } else {
-        uint32_t nd = 0;
+        uint32_t nd = 0, na = 0;
         const int row = tid;       // of the tile
         const bool leader = tc05::elect_one();     // the lane whose copies and waits for them are the warp's
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        // this thread's row from shared to tensor memory
+        auto keep_rows = [&]() -> bool {
+            if (!wt.wait_warp(&sm.a_full, na & 1)) return false;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                uint32_t r[32];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(sm.a[c] + row * 128 + ((q ^ (row & 7)) << 4));
+                    r[4 * q] = v.x; r[4 * q + 1] = v.y; r[4 * q + 2] = v.z; r[4 * q + 3] = v.w;
+                }
+                tc05::st_32x32b_x32(tmem + c * 32 + lanes, r);
+            }
+            tc05::wait_st();
+            tc05::fence_before_thread_sync();
+            warp_arrive(&sm.a_ready);
+            warp_arrive(&sm.a_free);
+            ++na;
+            return true;
+        };
         bool ok = true;
+        if ((int)blockIdx.x < items) ok = keep_rows();
         for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
             const ExpandItem it = expand_item(a, i, per);
             const bool live = row < it.valid;
@@ -270,20 +297,27 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                 for (int c = 0; c < m.P / 8; ++c) dst[c] = src ? src[c] : make_uint4(0, 0, 0, 0);
             }
             for (int h = it.h_first; ok && h < it.h_end; ++h, ++nd) {
-                ok = wt.wait_warp(&sm.d_full[nd & 1], (nd / 2) & 1);
-                if (!ok) break;
-                tc05::fence_after_thread_sync();
                 // 64 elements of the warp's 32 rows at a time
 #pragma unroll
-                for (int c0 = 0; c0 < kBuffer; c0 += 64) {
-                    const uint32_t src = tmem + (nd & 1) * kBuffer + c0 + lanes;
+                for (int c0 = 0; c0 < DN + DV; c0 += 64) {
+                    const bool value = c0 >= DN;
+                    const int at = value ? c0 - DN : c0, size = value ? DV : DN;
+                    if (at == 0) {
+                        if (ok) ok = wt.wait_warp(&sm.d_full[value], nd & 1);
+                        if (!ok) break;
+                        tc05::fence_after_thread_sync();
+                        // (the item's last product is complete: the next item's rows may take the place of this one's)
+                        if (value && h + 1 == it.h_end && i + (int)gridDim.x < items) ok = keep_rows();
+                        if (!ok) break;
+                    }
+                    const uint32_t src = tmem + kD + (value ? 128 : 0) + at + lanes;
                     uint32_t r[2][32];
                     tc05::ld_32x32b_x32(src, r[0]);
                     tc05::ld_32x32b_x32(src + 32, r[1]);
                     tc05::wait_ld();
-                    if (c0 + 64 == kBuffer) {
+                    if (at + 64 == size) {
                         tc05::fence_before_thread_sync();
-                        warp_arrive(&sm.d_free[nd & 1]);
+                        warp_arrive(&sm.d_free[value]);
                     }
                     // the copy out of the warp's staging rows before has read them
                     if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -300,9 +334,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                     tc05::fence_proxy_async_smem();
                     __syncwarp();
                     if (leader) {
-                        const bool value = c0 >= DN;
                         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(value ? &a.map_v_out : &a.map_k_out),
-                                     "r"(value ? c0 - DN : c0), "r"((int)(h * a.rows + it.row + warp * 32)), "r"(pa::smem_u32(sm.out + warp * 32 * 128)) : "memory");
+                                     "r"(at), "r"((int)(h * a.rows + it.row + warp * 32)), "r"(pa::smem_u32(sm.out + warp * 32 * 128)) : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                     __syncwarp();
