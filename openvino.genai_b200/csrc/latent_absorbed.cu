@@ -18,7 +18,7 @@ struct SeqPlan {
 };
 __device__ __forceinline__ SeqPlan seq_plan(const AbsorbedArgs& a, int s) {
     SeqView v;
-    if (!seq_view(a.m, s, v) || v.n == 0 || v.n > a.max_new) return SeqPlan{0, 0};
+    if (!seq_view(a.m, s, v) || v.n == 0 || !takes_absorbed(a.m, v)) return SeqPlan{0, 0};
     const int rows = kTile * a.row_tiles;
     return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTokens - 1) / kTokens};
 }
@@ -83,7 +83,7 @@ __device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&
     bool mine = false;
     if (threadIdx.x < NT) {
         SeqView v;
-        mine = t0 + (int)threadIdx.x < a.m.num_tokens && token_view(a.m, t0 + threadIdx.x, v) && v.n <= a.max_new;
+        mine = t0 + (int)threadIdx.x < a.m.num_tokens && token_view(a.m, t0 + threadIdx.x, v) && takes_absorbed(a.m, v);
         live[threadIdx.x] = mine;
     }
     return __syncthreads_or(mine) != 0;
@@ -854,7 +854,7 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     if (e == cudaSuccess) e = pa::launch_dependent(attend_kernel<R, BF>, a.groups * a.row_tiles, kThreads, sizeof(AttendSmem<R>), stream, a);
     if (e == cudaSuccess) {
         // tiles of 16 tokens where those of 64 would leave SMs without one; in an AUTO step most tokens may be the expanded form's
-        const int rows = a.max_new < m.num_tokens ? std::min(m.num_tokens, m.num_sequences) : m.num_tokens;
+        const int rows = m.form == PA_LATENT_AUTO ? std::min(m.num_tokens, m.num_sequences) : m.num_tokens;
         if (rows <= 16 || (long long)(rows + kTile - 1) / kTile * m.H < a.groups * a.row_tiles * 2 / 3) e = pa::launch_dependent(project_value_kernel<R, 16, BF>, (m.num_tokens + 15) / 16 * m.H, kValueThreads, sizeof(ValueSmem<R, 16>), stream, a);
         else e = pa::launch_dependent(project_value_kernel<R, 64, BF>, token_tiles * m.H, kValueThreads, sizeof(ValueSmem<R, 64>), stream, a);
     }

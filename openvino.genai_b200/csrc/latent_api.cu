@@ -115,8 +115,6 @@ bool make_map(CUtensorMap* map, int dtype, const void* base, int rank, const lon
 }
 
 // ---- scratch ------------------------------------------------------------------------------------------------------------
-// New tokens up to which a sequence of an AUTO step takes the absorbed form.
-constexpr int kAutoMaxNew = 64;
 
 // Expanded keys and values of as many heads as fit this are made at a time.
 constexpr size_t kExpandBytes = (size_t)1 << 30;
@@ -126,7 +124,7 @@ struct Scratch {
     size_t unit_prefix, block_prefix, starts, q_abs, part_o, part_ml, row_part;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
-    size_t tile_prefix, query_prefix, order, counter, k, v, k_rope;
+    size_t tile_prefix, query_prefix, order, heads_per_item, counter, k, v, k_rope;
     size_t total;
 };
 
@@ -141,7 +139,7 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
     if (form != PA_LATENT_EXPANDED) {
         const size_t rows = (size_t)tokens * d.num_heads;
         // in an AUTO step only the short sequences' rows have partial results
-        const int most = form == PA_LATENT_AUTO ? (int)std::min<long long>(tokens, (long long)sequences * kAutoMaxNew) : tokens;
+        const int most = form == PA_LATENT_AUTO ? (int)std::min<long long>(tokens, (long long)sequences * latent::kAutoMaxNew) : tokens;
         const size_t slots = (size_t)latent::absorbed_slots(most, sequences, d.num_heads, s.groups, s.row_tiles);
         s.unit_prefix = take(((size_t)sequences + 1) * sizeof(long long));
         s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
@@ -151,8 +149,8 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.part_ml = take(slots * latent::kTile * sizeof(float2));
         s.part_o = take(slots * latent::kTile * d.latent_size * sizeof(float));
     }
-    if (form == PA_LATENT_EXPANDED || (form == PA_LATENT_AUTO && tokens > kAutoMaxNew)) {
-        const int served = form == PA_LATENT_AUTO ? std::min(sequences, tokens / (kAutoMaxNew + 1)) : sequences;
+    if (form == PA_LATENT_EXPANDED || (form == PA_LATENT_AUTO && tokens > latent::kAutoFewNew)) {
+        const int served = form == PA_LATENT_AUTO ? std::min(sequences, tokens / (latent::kAutoFewNew + 1)) : sequences;
         s.rows = ((long long)block_indices * d.block_size / latent::kExpandTile + served) * latent::kExpandTile;
         const size_t head = (size_t)s.rows * (d.nope_size + d.value_size) * 2;
         s.heads = (int)std::max<size_t>(1, std::min<size_t>(d.num_heads, kExpandBytes / std::max<size_t>(1, head)));
@@ -160,6 +158,7 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.tile_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.query_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.order = take(((size_t)tokens / latent::kQueryTile + served) * sizeof(int2));
+        s.heads_per_item = take(sizeof(int));
         s.counter = take((size_t)s.passes * sizeof(int));
         s.k_rope = take((size_t)s.rows * 64 * 2);
         s.k = take((size_t)s.heads * s.rows * d.nope_size * 2);
@@ -197,7 +196,7 @@ latent::Step make_step(const pa_latent_handle* h, const Args* a) {
     const pa_latent_desc& d = h->desc;
     return latent::Step{d.num_heads, d.latent_size, d.rope_size, d.nope_size, d.value_size, d.block_size,
                         a->num_tokens, a->num_sequences, a->num_block_indices, a->num_blocks,
-                        a->past_lens, a->subsequence_begins, a->block_indices, a->block_indices_begins, h->status};
+                        a->past_lens, a->subsequence_begins, a->block_indices, a->block_indices_begins, h->status, PA_LATENT_AUTO};
 }
 
 int append(pa_latent_handle* h, const pa_latent_append_args* a) {
@@ -253,12 +252,11 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
     const Scratch s = plan_scratch(h, T, a->num_sequences, a->num_block_indices, a->form);
     rc = ensure_ws(h, s.total);
     if (rc != PA_OK) return rc;
-    const int max_new = a->form == PA_LATENT_ABSORBED ? INT_MAX : kAutoMaxNew;
     int launches = 0;
     if (a->form != PA_LATENT_EXPANDED) {
         latent::AbsorbedArgs k{};
         k.m = make_step(h, a);
-        k.max_new = max_new;
+        k.m.form = a->form;
         k.groups = s.groups; k.row_tiles = s.row_tiles;
         k.unit_prefix = (long long*)(h->ws + s.unit_prefix);
         k.block_prefix = (int*)(h->ws + s.block_prefix);
@@ -291,13 +289,14 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         if (s.heads * s.rows > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 rows of expanded keys");
         latent::ExpandedArgs k{};
         k.m = make_step(h, a);
-        k.min_new = a->form == PA_LATENT_EXPANDED ? 1 : kAutoMaxNew + 1;
+        k.m.form = a->form;
         k.rows = s.rows;
         k.tile_prefix = (int*)(h->ws + s.tile_prefix);
         k.query_prefix = (int*)(h->ws + s.query_prefix);
         k.order = (int2*)(h->ws + s.order);
         k.counter = (int*)(h->ws + s.counter);
-        k.passes = s.passes;
+        k.heads_per_item = (int*)(h->ws + s.heads_per_item);
+        k.passes = s.passes; k.ctas = h->sm_count; k.heads = s.heads;
         k.cache = a->cache;
         k.k_rope = h->ws + s.k_rope;
         k.output = a->output;

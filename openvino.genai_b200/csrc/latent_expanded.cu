@@ -4,6 +4,7 @@
 //   expand   k, v of every (128 context tokens, head), and the rotated key part gathered from its pages
 //   attend   256 new tokens of one head at a time
 #include <algorithm>
+#include <climits>
 
 #include "latent_tc.cuh"
 
@@ -29,7 +30,7 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         int c = 0, q = 0;
         if (s < B) {
             SeqView v;
-            if (seq_view(m, s, v) && v.n > 0 && v.n >= a.min_new) {
+            if (seq_view(m, s, v) && v.n > 0 && !takes_absorbed(m, v)) {
                 c = (int)(((long long)v.past + v.n + kExpandTile - 1) / kExpandTile);
                 q = (v.n + kQueryTile - 1) / kQueryTile;
             }
@@ -50,6 +51,16 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         __syncthreads();
     }
     if (tid == 0) { a.tile_prefix[B] = run_c; a.query_prefix[B] = run_q; }
+    if (tid >= 32 && tid < 64) {
+        // heads of an item of the expansion: the number whose last CTA ends first, at 7 parts a head and 4 for bringing the context tile in
+        const int per = lane + 1;
+        const long long items = (long long)run_c * ((a.heads + per - 1) / per);
+        long long cost = per <= a.heads ? (items + a.ctas - 1) / a.ctas * (7 * per + 4) : LLONG_MAX / 64;
+        cost = cost * 32 + lane;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) cost = min(cost, __shfl_xor_sync(0xffffffffu, cost, o));
+        if (lane == 0) *a.heads_per_item = (int)(cost % 32) + 1;
+    }
     __syncthreads();
     // counting sort of the query tiles by the context they see, the longest first, so that the last items to be drawn are short
     const int total = run_q;
@@ -128,12 +139,6 @@ struct ExpandItem {
     int block0, blocks;             // its blocks inside block_indices
 };
 
-__device__ __forceinline__ int expand_heads_per_item(const ExpandedArgs& a) {
-    // enough items for every CTA to have a few, else as many heads as pay for bringing the context tile in
-    const long long all = (long long)a.tile_prefix[a.m.num_sequences] * a.heads;
-    return (int)min(8ll, max(1ll, all / (gridDim.x * 3ll)));
-}
-
 __device__ __forceinline__ ExpandItem expand_item(const ExpandedArgs& a, int i, int per) {
     const int head_groups = (a.heads + per - 1) / per, tile = i / head_groups;
     ExpandItem it;
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
     const Waiter wt{&sm.abort_flag, m.status};
-    const int per = expand_heads_per_item(a), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
+    const int per = min(*a.heads_per_item, a.heads), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
     constexpr uint32_t kD = R / 2;       // tensor memory: the rows (two elements a column), then 128 columns each for keys and values
 
     if (warp == 4 || warp == 6) {
@@ -569,9 +574,13 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                     auto issue_o = [&](int X, int j) {
                         const bool fresh = X == 0 || j >= it.tiles[0];
                         const uint32_t d = tmem + kO + X * DV;
+                        if (fresh) {
+                            Ring<VS> next = v[X];
+                            next.next();
+                            ok = ok && wt.spin_warp(&sm.v_full[v[X].at], v[X].phase) && wt.spin_warp(&sm.v_full[next.at], next.phase);
+                        }
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            if (fresh) ok = ok && wt.spin_warp(&sm.v_full[v[X].at], v[X].phase);
                             ok = ok && wt.spin_warp(&sm.p_full[X][u], np[X] & 1);
                             if (!ok) return;
                             tc05::fence_after_thread_sync();
@@ -679,9 +688,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                     uint32_t p[32];
 #pragma unroll
                     for (int c = 0; c < 64; c += 2) {
-                        const float x = ex2(fmaf(__uint_as_float(s[q + (c >> 5)][c & 31]), c2, ref)), y = ex2(fmaf(__uint_as_float(s[q + (c >> 5)][(c & 31) + 1]), c2, ref));
-                        sum[c & 2] += x;
-                        sum[(c & 2) + 1] += y;
+                        float x, y;
+                        fma2(x, y, __uint_as_float(s[q + (c >> 5)][c & 31]), __uint_as_float(s[q + (c >> 5)][(c & 31) + 1]), c2, ref);
+                        x = ex2(x);
+                        y = ex2(y);
+                        add2(sum[c & 2], sum[(c & 2) + 1], x, y);
                         p[c >> 1] = pack2<BF>(x, y);
                     }
                     tc05::st_32x32b_x32(tmem_s + 16 * q, p);

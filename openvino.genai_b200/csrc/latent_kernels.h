@@ -19,7 +19,14 @@ struct Step {
     const int32_t* block_indices;
     const int32_t* block_indices_begins;
     uint32_t* status;
+    int form;        // pa_latent_form
 };
+
+// Form of a sequence in an AUTO step.  With n new tokens over L tokens of context the absorbed form costs a n L and the expanded one b n L + c L, so the
+// number of new tokens decides: with 4 and with 16 sequences of 2000 cached tokens by 64 heads, 64 new tokens each took 169 us absorbed and 223
+// expanded, 96 took 245 and 223, 128 322 and 221.  Short contexts leave the absorbed form with more results than work (16 sequences of 64 tokens by
+// 16 heads 67 and 32 us).
+constexpr int kAutoMaxNew = 80, kAutoFewNew = 16, kAutoContext = 8;
 
 struct AppendArgs {
     Step m;
@@ -57,7 +64,6 @@ struct __align__(16) SliceStart {
 
 struct AbsorbedArgs {
     Step m;
-    int max_new;                // sequences with more new tokens are left to the expanded form
     int groups, row_tiles;
     long long* unit_prefix;     // [num_sequences + 1]
     int* block_prefix;          // [num_sequences + 1]
@@ -83,14 +89,14 @@ constexpr int kQueryTile = 256;    // new tokens of a work item, in two halves
 
 struct ExpandedArgs {
     Step m;
-    int min_new;                // sequences with fewer new tokens are left to the absorbed form
     int h0, heads;              // heads of this pass
     long long rows;             // rows of a head's scratch
     int* tile_prefix;           // [num_sequences + 1] context tiles
     int* query_prefix;          // [num_sequences + 1] query tiles
     int2* order;                // (sequence, query tile), longest context first
+    int* heads_per_item;        // heads that a CTA makes keys and values of for one context tile
     int* counter;               // [passes] work counters
-    int pass, passes;
+    int pass, passes, ctas;
     const void* cache;
     void* k_rope;               // [rows][64] rotated key part (the same for every head)
     void* output;
@@ -131,6 +137,11 @@ __device__ __forceinline__ bool seq_view(const Step& m, int s, SeqView& v) {
     }
     v = SeqView{t0, t1 - t0, past, tb};
     return true;
+}
+
+__device__ __forceinline__ bool takes_absorbed(const Step& m, const SeqView& v) {
+    if (m.form != PA_LATENT_AUTO) return m.form == PA_LATENT_ABSORBED;
+    return v.n <= kAutoFewNew || (v.n <= kAutoMaxNew && (long long)v.n * kAutoContext <= (long long)v.past + v.n);
 }
 
 // The sequence that owns token t.  In a step of one token each that is sequence t, which two loads show; else a binary search.

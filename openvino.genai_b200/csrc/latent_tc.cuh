@@ -133,6 +133,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two additions or multiply-adds by one instruction.
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float factor, float term) {
+    asm("{\n\t.reg .b64 s, f, t;\n\tmov.b64 s, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\tmov.b64 t, {%5, %5};\n\tfma.rn.f32x2 s, s, f, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(factor), "f"(term));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
