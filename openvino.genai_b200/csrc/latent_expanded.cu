@@ -379,10 +379,15 @@ struct ExpandedSmem {
     // Rings of key atoms (128 tokens x 64 elements, NQ of them a tile) and of value units (64 tokens): each is freed by itself, so that a
     // tile and a part of the next fit beside the queries
     static constexpr int KS = DN == 128 ? 5 : 4, VS = DN == 128 && DV == 128 ? 3 : DV == 128 ? 4 : 6;
+    // One barrier says that all of a tile is there.  There are as many as tiles can have begun to arrive: a loader that came back to one whose tile
+    // is still under way would count into the wrong phase.
+    static constexpr int TK = (KS + NQ - 1) / NQ, TV = (VS + 1) / 2;
+    static_assert(TK == 2, "the loader and the products take turns between two barriers");
     alignas(1024) uint8_t q[2][NQ][128 * 128];
     alignas(1024) uint8_t k[KS][kExpandTile * 128];
     alignas(1024) uint8_t v[VS][NV][64 * 128];
-    uint64_t q_full[2], q_free[2], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2][2], o_done[2];
+    uint64_t q_full[2], q_free[2], k_full[TK], k_free[KS], v_full[TV], v_free[VS];
+    uint64_t s_full[2], p_full[2][2], o_done[2];
     uint64_t item_full[kItemSlots], item_free[kItemSlots];
     QueryItem item[kItemSlots];
     uint32_t tmem_base;
@@ -394,7 +399,7 @@ template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setma
 template <int DN, int DV, bool BF>
 __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(const __grid_constant__ ExpandedArgs a) {
     using Smem = ExpandedSmem<DN, DV>;
-    constexpr int NQ = Smem::NQ, NV = Smem::NV, KS = Smem::KS, VS = Smem::VS;
+    constexpr int NQ = Smem::NQ, NV = Smem::NV, KS = Smem::KS, VS = Smem::VS, TV = Smem::TV;
     constexpr uint32_t kO = 256;       // S_A, S_B: 128 columns each (P in the first 64), then O_A, O_B
     extern __shared__ __align__(1024) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
@@ -403,14 +408,16 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
             pa::mbar_init(&sm.q_full[x], 1);
+            pa::mbar_init(&sm.k_full[x], 1);
             pa::mbar_init(&sm.q_free[x], 1);
             pa::mbar_init(&sm.s_full[x], 1);
             pa::mbar_init(&sm.p_full[x][0], 4);
             pa::mbar_init(&sm.p_full[x][1], 4);
             pa::mbar_init(&sm.o_done[x], 1);
         }
-        for (int i = 0; i < KS; ++i) { pa::mbar_init(&sm.k_full[i], 1); pa::mbar_init(&sm.k_free[i], 1); }
-        for (int i = 0; i < VS; ++i) { pa::mbar_init(&sm.v_full[i], 1); pa::mbar_init(&sm.v_free[i], 1); }
+        for (int i = 0; i < KS; ++i) pa::mbar_init(&sm.k_free[i], 1);
+        for (int i = 0; i < VS; ++i) pa::mbar_init(&sm.v_free[i], 1);
+        for (int i = 0; i < TV; ++i) pa::mbar_init(&sm.v_full[i], 1);
         for (int i = 0; i < kItemSlots; ++i) { pa::mbar_init(&sm.item_full[i], 1); pa::mbar_init(&sm.item_free[i], 10); }
         pa::mbar_fence_init();
         sm.abort_flag = 0;
@@ -468,7 +475,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 for (int x = 0; ok && x < 2; ++x) {
                     if (it.tiles[x] == 0) continue;
                     if (nq[x] > 0) ok = wt.wait_warp(&sm.q_free[x], (nq[x] - 1) & 1);
-                    if (ok && lane == 0) {
+                    if (ok && tc05::elect_one()) {
                         pa::mbar_expect_tx(&sm.q_full[x], NQ * 128 * 128);
                         for (int c = 0; c < NQ - 1; ++c) tma_3d(sm.q[x][c], &a.map_qn, 64 * c, a.h0 + it.h, it.t0 + 128 * x, &sm.q_full[x]);
                         tma_3d(sm.q[x][NQ - 1], &a.map_qr, 0, a.h0 + it.h, it.t0 + 128 * x, &sm.q_full[x]);
@@ -478,14 +485,15 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 }
                 const int y0 = (int)(it.h * a.rows) + it.row;
                 auto load_k = [&](int j) {
+                    uint64_t* full = &sm.k_full[nk / NQ & 1];
                     for (int c = 0; ok && c < NQ; ++c, ++nk) {
                         const int st = nk % KS;
                         if (nk >= KS) ok = wt.wait_warp(&sm.k_free[st], (nk / KS - 1) & 1);
                         if (!ok) return;
-                        if (lane == 0) {
-                            pa::mbar_expect_tx(&sm.k_full[st], kExpandTile * 128);
-                            if (c + 1 < NQ) tma_2d(sm.k[st], &a.map_k, 64 * c, y0 + j * kExpandTile, &sm.k_full[st]);
-                            else tma_2d(sm.k[st], &a.map_k_rope, 0, it.row + j * kExpandTile, &sm.k_full[st]);
+                        if (tc05::elect_one()) {
+                            if (c == 0) pa::mbar_expect_tx(full, NQ * kExpandTile * 128);
+                            if (c + 1 < NQ) tma_2d(sm.k[st], &a.map_k, 64 * c, y0 + j * kExpandTile, full);
+                            else tma_2d(sm.k[st], &a.map_k_rope, 0, it.row + j * kExpandTile, full);
                         }
                         __syncwarp();
                     }
@@ -493,12 +501,10 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 for (int j = 0; ok && j < tiles; ++j) load_k(j);
             }
             if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
-                auto drain = [&](uint64_t* bar, uint32_t parity) {
-                    for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(bar, parity); ++k) {}
-                };
                 for (int x = 0; x < 2; ++x)
                     if (nq[x] > 0) drain(&sm.q_full[x], (nq[x] - 1) & 1);
-                for (uint32_t i = nk > KS ? nk - KS : 0; i < nk; ++i) drain(&sm.k_full[i % KS], (i / KS) & 1);
+                const uint32_t n = (nk + NQ - 1) / NQ;      // (the last may have begun only: its wait ends by the time that a copy can take)
+                for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) drain(&sm.k_full[i & 1], (i >> 1) & 1);
             }
         } else if (warp == 10) {
             // ======================= loader of the values ====================================================
@@ -512,16 +518,18 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                     const int st = nv % VS;
                     if (nv >= VS) ok = wt.wait_warp(&sm.v_free[st], (nv / VS - 1) & 1);
                     if (!ok) break;
-                    if (lane == 0) {
-                        pa::mbar_expect_tx(&sm.v_full[st], NV * 64 * 128);
-                        for (int c = 0; c < NV; ++c) tma_2d(sm.v[st][c], &a.map_v, 64 * c, y0 + 64 * u, &sm.v_full[st]);
+                    uint64_t* full = &sm.v_full[nv / 2 % TV];
+                    if (tc05::elect_one()) {
+                        if ((u & 1) == 0) pa::mbar_expect_tx(full, 2 * NV * 64 * 128);
+                        for (int c = 0; c < NV; ++c) tma_2d(sm.v[st][c], &a.map_v, 64 * c, y0 + 64 * u, full);
                     }
                     __syncwarp();
                 }
             }
-            if (sm.abort_flag)
-                for (uint32_t i = nv > VS ? nv - VS : 0; i < nv; ++i)
-                    for (uint32_t k = 0; k < (1u << 20) && !pa::mbar_try_wait(&sm.v_full[i % VS], (i / VS) & 1); ++k) {}
+            if (sm.abort_flag) {
+                const uint32_t n = (nv + 1) / 2;
+                for (uint32_t i = n > TV ? n - TV : 0; i < n; ++i) drain(&sm.v_full[i % TV], (i / TV) & 1);
+            }
         } else if (warp == 9) {
             // ======================= products ============================================================
             // The whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took 110 cycles to issue in
@@ -534,26 +542,20 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 const bool wide = m.P == 64;
                 Ring<KS> k[2];           // where each half is in the rings
                 Ring<VS> v[2];
-                uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+                uint32_t nt = 0, nq[2] = {0, 0}, np[2] = {0, 0};     // context tiles before this item; query tiles, P tiles so far
                 bool ok = true;
+                QueryItem it;
                 for (uint32_t ni = 0; ok; ++ni) {
-                    const int slot = ni % kItemSlots;
-                    if (!wt.spin_warp(&sm.item_full[slot], (ni / kItemSlots) & 1)) break;
-                    const QueryItem it = sm.item[slot];
-                    warp_arrive(&sm.item_free[slot]);
-                    if (it.h < 0) break;
+                    if (!fetch(ni, it) || it.h < 0) break;
                     const int tiles = max(it.tiles[0], it.tiles[1]);
                     const int last_half = it.tiles[1] > 0 ? 1 : 0;      // B sees no fewer tiles than A, where it has rows
+                    // S of tile j (whose keys are there), by the elected lane
                     auto issue_s = [&](int X, int j) {
-                        const bool fresh = X == 0 || j >= it.tiles[0];  // (else A has waited for these keys)
                         const uint32_t d = tmem + X * 128;
+                        Ring<KS> at = k[X];
 #pragma unroll
-                        for (int c = 0; c < NQ; ++c) {
-                            if (fresh) ok = ok && wt.spin_warp(&sm.k_full[k[X].at], k[X].phase);
-                            if (!ok) return;
-                            tc05::fence_after_thread_sync();
-                            const uint32_t da = dq + (X * NQ + c) * kAtom, db = dk + k[X].at * kAtom;
-                            if (tc05::elect_one()) {
+                        for (int c = 0; c < NQ; ++c, at.next()) {
+                            const uint32_t da = dq + (X * NQ + c) * kAtom, db = dk + at.at * kAtom;
                             if (c == 0) mma_ss<0>(d, da, db, idesc_s);
                             else mma_ss<1>(d, da, db, idesc_s);
                             mma_ss<1>(d, da + 2, db + 2, idesc_s);
@@ -561,66 +563,68 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                                 mma_ss<1>(d, da + 4, db + 4, idesc_s);
                                 mma_ss<1>(d, da + 6, db + 6, idesc_s);
                             }
-                            if (X == last_half) tc05::commit(&sm.k_free[k[X].at]);
-                            if (c + 1 == NQ) {
-                                tc05::commit(&sm.s_full[X]);
-                                if (j + 1 == it.tiles[X]) tc05::commit(&sm.q_free[X]);
-                            }
-                            }
-                            __syncwarp();
-                            k[X].next();
+                            if (X == last_half) tc05::commit(&sm.k_free[at.at]);
                         }
+                        tc05::commit(&sm.s_full[X]);
+                        if (j + 1 == it.tiles[X]) tc05::commit(&sm.q_free[X]);
                     };
-                    auto issue_o = [&](int X, int j) {
-                        const bool fresh = X == 0 || j >= it.tiles[0];
-                        const uint32_t d = tmem + kO + X * DV;
-                        if (fresh) {
-                            Ring<VS> next = v[X];
-                            next.next();
-                            ok = ok && wt.spin_warp(&sm.v_full[v[X].at], v[X].phase) && wt.spin_warp(&sm.v_full[next.at], next.phase);
-                        }
+                    auto past_keys = [&](int X) {
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            ok = ok && wt.spin_warp(&sm.p_full[X][u], np[X] & 1);
-                            if (!ok) return;
-                            tc05::fence_after_thread_sync();
-                            const uint32_t p = tmem + X * 128 + u * 32, db = dv + v[X].at * kUnit;
-                            if (tc05::elect_one()) {
-                            if (u == 0 && j == 0) mma_ts<0>(d, p, db, idesc_o);
-                            else mma_ts<1>(d, p, db, idesc_o);
-#pragma unroll
-                            for (int kk = 1; kk < 4; ++kk) mma_ts<1>(d, p + kk * 8, db + kk * 128, idesc_o);
-                            if (X == last_half) tc05::commit(&sm.v_free[v[X].at]);
-                            if (u == 1 && j + 1 == it.tiles[X]) tc05::commit(&sm.o_done[X]);
-                            }
-                            __syncwarp();
-                            v[X].next();
-                        }
-                        ++np[X];
+                        for (int c = 0; c < NQ; ++c) k[X].next();
                     };
 #pragma unroll
                     for (int X = 0; X < 2; ++X)
                         if (ok && it.tiles[X] > 0) {
-                            ok = wt.spin_warp(&sm.q_full[X], nq[X] & 1);
+                            ok = wt.spin_warp(&sm.q_full[X], nq[X] & 1) && wt.spin_warp(&sm.k_full[nt & 1], (nt >> 1) & 1);
                             ++nq[X];
-                            if (ok) issue_s(X, 0);
+                            tc05::fence_after_thread_sync();
+                            if (ok && tc05::elect_one()) issue_s(X, 0);
+                            __syncwarp();
+                            past_keys(X);
                         }
                     for (int j = 0; ok && j < tiles; ++j) {
 #pragma unroll
                         for (int X = 0; X < 2; ++X)
                             if (ok && j < it.tiles[X]) {
-                                issue_o(X, j);
-                                if (ok && j + 1 < it.tiles[X]) issue_s(X, j + 1);
+                                // what the loaders bring is waited for first (by A for B too, where both see the tile); the probabilities come later, and
+                                // nothing stands between them and their products
+                                const bool more = j + 1 < it.tiles[X];
+                                const uint32_t n = nt + j;
+                                if (X == 0 || j >= it.tiles[0]) ok = wt.spin_warp(&sm.v_full[n % TV], (n / TV) & 1);
+                                if (ok && more && (X == 0 || j + 1 >= it.tiles[0])) ok = wt.spin_warp(&sm.k_full[(n + 1) & 1], ((n + 1) >> 1) & 1);
+                                const uint32_t d = tmem + kO + X * DV, p = tmem + X * 128;
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    if (ok) ok = wt.spin_warp(&sm.p_full[X][u], np[X] & 1);
+                                    if (!ok) break;
+                                    tc05::fence_after_thread_sync();
+                                    const uint32_t db = dv + v[X].at * kUnit;
+                                    if (tc05::elect_one()) {
+                                        if (u == 0 && j == 0) mma_ts<0>(d, p + u * 32, db, idesc_o);
+                                        else mma_ts<1>(d, p + u * 32, db, idesc_o);
+#pragma unroll
+                                        for (int kk = 1; kk < 4; ++kk) mma_ts<1>(d, p + u * 32 + kk * 8, db + kk * 128, idesc_o);
+                                        if (X == last_half) tc05::commit(&sm.v_free[v[X].at]);
+                                        if (u == 1) {
+                                            if (more) issue_s(X, j + 1);
+                                            else tc05::commit(&sm.o_done[X]);
+                                        }
+                                    }
+                                    __syncwarp();
+                                    v[X].next();
+                                }
+                                ++np[X];
+                                if (more) past_keys(X);
                             }
                     }
 #pragma unroll
                     for (int X = 0; X < 2; ++X)      // past the tiles that only the other half sees
                         for (int j = it.tiles[X]; j < tiles; ++j) {
-#pragma unroll
-                            for (int c = 0; c < NQ; ++c) k[X].next();
+                            past_keys(X);
                             v[X].next();
                             v[X].next();
                         }
+                    nt += tiles;
                 }
             }
         }
@@ -639,6 +643,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             if (tiles == 0) continue;
             const int i = 128 * X + r;                      // row of the item
             const int limit = i < it.rows ? it.past + i + 1 : 0;
+            const int least = __reduce_min_sync(0xffffffffu, limit);
             float top = -INFINITY, l = 0.f;
             bool ok = true;
             for (int j = 0; j < tiles; ++j, ++n) {
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 for (int q = 0; q < 4; ++q) tc05::ld_32x32b_x32(tmem_s + 32 * q, s[q]);
                 tc05::wait_ld();
                 const int seen = limit - j * kExpandTile;
-                if (__any_sync(0xffffffffu, seen < kExpandTile)) {
+                if ((j + 1) * kExpandTile > least) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll

@@ -100,6 +100,11 @@ struct Waiter {
     }
 };
 
+// After an abort: until what was issued on `bar` has arrived, or a millisecond or two, which no copy takes
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    for (int k = 0; k < 4096 && !mbar_test(bar, parity); ++k) __nanosleep(400);
+}
+
 // Operand descriptors of 128-byte-swizzled tiles whose 8-row groups are GROUP bytes apart.  Their high words are constants, so only the low
 // word (address and, for operands whose rows run along M or N, the distance of 64-element atoms) is carried along; a step is an addition.
 __host__ __device__ constexpr uint32_t desc_high(uint32_t group_bytes) { return (group_bytes >> 4) | (1u << 14) | (2u << 29); }
