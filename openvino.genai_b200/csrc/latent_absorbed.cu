@@ -207,8 +207,11 @@ struct AttendSmem {
     static constexpr int NST = R == 512 ? 2 : 4;    // context tiles in flight
     alignas(1024) uint8_t q[kTile * R * 2];
     alignas(1024) uint8_t q_rope[kTile * 128];
+    // A tile is loaded, multiplied and freed in parts of 128 latent elements (64 tokens each), so that the next tile's parts arrive while the
+    // others of this one are still being multiplied, and S begins with the first
+    static constexpr int NQ = R / 128;
     struct Tile {
-        uint8_t c[kTokens * R * 2];
+        uint8_t c[NQ][kTokens * 256];               // [token / 8][element / 64][token % 8]
         uint8_t rope[kTokens * 128];
     };
     alignas(1024) Tile k[NST];
@@ -217,7 +220,7 @@ struct AttendSmem {
     float2 stat[2][kTile];                          // maximum and sum of the rows of a run
     volatile uint32_t grew[2];                      // the last tile (+ 1) in which a row's maximum grew
     volatile int event;                             // what the results warps are asked for: rescale after tile `event` - 1, or results (0)
-    uint64_t k_full[NST][2], k_free[NST][2];        // halves of tiles: loader -> products (bytes), products -> loader
+    uint64_t k_full[NST][NQ], k_free[NST][NQ];      // parts of tiles: loader -> products (bytes), products -> loader
     uint64_t q_full, q_free;
     uint64_t s_full[2], s_free[2];                  // products -> softmax, softmax -> products
     uint64_t p_full, o_done;                        // softmax -> products, products -> softmax and results
@@ -234,15 +237,16 @@ struct AttendSmem {
 template <int R, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AbsorbedArgs a) {
     using Smem = AttendSmem<R>;
-    constexpr int NC = R / 64, NST = Smem::NST, MT = R / 128;
-    constexpr uint32_t kGroup = NC * 1024;          // bytes from one group of eight tokens to the next
+    constexpr int NST = Smem::NST, NQ = Smem::NQ, MT = NQ;
+    constexpr uint32_t kGroup = 2048;               // bytes from one group of eight tokens of a part to the next
+    constexpr uint32_t kPart = kTokens * 256;
     constexpr uint32_t kTmemS = MT * kTile;         // O^T: MT x 64 columns, then S twice
     extern __shared__ __align__(1024) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < 2 * NST; ++i) { pa::mbar_init(&sm.k_full[0][i], 1); pa::mbar_init(&sm.k_free[0][i], 1); }
+        for (int i = 0; i < NQ * NST; ++i) { pa::mbar_init(&sm.k_full[0][i], 1); pa::mbar_init(&sm.k_free[0][i], 1); }
         pa::mbar_init(&sm.q_full, 1);
         pa::mbar_init(&sm.q_free, 1);
         for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.s_full[i], 1); pa::mbar_init(&sm.s_free[i], 4); pa::mbar_init(&sm.stat_full[i], 4); }
@@ -345,19 +349,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                         const int st = n % NST;
                         int group[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) group[i] = group_of(p0 + min(i, 2 * pieces - 1));
+                        for (int i = 0; i < 4; ++i) group[i] = group_of(min(p0 + min(i, 2 * pieces - 1), last_piece));
+                        const int count = min(2 * pieces, last_piece - p0 + 1);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int count = max(0, min(pieces, last_piece - (p0 + half * pieces) + 1));
-                            if (ok && n >= NST) ok = wt.wait_warp(&sm.k_free[st][half], (n / NST - 1) & 1);
+                        for (int q = 0; q < NQ; ++q) {
+                            if (n >= NST) ok = ok && wt.wait_warp(&sm.k_free[st][q], (n / NST - 1) & 1);
                             if (!ok) break;
                             if (tc05::elect_one()) {
-                                pa::mbar_expect_tx(&sm.k_full[st][half], count * piece * (R * 2 + 128));
-                                for (int i = 0; i < count; ++i) {
-                                    const int row = half * 32 + i * piece, g = pieces == 1 ? group[half] : i == 0 ? group[2 * half] : group[2 * half + 1];
-                                    tma_4d(sm.k[st].c + (row >> 3) * kGroup, &a.map_cache, 0, 0, 0, g, &sm.k_full[st][half], policy);
-                                    tma_3d(sm.k[st].rope + row * 128, &a.map_cache_rope, 0, 0, g, &sm.k_full[st][half], policy);
-                                }
+                                pa::mbar_expect_tx(&sm.k_full[st][q], count * piece * (q + 1 == NQ ? 256 + 128 : 256));
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (i < count) {
+                                        tma_4d(sm.k[st].c[q] + i * piece * 256, &a.map_cache_part, 0, 0, 2 * q, group[i], &sm.k_full[st][q], policy);
+                                        if (q + 1 == NQ) tma_3d(sm.k[st].rope + i * piece * 128, &a.map_cache_rope, 0, 0, group[i], &sm.k_full[st][q], policy);
+                                    }
                             }
                             __syncwarp();
                         }
@@ -386,9 +391,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
         // what was issued has to have arrived before the CTA's memory is given back
         if (sm.abort_flag) {
-            for (uint32_t k = 0; nq > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.q_full, (nq - 1) & 1); ++k) {}
-            for (uint32_t i = n > NST ? n - NST : 0; i < n; ++i)
-                for (uint32_t k = 0; k < (1u << 20) && !(pa::mbar_try_wait(&sm.k_full[i % NST][0], (i / NST) & 1) && pa::mbar_try_wait(&sm.k_full[i % NST][1], (i / NST) & 1)); ++k) {}
+            if (nq > 0) drain(&sm.q_full, (nq - 1) & 1);
+            for (uint32_t i = n + 1 > NST ? n + 1 - NST : 0; i <= n; ++i)      // (of tile n a part may be under way)
+                for (int q = 0; q < NQ; ++q) drain(&sm.k_full[i % NST][q], (i / NST) & 1);
         }
     } else if (warp == 5) {
         // ======================= S ========================================================================
@@ -407,20 +412,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             ++nq;
             for (int j = 0; ok && j < r.tiles; ++j, ++n) {
                 const int st = n % NST;
-                ok = (n < 2 || wt.spin_warp(&sm.s_free[n & 1], ((n >> 1) - 1) & 1)) && wt.spin_warp(&sm.k_full[st][0], (n / NST) & 1) &&
-                     wt.spin_warp(&sm.k_full[st][1], (n / NST) & 1);
-                if (!ok) break;
+                ok = n < 2 || wt.spin_warp(&sm.s_free[n & 1], ((n >> 1) - 1) & 1);
                 const uint32_t db = dk + st * kStage, dbr = dkr + st * kStage, d = tmem + kTmemS + (n & 1) * kTokens;
-                tc05::fence_after_thread_sync();
-                if (tc05::elect_one()) {
-#pragma unroll 4
-                    for (int c = 0; c < NC; ++c) {
-                        const uint32_t qa = dq + c * (kTile * 128 >> 4), kb = db + c * (1024 >> 4);
-                        if (c == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
-                        else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
 #pragma unroll
-                        for (int kk = 1; kk < 4; ++kk) mma_ss<1, 1024, kGroup>(d, qa + kk * 2, kb + kk * 2, idesc_s);
+                for (int q = 0; q < NQ; ++q) {
+                    ok = ok && wt.spin_warp(&sm.k_full[st][q], (n / NST) & 1);
+                    if (!ok) break;
+                    tc05::fence_after_thread_sync();
+                    if (tc05::elect_one()) {
+#pragma unroll
+                        for (int c = 2 * q; c < 2 * q + 2; ++c) {
+                            const uint32_t qa = dq + c * (kTile * 128 >> 4), kb = db + q * (kPart >> 4) + (c & 1) * (1024 >> 4);
+                            if (c == 0) mma_ss<0, 1024, kGroup>(d, qa, kb, idesc_s);
+                            else mma_ss<1, 1024, kGroup>(d, qa, kb, idesc_s);
+#pragma unroll
+                            for (int kk = 1; kk < 4; ++kk) mma_ss<1, 1024, kGroup>(d, qa + kk * 2, kb + kk * 2, idesc_s);
+                        }
                     }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (tc05::elect_one()) {
                     mma_ss<1>(d, dqr, dbr, idesc_s);
                     mma_ss<1>(d, dqr + 2, dbr + 2, idesc_s);
                     if (wide) {
@@ -459,16 +471,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 const uint32_t da = dv + n % NST * kStage;
                 if (tc05::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < kTokens / 16; ++kk) {
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const uint32_t d = tmem + mt * kTile;
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            const uint32_t d = tmem + mt * kTile, pa = da + mt * (2048 >> 4) + kk * (2 * kGroup >> 4);
+                        for (int kk = 0; kk < kTokens / 16; ++kk) {
+                            const uint32_t pa = da + mt * (kPart >> 4) + kk * (2 * kGroup >> 4);
                             if (kk == 0 && j == 0) mma_ss<0, kGroup>(d, pa, dp, idesc_o);
                             else mma_ss<1, kGroup>(d, pa, dp + kk * 2, idesc_o);
                         }
-                        if (kk == kTokens / 32 - 1) tc05::commit(&sm.k_free[n % NST][0]);
+                        tc05::commit(&sm.k_free[n % NST][mt]);
                     }
-                    tc05::commit(&sm.k_free[n % NST][1]);
                     tc05::commit(&sm.o_done);
                 }
                 __syncwarp();
@@ -604,12 +616,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                     // tokens behind the context: whatever lies there (stale bytes, not-a-number) meets probabilities of zero, which does not
                     // make it zero, so the latents are cleared
                     const int st = n % NST, valid = r.end - col0;
-                    if (!wt.wait_warp(&sm.k_full[st][0], (n / NST) & 1) || !wt.wait_warp(&sm.k_full[st][1], (n / NST) & 1)) { ok = false; break; }
+                    for (int q = 0; ok && q < NQ; ++q) ok = wt.wait_warp(&sm.k_full[st][q], (n / NST) & 1);
+                    if (!ok) break;
                     for (int i = tid; i < (kTokens - valid) * 8; i += 128) {
                         const int row = valid + i / 8;
 #pragma unroll
-                        for (int c = 0; c < NC; ++c)
-                            *reinterpret_cast<uint4*>(sm.k[st].c + (row >> 3) * kGroup + c * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int c = 0; c < 2 * NQ; ++c)
+                            *reinterpret_cast<uint4*>(sm.k[st].c[c >> 1] + (row >> 3) * kGroup + (c & 1) * 1024 + (row & 7) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 tc05::fence_proxy_async_smem();

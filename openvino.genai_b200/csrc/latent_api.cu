@@ -277,11 +277,11 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         const long long ca_size[4] = {64, 8, R / 64, groups}, ca_stride[3] = {W, 64, 8 * W}, cr_size[3] = {P, 8, groups}, cr_stride[2] = {W, 8 * W};
         const long long qa_size[3] = {64, (long long)T * H, R / 64}, qa_stride[2] = {W, 64}, qr_size[2] = {P, (long long)T * H}, qr_stride[1] = {W};
         const int box_tokens[3] = {64, 1, latent::kTile}, box_ku[3] = {64, d.nope_size, 1}, box_vu[3] = {64, d.value_size, 1};
-        const int box_q[3] = {64, latent::kTile, R / 64}, box_qr[2] = {64, latent::kTile}, box_c[4] = {64, 8, R / 64, std::min(d.block_size, latent::kTokens / 2) / 8}, box_cr[3] = {64, 8, box_c[3]};
+        const int box_q[3] = {64, latent::kTile, R / 64}, box_qr[2] = {64, latent::kTile}, box_c[4] = {64, 8, R / 64, std::min(d.block_size, latent::kTokens / 2) / 8}, box_cr[3] = {64, 8, box_c[3]}, box_cp[4] = {64, 8, 2, box_c[3]};
         if (!make_map(&k.map_qn, d.dtype, a->query_nope, 3, qn_size, qn_stride, box_tokens) || !make_map(&k.map_key_up, d.dtype, a->key_up, 3, ku_size, ku_stride, box_ku) ||
             !make_map(&k.map_value_up, d.dtype, a->value_up, 3, vu_size, vu_stride, box_vu) || !make_map(&k.map_q_abs, d.dtype, k.q_abs, 3, qa_size, qa_stride, box_q) ||
             !make_map(&k.map_q_abs_rope, d.dtype, (const uint16_t*)k.q_abs + R, 2, qr_size, qr_stride, box_qr) ||
-            !make_map(&k.map_cache, d.dtype, a->cache, 4, ca_size, ca_stride, box_c) || !make_map(&k.map_cache_rope, d.dtype, (const uint16_t*)a->cache + R, 3, cr_size, cr_stride, box_cr))
+            !make_map(&k.map_cache, d.dtype, a->cache, 4, ca_size, ca_stride, box_c) || !make_map(&k.map_cache_part, d.dtype, a->cache, 4, ca_size, ca_stride, box_cp) || !make_map(&k.map_cache_rope, d.dtype, (const uint16_t*)a->cache + R, 3, cr_size, cr_stride, box_cr))
             return fail(PA_ERR_CUDA, "a tensor map could not be made");
         LATENT_CUDA(latent::launch_absorbed(k, d.dtype, stream, &launches));
     }

@@ -76,7 +76,7 @@ struct AbsorbedArgs {
     int2* row_part;             // [num_tokens * H] a row's first partial result (slot * 64 + row of the tile) and how many it has
     void* output;
     float scale_log2;           // softmax scale * log2(e)
-    CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_rope, map_value_up;
+    CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_part, map_cache_rope, map_value_up;
 };
 // Largest number of slots a step can need.
 long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);
