@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
     }
     if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
     pa::grid_wait();
+    pa::grid_release();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -649,8 +650,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
 // A CTA joins the partial results of one head's rows of NT tokens and computes their output: D[value][token], K = R twice, because the joined sums
 // go in as two 16-bit pieces (high and low), so that the product does not see another rounding.  Few tokens take tiles of 16, so
 // that there are CTAs enough to join their rows.
-// Bound by the chain record -> statistics -> partial results -> product -> output for few tokens (one row 8 us behind its predecessor; joining in a
-// kernel of its own took 7 us more, and 38 where 74 CTAs had a part of one row), by the partial results' bytes for many.
+// Bound by the chain row -> record -> statistics -> partial results -> product -> output, not by the partial results' bytes (22 MB for 96 rows by
+// 16 heads of up to 15 pieces, in 7 us).  So a row belongs to a warp from its record to its place in shared memory, with the pieces of the statistics
+// dealt over the lanes and the first pieces under way before their weights: the same call took 67.5 us with the pieces of one row after another
+// dealt over the block, 50.0 so.  Joining in a kernel of its own took 7 us more than either.
 constexpr int kJoinWarps = 16, kJoinThreads = 32 * kJoinWarps;
 constexpr int kValueThreads = kJoinThreads + 32;     // warps 0 - 15: joining, then (0 - 3) output; 16: weights and products
 
@@ -660,7 +663,6 @@ struct ValueSmem {
     alignas(1024) uint8_t o[2][NC][NT * 128];                    // joined rows, high and low pieces
     alignas(1024) uint8_t w[NW][128 * 128];
     uint64_t w_full[NW], w_free[NW], o_full, done;
-    struct Row { int first, pieces; float top, inv, k0, k1; } row[NT];   // first partial row, how many, their maximum, 1 / denominator, weights of the first two
     bool live[NT];
     uint32_t tmem_base;
     int abort_flag;
@@ -681,28 +683,33 @@ __global__ void __launch_bounds__(kValueThreads) project_value_kernel(const __gr
         pa::mbar_init(&sm.done, 1);
         pa::mbar_fence_init();
         sm.abort_flag = 0;
-        for (int c = 0; c < NC; ++c) prefetch_3d(&a.map_value_up, c * 64, 0, h);
     }
-    if (warp == kJoinWarps) tc05::tmem_alloc(&sm.tmem_base, 64);
+    // (what does not come from the kernel before: its CTAs have all begun, so what precedes them is complete)
+    if (!tile_rows(a, t0, sm.live)) {
+        pa::grid_wait();
+        return;
+    }
+    auto load_weights = [&](int c) {
+        if (tc05::elect_one()) {
+            pa::mbar_expect_tx(&sm.w_full[c % NW], m.Dv * 128);
+            tma_3d(sm.w[c % NW], &a.map_value_up, c * 64, 0, h, &sm.w_full[c % NW]);
+        }
+        __syncwarp();
+    };
+    if (warp == kJoinWarps) {
+        tc05::tmem_alloc(&sm.tmem_base, 64);
+        for (int c = 0; c < min(NW, NC); ++c) load_weights(c);
+    }
     pa::grid_wait();
     tc05::fence_before_thread_sync();
-    const bool any = tile_rows(a, t0, sm.live);
+    __syncthreads();
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
     const Waiter wt{&sm.abort_flag, m.status};
-    if (!any) {
-        // (nothing to do for these tokens)
-    } else if (warp == kJoinWarps) {
+    if (warp == kJoinWarps) {
         bool ok = true;
         const uint32_t idesc = tc05::instr_desc_f16(m.Dv, NT, BF ? 1 : 0, 0, 0), dw = desc_low(sm.w), doh = desc_low(sm.o[0]), dol = desc_low(sm.o[1]);
-        auto load = [&](int c) {
-            if (tc05::elect_one()) {
-                pa::mbar_expect_tx(&sm.w_full[c % NW], m.Dv * 128);
-                tma_3d(sm.w[c % NW], &a.map_value_up, c * 64, 0, h, &sm.w_full[c % NW]);
-            }
-            __syncwarp();
-        };
-        for (int c = 0; c < NW; ++c) load(c);
+        int loaded = min(NW, NC);
         ok = wt.wait_warp(&sm.o_full, 0);
         for (int c = 0; ok && c < NC; ++c) {
             ok = wt.wait_warp(&sm.w_full[c % NW], (c / NW) & 1);
@@ -722,111 +729,124 @@ __global__ void __launch_bounds__(kValueThreads) project_value_kernel(const __gr
             __syncwarp();
             if (c + NW < NC) {
                 ok = wt.wait_warp(&sm.w_free[c % NW], (c / NW) & 1);
-                if (ok) load(c + NW);
+                if (ok) { load_weights(c + NW); ++loaded; }
             }
         }
+        if (!ok)
+            for (int c = max(0, loaded - NW); c < loaded; ++c) drain(&sm.w_full[c % NW], (c / NW) & 1);
     } else {
         const int step = a.row_tiles * kTile;        // from a row's partial result to the next
-        // a warp per row: the pieces' common maximum, and the denominator
-        for (int r = warp; r < NT; r += kJoinWarps) {
-            typename Smem::Row row{0, 0, 0.f, 0.f, 0.f, 0.f};
-            if (sm.live[r]) {
-                const int2 part = a.row_part[(long long)(t0 + r) * m.H + h];
-                row.first = part.x;
-                row.pieces = part.y;
-                float2 mine = make_float2(-INFINITY, 0.f);
-                float top = -INFINITY, sum = 0.f;
-                for (int i = lane; i < part.y; i += 32) {
-                    const float2 ml = a.part_ml[part.x + (long long)i * step];
-                    if (i == lane) mine = ml;
-                    if (ml.y > 0.f) {                // (a piece whose tiles the row does not see has no sums)
-                        const float t = fmaxf(top, ml.x);
-                        sum = sum * ex2(top - t) + ml.y * ex2(ml.x - t);
-                        top = t;
-                    }
-                }
-                row.top = pa::warp_max(top);
-                row.inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - row.top));
-                const float k = mine.y > 0.f ? ex2(mine.x - row.top) * row.inv : 0.f;
-                row.k0 = __shfl_sync(0xffffffffu, k, 0);
-                row.k1 = __shfl_sync(0xffffffffu, k, 1);
-            }
-            if (lane == 0) sm.row[r] = row;
-        }
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kJoinThreads) : "memory"); };   // (the joining warps; none of them can have left)
-        meet();
-        constexpr int kPer = R / 4, kAtOnce = kJoinThreads / kPer;   // threads of a row, four latent elements each; rows at a time
-        const int e = tid % kPer;
-        auto load = [&](const typename Smem::Row& row, int i) { return *reinterpret_cast<const float4*>(a.part_o + (row.first + (long long)i * step) * R + 4 * e); };
-        auto add = [](float (&y)[4], float k, const float4& p) { y[0] += k * p.x; y[1] += k * p.y; y[2] += k * p.z; y[3] += k * p.w; };
-        auto weight = [&](const typename Smem::Row& row, int i) {
-            const float2 ml = a.part_ml[row.first + (long long)i * step];
-            return ml.y > 0.f ? ex2(ml.x - row.top) * row.inv : 0.f;
-        };
-        auto store = [&](int r, const float (&y)[4]) {
+        // element quad `e` of row `r`, swizzled by the row
+        auto store = [&](int r, int e, const float (&y)[4]) {
             uint32_t hi[2], lo[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
                 lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
             }
-            const uint32_t at = r * 128 + (((e % 16 >> 1) ^ (r & 7)) << 4) + (e & 1) * 8;      // swizzled by the row
+            const uint32_t at = r * 128 + (((e % 16 >> 1) ^ (r & 7)) << 4) + (e & 1) * 8;
             *reinterpret_cast<uint2*>(sm.o[0][e / 16] + at) = make_uint2(hi[0], hi[1]);
             *reinterpret_cast<uint2*>(sm.o[1][e / 16] + at) = make_uint2(lo[0], lo[1]);
         };
-        if (NT == 16 && sm.row[0].pieces > 8) {
-            // few rows of many pieces: all threads on a row, its pieces dealt out
-            __shared__ float4 sh[kAtOnce][kPer];
-            for (int r = 0; r < NT; ++r) {
-                const typename Smem::Row row = sm.row[r];
-                float y[4] = {0.f, 0.f, 0.f, 0.f};
-                if (row.pieces > 0) {
-#pragma unroll 8
-                    for (int i = tid / kPer; i < row.pieces; i += kAtOnce) {
-                        const float k = weight(row, i);
-                        const float4 p = load(row, i);
-                        if (k != 0.f) add(y, k, p);
-                    }
-                    sh[tid / kPer][e] = make_float4(y[0], y[1], y[2], y[3]);
-                    meet();
-                    if (tid < kPer) {
+        // A warp has a row (of 64: one of every sixteen), or rows that are fewer than the warps have several each, which deal out the pieces.
+        // A lane has four elements of every 128, and the statistics of one of 32 pieces; the first pieces are under way before their weights are known.
+        constexpr int V = R / 128, kRows = NT / kJoinWarps, U = NT == 16 ? 4 : 2;
+        int rows = NT, spread = 0;
+        if (NT == 16) {
+            rows = 32 - __clz(__ballot_sync(0xffffffffu, lane < NT && sm.live[lane % NT]));
+            spread = 4 - (32 - __clz(rows - 1));
+        }
+        const int each = 1 << spread, mine = warp & (each - 1);
+        int2 part[kRows];
+        float2 ml[kRows];
+        float4 p[2][U][V];
 #pragma unroll
-                        for (int d = 1; d < kAtOnce; ++d) add(y, 1.f, sh[d][e]);
-                    }
-                    meet();
+        for (int u = 0; u < kRows; ++u) {
+            const int r = (warp >> spread) + u * kJoinWarps;
+            part[u] = sm.live[r] ? a.row_part[(long long)(t0 + r) * m.H + h] : make_int2(0, 0);
+        }
+        auto load = [&](float4 (&q)[V], const int2& row, int piece) {
+            const float4* src = reinterpret_cast<const float4*>(a.part_o + (row.x + (long long)piece * step) * R) + lane;
+#pragma unroll
+            for (int v = 0; v < V; ++v) q[v] = src[32 * v];
+        };
+        auto first = [&](int u) {
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+                if (mine + k * each < part[u].y) load(p[u & 1][k], part[u], mine + k * each);
+        };
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) ml[u] = lane < part[u].y ? a.part_ml[part[u].x + (long long)lane * step] : make_float2(-INFINITY, 0.f);
+        first(0);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int r = (warp >> spread) + u * kJoinWarps, pieces = part[u].y;
+            if (u + 1 < kRows) first(u + 1);
+            // the pieces' common maximum, and the denominator (a piece whose tiles the row does not see has no sums)
+            float top = ml[u].y > 0.f ? ml[u].x : -INFINITY, sum = ml[u].y > 0.f ? ml[u].y : 0.f;
+            for (int i = lane + 32; i < pieces; i += 32) {
+                const float2 other = a.part_ml[part[u].x + (long long)i * step];
+                if (other.y > 0.f) {
+                    const float t = fmaxf(top, other.x);
+                    sum = (top == -INFINITY ? 0.f : sum * ex2(top - t)) + other.y * ex2(other.x - t);
+                    top = t;
                 }
-                if (tid < kPer) store(r, y);
             }
-        } else {
-            // four rows a thread, two pieces of each under way together (most rows have no more)
-            for (int r0 = tid / kPer; r0 < NT; r0 += 4 * kAtOnce) {
-                float y[4][4] = {};
-                int most = 0;
+            const float most = pa::warp_max(top), inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - most));
+            float y[V][4] = {};
+            for (int base = 0; base < pieces; base += 32 * each) {
+                const int i = base + mine + lane * each, count = min(32, (pieces - base - mine + each - 1) >> spread);
+                float2 own = ml[u];
+                if (base > 0 || each > 1) own = i < pieces ? a.part_ml[part[u].x + (long long)i * step] : make_float2(-INFINITY, 0.f);
+                const float weight = own.y > 0.f ? ex2(own.x - most) * inv : 0.f;
+                for (int j = 0; j < count; j += U) {
+                    if (base + j > 0) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (r0 + u * kAtOnce < NT) most = max(most, sm.row[r0 + u * kAtOnce].pieces);
-                for (int i = 0; i < most; i += 2) {
-                    float4 p[4][2];
-                    float k[4][2];
+                        for (int k = 0; k < U; ++k)
+                            if (j + k < count) load(p[u & 1][k], part[u], base + mine + (j + k) * each);
+                    }
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = r0 + u * kAtOnce;
-                        const int left = r < NT ? sm.row[r].pieces - i : 0;
+                    for (int k = 0; k < U; ++k) {
+                        const float f = __shfl_sync(0xffffffffu, weight, j + k);
+                        if (f != 0.f) {      // (a piece without sums has no results either)
 #pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            p[u][v] = left > v ? load(sm.row[r], i + v) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            k[u][v] = left > v ? (i == 0 ? (v ? sm.row[r].k1 : sm.row[r].k0) : weight(sm.row[r], i + v)) : 0.f;
+                            for (int v = 0; v < V; ++v) {
+                                const float4& q = p[u & 1][k][v];
+                                y[v][0] += f * q.x; y[v][1] += f * q.y; y[v][2] += f * q.z; y[v][3] += f * q.w;
+                            }
                         }
                     }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-#pragma unroll
-                        for (int v = 0; v < 2; ++v)
-                            if (k[u][v] != 0.f) add(y[u], k[u][v], p[u][v]);      // (a piece without sums has no results either)
                 }
+            }
+            if (each == 1) {
+                if (pieces > 0) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (r0 + u * kAtOnce < NT) store(r0 + u * kAtOnce, y[u]);
+                    for (int v = 0; v < V; ++v) store(r, lane + 32 * v, y[v]);
+                }
+            } else {
+                // the sums of a row's warps, in turn where the rows will be
+                float4* sums = reinterpret_cast<float4*>(sm.o);
+                static_assert(NT != 16 || sizeof(sm.o) == kJoinWarps * R * 4, "");
+#pragma unroll
+                for (int v = 0; v < V; ++v) sums[warp * (R / 4) + lane + 32 * v] = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
+                meet();
+                float z[2][4] = {};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {      // (at most eight rows)
+                    const int unit = tid + x * kJoinThreads;
+                    if (unit < rows * (R / 4))
+                        for (int k = 0; k < each; ++k) {
+                            const float4 q = sums[((unit / (R / 4) << spread) + k) * (R / 4) + unit % (R / 4)];
+                            z[x][0] += q.x; z[x][1] += q.y; z[x][2] += q.z; z[x][3] += q.w;
+                        }
+                }
+                meet();
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int unit = tid + x * kJoinThreads;
+                    if (unit < rows * (R / 4)) store(unit / (R / 4), unit % (R / 4), z[x]);
+                }
             }
         }
         tc05::fence_proxy_async_smem();
