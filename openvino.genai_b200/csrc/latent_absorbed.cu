@@ -15,45 +15,52 @@ namespace {
 struct SeqPlan {
     int blocks;          // row blocks
     long long tiles;     // context tiles of each
+    int tokens;
 };
 __device__ __forceinline__ SeqPlan seq_plan(const AbsorbedArgs& a, int s) {
     SeqView v;
-    if (!seq_view(a.m, s, v) || v.n == 0 || !takes_absorbed(a.m, v)) return SeqPlan{0, 0};
+    if (!seq_view(a.m, s, v) || v.n == 0 || !takes_absorbed(a.m, v)) return SeqPlan{0, 0, 0};
     const int rows = kTile * a.row_tiles;
-    return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTokens - 1) / kTokens};
+    return SeqPlan{(int)(((long long)v.n * a.m.H + rows - 1) / rows), ((long long)v.past + v.n + kTokens - 1) / kTokens, v.n};
 }
 
 // Exclusive prefix sums over the sequences, by one block of 128 threads.
 __device__ void build_plan(const AbsorbedArgs& a) {
-    __shared__ long long sh_u[4], run_u;
+    __shared__ long long sh_u[4], run_u, sh_t[4], run_t;
     __shared__ int sh_b[4], run_b;
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = a.m.num_sequences;
-    if (tid == 0) { run_u = 0; run_b = 0; }
+    const Step& m = a.m;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = m.num_sequences;
+    if (tid == 0) { run_u = run_t = 0; run_b = 0; }
     __syncthreads();
     for (int base = 0; base < B; base += 128) {
         const int s = base + tid;
-        const SeqPlan p = s < B ? seq_plan(a, s) : SeqPlan{0, 0};
-        long long u = p.blocks * p.tiles;
+        const SeqPlan p = s < B ? seq_plan(a, s) : SeqPlan{0, 0, 0};
+        long long u = p.blocks * p.tiles, k = p.tokens;
         int b = p.blocks;
         const long long mine_u = u;
         const int mine_b = b;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long pu = __shfl_up_sync(0xffffffffu, u, o);
+            const long long pu = __shfl_up_sync(0xffffffffu, u, o), pk = __shfl_up_sync(0xffffffffu, k, o);
             const int pb = __shfl_up_sync(0xffffffffu, b, o);
-            if (lane >= o) { u += pu; b += pb; }
+            if (lane >= o) { u += pu; b += pb; k += pk; }
         }
-        if (lane == 31) { sh_u[wid] = u; sh_b[wid] = b; }
+        if (lane == 31) { sh_u[wid] = u; sh_b[wid] = b; sh_t[wid] = k; }
         __syncthreads();
-        long long off_u = run_u;
+        long long off_u = run_u, off_t = run_t;
         int off_b = run_b;
-        for (int w = 0; w < wid; ++w) { off_u += sh_u[w]; off_b += sh_b[w]; }
-        if (s < B) { a.unit_prefix[s] = off_u + u - mine_u; a.block_prefix[s] = off_b + b - mine_b; }
+        for (int w = 0; w < wid; ++w) { off_u += sh_u[w]; off_b += sh_b[w]; off_t += sh_t[w]; }
+        if (s < B) { a.unit_prefix[s] = off_u + u - mine_u; a.block_prefix[s] = off_b + b - mine_b; a.token_prefix[s] = (int)(off_t + k - p.tokens); }
         __syncthreads();
-        if (tid == 127) { run_u = off_u + u; run_b = off_b + b; }
+        if (tid == 127) { run_u = off_u + u; run_b = off_b + b; run_t = off_t + k; }
         __syncthreads();
     }
-    if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; }
+    // Prefix sums that fall can give sequences the same tokens, more in all than the workspace has rows for: such a step gets no plan.
+    if (tid == 0 && run_t > m.num_tokens) {
+        atomicOr(m.status, PA_DEV_BAD_BEGINS);
+        run_u = run_t = 0;
+    }
+    if (tid == 0) { a.unit_prefix[B] = run_u; a.block_prefix[B] = run_b; a.token_prefix[B] = (int)run_t; }
     __syncthreads();
     // where every slice begins, so that a CTA of the attention has one record to read instead of a search
     const long long total = run_u, per = total > 0 ? (total + a.groups - 1) / a.groups : 1;
@@ -663,20 +670,25 @@ struct ValueSmem {
     alignas(1024) uint8_t o[2][NC][NT * 128];                    // joined rows, high and low pieces
     alignas(1024) uint8_t w[NW][128 * 128];
     uint64_t w_full[NW], w_free[NW], o_full, done;
-    bool live[NT];
+    int token[NT];
     uint32_t tmem_base;
     int abort_flag;
 };
 
 template <int R, int NT, bool BF>
-__global__ void __launch_bounds__(kValueThreads) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
+__global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) project_value_kernel(const __grid_constant__ AbsorbedArgs a) {
     using Smem = ValueSmem<R, NT>;
     constexpr int NC = Smem::NC, NW = Smem::NW;
     extern __shared__ __align__(1024) uint8_t smem[];
     Smem& sm = *reinterpret_cast<Smem*>(smem);
     const Step& m = a.m;
     const int tid = threadIdx.x, warp = warp_id(), lane = tid & 31;
-    const int h = blockIdx.x % m.H, t0 = blockIdx.x / m.H * NT;
+    // (the plan and the step's tables do not come from the kernel before: its CTAs have all begun, so what precedes them is complete)
+    const int B = m.num_sequences, count = a.token_prefix[B], tiles = (count + NT - 1) / NT * m.H;
+    if ((int)blockIdx.x >= tiles) {
+        pa::grid_wait();
+        return;
+    }
     if (tid == kJoinThreads) {
         for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
         pa::mbar_init(&sm.o_full, kJoinWarps);
@@ -684,197 +696,207 @@ __global__ void __launch_bounds__(kValueThreads) project_value_kernel(const __gr
         pa::mbar_fence_init();
         sm.abort_flag = 0;
     }
-    // (what does not come from the kernel before: its CTAs have all begun, so what precedes them is complete)
-    if (!tile_rows(a, t0, sm.live)) {
-        pa::grid_wait();
-        return;
-    }
-    auto load_weights = [&](int c) {
-        if (tc05::elect_one()) {
-            pa::mbar_expect_tx(&sm.w_full[c % NW], m.Dv * 128);
-            tma_3d(sm.w[c % NW], &a.map_value_up, c * 64, 0, h, &sm.w_full[c % NW]);
-        }
-        __syncwarp();
-    };
-    if (warp == kJoinWarps) {
-        tc05::tmem_alloc(&sm.tmem_base, 64);
-        for (int c = 0; c < min(NW, NC); ++c) load_weights(c);
-    }
-    pa::grid_wait();
-    tc05::fence_before_thread_sync();
     __syncthreads();
-    tc05::fence_after_thread_sync();
-    const uint32_t tmem = sm.tmem_base;
+    if (warp == kJoinWarps) tc05::tmem_alloc(&sm.tmem_base, 64);
     const Waiter wt{&sm.abort_flag, m.status};
-    if (warp == kJoinWarps) {
-        bool ok = true;
-        const uint32_t idesc = tc05::instr_desc_f16(m.Dv, NT, BF ? 1 : 0, 0, 0), dw = desc_low(sm.w), doh = desc_low(sm.o[0]), dol = desc_low(sm.o[1]);
-        int loaded = min(NW, NC);
-        ok = wt.wait_warp(&sm.o_full, 0);
-        for (int c = 0; ok && c < NC; ++c) {
-            ok = wt.wait_warp(&sm.w_full[c % NW], (c / NW) & 1);
-            if (!ok) break;
-            tc05::fence_after_thread_sync();
-            const uint32_t da = dw + c % NW * (128 * 128 >> 4), dh = doh + c * (NT * 128 >> 4), dl = dol + c * (NT * 128 >> 4);
+    uint32_t parity = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
+        const int h = tile % m.H, c0 = tile / m.H * NT, rows = min(NT, count - c0);
+        if (tid < rows) {      // the tile's tokens: of those of this form the ones from number c0
+            const int c = c0 + tid;
+            int lo = 0, hi = B;
+            if (c < B && a.token_prefix[c] == c && a.token_prefix[c + 1] == c + 1) lo = c;
+            else
+                while (hi - lo > 1) {        // token_prefix[lo] <= c < token_prefix[hi]
+                    const int mid = (lo + hi) >> 1;
+                    if (a.token_prefix[mid] <= c) lo = mid; else hi = mid;
+                }
+            sm.token[tid] = m.subsequence_begins[lo] + c - a.token_prefix[lo];
+        }
+        auto load_weights = [&](int c) {
             if (tc05::elect_one()) {
-                if (c == 0) mma_ss<0>(tmem, da, dh, idesc);
-                else mma_ss<1>(tmem, da, dh, idesc);
-#pragma unroll
-                for (int kk = 1; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dh + 2 * kk, idesc);
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dl + 2 * kk, idesc);
-                tc05::commit(&sm.w_free[c % NW]);
-                if (c + 1 == NC) tc05::commit(&sm.done);
+                pa::mbar_expect_tx(&sm.w_full[c % NW], m.Dv * 128);
+                tma_3d(sm.w[c % NW], &a.map_value_up, c * 64, 0, h, &sm.w_full[c % NW]);
             }
             __syncwarp();
-            if (c + NW < NC) {
-                ok = wt.wait_warp(&sm.w_free[c % NW], (c / NW) & 1);
-                if (ok) { load_weights(c + NW); ++loaded; }
-            }
-        }
-        if (!ok)
-            for (int c = max(0, loaded - NW); c < loaded; ++c) drain(&sm.w_full[c % NW], (c / NW) & 1);
-    } else {
-        const int step = a.row_tiles * kTile;        // from a row's partial result to the next
-        auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kJoinThreads) : "memory"); };   // (the joining warps; none of them can have left)
-        // element quad `e` of row `r`, swizzled by the row
-        auto store = [&](int r, int e, const float (&y)[4]) {
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
-                lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
-            }
-            const uint32_t at = r * 128 + (((e % 16 >> 1) ^ (r & 7)) << 4) + (e & 1) * 8;
-            *reinterpret_cast<uint2*>(sm.o[0][e / 16] + at) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(sm.o[1][e / 16] + at) = make_uint2(lo[0], lo[1]);
         };
-        // A warp has a row (of 64: one of every sixteen), or rows that are fewer than the warps have several each, which deal out the pieces.
-        // A lane has four elements of every 128, and the statistics of one of 32 pieces; the first pieces are under way before their weights are known.
-        constexpr int V = R / 128, kRows = NT / kJoinWarps, U = NT == 16 ? 4 : 2;
-        int rows = NT, spread = 0;
-        if (NT == 16) {
-            rows = 32 - __clz(__ballot_sync(0xffffffffu, lane < NT && sm.live[lane % NT]));
-            spread = 4 - (32 - __clz(rows - 1));
-        }
-        const int each = 1 << spread, mine = warp & (each - 1);
-        int2 part[kRows];
-        float2 ml[kRows];
-        float4 p[2][U][V];
+        if (warp == kJoinWarps)
+            for (int c = 0; c < NW; ++c) load_weights(c);
+        if (tile == (int)blockIdx.x) pa::grid_wait();
+        tc05::fence_before_thread_sync();
+        __syncthreads();
+        tc05::fence_after_thread_sync();
+        const uint32_t tmem = sm.tmem_base;
+        if (warp == kJoinWarps) {
+            bool ok = true;
+            const uint32_t idesc = tc05::instr_desc_f16(m.Dv, NT, BF ? 1 : 0, 0, 0), dw = desc_low(sm.w), doh = desc_low(sm.o[0]), dol = desc_low(sm.o[1]);
+            constexpr uint32_t kTurns = NC / NW;      // uses of a buffer to a tile
+            static_assert(NC % NW == 0, "");
+            int loaded = NW;
+            ok = wt.wait_warp(&sm.o_full, parity);
+            for (int c = 0; ok && c < NC; ++c) {
+                ok = wt.wait_warp(&sm.w_full[c % NW], (kTurns * parity + c / NW) & 1);
+                if (!ok) break;
+                tc05::fence_after_thread_sync();
+                const uint32_t da = dw + c % NW * (128 * 128 >> 4), dh = doh + c * (NT * 128 >> 4), dl = dol + c * (NT * 128 >> 4);
+                if (tc05::elect_one()) {
+                    if (c == 0) mma_ss<0>(tmem, da, dh, idesc);
+                    else mma_ss<1>(tmem, da, dh, idesc);
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            const int r = (warp >> spread) + u * kJoinWarps;
-            part[u] = sm.live[r] ? a.row_part[(long long)(t0 + r) * m.H + h] : make_int2(0, 0);
-        }
-        auto load = [&](float4 (&q)[V], const int2& row, int piece) {
-            const float4* src = reinterpret_cast<const float4*>(a.part_o + (row.x + (long long)piece * step) * R) + lane;
+                    for (int kk = 1; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dh + 2 * kk, idesc);
 #pragma unroll
-            for (int v = 0; v < V; ++v) q[v] = src[32 * v];
-        };
-        auto first = [&](int u) {
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (mine + k * each < part[u].y) load(p[u & 1][k], part[u], mine + k * each);
-        };
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) ml[u] = lane < part[u].y ? a.part_ml[part[u].x + (long long)lane * step] : make_float2(-INFINITY, 0.f);
-        first(0);
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            const int r = (warp >> spread) + u * kJoinWarps, pieces = part[u].y;
-            if (u + 1 < kRows) first(u + 1);
-            // the pieces' common maximum, and the denominator (a piece whose tiles the row does not see has no sums)
-            float top = ml[u].y > 0.f ? ml[u].x : -INFINITY, sum = ml[u].y > 0.f ? ml[u].y : 0.f;
-            for (int i = lane + 32; i < pieces; i += 32) {
-                const float2 other = a.part_ml[part[u].x + (long long)i * step];
-                if (other.y > 0.f) {
-                    const float t = fmaxf(top, other.x);
-                    sum = (top == -INFINITY ? 0.f : sum * ex2(top - t)) + other.y * ex2(other.x - t);
-                    top = t;
+                    for (int kk = 0; kk < 4; ++kk) mma_ss<1>(tmem, da + 2 * kk, dl + 2 * kk, idesc);
+                    tc05::commit(&sm.w_free[c % NW]);
+                    if (c + 1 == NC) tc05::commit(&sm.done);
+                }
+                __syncwarp();
+                if (c + NW < NC) {
+                    ok = wt.wait_warp(&sm.w_free[c % NW], (kTurns * parity + c / NW) & 1);
+                    if (ok) { load_weights(c + NW); ++loaded; }
                 }
             }
-            const float most = pa::warp_max(top), inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - most));
-            float y[V][4] = {};
-            for (int base = 0; base < pieces; base += 32 * each) {
-                const int i = base + mine + lane * each, count = min(32, (pieces - base - mine + each - 1) >> spread);
-                float2 own = ml[u];
-                if (base > 0 || each > 1) own = i < pieces ? a.part_ml[part[u].x + (long long)i * step] : make_float2(-INFINITY, 0.f);
-                const float weight = own.y > 0.f ? ex2(own.x - most) * inv : 0.f;
-                for (int j = 0; j < count; j += U) {
-                    if (base + j > 0) {
+            if (!ok)
+                for (int c = max(0, loaded - NW); c < loaded; ++c) drain(&sm.w_full[c % NW], (kTurns * parity + c / NW) & 1);
+        } else {
+            const int step = a.row_tiles * kTile;        // from a row's partial result to the next
+            auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(kJoinThreads) : "memory"); };   // (the joining warps; none of them can have left)
+            // element quad `e` of row `r`, swizzled by the row
+            auto store = [&](int r, int e, const float (&y)[4]) {
+                uint32_t hi[2], lo[2];
 #pragma unroll
-                        for (int k = 0; k < U; ++k)
-                            if (j + k < count) load(p[u & 1][k], part[u], base + mine + (j + k) * each);
+                for (int i = 0; i < 2; ++i) {
+                    hi[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
+                    lo[i] = pack2<BF>(y[2 * i] - unpack1<BF>((uint16_t)hi[i]), y[2 * i + 1] - unpack1<BF>((uint16_t)(hi[i] >> 16)));
+                }
+                const uint32_t at = r * 128 + (((e % 16 >> 1) ^ (r & 7)) << 4) + (e & 1) * 8;
+                *reinterpret_cast<uint2*>(sm.o[0][e / 16] + at) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(sm.o[1][e / 16] + at) = make_uint2(lo[0], lo[1]);
+            };
+            // A warp has a row (of 64: one of every sixteen), or rows that are fewer than the warps have several each, which deal out the pieces.
+            // A lane has four elements of every 128, and the statistics of one of 32 pieces; the first pieces are under way before their weights are known.
+            constexpr int V = R / 128, kRows = NT / kJoinWarps, U = NT == 16 ? 4 : 2;
+            const int spread = NT == 16 ? 4 - (32 - __clz(rows - 1)) : 0;
+            const int each = 1 << spread, mine = warp & (each - 1);
+            int2 part[kRows];
+            float2 ml[kRows];
+            float4 p[2][U][V];
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) {
+                const int r = (warp >> spread) + u * kJoinWarps;
+                part[u] = r < rows ? a.row_part[(long long)sm.token[r] * m.H + h] : make_int2(0, 0);
+            }
+            auto load = [&](float4 (&q)[V], const int2& row, int piece) {
+                const float4* src = reinterpret_cast<const float4*>(a.part_o + (row.x + (long long)piece * step) * R) + lane;
+#pragma unroll
+                for (int v = 0; v < V; ++v) q[v] = src[32 * v];
+            };
+            auto first = [&](int u) {
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (mine + k * each < part[u].y) load(p[u & 1][k], part[u], mine + k * each);
+            };
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) ml[u] = lane < part[u].y ? a.part_ml[part[u].x + (long long)lane * step] : make_float2(-INFINITY, 0.f);
+            first(0);
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) {
+                const int r = (warp >> spread) + u * kJoinWarps, pieces = part[u].y;
+                if (u + 1 < kRows) first(u + 1);
+                // the pieces' common maximum, and the denominator (a piece whose tiles the row does not see has no sums)
+                float top = ml[u].y > 0.f ? ml[u].x : -INFINITY, sum = ml[u].y > 0.f ? ml[u].y : 0.f;
+                for (int i = lane + 32; i < pieces; i += 32) {
+                    const float2 other = a.part_ml[part[u].x + (long long)i * step];
+                    if (other.y > 0.f) {
+                        const float t = fmaxf(top, other.x);
+                        sum = (top == -INFINITY ? 0.f : sum * ex2(top - t)) + other.y * ex2(other.x - t);
+                        top = t;
                     }
+                }
+                const float most = pa::warp_max(top), inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - most));
+                float y[V][4] = {};
+                for (int base = 0; base < pieces; base += 32 * each) {
+                    const int i = base + mine + lane * each, count = min(32, (pieces - base - mine + each - 1) >> spread);
+                    float2 own = ml[u];
+                    if (base > 0 || each > 1) own = i < pieces ? a.part_ml[part[u].x + (long long)i * step] : make_float2(-INFINITY, 0.f);
+                    const float weight = own.y > 0.f ? ex2(own.x - most) * inv : 0.f;
+                    for (int j = 0; j < count; j += U) {
+                        if (base + j > 0) {
 #pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        const float f = __shfl_sync(0xffffffffu, weight, j + k);
-                        if (f != 0.f) {      // (a piece without sums has no results either)
+                            for (int k = 0; k < U; ++k)
+                                if (j + k < count) load(p[u & 1][k], part[u], base + mine + (j + k) * each);
+                        }
 #pragma unroll
-                            for (int v = 0; v < V; ++v) {
-                                const float4& q = p[u & 1][k][v];
-                                y[v][0] += f * q.x; y[v][1] += f * q.y; y[v][2] += f * q.z; y[v][3] += f * q.w;
+                        for (int k = 0; k < U; ++k) {
+                            const float f = __shfl_sync(0xffffffffu, weight, j + k);
+                            if (f != 0.f) {      // (a piece without sums has no results either)
+#pragma unroll
+                                for (int v = 0; v < V; ++v) {
+                                    const float4& q = p[u & 1][k][v];
+                                    y[v][0] += f * q.x; y[v][1] += f * q.y; y[v][2] += f * q.z; y[v][3] += f * q.w;
+                                }
                             }
                         }
                     }
                 }
-            }
-            if (each == 1) {
-                if (pieces > 0) {
+                if (each == 1) {
+                    if (pieces > 0) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) store(r, lane + 32 * v, y[v]);
+                        for (int v = 0; v < V; ++v) store(r, lane + 32 * v, y[v]);
+                    }
+                } else {
+                    // the sums of a row's warps, in turn where the rows will be
+                    float4* sums = reinterpret_cast<float4*>(sm.o);
+                    static_assert(NT != 16 || sizeof(sm.o) == kJoinWarps * R * 4, "");
+#pragma unroll
+                    for (int v = 0; v < V; ++v) sums[warp * (R / 4) + lane + 32 * v] = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
+                    meet();
+                    float z[2][4] = {};
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {      // (at most eight rows)
+                        const int unit = tid + x * kJoinThreads;
+                        if (unit < rows * (R / 4))
+                            for (int k = 0; k < each; ++k) {
+                                const float4 q = sums[((unit / (R / 4) << spread) + k) * (R / 4) + unit % (R / 4)];
+                                z[x][0] += q.x; z[x][1] += q.y; z[x][2] += q.z; z[x][3] += q.w;
+                            }
+                    }
+                    meet();
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int unit = tid + x * kJoinThreads;
+                        if (unit < rows * (R / 4)) store(unit / (R / 4), unit % (R / 4), z[x]);
+                    }
                 }
-            } else {
-                // the sums of a row's warps, in turn where the rows will be
-                float4* sums = reinterpret_cast<float4*>(sm.o);
-                static_assert(NT != 16 || sizeof(sm.o) == kJoinWarps * R * 4, "");
+            }
+            tc05::fence_proxy_async_smem();
+            warp_arrive(&sm.o_full);
+            if (warp < 4) {
+                const bool ok = wt.wait_warp(&sm.done, parity);
+                tc05::fence_after_thread_sync();
+                // 128 rows: a warp has 32 of them; 64 rows: 16, in the first half of its lanes
+                const int d = m.Dv == 128 ? 32 * warp + lane : 16 * warp + lane;
+                if (ok) {
+                    uint16_t* dst = (uint16_t*)a.output + (long long)h * m.Dv + d;
 #pragma unroll
-                for (int v = 0; v < V; ++v) sums[warp * (R / 4) + lane + 32 * v] = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
-                meet();
-                float z[2][4] = {};
+                    for (int g = 0; g < NT; g += 16) {
+                        uint32_t r[16];
+                        tc05::ld_32x32b_x16(tmem + ((uint32_t)(warp * 32) << 16) + g, r);
+                        tc05::wait_ld();
+                        if (m.Dv == 128 || lane < 16) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {      // (at most eight rows)
-                    const int unit = tid + x * kJoinThreads;
-                    if (unit < rows * (R / 4))
-                        for (int k = 0; k < each; ++k) {
-                            const float4 q = sums[((unit / (R / 4) << spread) + k) * (R / 4) + unit % (R / 4)];
-                            z[x][0] += q.x; z[x][1] += q.y; z[x][2] += q.z; z[x][3] += q.w;
+                            for (int c = 0; c < 16; ++c)
+                                if (g + c < rows) dst[(long long)sm.token[g + c] * m.H * m.Dv] = pack1<BF>(__uint_as_float(r[c]));
                         }
-                }
-                meet();
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int unit = tid + x * kJoinThreads;
-                    if (unit < rows * (R / 4)) store(unit / (R / 4), unit % (R / 4), z[x]);
-                }
-            }
-        }
-        tc05::fence_proxy_async_smem();
-        warp_arrive(&sm.o_full);
-        if (warp < 4) {
-            const bool ok = wt.wait_warp(&sm.done, 0);
-            tc05::fence_after_thread_sync();
-            // 128 rows: a warp has 32 of them; 64 rows: 16, in the first half of its lanes
-            const int d = m.Dv == 128 ? 32 * warp + lane : 16 * warp + lane;
-            if (ok) {
-                uint16_t* dst = (uint16_t*)a.output + ((long long)t0 * m.H + h) * m.Dv + d;
-#pragma unroll
-                for (int c0 = 0; c0 < NT; c0 += 16) {
-                    uint32_t r[16];
-                    tc05::ld_32x32b_x16(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
-                    tc05::wait_ld();
-                    if (m.Dv == 128 || lane < 16) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            if (sm.live[c0 + c]) dst[(long long)(c0 + c) * m.H * m.Dv] = pack1<BF>(__uint_as_float(r[c]));
                     }
                 }
             }
         }
+        tc05::fence_before_thread_sync();
+        __syncthreads();
+        tc05::fence_after_thread_sync();
+        if (*(volatile int*)&sm.abort_flag) break;
     }
-    tc05::fence_before_thread_sync();
-    __syncthreads();
-    if (warp == kJoinWarps) tc05::tmem_dealloc(tmem, 64);
+    if (warp == kJoinWarps) tc05::tmem_dealloc(sm.tmem_base, 64);
 }
 
 int query_smem(const Step& m) { return 2 * m.Dn * 128 + m.Dn / 64 * 8192; }
@@ -888,8 +910,10 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     if (e == cudaSuccess) {
         // tiles of 16 tokens where those of 64 would leave SMs without one; in an AUTO step most tokens may be the expanded form's
         const int rows = m.form == PA_LATENT_AUTO ? std::min(m.num_tokens, m.num_sequences) : m.num_tokens;
-        if (rows <= 16 || (long long)(rows + kTile - 1) / kTile * m.H < a.groups * a.row_tiles * 2 / 3) e = pa::launch_dependent(project_value_kernel<R, 16, BF>, (m.num_tokens + 15) / 16 * m.H, kValueThreads, sizeof(ValueSmem<R, 16>), stream, a);
-        else e = pa::launch_dependent(project_value_kernel<R, 64, BF>, token_tiles * m.H, kValueThreads, sizeof(ValueSmem<R, 64>), stream, a);
+        const int sms = a.groups * a.row_tiles, few = (m.num_tokens + 15) / 16 * m.H, many = token_tiles * m.H;
+        if (rows <= 16 || (long long)(rows + kTile - 1) / kTile * m.H < sms * 2 / 3)
+            e = pa::launch_dependent(project_value_kernel<R, 16, BF>, std::min(few, R == 256 ? 2 * sms : sms), kValueThreads, sizeof(ValueSmem<R, 16>), stream, a);
+        else e = pa::launch_dependent(project_value_kernel<R, 64, BF>, std::min(many, sms), kValueThreads, sizeof(ValueSmem<R, 64>), stream, a);
     }
     *launches += 3;
     return e;

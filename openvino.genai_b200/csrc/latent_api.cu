@@ -121,7 +121,7 @@ constexpr size_t kExpandBytes = (size_t)1 << 30;
 
 struct Scratch {
     int row_tiles, groups;
-    size_t unit_prefix, block_prefix, starts, q_abs, part_o, part_ml, row_part;
+    size_t unit_prefix, block_prefix, token_prefix, starts, q_abs, part_o, part_ml, row_part;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
     size_t tile_prefix, query_prefix, order, heads_per_item, counter, k, v, k_rope;
@@ -143,6 +143,7 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         const size_t slots = (size_t)latent::absorbed_slots(most, sequences, d.num_heads, s.groups, s.row_tiles);
         s.unit_prefix = take(((size_t)sequences + 1) * sizeof(long long));
         s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
+        s.token_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.starts = take(s.groups * sizeof(latent::SliceStart));
         s.q_abs = take(rows * (d.latent_size + d.rope_size) * 2);
         s.row_part = take(rows * sizeof(int2));
@@ -260,6 +261,7 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         k.groups = s.groups; k.row_tiles = s.row_tiles;
         k.unit_prefix = (long long*)(h->ws + s.unit_prefix);
         k.block_prefix = (int*)(h->ws + s.block_prefix);
+        k.token_prefix = (int*)(h->ws + s.token_prefix);
         k.starts = (latent::SliceStart*)(h->ws + s.starts);
         k.q_rope = a->query_rope; k.qr_token = rt; k.qr_head = rh;
         k.q_abs = h->ws + s.q_abs;

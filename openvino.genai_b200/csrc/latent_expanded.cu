@@ -17,11 +17,12 @@ constexpr int kBuckets = 1024;
 __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constant__ ExpandedArgs a) {
     __shared__ int sh_c[8], sh_q[8], run_c, run_q;
     __shared__ int bucket[kBuckets];
+    __shared__ unsigned long long all_c, all_t;
     const Step& m = a.m;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = m.num_sequences;
     pa::grid_wait();
     pa::grid_release();
-    if (tid == 0) { run_c = 0; run_q = 0; }
+    if (tid == 0) { run_c = 0; run_q = 0; all_c = all_t = 0; }
     for (int i = tid; i < a.passes; i += 256) a.counter[i] = 0;
     for (int i = tid; i < kBuckets; i += 256) bucket[i] = 0;
     __syncthreads();
@@ -33,6 +34,8 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
             if (seq_view(m, s, v) && v.n > 0 && !takes_absorbed(m, v)) {
                 c = (int)(((long long)v.past + v.n + kExpandTile - 1) / kExpandTile);
                 q = (v.n + kQueryTile - 1) / kQueryTile;
+                atomicAdd(&all_c, (unsigned long long)c);
+                atomicAdd(&all_t, (unsigned long long)v.n);
             }
         }
         const int mine_c = c, mine_q = q;
@@ -49,6 +52,15 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         __syncthreads();
         if (tid == 255) { run_c = off_c + c; run_q = off_q + q; }
         __syncthreads();
+    }
+    // Prefix sums that fall can give sequences the same tokens or blocks, more in all than the workspace has rows for: such a step gets no plan.
+    if (all_t > (unsigned long long)m.num_tokens || all_c * kExpandTile > (unsigned long long)a.rows) {
+        if (tid == 0) {
+            atomicOr(m.status, PA_DEV_BAD_BEGINS);
+            a.tile_prefix[B] = a.query_prefix[B] = 0;
+            *a.heads_per_item = 1;
+        }
+        return;
     }
     if (tid == 0) { a.tile_prefix[B] = run_c; a.query_prefix[B] = run_q; }
     if (tid >= 32 && tid < 64) {

@@ -67,6 +67,7 @@ struct AbsorbedArgs {
     int groups, row_tiles;
     long long* unit_prefix;     // [num_sequences + 1]
     int* block_prefix;          // [num_sequences + 1]
+    int* token_prefix;          // [num_sequences + 1], tokens of the sequences of this form
     SliceStart* starts;         // [groups]
     const void* q_rope;
     long long qr_token, qr_head;

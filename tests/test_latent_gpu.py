@@ -277,6 +277,23 @@ def test_bad_metadata_is_reported_and_other_sequences_are_served(pkg, form, what
     st.check(torch.where(torch.isnan(out), torch.zeros_like(out), out) if bad is None else out, rows=[0, 2] if bad else [0])
 
 
+@pytest.mark.parametrize("form", ["absorbed", "expanded"])
+@pytest.mark.parametrize("what", ["subsequence_begins", "block_indices_begins"])
+def test_falling_prefix_sums_write_nothing(pkg, form, what):
+    """Sequences that are given the same tokens, or the same blocks, several times over: more rows in all than the step's workspace has."""
+    st = LH.Step([200, 0, 200, 0, 200], [40, 0, 40, 0, 40], heads=6, bs=16, seed=4)
+    op = st.operator(pkg)
+    x = st.device_inputs()
+    last = int(x[what][-1])
+    x[what].copy_(torch.tensor([0, last, 0, last, 0, last], dtype=torch.int32))
+    x["past_lens"].fill_(0 if what == "subsequence_begins" else last * 16 - 40)
+    if what == "block_indices_begins" and form == "absorbed":      # (its workspace goes by the tokens only: the sequences that are left are served)
+        st.attend(op, form, x)
+    else:
+        assert bool(torch.isnan(st.attend(op, form, x)).all())
+    assert op.device_status() & BAD_BEGINS
+
+
 def test_append_reports_positions_outside_the_table_and_bad_blocks(pkg):
     st = LH.Step([4, 6], [3, 2], heads=3, seed=2)
     x = st.append_inputs(rope_table=st.rope_table[:7].contiguous().cuda())
