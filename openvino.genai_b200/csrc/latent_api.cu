@@ -124,7 +124,8 @@ struct Scratch {
     size_t unit_prefix, block_prefix, token_prefix, starts, q_abs, part_o, part_ml, row_part;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
-    size_t tile_prefix, query_prefix, order, heads_per_item, counter, k, v, k_rope;
+    size_t tile_prefix, query_prefix, order, heads_per_item, counter, arrived, split_o, split_ml, k, v, k_rope;
+    int part_slots;
     size_t total;
 };
 
@@ -158,8 +159,13 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.passes = (d.num_heads + s.heads - 1) / s.heads;
         s.tile_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.query_prefix = take(((size_t)sequences + 1) * sizeof(int));
-        s.order = take(((size_t)tokens / latent::kQueryTile + served) * sizeof(int2));
-        s.heads_per_item = take(sizeof(int));
+        s.part_slots = 2 * h->sm_count / s.heads * s.heads;      // (a pass of so many heads as CTAs cuts no context)
+        if (s.heads >= h->sm_count) s.part_slots = 0;
+        s.order = take(((size_t)tokens / latent::kQueryTile + served + s.part_slots) * sizeof(latent::PieceOfQuery));
+        s.arrived = take((size_t)s.passes * s.part_slots * 8 * sizeof(int));
+        s.split_o = take((size_t)s.part_slots * latent::kQueryTile * d.value_size * sizeof(float));
+        s.split_ml = take((size_t)s.part_slots * latent::kQueryTile * sizeof(float2));
+        s.heads_per_item = take(2 * sizeof(int));
         s.counter = take((size_t)s.passes * sizeof(int));
         s.k_rope = take((size_t)s.rows * 64 * 2);
         s.k = take((size_t)s.heads * s.rows * d.nope_size * 2);
@@ -295,7 +301,12 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         k.rows = s.rows;
         k.tile_prefix = (int*)(h->ws + s.tile_prefix);
         k.query_prefix = (int*)(h->ws + s.query_prefix);
-        k.order = (int2*)(h->ws + s.order);
+        k.order = (latent::PieceOfQuery*)(h->ws + s.order);
+        k.items = (int*)(h->ws + s.heads_per_item) + 1;
+        k.arrived = (int*)(h->ws + s.arrived);
+        k.part_slots = s.part_slots;
+        k.part_o = (float*)(h->ws + s.split_o);
+        k.part_ml = (float2*)(h->ws + s.split_ml);
         k.counter = (int*)(h->ws + s.counter);
         k.heads_per_item = (int*)(h->ws + s.heads_per_item);
         k.passes = s.passes; k.ctas = h->sm_count; k.heads = s.heads;

@@ -14,28 +14,34 @@ namespace {
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------
 constexpr int kBuckets = 1024;
+constexpr int kListed = 1024;       // query tiles that are listed in shared memory; later ones are searched for
 __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constant__ ExpandedArgs a) {
     __shared__ int sh_c[8], sh_q[8], run_c, run_q;
     __shared__ int bucket[kBuckets];
-    __shared__ unsigned long long all_c, all_t;
+    __shared__ int3 listed[kListed];     // sequence, query tile, context tiles
+    __shared__ unsigned long long all_c, all_t, work;
+    __shared__ int deepest, cuts[32], longest, pieces_sum, slots;
     const Step& m = a.m;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = m.num_sequences;
     pa::grid_wait();
     pa::grid_release();
-    if (tid == 0) { run_c = 0; run_q = 0; all_c = all_t = 0; }
+    if (tid == 0) { run_c = 0; run_q = 0; all_c = all_t = work = 0; deepest = pieces_sum = slots = 0; }
+    if (tid < 32) cuts[tid] = 0;
     for (int i = tid; i < a.passes; i += 256) a.counter[i] = 0;
+    for (int i = tid; i < a.passes * a.part_slots * 8; i += 256) a.arrived[i] = 0;
     for (int i = tid; i < kBuckets; i += 256) bucket[i] = 0;
     __syncthreads();
     for (int base = 0; base < B; base += 256) {
         const int s = base + tid;
         int c = 0, q = 0;
+        SeqView v{0, 0, 0, 0};
         if (s < B) {
-            SeqView v;
             if (seq_view(m, s, v) && v.n > 0 && !takes_absorbed(m, v)) {
                 c = (int)(((long long)v.past + v.n + kExpandTile - 1) / kExpandTile);
                 q = (v.n + kQueryTile - 1) / kQueryTile;
                 atomicAdd(&all_c, (unsigned long long)c);
                 atomicAdd(&all_t, (unsigned long long)v.n);
+                atomicMax(&deepest, c);
             }
         }
         const int mine_c = c, mine_q = q;
@@ -49,6 +55,13 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         int off_c = run_c, off_q = run_q;
         for (int w = 0; w < wid; ++w) { off_c += sh_c[w]; off_q += sh_q[w]; }
         if (s < B) { a.tile_prefix[s] = off_c + c - mine_c; a.query_prefix[s] = off_q + q - mine_q; }
+        unsigned long long sum = 0;
+        for (int k = 0; k < mine_q; ++k) {
+            const int at = off_q + q - mine_q + k, tiles = (int)(((long long)v.past + min(v.n, (k + 1) * kQueryTile) + kExpandTile - 1) / kExpandTile);
+            if (at < kListed) listed[at] = make_int3(s, k, tiles);
+            sum += tiles;
+        }
+        if (mine_q > 0) atomicAdd(&work, sum);
         __syncthreads();
         if (tid == 255) { run_c = off_c + c; run_q = off_q + q; }
         __syncthreads();
@@ -57,8 +70,9 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
     if (all_t > (unsigned long long)m.num_tokens || all_c * kExpandTile > (unsigned long long)a.rows) {
         if (tid == 0) {
             atomicOr(m.status, PA_DEV_BAD_BEGINS);
-            a.tile_prefix[B] = a.query_prefix[B] = 0;
+            a.tile_prefix[B] = 0;
             *a.heads_per_item = 1;
+            *a.items = 0;
         }
         return;
     }
@@ -74,9 +88,17 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         if (lane == 0) *a.heads_per_item = (int)(cost % 32) + 1;
     }
     __syncthreads();
-    // counting sort of the query tiles by the context they see, the longest first, so that the last items to be drawn are short
+    // Query tiles are cut along their context where they are too few for the CTAs: into the pieces whose rounds over the CTAs end first, at two tiles to a
+    // piece for its beginning and end, and three for the joining.  None is shorter than a CTA's share of all tiles, and a cut tile has more than one
+    // piece's worth, so that there are at most 2 * ctas pieces of cut ones.  (Three prompts by 16 heads, 96 tiles of up to 20 x 128 context tokens, beside 40
+    // rows of one token: 146 us uncut, 134 in pieces of at most 12, 151 in pieces of 8, which take a second round.)
     const int total = run_q;
-    auto place = [&](int i, int& s, int& qt) {
+    auto place = [&](int i, int& s, int& qt) {       // context tiles of query tile i
+        if (i < kListed) {
+            s = listed[i].x;
+            qt = listed[i].y;
+            return listed[i].z;
+        }
         int lo = 0, hi = B;   // query_prefix[lo] <= i < query_prefix[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -85,12 +107,39 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         s = lo;
         qt = i - a.query_prefix[lo];
         const int n = m.subsequence_begins[lo + 1] - m.subsequence_begins[lo];
-        const int tiles = (m.past_lens[lo] + min(n, (qt + 1) * kQueryTile) + kExpandTile - 1) / kExpandTile;
-        return kBuckets - 1 - min(tiles, kBuckets - 1);
+        return (m.past_lens[lo] + min(n, (qt + 1) * kQueryTile) + kExpandTile - 1) / kExpandTile;
     };
+    const long long share = ((long long)work * a.heads + a.ctas - 1) / a.ctas;
+    const bool few = a.part_slots > 0 && deepest > share && total <= kListed;
+    if (few) {
+        const int most = max((deepest + lane) / (lane + 1), (int)share);      // a warp for every eighth tile, a lane for every length
+        int pieces = 0;
+        for (int i = wid; i < total; i += 8) {
+            int s, qt;
+            pieces += (place(i, s, qt) + most - 1) / most;
+        }
+        atomicAdd(&cuts[lane], pieces);
+        __syncthreads();
+        if (tid < 32) {
+            const long long rounds = ((long long)cuts[lane] * a.heads + a.ctas - 1) / a.ctas;
+            long long cost = (rounds * (most + 2) + (lane > 0 ? 3 : 0)) * 32 + lane;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) cost = min(cost, __shfl_xor_sync(0xffffffffu, cost, o));
+            if (lane == cost % 32) longest = most;
+        }
+    } else if (tid == 0) longest = INT_MAX / 2;
+    __syncthreads();
+    auto cut = [&](int tiles, int& length) {         // pieces of a query tile, and their length
+        const int pieces = (tiles + longest - 1) / longest;
+        length = (tiles + pieces - 1) / pieces;
+        return (tiles + length - 1) / length;
+    };
+    // counting sort of the pieces by length, the longest first, so that the last items to be drawn are short
     for (int i = tid; i < total; i += 256) {
-        int s, qt;
-        atomicAdd(&bucket[place(i, s, qt)], 1);
+        int s, qt, length;
+        const int tiles = place(i, s, qt), pieces = cut(tiles, length);
+        for (int k = 0; k < pieces; ++k) atomicAdd(&bucket[kBuckets - 1 - min(min(length, tiles - k * length), kBuckets - 1)], 1);
+        atomicAdd(&pieces_sum, pieces);
     }
     __syncthreads();
     if (tid < 32) {          // exclusive prefix sum over the buckets
@@ -108,10 +157,12 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
         }
     }
     __syncthreads();
+    if (tid == 0) *a.items = pieces_sum;
     for (int i = tid; i < total; i += 256) {
-        int s, qt;
-        const int b = place(i, s, qt);
-        a.order[atomicAdd(&bucket[b], 1)] = make_int2(s, qt);
+        int s, qt, length;
+        const int tiles = place(i, s, qt), pieces = cut(tiles, length), slot = pieces > 1 ? atomicAdd(&slots, pieces) : -1;
+        for (int k = 0; k < pieces; ++k)
+            a.order[atomicAdd(&bucket[kBuckets - 1 - min(min(length, tiles - k * length), kBuckets - 1)], 1)] = PieceOfQuery{s, qt, k, length, slot};
     }
 }
 
@@ -383,6 +434,8 @@ struct QueryItem {
     int past;            // context its first row sees, less one
     int row;             // first row of the sequence's context in the scratch
     int tiles[2];        // context tiles of each half
+    int slot, piece;     // partial result of the first piece, -1: the whole context; number of the piece
+    int pieces[2];       // of each half
 };
 
 template <int DN, int DV>
@@ -453,7 +506,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
         reg_dec<kOtherRegs>();
         if (warp == 8) {
             // ======================= loader =============================================================
-            const int items = a.query_prefix[m.num_sequences] * a.heads;
+            const int items = *a.items * a.heads;
             uint32_t ni = 0, nk = 0, nq[2] = {0, 0};
             bool ok = true;
             while (ok) {
@@ -463,17 +516,22 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 QueryItem it;
                 it.h = -1;
                 if (i < items) {
-                    const int2 at = a.order[i / a.heads];
+                    const PieceOfQuery at = a.order[i / a.heads];
                     SeqView v;
-                    seq_view(m, at.x, v);
+                    seq_view(m, at.s, v);
+                    const int first = at.piece * at.length, past = v.past + at.tile * kQueryTile;
                     it.h = i % a.heads;
-                    it.t0 = v.t0 + at.y * kQueryTile;
-                    it.rows = min(kQueryTile, v.n - at.y * kQueryTile);
-                    it.past = v.past + at.y * kQueryTile;
-                    it.row = a.tile_prefix[at.x] * kExpandTile;
+                    it.t0 = v.t0 + at.tile * kQueryTile;
+                    it.rows = min(kQueryTile, v.n - at.tile * kQueryTile);
+                    it.past = past - first * kExpandTile;
+                    it.row = (a.tile_prefix[at.s] + first) * kExpandTile;
+                    it.slot = at.slot < 0 ? -1 : at.slot * a.heads + it.h;
+                    it.piece = at.piece;
                     for (int x = 0; x < 2; ++x) {
                         const int last = min(it.rows, 128 * (x + 1));     // rows up to the half's end
-                        it.tiles[x] = last > 128 * x ? (it.past + last + kExpandTile - 1) / kExpandTile : 0;
+                        const int tiles = last > 128 * x ? (past + last + kExpandTile - 1) / kExpandTile : 0;
+                        it.tiles[x] = min(max(tiles - first, 0), at.length);
+                        it.pieces[x] = (tiles + at.length - 1) / at.length;
                     }
                 }
                 const int slot = ni % kItemSlots;
@@ -722,20 +780,70 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             if (!ok || !wt.wait_warp(&sm.o_done[X], no & 1)) break;
             ++no;
             tc05::fence_after_thread_sync();
-            const float inv = 1.f / l;
             uint4* dst = reinterpret_cast<uint4*>((uint16_t*)a.output + ((long long)(it.t0 + i) * m.H + a.h0 + it.h) * DV);
+            auto put = [&](int q, const uint32_t (&o)[32], float factor) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = pack2<BF>(__uint_as_float(o[c + 2 * e]) * factor, __uint_as_float(o[c + 2 * e + 1]) * factor);
+                    dst[4 * q + c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            };
+            // of a cut context: rows of sums, four elements of 256 rows together
+            float4* part = reinterpret_cast<float4*>(a.part_o) + (long long)(it.slot + it.piece * a.heads) * (DV / 4) * kQueryTile + i;
 #pragma unroll 1
             for (int q = 0; q < DV / 32; ++q) {
                 uint32_t o[32];
                 tc05::ld_32x32b_x32(tmem_o + 32 * q, o);
                 tc05::wait_ld();
-                if (limit > 0) {
+                if (i < it.rows) {
+                    if (it.slot < 0) put(q, o, 1.f / l);
+                    else
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        uint32_t w[4];
+                        for (int c = 0; c < 32; c += 4)
+                            part[(8 * q + c / 4) * kQueryTile] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+                }
+            }
+            if (it.slot >= 0) {
+                // The warp that is the last of its rows' pieces joins them, in the pieces' order.
+                if (i < it.rows) a.part_ml[(long long)(it.slot + it.piece * a.heads) * kQueryTile + i] = make_float2(top, l);
+                __threadfence();
+                __syncwarp();
+                int before = 0;
+                if (lane == 0) before = atomicAdd(a.arrived + ((long long)a.pass * a.part_slots + it.slot) * 8 + warp, 1);
+                if (__shfl_sync(0xffffffffu, before, 0) + 1 == it.pieces[X]) {
+                    __threadfence();
+                    if (i < it.rows) {
+                        const float2* ml = a.part_ml + (long long)it.slot * kQueryTile + i;
+                        const long long step = (long long)a.heads * kQueryTile;
+                        float most = -INFINITY, sum = 0.f;
+                        for (int k = 0; k < it.pieces[X]; ++k) {
+                            const float2 x = __ldcg(ml + k * step);
+                            if (x.y == 0.f) continue;       // (a piece that the row does not see)
+                            const float to = fmaxf(most, x.x);
+                            sum = (most == -INFINITY ? 0.f : sum * ex2(most - to)) + x.y * ex2(x.x - to);
+                            most = to;
+                        }
+                        part = reinterpret_cast<float4*>(a.part_o) + (long long)it.slot * (DV / 4) * kQueryTile + i;
+#pragma unroll 1
+                        for (int q = 0; q < DV / 32; ++q) {
+                            float y[32] = {};
+#pragma unroll 2
+                            for (int k = 0; k < it.pieces[X]; ++k) {
+                                const float2 x = __ldcg(ml + k * step);
+                                const float f = x.y == 0.f ? 0.f : ex2(x.x - most);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack2<BF>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
-                        dst[4 * q + c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                                for (int c = 0; c < 32; c += 4) {
+                                    const float4 z = __ldcg(part + k * step * (DV / 4) + (8 * q + c / 4) * kQueryTile);
+                                    y[c] += f * z.x; y[c + 1] += f * z.y; y[c + 2] += f * z.z; y[c + 3] += f * z.w;
+                                }
+                            }
+                            uint32_t o[32];
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(y[c]);
+                            put(q, o, 1.f / sum);
+                        }
                     }
                 }
             }

@@ -88,13 +88,24 @@ cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t strea
 constexpr int kExpandTile = 128;   // context tokens of a tile
 constexpr int kQueryTile = 256;    // new tokens of a work item, in two halves
 
+// A query tile's piece of context: `length` tiles from number piece * length.
+struct PieceOfQuery {
+    int s, tile, piece, length;
+    int slot;                   // of the tile's first piece, -1: the only one
+};
+
 struct ExpandedArgs {
     Step m;
     int h0, heads;              // heads of this pass
     long long rows;             // rows of a head's scratch
     int* tile_prefix;           // [num_sequences + 1] context tiles
     int* query_prefix;          // [num_sequences + 1] query tiles
-    int2* order;                // (sequence, query tile), longest context first
+    PieceOfQuery* order;        // the longest first
+    int* items;                 // their number
+    int* arrived;               // [passes][part_slots][8] pieces done, of every 32 rows
+    int part_slots;             // (pieces, heads) of query tiles with more than one piece
+    float* part_o;              // [part_slots][value / 4][kQueryTile][4] their sums
+    float2* part_ml;            // [part_slots][kQueryTile] maximum and denominator
     int* heads_per_item;        // heads that a CTA makes keys and values of for one context tile
     int* counter;               // [passes] work counters
     int pass, passes, ctas;

@@ -252,6 +252,19 @@ def test_offsets_beyond_32_bits(pkg, form):
 
 
 # ---- bad metadata ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sizes,dtype,bs", [(LH.WIDE, "bf16", 64), (LH.SMALL, "f16", 16), (LH.MIXED, "bf16", 32)])
+@pytest.mark.parametrize("heads,past,new", [(1, [9000], [1]), (3, [2500, 0, 1300, 5000], [300, 200, 129, 1]), (2, [4096 - 256, 4000], [256, 257])])
+def test_contexts_that_are_cut(pkg, heads, past, new, sizes, dtype, bs):
+    """Few query tiles over long contexts: their pieces are computed apart and joined."""
+    st = LH.Step(past, new, heads=heads, sizes=sizes, bs=bs, dtype=dtype, seed=21)
+    op = st.operator(pkg)
+    x = st.device_inputs()
+    first = st.attend(op, "expanded", x)
+    st.check(first)
+    assert torch.equal(first, st.attend(op, "expanded", x))      # the pieces join in their order, whichever is last
+    assert op.device_status() == 0
+
+
 BAD_INDEX, BAD_BEGINS, BAD_PAST, BAD_ROTATION = 1, 2, 4, 8
 
 
