@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     }
     if (warp == 5) tc05::tmem_alloc(&sm.tmem_base, 512);
     pa::grid_wait();
+    pa::grid_release();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -488,7 +489,6 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
         sm.abort_flag = 0;
     }
     if (warp == 9) tc05::tmem_alloc(&sm.tmem_base, 512);
-    pa::grid_wait();
     tc05::fence_before_thread_sync();
     __syncthreads();
     tc05::fence_after_thread_sync();
@@ -510,9 +510,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             uint32_t ni = 0, nk = 0, nq[2] = {0, 0};
             bool ok = true;
             while (ok) {
-                int i = 0;
-                if (lane == 0) i = atomicAdd(a.counter + a.pass, 1);
-                i = __shfl_sync(0xffffffffu, i, 0);
+                int i = blockIdx.x;              // the first item goes by the CTA's number, later ones by turn
+                if (ni > 0) {
+                    if (lane == 0) i = gridDim.x + atomicAdd(a.counter + a.pass, 1);
+                    i = __shfl_sync(0xffffffffu, i, 0);
+                }
                 QueryItem it;
                 it.h = -1;
                 if (i < items) {
@@ -534,6 +536,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         it.pieces[x] = (tiles + at.length - 1) / at.length;
                     }
                 }
+                // (the plan and the step's tables do not come from the kernel before, whose CTAs have all begun; keys and values do)
+                if (ni == 0) pa::grid_wait();
                 const int slot = ni % kItemSlots;
                 if (ni >= kItemSlots) ok = wt.wait_warp(&sm.item_free[slot], (ni / kItemSlots - 1) & 1);
                 if (!ok) break;
@@ -578,6 +582,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             }
         } else if (warp == 10) {
             // ======================= loader of the values ====================================================
+            pa::grid_wait();
             uint32_t nv = 0;
             bool ok = true;
             QueryItem it;
@@ -827,22 +832,26 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         }
                         part = reinterpret_cast<float4*>(a.part_o) + (long long)it.slot * (DV / 4) * kQueryTile + i;
 #pragma unroll 1
-                        for (int q = 0; q < DV / 32; ++q) {
-                            float y[32] = {};
+                        for (int q = 0; q < DV / 32; q += 2) {
+                            float y[2][32] = {};
 #pragma unroll 2
                             for (int k = 0; k < it.pieces[X]; ++k) {
                                 const float2 x = __ldcg(ml + k * step);
                                 const float f = x.y == 0.f ? 0.f : ex2(x.x - most);
 #pragma unroll
-                                for (int c = 0; c < 32; c += 4) {
+                                for (int c = 0; c < 64; c += 4) {
                                     const float4 z = __ldcg(part + k * step * (DV / 4) + (8 * q + c / 4) * kQueryTile);
-                                    y[c] += f * z.x; y[c + 1] += f * z.y; y[c + 2] += f * z.z; y[c + 3] += f * z.w;
+                                    float* to = &y[c >> 5][c & 31];
+                                    to[0] += f * z.x; to[1] += f * z.y; to[2] += f * z.z; to[3] += f * z.w;
                                 }
                             }
-                            uint32_t o[32];
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(y[c]);
-                            put(q, o, 1.f / sum);
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t o[32];
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(y[e][c]);
+                                put(q + e, o, 1.f / sum);
+                            }
                         }
                     }
                 }
