@@ -902,13 +902,13 @@ __global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) p
     if (warp == kJoinWarps) tc05::tmem_dealloc(sm.tmem_base, 64);
 }
 
-int query_smem(const Step& m) { return 2 * m.Dn * 128 + m.Dn / 64 * 8192; }
+int query_smem(int Dn) { return 2 * Dn * 128 + Dn / 64 * 8192; }
 
 template <int R, bool BF>
 cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
     const Step& m = a.m;
     const int token_tiles = (m.num_tokens + kTile - 1) / kTile;
-    cudaError_t e = pa::launch_dependent(project_query_kernel<BF>, 1 + token_tiles * m.H * (R / 128), 128, query_smem(m), stream, a);
+    cudaError_t e = pa::launch_dependent(project_query_kernel<BF>, 1 + token_tiles * m.H * (R / 128), 128, query_smem(m.Dn), stream, a);
     if (e == cudaSuccess) e = pa::launch_dependent(attend_kernel<R, BF>, a.groups * a.row_tiles, kThreads, sizeof(AttendSmem<R>), stream, a);
     if (e == cudaSuccess) {
         // tiles of 16 tokens where those of 64 would leave SMs without one; in an AUTO step most tokens may be the expanded form's
@@ -924,7 +924,8 @@ cudaError_t launch(const AbsorbedArgs& a, cudaStream_t stream, int* launches) {
 
 template <int R, bool BF>
 cudaError_t prepare(const Step& m) {
-    cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, query_smem(m));
+    // (for the largest size: the kernel serves operators of several, and the limit is the kernel's)
+    cudaError_t e = cudaFuncSetAttribute(project_query_kernel<BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, query_smem(128));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_kernel<R, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(AttendSmem<R>));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<R, 16, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ValueSmem<R, 16>));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(project_value_kernel<R, 64, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ValueSmem<R, 64>));

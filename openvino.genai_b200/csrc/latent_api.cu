@@ -33,6 +33,7 @@ int fail(int code, const char* msg) {
 }
 
 int fail_cuda(const char* what, cudaError_t e) {
+    cudaGetLastError();      // (told to this caller, not to whoever asks the runtime next)
     pa::set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
     return PA_ERR_CUDA;
 }

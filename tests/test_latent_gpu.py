@@ -265,6 +265,16 @@ def test_contexts_that_are_cut(pkg, heads, past, new, sizes, dtype, bs):
     assert op.device_status() == 0
 
 
+@pytest.mark.parametrize("form", ["absorbed", "expanded", "auto"])
+def test_operators_of_several_sizes_take_turns(pkg, form):
+    steps = [LH.Step([70, 200], [1, 90], heads=4, sizes=sizes, bs=32, seed=7) for sizes in (LH.WIDE, LH.SMALL, LH.MIXED)]
+    ops = [st.operator(pkg) for st in steps]
+    for _ in range(2):
+        for st, op in zip(steps, ops):
+            st.check(st.attend(op, form))
+            assert op.device_status() == 0
+
+
 BAD_INDEX, BAD_BEGINS, BAD_PAST, BAD_ROTATION = 1, 2, 4, 8
 
 
