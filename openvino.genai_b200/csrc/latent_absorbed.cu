@@ -101,7 +101,8 @@ __device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&
 
 // ---- q~ = key_up^T q ----------------------------------------------------------------------------------------------------
 // A CTA computes 128 latent elements of 64 tokens of one head: D[latent][token] with the weight's rows (d, latent contiguous) as an
-// MN-major operand, one tile of each operand, so the CTAs of an SM overlap one another's loads, products and stores.
+// MN-major operand, one tile of each operand, so the CTAs of an SM overlap one another's loads, products and stores.  q~ is rounded to 16 bits: it is
+// an operand of the attention's products.  9 us for one row by 128 heads (34 MB of weights), 6 of them the chain plan -> loads -> product -> stores.
 template <bool BF>
 __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constant__ AbsorbedArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -189,10 +190,13 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
 //   S[row][token]     = Q~ K^T          M 64, N 64, K R + P; two buffers, so that S of the next tile is computed beside a softmax
 //   O^T[latent][row] += K^T P^T         M 128 (R / 128 times), N 64, K 64: the tile is read MN-major from the same image, and the
 //                                       rows (heads) are columns, so few heads leave no tensor-memory lane idle
-// A tile lies in shared memory in groups of eight tokens, [group][64-element chunk][8 tokens][64]: that is one box of a four-dimensional view of
-// the cache, so a block is two copies (the rotated part is the other); issuing one for every chunk took 900 cycles.  Its halves of 32 tokens come
-// and are freed by themselves.
+// A tile lies in shared memory in parts of 128 latent elements, a part in groups of eight tokens, [group][64-element chunk][8 tokens][64]: that is one box of
+// a four-dimensional view of the cache.  Two tiles of 512 are all that fits beside the query rows, so the parts come, are multiplied and are freed by
+// themselves: one row over 120 k tokens by 128 heads 80.0 us with halves of 32 tokens, 77.5 so.
 // S and O are issued by a warp each: one warp for both had to look at two barriers in turn, and a look, with what follows it, is 200 cycles.
+// Weights and q~ go in as 16 bits, because both operands of a step have one type; maxima, sums and O are 32 bits, O unscaled until the pieces are joined.
+// 64 rows by 128 heads over 259,540 tokens (338 MB): 108 us, tensor pipe 50 % busy, HBM 39 %.  A tile takes 3200 cycles of which the products are 1950; the
+// rest is the chain S -> softmax (1150) -> P -> O -> tile free -> load (1500, from the L2 cache) with two tiles in flight.
 // Tiles of 32 tokens, four in flight, were no faster: an M 64, N 32 step takes 26 cycles, one of N 64 33.
 constexpr int kSlots = 4;               // depth of the queue of runs
 constexpr int kThreads = 384;           // warps 0 - 3: softmax, 4: loader, 5: S, 6: O, 8 - 11: rescaling and results (a warp reads the tensor-memory lanes of its number mod 4)

@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
     __syncthreads();
     // Query tiles are cut along their context where they are too few for the CTAs: into the pieces whose rounds over the CTAs end first, at two tiles to a
     // piece for its beginning and end, and three for the joining.  None is shorter than a CTA's share of all tiles, and a cut tile has more than one
-    // piece's worth, so that there are at most 2 * ctas pieces of cut ones.  (Three prompts by 16 heads, 96 tiles of up to 20 x 128 context tokens, beside 40
-    // rows of one token: 146 us uncut, 134 in pieces of at most 12, 151 in pieces of 8, which take a second round.)
+    // piece's worth, so that there are at most 2 * ctas pieces of cut ones.  (Three prompts by 16 heads, 96 tiles of 7 to 19 x 128 context tokens, beside 40
+    // rows of one token: 146 us uncut, 134 in pieces of at most 10, 151 in pieces of 8, which take a second round.)
     const int total = run_q;
     auto place = [&](int i, int& s, int& qt) {       // context tiles of query tile i
         if (i < kListed) {
@@ -171,7 +171,9 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
 // weights streamed in chunks of 64 latent elements.  Keys and values have an accumulator each, so that one is written out while the other is
 // computed.  The rows go from the cache to shared memory (the next tile's beside this one's products) and from there to tensor memory, because an
 // M 128, N 128 step with both operands in shared memory takes all of that memory's bandwidth and leaves none for the weights to come in:
-// 129 us for 10 k rows by 32 heads of 512 -> 128 + 128.
+// 13,143 rows by 32 heads of 512 -> 128 + 128 take 112 us (tensor pipe 49 % busy, 157 MB of the results written back).  A head's tile takes 7000 cycles
+// and its products 4096: the weights, which every tile brings in again from the L2 cache, arrive no faster beside them.
+// Keys and values are rounded to 16 bits, as operands of the attention's products.
 constexpr int kExpandThreads = 224;    // warps 0 - 3: output, 4: rows and even chunks of weights, 5: products, 6: odd chunks (one warp takes 450 cycles a chunk, the products 256)
 
 // A place in a ring of N barriers and the phase that it waits for.
@@ -423,6 +425,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
 // with P read from TMEM; the tensor core computes P V and the next S of one half beside the softmax of the other.
 // Warps 0 - 3 and 4 - 7: softmax of A and B, a thread per row; 8: queries and keys, 9: products, 10: values;
 // 11 fills the warpgroup whose registers go to the softmax.
+// P is rounded to 16 bits because P and V are one type to the tensor core; S, maxima, sums and O are 32 bits, O is divided once.
+// 4 prompts of 1313 - 1891 tokens over 1280 - 1936 by 32 heads (334 GFLOP): 325 us, 1030 TFLOP/s, tensor pipe 53 % busy.  A context tile of both
+// halves takes 3850 cycles and its products 2560.  A half's chain is softmax 1840 (maximum 380, 650 for the exponentials of 64 tokens, which is their
+// unit's rate) and products 1470, and S may not be overwritten before P is read: O, S and P of both halves fill the tensor memory.  Slower, by the call:
+// a third of the exponentials by polynomials (+2 %), the maximum beside the exponentials of a stale one (+1 %), one wait for keys, values and
+// P (+3 %), a warp for each half's products (+9 %).
 constexpr int kAttendThreads = 384;
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 and 128 threads of the 384 x 168 that the CTA is launched with
 constexpr int kItemSlots = 4;

@@ -23,9 +23,9 @@ struct Step {
 };
 
 // Form of a sequence in an AUTO step.  With n new tokens over L tokens of context the absorbed form costs a n L and the expanded one b n L + c L, so the
-// number of new tokens decides: with 4 and with 16 sequences of 2000 cached tokens by 64 heads, 64 new tokens each took 169 us absorbed and 223
-// expanded, 96 took 245 and 223, 128 322 and 221.  Short contexts leave the absorbed form with more results than work (16 sequences of 64 tokens by
-// 16 heads 67 and 32 us).
+// number of new tokens decides: with 4 sequences of 2000 cached tokens by 64 heads, 64 new tokens each took 158 us absorbed and 220
+// expanded, 96 took 225 and 222, 128 299 and 219 (with 16 sequences 622 and 898, 913 and 889, 1229 and 884).  Short contexts leave the absorbed form with
+// more results than work (16 sequences of 64 tokens by 16 heads 62 and 35 us).
 constexpr int kAutoMaxNew = 80, kAutoFewNew = 16, kAutoContext = 8;
 
 struct AppendArgs {

@@ -10,7 +10,6 @@
 
 namespace latent {
 
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(pa::smem_u32(dst)),

@@ -1,6 +1,7 @@
 """Latent attention on the GPU against its definition in 64 bits: the cache append, both forms of the attention, odd lengths, strides,
 streams, bad metadata."""
 import math
+import pathlib
 
 import numpy as np
 import pytest
@@ -273,6 +274,16 @@ def test_operators_of_several_sizes_take_turns(pkg, form):
         for st, op in zip(steps, ops):
             st.check(st.attend(op, form))
             assert op.device_status() == 0
+
+
+def test_example_layer():
+    """The layer of integration/latent_layer.py over mixed steps.  Seven roundings to bfloat16 (2^-9 each) lie between its input and its output:
+    projections, rotation or norm, q~ or keys and values, weights, output, projection."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("latent_layer", pathlib.Path(__file__).resolve().parents[1] / "integration" / "latent_layer.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main() < 7 * 2.0 ** -9
 
 
 BAD_INDEX, BAD_BEGINS, BAD_PAST, BAD_ROTATION = 1, 2, 4, 8
