@@ -276,6 +276,21 @@ def test_operators_of_several_sizes_take_turns(pkg, form):
             assert op.device_status() == 0
 
 
+@pytest.mark.parametrize("heads,past,new", [(32, [120000], [200]), (24, [90000, 40000, 3], [300, 5, 40])])
+def test_scratch_of_several_passes(pkg, heads, past, new):
+    """Keys and values of these contexts do not fit the scratch at once: the heads are served in passes, their contexts cut in each.  Each form is within
+    2 u of the definition, so the two are within 4 u of one another."""
+    st = LH.Step(past, new, heads=heads, bs=64, seed=3)
+    op = st.operator(pkg)
+    x = st.device_inputs()
+    absorbed = st.attend(op, "absorbed", x).double()
+    before = op.launch_count()
+    expanded = st.attend(op, "expanded", x)
+    assert op.launch_count() - before == 5      # the plan, two passes of two
+    assert float((expanded.double() - absorbed).norm() / absorbed.norm()) < 4 * LH.UNIT["bf16"]
+    assert torch.equal(expanded, st.attend(op, "expanded", x)) and op.device_status() == 0
+
+
 def test_example_layer():
     """The layer of integration/latent_layer.py over mixed steps.  Seven roundings to bfloat16 (2^-9 each) lie between its input and its output:
     projections, rotation or norm, q~ or keys and values, weights, output, projection."""
