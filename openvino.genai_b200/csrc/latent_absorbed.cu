@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) p
 #pragma unroll
             for (int u = 0; u < kRows; ++u) {
                 const int r = (warp >> spread) + u * kJoinWarps;
-                part[u] = r < rows ? a.row_part[(long long)sm.token[r] * m.H + h] : make_int2(0, 0);
+                part[u] = r < rows ? checked_part(a.row_part[(long long)sm.token[r] * m.H + h], step, a.part_rows) : make_int2(0, 0);
             }
             auto load = [&](float4 (&q)[V], const int2& row, int piece) {
                 const float4* src = reinterpret_cast<const float4*>(a.part_o + (row.x + (long long)piece * step) * R) + lane;

@@ -122,6 +122,7 @@ constexpr size_t kExpandBytes = (size_t)1 << 30;
 
 struct Scratch {
     int row_tiles, groups;
+    long long part_rows;
     size_t unit_prefix, block_prefix, token_prefix, starts, q_abs, part_o, part_ml, row_part;
     int heads, passes;       // expanded: heads of a pass
     long long rows;
@@ -142,15 +143,15 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         const size_t rows = (size_t)tokens * d.num_heads;
         // in an AUTO step only the short sequences' rows have partial results
         const int most = form == PA_LATENT_AUTO ? (int)std::min<long long>(tokens, (long long)sequences * latent::kAutoMaxNew) : tokens;
-        const size_t slots = (size_t)latent::absorbed_slots(most, sequences, d.num_heads, s.groups, s.row_tiles);
+        s.part_rows = latent::absorbed_slots(most, sequences, d.num_heads, s.groups, s.row_tiles) * latent::kTile;
         s.unit_prefix = take(((size_t)sequences + 1) * sizeof(long long));
         s.block_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.token_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.starts = take(s.groups * sizeof(latent::SliceStart));
         s.q_abs = take(rows * (d.latent_size + d.rope_size) * 2);
         s.row_part = take(rows * sizeof(int2));
-        s.part_ml = take(slots * latent::kTile * sizeof(float2));
-        s.part_o = take(slots * latent::kTile * d.latent_size * sizeof(float));
+        s.part_ml = take((size_t)s.part_rows * sizeof(float2));
+        s.part_o = take((size_t)s.part_rows * d.latent_size * sizeof(float));
     }
     if (form == PA_LATENT_EXPANDED || (form == PA_LATENT_AUTO && tokens > latent::kAutoFewNew)) {
         const int served = form == PA_LATENT_AUTO ? std::min(sequences, tokens / (latent::kAutoFewNew + 1)) : sequences;
@@ -275,6 +276,7 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
         k.part_o = (float*)(h->ws + s.part_o);
         k.part_ml = (float2*)(h->ws + s.part_ml);
         k.row_part = (int2*)(h->ws + s.row_part);
+        k.part_rows = s.part_rows;
         k.output = a->output;
         k.scale_log2 = scale * 1.4426950408889634f;
         const int W = R + P;

@@ -75,10 +75,17 @@ struct AbsorbedArgs {
     float* part_o;              // [slot][64][R]
     float2* part_ml;            // [slot][64] maximum (base 2, scaled) and sum
     int2* row_part;             // [num_tokens * H] a row's first partial result (slot * 64 + row of the tile) and how many it has
+    long long part_rows;        // rows of part_o and part_ml
     void* output;
     float scale_log2;           // softmax scale * log2(e)
     CUtensorMap map_qn, map_key_up, map_q_abs, map_q_abs_rope, map_cache, map_cache_part, map_cache_rope, map_value_up;
 };
+// A row's record as the join may follow it: its `part.y` partial results lie `step` rows apart among the `rows` of the scratch.  A record that the
+// attention left unwritten, because a wait of its CTA ran out, is whatever an earlier call had there: one that leads outside has no results.
+__host__ __device__ inline int2 checked_part(int2 part, int step, long long rows) {
+    const bool inside = part.x >= 0 && part.y > 0 && part.x + (part.y - 1LL) * step < rows;
+    return inside ? part : make_int2(0, 0);
+}
 // Largest number of slots a step can need.
 long long absorbed_slots(int tokens, int sequences, int heads, int groups, int row_tiles);
 cudaError_t launch_absorbed(const AbsorbedArgs& a, int dtype, cudaStream_t stream, int* launches);
