@@ -7,6 +7,7 @@ import struct
 PA_LATENT_AUTO = 0
 PA_LATENT_ABSORBED = 1
 PA_LATENT_EXPANDED = 2
+PA_DEV_WAIT_TIMEOUT_LATENT = 0x10000000
 
 
 class pa_latent_desc(C.Structure):

@@ -106,7 +106,7 @@ __device__ __forceinline__ bool tile_rows(const AbsorbedArgs& a, int t0, bool (&
 template <bool BF>
 __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constant__ AbsorbedArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full, done;
+    __shared__ uint64_t full, done, idle;
     __shared__ bool live[kTile];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag;
@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
     if (tid == 0) {
         pa::mbar_init(&full, 1);
         pa::mbar_init(&done, 1);
+        pa::mbar_init(&idle, 1);
         pa::mbar_fence_init();
         abort_flag = 0;
         for (int c = 0; c < 2; ++c) prefetch_3d(&a.map_key_up, part * 128 + c * 64, 0, h);
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
     tc05::fence_before_thread_sync();
     const bool any = tile_rows(a, t0, live);
     tc05::fence_after_thread_sync();
-    const Waiter wt{&abort_flag, m.status};
+    const Waiter wt{&abort_flag, m.status, m.wait_polls};
     const uint32_t tmem = tmem_base;
     bool ok = wt.wait(&full, 0);
     if (any && warp == 0 && __all_sync(0xffffffffu, ok)) {
@@ -180,7 +181,13 @@ __global__ void __launch_bounds__(128) project_query_kernel(const __grid_constan
     }
     tc05::fence_before_thread_sync();
     __syncthreads();
-    if (warp == 0) tc05::tmem_dealloc(tmem, 64);
+    if (warp == 0) {
+        if (*(volatile int*)&abort_flag) {
+            drain(&full, 0);
+            drain_products(&idle);
+        }
+        tc05::tmem_dealloc(tmem, 64);
+    }
     (void)lane;
 }
 
@@ -239,6 +246,7 @@ struct AttendSmem {
     uint64_t s_full[2], s_free[2];                  // products -> softmax, softmax -> products
     uint64_t p_full, o_done;                        // softmax -> products, products -> softmax and results
     uint64_t asked, answered;                       // products -> results, results -> products
+    uint64_t idle[2];                               // after an abort, of the two warps that issue products
     // softmax -> results, runs in turn.  The softmax gets at most a run ahead of the results: a tile's P waits for the products of the tile
     // before, and a run's first products wait for the results of the run before
     uint64_t stat_full[2];
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         for (int i = 0; i < NQ * NST; ++i) { pa::mbar_init(&sm.k_full[0][i], 1); pa::mbar_init(&sm.k_free[0][i], 1); }
         pa::mbar_init(&sm.q_full, 1);
         pa::mbar_init(&sm.q_free, 1);
-        for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.s_full[i], 1); pa::mbar_init(&sm.s_free[i], 4); pa::mbar_init(&sm.stat_full[i], 4); }
+        for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.s_full[i], 1); pa::mbar_init(&sm.s_free[i], 4); pa::mbar_init(&sm.stat_full[i], 4); pa::mbar_init(&sm.idle[i], 1); }
         pa::mbar_init(&sm.p_full, 4);
         pa::mbar_init(&sm.o_done, 1);
         pa::mbar_init(&sm.asked, 1);
@@ -280,7 +288,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
     __syncthreads();
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
-    const Waiter wt{&sm.abort_flag, m.status};
+    const Waiter wt{&sm.abort_flag, m.status, m.wait_polls};
+    uint32_t queries = 0, parts = 0;      // loader: query tiles and parts of context tiles that it has asked for
     // The next run of the queue; false: a wait ran out.
     auto fetch = [&](uint32_t n, Run& r) -> bool {
         const int slot = n % kSlots;
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         int s = start.s, block = start.block, first = start.first, left = start.units;     // left: units of the slice
         SeqView v{start.t0, start.n, start.past, start.tb};
         int blocks = start.blocks, tiles = start.tiles, block0 = start.block0;
-        uint32_t n = 0, nr = 0, nq = 0;      // tiles, queue entries, query tiles so far
+        uint32_t n = 0, nr = 0;              // tiles, queue entries so far
         const uint64_t policy = evict_first();
         bool ok = true, bad_index = false;
         auto publish = [&](const Run& r) -> bool {
@@ -335,14 +344,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                 r.pieces = first > 0 ? 0 : 1 + max(0, tiles - left + start.per - 1) / start.per;
                 ok = publish(r);
                 if (ok && r.tiles > 0) {
-                    if (nq > 0) ok = wt.wait_warp(&sm.q_free, (nq - 1) & 1);
+                    if (queries > 0) ok = wt.wait_warp(&sm.q_free, (queries - 1) & 1);
                     if (ok && tc05::elect_one()) {
                         pa::mbar_expect_tx(&sm.q_full, kTile * (R * 2 + 128));     // (rows behind the tile's are other rows' or zeros)
                         tma_3d(sm.q, &a.map_q_abs, 0, (int)r.grow0, 0, &sm.q_full);
                         tma_2d(sm.q_rope, &a.map_q_abs_rope, 0, (int)r.grow0, &sm.q_full);
                     }
                     __syncwarp();
-                    ++nq;
+                    queries += ok;
                     // pieces of a half tile: 32 tokens of a block, or two blocks of 16 (all powers of two)
                     const int bs_log2 = 31 - __clz(m.bs), piece_log2 = min(bs_log2, 5), piece = 1 << piece_log2, pieces = 32 >> piece_log2;
                     const int sub_log2 = bs_log2 - piece_log2, last_piece = (r.end - 1) >> piece_log2;
@@ -380,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
                                     }
                             }
                             __syncwarp();
+                            ++parts;
                         }
                         // tiles to come go to the L2 cache meanwhile (the CTAs of a group take turns): two tiles in flight do not cover the memory's latency
                         for (int ahead = j == 0 ? NST : kAheadOf<R>; ahead <= kAheadOf<R>; ++ahead)
@@ -404,12 +414,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
             publish(r);
         }
         if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
-        // what was issued has to have arrived before the CTA's memory is given back
-        if (sm.abort_flag) {
-            if (nq > 0) drain(&sm.q_full, (nq - 1) & 1);
-            for (uint32_t i = n + 1 > NST ? n + 1 - NST : 0; i <= n; ++i)      // (of tile n a part may be under way)
-                for (int q = 0; q < NQ; ++q) drain(&sm.k_full[i % NST][q], (i / NST) & 1);
-        }
     } else if (warp == 5) {
         // ======================= S ========================================================================
         // (the whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took twice as long to issue)
@@ -657,6 +661,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         }
     }
     __syncthreads();
+    if (*(volatile int*)&sm.abort_flag) {
+        if (warp == 4) {
+            constexpr uint32_t kParts = NST * NQ;
+            if (queries > 0) drain(&sm.q_full, (queries - 1) & 1);
+            for (uint32_t i = parts > kParts ? parts - kParts : 0; i < parts; ++i) drain(&sm.k_full[0][0] + i % kParts, (i / kParts) & 1);
+        } else if (warp == 5 || warp == 6) drain_products(&sm.idle[warp - 5]);
+        __syncthreads();
+    }
     if (warp == 5) tc05::tmem_dealloc(tmem, 512);
 }
 
@@ -676,7 +688,7 @@ struct ValueSmem {
     static constexpr int NC = R / 64, NW = 4;                    // chunks of 64 latent elements, of which weights are in flight
     alignas(1024) uint8_t o[2][NC][NT * 128];                    // joined rows, high and low pieces
     alignas(1024) uint8_t w[NW][128 * 128];
-    uint64_t w_full[NW], w_free[NW], o_full, done;
+    uint64_t w_full[NW], w_free[NW], o_full, done, idle;
     int token[NT];
     uint32_t tmem_base;
     int abort_flag;
@@ -700,12 +712,13 @@ __global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) p
         for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
         pa::mbar_init(&sm.o_full, kJoinWarps);
         pa::mbar_init(&sm.done, 1);
+        pa::mbar_init(&sm.idle, 1);
         pa::mbar_fence_init();
         sm.abort_flag = 0;
     }
     __syncthreads();
     if (warp == kJoinWarps) tc05::tmem_alloc(&sm.tmem_base, 64);
-    const Waiter wt{&sm.abort_flag, m.status};
+    const Waiter wt{&sm.abort_flag, m.status, m.wait_polls};
     uint32_t parity = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
         const int h = tile % m.H, c0 = tile / m.H * NT, rows = min(NT, count - c0);
@@ -903,7 +916,10 @@ __global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) p
         tc05::fence_after_thread_sync();
         if (*(volatile int*)&sm.abort_flag) break;
     }
-    if (warp == kJoinWarps) tc05::tmem_dealloc(sm.tmem_base, 64);
+    if (warp == kJoinWarps) {
+        if (*(volatile int*)&sm.abort_flag) drain_products(&sm.idle);
+        tc05::tmem_dealloc(sm.tmem_base, 64);
+    }
 }
 
 int query_smem(int Dn) { return 2 * Dn * 128 + Dn / 64 * 8192; }

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <new>
 #include <string>
 
@@ -23,6 +24,7 @@ struct pa_latent_handle {
     uint8_t* ws = nullptr;        // kernel scratch
     size_t ws_bytes = 0;
     int64_t launches = 0;
+    uint32_t wait_polls = latent::kWaitPolls;   // env PA_B200_LATENT_TEST_WAIT_POLLS: the kernels' bounded waits are made to run out
 };
 
 namespace {
@@ -205,7 +207,7 @@ latent::Step make_step(const pa_latent_handle* h, const Args* a) {
     const pa_latent_desc& d = h->desc;
     return latent::Step{d.num_heads, d.latent_size, d.rope_size, d.nope_size, d.value_size, d.block_size,
                         a->num_tokens, a->num_sequences, a->num_block_indices, a->num_blocks,
-                        a->past_lens, a->subsequence_begins, a->block_indices, a->block_indices_begins, h->status, PA_LATENT_AUTO};
+                        a->past_lens, a->subsequence_begins, a->block_indices, a->block_indices_begins, h->status, PA_LATENT_AUTO, h->wait_polls};
 }
 
 int append(pa_latent_handle* h, const pa_latent_append_args* a) {
@@ -364,6 +366,7 @@ int pa_b200_latent_create(const pa_latent_desc* desc, int device, pa_latent_hand
         h->desc = *desc;
         h->device = device;
         h->sm_count = prop.multiProcessorCount;
+        if (const char* e = std::getenv("PA_B200_LATENT_TEST_WAIT_POLLS")) h->wait_polls = (uint32_t)std::max(0, std::min(std::atoi(e), (int)latent::kWaitPolls));
         cudaError_t e = cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking);
         if (e == cudaSuccess) e = cudaMalloc((void**)&h->status, 256);
         if (e == cudaSuccess) e = cudaMemset(h->status, 0, 256);

@@ -193,6 +193,8 @@ struct ExpandSmem {
     alignas(1024) uint8_t out[kExpandTile * 128];            // 64 elements of every row on their way to global memory
     uint64_t a_full, a_free, a_ready;                        // rows in shared memory, read, in tensor memory
     uint64_t w_full[NW], w_free[NW], d_full[2], d_free[2];   // weights; accumulators of keys and values
+    uint64_t idle;                                           // after an abort
+    uint32_t asked[3];                                       // the loaders' last words: context tiles, chunks of weights up to each one's last
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -238,6 +240,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
         pa::mbar_init(&sm.a_full, 1);
         pa::mbar_init(&sm.a_free, 4);
         pa::mbar_init(&sm.a_ready, 4);
+        pa::mbar_init(&sm.idle, 1);
         for (int i = 0; i < NW; ++i) { pa::mbar_init(&sm.w_full[i], 1); pa::mbar_init(&sm.w_free[i], 1); }
         for (int i = 0; i < 2; ++i) { pa::mbar_init(&sm.d_full[i], 1); pa::mbar_init(&sm.d_free[i], 4); }
         pa::mbar_fence_init();
@@ -250,15 +253,15 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
     __syncthreads();
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
-    const Waiter wt{&sm.abort_flag, m.status};
+    const Waiter wt{&sm.abort_flag, m.status, m.wait_polls};
     const int per = min(*a.heads_per_item, a.heads), items = a.tile_prefix[m.num_sequences] * ((a.heads + per - 1) / per);
     constexpr uint32_t kD = R / 2;       // tensor memory: the rows (two elements a column), then 128 columns each for keys and values
 
     if (warp == 4 || warp == 6) {
         const bool even = warp == 4;
-        uint32_t n = 0, na = 0;
+        uint32_t n = 0, tiles = 0, chunks = 0;
         bool ok = true, bad_index = false;
-        for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++na) {
+        for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
             const ExpandItem it = expand_item(a, i, per);
             if (even) {
                 int page = 0;
@@ -266,8 +269,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                     page = m.block_indices[it.block0 + lane];
                     if (page < 0 || page >= m.num_blocks) { page = 0; bad_index = true; }
                 }
-                if (na > 0) ok = wt.wait_warp(&sm.a_free, (na - 1) & 1);
+                if (tiles > 0) ok = wt.wait_warp(&sm.a_free, (tiles - 1) & 1);
                 if (!ok) break;
+                ++tiles;
                 if (tc05::elect_one()) pa::mbar_expect_tx(&sm.a_full, it.blocks * m.bs * 128 * NC);
                 __syncwarp();
                 for (int b = 0; b < it.blocks; ++b) {
@@ -287,13 +291,13 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
                         tma_3d(sm.w[st], x < NC ? &a.map_key_up : &a.map_value_up, 64 * (x % NC), 0, a.h0 + h, &sm.w_full[st]);
                     }
                     __syncwarp();
+                    if (ok) chunks = n + 1;
                 }
         }
         if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(m.status, PA_DEV_BAD_BLOCK_INDEX);
-        if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
-            for (uint32_t k = 0; even && na > 0 && k < (1u << 20) && !pa::mbar_try_wait(&sm.a_full, (na - 1) & 1); ++k) {}
-            for (uint32_t i = n > NW ? n - NW : 0; i < n; ++i)
-                for (uint32_t k = 0; (i & 1) != (even ? 1u : 0u) && k < (1u << 20) && !pa::mbar_try_wait(&sm.w_full[i % NW], (i / NW) & 1); ++k) {}
+        if (lane == 0) {
+            if (even) sm.asked[0] = tiles;
+            sm.asked[even ? 1 : 2] = chunks;
         }
     } else if (warp == 5) {
         constexpr uint32_t idesc_k = tc05::instr_desc_f16(128, DN, BF ? 1 : 0, 0, 0), idesc_v = tc05::instr_desc_f16(128, DV, BF ? 1 : 0, 0, 0);
@@ -417,6 +421,15 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_kernel(const __grid_
         __syncwarp();
     }
     __syncthreads();
+    if (*(volatile int*)&sm.abort_flag) {
+        if (warp == 4 || warp == 6) {
+            const uint32_t tiles = sm.asked[0], chunks = sm.asked[warp == 4 ? 1 : 2];
+            if (warp == 4 && tiles > 0) drain(&sm.a_full, (tiles - 1) & 1);
+            for (uint32_t i = chunks > NW ? chunks - NW : 0; i < chunks; ++i)      // (every other one is this warp's)
+                if ((i & 1) == (warp == 6 ? 1u : 0u)) drain(&sm.w_full[i % NW], (i / NW) & 1);
+        } else if (warp == 5) drain_products(&sm.idle);
+        __syncthreads();
+    }
     if (warp == 5) tc05::tmem_dealloc(tmem, 512);
 }
 
@@ -462,6 +475,8 @@ struct ExpandedSmem {
     alignas(1024) uint8_t v[VS][NV][64 * 128];
     uint64_t q_full[2], q_free[2], k_full[TK], k_free[KS], v_full[TV], v_free[VS];
     uint64_t s_full[2], p_full[2][2], o_done[2];
+    uint64_t idle;             // after an abort
+    uint32_t asked[4];         // the loaders' last words: query tiles of both halves, key atoms, value units that they have asked for
     uint64_t item_full[kItemSlots], item_free[kItemSlots];
     QueryItem item[kItemSlots];
     uint32_t tmem_base;
@@ -489,6 +504,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
             pa::mbar_init(&sm.p_full[x][1], 4);
             pa::mbar_init(&sm.o_done[x], 1);
         }
+        pa::mbar_init(&sm.idle, 1);
         for (int i = 0; i < KS; ++i) pa::mbar_init(&sm.k_free[i], 1);
         for (int i = 0; i < VS; ++i) pa::mbar_init(&sm.v_free[i], 1);
         for (int i = 0; i < TV; ++i) pa::mbar_init(&sm.v_full[i], 1);
@@ -501,7 +517,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
     __syncthreads();
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
-    const Waiter wt{&sm.abort_flag, m.status};
+    const Waiter wt{&sm.abort_flag, m.status, m.wait_polls};
     auto fetch = [&](uint32_t n, QueryItem& it) -> bool {
         const int slot = n % kItemSlots;
         if (!wt.wait_warp(&sm.item_full[slot], (n / kItemSlots) & 1)) return false;
@@ -563,7 +579,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                         tma_3d(sm.q[x][NQ - 1], &a.map_qr, 0, a.h0 + it.h, it.t0 + 128 * x, &sm.q_full[x]);
                     }
                     __syncwarp();
-                    ++nq[x];
+                    nq[x] += ok;
                 }
                 const int y0 = (int)(it.h * a.rows) + it.row;
                 auto load_k = [&](int j) {
@@ -582,12 +598,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                 };
                 for (int j = 0; ok && j < tiles; ++j) load_k(j);
             }
-            if (sm.abort_flag) {     // what was issued has to have arrived before the CTA's memory is given back
-                for (int x = 0; x < 2; ++x)
-                    if (nq[x] > 0) drain(&sm.q_full[x], (nq[x] - 1) & 1);
-                const uint32_t n = (nk + NQ - 1) / NQ;      // (the last may have begun only: its wait ends by the time that a copy can take)
-                for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) drain(&sm.k_full[i & 1], (i >> 1) & 1);
-            }
+            if (lane == 0) { sm.asked[0] = nq[0]; sm.asked[1] = nq[1]; sm.asked[2] = nk; }
         } else if (warp == 10) {
             // ======================= loader of the values ====================================================
             pa::grid_wait();
@@ -609,10 +620,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                     __syncwarp();
                 }
             }
-            if (sm.abort_flag) {
-                const uint32_t n = (nv + 1) / 2;
-                for (uint32_t i = n > TV ? n - TV : 0; i < n; ++i) drain(&sm.v_full[i % TV], (i / TV) & 1);
-            }
+            if (lane == 0) sm.asked[3] = nv;
         } else if (warp == 9) {
             // ======================= products ============================================================
             // The whole warp runs the loop and one elected lane issues: in code that a single lane runs, an instruction took 110 cycles to issue in
@@ -868,6 +876,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
         }
     }
     __syncthreads();
+    if (*(volatile int*)&sm.abort_flag) {
+        // (of a tile that has only begun to be asked for, the rest never comes: that wait ends by the time that a copy can take)
+        if (warp == 8) {
+            for (int x = 0; x < 2; ++x)
+                if (sm.asked[x] > 0) drain(&sm.q_full[x], (sm.asked[x] - 1) & 1);
+            const uint32_t n = (sm.asked[2] + NQ - 1) / NQ;
+            for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i) drain(&sm.k_full[i & 1], (i >> 1) & 1);
+        } else if (warp == 10) {
+            const uint32_t n = (sm.asked[3] + 1) / 2;
+            for (uint32_t i = n > TV ? n - TV : 0; i < n; ++i) drain(&sm.v_full[i % TV], (i / TV) & 1);
+        } else if (warp == 9) drain_products(&sm.idle);
+        __syncthreads();
+    }
     if (warp == 9) tc05::tmem_dealloc(tmem, 512);
 }
 

@@ -20,7 +20,9 @@ struct Step {
     const int32_t* block_indices_begins;
     uint32_t* status;
     int form;        // pa_latent_form
+    uint32_t wait_polls;   // looks at a barrier before a wait on it gives up
 };
+constexpr uint32_t kWaitPolls = 1u << 22;
 
 // Form of a sequence in an AUTO step.  With n new tokens over L tokens of context the absorbed form costs a n L and the expanded one b n L + c L, so the
 // number of new tokens decides: with 4 sequences of 2000 cached tokens by 64 heads, 64 new tokens each took 158 us absorbed and 220

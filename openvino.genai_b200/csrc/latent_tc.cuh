@@ -69,17 +69,19 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Waits of a CTA's roles on one another are bounded: one that runs out raises `abort`, which all others poll, and sets the status bit.
+// Waits of a CTA's roles on one another are bounded: one that runs out raises `abort`, which all others poll, and sets the status bit.  The CTA's roles
+// then end where they are; once all have, what they had under way is waited for (drain, drain_products) before its memory goes back.
 struct Waiter {
     volatile int* abort;
     uint32_t* status;
+    uint32_t polls;
     __device__ __forceinline__ bool give_up() const {
         *abort = 1;
         atomicOr(status, PA_DEV_WAIT_TIMEOUT_LATENT);
         return false;
     }
     __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
-        for (uint32_t i = 0; i < (1u << 22); ++i) {
+        for (uint32_t i = 0; i < polls; ++i) {
             if (pa::mbar_try_wait(bar, parity)) return true;
             if ((i & 255u) == 255u && *abort) return false;
         }
@@ -90,7 +92,7 @@ struct Waiter {
     // 1100 - 2048 new tokens by 32 heads 431 -> 357 us).
     __device__ __forceinline__ bool spin_warp(uint64_t* bar, uint32_t parity) const {
         bool ok = false;
-        for (uint32_t i = 0; i < (1u << 26); ++i) {
+        for (uint32_t i = 0; i < polls << 4; ++i) {
             if (mbar_test(bar, parity)) { ok = true; break; }
             if ((i & 1023u) == 1023u && *abort) break;
         }
@@ -102,6 +104,12 @@ struct Waiter {
 // After an abort: until what was issued on `bar` has arrived, or a millisecond or two, which no copy takes
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
     for (int k = 0; k < 4096 && !mbar_test(bar, parity); ++k) __nanosleep(400);
+}
+// The same for the products of this warp's elected lane; `idle` has had no arrival yet.
+__device__ __forceinline__ void drain_products(uint64_t* idle) {
+    if (tc05::elect_one()) tc05::commit(idle);
+    __syncwarp();
+    drain(idle, 0);
 }
 
 // Operand descriptors of 128-byte-swizzled tiles whose 8-row groups are GROUP bytes apart.  Their high words are constants, so only the low
