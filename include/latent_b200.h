@@ -81,7 +81,9 @@ enum pa_latent_form {
     PA_LATENT_EXPANDED = 2
 };
 
-/* Attention of the new tokens over the cache, which holds their own rows already (pa_b200_latent_append first). */
+/* Attention of the new tokens over the cache, which holds their own rows already (pa_b200_latent_append first).
+ * A row whose logits hold not-a-number or plus infinity has no softmax and its output is not finite, whichever form serves it; nor is that of one whose
+ * intermediates leave the type (with F16: key_up[h]^T query_nope beyond 65504 in the absorbed form, keys and values beyond it in the expanded one). */
 typedef struct pa_latent_attention_args {
     uint32_t struct_size;
     const void* query_nope;        /* [num_tokens, num_heads, nope_size] */

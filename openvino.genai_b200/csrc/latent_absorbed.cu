@@ -822,23 +822,26 @@ __global__ void __launch_bounds__(kValueThreads, R == 256 && NT == 16 ? 2 : 1) p
             for (int u = 0; u < kRows; ++u) {
                 const int r = (warp >> spread) + u * kJoinWarps, pieces = part[u].y;
                 if (u + 1 < kRows) first(u + 1);
-                // the pieces' common maximum, and the denominator (a piece whose tiles the row does not see has no sums)
-                float top = ml[u].y > 0.f ? ml[u].x : -INFINITY, sum = ml[u].y > 0.f ? ml[u].y : 0.f;
+                // the pieces' common maximum, and the denominator.  A piece whose tiles the row does not see has a sum of zero and is passed over; one
+                // whose logits hold not-a-number or infinity has a sum that is not-a-number, which goes through to the row
+                float top = ml[u].y != 0.f ? ml[u].x : -INFINITY, sum = ml[u].y;
                 for (int i = lane + 32; i < pieces; i += 32) {
                     const float2 other = a.part_ml[part[u].x + (long long)i * step];
-                    if (other.y > 0.f) {
+                    if (other.y != 0.f) {
                         const float t = fmaxf(top, other.x);
-                        sum = (top == -INFINITY ? 0.f : sum * ex2(top - t)) + other.y * ex2(other.x - t);
+                        sum = (sum == 0.f ? 0.f : sum * ex2(top - t)) + other.y * ex2(other.x - t);
                         top = t;
                     }
                 }
-                const float most = pa::warp_max(top), inv = 1.f / pa::warp_sum(top == -INFINITY ? 0.f : sum * ex2(top - most));
-                float y[V][4] = {};
+                const float most = pa::warp_max(top), inv = 1.f / pa::warp_sum(sum == 0.f ? 0.f : sum * ex2(top - most));
+                float y[V][4];
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[v][0] = y[v][1] = y[v][2] = y[v][3] = 0.f * inv;      // (not-a-number for a row without any sum, or whose sum is)
                 for (int base = 0; base < pieces; base += 32 * each) {
                     const int i = base + mine + lane * each, count = min(32, (pieces - base - mine + each - 1) >> spread);
                     float2 own = ml[u];
                     if (base > 0 || each > 1) own = i < pieces ? a.part_ml[part[u].x + (long long)i * step] : make_float2(-INFINITY, 0.f);
-                    const float weight = own.y > 0.f ? ex2(own.x - most) * inv : 0.f;
+                    const float weight = own.y != 0.f ? ex2(own.x - most) * inv : 0.f;
                     for (int j = 0; j < count; j += U) {
                         if (base + j > 0) {
 #pragma unroll

@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) expanded_attend_kernel(cons
                             const float2 x = __ldcg(ml + k * step);
                             if (x.y == 0.f) continue;       // (a piece that the row does not see)
                             const float to = fmaxf(most, x.x);
-                            sum = (most == -INFINITY ? 0.f : sum * ex2(most - to)) + x.y * ex2(x.x - to);
+                            sum = (sum == 0.f ? 0.f : sum * ex2(most - to)) + x.y * ex2(x.x - to);
                             most = to;
                         }
                         part = reinterpret_cast<float4*>(a.part_o) + (long long)it.slot * (DV / 4) * kQueryTile + i;
