@@ -117,7 +117,7 @@ int pa_b200_latent_append(pa_latent_handle* h, const pa_latent_append_args* args
 int pa_b200_latent_attention(pa_latent_handle* h, const pa_latent_attention_args* args);
 
 /* The handle's scratch grows when a call needs more (cudaMalloc, never inside a stream capture).  After reserve, attention calls of no more
- * tokens, sequences and block indices, in the same or a narrower form, do not allocate. */
+ * tokens, sequences and block indices, in the same form or, behind an AUTO reserve, in any, do not allocate. */
 int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices, int32_t form);
 
 /* Reads (and clears) the device status word; synchronises the device's work on it. */

@@ -133,6 +133,8 @@ struct Scratch {
     size_t total;
 };
 
+// The scratch of a step.  `total` does not fall where tokens, sequences or block indices grow (what goes by the number of heads in a pass, which falls,
+// takes its upper bound), so that the scratch of the largest step holds every smaller one of its form.
 Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int block_indices, int form) {
     const pa_latent_desc& d = h->desc;
     Scratch s{};
@@ -165,18 +167,29 @@ Scratch plan_scratch(const pa_latent_handle* h, int tokens, int sequences, int b
         s.query_prefix = take(((size_t)sequences + 1) * sizeof(int));
         s.part_slots = 2 * h->sm_count / s.heads * s.heads;      // (a pass of so many heads as CTAs cuts no context)
         if (s.heads >= h->sm_count) s.part_slots = 0;
-        s.order = take(((size_t)tokens / latent::kQueryTile + served + s.part_slots) * sizeof(latent::PieceOfQuery));
-        s.arrived = take((size_t)s.passes * s.part_slots * 8 * sizeof(int));
-        s.split_o = take((size_t)s.part_slots * latent::kQueryTile * d.value_size * sizeof(float));
-        s.split_ml = take((size_t)s.part_slots * latent::kQueryTile * sizeof(float2));
+        const size_t most_slots = 2 * (size_t)h->sm_count;
+        s.order = take(((size_t)tokens / latent::kQueryTile + served + most_slots) * sizeof(latent::PieceOfQuery));
+        s.arrived = take((size_t)s.passes * most_slots * 8 * sizeof(int));
+        s.split_o = take(most_slots * latent::kQueryTile * d.value_size * sizeof(float));
+        s.split_ml = take(most_slots * latent::kQueryTile * sizeof(float2));
         s.heads_per_item = take(2 * sizeof(int));
         s.counter = take((size_t)s.passes * sizeof(int));
         s.k_rope = take((size_t)s.rows * 64 * 2);
-        s.k = take((size_t)s.heads * s.rows * d.nope_size * 2);
-        s.v = take((size_t)s.heads * s.rows * d.value_size * 2);
+        // keys and values: all heads', or as much as a pass may take
+        s.k = take(std::min(d.num_heads * head, std::max(kExpandBytes, head)) + align_up(1));
+        s.v = s.k + align_up((size_t)s.heads * s.rows * d.nope_size * 2);
     }
     s.total = off;
     return s;
+}
+
+// What a reserve makes room for: an AUTO step's, and that of the same step in either form (the absorbed form by itself has partial results of all
+// rows, the expanded one tiles of every sequence).
+size_t reserved_bytes(const pa_latent_handle* h, int tokens, int sequences, int block_indices, int form) {
+    size_t bytes = plan_scratch(h, tokens, sequences, block_indices, form).total;
+    if (form == PA_LATENT_AUTO)
+        for (int narrower : {PA_LATENT_ABSORBED, PA_LATENT_EXPANDED}) bytes = std::max(bytes, plan_scratch(h, tokens, sequences, block_indices, narrower).total);
+    return bytes;
 }
 
 int ensure_ws(pa_latent_handle* h, size_t bytes) {
@@ -409,7 +422,7 @@ int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_
         if (form != PA_LATENT_AUTO && form != PA_LATENT_ABSORBED && form != PA_LATENT_EXPANDED) return fail(PA_ERR_INVALID_ARG, "unknown form");
         DeviceScope scope(h->device);
         LATENT_CUDA(scope.error);
-        return ensure_ws(h, plan_scratch(h, num_tokens, num_sequences, num_block_indices, form).total);
+        return ensure_ws(h, reserved_bytes(h, num_tokens, num_sequences, num_block_indices, form));
     });
 }
 
