@@ -116,8 +116,9 @@ int pa_b200_latent_destroy(pa_latent_handle* h);
 int pa_b200_latent_append(pa_latent_handle* h, const pa_latent_append_args* args);
 int pa_b200_latent_attention(pa_latent_handle* h, const pa_latent_attention_args* args);
 
-/* The handle's scratch grows when a call needs more (cudaMalloc, never inside a stream capture).  After reserve, attention calls of no more
- * tokens, sequences and block indices, in the same form or, behind an AUTO reserve, in any, do not allocate. */
+/* The handle's scratch grows when a call needs more (cudaMalloc; inside a stream capture such a call is PA_ERR_TOO_LARGE).  After reserve, attention
+ * calls of no more tokens, sequences and block indices, in the same form or, behind an AUTO reserve, in any, do not allocate.  A graph names the scratch
+ * of its capture, which the handle keeps until it is destroyed, whatever grows since; replays and calls of one handle stay ordered on one stream. */
 int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices, int32_t form);
 
 /* Reads (and clears) the device status word; synchronises the device's work on it. */

@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <new>
 #include <string>
+#include <vector>
 
 #include "latent_kernels.h"
 
@@ -23,6 +24,8 @@ struct pa_latent_handle {
     uint32_t* status = nullptr;   // device status word
     uint8_t* ws = nullptr;        // kernel scratch
     size_t ws_bytes = 0;
+    bool captured = false;        // a stream capture has named the scratch
+    std::vector<uint8_t*> retired;   // scratch of captures, outgrown since: their graphs may still run
     int64_t launches = 0;
     uint32_t wait_polls = latent::kWaitPolls;   // env PA_B200_LATENT_TEST_WAIT_POLLS: the kernels' bounded waits are made to run out
 };
@@ -192,10 +195,15 @@ size_t reserved_bytes(const pa_latent_handle* h, int tokens, int sequences, int 
     return bytes;
 }
 
-int ensure_ws(pa_latent_handle* h, size_t bytes) {
-    if (bytes <= h->ws_bytes) return PA_OK;
-    if (h->ws) LATENT_CUDA(cudaFree(h->ws));   // (waits for the work that uses it)
-    h->ws = nullptr; h->ws_bytes = 0;
+int ensure_ws(pa_latent_handle* h, size_t bytes, bool capturing) {
+    if (bytes <= h->ws_bytes) {
+        h->captured |= capturing;
+        return PA_OK;
+    }
+    if (capturing) return fail(PA_ERR_TOO_LARGE, "the scratch would have to grow inside a stream capture: pa_b200_latent_reserve for the step beforehand");
+    if (h->captured) h->retired.push_back(h->ws);
+    else if (h->ws) LATENT_CUDA(cudaFree(h->ws));   // (waits for the work that uses it)
+    h->ws = nullptr; h->ws_bytes = 0; h->captured = false;
     const size_t want = (bytes + bytes / 4 + (1 << 20) - 1) >> 20 << 20;
     LATENT_CUDA(cudaMalloc((void**)&h->ws, want));
     h->ws_bytes = want;
@@ -274,7 +282,9 @@ int attention(pa_latent_handle* h, const pa_latent_attention_args* a) {
     const cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
     const float scale = a->scale != 0.f ? a->scale : 1.f / sqrtf((float)(d.nope_size + P));
     const Scratch s = plan_scratch(h, T, a->num_sequences, a->num_block_indices, a->form);
-    rc = ensure_ws(h, s.total);
+    cudaStreamCaptureStatus capture;
+    LATENT_CUDA(cudaStreamIsCapturing(stream, &capture));
+    rc = ensure_ws(h, s.total, capture != cudaStreamCaptureStatusNone);
     if (rc != PA_OK) return rc;
     int launches = 0;
     if (a->form != PA_LATENT_EXPANDED) {
@@ -401,6 +411,7 @@ int pa_b200_latent_destroy(pa_latent_handle* h) {
     DeviceScope scope(h->device);
     if (h->stream) cudaStreamSynchronize(h->stream);
     if (h->ws) cudaFree(h->ws);   // (waits for the work that uses it)
+    for (uint8_t* p : h->retired) cudaFree(p);
     if (h->status) cudaFree(h->status);
     if (h->stream) cudaStreamDestroy(h->stream);
     delete h;
@@ -422,7 +433,7 @@ int pa_b200_latent_reserve(pa_latent_handle* h, int32_t num_tokens, int32_t num_
         if (form != PA_LATENT_AUTO && form != PA_LATENT_ABSORBED && form != PA_LATENT_EXPANDED) return fail(PA_ERR_INVALID_ARG, "unknown form");
         DeviceScope scope(h->device);
         LATENT_CUDA(scope.error);
-        return ensure_ws(h, reserved_bytes(h, num_tokens, num_sequences, num_block_indices, form));
+        return ensure_ws(h, reserved_bytes(h, num_tokens, num_sequences, num_block_indices, form), false);
     });
 }
 

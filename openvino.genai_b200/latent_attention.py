@@ -152,7 +152,8 @@ class LatentAttention:
             self._check(rc)
 
     def reserve(self, num_tokens: int, num_sequences: int, num_block_indices: int, form: str = "auto") -> None:
-        """Grows the scratch for steps of up to this size, so that `attend` does not allocate (stream captures need that)."""
+        """Grows the scratch for steps of up to this size, so that `attend` does not allocate (inside a stream capture it would be refused).  A
+        captured graph needs the operator for as long as it is replayed."""
         self._check(self.lib.pa_b200_latent_reserve(self._h, num_tokens, num_sequences, num_block_indices, _FORMS[form]))
 
     def device_status(self) -> int:
