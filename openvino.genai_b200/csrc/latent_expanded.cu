@@ -26,6 +26,8 @@ __global__ void __launch_bounds__(256) expanded_plan_kernel(const __grid_constan
     pa::grid_wait();
     pa::grid_release();
     if (tid == 0) { run_c = 0; run_q = 0; all_c = all_t = work = 0; deepest = pieces_sum = slots = 0; }
+    // (every sequence looks at its own slice of the prefix sums; tokens in front of the first and behind the last are nobody's)
+    if (tid == 0 && (m.subsequence_begins[0] != 0 || m.subsequence_begins[B] != m.num_tokens)) atomicOr(m.status, PA_DEV_BAD_BEGINS);
     if (tid < 32) cuts[tid] = 0;
     for (int i = tid; i < a.passes; i += 256) a.counter[i] = 0;
     for (int i = tid; i < a.passes * a.part_slots * 8; i += 256) a.arrived[i] = 0;
