@@ -94,6 +94,11 @@ class LatentAttention:
         # 1 = cudaStreamLegacy: a null handle would select the operator's own stream
         return inputs.get("stream") or torch._C._cuda_getCurrentRawStream(self._ordinal) or 1
 
+    def _form(self, form: str) -> int:
+        if form not in _FORMS:
+            raise self._err(f"unknown form {form!r}: one of {', '.join(_FORMS)}")
+        return _FORMS[form]
+
     # ---- the operators -------------------------------------------------------------------------
     def append(self, inputs: dict, outputs: Optional[dict] = None) -> None:
         """inputs: latent [T, latent + rope], norm_weight [latent] (optional) with norm_eps, rope_table f32 [rows, rope] (cos | sin),
@@ -132,8 +137,7 @@ class LatentAttention:
         """inputs: query_nope [T, heads, nope], query_rope [T, heads, rope] (rotated), key_up [heads, nope, latent],
         value_up [heads, value, latent], scale (default 1/sqrt(nope + rope)), cache and the paged metadata.
         outputs: output [T, heads * value].  form: "absorbed", "expanded", or "auto" (each sequence in the one that suits it)."""
-        if form not in _FORMS:
-            raise self._err(f"unknown form {form!r}: one of {', '.join(_FORMS)}")
+        self._form(form)
         nope, rope, key_up, value_up, output = inputs["query_nope"], inputs["query_rope"], inputs["key_up"], inputs["value_up"], outputs["output"]
         n, r = self._rows("query_nope", nope, self._nope_shape), self._rows("query_rope", rope, self._rope_shape)
         k, v = self._rows("key_up", key_up, self._key_shape), self._rows("value_up", value_up, self._value_shape)
@@ -154,7 +158,7 @@ class LatentAttention:
     def reserve(self, num_tokens: int, num_sequences: int, num_block_indices: int, form: str = "auto") -> None:
         """Grows the scratch for steps of up to this size, so that `attend` does not allocate (inside a stream capture it would be refused).  A
         captured graph needs the operator for as long as it is replayed."""
-        self._check(self.lib.pa_b200_latent_reserve(self._h, num_tokens, num_sequences, num_block_indices, _FORMS[form]))
+        self._check(self.lib.pa_b200_latent_reserve(self._h, num_tokens, num_sequences, num_block_indices, self._form(form)))
 
     def device_status(self) -> int:
         """Reads and clears the device status word (PA_DEV_* bits)."""

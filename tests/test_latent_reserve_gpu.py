@@ -122,3 +122,14 @@ def test_a_capture_that_would_have_to_grow_the_scratch_is_refused(pkg):
     assert bool((out == 0).all())
     st.check(st.attend(op, inputs=x))
     assert op.device_status() == 0
+
+
+def test_refusals(pkg):
+    from openvino_genai_b200 import GenaiB200Error
+    op = pkg.LatentAttention(8, *LH.WIDE, BLOCK, torch.bfloat16)
+    with pytest.raises(GenaiB200Error, match="unknown form"):
+        op.reserve(10, 2, 3, "both")
+    for sizes in ((-1, 2, 3), (1, -2, 3), (1, 2, -3)):
+        with pytest.raises(GenaiB200Error, match="negative"):
+            op.reserve(*sizes)
+    op.reserve(0, 0, 0)
