@@ -1,3 +1,4 @@
+import gc
 import sys
 from pathlib import Path
 
@@ -10,6 +11,25 @@ if str(ROOT) not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (run with -m gpu on the GPU box)")
+
+
+_by_exception = set()
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_makereport(item, call):
+    """A test that ends by an exception (a skip in its body, a failure) leaves its frames, and the device memory of what they hold, in reference
+    cycles: they go at once, not in the middle of a later test that compares the free device memory."""
+    yield
+    if call.excinfo is not None:
+        _by_exception.add(item.nodeid)
+
+
+@pytest.hookimpl(trylast=True)
+def pytest_runtest_logfinish(nodeid, location):
+    if nodeid in _by_exception:
+        _by_exception.remove(nodeid)
+        gc.collect()
 
 
 @pytest.fixture(scope="session")
