@@ -29,7 +29,8 @@ extern "C" {
 /* Device status bit, beside those of pa_b200.h: a bounded wait of an attention kernel ran out; the step's output is incomplete. */
 #define PA_DEV_WAIT_TIMEOUT_LATENT 0x10000000u
 
-/* Static attributes of one layer. */
+/* Static attributes of a layer.  Layers of the same attributes share a handle, whose scratch (gigabytes for long prompts by many heads) then serves them in
+ * turn: every call brings its own weights, cache and metadata. */
 typedef struct pa_latent_desc {
     uint32_t struct_size; /* sizeof(pa_latent_desc)                                               */
     int32_t num_heads;    /* 1 .. 1024                                                            */
@@ -76,7 +77,10 @@ typedef struct pa_latent_append_args {
 } pa_latent_append_args;
 
 enum pa_latent_form {
-    PA_LATENT_AUTO = 0,      /* every sequence in the form that suits its number of new tokens */
+    /* Every sequence in the form that suits its number of new tokens.  Which that is, is known on the device only: the expanded form's scratch and passes
+     * go by the block tables of the whole step, and both forms' kernels are launched as soon as there are more than 16 tokens.  A step that the
+     * caller knows to hold single tokens and drafts only, or prompts only, is served faster and in less scratch by its form's name. */
+    PA_LATENT_AUTO = 0,
     PA_LATENT_ABSORBED = 1,
     PA_LATENT_EXPANDED = 2
 };

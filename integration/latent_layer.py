@@ -26,15 +26,15 @@ class LatentLayer:
         self.op = LatentAttention(heads, latent, rope, nope, value, block_size, torch.bfloat16)
         self.cache = self.op.allocate_cache(blocks)
 
-    def step(self, x, metadata):
-        """x: [tokens, hidden].  metadata: past_lens, subsequence_begins, block_indices, block_indices_begins."""
+    def step(self, x, metadata, form="auto"):
+        """x: [tokens, hidden].  metadata: past_lens, subsequence_begins, block_indices, block_indices_begins.  form: what the caller knows of the step."""
         heads, latent, rope, nope, value = self.sizes
         q = (x @ self.query.T).view(-1, heads, nope + rope)
         inputs = {"cache": self.cache, "latent": x @ self.down.T, "norm_weight": self.norm_weight, "norm_eps": 1e-6, "rope_table": self.rope_table,
                   "query_nope": q[..., :nope], "query_rope": q[..., nope:], "key_up": self.up[:, :nope], "value_up": self.up[:, nope:], **metadata}
         self.op.append(inputs, {"query_rope": inputs["query_rope"]})
         o = torch.empty((x.shape[0], heads * value), dtype=x.dtype, device=x.device)
-        self.op.attend(inputs, {"output": o})
+        self.op.attend(inputs, {"output": o}, form=form)
         return o @ self.out.T
 
     def whole(self, x):
@@ -74,7 +74,8 @@ def serve(layer, sequences, chunk=128, block_size=32):
         cumulative = lambda v: [sum(v[:i]) for i in range(len(v) + 1)]
         metadata = {"past_lens": i32([done[s] for s in live]), "subsequence_begins": i32(cumulative(new)),
                     "block_indices": i32([b for s in live for b in blocks[s]]), "block_indices_begins": i32(cumulative([len(blocks[s]) for s in live]))}
-        y = layer.step(torch.cat([sequences[s][done[s]:done[s] + n] for s, n in zip(live, new)]), metadata)
+        # (the lengths are known here: steps of single tokens only need nothing of the expanded form)
+        y = layer.step(torch.cat([sequences[s][done[s]:done[s] + n] for s, n in zip(live, new)]), metadata, "absorbed" if max(new) == 1 else "auto")
         for s, n, rows in zip(live, new, y.split(new)):
             out[s][done[s]:done[s] + n] = rows
             done[s] += n

@@ -28,6 +28,9 @@ constexpr uint32_t kWaitPolls = 1u << 22;
 // number of new tokens decides: with 4 sequences of 2000 cached tokens by 64 heads, 64 new tokens each took 158 us absorbed and 220
 // expanded, 96 took 225 and 222, 128 299 and 219 (with 16 sequences 622 and 898, 913 and 889, 1229 and 884).  Short contexts leave the absorbed form with
 // more results than work (16 sequences of 64 tokens by 16 heads 62 and 35 us).
+// The rule runs on the device, so the host lays out and launches the expanded form for whatever the whole step's block tables allow: 64 rows over
+// 259,540 tokens by 128 heads take 137 us, 3 launches and 60 MiB in the absorbed form and 211 us, 36 launches (33 find no work) and 1424 MiB under AUTO; 4
+// prompts by 32 heads 450 us expanded and 547 under AUTO, whose query projection loads before it knows that no token is its own.
 constexpr int kAutoMaxNew = 80, kAutoFewNew = 16, kAutoContext = 8;
 
 struct AppendArgs {

@@ -20,7 +20,8 @@ _FORMS = {"auto": A.PA_LATENT_AUTO, "absorbed": A.PA_LATENT_ABSORBED, "expanded"
 
 
 class LatentAttention:
-    """One layer's operator instance (owns a C-ABI handle and its scratch)."""
+    """The operator for layers of one geometry (owns a C-ABI handle and its scratch).  One instance serves all such layers of a model in turn: every call
+    brings its own weights, cache and metadata, and the scratch of a step can be gigabytes."""
 
     def __init__(self, num_heads: int, latent_size: int, rope_size: int, nope_size: int, value_size: int, block_size: int,
                  dtype: torch.dtype = torch.bfloat16, device: int = 0):
@@ -136,7 +137,8 @@ class LatentAttention:
     def attend(self, inputs: dict, outputs: dict, form: str = "auto") -> None:
         """inputs: query_nope [T, heads, nope], query_rope [T, heads, rope] (rotated), key_up [heads, nope, latent],
         value_up [heads, value, latent], scale (default 1/sqrt(nope + rope)), cache and the paged metadata.
-        outputs: output [T, heads * value].  form: "absorbed", "expanded", or "auto" (each sequence in the one that suits it)."""
+        outputs: output [T, heads * value].  form: "absorbed", "expanded", or "auto": each sequence in the one that suits it, which the device finds out.
+        A step known to hold single tokens and drafts only ("absorbed"), or prompts only ("expanded"), is faster by name and takes less scratch."""
         self._form(form)
         nope, rope, key_up, value_up, output = inputs["query_nope"], inputs["query_rope"], inputs["key_up"], inputs["value_up"], outputs["output"]
         n, r = self._rows("query_nope", nope, self._nope_shape), self._rows("query_rope", rope, self._rope_shape)
