@@ -187,7 +187,7 @@ def _cache(case, blocks, g, value):
 def _quantise(x):
     """Bytes, scale and zero-point of the last dimension's rows, in the operator's documented steps of 32 bits."""
     mn, mx = x.amin(-1), x.amax(-1)
-    scale = (mx - mn) / 255.0
+    scale = (mx - mn) / torch.full_like(mx, 255.0)      # (by a number torch would multiply with its reciprocal)
     scale = torch.where(scale > 0, scale, torch.ones_like(scale))
     zp, inv = -mn / scale, 1.0 / scale
     q = (x.double() * inv.double()[..., None] + zp.double()[..., None]).float()      # one rounding, as a fused multiply-add has
