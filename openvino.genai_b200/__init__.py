@@ -46,6 +46,8 @@ def load_library(build_if_missing: bool = False) -> ctypes.CDLL:
     _abi.bind(lib, _eviction_abi.EVICTION_SYMBOLS)
     from . import _latent_abi
     _abi.bind(lib, _latent_abi.LATENT_SYMBOLS)
+    from . import _masked_abi
+    _abi.bind(lib, _masked_abi.MASKED_SYMBOLS)
     _lib = lib
     return lib
 

@@ -1,0 +1,253 @@
+// Entry points of include/masked_b200.h: argument checks, scratch, launch sequence of a masked step and of the acceptance of drafts.
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <string>
+
+#include "pa_handle.h"
+
+namespace {
+
+int fail(int code, const char* msg) {
+    pa::set_last_error(msg);
+    return code;
+}
+
+int fail_cuda(const char* what, cudaError_t e) {
+    cudaGetLastError();   // (told to this caller, not to whoever asks the runtime next)
+    pa::set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return PA_ERR_CUDA;
+}
+
+#define MASKED_CUDA(expr)                                   \
+    do {                                                    \
+        const cudaError_t _e = (expr);                      \
+        if (_e != cudaSuccess) return fail_cuda(#expr, _e); \
+    } while (0)
+
+// The body of an entry point: what it throws (the text of an error may not find memory) ends here.
+template <class F>
+int guarded(F&& body) {
+    try {
+        return body();
+    } catch (...) {
+        return PA_ERR_CUDA;
+    }
+}
+
+// The caller's current device is put back when the call returns.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t error;
+    explicit DeviceScope(int device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Scratch of a masked step.  No part falls where tokens, sequences or block indices grow, so the scratch of the largest step holds every smaller one.
+struct Scratch {
+    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, items, splits, part_o, part_ml, total;
+    int part_slots;
+};
+Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
+    const pa::CacheGeom& g = h->g;
+    const int G = g.Hq / g.Hkv, HK = g.Hkv * ((G + 15) / 16), RT = std::min(G, 16);
+    Scratch s{};
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += (bytes + 255) / 256 * 256; return at; };
+    const size_t B = (size_t)sequences, workers = (size_t)pa::decode_max_workers(h->sm_count), slots = B * HK + workers;
+    s.header = take(sizeof(pa::PlanHeader));
+    s.tile_prefix = take((B + 1) * sizeof(int));
+    s.ptile_prefix = take((B + 1) * sizeof(int));
+    s.worker_start = take(workers * sizeof(pa::WorkerStart));
+    s.stream_done = take(std::max<size_t>(B, 1) * HK * sizeof(int));
+    s.decode_o = take(slots * RT * g.D * sizeof(float));
+    s.decode_ml = take(slots * RT * 2 * sizeof(float));
+    s.tree_words = take((size_t)tokens * pa::kTreeWords * sizeof(uint32_t));
+    s.tree_depth = take((size_t)tokens * sizeof(int));
+    s.part_slots = 2 * h->sm_count;
+    s.items = take(((size_t)tokens * G / pa::kPrefillItemRows + B + s.part_slots) * sizeof(pa::MaskItem));
+    s.splits = take((size_t)s.part_slots * sizeof(pa::MaskSplit));
+    s.part_o = take((size_t)s.part_slots * pa::kPrefillItemRows * g.D * sizeof(float));
+    s.part_ml = take((size_t)s.part_slots * pa::kPrefillItemRows * sizeof(float2));
+    s.total = off;
+    return s;
+}
+
+int ensure_scratch(pa_handle* h, size_t bytes, cudaStream_t stream) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (stream) MASKED_CUDA(cudaStreamIsCapturing(stream, &capture));
+    const bool capturing = capture != cudaStreamCaptureStatusNone;
+    if (bytes <= h->mws_bytes) {
+        h->mws_captured |= capturing;
+        return PA_OK;
+    }
+    if (capturing) return fail(PA_ERR_TOO_LARGE, "the scratch would have to grow inside a stream capture: pa_b200_masked_reserve for the step beforehand");
+    if (h->mws_captured) h->mws_retired.push_back(h->mws);
+    else if (h->mws) MASKED_CUDA(cudaFree(h->mws));   // (waits for the work that uses it)
+    h->mws = nullptr; h->mws_bytes = 0; h->mws_captured = false;
+    const size_t want = (bytes + bytes / 4 + (1 << 20) - 1) >> 20 << 20;
+    MASKED_CUDA(cudaMalloc((void**)&h->mws, want));
+    h->mws_bytes = want;
+    return PA_OK;
+}
+
+int validate_masked(const pa_handle* h, const pa_forward_args* a, const pa_mask_args* m, bool host) {
+    const int rc = pa::validate_forward_args(h, a);
+    if (rc != PA_OK) return rc;
+    if (!m || m->struct_size != sizeof(pa_mask_args)) return fail(PA_ERR_INVALID_ARG, "pa_mask_args: NULL or struct_size mismatch");
+    if (m->sliding_window < 0 || m->sink_tokens < 0) return fail(PA_ERR_INVALID_ARG, "negative sliding_window or sink_tokens");
+    if (a->sliding_window != 0 && a->sliding_window != m->sliding_window) return fail(PA_ERR_INVALID_ARG, "two different sliding windows");
+    if (a->scores) return fail(PA_ERR_UNSUPPORTED, "a masked step has no score output");
+    if (!(a->scale >= 0.f) || a->scale > 3.0e38f) return fail(PA_ERR_INVALID_ARG, "scale is negative or not finite");
+    if (a->num_tokens == 0 || a->num_sequences == 0) return PA_OK;
+    if (a->num_blocks == 0) return fail(PA_ERR_INVALID_ARG, "the cache has no blocks");
+    if (!aligned(a->key_cache) || !aligned(a->value_cache)) return fail(PA_ERR_UNSUPPORTED, "a cache is not 16-byte aligned");
+    if (!host && (!aligned(a->query) || !aligned(a->output))) return fail(PA_ERR_UNSUPPORTED, "query or output is not 16-byte aligned");
+    if ((long long)a->num_tokens * h->g.Hq > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
+    if ((long long)a->num_block_indices * h->g.bs > INT_MAX - 4096) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of context in one call");
+    return PA_OK;
+}
+
+}  // namespace
+
+namespace pa {
+
+int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& mask, cudaStream_t stream) {
+    if (a->num_sequences == 0 || a->num_tokens == 0) return PA_OK;
+    const Scratch s = plan_scratch(h, a->num_tokens, a->num_sequences);
+    const int rc = ensure_scratch(h, s.total, stream);
+    if (rc != PA_OK) return rc;
+    const int G = h->g.Hq / h->g.Hkv, HK = h->g.Hkv * ((G + 15) / 16);
+    KernelArgs k;
+    std::memset(&k, 0, sizeof(k));
+    k.g = h->g;
+    k.query = a->query; k.key = a->key; k.value = a->value; k.output = a->output;
+    k.num_tokens = a->num_tokens;
+    k.key_cache = a->key_cache; k.value_cache = a->value_cache; k.num_blocks = a->num_blocks;
+    k.past_lens = a->past_lens; k.subsequence_begins = a->subsequence_begins;
+    k.block_indices = a->block_indices; k.block_indices_begins = a->block_indices_begins;
+    k.num_block_indices = a->num_block_indices;
+    k.num_sequences = a->num_sequences; k.max_context_len = a->max_context_len;
+    k.scale = a->scale;
+    k.rotated_block_indices = a->rotated_block_indices; k.rotation_deltas = a->rotation_deltas;
+    k.num_rotated_blocks = a->num_rotated_blocks;
+    k.rotation_trig_lut = a->rotation_trig_lut; k.rotation_lut_rows = a->rotation_lut_rows;
+    k.status = h->status;
+    uint8_t* const ws = h->mws;
+    k.plan = (PlanHeader*)(ws + s.header);
+    k.tile_prefix = (int*)(ws + s.tile_prefix);
+    k.ptile_prefix = (int*)(ws + s.ptile_prefix);
+    k.worker_start = (WorkerStart*)(ws + s.worker_start);
+    k.stream_done = (int*)(ws + s.stream_done);
+    k.part_o = (float*)(ws + s.decode_o);
+    k.part_ml = (float*)(ws + s.decode_ml);
+    k.rows_per_tile = std::min(G, 16);
+    // upper bound of the tiles of rows with one new token: all tiles of their block tables, or what their windows leave
+    long long tiles = (long long)a->num_block_indices * h->g.bs / 32 + a->num_sequences;
+    if (mask.sliding_window > 0)
+        tiles = std::min(tiles, (long long)a->num_sequences * (((long long)mask.sliding_window + 31) / 32 + ((long long)mask.sink_tokens + 31) / 32 + 1));
+    k.max_tiles = tiles * HK;
+    MaskParams& m = k.m;
+    m.on = 1;
+    m.window = mask.sliding_window;
+    m.sinks = mask.sink_tokens;
+    m.parents = mask.tree_parents;
+    m.tree_words = (uint32_t*)(ws + s.tree_words);
+    m.tree_depth = (int*)(ws + s.tree_depth);
+    m.tree_blocks = mask.tree_parents ? a->num_sequences : 0;
+    m.sm_count = h->sm_count;
+    m.items = (MaskItem*)(ws + s.items);
+    m.splits = (MaskSplit*)(ws + s.splits);
+    m.part_slots = s.part_slots;
+    m.part_o = (float*)(ws + s.part_o);
+    m.part_ml = (float2*)(ws + s.part_ml);
+    int launches = 0;
+    if (a->num_rotated_blocks > 0) { MASKED_CUDA(launch_rotate(k, stream)); ++launches; }
+    MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;
+    MASKED_CUDA(launch_masked_rows(k, stream, &launches));
+    h->launches += launches;
+    return PA_OK;
+}
+
+int forward_windowed(pa_handle* h, const pa_forward_args* a, bool host) {
+    const pa_mask_args m{sizeof(pa_mask_args), a->sliding_window, 0, nullptr};
+    return host ? pa_b200_forward_masked_host(h, a, &m) : pa_b200_forward_masked(h, a, &m);
+}
+
+}  // namespace pa
+
+extern "C" {
+
+int pa_b200_forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args* mask) {
+    return guarded([&] {
+        const int rc = validate_masked(h, a, mask, /*host=*/false);
+        if (rc != PA_OK) return rc;
+        DeviceScope scope(h->device);
+        MASKED_CUDA(scope.error);
+        return pa::forward_masked(h, a, *mask, a->stream ? (cudaStream_t)a->stream : h->stream);
+    });
+}
+
+int pa_b200_forward_masked_host(pa_handle* h, const pa_forward_args* a, const pa_mask_args* mask) {
+    return guarded([&] {
+        const int rc = validate_masked(h, a, mask, /*host=*/true);
+        if (rc != PA_OK) return rc;
+        DeviceScope scope(h->device);
+        MASKED_CUDA(scope.error);
+        return pa::forward_host(h, a, mask);
+    });
+}
+
+int pa_b200_masked_reserve(pa_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices) {
+    return guarded([&] {
+        if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
+        if (num_tokens < 0 || num_sequences < 0 || num_block_indices < 0) return fail(PA_ERR_INVALID_ARG, "negative size");
+        if (num_sequences > 65535) return fail(PA_ERR_TOO_LARGE, "more than 65535 sequences in one call");
+        DeviceScope scope(h->device);
+        MASKED_CUDA(scope.error);
+        return ensure_scratch(h, plan_scratch(h, num_tokens, num_sequences).total, nullptr);
+    });
+}
+
+int pa_b200_tree_accept(pa_handle* h, const pa_tree_accept_args* a) {
+    return guarded([&] {
+        if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
+        if (!a || a->struct_size != sizeof(pa_tree_accept_args)) return fail(PA_ERR_INVALID_ARG, "pa_tree_accept_args: NULL or struct_size mismatch");
+        if (a->num_tokens < 0 || a->num_sequences < 0 || a->num_block_indices < 0 || a->num_blocks < 0 || a->num_layers < 0)
+            return fail(PA_ERR_INVALID_ARG, "negative size");
+        if (a->num_sequences > 65535) return fail(PA_ERR_TOO_LARGE, "more than 65535 sequences in one call");
+        if (a->num_sequences == 0) return (int)PA_OK;
+        if (a->max_path < 1 || a->max_path > PA_TREE_MAX_TOKENS) return fail(PA_ERR_INVALID_ARG, "max_path must be 1 to 256");
+        if (!a->past_lens || !a->subsequence_begins || !a->block_indices_begins || !a->path || !a->num_accepted || !a->next_token)
+            return fail(PA_ERR_INVALID_ARG, "NULL metadata or output pointer");
+        if (a->num_tokens > 0 && (!a->tree_parents || !a->draft_tokens || !a->sampled_tokens)) return fail(PA_ERR_INVALID_ARG, "NULL token pointer");
+        if (a->num_block_indices > 0 && !a->block_indices) return fail(PA_ERR_INVALID_ARG, "NULL block_indices");
+        if ((long long)a->num_block_indices * h->g.bs > INT_MAX - 4096) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of context in one call");
+        if ((long long)a->num_blocks * h->g.bs > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of cache");
+        if (a->num_layers > 0 && (!a->key_caches || !a->value_caches)) return fail(PA_ERR_INVALID_ARG, "NULL array of caches");
+        if (a->num_layers > 0 && a->num_blocks == 0) return fail(PA_ERR_INVALID_ARG, "the cache has no blocks");
+        for (int i = 0; i < a->num_layers; ++i) {
+            if (!a->key_caches[i] || !a->value_caches[i]) return fail(PA_ERR_INVALID_ARG, "NULL cache pointer");
+            if (!aligned(a->key_caches[i]) || !aligned(a->value_caches[i])) return fail(PA_ERR_UNSUPPORTED, "a cache is not 16-byte aligned");
+        }
+        DeviceScope scope(h->device);
+        MASKED_CUDA(scope.error);
+        const pa::TreeAcceptArgs t{h->g, a->tree_parents, a->draft_tokens, a->sampled_tokens, a->past_lens, a->subsequence_begins, a->block_indices,
+                                   a->block_indices_begins, a->num_tokens, a->num_sequences, a->num_block_indices, a->num_blocks, a->max_path,
+                                   a->path, a->num_accepted, a->next_token, a->new_past_lens, h->status};
+        int launches = 0;
+        MASKED_CUDA(pa::launch_tree_accept(t, a->key_caches, a->value_caches, a->num_layers, a->stream ? (cudaStream_t)a->stream : h->stream, &launches));
+        h->launches += launches;
+        return (int)PA_OK;
+    });
+}
+
+}  // extern "C"

@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "pa_handle.h"
 #include "pa_kernels.h"
 
 namespace {
@@ -37,28 +38,6 @@ size_t act_bytes(int dt) { return dt == PA_DTYPE_F32 ? 4 : 2; }
 namespace pa {
 void set_last_error(const std::string& msg) { g_last_error = msg; }
 }  // namespace pa
-
-struct pa_handle {
-    pa_model_desc desc;
-    pa::CacheGeom g;
-    int device = 0;
-    int sm_count = 148;
-    cudaStream_t stream = nullptr;
-    uint8_t* ws = nullptr;       // kernel scratch
-    size_t ws_bytes = 0;
-    uint32_t* status = nullptr;  // device status word
-    uint8_t* stage_dev = nullptr;  // device copies of host tensors (forward_host)
-    size_t stage_dev_bytes = 0;
-    uint8_t* stage_host = nullptr;  // pinned
-    size_t stage_host_bytes = 0;
-    int64_t launches = 0;
-    int last_prefill_kernel = PA_PREFILL_NONE;
-    bool force_generic_prefill = false;        // env PA_B200_GENERIC_PREFILL=1: cross-check path
-    bool test_drop_copy = false;               // env PA_B200_TEST_DROP_FIRST_COPY=1: the decode kernel's bounded wait is made to run out
-    bool timing = false;                       // record events around the split-K decode kernel
-    std::vector<cudaEvent_t> ev;               // pairs, created on demand
-    size_t ev_used = 0;
-};
 
 namespace {
 
@@ -152,7 +131,7 @@ int ensure_stage(pa_handle* h, size_t bytes) {
 int validate_args(const pa_handle* h, const pa_forward_args* a) {
     if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
     if (!a || a->struct_size != sizeof(pa_forward_args)) return fail(PA_ERR_INVALID_ARG, "pa_forward_args: NULL or struct_size mismatch");
-    if (a->sliding_window != 0) return fail(PA_ERR_UNSUPPORTED, "sliding_window is not supported");
+    if (a->sliding_window < 0) return fail(PA_ERR_INVALID_ARG, "negative sliding_window");
     if (a->alibi_slopes != nullptr) return fail(PA_ERR_UNSUPPORTED, "alibi_slopes is not supported");
     if (a->num_tokens < 0 || a->num_sequences < 0 || a->num_blocks < 0 || a->num_block_indices < 0 || a->max_context_len < 0)
         return fail(PA_ERR_INVALID_ARG, "negative size");
@@ -322,6 +301,8 @@ int pa_b200_destroy(pa_handle* h) {
     cudaSetDevice(h->device);
     if (h->stream) cudaStreamSynchronize(h->stream);
     if (h->ws) cudaFree(h->ws);
+    if (h->mws) cudaFree(h->mws);
+    for (uint8_t* p : h->mws_retired) cudaFree(p);
     if (h->status) cudaFree(h->status);
     if (h->stage_dev) cudaFree(h->stage_dev);
     if (h->stage_host) cudaFreeHost(h->stage_host);
@@ -352,6 +333,7 @@ int pa_b200_reserve(pa_handle* h, int32_t num_tokens, int32_t num_sequences, int
 int pa_b200_forward(pa_handle* h, const pa_forward_args* a) {
     int rc = validate_args(h, a);
     if (rc != PA_OK) return rc;
+    if (a->sliding_window > 0) return pa::forward_windowed(h, a, /*host=*/false);
     PA_CUDA(cudaSetDevice(h->device));
     cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
     return run_forward(h, a, stream);
@@ -462,6 +444,18 @@ int pa_b200_get_kernel_timing(pa_handle* h, double* total_ms, int64_t* timed_lau
 int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
     int rc = validate_args(h, a);
     if (rc != PA_OK) return rc;
+    if (a->sliding_window > 0) return pa::forward_windowed(h, a, /*host=*/true);
+    return pa::forward_host(h, a, nullptr);
+}
+
+}  // extern "C"
+
+namespace pa {
+
+int validate_forward_args(const pa_handle* h, const pa_forward_args* a) { return validate_args(h, a); }
+
+int forward_host(pa_handle* h, const pa_forward_args* a, const pa_mask_args* mask) {
+    int rc = PA_OK;
     if (a->num_sequences == 0 || a->num_tokens == 0) return PA_OK;
     PA_CUDA(cudaSetDevice(h->device));
     cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
@@ -472,7 +466,7 @@ int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
     const size_t B = (size_t)a->num_sequences;
 
     struct Item { const void* src; size_t bytes; size_t off; };
-    Item in[11];
+    Item in[12];
     int n_in = 0;
     size_t off = 0;
     auto add = [&](const void* src, size_t bytes) {
@@ -493,6 +487,7 @@ int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
         o_rd = add(a->rotation_deltas, (size_t)a->num_rotated_blocks * 4);
         o_lut = add(a->rotation_trig_lut, (size_t)a->rotation_lut_rows * g.D * 4);
     }
+    const size_t o_tree = mask && mask->tree_parents ? add(mask->tree_parents, (size_t)a->num_tokens * 4) : 0;
     const int n_meta = n_in;
     const size_t meta_bytes = off;
     const size_t o_q = add(a->query, q_bytes);
@@ -534,7 +529,13 @@ int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
         d.rotation_deltas = (const int32_t*)(base + o_rd);
         d.rotation_trig_lut = (const float*)(base + o_lut);
     }
-    rc = run_forward(h, &d, stream);
+    if (mask) {
+        pa_mask_args m = *mask;
+        if (m.tree_parents) m.tree_parents = (const int32_t*)(base + o_tree);
+        rc = forward_masked(h, &d, m, stream);
+    } else {
+        rc = run_forward(h, &d, stream);
+    }
     if (rc != PA_OK) return rc;
     PA_CUDA(cudaMemcpyAsync(a->output, base + o_out, q_bytes, cudaMemcpyDeviceToHost, stream));
     if (a->scores) PA_CUDA(cudaMemcpyAsync(a->scores, base + o_scores, (size_t)a->scores_len * 4, cudaMemcpyDeviceToHost, stream));
@@ -550,4 +551,4 @@ int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
     return PA_OK;
 }
 
-}  // extern "C"
+}  // namespace pa

@@ -5,6 +5,7 @@
 // handful of shuffles.
 #include <algorithm>
 
+#include "masked.cuh"
 #include "pa_common.cuh"
 #include "pa_kernels.h"
 
@@ -27,7 +28,133 @@ __device__ __forceinline__ int find_sequence(const int32_t* begins, int num_seq,
 __device__ __forceinline__ int seq_tiles(const KernelArgs& a, int s) {
     SeqView v;
     if (!seq_view(a, s, v) || v.n != 1) return 0;
+    if (a.m.on) return vis_tiles<32>(v.past + 1, window_lo(a.m, v.past + 1), a.m.sinks).count + a.decode_phantom;
     return (v.past + 1 + 31) / 32 + a.decode_phantom;
+}
+
+// Masked steps: the pieces of the chunks' q tiles.  A piece is what a CTA of the tensor-core kernel takes at a time, per kv head.  When there are few q
+// tiles they are cut along their context, by the length that lets the SMs end soonest: piece lengths from "two pieces an SM" up to whole
+// q tiles are tried side by side, and a piece costs kPieceCost tiles beside its own (its start, its partial result, the join).
+constexpr int kPieceCost = 6;
+constexpr int kSortTiles = 512;   // q tiles up to which the longest come first
+__device__ void build_mask_items(const KernelArgs& a, int total_p) {
+    __shared__ int sh_nt[kSortTiles];
+    __shared__ unsigned long long sh_best;
+    __shared__ int sh_pieces;
+    const int tid = threadIdx.x, B = a.num_sequences, G = a.g.Hq / a.g.Hkv, Hkv = a.g.Hkv, sms = a.m.sm_count;
+    if (tid == 0) { a.ptile_prefix[B] = total_p; sh_best = ~0ull; sh_pieces = 0; a.plan->total_splits = 0; a.plan->total_mitems = total_p; }
+    __syncthreads();   // the prefix sums are visible to the whole block
+    auto describe = [&](int t, SeqView& sv, int& row0, bool& tree) {
+        int lo = 0, hi = B;   // ptile_prefix[lo] <= t < ptile_prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.ptile_prefix[mid] <= t) lo = mid; else hi = mid;
+        }
+        seq_view(a, lo, sv);
+        row0 = (t - a.ptile_prefix[lo]) * kPrefillItemRows;
+        tree = has_tree(a, sv.t0, sv.n);
+        const QTile q = q_tile(a.m, sv.past, sv.n, G, row0, tree);
+        return max(q.cnt[0], q.cnt[1]);
+    };
+    if (total_p > kSortTiles) {   // in the order of the sequences, whole
+        for (int t = tid; t < total_p; t += 256) {
+            SeqView sv;
+            int row0;
+            bool tree;
+            const int nt = describe(t, sv, row0, tree);
+            a.m.items[t] = MaskItem{sv.t0, sv.n, sv.past, sv.tb, row0, 0, nt, -1, tree, {0, 0, 0}};
+        }
+        return;
+    }
+    int total = 0, most = 0;
+    for (int t = tid; t < total_p; t += 256) {
+        SeqView sv;
+        int row0;
+        bool tree;
+        sh_nt[t] = describe(t, sv, row0, tree);
+    }
+    __syncthreads();
+    int len = 0x7fffffff;   // tiles of a piece
+    const long long cap = a.m.part_slots / Hkv;   // pieces there is room for, per kv head
+    if ((long long)total_p * Hkv < 2LL * sms && total_p > 0 && cap > 0) {
+        for (int t = 0; t < total_p; ++t) { total += sh_nt[t]; most = max(most, sh_nt[t]); }   // (every thread: at most 2 * SMs of them)
+        const int least = max(4, (int)(((long long)total * Hkv + 2 * sms - 1) / (2 * sms)));
+        // candidate lengths, evenly spread from `least` to `most`; the last is "whole"
+        const int c = least + (int)((long long)max(most - least, 0) * tid / 255);
+        long long pieces = 0;
+        for (int t = 0; t < total_p; ++t) pieces += (sh_nt[t] + c - 1) / c;
+        const long long waves = (pieces * Hkv + sms - 1) / sms;
+        long long cost;
+        const long long even = max((long long)min(c, most), waves * ((total + pieces - 1) / pieces));   // tiles of the busiest SM
+        if (pieces == total_p) cost = even + waves * (kPieceCost / 2);
+        else cost = pieces <= cap ? even + waves * kPieceCost : (1LL << 30);
+        atomicMin(&sh_best, (unsigned long long)cost << 32 | (unsigned)(0x7fffffff - c));   // of equal ones the longest pieces
+        __syncthreads();
+        len = max(4, 0x7fffffff - (int)(sh_best & 0xffffffffu));
+    }
+    int my_pieces = 0;
+    for (int t = tid; t < total_p; t += 256) {
+        // rank by length, and the pieces in front
+        const int mine = sh_nt[t];
+        int first = 0, split_rank = 0, split_first = 0;
+        for (int u = 0; u < total_p; ++u) {
+            const int nt = sh_nt[u];
+            if (nt > mine || (nt == mine && u < t)) {
+                const int k = (nt - 1) / len + 1;
+                first += k;
+                if (k > 1) { ++split_rank; split_first += k; }
+            }
+        }
+        SeqView sv;
+        int row0;
+        bool tree;
+        describe(t, sv, row0, tree);
+        const int k = (mine - 1) / len + 1;
+        for (int i = 0; i < k; ++i)
+            a.m.items[first + i] = MaskItem{sv.t0, sv.n, sv.past, sv.tb, row0, i * len, min(mine, (i + 1) * len), k > 1 ? (split_first + i) * Hkv : -1, tree, {0, 0, 0}};
+        if (k > 1) {
+            a.m.splits[split_rank] = MaskSplit{sv.t0, sv.n, sv.past, row0, split_first * Hkv, k, len, tree};
+            atomicAdd(&a.plan->total_splits, 1);
+        }
+        my_pieces += k;
+    }
+    atomicAdd(&sh_pieces, my_pieces);
+    __syncthreads();
+    if (tid == 0) a.plan->total_mitems = sh_pieces;
+}
+
+// Masked steps: ancestors and depths of one sequence's tree, one block of 256 threads, a token each.  Parents are in front of their children, so a
+// walk up ends.
+__device__ void build_tree(const KernelArgs& a, int s) {
+    __shared__ int sh_parent[kTreeMax];
+    static_assert(kTreeMax == 256, "a thread per token");
+    SeqView sv;
+    const bool ok = seq_view(a, s, sv) && sv.n <= kTreeMax && has_tree(a, sv.t0, sv.n);   // the same for the whole block
+    if (!ok) return;
+    const int i = threadIdx.x;
+    if (i < sv.n) {
+        int p = a.m.parents[sv.t0 + i];
+        if (p < -1 || p >= i) { atomicOr(a.status, PA_DEV_BAD_TREE); p = -1; }
+        sh_parent[i] = p;
+    }
+    __syncthreads();
+    if (i < sv.n) {
+        int depth = 0;
+        for (int q = sh_parent[i]; q >= 0; q = sh_parent[q]) ++depth;
+        uint32_t w[kTreeWords];
+#pragma unroll
+        for (int k = 0; k < kTreeWords; ++k) w[k] = 0u;
+        int d = depth;   // of q
+        for (int q = i; q >= 0; q = sh_parent[q], --d) {
+            const bool sees = a.m.window == 0 || depth - d < a.m.window || sv.past + d < a.m.sinks;
+#pragma unroll
+            for (int k = 0; k < kTreeWords; ++k) w[k] |= sees && (q >> 5) == k ? 1u << (q & 31) : 0u;
+        }
+        uint4* dst = reinterpret_cast<uint4*>(a.m.tree_words + (long long)(sv.t0 + i) * kTreeWords);
+        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        a.m.tree_depth[sv.t0 + i] = depth;
+    }
 }
 
 // Builds the decode plan with one block of 256 threads: the exclusive prefix sum of the per-row
@@ -52,6 +179,10 @@ __device__ void build_decode_plan(const KernelArgs& a) {
         if (s < B) {
             SeqView sv;
             if (n == 0 && seq_view(a, s, sv) && sv.n > 1) np = (sv.n * G + kPrefillItemRows - 1) / kPrefillItemRows;
+            if (np > 0 && a.m.on && sv.n > kTreeMax && has_tree(a, sv.t0, sv.n)) {   // a tree of too many tokens: no output
+                atomicOr(a.status, PA_DEV_BAD_TREE);
+                np = 0;
+            }
         }
         int v = n, vp = np;
 #pragma unroll
@@ -105,6 +236,17 @@ __device__ void build_decode_plan(const KernelArgs& a) {
     // The prefill kernel hands out (q tile, kv head) items from a counter.  Longest context first keeps the last items
     // short, so the CTAs finish together; sequence order leaves a long item for the end.
     const int total_p = sh_run_p;
+    if (a.m.on) {
+        build_mask_items(a, total_p);
+        if (tid == 0) {
+            a.tile_prefix[B] = sh_run;
+            a.plan->total_tiles = sh_run * HK;
+            a.ptile_prefix[B] = total_p;
+            a.plan->total_ptiles = total_p;
+            a.plan->next_pitem = 0;
+        }
+        return;
+    }
     const bool sort_items = a.pitem_order != nullptr && total_p > 1 && total_p <= kPrefillSortCap;
     if (sort_items) {
         __shared__ int sh_cost[kPrefillSortCap];
@@ -341,6 +483,13 @@ __global__ void __launch_bounds__(256) write_kv_kernel(KernelArgs a) {
                 return;
             }
             first_block = 2;
+        }
+        if (a.m.on && a.m.tree_blocks > 0) {   // masked steps (without scores): a block per sequence for its tree
+            if ((int)blockIdx.x <= a.m.tree_blocks) {
+                build_tree(a, blockIdx.x - 1);
+                return;
+            }
+            first_block = 1 + a.m.tree_blocks;
         }
     }
     if constexpr (GROUPS) {
@@ -594,7 +743,7 @@ __global__ void __launch_bounds__(256) copy_blocks_kernel(uint8_t* key_cache, ui
 cudaError_t launch_write_kv(const KernelArgs& a, cudaStream_t stream, bool with_plan) {
     if (a.num_tokens <= 0 && !with_plan) return cudaSuccess;
     const long long warps = (long long)a.num_tokens * a.g.Hkv;
-    const int plan_blocks = (with_plan ? 1 : 0) + (with_plan && a.scores && a.score_aggregation_window ? 1 : 0);
+    const int plan_blocks = (with_plan ? 1 : 0) + (with_plan && a.scores && a.score_aggregation_window ? 1 : 0) + (with_plan && a.m.on ? a.m.tree_blocks : 0);
     // Chunks go in groups of 32 tokens once they have enough rows (tokens x kv heads) to give every SM a few.  Decode rows, each in a
     // block of its own, are better off with a warp per row: their u8 value bytes are scattered one by one, 4096 of them by one CTA
     // instead of four.  The line lies where the chunks' gain pays for that (us, warp per row | groups; a 600-token chunk is "600"):

@@ -17,6 +17,8 @@ struct PlanHeader {
     int total_ptiles;  // kPrefillItemRows-row q tiles of all prefill chunks (per kv head)
     int next_pitem;    // work counter of the prefill kernel: next (q tile, kv head) item to hand out
     int pitems_sorted; // 1: pitem_order lists the q tiles by decreasing context length
+    int total_mitems;  // masked steps: pieces of q tiles (per kv head)
+    int total_splits;  // masked steps: q tiles that are cut into several pieces
 };
 
 constexpr int kPrefillSortCap = 2048;  // q tiles (per kv head) up to which the plan step orders them
@@ -61,6 +63,42 @@ __host__ __device__ inline DecodeSlices decode_slices(int total_tiles, int all_w
     if (d.per1 < 1) d.per1 = 1;
     return d;
 }
+
+// ---- masked steps (include/masked_b200.h; masked.cuh) --------------------------------------------------
+constexpr int kTreeMax = 256;              // PA_TREE_MAX_TOKENS
+constexpr int kTreeWords = kTreeMax / 32;
+constexpr int kTreeNone = -2;              // PA_TREE_NONE
+
+// A piece of a q tile's work: tiles [j0, j1) of the q tile's list of 64-token context tiles.
+struct __align__(16) MaskItem {
+    int t0, n_new, past, tb;   // of the sequence: first row, new tokens, cached tokens, begin of its block table
+    int row0;                  // first (token, head) pair of the q tile
+    int j0, j1;
+    int part;                  // partial result of kv head 0, -1: the q tile is in one piece
+    int tree;
+    int pad[3];
+};
+// A q tile in several pieces, whose partial results are joined.
+struct __align__(16) MaskSplit {
+    int t0, n_new, past, row0;
+    int first_part;            // partial result of kv head 0 of the first piece; the next piece's is Hkv further
+    int pieces, len;           // tiles of a piece
+    int tree;
+};
+struct MaskParams {
+    int on;                    // 0: causal rows, nothing else below is read
+    int window, sinks;
+    const int32_t* parents;    // [num_tokens] or null
+    uint32_t* tree_words;      // [num_tokens][kTreeWords] ancestors of a token and itself, those its window leaves
+    int* tree_depth;           // [num_tokens]
+    int tree_blocks;           // blocks of the cache write that make them: one per sequence, 0 without trees
+    int sm_count;
+    MaskItem* items;
+    MaskSplit* splits;         // [2 * sm_count]
+    int part_slots;            // partial results there is room for
+    float* part_o;             // [part_slots][256][D]
+    float2* part_ml;           // [part_slots][256] row maximum (base 2, scaled) and sum
+};
 
 // Everything a kernel needs, passed by value.  All pointers are device memory.
 struct KernelArgs {
@@ -116,6 +154,7 @@ struct KernelArgs {
                            // with one new token and a non-zero window (8 slots per head tile when the GQA group has at
                            // most 8 heads); null: every sequence goes through the score kernel
     long long scores_len;
+    MaskParams m;
 };
 
 // Device-side marshalling of the operator's inputs (pa_marshal.cu); all pointers are device memory.
@@ -178,6 +217,30 @@ bool prefill_tc_supported(const CacheGeom& g);
 bool prefill_mma_supported(const CacheGeom& g);
 cudaError_t launch_prefill_mma(const KernelArgs& a, cudaStream_t stream, long long max_items, int* launches);
 cudaError_t launch_prefill_tc(const KernelArgs& a, cudaStream_t stream, int sm_count, long long max_items, int* launches);
+
+// Masked steps: rows of chunks one by one on CUDA cores (masked_rows.cu); what the acceptance of drafts does (tree_accept.cu).
+cudaError_t launch_masked_rows(const KernelArgs& a, cudaStream_t stream, int* launches);
+
+constexpr int kMoveLayers = 96;   // layers of one launch that moves accepted tokens (their pointers travel as kernel arguments)
+struct TreeAcceptArgs {
+    CacheGeom g;
+    const int32_t* parents;
+    const int64_t* draft;
+    const int64_t* sampled;
+    const int32_t *past_lens, *subsequence_begins, *block_indices, *block_indices_begins;
+    int num_tokens, num_sequences, num_block_indices, num_blocks, max_path;
+    int32_t* path;
+    int32_t* num_accepted;
+    int64_t* next_token;
+    int32_t* new_past_lens;
+    uint32_t* status;
+};
+struct TreeMoveArgs {
+    TreeAcceptArgs t;
+    int num_layers;
+    uint8_t* cache[2][kMoveLayers];
+};
+cudaError_t launch_tree_accept(const TreeAcceptArgs& a, void* const* key_caches, void* const* value_caches, int num_layers, cudaStream_t stream, int* launches);
 
 // SnapKV-style score output: scores[pos] = sum over q heads and the last W rows of each chunk of
 // the softmax probabilities, using the log-sum-exp the attention kernels exported.

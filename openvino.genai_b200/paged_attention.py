@@ -6,6 +6,10 @@ extension op would receive the same tensors in `evaluate(outputs, inputs)`
 (tests/cpp/custom_op/custom_add.cpp:49-80).  `PagedAttentionExtension.evaluate` takes them by
 those names and forwards to the C ABI: device tensors go to pa_b200_forward, host tensors to
 pa_b200_forward_host.  Errors raise GenaiB200Error where the reference raises ov::Exception.
+
+A step whose inputs name a `sliding_window` (with `sink_tokens`) or `tree_parents` goes to pa_b200_forward_masked
+(include/masked_b200.h): rows see a window of their context and its first few tokens, or the tree of drafts that they are part
+of.  `tree_accept` follows the sampled tokens down the trees behind such a step and moves what was accepted.
 """
 from __future__ import annotations
 
@@ -15,7 +19,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from . import _abi
+from . import _abi, _masked_abi as M
 
 _ACT = {torch.float32: _abi.PA_DTYPE_F32, torch.float16: _abi.PA_DTYPE_F16, torch.bfloat16: _abi.PA_DTYPE_BF16}
 _CACHE = {"f16": _abi.PA_DTYPE_F16, "bf16": _abi.PA_DTYPE_BF16, "u8": _abi.PA_DTYPE_U8}
@@ -32,6 +36,8 @@ def _ptr(t) -> Optional[int]:
 class PagedAttentionExtension:
     """One attention layer's operator instance (owns a C-ABI handle and its scratch)."""
 
+    TREE_NONE = M.PA_TREE_NONE
+
     def __init__(self, num_q_heads: int, num_kv_heads: int, head_size: int, block_size: int,
                  act_dtype: torch.dtype = torch.float16, cache_dtype: str = "f16", device: int = 0):
         from . import GenaiB200Error, load_library
@@ -44,6 +50,9 @@ class PagedAttentionExtension:
         self.device = device
         self.num_q_heads, self.num_kv_heads, self.head_size, self.block_size = num_q_heads, num_kv_heads, head_size, block_size
         self._h = C.c_void_p()
+        self._where = torch.device("cuda", device)
+        self._cache_bytes = 0    # of a block: asked for once
+        self._forward_buffer, self._mask_buffer, self._accept_buffer = (C.create_string_buffer(p.size) for p in (M.FORWARD_ARGS, M.MASK_ARGS, M.ACCEPT_ARGS))
         self._check(self.lib.pa_b200_create(C.byref(self.desc), device, C.byref(self._h)))
 
     def __del__(self):
@@ -116,7 +125,17 @@ class PagedAttentionExtension:
 
     def evaluate(self, inputs: dict, outputs: dict) -> None:
         """inputs / outputs are keyed by the reference's tensor names; `output` (and `scores`)
-        must be preallocated by the caller, who owns every buffer."""
+        must be preallocated by the caller, who owns every buffer.
+
+        Masks: `sliding_window` W > 0 leaves a row at position p the cached positions above p - W and, with `sink_tokens` S, those
+        below S; `tree_parents` (i32 [T], an index among the sequence's new tokens that is smaller than the token's own, -1: it follows
+        the last cached token, TREE_NONE at a sequence's first token: no tree) makes a sequence's new tokens a tree of drafts, whose rows
+        see the cache, their ancestors and themselves, at position past_len + depth.  Blocks that no row sees are not looked up.  A step under
+        a mask has no `scores`."""
+        window, sinks, parents = inputs.get("sliding_window") or 0, inputs.get("sink_tokens") or 0, inputs.get("tree_parents")
+        if window or sinks or parents is not None:
+            self._evaluate_masked(inputs, outputs, window, sinks, parents)
+            return
         q = inputs["query"]
         host = isinstance(q, np.ndarray) or (isinstance(q, torch.Tensor) and not q.is_cuda)
         mcl = inputs.get("max_context_len")
@@ -130,6 +149,118 @@ class PagedAttentionExtension:
                               inputs.get("rotation_trig_lut"), inputs.get("stream"),
                               inputs.get("sliding_window", 0), inputs.get("alibi_slopes"))
         self.forward_args(args, host=host)
+
+    # ---- masked steps --------------------------------------------------------------------------
+    # (the checks run before every launch: a small step's time is the host's)
+    def _refuse(self, name: str, t, expected: str):
+        what = f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise self._err(f"{name}: expected {expected} on {self._where}, got {what}")
+
+    def _whole(self, name: str, t, dtype: torch.dtype, shape: tuple) -> int:
+        """The address of a contiguous device tensor of this type and shape."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != self._where or t.shape != shape or not t.is_contiguous():
+            self._refuse(name, t, f"contiguous {dtype} {list(shape)}")
+        return t.data_ptr()
+
+    def _blocks(self, name: str, t) -> int:
+        """Blocks of a cache tensor: contiguous, of any type, in the operator's layout."""
+        if not self._cache_bytes:
+            self._cache_bytes = self.cache_layout().key_block_bytes
+        if not isinstance(t, torch.Tensor) or t.device != self._where or not t.is_contiguous() or t.nbytes % self._cache_bytes:
+            self._refuse(name, t, f"a contiguous tensor of whole blocks of {self._cache_bytes} bytes")
+        return t.nbytes // self._cache_bytes
+
+    def _paged(self, inputs: dict) -> tuple:
+        """Addresses of the paged metadata, number of sequences and of block indices."""
+        past, blocks = inputs["past_lens"], inputs["block_indices"]
+        B, n = past.shape[0] if isinstance(past, torch.Tensor) and past.dim() else 0, blocks.shape[0] if isinstance(blocks, torch.Tensor) and blocks.dim() else 0
+        i32, whole = torch.int32, self._whole
+        return (whole("past_lens", past, i32, (B,)), whole("subsequence_begins", inputs["subsequence_begins"], i32, (B + 1,)),
+                whole("block_indices", blocks, i32, (n,)), whole("block_indices_begins", inputs["block_indices_begins"], i32, (B + 1,))), B, n
+
+    def _stream(self, inputs: dict) -> int:
+        # 1 = cudaStreamLegacy: a null handle would select the operator's own stream
+        return inputs.get("stream") or torch._C._cuda_getCurrentRawStream(self.device) or 1
+
+    def _evaluate_masked(self, inputs: dict, outputs: dict, window: int, sinks: int, parents) -> None:
+        if inputs.get("score_aggregation_window") is not None or outputs.get("scores") is not None:
+            raise self._err("a masked step has no score output")
+        if inputs.get("alibi_slopes") is not None:
+            raise self._err("alibi_slopes is not supported")
+        query, key_cache, value_cache = inputs["query"], inputs["key_cache"], inputs["value_cache"]
+        limit = inputs.get("max_context_len")
+        limit = 0 if limit is None else int(limit)
+        scale = inputs.get("scale")
+        scale = 0.0 if scale is None else float(scale)
+        if isinstance(query, np.ndarray) or (isinstance(query, torch.Tensor) and not query.is_cuda):
+            if parents is not None and (parents.shape != (query.shape[0],) or str(parents.dtype).split(".")[-1] != "int32" or getattr(parents, "is_cuda", False)):
+                raise self._err("tree_parents: expected host int32 of one entry per token")
+            args = self.make_args(query, inputs["key"], inputs["value"], outputs["output"], key_cache, value_cache, inputs["past_lens"], inputs["subsequence_begins"],
+                                  inputs["block_indices"], inputs["block_indices_begins"], scale, limit, None, None, inputs.get("rotated_block_indices"),
+                                  inputs.get("rotation_deltas"), inputs.get("rotation_trig_lut"), inputs.get("stream"))
+            mask = M.pa_mask_args(C.sizeof(M.pa_mask_args), window, sinks, _ptr(parents))
+            self._check(self.lib.pa_b200_forward_masked_host(self._h, C.byref(args), C.byref(mask)))
+            return
+        whole, act = self._whole, self.act_dtype
+        T = query.shape[0] if isinstance(query, torch.Tensor) and query.dim() else 0
+        rows, kv_rows = (T, self.num_q_heads * self.head_size), (T, self.num_kv_heads * self.head_size)
+        meta, B, num_indices = self._paged(inputs)
+        num_blocks = self._blocks("key_cache", key_cache)
+        if self._blocks("value_cache", value_cache) != num_blocks:
+            raise self._err("key_cache and value_cache differ in blocks")
+        rotated = (0, 0, 0, 0, 0)
+        if inputs.get("rotated_block_indices") is not None:
+            blocks, table = inputs["rotated_block_indices"], inputs["rotation_trig_lut"]
+            n = blocks.shape[0]
+            rotated = (whole("rotated_block_indices", blocks, torch.int32, (n,)),
+                       whole("rotation_deltas", inputs["rotation_deltas"], torch.int32, tuple(inputs["rotation_deltas"].shape) if inputs["rotation_deltas"].numel() == n else (n,)),
+                       n, whole("rotation_trig_lut", table, torch.float32, (table.shape[0], self.head_size)), table.shape[0])
+        M.FORWARD_ARGS.pack_into(self._forward_buffer, 0, M.FORWARD_ARGS.size, whole("query", query, act, rows), whole("key", inputs["key"], act, kv_rows),
+                                 whole("value", inputs["value"], act, kv_rows), whole("output", outputs["output"], act, rows), T, key_cache.data_ptr(),
+                                 value_cache.data_ptr(), num_blocks, *meta, B, num_indices, limit, scale, 0, 0, 0, 0, 0, *rotated, self._stream(inputs))
+        M.MASK_ARGS.pack_into(self._mask_buffer, 0, M.MASK_ARGS.size, window, sinks, 0 if parents is None else whole("tree_parents", parents, torch.int32, (T,)))
+        rc = self.lib.pa_b200_forward_masked(self._h, self._forward_buffer, self._mask_buffer)
+        if rc:
+            self._check(rc)
+
+    def masked_reserve(self, num_tokens: int, num_sequences: int, num_block_indices: int) -> None:
+        """Grows the scratch for masked steps of up to this size, so that they do not allocate (inside a stream capture they would be
+        refused).  A captured graph needs the operator for as long as it is replayed."""
+        self._check(self.lib.pa_b200_masked_reserve(self._h, num_tokens, num_sequences, num_block_indices))
+
+    def tree_accept(self, inputs: dict, outputs: dict) -> None:
+        """Judges trees of drafts behind a step that had them, and makes the accepted tokens the cache's newest.
+
+        inputs: tree_parents i32 [T] (as `evaluate` takes it), draft_tokens i64 [T] (the step's input ids; a sequence's first one is
+        certain), sampled_tokens i64 [T] (what was sampled behind each of them), the paged metadata, and key_caches / value_caches: a
+        sequence of the layers' caches (may be left out: nothing is moved).  From an accepted token the path goes on to its
+        first child whose id was sampled behind it.
+        outputs: path i32 [B, max_path] (accepted tokens, -1 behind them), num_accepted i32 [B], next_token i64 [B] (sampled behind
+        the last accepted token), new_past_lens i32 [B] (optional, may be past_lens).  A sequence without a tree keeps all its tokens."""
+        whole, i32, i64 = self._whole, torch.int32, torch.int64
+        parents, path = inputs["tree_parents"], outputs["path"]
+        T = parents.shape[0] if isinstance(parents, torch.Tensor) and parents.dim() else 0
+        meta, B, num_indices = self._paged(inputs)
+        keys, values = inputs.get("key_caches") or (), inputs.get("value_caches") or ()
+        if len(keys) != len(values):
+            raise self._err("key_caches and value_caches differ in layers")
+        counts = {self._blocks(name, t) for name, group in (("key_caches", keys), ("value_caches", values)) for t in group}
+        if len(counts) > 1:
+            raise self._err("the layers' caches differ in blocks")
+        if not isinstance(path, torch.Tensor) or path.dim() != 2:
+            self._refuse("path", path, "contiguous int32 [sequences, max_path]")
+        layers = len(keys)
+        addresses = tuple((C.c_void_p * layers)(*(t.data_ptr() for t in group)) for group in (keys, values))
+        past_out = outputs.get("new_past_lens")
+        M.ACCEPT_ARGS.pack_into(self._accept_buffer, 0, M.ACCEPT_ARGS.size, whole("tree_parents", parents, i32, (T,)),
+                                whole("draft_tokens", inputs["draft_tokens"], i64, (T,)), whole("sampled_tokens", inputs["sampled_tokens"], i64, (T,)), *meta, T, B,
+                                num_indices, counts.pop() if counts else 0, path.shape[1], layers, C.addressof(addresses[0]), C.addressof(addresses[1]),
+                                whole("path", path, i32, (B, path.shape[1])), whole("num_accepted", outputs["num_accepted"], i32, (B,)),
+                                whole("next_token", outputs["next_token"], i64, (B,)), 0 if past_out is None else whole("new_past_lens", past_out, i32, (B,)),
+                                self._stream(inputs))
+        rc = self.lib.pa_b200_tree_accept(self._h, self._accept_buffer)
+        if rc:
+            self._check(rc)
 
     def device_status(self) -> int:
         bits = C.c_uint32(0)

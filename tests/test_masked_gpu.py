@@ -1,0 +1,247 @@
+"""Masked attention on the GPU (include/masked_b200.h): windows with sinks, trees of drafts, both, against 64 bits, with everything poisoned that no row sees."""
+import numpy as np
+import pytest
+import torch
+
+from tests import masked_harness as H
+
+pytestmark = pytest.mark.gpu
+CACHES = [("f16", "f16"), ("bf16", "bf16"), ("bf16", "u8"), ("f16", "u8"), ("f32", "bf16"), ("f16", "bf16"), ("f32", "f16"), ("f32", "u8")]
+
+
+def _whole(step):
+    out, kc, vc, status = step.run()
+    assert status == 0
+    step.check(out)
+    k, v = step.cache_after()
+    same = lambda a, b: torch.equal(a, b)
+    assert same(kc, k) and same(vc, v), "the caches differ from what the step writes"
+
+
+@pytest.mark.parametrize("act,cache", CACHES)
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 32), (128, 16), (64, 32)])
+def test_rows_under_a_window(act, cache, d, bs):
+    past = [0, 1, 4, 31, 32, 33, 63, 64, 99, 100, 101, 500, 1000, 1023]
+    for window, sinks in ((1, 0), (5, 2), (33, 4), (64, 64), (100, 0), (257, 33)):
+        _whole(H.Step(past, [1] * len(past), d=d, bs=bs, act=act, cache=cache, window=window, sinks=sinks, seed=window))
+
+
+@pytest.mark.parametrize("act,cache", CACHES)
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 32)])
+def test_prompts_under_a_window(act, cache, d, bs):
+    for window, sinks in ((1, 0), (7, 3), (64, 0), (130, 70), (5000, 4)):
+        _whole(H.Step([0, 0, 3, 77, 600], [2, 300, 64, 129, 70], d=d, bs=bs, act=act, cache=cache, window=window, sinks=sinks, seed=window))
+
+
+@pytest.mark.parametrize("act,cache", CACHES)
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 32)])
+def test_trees(act, cache, d, bs):
+    rng = np.random.default_rng(3)
+    new = [1, 2, 5, 17, 64, 65, 128]
+    past = [9, 0, 63, 64, 100, 1, 700]
+    for bushy in (1, 3):
+        _whole(H.Step(past, new, d=d, bs=bs, act=act, cache=cache, trees=[H.tree(rng, n, bushy) for n in new], seed=bushy))
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "u8"), ("f32", "bf16")])
+def test_trees_under_a_window(act, cache):
+    rng = np.random.default_rng(4)
+    new, past = [1, 7, 30, 100, 33], [40, 0, 90, 300, 31]
+    for window, sinks in ((1, 0), (2, 1), (3, 50), (20, 4), (90, 310)):
+        _whole(H.Step(past, new, act=act, cache=cache, window=window, sinks=sinks, trees=[H.tree(rng, n, 1) for n in new], seed=window))
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (7, 1), (12, 1), (16, 1), (40, 2), (28, 4)])
+@pytest.mark.parametrize("cache", ["f16", "u8"])
+def test_head_layouts_and_mixed_steps(hq, hkv, cache):
+    """Single tokens, prompts, trees and sequences without tokens in one step."""
+    rng = np.random.default_rng(5)
+    new, past = [1, 40, 12, 0, 1, 150, 3, 0], [200, 30, 120, 50, 0, 5, 64, 0]
+    trees = [None, None, H.tree(rng, 12), None, None, None, H.tree(rng, 3), None]
+    for window, sinks in ((0, 0), (48, 2)):
+        _whole(H.Step(past, new, hq=hq, hkv=hkv, d=128, bs=32, cache=cache, window=window, sinks=sinks, trees=trees, seed=hq))
+
+
+def test_the_largest_tree_is_a_chain_of_256_and_more_is_skipped():
+    chain = list(range(-1, 255))
+    _whole(H.Step([10, 300], [256, 256], trees=[chain, [-1] * 256], seed=1))
+    big = H.Step([10, 5, 7], [257, 4, 1], trees=[list(range(-1, 256)), [-1, 0, 1, 0], None], seed=2)
+    out, kc, vc, status = big.run()
+    assert status == H.M.PA_DEV_BAD_TREE
+    assert bool((out[:257] == 77).all()), "rows of a tree that is too large are left as they were"
+    big.check(out, rows=slice(257, None))
+    k, v = big.cache_after()
+    assert torch.equal(kc, k) and torch.equal(vc, v)
+
+
+def test_bad_parents_count_as_followers_of_the_cache():
+    for bad in (5, 3, 100, -3, -2147483648, 2147483647):
+        step = H.Step([33], [5], trees=[[-1, 0, 1, -1, 2]], seed=3)      # token 3: the tree as it will be taken
+        step.parents[3] = bad
+        out, _, _, status = step.run()
+        assert status == H.M.PA_DEV_BAD_TREE
+        step.check(out)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "u8"])
+def test_a_long_context_is_cut_and_joined(cache):
+    rng = np.random.default_rng(6)
+    act = "bf16" if cache == "bf16" else "f16"
+    _whole(H.Step([7001, 3], [30, 2], hq=8, hkv=2, d=128, bs=32, act=act, cache=cache, trees=[H.tree(rng, 30), H.tree(rng, 2)], seed=4))
+    _whole(H.Step([9000], [40], hq=8, hkv=1, d=128, bs=32, act=act, cache=cache, window=6000, sinks=100, seed=5))
+    _whole(H.Step([20000], [1], hq=8, hkv=1, d=128, bs=32, act=act, cache=cache, window=15000, sinks=100, seed=6))
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "u8"), ("f32", "bf16")])
+def test_what_a_row_does_not_see_takes_no_part_in_it(act, cache):
+    """Not-a-number and infinities at positions that some rows of a sequence see and others do not."""
+    rng = np.random.default_rng(7)
+    for value in (float("nan"), float("inf")):
+        for trees, window, sinks in (([H.tree(rng, 20)], 4, 0), ([None], 16, 2)):
+            step = H.Step([40], [20], act=act, cache=cache, window=window, sinks=sinks, trees=trees, seed=8)
+            first = int(np.argmax(step.sees[0].any(0)[sinks:])) + sinks      # the lowest position in any row's window
+            where = torch.zeros((step.pool, step.bs), dtype=torch.bool, device=step.dev)
+            where[int(step.table[first // step.bs]), first % step.bs] = True
+            step.poison(where, value)
+            out, _, _, status = step.run()
+            blind = torch.from_numpy(~step.sees[0][:, first]).to(step.dev)
+            assert status == 0 and 0 < int(blind.sum()) < 20
+            step.check(out, rows=blind)
+            assert not bool(torch.isfinite(out[~blind]).all(1).any()), "a row that sees it has no finite result"
+
+
+def test_large_queries_and_a_scale_of_ones_own():
+    for cache in ("f16", "u8"):
+        _whole(H.Step([100, 50], [1, 40], act="f32", cache=cache, window=60, sinks=2, magnitude=300.0, scale=1e-3, seed=9))
+    _whole(H.Step([100, 50], [1, 40], act="bf16", cache="bf16", window=60, scale=0.5, magnitude=0.5, seed=10))
+
+
+def test_a_window_of_the_whole_context_is_the_causal_step():
+    """pa_b200_forward by itself, with a window through its own argument, and through the masked call."""
+    for cache in ("f16", "u8"):
+        wide = H.Step([300, 40, 0], [1, 50, 20], cache=cache, window=1 << 30, seed=11)
+        out, kc, vc, status = wide.run()
+        assert status == 0
+        plain = H.Step([300, 40, 0], [1, 50, 20], cache=cache, seed=11)
+        ref, kc2, vc2, status = plain.run()
+        assert status == 0 and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+        wide.check(out)
+        plain.check(ref)
+        op = wide.operator()
+        x = wide.inputs(wide.packed["key"].clone(), wide.packed["value"].clone())
+        x.pop("sink_tokens"), x.pop("sliding_window")
+        y = torch.zeros_like(out)
+        args = op.make_args(x["query"], x["key"], x["value"], y, x["key_cache"], x["value_cache"], x["past_lens"], x["subsequence_begins"], x["block_indices"],
+                            x["block_indices_begins"], None, 350, sliding_window=9)
+        op.forward_args(args)
+        torch.cuda.synchronize()
+        narrow = H.Step([300, 40, 0], [1, 50, 20], cache=cache, window=9, seed=11)
+        narrow.check(y)
+
+
+def test_host_tensors():
+    rng = np.random.default_rng(8)
+    for trees, window in (([H.tree(rng, 9), None], 0), (None, 20)):
+        step = H.Step([50, 30], [9, 1], trees=trees, window=window, seed=12)
+        dev = step.inputs(step.packed["key"].clone(), step.packed["value"].clone())
+        host = {k: v.cpu() if isinstance(v, torch.Tensor) and "cache" not in k else v for k, v in dev.items()}
+        out = torch.zeros((step.T, step.hq * step.d), dtype=torch.float16)
+        op = step.operator()
+        op.evaluate(host, {"output": out})
+        step.check(out.to(step.dev))
+
+
+def test_captured_steps_replay_beside_larger_ones():
+    """Two graphs of one operator, a larger step between them that outgrows their scratch, inputs changed before the replays."""
+    rng = np.random.default_rng(9)
+    small = [H.Step([90, 40], [6, 1], trees=[H.tree(rng, 6), None], window=w, seed=20 + w) for w in (0, 30)]
+    op = small[0].operator()
+    with pytest.raises(H.pkg.GenaiB200Error, match="capture"):
+        g = torch.cuda.CUDAGraph()
+        s = small[0]
+        kc, vc, out = s.packed["key"].clone(), s.packed["value"].clone(), torch.zeros((s.T, s.hq * s.d), dtype=torch.float16, device=s.dev)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            op.evaluate(s.inputs(kc, vc), {"output": out})
+    op.masked_reserve(7, 2, 16)
+    graphs = []
+    for s in small:
+        kc, vc, out = s.packed["key"].clone(), s.packed["value"].clone(), torch.zeros((s.T, s.hq * s.d), dtype=torch.float16, device=s.dev)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            op.evaluate(s.inputs(kc, vc), {"output": out})
+        graphs.append((g, out, s, kc, vc))      # (a graph names its caches)
+    big = H.Step([3000] * 40, [60] * 40, window=100, seed=30)
+    _, _, _, status = big.run(op)
+    for g, out, s, _, _ in graphs * 2:
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        s.check(out)
+    assert op.device_status() == 0
+
+
+def test_two_operators_on_two_streams():
+    steps = [H.Step([500, 20], [30, 1], cache=c, window=77, sinks=3, seed=31) for c in ("f16", "u8")]
+    ops = [s.operator() for s in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    outs = []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, op, stream in zip(steps, ops, streams):
+            with torch.cuda.stream(stream):
+                out = torch.zeros((s.T, s.hq * s.d), dtype=torch.float16, device=s.dev)
+                op.evaluate(s.inputs(s.packed["key"].clone(), s.packed["value"].clone()), {"output": out})
+                outs.append((s, out))
+    torch.cuda.synchronize()
+    for s, out in outs:
+        s.check(out)
+
+
+def test_bad_metadata_and_pages_set_a_status_bit_and_touch_nothing_else():
+    step = H.Step([100, 70, 90], [1, 30, 12], trees=[None, None, H.tree(np.random.default_rng(1), 12)], window=64, seed=13)
+    op = step.operator()
+    for name, at, value, rows in (("past_lens", 1, -1, slice(1, 31)), ("past_lens", 2, 10 ** 9, slice(31, 43)), ("past_lens", 0, 2147483647, slice(0, 1))):
+        keep = step.meta[name].clone()
+        step.meta[name][at] = value
+        out, _, _, status = step.run(op)
+        assert status & 0x6
+        assert bool((out[rows] == 77).all())
+        others = [r for r in range(step.T) if r not in range(*rows.indices(step.T))]
+        step.check(out, rows=torch.tensor(others, device=step.dev))
+        step.meta[name] = keep
+    # a page that a row sees with a number out of range: reported, the others' rows are right
+    keep = step.meta["block_indices"].clone()
+    at = int(step.first[1]) + 100 // step.bs - 1
+    for bad in (-1, step.pool, 2147483647):
+        step.meta["block_indices"][at] = bad
+        out, _, _, status = step.run(op)
+        assert status & 1
+        step.check(out, rows=torch.tensor([0] + list(range(31, 43)), device=step.dev))
+    step.meta["block_indices"] = keep
+    out, _, _, status = step.run(op)
+    assert status == 0
+    step.check(out)
+
+
+def test_refusals_of_tensors():
+    step = H.Step([30], [4], trees=[[-1, 0, 0, 1]], window=8, seed=14)
+    op = step.operator()
+    good = step.inputs(step.packed["key"].clone(), step.packed["value"].clone())
+    out = torch.zeros((4, step.hq * step.d), dtype=torch.float16, device=step.dev)
+    wide = torch.zeros((4, 2 * step.hq * step.d), dtype=torch.float16, device=step.dev)
+    for change in ({"sliding_window": -1}, {"sink_tokens": -1}, {"tree_parents": step.parents.long()}, {"tree_parents": step.parents[:3]}, {"tree_parents": step.parents.cpu()},
+                   {"query": step.query.float()}, {"query": wide[:, ::2]}, {"query": step.query[:3]}, {"key": step.key[:, :-1]}, {"past_lens": step.meta["past_lens"].long()},
+                   {"block_indices_begins": step.meta["block_indices_begins"][:1]}, {"key_cache": good["key_cache"].flatten()[:-16]},
+                   {"score_aggregation_window": step.meta["past_lens"]}, {"alibi_slopes": torch.zeros(8, device=step.dev)}, {"scale": -1.0}, {"scale": float("nan")},
+                   {"scale": float("inf")}):
+        with pytest.raises(H.pkg.GenaiB200Error):
+            op.evaluate({**good, **change}, {"output": out})
+    for bad in (wide[:, ::2], wide.flatten()[1:1 + out.numel()].view_as(out), out.cpu()):
+        with pytest.raises(H.pkg.GenaiB200Error):
+            op.evaluate(good, {"output": bad})
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())
+    op.evaluate(good, {"output": out})
+    step.check(out)
