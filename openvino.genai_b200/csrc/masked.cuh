@@ -92,4 +92,77 @@ __host__ __device__ __forceinline__ QTile q_tile(const MaskParams& m, int past, 
     return q;
 }
 
+// One query row on CUDA cores, by one warp: lane l owns dims {l + 32 i}, online softmax over the positions that the row sees, read back from the paged
+// cache; what it does not see is not read.  Any cache type, head size and mask: for rows that no other kernel serves, and for those
+// whose tile held something that is not finite and that they do not see (0 times it is not 0 in a product).
+template <int D>
+static __device__ __noinline__ void masked_row(const KernelArgs& a, int t, int hq) {
+    constexpr int PER = D / 32;
+    const int lane = threadIdx.x & 31, hk = hq / (a.g.Hq / a.g.Hkv), bs = a.g.bs;
+    int lo = 0, hi = a.num_sequences;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.subsequence_begins[mid] <= t) lo = mid; else hi = mid;
+    }
+    SeqView sv;
+    if (!seq_view(a, lo, sv) || sv.n <= 1 || t < sv.t0 || t >= sv.t0 + sv.n) return;
+    const bool tree = has_tree(a, sv.t0, sv.n);
+    if (tree && sv.n > kTreeMax) { atomicOr(a.status, PA_DEV_BAD_TREE); return; }
+    const RowMask rm = row_mask(a, sv.t0, sv.past, t - sv.t0, tree);
+    const float scale = (a.scale != 0.f ? a.scale : rsqrtf((float)D)) * 1.4426950408889634f;
+    float q[PER], acc[PER];
+    const long long row = (long long)t * a.g.Hq + hq;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        q[i] = load_act(a.query, row * D + lane + 32 * i, a.g.act) * scale;
+        acc[i] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    const VisTiles v = vis_tiles<32>(tree ? sv.past + sv.n : rm.ctx, rm.lo, a.m.sinks);
+    for (int i = 0; i < v.count; ++i) {
+        const int pos0 = 32 * v.tile(i);
+        for (uint32_t w = row_bits32(a, rm, pos0); w; w &= w - 1) {
+            const int pos = pos0 + __ffs(w) - 1;
+            const int blk = a.block_indices[sv.tb + pos / bs];
+            if (blk < 0 || blk >= a.num_blocks) {
+                atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
+                continue;
+            }
+            const long long rec = (long long)blk * a.g.block_bytes + (long long)hk * a.g.head_bytes;
+            const int slot = pos % bs;
+            const uint8_t* kr = (const uint8_t*)a.key_cache + rec;
+            const uint8_t* vr = (const uint8_t*)a.value_cache + rec;
+            float s = 0.f, val[PER];
+            if (a.g.cache == PA_DTYPE_U8) {
+                const float* kp = (const float*)(kr + (long long)bs * D);
+                const float* vp = (const float*)(vr + (long long)bs * D);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int d = lane + 32 * e;
+                    s += q[e] * dequant_one(kr[(long long)slot * D + d], kp[slot], kp[bs + slot]);
+                    val[e] = dequant_one(vr[(long long)d * bs + slot], vp[slot], vp[bs + slot]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const long long at = (long long)slot * D + lane + 32 * e;
+                    s += q[e] * load_act(kr, at, a.g.cache);
+                    val[e] = load_act(vr, at, a.g.cache);
+                }
+            }
+            s = warp_sum(s);
+            const float m_new = fmaxf(m, s);
+            const float f = m_new == -INFINITY ? 1.f : exp2f(m - m_new), p = m_new == -INFINITY ? 0.f : exp2f(s - m_new);
+            l = l * f + p;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] = acc[e] * f + p * val[e];
+            m = m_new;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) store_act(a.output, row * D + lane + 32 * i, a.g.act, acc[i] / l);
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
 }  // namespace pa

@@ -53,7 +53,7 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 
 // Scratch of a masked step.  No part falls where tokens, sequences or block indices grow, so the scratch of the largest step holds every smaller one.
 struct Scratch {
-    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, items, splits, part_o, part_ml, total;
+    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, splits, part_o, part_ml, total;
     int part_slots;
 };
 Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
@@ -72,6 +72,7 @@ Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     s.decode_ml = take(slots * RT * 2 * sizeof(float));
     s.tree_words = take((size_t)tokens * pa::kTreeWords * sizeof(uint32_t));
     s.tree_depth = take((size_t)tokens * sizeof(int));
+    s.redo = take((size_t)tokens * g.Hq * sizeof(int));
     s.part_slots = 2 * h->sm_count;
     s.items = take(((size_t)tokens * G / pa::kPrefillItemRows + B + s.part_slots) * sizeof(pa::MaskItem));
     s.splits = take((size_t)s.part_slots * sizeof(pa::MaskSplit));
@@ -166,13 +167,27 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     m.sm_count = h->sm_count;
     m.items = (MaskItem*)(ws + s.items);
     m.splits = (MaskSplit*)(ws + s.splits);
+    m.redo = (int*)(ws + s.redo);
     m.part_slots = s.part_slots;
+    // As many tokens as sequences: single tokens, almost always, and no launches for chunks; what of them there is beside sequences without
+    // tokens, the device finds out
+    m.rows_in_decode = a->num_tokens > 1 && a->num_tokens == a->num_sequences;
     m.part_o = (float*)(ws + s.part_o);
     m.part_ml = (float2*)(ws + s.part_ml);
+    k.decode_all_workers = decode_launch_workers(k, h->sm_count);
     int launches = 0;
     if (a->num_rotated_blocks > 0) { MASKED_CUDA(launch_rotate(k, stream)); ++launches; }
     MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;
-    MASKED_CUDA(launch_masked_rows(k, stream, &launches));
+    MASKED_CUDA(launch_decode(k, stream, h->sm_count, &launches));
+    if (a->num_tokens > 1 && !m.rows_in_decode) {
+        const long long max_items = (long long)a->num_tokens * G / kPrefillItemRows * h->g.Hkv + (long long)a->num_sequences * h->g.Hkv + s.part_slots;
+        if (prefill_tc_supported(h->g)) {
+            MASKED_CUDA(launch_prefill_tc(k, stream, h->sm_count, max_items, &launches));
+            MASKED_CUDA(launch_masked_join(k, stream, &launches));
+        } else {
+            MASKED_CUDA(launch_masked_rows(k, stream, &launches));
+        }
+    }
     h->launches += launches;
     return PA_OK;
 }

@@ -42,7 +42,7 @@ __device__ void build_mask_items(const KernelArgs& a, int total_p) {
     __shared__ unsigned long long sh_best;
     __shared__ int sh_pieces;
     const int tid = threadIdx.x, B = a.num_sequences, G = a.g.Hq / a.g.Hkv, Hkv = a.g.Hkv, sms = a.m.sm_count;
-    if (tid == 0) { a.ptile_prefix[B] = total_p; sh_best = ~0ull; sh_pieces = 0; a.plan->total_splits = 0; a.plan->total_mitems = total_p; }
+    if (tid == 0) { a.ptile_prefix[B] = total_p; sh_best = ~0ull; sh_pieces = 0; a.plan->total_splits = 0; a.plan->total_redo = 0; a.plan->total_mitems = total_p; }
     __syncthreads();   // the prefix sums are visible to the whole block
     auto describe = [&](int t, SeqView& sv, int& row0, bool& tree) {
         int lo = 0, hi = B;   // ptile_prefix[lo] <= t < ptile_prefix[hi]

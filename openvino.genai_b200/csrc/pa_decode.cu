@@ -19,12 +19,15 @@
 // read from HBM once for all q heads that share it.  Softmax is online with a lazily updated
 // reference maximum.  A stream cut by slice boundaries is merged by the warp whose partial
 // completes it (one atomic counter per stream, no waiting).
+// Rows under a sliding window (WIN; include/masked_b200.h): a stream's tiles are those that hold a position its row sees, the sinks' and then the
+// window's; the loader steps over the gap between them, and a stage's descriptor holds the bits of its visible tokens.
 // HBM-bound: 2*Hkv*(D+8) bytes per context token for the u8 cache.
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
 #include <cstdlib>
 
+#include "masked.cuh"
 #include "pa_common.cuh"
 #include "pa_kernels.h"
 
@@ -45,7 +48,7 @@ enum : int { kFirst = 1, kLast = 2, kEnd = 4 };
 // What the loader records for each ring stage; read by the whole warp when the tile is consumed.
 struct __align__(16) StageDesc {
     int flags;  // kFirst (run starts: load Q, clear state) | kLast (run ends: publish) | kEnd
-    int valid;  // live tokens in the tile (1..32)
+    int valid;  // live tokens in the tile (1..32); under a window the bits of those that the row sees
     int run;    // index of the run's record in the warp's run ring
     int tok0;   // context position of the tile's first token
 };
@@ -100,8 +103,8 @@ __device__ unsigned long long g_decode_prof[8192 * 8];   // per worker: start, f
 
 // SC: the launch keeps the scaled logits of rows whose scores are wanted (a.score_raw is set); a
 // separate instantiation so that steps without a score output run the same code as before.
-template <int D, int BS, int CACHE, bool HI, bool SC>
-__global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2) ? 2 : 3) decode_kernel(KernelArgs a) {
+template <int D, int BS, int CACHE, bool HI, bool SC, bool WIN>
+__global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2) ? 2 : 3) decode_kernel(const __grid_constant__ KernelArgs a) {
     using Cfg = DecodeCfg<D, BS, CACHE>;
     constexpr bool U8 = Cfg::U8;
     constexpr bool BF16 = Cfg::BF16;
@@ -146,6 +149,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         const int4 hi4 = __ldcg(reinterpret_cast<const int4*>(a.worker_start + wid) + 1);
         ws0 = WorkerStart{lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
     }
+    int chunk_items = 0;   // chunks in a step that was not thought to hold any
+    if constexpr (WIN) chunk_items = a.m.rows_in_decode ? __ldcg(&a.plan->total_mitems) : 0;
     const int total_tiles = ws0.s != -1 ? ws0.total_tiles : a.plan->total_tiles;   // all streams
     const DecodeSlices sl = decode_slices(total_tiles, all_workers);
     int g_tile = 0, g_end = 0;       // next global tile to load, end of the slice
@@ -157,12 +162,17 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     int w_blk0 = 0, tbl = 0;                 // block window: lane j holds block_indices[r_tb + w_blk0 + j]
     bool r_first = false;
     bool dropped_once = false;
+    // under a window r_tok and r_end count the tokens of the listed tiles: from r_split on they are r_gap short of the context's
+    int r_split = 0, r_gap = 0, r_lo = 0;
+    auto context_tok = [&](int tok) { return WIN && tok >= r_split ? tok + r_gap : tok; };
 
     auto load_window = [&](int first_block) {
         w_blk0 = first_block;
         const int bi = first_block + lane;
         int blk = 0;
-        if (bi < r_nb) {
+        // (blocks that the row does not see may have any number)
+        const bool seen = !WIN || (bi * BS < r_end + (r_tok >= r_split || r_end > r_split ? r_gap : 0) && (bi * BS < a.m.sinks || (bi + 1) * BS > r_lo));
+        if (bi < r_nb && seen) {
             blk = a.block_indices[r_tb + bi];
             if (blk < 0 || blk >= a.num_blocks) { blk = 0; bad_index = true; }
         }
@@ -173,7 +183,13 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     auto start_run = [&](int tile0, int p0, int ctx, int t0row) {
         const int ntile = min(r_tiles - tile0, g_end - g_tile);
         r_tok = tile0 * kTile;
-        r_end = min(ctx, (tile0 + ntile) * kTile);
+        if constexpr (WIN) {
+            r_lo = window_lo(a.m, ctx);
+            const VisTiles v = vis_tiles<kTile>(ctx, r_lo, a.m.sinks);
+            r_split = v.split * kTile;
+            r_gap = v.gap * kTile;
+        }
+        r_end = min(ctx - r_gap, (tile0 + ntile) * kTile);
         const int s_begin = p0 * HK + r_hkp * r_tiles;             // global tile range of the stream
         const int first_w = sl.worker_of(s_begin), last_w = sl.worker_of(s_begin + r_tiles - 1);
         const int stream = r_s * HK + r_hkp;
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         }
         g_tile += ntile;
         r_first = true;
-        load_window(r_tok / BS);
+        load_window(context_tok(r_tok) / BS);
     };
     // Moves the loader to its next run: the first tile of the next stream of the slice.  False when the slice is done.
     auto advance = [&]() -> bool {
@@ -259,7 +275,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         const int hk = r_hkp / gtiles;
         const uint8_t* kc = (const uint8_t*)a.key_cache + (long long)hk * a.g.head_bytes;
         const uint8_t* vc = (const uint8_t*)a.value_cache + (long long)hk * a.g.head_bytes;
-        const int bi0 = r_tok / BS;
+        const int c_tok = context_tok(r_tok);   // the tile's first position in the context
+        const int bi0 = c_tok / BS;
         if (bi0 + Cfg::NREC - 1 - w_blk0 >= 32) load_window(bi0);
 #ifdef PA_DECODE_PROF
         prof_adv += clock64() - prof_a0;
@@ -268,7 +285,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         bool live[Cfg::NREC];
 #pragma unroll
         for (int r = 0; r < Cfg::NREC; ++r) {
-            live[r] = (bi0 + r) * BS < r_end;
+            live[r] = (bi0 + r) * BS < r_end + (c_tok - r_tok);
+            if constexpr (WIN) live[r] = live[r] && ((bi0 + r) * BS < a.m.sinks || (bi0 + r + 1) * BS > r_lo);
             blocks[r] = __shfl_sync(0xffffffffu, tbl, (bi0 + r - w_blk0) & 31);
         }
         if constexpr (U8) {
@@ -318,10 +336,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
                 }
             cp_async_commit();
         }
-        const int valid = min(kTile, r_end - r_tok);
+        const int valid = WIN ? (int)causal_bits32(c_tok, r_end + (c_tok - r_tok), r_lo, a.m.sinks) : min(kTile, r_end - r_tok);
         const bool last = r_tok + kTile >= r_end;
         if (lane == 0)
-            descs[slot] = StageDesc{(r_first ? kFirst : 0) | (last ? kLast : 0), valid, r_seq % kRunRing, r_tok};
+            descs[slot] = StageDesc{(r_first ? kFirst : 0) | (last ? kLast : 0), valid, r_seq % kRunRing, c_tok};
         r_first = false;
         r_tok += kTile;
     };
@@ -377,6 +395,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
 #endif
         const uint8_t* st = ring + slot * Cfg::STAGE;
         const int valid = d.valid;
+        auto live = [&](int tk) { return WIN ? ((unsigned)valid >> tk & 1u) != 0u : tk < valid; };   // does the row see the tile's token tk
 
         if (d.flags & kFirst) {
             // ---- Q fragments of the run -------------------------------------------------------------
@@ -460,7 +479,15 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         }
 
         if constexpr (!U8) {
-            if (valid < kTile) {  // stale rows of a partly filled block may hold NaN bit patterns
+            if constexpr (WIN) {
+                if (valid != -1) {   // what the row does not see may hold anything
+                    constexpr int CPR = D / 8;
+                    for (int i = lane; i < kTile * CPR; i += 32)
+                        if (!live(i / CPR))
+                            *reinterpret_cast<uint4*>(const_cast<uint8_t*>(st) + Cfg::HALF_STAGE + (i / CPR) * 2 * D + (i % CPR << 4)) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+            } else if (valid < kTile) {  // stale rows of a partly filled block may hold NaN bit patterns
                 constexpr int CPR = D / 8;
                 for (int i = lane; i < (kTile - valid) * CPR; i += 32) {
                     const int row = valid + i / CPR, ch = i % CPR;
@@ -530,7 +557,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
                 const float2 vz = *reinterpret_cast<const float2*>(vp + 4 * BS + 4 * (tk % BS));
                 vsc[j][0] = vs.x; vsc[j][1] = vs.y; vzp[j][0] = vz.x + 1024.f; vzp[j][1] = vz.y + 1024.f;
             }
-            const bool ok0 = tk < valid, ok1 = tk + 1 < valid;
+            const bool ok0 = live(tk), ok1 = live(tk + 1);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 float s0 = sacc[j][2 * r], s1 = sacc[j][2 * r + 1];
@@ -587,9 +614,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
                 if constexpr (U8) {
                     const int tk = 8 * c + 2 * j;
                     // masked tokens have p == 0; the select keeps garbage scale bits (NaN) out
-                    packed = pack_h2(tk < valid ? p0 * vsc[j][0] : 0.f, tk + 1 < valid ? p1 * vsc[j][1] : 0.f);
+                    packed = pack_h2(live(tk) ? p0 * vsc[j][0] : 0.f, live(tk + 1) ? p1 * vsc[j][1] : 0.f);
                     const __half2 h = *reinterpret_cast<__half2*>(&packed);
-                    zsum += (tk < valid ? __low2float(h) * vzp[j][0] : 0.f) + (tk + 1 < valid ? __high2float(h) * vzp[j][1] : 0.f);
+                    zsum += (live(tk) ? __low2float(h) * vzp[j][0] : 0.f) + (live(tk + 1) ? __high2float(h) * vzp[j][1] : 0.f);
                 } else if constexpr (BF16) {
                     packed = pack_bf2(p0, p1);
                 } else {
@@ -749,6 +776,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     }
     if constexpr (!U8) cp_async_wait<0>();
     if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
+    if constexpr (WIN) {
+        if (chunk_items > 0)
+            for (long long row = wid; row < (long long)a.num_tokens * a.g.Hq; row += all_workers) masked_row<D>(a, (int)(row / a.g.Hq), (int)(row % a.g.Hq));
+    }
 #ifdef PA_DECODE_PROF
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(prof_t[3]));
     if (lane == 0 && wid < 8192) {
@@ -771,16 +802,24 @@ long long decode_ctas(const KernelArgs& a, int per_sm, int sm_count) {
     return std::max(1LL, std::min((long long)std::min(per_sm, kDecodeMaxCtasPerSm) * sm_count, cap));
 }
 
+template <int D, int BS, int CACHE>
+auto pick_kernel(bool hi, bool sc, bool masked) {
+    auto kern = hi ? (sc ? decode_kernel<D, BS, CACHE, true, true, false> : decode_kernel<D, BS, CACHE, true, false, false>)
+                   : (sc ? decode_kernel<D, BS, CACHE, false, true, false> : decode_kernel<D, BS, CACHE, false, false, false>);
+    if (masked) kern = hi ? decode_kernel<D, BS, CACHE, true, false, true> : decode_kernel<D, BS, CACHE, false, false, true>;
+    return kern;
+}
+
 // Resident CTAs per SM of one instantiation on the current device; the shared-memory opt-in and the
 // occupancy query are made once per (instantiation, device), not on every step.
 template <int D, int BS, int CACHE>
 int occupancy_t(const KernelArgs& a) {
     using Cfg = DecodeCfg<D, BS, CACHE>;
     constexpr int kMaxDevices = 64;
-    static std::atomic<int> cache[4][kMaxDevices];   // 0 = unknown, else per_sm + 1
+    static std::atomic<int> cache[6][kMaxDevices];   // 0 = unknown, else per_sm + 1
     const bool hi = a.g.Hq / a.g.Hkv > 8;
     const bool sc = a.score_raw != nullptr && a.score_aggregation_window != nullptr;
-    const int slot = (hi ? 2 : 0) + (sc ? 1 : 0);
+    const int slot = (hi ? 3 : 0) + (a.m.on ? 2 : sc ? 1 : 0);
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const bool cached = dev >= 0 && dev < kMaxDevices;
@@ -788,8 +827,7 @@ int occupancy_t(const KernelArgs& a) {
         const int v = cache[slot][dev].load(std::memory_order_acquire);
         if (v > 0) return v - 1;
     }
-    auto kern = hi ? (sc ? decode_kernel<D, BS, CACHE, true, true> : decode_kernel<D, BS, CACHE, true, false>)
-                   : (sc ? decode_kernel<D, BS, CACHE, false, true> : decode_kernel<D, BS, CACHE, false, false>);
+    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, a.m.on != 0);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM) != cudaSuccess) return 0;
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kDecodeWarps * 32, Cfg::SMEM) != cudaSuccess) return 0;
@@ -803,8 +841,7 @@ cudaError_t launch_decode_t(const KernelArgs& a, cudaStream_t stream, int sm_cou
     const int G = a.g.Hq / a.g.Hkv;
     const bool hi = G > 8;
     const bool sc = a.score_raw != nullptr && a.score_aggregation_window != nullptr;
-    auto kern = hi ? (sc ? decode_kernel<D, BS, CACHE, true, true> : decode_kernel<D, BS, CACHE, true, false>)
-                   : (sc ? decode_kernel<D, BS, CACHE, false, true> : decode_kernel<D, BS, CACHE, false, false>);
+    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, a.m.on != 0);
     const int per_sm = occupancy_t<D, BS, CACHE>(a);
     if (per_sm < 1) return cudaErrorLaunchOutOfResources;
     const long long ctas = decode_ctas(a, per_sm, sm_count);

@@ -19,6 +19,7 @@ struct PlanHeader {
     int pitems_sorted; // 1: pitem_order lists the q tiles by decreasing context length
     int total_mitems;  // masked steps: pieces of q tiles (per kv head)
     int total_splits;  // masked steps: q tiles that are cut into several pieces
+    int total_redo;    // masked steps: rows that are computed again
 };
 
 constexpr int kPrefillSortCap = 2048;  // q tiles (per kv head) up to which the plan step orders them
@@ -95,6 +96,8 @@ struct MaskParams {
     int sm_count;
     MaskItem* items;
     MaskSplit* splits;         // [2 * sm_count]
+    int* redo;                 // [num_tokens * Hq] rows (token * Hq + head) that are not finite and are computed again, one by one
+    int rows_in_decode;        // the step has no launch for chunks: the decode kernel's warps see to those that it holds all the same
     int part_slots;            // partial results there is room for
     float* part_o;             // [part_slots][256][D]
     float2* part_ml;           // [part_slots][256] row maximum (base 2, scaled) and sum
@@ -220,6 +223,7 @@ cudaError_t launch_prefill_tc(const KernelArgs& a, cudaStream_t stream, int sm_c
 
 // Masked steps: rows of chunks one by one on CUDA cores (masked_rows.cu); what the acceptance of drafts does (tree_accept.cu).
 cudaError_t launch_masked_rows(const KernelArgs& a, cudaStream_t stream, int* launches);
+cudaError_t launch_masked_join(const KernelArgs& a, cudaStream_t stream, int* launches);   // of q tiles in pieces (masked_join.cu)
 
 constexpr int kMoveLayers = 96;   // layers of one launch that moves accepted tokens (their pointers travel as kernel arguments)
 struct TreeAcceptArgs {

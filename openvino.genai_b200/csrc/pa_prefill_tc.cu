@@ -34,10 +34,14 @@
 // register file with setmaxnreg once their roles start: 160 registers per softmax thread, 104 per converter thread, 88 for
 // the rest (one warp of each warpgroup shares a scheduler's 16 K registers).
 // Every wait is bounded; a wait that runs out raises a flag that all roles poll.
+// Masked steps (MK; include/masked_b200.h): an item is a piece of a q tile's list of context tiles (build_mask_items); a tile of which a row
+// sees a part takes that part from a word of bits; tokens that no row of the item sees go in as zeros and their blocks are not looked up; a piece
+// leaves its rows' sums, maxima and unnormalised results to masked_join_kernel.
 // Tensor-bound for long contexts: 4 * Hq * D flops per (new token, context token) pair.
 #include <algorithm>
 #include <cstdio>
 
+#include "masked.cuh"
 #include "pa_common.cuh"
 #include "pa_kernels.h"
 #include "tc05.cuh"
@@ -81,13 +85,24 @@ struct Item {
     const int32_t* table;
 };
 
-template <int BS, int CT, int D>
+// A masked step's item: tiles [j0, j0 + ntiles) of the q tile's list.
+struct MaskedItem : Item {
+    VisTiles v;
+    int lo;              // positions below it, beyond the sinks, are seen by no row
+    int j0;
+    int part;            // partial result, -1: the q tile is in one piece
+    int tree;
+};
+template <bool MK> struct ItemOf { using type = Item; };
+template <> struct ItemOf<true> { using type = MaskedItem; };
+
+template <int BS, int CT, int D, bool MK>
 struct PrefillSmem16;
-template <int BS, int CT, int D>
+template <int BS, int CT, int D, bool MK>
 struct PrefillSmem;
 
-template <int BS, int D>
-struct PrefillSmem<BS, PA_DTYPE_U8, D> {
+template <int BS, int D, bool MK>
+struct PrefillSmem<BS, PA_DTYPE_U8, D, MK> {
     static constexpr int NO = D + kDx;   // UMMA N of P.V
     static constexpr int NST = kStages;
     static constexpr int REC = BS * (D + 8);
@@ -116,19 +131,19 @@ struct PrefillSmem<BS, PA_DTYPE_U8, D> {
     alignas(8) uint64_t item_full[kItemSlots];   // loader -> every other warp
     alignas(8) uint64_t item_free[kItemSlots];   // every other warp -> loader: the slot has been read
     int item_ring[kItemSlots];
-    Item item_desc[kItemSlots];   // the loader locates an item once for every role
+    typename ItemOf<MK>::type item_desc[kItemSlots];   // the loader locates an item once for every role
     uint32_t tmem_base;
     volatile int abort;
 };
 
 // f16 / bf16 cache: operand tiles only.  The bf16 variant has no denominator columns (P takes their place in tensor memory
 // as two bf16 pieces, and the rows sum their own probabilities).
-template <int BS, int D>
-struct PrefillSmem<BS, PA_DTYPE_F16, D> : PrefillSmem16<BS, PA_DTYPE_F16, D> {};
-template <int BS, int D>
-struct PrefillSmem<BS, PA_DTYPE_BF16, D> : PrefillSmem16<BS, PA_DTYPE_BF16, D> {};
+template <int BS, int D, bool MK>
+struct PrefillSmem<BS, PA_DTYPE_F16, D, MK> : PrefillSmem16<BS, PA_DTYPE_F16, D, MK> {};
+template <int BS, int D, bool MK>
+struct PrefillSmem<BS, PA_DTYPE_BF16, D, MK> : PrefillSmem16<BS, PA_DTYPE_BF16, D, MK> {};
 
-template <int BS, int CT, int D>
+template <int BS, int CT, int D, bool MK>
 struct PrefillSmem16 {
     static constexpr int NO = CT == PA_DTYPE_BF16 ? D : D + kDx;
     static constexpr int NREC = kKv / BS;
@@ -150,7 +165,7 @@ struct PrefillSmem16 {
     alignas(8) uint64_t item_full[kItemSlots];
     alignas(8) uint64_t item_free[kItemSlots];
     int item_ring[kItemSlots];
-    Item item_desc[kItemSlots];   // the loader locates an item once for every role
+    typename ItemOf<MK>::type item_desc[kItemSlots];   // the loader locates an item once for every role
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -273,6 +288,29 @@ __device__ __forceinline__ Item locate_item(const KernelArgs& a, int item, int G
     return it;
 }
 
+__device__ __forceinline__ MaskedItem locate_masked(const KernelArgs& a, int item, int G, int Hkv) {
+    const int4* src = reinterpret_cast<const int4*>(a.m.items + item / Hkv);
+    const int4 x = __ldcg(src), y = __ldcg(src + 1), z = __ldcg(src + 2);
+    MaskedItem it;
+    it.s = 0;
+    it.hk = item % Hkv;
+    it.t0 = x.x; it.n_new = x.y; it.past = x.z;
+    it.table = a.block_indices + x.w;
+    it.row0 = y.x; it.j0 = y.y;
+    it.part = y.w < 0 ? -1 : y.w + it.hk;
+    it.tree = z.x;
+    const QTile q = q_tile(a.m, it.past, it.n_new, G, it.row0, it.tree);
+    it.v = q.v;
+    it.lo = q.lo;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        it.ctx_hi[h] = q.ctx_hi[h];
+        it.nt[h] = max(0, min(q.cnt[h], y.z) - it.j0);
+    }
+    it.ntiles = max(it.nt[0], it.nt[1]);
+    return it;
+}
+
 #ifdef PA_PREFILL_PROF
 // role (0, 1 softmax A, B; 2 converter; 3 mma; 4 loader; 5 second mma warp), event, tile 64..67 of CTA 0; 0: not met.  (In global
 // memory: the 16-bit variants use all shared memory there is.)
@@ -280,9 +318,10 @@ constexpr int kTraceRoles = 6;
 __device__ long long trace[kTraceRoles][8][4];
 #endif
 
-template <int BS, int CT, int D>
+template <int BS, int CT, int D, bool MK>
 __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
-    using Smem = PrefillSmem<BS, CT, D>;
+    using Smem = PrefillSmem<BS, CT, D, MK>;
+    using It = typename ItemOf<MK>::type;
     constexpr bool U8 = CT == PA_DTYPE_U8, BF = CT == PA_DTYPE_BF16;
     constexpr int kD = D, kNo = Smem::NO, kTmemP = 2 * kKv + 2 * kNo, NST = Smem::NST;
     constexpr int kPCols = BF ? kKv : kKv / 2;   // tensor-memory columns of one half's P: f16, or bf16 high + low pieces
@@ -295,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
     const int G = a.g.Hq / a.g.Hkv;
     const int Hkv = a.g.Hkv;
     grid_wait();
-    const int total_items = a.plan->total_ptiles * Hkv;
+    const int total_items = (MK ? a.plan->total_mitems : a.plan->total_ptiles) * Hkv;
     const float qscale = (a.scale != 0.f ? a.scale : rsqrtf((float)kD)) * kLog2eP;
 
     if (tid == 0) {
@@ -380,13 +419,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
     // Work items come from a global counter: the loader draws them and publishes each through a
     // small ring, so that all roles of the CTA walk the same sequence.  -1 ends the sequence, -2
     // reports a wait that ran out.
-    auto fetch_item = [&](uint32_t k, Item& it) -> int {
+    auto fetch_item = [&](uint32_t k, It& it) -> int {
         const int slot = k & (kItemSlots - 1);
         if (!wait_warp(&sm.item_full[slot], (k / kItemSlots) & 1, 0)) return -2;
         const int item = sm.item_ring[slot];
         if (item >= 0) it = sm.item_desc[slot];
         warp_arrive(&sm.item_free[slot]);
         return item;
+    };
+
+    // first context position of an item's j-th tile; whether any row of the item sees a position
+    auto tile_pos = [&](const It& it, int j) -> int {
+        if constexpr (MK) return it.v.tile(it.j0 + j) * kKv;
+        else return j * kKv;
+    };
+    auto seen = [&](const It& it, int ctx_hi, int pos) -> bool {
+        if constexpr (MK) return pos < ctx_hi && (pos < a.m.sinks || pos >= it.lo);
+        else return pos < ctx_hi;
     };
 
     if (warp >= kWarpMma) reg_dec<PA_TC_REG_MISC>();   // the fourth warpgroup: mma, loader, second mma; what is left over keeps it whole
@@ -400,14 +449,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         const uint32_t tmem_p = tmem + kTmemP + kPCols * X + lane_base;
         uint32_t n = 0;   // tiles of this half so far, over all items
         uint32_t ik = 0;
-        Item it;
+        It it;
         // This thread's row of the item in work; the next item's is staged before this one's epilogue.
         struct Row {
             long long off;   // (token, q head) row of query / output
             int ctx;         // context it sees
             bool live;
             float qs;        // softmax scale: the kernel's, divided by the row's prescale
-        } row{0, 0, false, qscale};
+            int lo, tok;     // masked: begin of its window; its token's row of tree words, -1: no tree
+        } row{0, 0, false, qscale, 0, -1};
         // The next item with rows in this half: 1, none left: 0, a wait ran out: -1
         auto next_item = [&]() -> int {
             for (;;) {
@@ -427,7 +477,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             const int flat = it.row0 + X * kRows + r;
             const int tok = flat / G, hq = it.hk * G + flat % G;
             row.live = tok < it.n_new;
-            row.ctx = row.live ? it.past + tok + 1 : it.ctx_hi[X];
+            if constexpr (MK) {
+                row.tok = -1;
+                row.ctx = 0x7fffffff; row.lo = 0;   // (a row that is none sees zeros)
+                if (row.live) {
+                    if (it.tree) {
+                        row.tok = it.t0 + tok;
+                        row.ctx = it.past;
+                        row.lo = window_lo(a.m, it.past + __ldcg(a.m.tree_depth + row.tok) + 1);
+                    } else {
+                        row.ctx = it.past + tok + 1;
+                        row.lo = window_lo(a.m, row.ctx);
+                    }
+                }
+            } else {
+                row.ctx = row.live ? it.past + tok + 1 : it.ctx_hi[X];
+            }
             row.off = ((long long)(it.t0 + (row.live ? tok : 0)) * a.g.Hq + hq);
             row.qs = qscale;
             const int wrow = r & ~31;                                  // the warp's first row
@@ -580,11 +645,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         while (have) {
             const int nt = it.nt[X], my_ctx = row.ctx;
             const float qs = row.qs;
+            int my_lo = 0, my_tok = -1;
+            if constexpr (MK) { my_lo = row.lo; my_tok = row.tok; }
 
             float m_run = -INFINITY;   // running maximum of q.k' (before the softmax scale)
             float l_own = 0.f;         // bf16 variant: the row's own sum of probabilities
             for (int j = 0; j < nt; ++j, ++n) {
-                const int col0 = j * kKv;
+                const int col0 = tile_pos(it, j);
                 if (!wait_warp(&sm.s_full[X], n & 1, 0)) goto done;
                 if ((warp & 3) == 0) PA_TRACE(X, 0, n);
                 tc05::fence_after_thread_sync();
@@ -602,7 +669,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     warp_arrive(&sm.s_read[X]);
                 }
                 if ((warp & 3) == 0) PA_TRACE(X, 1, n);
-                if (col0 + kKv > my_ctx) {     // diagonal tile: hide what this row cannot see
+                if constexpr (MK) {            // a tile that this row does not see as a whole
+                    if (col0 + kKv > my_ctx || (col0 < my_lo && col0 + kKv > a.m.sinks)) {
+                        uint64_t w = causal_bits(col0, my_ctx, my_lo, a.m.sinks);
+                        if (my_tok >= 0 && col0 + kKv > it.past) w |= tree_bits64(a.m.tree_words + (long long)my_tok * kTreeWords, col0 - it.past);
+                        const uint32_t w0 = (uint32_t)w, w1 = (uint32_t)(w >> 32);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            sv[c] = (w0 >> c) & 1u ? sv[c] : -INFINITY;
+                            sv[32 + c] = (w1 >> c) & 1u ? sv[32 + c] : -INFINITY;
+                        }
+                    }
+                } else if (col0 + kKv > my_ctx) {     // diagonal tile: hide what this row cannot see
                     const int nvis = my_ctx - col0;   // may be <= 0
 #pragma unroll
                     for (int c = 0; c < kKv; ++c) sv[c] = c < nvis ? sv[c] : -INFINITY;
@@ -613,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 float alpha = 1.f;
                 bool rescale = false;
                 if (j == 0) {
-                    m_run = mx;      // finite: column 0 of tile 0 is visible to every row
+                    m_run = mx;      // finite: column 0 of tile 0 is visible to every row (masked: of a first tile a row may see nothing)
                 } else {
                     const bool grow = (mx - m_run) * qs > kLazy;
                     rescale = __any_sync(0xffffffffu, grow);
@@ -622,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 if constexpr (BF) l_own *= alpha;
                 // P = 2^(qs * (s - m)) in f16 pairs: the exponent is rounded to f16 first, which costs
                 // at most 2^-12 of the exponent's magnitude in relative error of p
-                const float mq = m_run * qs;
+                const float mq = MK && m_run == -INFINITY ? 0.f : m_run * qs;   // (nothing seen yet: every p is 0)
                 uint32_t pw[kKv / 2];
                 uint32_t pl[BF ? kKv / 2 : 1];   // bf16 variant: the low pieces, p = high + low up to 2^-17 p
 #pragma unroll
@@ -678,6 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             // ---- the next item's rows, so that its first logits are computed beside this item's last P.V and epilogue (its
             // first P, which starts a new O, comes after) ---------------------------------------------------
             const Row cur = row;
+            int part = -1;
+            if constexpr (MK) part = it.part;
             have = next_item();
             if (have < 0) goto done;
             if (have) stage_q();
@@ -694,12 +774,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     if constexpr (U8) z = __uint_as_float(zr[0]) + __uint_as_float(zr[1]) + __uint_as_float(zr[2]);
                     l_run = __uint_as_float(zr[U8 ? 3 : 0]);
                 }
-                const float inv = 1.f / l_run;
+                const bool whole = !MK || part < 0;   // else a piece: unnormalised, to the scratch
+                const float inv = whole ? 1.f / l_run : 1.f;
                 // 128 bytes of every row at a time, turned around in shared memory so that eight lanes store one row's piece (a
                 // thread storing its own row touched 32 lines with every store: 7 k cycles an item)
                 uint8_t* const stg = sm.out_stage[warp];
-                const int own = cur.live ? (int)cur.off : -1;
+                const int own = cur.live ? (whole ? (int)cur.off : X * kRows + r) : -1;
+                uint8_t* const dst = whole ? (uint8_t*)a.output : (uint8_t*)(a.m.part_o + (long long)part * kPrefillItemRows * kD);
                 const int c8 = lane & 7;
+                bool finite = true;   // masked: a result that is not may come from what the row does not see
                 auto put = [&](int c, const uint4& w) { *reinterpret_cast<uint4*>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) = w; };
                 auto send = [&](int piece, int row_bytes) {   // the piece of every row of the warp
                     __syncwarp();
@@ -707,11 +790,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     for (int i = 0; i < 8; ++i) {
                         const int rr = 4 * i + (lane >> 3), o = __shfl_sync(0xffffffffu, own, rr);
                         const uint4 w = *reinterpret_cast<const uint4*>(stg + rr * 128 + ((c8 ^ (rr & 7)) << 4));
-                        if (o >= 0) *reinterpret_cast<uint4*>((uint8_t*)a.output + (long long)o * row_bytes + 128 * piece + 16 * c8) = w;
+                        if (o >= 0) *reinterpret_cast<uint4*>(dst + (long long)o * row_bytes + 128 * piece + 16 * c8) = w;
                     }
                     __syncwarp();
                 };
-                if (a.g.act == PA_DTYPE_F32) {
+                if (a.g.act == PA_DTYPE_F32 || !whole) {
 #pragma unroll
                     for (int q4 = 0; q4 < kD / 32; ++q4) {
                         uint32_t t[32];
@@ -721,7 +804,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                         for (int c = 0; c < 8; ++c) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = __float_as_uint((__uint_as_float(t[4 * c + e]) - z) * inv);
+                            for (int e = 0; e < 4; ++e) {
+                                w[e] = __float_as_uint((__uint_as_float(t[4 * c + e]) - z) * inv);
+                                if constexpr (MK) finite = finite && !not_finite(__uint_as_float(w[e]));
+                            }
                             put(c, make_uint4(w[0], w[1], w[2], w[3]));
                         }
                         send(q4, kD * 4);
@@ -742,6 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                                 for (int e = 0; e < 4; ++e) {
                                     const float v0 = (__uint_as_float(t[8 * c + 2 * e]) - z) * inv, v1 = (__uint_as_float(t[8 * c + 2 * e + 1]) - z) * inv;
                                     w[e] = f16 ? pack_h2(v0, v1) : pack_bf2(v0, v1);
+                                    if constexpr (MK) finite = finite && !not_finite(v0) && !not_finite(v1);
                                 }
                                 put(4 * h + c, make_uint4(w[0], w[1], w[2], w[3]));
                             }
@@ -749,7 +836,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                         send(q, kD * 2);
                     }
                 }
-                if (cur.live && a.lse) a.lse[cur.off] = (m_run * cur.qs + log2f(l_run)) * kLn2P;
+                if (MK && whole && cur.live && !finite) a.m.redo[atomicAdd(&a.plan->total_redo, 1)] = (int)cur.off;
+                if (MK && !whole) {
+                    if (cur.live) a.m.part_ml[(long long)part * kPrefillItemRows + X * kRows + r] = make_float2(m_run * cur.qs, l_run);
+                } else if (cur.live && a.lse) {
+                    a.lse[cur.off] = (m_run * cur.qs + log2f(l_run)) * kLn2P;
+                }
             }
             tc05::fence_before_thread_sync();
         }
@@ -760,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         if constexpr (U8) {
         uint32_t t = 0;   // tiles so far, over all items
         for (uint32_t ik = 0;; ++ik) {
-            Item it;
+            It it;
             const int item = fetch_item(ik, it);
             if (item == -2) goto done;
             if (item < 0) break;
@@ -768,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             for (int j = 0; j < it.ntiles; ++j, ++t) {
                 const int st = t & 1;
                 const uint32_t use = t >> 1;
-                const int live_tokens = min(kKv, ctx_hi - j * kKv);
+                const int pos0 = tile_pos(it, j);
                 const uint8_t* raw_k = sm.raw_k[st];
                 const uint8_t* raw_v = sm.raw_v[st];
                 if (!wait_warp(&sm.raw_full[st], use & 1, 0)) goto done;
@@ -781,7 +873,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     const int u = ctid + 128 * i;
                     const int token = u / (kD / 16), seg = u % (kD / 16);
                     uint4 lo4 = make_uint4(0u, 0u, 0u, 0u), hi4 = lo4;
-                    if (token < live_tokens) {
+                    if (seen(it, ctx_hi, pos0 + token)) {
                         const uint8_t* rec = raw_k + (token / BS) * Smem::RSTRIDE;
                         const __half ksh = f2h(*reinterpret_cast<const float*>(rec + BS * kD + 4 * (token % BS)));
                         bytes16_to_h(*reinterpret_cast<const uint4*>(rec + (token % BS) * kD + 16 * seg), lo4, hi4);
@@ -793,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 }
                 if (ctid < kKv) {
                     const int token = ctid;
-                    const bool ok = token < live_tokens;
+                    const bool ok = seen(it, ctx_hi, pos0 + token);
                     const float* kp = reinterpret_cast<const float*>(raw_k + (token / BS) * Smem::RSTRIDE + BS * kD);
                     const float ksf = __half2float(f2h(kp[token % BS]));
                     __half zh, zm, zl;
@@ -813,8 +905,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 float vs0 = 0.f, vs1 = 0.f;
                 {
                     const int t0k = 2 * lane, t1k = 2 * lane + 1;
-                    if (t0k < live_tokens) vs0 = *reinterpret_cast<const float*>(raw_v + (t0k / BS) * Smem::RSTRIDE + BS * kD + 4 * (t0k % BS));
-                    if (t1k < live_tokens) vs1 = *reinterpret_cast<const float*>(raw_v + (t1k / BS) * Smem::RSTRIDE + BS * kD + 4 * (t1k % BS));
+                    if (seen(it, ctx_hi, pos0 + t0k)) vs0 = *reinterpret_cast<const float*>(raw_v + (t0k / BS) * Smem::RSTRIDE + BS * kD + 4 * (t0k % BS));
+                    if (seen(it, ctx_hi, pos0 + t1k)) vs1 = *reinterpret_cast<const float*>(raw_v + (t1k / BS) * Smem::RSTRIDE + BS * kD + 4 * (t1k % BS));
                 }
                 const uint32_t s2 = pack_h2(vs0, vs1);
                 sm.v_tab[cwarp][lane] = make_uint2(s2, hmul2_bits(s2, 0xE400E400u));
@@ -848,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 }
                 if (ctid < kKv) {
                     const int token = ctid;
-                    const bool ok = token < live_tokens;
+                    const bool ok = seen(it, ctx_hi, pos0 + token);
                     const float* vp = reinterpret_cast<const float*>(raw_v + (token / BS) * Smem::RSTRIDE + BS * kD);
                     const float vsf = __half2float(f2h(vp[token % BS]));
                     __half zh, zm, zl;
@@ -877,7 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             uint32_t t = 0;
             bool bad_index = false;
             for (uint32_t ik = 0;; ++ik) {
-                Item it;
+                It it;
                 const int item = fetch_item(ik, it);
                 if (item == -2) goto done;
                 if (item < 0) break;
@@ -887,14 +979,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 for (int j = 0; j < it.ntiles; ++j, ++t) {
                     const int st = t % NST, stp = (t + NST - 1) % NST;
                     const uint32_t use = t / NST;
-                    const int live_tokens = min(kKv, ctx_hi - j * kKv);
+                    const int pos0 = tile_pos(it, j);
                     long long off[NU];   // byte offset of this thread's chunk of token trow + TP u; -1: beyond the context
 #pragma unroll
                     for (int u = 0; u < NU; ++u) {
                         const int token = trow + TP * u;
                         off[u] = -1;
-                        if (token < live_tokens) {
-                            int blk = it.table[j * Smem::NREC + token / BS];
+                        if (seen(it, ctx_hi, pos0 + token)) {
+                            int blk = it.table[pos0 / BS + token / BS];
                             if (blk < 0 || blk >= a.num_blocks) { blk = 0; bad_index = true; }
                             off[u] = (long long)blk * a.g.block_bytes + (long long)(token % BS) * (kD * 2);
                         }
@@ -1015,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             if constexpr (U8) {
                 uint32_t n[2] = {0, 0}, iq[2] = {0, 0};
                 for (uint32_t ik = 0;; ++ik) {
-                    Item it;
+                    It it;
                     const int item = fetch_item(ik, it);
                     if (item == -2) goto done;
                     if (item < 0) break;
@@ -1067,7 +1159,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 const int X = warp == kWarpMma ? 0 : 1;
                 uint32_t n = 0, iq = 0;   // tiles and items of this half
                 for (uint32_t ik = 0;; ++ik) {
-                    Item it;
+                    It it;
                     const int item = fetch_item(ik, it);
                     if (item == -2) goto done;
                     if (item < 0) break;
@@ -1133,9 +1225,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 }
                 int item = atomicAdd(&a.plan->next_pitem, 1);
                 if (item >= total_items) item = -1;
-                Item it{};
+                It it{};
                 if (item >= 0) {
-                    it = locate_item(a, item, G, Hkv);
+                    if constexpr (MK) it = locate_masked(a, item, G, Hkv);
+                    else it = locate_item(a, item, G, Hkv);
                     sm.item_desc[slot] = it;
                 }
                 sm.item_ring[slot] = item;
@@ -1148,15 +1241,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 for (int j = 0; j < it.ntiles; ++j, ++t) {
                     const int st = t & 1;
                     const uint32_t use = t >> 1;
+                    const int pos0 = tile_pos(it, j);
                     if (use > 0 && !wait(&sm.raw_free[st], (use - 1) & 1, 0)) goto done;
                     PA_TRACE(4, 0, t);
                     uint32_t bytes = 0;
                     int blocks[Smem::NREC];
 #pragma unroll
                     for (int r = 0; r < Smem::NREC; ++r) {
-                        const int bi = j * Smem::NREC + r;
+                        const int bi = pos0 / BS + r;
                         int blk = -1;
-                        if (bi * BS < ctx_hi) {
+                        bool any = bi * BS < ctx_hi;
+                        if constexpr (MK) any = any && (bi * BS < a.m.sinks || (bi + 1) * BS > it.lo);
+                        if (any) {
                             blk = it.table[bi];
                             if (blk < 0 || blk >= a.num_blocks) { blk = 0; bad_index = true; }
                             bytes += 2 * Smem::REC;
@@ -1205,16 +1301,20 @@ bool prefill_tc_supported(const CacheGeom& g) {
 }
 
 namespace {
-template <int BS, int CT, int D>
+template <int BS, int CT, int D, bool MK>
 cudaError_t launch_tc_t(const KernelArgs& a, cudaStream_t stream, int grid) {
-    const int bytes = (int)sizeof(PrefillSmem<BS, CT, D>) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<BS, CT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = (int)sizeof(PrefillSmem<BS, CT, D, MK>) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<BS, CT, D, MK>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    return launch_dependent(prefill_tc_kernel<BS, CT, D>, dim3(grid), dim3(kThreads), bytes, stream, a);
+    return launch_dependent(prefill_tc_kernel<BS, CT, D, MK>, dim3(grid), dim3(kThreads), bytes, stream, a);
+}
+template <int CT, int D, bool MK>
+cudaError_t launch_tc_bs(const KernelArgs& a, cudaStream_t stream, int grid) {
+    return a.g.bs == 32 ? launch_tc_t<32, CT, D, MK>(a, stream, grid) : launch_tc_t<16, CT, D, MK>(a, stream, grid);
 }
 template <int CT, int D>
-cudaError_t launch_tc_bs(const KernelArgs& a, cudaStream_t stream, int grid) {
-    return a.g.bs == 32 ? launch_tc_t<32, CT, D>(a, stream, grid) : launch_tc_t<16, CT, D>(a, stream, grid);
+cudaError_t launch_tc_mk(const KernelArgs& a, cudaStream_t stream, int grid) {
+    return a.m.on ? launch_tc_bs<CT, D, true>(a, stream, grid) : launch_tc_bs<CT, D, false>(a, stream, grid);
 }
 }  // namespace
 
@@ -1222,9 +1322,9 @@ cudaError_t launch_prefill_tc(const KernelArgs& a, cudaStream_t stream, int sm_c
     if (max_items <= 0) return cudaSuccess;
     const int grid = (int)std::min<long long>(max_items, sm_count);
     cudaError_t e;
-    if (a.g.cache == PA_DTYPE_U8) e = a.g.D == 128 ? launch_tc_bs<PA_DTYPE_U8, 128>(a, stream, grid) : launch_tc_bs<PA_DTYPE_U8, 64>(a, stream, grid);
-    else if (a.g.cache == PA_DTYPE_F16) e = a.g.D == 128 ? launch_tc_bs<PA_DTYPE_F16, 128>(a, stream, grid) : launch_tc_bs<PA_DTYPE_F16, 64>(a, stream, grid);
-    else e = a.g.D == 128 ? launch_tc_bs<PA_DTYPE_BF16, 128>(a, stream, grid) : launch_tc_bs<PA_DTYPE_BF16, 64>(a, stream, grid);
+    if (a.g.cache == PA_DTYPE_U8) e = a.g.D == 128 ? launch_tc_mk<PA_DTYPE_U8, 128>(a, stream, grid) : launch_tc_mk<PA_DTYPE_U8, 64>(a, stream, grid);
+    else if (a.g.cache == PA_DTYPE_F16) e = a.g.D == 128 ? launch_tc_mk<PA_DTYPE_F16, 128>(a, stream, grid) : launch_tc_mk<PA_DTYPE_F16, 64>(a, stream, grid);
+    else e = a.g.D == 128 ? launch_tc_mk<PA_DTYPE_BF16, 128>(a, stream, grid) : launch_tc_mk<PA_DTYPE_BF16, 64>(a, stream, grid);
     if (e != cudaSuccess) return e;
     ++*launches;
     return cudaSuccess;

@@ -245,3 +245,13 @@ def test_refusals_of_tensors():
     assert bool((out == 0).all())
     op.evaluate(good, {"output": out})
     step.check(out)
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "u8"), ("f32", "bf16")])
+def test_chunks_beside_sequences_without_tokens(act, cache):
+    """As many tokens as sequences, or fewer, and chunks among them all the same."""
+    rng = np.random.default_rng(2)
+    for new in ([0, 2], [3, 0, 0], [0, 0, 2, 1, 0, 0], [1, 5, 0, 0, 0, 0], [0, 4, 0, 0, 0, 0, 0]):
+        past = [int(rng.integers(0, 90)) for _ in new]
+        _whole(H.Step(past, new, act=act, cache=cache, window=20, sinks=2, seed=len(new)))
+        _whole(H.Step(past, new, act=act, cache=cache, trees=[H.tree(rng, n) if n > 1 else None for n in new], seed=len(new)))
