@@ -64,86 +64,88 @@ __global__ void __launch_bounds__(kTreeMax) tree_walk_kernel(TreeAcceptArgs a) {
         const int last = walk ? at : accepted - 1;
         a.num_accepted[s] = accepted;
         a.next_token[s] = accepted > 0 ? a.sampled[v.t0 + last] : -1;
+        if (a.new_past_lens) a.new_past_lens[s] = a.past_lens[s] + accepted;
     }
 }
 
-// Rows of one (sequence, layer, keys or values) per block.  A row moves from past + path[k] to past + k <= past + path[k]: nothing that a later move
-// reads is written by an earlier one, but a row may be both read and written, so all rows of a head are read before the first is written.
-template <int D>
-__global__ void __launch_bounds__(256) tree_move_kernel(const __grid_constant__ TreeMoveArgs m) {
-    const TreeAcceptArgs& a = m.t;
-    __shared__ int sh_src[kTreeMax], sh_dst[kTreeMax];   // slots (block * bs + slot), -1: stays
-    grid_wait();
-    const int s = blockIdx.x, layer = blockIdx.y >> 1, value = blockIdx.y & 1, tid = threadIdx.x;
-    SeqView v;
-    accept_view(a, s, v, false);
-    const bool walk = v.n > 0 && v.n <= kTreeMax && a.parents[v.t0] != kTreeNone;
-    const int count = walk ? min(a.num_accepted[s], a.max_path) : 0;
-    bool moves = false;
-    if (tid < count) {
-        const int from = a.path[(long long)s * a.max_path + tid];
-        int src = -1, dst = -1;
-        if (from != tid) {
-            const int p0 = v.past + from, p1 = v.past + tid;
-            const int b0 = a.block_indices[v.tb + p0 / a.g.bs], b1 = a.block_indices[v.tb + p1 / a.g.bs];
-            if (b0 < 0 || b0 >= a.num_blocks || b1 < 0 || b1 >= a.num_blocks) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
-            else { src = b0 * a.g.bs + p0 % a.g.bs; dst = b1 * a.g.bs + p1 % a.g.bs; moves = true; }
+// The accepted rows of one sequence, a block for the keys or the values of a layer at a time.  A row moves from past + path[k] to past + k, never
+// up: a later row's place is not overwritten by an earlier one's move, so a thread that owns the same bytes of every row and goes along the path reads each of
+// them in time.  Token-minor u8 values are single bytes out of 32-byte sectors: what bounds the move of a batch of trees (64 trees, 32 layers: 26 MB of
+// rows in some 300 MB of sectors, 0.05 ms of HBM).  kMoveBatch rows' loads are under way before the first store; more of them, or several pieces a thread,
+// cost registers and so blocks beside one another (54 | 75 us).
+constexpr int kMoveBatch = 4;
+constexpr int kMoveThreads = 256;
+
+// Unit u of `units` of every row: unit(u) is where a row's unit lies in slot 0 of block 0, slot(x) the offset of slot x.
+template <class T, class Unit, class Slot>
+__device__ __forceinline__ void move_rows(uint8_t* cache, int units, int count, const int* src, const int* dst, int bs, long long block_bytes, Unit&& unit, Slot&& slot) {
+    for (int u = threadIdx.x; u < units; u += kMoveThreads) {
+        uint8_t* const base = cache + unit(u);
+        for (int k0 = 0; k0 < count; k0 += kMoveBatch) {
+            T w[kMoveBatch];
+#pragma unroll
+            for (int k = 0; k < kMoveBatch; ++k)
+                if (k0 + k < count) w[k] = *reinterpret_cast<const T*>(base + (long long)(src[k0 + k] / bs) * block_bytes + slot(src[k0 + k] % bs));
+#pragma unroll
+            for (int k = 0; k < kMoveBatch; ++k)
+                if (k0 + k < count) *reinterpret_cast<T*>(base + (long long)(dst[k0 + k] / bs) * block_bytes + slot(dst[k0 + k] % bs)) = w[k];
         }
-        sh_src[tid] = src;
-        sh_dst[tid] = dst;
     }
-    if (!__syncthreads_or(moves)) return;
-    uint8_t* const cache = m.cache[value][layer];
-    const int bs = a.g.bs;
-    // a thread's own elements of every row: no two threads touch the same bytes, so a thread that goes along the path in order reads
-    // each of them before it is overwritten
-    if (a.g.cache != PA_DTYPE_U8) {
-        constexpr int CH = D / 8;   // 16-byte chunks of a row
-        for (int u = tid; u < a.g.Hkv * CH; u += 256) {
-            uint8_t* const head = cache + (long long)(u / CH) * a.g.head_bytes + 16 * (u % CH);
-            for (int k = 0; k < count; ++k) {
-                if (sh_src[k] < 0) continue;
-                const uint4 w = *reinterpret_cast<const uint4*>(head + (long long)(sh_src[k] / bs) * a.g.block_bytes + (long long)(sh_src[k] % bs) * D * 2);
-                *reinterpret_cast<uint4*>(head + (long long)(sh_dst[k] / bs) * a.g.block_bytes + (long long)(sh_dst[k] % bs) * D * 2) = w;
-            }
+}
+
+template <int D, int BS>
+__global__ void __launch_bounds__(kMoveThreads) tree_move_kernel(const __grid_constant__ TreeMoveArgs m) {
+    const TreeAcceptArgs& a = m.t;
+    __shared__ int sh_src[kTreeMax], sh_dst[kTreeMax];   // slots (block * BS + slot) of the rows that move
+    __shared__ int sh_moves[kTreeMax / 32];
+    grid_wait();
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kMoveWarps = kMoveThreads / 32;
+    static_assert(kMoveThreads == kTreeMax, "a thread per place of a path");
+    const int tb = a.block_indices_begins[s], count = a.num_accepted[s];
+    const int from = tid < a.max_path ? a.path[(long long)s * a.max_path + tid] : -1;   // (-1 everywhere without a tree, and where the metadata are bad)
+    const int past = a.past_lens[s] - (a.new_past_lens == a.past_lens ? count : 0);     // (the walk has written the new ones)
+    int src = -1, dst = -1;
+    if (from >= 0 && from != tid) {
+        const int p0 = past + from, p1 = past + tid;
+        const int b0 = a.block_indices[tb + p0 / BS], b1 = a.block_indices[tb + p1 / BS];
+        if (b0 < 0 || b0 >= a.num_blocks || b1 < 0 || b1 >= a.num_blocks) {
+            if (blockIdx.y == 0) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
+        } else {
+            src = b0 * BS + p0 % BS;
+            dst = b1 * BS + p1 % BS;
         }
+    }
+    // the list of moves, in the order of the path
+    const uint32_t mine = __ballot_sync(0xffffffffu, src >= 0);
+    if (lane == 0) sh_moves[warp] = __popc(mine);
+    __syncthreads();
+    int at = __popc(mine & ((1u << lane) - 1u)), moves = 0;
+    for (int w = 0; w < kMoveWarps; ++w) {
+        if (w < warp) at += sh_moves[w];
+        moves += sh_moves[w];
+    }
+    if (src >= 0) { sh_src[at] = src; sh_dst[at] = dst; }
+    if (moves == 0) return;
+    __syncthreads();
+    const bool u8 = a.g.cache == PA_DTYPE_U8;
+    const int heads = a.g.Hkv;
+    const long long hb = a.g.head_bytes, bb = a.g.block_bytes;
+    uint8_t* const cache = m.cache[blockIdx.y & 1][blockIdx.y >> 1];
+    const bool value = (blockIdx.y & 1) != 0;
+    if (!u8) {
+        constexpr int CH = D / 8;   // 16-byte pieces of a row
+        move_rows<uint4>(cache, heads * CH, moves, sh_src, sh_dst, BS, bb, [&](int u) { return (u / CH) * hb + 16 * (u % CH); }, [](int x) { return x * D * 2; });
         return;
     }
     if (!value) {
         constexpr int CH = D / 16;
-        for (int u = tid; u < a.g.Hkv * CH; u += 256) {
-            uint8_t* const head = cache + (long long)(u / CH) * a.g.head_bytes + 16 * (u % CH);
-            for (int k = 0; k < count; ++k) {
-                if (sh_src[k] < 0) continue;
-                const uint4 w = *reinterpret_cast<const uint4*>(head + (long long)(sh_src[k] / bs) * a.g.block_bytes + (long long)(sh_src[k] % bs) * D);
-                *reinterpret_cast<uint4*>(head + (long long)(sh_dst[k] / bs) * a.g.block_bytes + (long long)(sh_dst[k] % bs) * D) = w;
-            }
-        }
-    } else {   // value bytes are token-minor: [D][bs]
-        for (int u = tid; u < a.g.Hkv * D; u += 256) {
-            uint8_t* const head = cache + (long long)(u / D) * a.g.head_bytes + (long long)(u % D) * bs;
-            for (int k = 0; k < count; ++k) {
-                if (sh_src[k] < 0) continue;
-                const uint8_t b = head[(long long)(sh_src[k] / bs) * a.g.block_bytes + sh_src[k] % bs];
-                head[(long long)(sh_dst[k] / bs) * a.g.block_bytes + sh_dst[k] % bs] = b;
-            }
-        }
+        move_rows<uint4>(cache, heads * CH, moves, sh_src, sh_dst, BS, bb, [&](int u) { return (u / CH) * hb + 16 * (u % CH); }, [](int x) { return x * D; });
+    } else {
+        move_rows<uint8_t>(cache, heads * D, moves, sh_src, sh_dst, BS, bb, [&](int u) { return (u / D) * hb + (u % D) * BS; }, [](int x) { return x; });
     }
-    for (int u = tid; u < a.g.Hkv * 2; u += 256) {   // scales and zero-points
-        uint8_t* const head = cache + (long long)(u >> 1) * a.g.head_bytes + (long long)bs * D + (long long)(u & 1) * bs * 4;
-        for (int k = 0; k < count; ++k) {
-            if (sh_src[k] < 0) continue;
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(head + (long long)(sh_src[k] / bs) * a.g.block_bytes + 4 * (sh_src[k] % bs));
-            *reinterpret_cast<uint32_t*>(head + (long long)(sh_dst[k] / bs) * a.g.block_bytes + 4 * (sh_dst[k] % bs)) = w;
-        }
-    }
-}
-
-// new_past_lens comes last: it may be past_lens, which the moves read.
-__global__ void __launch_bounds__(256) tree_past_kernel(TreeAcceptArgs a) {
-    grid_wait();
-    const int s = blockIdx.x * 256 + threadIdx.x;
-    if (s < a.num_sequences) a.new_past_lens[s] = a.past_lens[s] + a.num_accepted[s];
+    // scales and zero-points
+    move_rows<uint32_t>(cache, heads * 2, moves, sh_src, sh_dst, BS, bb, [&](int u) { return (u >> 1) * hb + BS * D + (u & 1) * BS * 4; }, [](int x) { return 4 * x; });
 }
 
 }  // namespace
@@ -161,13 +163,10 @@ cudaError_t launch_tree_accept(const TreeAcceptArgs& a, void* const* key_caches,
             m.cache[0][i] = (uint8_t*)key_caches[l0 + i];
             m.cache[1][i] = (uint8_t*)value_caches[l0 + i];
         }
-        const dim3 grid(a.num_sequences, 2 * m.num_layers);
-        e = a.g.D == 128 ? launch_dependent(tree_move_kernel<128>, grid, dim3(256), 0, stream, m) : launch_dependent(tree_move_kernel<64>, grid, dim3(256), 0, stream, m);
-        if (e != cudaSuccess) return e;
-        ++*launches;
-    }
-    if (a.new_past_lens) {
-        e = launch_dependent(tree_past_kernel, dim3((a.num_sequences + 255) / 256), dim3(256), 0, stream, a);
+        const dim3 grid(a.num_sequences, 2 * m.num_layers);   // a block per layer's keys or values
+        auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, dim3(kMoveThreads), 0, stream, m); };
+        if (a.g.D == 128) e = a.g.bs == 32 ? launch(tree_move_kernel<128, 32>) : launch(tree_move_kernel<128, 16>);
+        else e = a.g.bs == 32 ? launch(tree_move_kernel<64, 32>) : launch(tree_move_kernel<64, 16>);
         if (e != cudaSuccess) return e;
         ++*launches;
     }

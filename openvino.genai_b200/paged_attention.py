@@ -14,6 +14,7 @@ of.  `tree_accept` follows the sampled tokens down the trees behind such a step 
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional
 
 import numpy as np
@@ -31,6 +32,13 @@ def _ptr(t) -> Optional[int]:
     if isinstance(t, np.ndarray):
         return t.ctypes.data
     return t.data_ptr()
+
+
+def _alike(tensors) -> bool:
+    """Whether all of them are contiguous tensors of one type, size and device."""
+    T = torch.Tensor
+    return set(map(type, tensors)) <= {T} and all(map(T.is_contiguous, tensors)) and \
+        max(len(set(map(f, tensors))) for f in (T.get_device, T.numel, operator.attrgetter("dtype"))) <= 1
 
 
 class PagedAttentionExtension:
@@ -244,17 +252,20 @@ class PagedAttentionExtension:
         keys, values = inputs.get("key_caches") or (), inputs.get("value_caches") or ()
         if len(keys) != len(values):
             raise self._err("key_caches and value_caches differ in layers")
-        counts = {self._blocks(name, t) for name, group in (("key_caches", keys), ("value_caches", values)) for t in group}
-        if len(counts) > 1:
-            raise self._err("the layers' caches differ in blocks")
+        caches = (*keys, *values)
+        if not _alike(caches):    # (a model's worth of tensors: who is not like the others is asked for by name)
+            counts = {self._blocks("key_caches and value_caches", t) for t in caches}
+            if len(counts) > 1:
+                raise self._err("the layers' caches differ in blocks")
+        num_blocks = self._blocks("key_caches", caches[0]) if caches else 0
         if not isinstance(path, torch.Tensor) or path.dim() != 2:
             self._refuse("path", path, "contiguous int32 [sequences, max_path]")
         layers = len(keys)
-        addresses = tuple((C.c_void_p * layers)(*(t.data_ptr() for t in group)) for group in (keys, values))
+        addresses = tuple((C.c_void_p * layers)(*map(torch.Tensor.data_ptr, group)) for group in (keys, values))
         past_out = outputs.get("new_past_lens")
         M.ACCEPT_ARGS.pack_into(self._accept_buffer, 0, M.ACCEPT_ARGS.size, whole("tree_parents", parents, i32, (T,)),
                                 whole("draft_tokens", inputs["draft_tokens"], i64, (T,)), whole("sampled_tokens", inputs["sampled_tokens"], i64, (T,)), *meta, T, B,
-                                num_indices, counts.pop() if counts else 0, path.shape[1], layers, C.addressof(addresses[0]), C.addressof(addresses[1]),
+                                num_indices, num_blocks, path.shape[1], layers, C.addressof(addresses[0]), C.addressof(addresses[1]),
                                 whole("path", path, i32, (B, path.shape[1])), whole("num_accepted", outputs["num_accepted"], i32, (B,)),
                                 whole("next_token", outputs["next_token"], i64, (B,)), 0 if past_out is None else whole("new_past_lens", past_out, i32, (B,)),
                                 self._stream(inputs))

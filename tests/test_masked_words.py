@@ -50,9 +50,9 @@ def test_refusals_without_a_handle(pkg):
 
 def test_kernels_behind_the_masks_are_dependents_and_wait():
     """As those of a causal step: launched as programmatic dependents, waiting for the kernel before them on every path."""
-    for name in ("masked_rows.cu", "tree_accept.cu"):
+    for name in ("masked_rows.cu", "masked_join.cu", "tree_accept.cu"):
         text = re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
-        launched = "".join(re.findall(r"launch_dependent\([^;]*;", text))
+        launched = "".join(re.findall(r"launch_dependent\([^;]*;|launch\([^;]*;", text))
         kernels = re.findall(r"__global__ void (?:__launch_bounds__\([^{;]*?\)\s+)?(\w+)\([^{]*\{(.*?)\n\}", text, flags=re.S)
         assert kernels and "<<<" not in text
         for kernel, body in kernels:
