@@ -5,6 +5,7 @@
 #include <string>
 
 #include "pa_handle.h"
+#include "tensor_map.h"
 
 namespace {
 
@@ -53,8 +54,7 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 
 // Scratch of a masked step.  No part falls where tokens, sequences or block indices grow, so the scratch of the largest step holds every smaller one.
 struct Scratch {
-    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, splits, part_o, part_ml, total;
-    int part_slots;
+    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, part_o, part_ml, total;
 };
 Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     const pa::CacheGeom& g = h->g;
@@ -73,11 +73,12 @@ Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     s.tree_words = take((size_t)tokens * pa::kTreeWords * sizeof(uint32_t));
     s.tree_depth = take((size_t)tokens * sizeof(int));
     s.redo = take((size_t)tokens * g.Hq * sizeof(int));
-    s.part_slots = 2 * h->sm_count;
-    s.items = take(((size_t)tokens * G / pa::kPrefillItemRows + B + s.part_slots) * sizeof(pa::MaskItem));
-    s.splits = take((size_t)s.part_slots * sizeof(pa::MaskSplit));
-    s.part_o = take((size_t)s.part_slots * pa::kPrefillItemRows * g.D * sizeof(float));
-    s.part_ml = take((size_t)s.part_slots * pa::kPrefillItemRows * sizeof(float2));
+    const size_t q_tiles = (size_t)tokens * G / pa::kPrefillItemRows + B, pieces = 2 * (size_t)h->sm_count;
+    s.items = take(q_tiles * sizeof(pa::MaskItem));
+    s.item_prefix = take((q_tiles + 1) * sizeof(long long));
+    s.starts = take(((size_t)h->sm_count + 1) * sizeof(pa::MaskStart));
+    s.part_o = take(pieces * pa::kPrefillItemRows * g.D * sizeof(float));
+    s.part_ml = take(pieces * pa::kPrefillItemRows * sizeof(float2));
     s.total = off;
     return s;
 }
@@ -113,6 +114,7 @@ int validate_masked(const pa_handle* h, const pa_forward_args* a, const pa_mask_
     if (!aligned(a->key_cache) || !aligned(a->value_cache)) return fail(PA_ERR_UNSUPPORTED, "a cache is not 16-byte aligned");
     if (!host && (!aligned(a->query) || !aligned(a->output))) return fail(PA_ERR_UNSUPPORTED, "query or output is not 16-byte aligned");
     if ((long long)a->num_tokens * h->g.Hq > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
+    if ((long long)a->num_blocks * h->g.Hkv > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 blocks of heads in one cache");
     if ((long long)a->num_block_indices * h->g.bs > INT_MAX - 4096) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of context in one call");
     return PA_OK;
 }
@@ -166,9 +168,9 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     m.tree_blocks = mask.tree_parents ? a->num_sequences : 0;
     m.sm_count = h->sm_count;
     m.items = (MaskItem*)(ws + s.items);
-    m.splits = (MaskSplit*)(ws + s.splits);
+    m.item_prefix = (long long*)(ws + s.item_prefix);
+    m.starts = (MaskStart*)(ws + s.starts);
     m.redo = (int*)(ws + s.redo);
-    m.part_slots = s.part_slots;
     // As many tokens as sequences: single tokens, almost always, and no launches for chunks; what of them there is beside sequences without
     // tokens, the device finds out
     m.rows_in_decode = a->num_tokens > 1 && a->num_tokens == a->num_sequences;
@@ -180,9 +182,14 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;
     MASKED_CUDA(launch_decode(k, stream, h->sm_count, &launches));
     if (a->num_tokens > 1 && !m.rows_in_decode) {
-        const long long max_items = (long long)a->num_tokens * G / kPrefillItemRows * h->g.Hkv + (long long)a->num_sequences * h->g.Hkv + s.part_slots;
         if (prefill_tc_supported(h->g)) {
-            MASKED_CUDA(launch_prefill_tc(k, stream, h->sm_count, max_items, &launches));
+            if (h->g.cache != PA_DTYPE_U8) {
+                const long long size[3] = {h->g.D, h->g.bs, (long long)a->num_blocks * h->g.Hkv}, stride[2] = {h->g.D, (long long)h->g.bs * h->g.D};
+                const int box[3] = {64, h->g.bs, 1};
+                if (!make_map(&m.map_k, h->g.cache, a->key_cache, 3, size, stride, box) || !make_map(&m.map_v, h->g.cache, a->value_cache, 3, size, stride, box))
+                    return fail(PA_ERR_CUDA, "a tensor map could not be made");
+            }
+            MASKED_CUDA(launch_prefill_tc(k, stream, h->sm_count, /*max_items=*/h->sm_count, &launches));
             MASKED_CUDA(launch_masked_join(k, stream, &launches));
         } else {
             MASKED_CUDA(launch_masked_rows(k, stream, &launches));

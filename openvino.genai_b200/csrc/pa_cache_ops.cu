@@ -32,95 +32,94 @@ __device__ __forceinline__ int seq_tiles(const KernelArgs& a, int s) {
     return (v.past + 1 + 31) / 32 + a.decode_phantom;
 }
 
-// Masked steps: the pieces of the chunks' q tiles.  A piece is what a CTA of the tensor-core kernel takes at a time, per kv head.  When there are few q
-// tiles they are cut along their context, by the length that lets the SMs end soonest: piece lengths from "two pieces an SM" up to whole
-// q tiles are tried side by side, and a piece costs kPieceCost tiles beside its own (its start, its partial result, the join).
-constexpr int kPieceCost = 6;
-constexpr int kSortTiles = 512;   // q tiles up to which the longest come first
+// Masked steps: the chunks' q tiles, and the CTAs' slices of their tiles.  The lists of all (q tile, kv head) one behind the other, each followed by
+// kMaskPhantom tiles that do not exist, are cut into equal slices, one a CTA of the tensor-core kernel: whatever the mix of long and short lists is, the SMs
+// end together, and at most one list a CTA is cut at either end (masked_join_kernel joins those).
 __device__ void build_mask_items(const KernelArgs& a, int total_p) {
-    __shared__ int sh_nt[kSortTiles];
-    __shared__ unsigned long long sh_best;
-    __shared__ int sh_pieces;
-    const int tid = threadIdx.x, B = a.num_sequences, G = a.g.Hq / a.g.Hkv, Hkv = a.g.Hkv, sms = a.m.sm_count;
-    if (tid == 0) { a.ptile_prefix[B] = total_p; sh_best = ~0ull; sh_pieces = 0; a.plan->total_splits = 0; a.plan->total_redo = 0; a.plan->total_mitems = total_p; }
+    __shared__ long long sh_sum[8];
+    __shared__ long long sh_total;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, B = a.num_sequences, G = a.g.Hq / a.g.Hkv, Hkv = a.g.Hkv, ctas = a.m.sm_count;
+    if (tid == 0) { a.ptile_prefix[B] = total_p; sh_total = 0; }
     __syncthreads();   // the prefix sums are visible to the whole block
-    auto describe = [&](int t, SeqView& sv, int& row0, bool& tree) {
-        int lo = 0, hi = B;   // ptile_prefix[lo] <= t < ptile_prefix[hi]
+    for (int base = 0; base < total_p; base += 256) {
+        const int t = base + tid;
+        int cost = 0;
+        if (t < total_p) {
+            int lo = 0, hi = B;   // ptile_prefix[lo] <= t < ptile_prefix[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.ptile_prefix[mid] <= t) lo = mid; else hi = mid;
+            }
+            SeqView sv;
+            seq_view(a, lo, sv);
+            const int row0 = (t - a.ptile_prefix[lo]) * kPrefillItemRows;
+            const bool tree = has_tree(a, sv.t0, sv.n);
+            const QTile q = q_tile(a.m, sv.past, sv.n, G, row0, tree);
+            const int nt = max(q.cnt[0], q.cnt[1]);
+            a.m.items[t] = MaskItem{sv.t0, sv.n, sv.past, sv.tb, row0, nt, tree, 0};
+            cost = nt + kMaskPhantom;
+        }
+        long long v = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) sh_sum[wid] = v;
+        __syncthreads();
+        long long off = sh_total;
+        for (int w = 0; w < wid; ++w) off += sh_sum[w];
+        if (t < total_p) a.m.item_prefix[t] = off + v - cost;
+        __syncthreads();
+        if (tid == 255) sh_total = off + v;
+        __syncthreads();
+    }
+    if (tid == 0) { a.m.item_prefix[total_p] = sh_total; a.plan->total_mitems = total_p; a.plan->total_redo = 0; }
+    __syncthreads();
+    // Slices of equal cost; uncut, they begin at the nearest list instead.  Cutting costs its CTAs a partial result each and the step a join, some
+    // kMaskCut tiles' time in all, so it is done where the longest uncut slice is longer by more than that.
+    __shared__ int sh_longest;
+    if (tid == 0) sh_longest = 0;
+    __syncthreads();
+    const long long all = sh_total * Hkv;
+    const long long per = max((all + ctas - 1) / ctas, (long long)(kMaskLeast + kMaskPhantom));
+    auto start_of = [&](int w, bool cut, long long& cost_in_front) {
+        MaskStart st{total_p, 0, 0, 0};
+        const long long pos = w * per;
+        cost_in_front = all;
+        if (pos >= all) return st;
+        int lo = 0, hi = total_p;   // item_prefix[lo] * Hkv <= pos < item_prefix[hi] * Hkv
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (a.ptile_prefix[mid] <= t) lo = mid; else hi = mid;
+            if (a.m.item_prefix[mid] * Hkv <= pos) lo = mid; else hi = mid;
         }
-        seq_view(a, lo, sv);
-        row0 = (t - a.ptile_prefix[lo]) * kPrefillItemRows;
-        tree = has_tree(a, sv.t0, sv.n);
-        const QTile q = q_tile(a.m, sv.past, sv.n, G, row0, tree);
-        return max(q.cnt[0], q.cnt[1]);
+        const int cost = (int)(a.m.item_prefix[lo + 1] - a.m.item_prefix[lo]), nt = cost - kMaskPhantom;
+        const long long in = pos - a.m.item_prefix[lo] * Hkv;
+        st.q = lo;
+        st.hk = (int)(in / cost);
+        st.j = (int)(in % cost);
+        cost_in_front = pos - st.j;
+        if (cut ? st.j < kMaskSnap : 2 * st.j < cost) {
+            st.j = 0;
+        } else if (!cut || st.j > nt - kMaskSnap) {
+            st.j = 0;
+            cost_in_front += cost;
+            if (++st.hk == Hkv) { st.hk = 0; ++st.q; }
+        }
+        return st;
     };
-    if (total_p > kSortTiles) {   // in the order of the sequences, whole
-        for (int t = tid; t < total_p; t += 256) {
-            SeqView sv;
-            int row0;
-            bool tree;
-            const int nt = describe(t, sv, row0, tree);
-            a.m.items[t] = MaskItem{sv.t0, sv.n, sv.past, sv.tb, row0, 0, nt, -1, tree, {0, 0, 0}};
-        }
-        return;
-    }
-    int total = 0, most = 0;
-    for (int t = tid; t < total_p; t += 256) {
-        SeqView sv;
-        int row0;
-        bool tree;
-        sh_nt[t] = describe(t, sv, row0, tree);
+    for (int w = tid; w < ctas; w += 256) {
+        long long from, to;
+        start_of(w, false, from);
+        start_of(w + 1, false, to);
+        atomicMax(&sh_longest, (int)min(to - from, 0x7fffffffLL));
     }
     __syncthreads();
-    int len = 0x7fffffff;   // tiles of a piece
-    const long long cap = a.m.part_slots / Hkv;   // pieces there is room for, per kv head
-    if ((long long)total_p * Hkv < 2LL * sms && total_p > 0 && cap > 0) {
-        for (int t = 0; t < total_p; ++t) { total += sh_nt[t]; most = max(most, sh_nt[t]); }   // (every thread: at most 2 * SMs of them)
-        const int least = max(4, (int)(((long long)total * Hkv + 2 * sms - 1) / (2 * sms)));
-        // candidate lengths, evenly spread from `least` to `most`; the last is "whole"
-        const int c = least + (int)((long long)max(most - least, 0) * tid / 255);
-        long long pieces = 0;
-        for (int t = 0; t < total_p; ++t) pieces += (sh_nt[t] + c - 1) / c;
-        const long long waves = (pieces * Hkv + sms - 1) / sms;
-        long long cost;
-        const long long even = max((long long)min(c, most), waves * ((total + pieces - 1) / pieces));   // tiles of the busiest SM
-        if (pieces == total_p) cost = even + waves * (kPieceCost / 2);
-        else cost = pieces <= cap ? even + waves * kPieceCost : (1LL << 30);
-        atomicMin(&sh_best, (unsigned long long)cost << 32 | (unsigned)(0x7fffffff - c));   // of equal ones the longest pieces
-        __syncthreads();
-        len = max(4, 0x7fffffff - (int)(sh_best & 0xffffffffu));
+    const bool cut = sh_longest > per + kMaskCut;
+    for (int w = tid; w <= ctas; w += 256) {
+        long long unused;
+        a.m.starts[w] = start_of(w, cut, unused);
     }
-    int my_pieces = 0;
-    for (int t = tid; t < total_p; t += 256) {
-        // rank by length, and the pieces in front
-        const int mine = sh_nt[t];
-        int first = 0, split_rank = 0, split_first = 0;
-        for (int u = 0; u < total_p; ++u) {
-            const int nt = sh_nt[u];
-            if (nt > mine || (nt == mine && u < t)) {
-                const int k = (nt - 1) / len + 1;
-                first += k;
-                if (k > 1) { ++split_rank; split_first += k; }
-            }
-        }
-        SeqView sv;
-        int row0;
-        bool tree;
-        describe(t, sv, row0, tree);
-        const int k = (mine - 1) / len + 1;
-        for (int i = 0; i < k; ++i)
-            a.m.items[first + i] = MaskItem{sv.t0, sv.n, sv.past, sv.tb, row0, i * len, min(mine, (i + 1) * len), k > 1 ? (split_first + i) * Hkv : -1, tree, {0, 0, 0}};
-        if (k > 1) {
-            a.m.splits[split_rank] = MaskSplit{sv.t0, sv.n, sv.past, row0, split_first * Hkv, k, len, tree};
-            atomicAdd(&a.plan->total_splits, 1);
-        }
-        my_pieces += k;
-    }
-    atomicAdd(&sh_pieces, my_pieces);
-    __syncthreads();
-    if (tid == 0) a.plan->total_mitems = sh_pieces;
 }
 
 // Masked steps: ancestors and depths of one sequence's tree, one block of 256 threads, a token each.  Parents are in front of their children, so a

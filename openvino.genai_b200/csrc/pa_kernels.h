@@ -1,6 +1,7 @@
 // Internal launch interface between the C ABI (pa_api.cu) and the kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,8 +18,7 @@ struct PlanHeader {
     int total_ptiles;  // kPrefillItemRows-row q tiles of all prefill chunks (per kv head)
     int next_pitem;    // work counter of the prefill kernel: next (q tile, kv head) item to hand out
     int pitems_sorted; // 1: pitem_order lists the q tiles by decreasing context length
-    int total_mitems;  // masked steps: pieces of q tiles (per kv head)
-    int total_splits;  // masked steps: q tiles that are cut into several pieces
+    int total_mitems;  // masked steps: q tiles
     int total_redo;    // masked steps: rows that are computed again
 };
 
@@ -70,22 +70,23 @@ constexpr int kTreeMax = 256;              // PA_TREE_MAX_TOKENS
 constexpr int kTreeWords = kTreeMax / 32;
 constexpr int kTreeNone = -2;              // PA_TREE_NONE
 
-// A piece of a q tile's work: tiles [j0, j1) of the q tile's list of 64-token context tiles.
+// A q tile of a masked step (256 rows of a chunk, per kv head) and its list of 64-token context tiles.
 struct __align__(16) MaskItem {
     int t0, n_new, past, tb;   // of the sequence: first row, new tokens, cached tokens, begin of its block table
     int row0;                  // first (token, head) pair of the q tile
-    int j0, j1;
-    int part;                  // partial result of kv head 0, -1: the q tile is in one piece
+    int nt;                    // tiles of the list
     int tree;
-    int pad[3];
+    int pad;
 };
-// A q tile in several pieces, whose partial results are joined.
-struct __align__(16) MaskSplit {
-    int t0, n_new, past, row0;
-    int first_part;            // partial result of kv head 0 of the first piece; the next piece's is Hkv further
-    int pieces, len;           // tiles of a piece
-    int tree;
+// Where a CTA's slice of all (q tile, kv head, tile) begins; it ends where the next one's begins.
+struct __align__(16) MaskStart {
+    int q, hk, j;
+    int pad;
 };
+constexpr int kMaskPhantom = 4;   // what a q tile costs beside its tiles, in tiles: its rows' way in and out
+constexpr int kMaskLeast = 4;     // tiles that a CTA is given at least
+constexpr int kMaskCut = 14;      // what cutting lists between CTAs costs, in tiles
+constexpr int kMaskSnap = 2;      // a slice does not begin so near to either end of a q tile's list
 struct MaskParams {
     int on;                    // 0: causal rows, nothing else below is read
     int window, sinks;
@@ -95,12 +96,13 @@ struct MaskParams {
     int tree_blocks;           // blocks of the cache write that make them: one per sequence, 0 without trees
     int sm_count;
     MaskItem* items;
-    MaskSplit* splits;         // [2 * sm_count]
+    long long* item_prefix;    // [q tiles + 1] tiles and phantoms in front of a q tile, of one kv head
+    MaskStart* starts;         // [sm_count + 1]
     int* redo;                 // [num_tokens * Hq] rows (token * Hq + head) that are not finite and are computed again, one by one
     int rows_in_decode;        // the step has no launch for chunks: the decode kernel's warps see to those that it holds all the same
-    int part_slots;            // partial results there is room for
-    float* part_o;             // [part_slots][256][D]
-    float2* part_ml;           // [part_slots][256] row maximum (base 2, scaled) and sum
+    float* part_o;             // [2 * sm_count][256][D] partial results: 2 w of CTA w's first list, if that began in front of it, 2 w + 1 of its last one
+    float2* part_ml;           // [2 * sm_count][256] row maximum (base 2, scaled) and sum
+    alignas(64) CUtensorMap map_k, map_v;   // 16-bit caches: [num_blocks * Hkv][block_size][D], boxes of 64 elements of a block's tokens
 };
 
 // Everything a kernel needs, passed by value.  All pointers are device memory.

@@ -34,12 +34,14 @@
 // register file with setmaxnreg once their roles start: 160 registers per softmax thread, 104 per converter thread, 88 for
 // the rest (one warp of each warpgroup shares a scheduler's 16 K registers).
 // Every wait is bounded; a wait that runs out raises a flag that all roles poll.
-// Masked steps (MK; include/masked_b200.h): an item is a piece of a q tile's list of context tiles (build_mask_items); a tile of which a row
+// Masked steps (MK; include/masked_b200.h): a CTA has a slice of the q tiles' lists of context tiles (build_mask_items) and no counter; a tile of which a row
 // sees a part takes that part from a word of bits; tokens that no row of the item sees go in as zeros and their blocks are not looked up; a piece
-// leaves its rows' sums, maxima and unnormalised results to masked_join_kernel.
+// leaves its rows' sums, maxima and unnormalised results to masked_join_kernel.  Few rows (one half's worth) are worked on by both halves, a tile each in
+// turn.  The u8 cache has a warp for each half's products here too, S of a tile ahead of the P.V before it.
 // Tensor-bound for long contexts: 4 * Hq * D flops per (new token, context token) pair.
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "masked.cuh"
 #include "pa_common.cuh"
@@ -61,6 +63,15 @@ constexpr float kLazy = 4.f;   // log2 of the growth of a row maximum that force
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 
+#ifndef PA_X_TWO
+#define PA_X_TWO MK
+#endif
+#ifndef PA_X_NEWCONV
+#define PA_X_NEWCONV 1
+#endif
+#ifndef PA_X_CHAIN
+#define PA_X_CHAIN 1
+#endif
 constexpr int kSoftmaxWarps = 8, kConvWarps = 4;
 constexpr int kWarpMma = kSoftmaxWarps + kConvWarps, kWarpLoad = kWarpMma + 1, kWarpMma2 = kWarpMma + 2;   // the second mma warp: 16-bit caches
 constexpr int kThreads = 512;   // four warpgroups: softmax A, softmax B, converter / copy warps, {mma, loader, second mma (16-bit caches) or idle, idle}
@@ -85,13 +96,16 @@ struct Item {
     const int32_t* table;
 };
 
-// A masked step's item: tiles [j0, j0 + ntiles) of the q tile's list.
+// A masked step's item: tiles [j0, j0 + ntiles) of the q tile's list.  Where the q tile has rows for half A only, half B takes them too (`dup`): the
+// halves take the tiles in turn, and half A joins both results.
 struct MaskedItem : Item {
     VisTiles v;
     int lo;              // positions below it, beyond the sinks, are seen by no row
     int j0;
-    int part;            // partial result, -1: the q tile is in one piece
-    int tree;
+    int part;            // partial result, -1: the list is in one piece
+    int tree, dup;
+    __device__ __forceinline__ bool uses(int x, int j) const { return dup ? (j & 1) == x : j < nt[x]; }
+    __device__ __forceinline__ int own(int j) const { return dup ? j >> 1 : j; }   // tile j among those of its half
 };
 template <bool MK> struct ItemOf { using type = Item; };
 template <> struct ItemOf<true> { using type = MaskedItem; };
@@ -117,6 +131,7 @@ struct PrefillSmem<BS, PA_DTYPE_U8, D, MK> {
     alignas(128) uint8_t raw_v[kStages][NREC * RSTRIDE];
     alignas(128) uint8_t out_stage[kSoftmaxWarps][32 * 128];   // 128 bytes of each of a warp's rows on their way to global memory
     alignas(16) uint2 v_tab[kConvWarps][kKv / 2];  // per converter warp: (scale, -1024 * scale) f16 pairs of two tokens
+    alignas(16) uint2 tok_scale[MK ? kConvWarps : 1][MK ? kKv : 1];   // masked, per converter warp: (scale, -1024 * scale) of a token, each as a pair of equal f16
     alignas(8) uint64_t raw_full[kStages];   // loader -> converter (transaction bytes)
     alignas(8) uint64_t raw_free[kStages];   // converter -> loader
     alignas(8) uint64_t k_full[kStages];     // converter -> mma
@@ -132,6 +147,7 @@ struct PrefillSmem<BS, PA_DTYPE_U8, D, MK> {
     alignas(8) uint64_t item_free[kItemSlots];   // every other warp -> loader: the slot has been read
     int item_ring[kItemSlots];
     typename ItemOf<MK>::type item_desc[kItemSlots];   // the loader locates an item once for every role
+    alignas(8) uint64_t join_full, join_free;   // masked: half B -> half A: its rows' maxima and sums lie in its warps' out_stage; A -> B: it has read B's results
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -153,8 +169,9 @@ struct PrefillSmem16 {
     alignas(1024) uint8_t vt[NST][kKv * D * 2];   // the same image read as an MN-major operand: atoms of 64 dims, 8-token groups 1024 bytes apart
     alignas(128) uint8_t out_stage[kSoftmaxWarps][32 * 128];
     alignas(128) uint8_t ones[16 * 16 * 2];           // unswizzled K-major [16 rows][16 tokens]: row 0 all ones
-    alignas(8) uint64_t k_full[NST];     // copy warps -> mma
-    alignas(8) uint64_t v_full[NST];
+    alignas(8) uint64_t k_full[NST];     // copy warps -> mma (masked: the loader's copies)
+    alignas(8) uint64_t v_full[NST];     // (masked: the warps that clear rows, of tiles that are not seen as a whole)
+    alignas(8) uint64_t v_land[NST];     // masked: the loader's copies of values
     alignas(8) uint64_t k_free[NST];     // mma (commit) -> copy warps
     alignas(8) uint64_t v_free[NST];
     alignas(8) uint64_t q_full[2];
@@ -166,6 +183,7 @@ struct PrefillSmem16 {
     alignas(8) uint64_t item_free[kItemSlots];
     int item_ring[kItemSlots];
     typename ItemOf<MK>::type item_desc[kItemSlots];   // the loader locates an item once for every role
+    alignas(8) uint64_t join_full, join_free;   // masked: half B -> half A: its rows' maxima and sums lie in its warps' out_stage; A -> B: it has read B's results
     uint32_t tmem_base;
     volatile int abort;
 };
@@ -182,6 +200,19 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// (a, b) * s + t, two at a time
+__device__ __forceinline__ float2 fma_pair(float a, float b, float s, float t) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a), "f"(b), "f"(s), "f"(t));
+    return r;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
 }
 __device__ __forceinline__ uint32_t ex2_h2(uint32_t x) {
     uint32_t y;
@@ -247,6 +278,17 @@ __device__ __forceinline__ void scale16(uint4& lo4, uint4& hi4, __half sc) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+// (1024 + byte) -> byte * scale for eight values of one scale; sc = (scale, -1024 * scale) as f16 pairs.  `slow`: the scale may be 32 or more (scale16).
+__device__ __forceinline__ void scale_pair(uint4& w4, uint2 sc, bool slow) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&w4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE400E400u), sc.x) : hfma2_bits(w[k], sc.x, sc.y);
+}
 // One arrival for the whole warp, after every lane's preceding writes.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
@@ -288,28 +330,43 @@ __device__ __forceinline__ Item locate_item(const KernelArgs& a, int item, int G
     return it;
 }
 
-__device__ __forceinline__ MaskedItem locate_masked(const KernelArgs& a, int item, int G, int Hkv) {
-    const int4* src = reinterpret_cast<const int4*>(a.m.items + item / Hkv);
-    const int4 x = __ldcg(src), y = __ldcg(src + 1), z = __ldcg(src + 2);
-    MaskedItem it;
-    it.s = 0;
-    it.hk = item % Hkv;
-    it.t0 = x.x; it.n_new = x.y; it.past = x.z;
-    it.table = a.block_indices + x.w;
-    it.row0 = y.x; it.j0 = y.y;
-    it.part = y.w < 0 ? -1 : y.w + it.hk;
-    it.tree = z.x;
-    const QTile q = q_tile(a.m, it.past, it.n_new, G, it.row0, it.tree);
-    it.v = q.v;
-    it.lo = q.lo;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        it.ctx_hi[h] = q.ctx_hi[h];
-        it.nt[h] = max(0, min(q.cnt[h], y.z) - it.j0);
+// Walks CTA w's slice: the next piece of a list, false when there is none.
+struct MaskWalk {
+    MaskStart at, end;
+    int Hkv, w;
+    __device__ __forceinline__ MaskWalk(const KernelArgs& a, int cta) : Hkv(a.g.Hkv), w(cta) {
+        const int4 s = __ldcg(reinterpret_cast<const int4*>(a.m.starts + cta)), e = __ldcg(reinterpret_cast<const int4*>(a.m.starts + cta + 1));
+        at = MaskStart{s.x, s.y, s.z, 0};
+        end = MaskStart{e.x, e.y, e.z, 0};
     }
-    it.ntiles = max(it.nt[0], it.nt[1]);
-    return it;
-}
+    template <bool DUP>
+    __device__ __forceinline__ bool next(const KernelArgs& a, int G, MaskedItem& it) {
+        const bool last = at.q == end.q && at.hk == end.hk;
+        if (at.q > end.q || (at.q == end.q && (at.hk > end.hk || (last && at.j >= end.j)))) return false;
+        const int4* src = reinterpret_cast<const int4*>(a.m.items + at.q);
+        const int4 x = __ldcg(src), y = __ldcg(src + 1);
+        it.s = 0;
+        it.hk = at.hk;
+        it.t0 = x.x; it.n_new = x.y; it.past = x.z;
+        it.table = a.block_indices + x.w;
+        it.row0 = y.x; it.j0 = at.j;
+        it.tree = y.z;
+        const int end_j = last ? end.j : y.y, len = end_j - at.j;
+        it.part = at.j > 0 ? 2 * w : end_j < y.y ? 2 * w + 1 : -1;
+        const QTile q = q_tile(a.m, it.past, it.n_new, G, it.row0, it.tree);
+        it.v = q.v;
+        it.lo = q.lo;
+        it.dup = DUP && q.cnt[1] == 0;
+        it.ctx_hi[0] = q.ctx_hi[0];
+        it.ctx_hi[1] = it.dup ? q.ctx_hi[0] : q.ctx_hi[1];
+        it.nt[0] = it.dup ? (len + 1) / 2 : max(0, min(q.cnt[0], end_j) - at.j);
+        it.nt[1] = it.dup ? len / 2 : max(0, min(q.cnt[1], end_j) - at.j);
+        it.ntiles = it.dup ? len : max(it.nt[0], it.nt[1]);
+        at.j = 0;
+        if (++at.hk == Hkv) { at.hk = 0; ++at.q; }
+        return true;
+    }
+};
 
 #ifdef PA_PREFILL_PROF
 // role (0, 1 softmax A, B; 2 converter; 3 mma; 4 loader; 5 second mma warp), event, tile 64..67 of CTA 0; 0: not met.  (In global
@@ -318,13 +375,25 @@ constexpr int kTraceRoles = 6;
 __device__ long long trace[kTraceRoles][8][4];
 #endif
 
+template <bool MK>
+__device__ __forceinline__ auto make_walk(const KernelArgs& a) {
+    if constexpr (MK) return MaskWalk(a, blockIdx.x);
+    else return 0;
+}
+
 template <int BS, int CT, int D, bool MK>
-__global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_constant__ KernelArgs a) {
     using Smem = PrefillSmem<BS, CT, D, MK>;
     using It = typename ItemOf<MK>::type;
     constexpr bool U8 = CT == PA_DTYPE_U8, BF = CT == PA_DTYPE_BF16;
     constexpr int kD = D, kNo = Smem::NO, kTmemP = 2 * kKv + 2 * kNo, NST = Smem::NST;
-    constexpr int kPCols = BF ? kKv : kKv / 2;   // tensor-memory columns of one half's P: f16, or bf16 high + low pieces
+    constexpr bool PL = BF && !MK;               // P as two bf16 pieces.  (Masked steps: one, as in the decode kernel: P's 2^-9 beside the output's own, 2.3e-3 of the
+                                                 // result in all instead of 1.7e-3, for a third of the products)
+    // Masked: code that runs once an item stays in loops.  Straight through it is thousands of instructions that come from L2 every time: an epilogue
+    // took 10 k cycles.
+    constexpr int kRolled = MK ? 1 : 16;
+    constexpr bool TwoMma = !U8 || PA_X_TWO;     // a warp issues the products of each half
+    constexpr int kPCols = PL ? kKv : kKv / 2;   // tensor-memory columns of one half's P: f16, or bf16 high + low pieces
     constexpr int kFmt = BF ? 1 : 0;
     static_assert(!U8 || NST == 2, "the converter and the loader of the u8 variant index two stages");
     static_assert(kTmemP + 2 * kPCols <= kTmemCols, "S, O and P of both halves fit the tensor memory");
@@ -334,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
     const int G = a.g.Hq / a.g.Hkv;
     const int Hkv = a.g.Hkv;
     grid_wait();
-    const int total_items = (MK ? a.plan->total_mitems : a.plan->total_ptiles) * Hkv;
+    const int total_items = MK ? 0 : a.plan->total_ptiles * Hkv;
     const float qscale = (a.scale != 0.f ? a.scale : rsqrtf((float)kD)) * kLog2eP;
 
     if (tid == 0) {
@@ -344,10 +413,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 mbar_init(&sm.raw_full[i], 1);
                 mbar_init(&sm.raw_free[i], kConvWarps);
             }
-            mbar_init(&sm.k_full[i], kConvWarps);
-            mbar_init(&sm.v_full[i], kConvWarps);
-            mbar_init(&sm.k_free[i], U8 ? 1 : 2);   // one arrival per mma warp
-            mbar_init(&sm.v_free[i], U8 ? 1 : 2);
+            if constexpr (!U8 && MK) {
+                mbar_init(&sm.k_full[i], 1);
+                mbar_init(&sm.v_full[i], kConvWarps);
+                mbar_init(&sm.v_land[i], 1);
+            } else if constexpr (U8 && MK && PA_X_NEWCONV) {
+                mbar_init(&sm.k_full[i], kConvWarps / 2);   // half of the converter's warps each
+                mbar_init(&sm.v_full[i], kConvWarps / 2);
+            } else {
+                mbar_init(&sm.k_full[i], kConvWarps);
+                mbar_init(&sm.v_full[i], kConvWarps);
+            }
+            mbar_init(&sm.k_free[i], TwoMma ? 2 : 1);   // one arrival per mma warp
+            mbar_init(&sm.v_free[i], TwoMma ? 2 : 1);
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -360,7 +438,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
 #pragma unroll
         for (int i = 0; i < kItemSlots; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_free[i], kWarpMma + (U8 ? 1 : 2));
+            mbar_init(&sm.item_free[i], kWarpMma + (TwoMma ? 2 : 1));
+        }
+        if constexpr (MK) {
+            mbar_init(&sm.join_full, kRows / 32);
+            mbar_init(&sm.join_free, kRows / 32);
         }
         mbar_fence_init();
         sm.abort = 0;
@@ -385,6 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
     tc05::fence_after_thread_sync();
     const uint32_t tmem = sm.tmem_base;
 
+    [[maybe_unused]] uint32_t begun = 0, begun_v = 0;   // masked: tiles whose copies the loader has begun; whose values'
     // A wait that runs out raises sm.abort; every waiter polls the flag, so all roles unwind.
     // `cat` names the wait for the optional cycle accounting (-DPA_PREFILL_PROF).
 #ifdef PA_PREFILL_PROF
@@ -429,13 +512,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
     };
 
     // first context position of an item's j-th tile; whether any row of the item sees a position
-    auto tile_pos = [&](const It& it, int j) -> int {
+    auto tile_pos = [&](const It& it, int j) -> int {   // (j counts the item's tiles, those of both halves)
         if constexpr (MK) return it.v.tile(it.j0 + j) * kKv;
         else return j * kKv;
     };
     auto seen = [&](const It& it, int ctx_hi, int pos) -> bool {
         if constexpr (MK) return pos < ctx_hi && (pos < a.m.sinks || pos >= it.lo);
         else return pos < ctx_hi;
+    };
+
+    // whether every token of a tile is seen by some row of the item
+    [[maybe_unused]] auto whole_tile = [&](const It& it, int ctx_hi, int pos0) -> bool {
+        if constexpr (MK) return pos0 + kKv <= ctx_hi && (pos0 >= it.lo || pos0 + kKv <= a.m.sinks);
+        else return false;
     };
 
     if (warp >= kWarpMma) reg_dec<PA_TC_REG_MISC>();   // the fourth warpgroup: mma, loader, second mma; what is left over keeps it whole
@@ -449,6 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         const uint32_t tmem_p = tmem + kTmemP + kPCols * X + lane_base;
         uint32_t n = 0;   // tiles of this half so far, over all items
         uint32_t ik = 0;
+        uint32_t joins = 0;        // masked: items whose results both halves hold, so far
+        bool joins_open = false;   // half B: the last of them has not been read yet
         It it;
         // This thread's row of the item in work; the next item's is staged before this one's epilogue.
         struct Row {
@@ -472,27 +563,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         // completed, so the tile is free.  16-bit rows: kD / 8 lanes take one row in 16-byte chunks, all loads of the warp's 32
         // rows in flight together (64 registers, free between items; cp.async where the row goes in as it is).  One thread per
         // row touched 32 lines with every load and, behind a branch on the type, had one load in flight: 10 k cycles an item.
-        auto stage_q = [&]() {
+        [[maybe_unused]] auto stage_q = [&]() {
             constexpr int CH = kD / 8, RP = 32 / CH;   // chunks of a row, rows per pass; CH passes
             const int flat = it.row0 + X * kRows + r;
             const int tok = flat / G, hq = it.hk * G + flat % G;
             row.live = tok < it.n_new;
-            if constexpr (MK) {
-                row.tok = -1;
-                row.ctx = 0x7fffffff; row.lo = 0;   // (a row that is none sees zeros)
-                if (row.live) {
-                    if (it.tree) {
-                        row.tok = it.t0 + tok;
-                        row.ctx = it.past;
-                        row.lo = window_lo(a.m, it.past + __ldcg(a.m.tree_depth + row.tok) + 1);
-                    } else {
-                        row.ctx = it.past + tok + 1;
-                        row.lo = window_lo(a.m, row.ctx);
-                    }
-                }
-            } else {
-                row.ctx = row.live ? it.past + tok + 1 : it.ctx_hi[X];
-            }
+            row.ctx = row.live ? it.past + tok + 1 : it.ctx_hi[X];
             row.off = ((long long)(it.t0 + (row.live ? tok : 0)) * a.g.Hq + hq);
             row.qs = qscale;
             const int wrow = r & ~31;                                  // the warp's first row
@@ -639,9 +715,184 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             tc05::fence_proxy_async_smem();
             warp_arrive(&sm.q_full[X]);
         };
+        // Masked, 16-bit activations: the rows go into the operand tile as they are, asynchronously (stage_begin), and are looked through and converted
+        // where they lie (stage_end), in short loops; between the two lies the epilogue of the item before.
+        [[maybe_unused]] auto place_row = [&] {
+            int flat = it.row0 + X * kRows + r;
+            if constexpr (MK) flat -= it.dup ? X * kRows : 0;
+            const int tok = flat / G, hq = it.hk * G + flat % G;
+            row.live = tok < it.n_new;
+            row.off = (long long)(it.t0 + (row.live ? tok : 0)) * a.g.Hq + hq;
+            row.qs = qscale;
+            if constexpr (MK) {
+                row.tok = -1;
+                row.ctx = 0x7fffffff; row.lo = 0;   // (a row that is none sees zeros)
+                if (row.live && it.tree) {
+                    row.tok = it.t0 + tok;
+                    row.ctx = it.past;
+                    row.lo = window_lo(a.m, it.past + __ldcg(a.m.tree_depth + row.tok) + 1);
+                } else if (row.live) {
+                    row.ctx = it.past + tok + 1;
+                    row.lo = window_lo(a.m, row.ctx);
+                }
+            }
+        };
+        constexpr int CH = kD / 8, RP = 32 / CH;   // 16-byte chunks of a row, rows of a warp side by side
+        [[maybe_unused]] auto stage_begin = [&] {
+            place_row();
+            if (a.g.act == PA_DTYPE_F32) return;
+            const int own = row.live ? (int)row.off : -1, ch = lane % CH, sub = lane / CH;
+            uint8_t* const dst = sq + (ch / 8) * (kRows * 128);
+            const uint4* const src = reinterpret_cast<const uint4*>(a.query) + ch;
+#pragma unroll 4
+            for (int i = 0; i < CH; ++i) {
+                const int o = __shfl_sync(0xffffffffu, own, RP * i + sub);
+                cp_async16_zfill(dst + sw128((r & ~31) + RP * i + sub, ch & 7), src + (long long)max(o, 0) * CH, o >= 0 ? 16u : 0u);
+            }
+            cp_async_commit();
+        };
+        [[maybe_unused]] auto stage_end = [&] {
+            const int ch = lane % CH, sub = lane / CH, wrow = r & ~31;
+            uint8_t* const dst = sq + (ch / 8) * (kRows * 128);
+            float qsum = 0.f;
+            // the row whose sum this thread ends up with: of turn ch % (CH / 4), the one that its upper two bits choose
+            int sum_row = wrow + RP * (4 * (ch & (CH / 4 - 1)) + (ch >> (CH == 16 ? 2 : 1))) + sub;
+            auto sum8 = [](const uint4& w) {      // of the f16 values the tensor core will see
+                const __half2* h = reinterpret_cast<const __half2*>(&w);
+                float s4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s4[e] = __low2float(h[e]) + __high2float(h[e]);
+                return (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            };
+            auto pack8 = [](const float (&v)[8], float mul) {
+                return make_uint4(pack_h2(v[0] * mul, v[1] * mul), pack_h2(v[2] * mul, v[3] * mul), pack_h2(v[4] * mul, v[5] * mul), pack_h2(v[6] * mul, v[7] * mul));
+            };
+            // large queries: an exact power of two that keeps row and sum inside the f16 range, taken back out by the row's softmax scale (as stage_q says)
+            auto prescale = [](float amax) {
+                float mul = 1.f;
+                if (amax > 256.f && amax < INFINITY) {
+                    int ex;
+                    frexpf(amax, &ex);
+                    mul = ldexpf(1.f, 8 - ex);
+                }
+                return mul;
+            };
+            if (a.g.act != PA_DTYPE_F32) {
+                cp_async_wait<0>();
+                __syncwarp();
+                if constexpr (!BF) {
+                    const bool f16 = a.g.act == PA_DTYPE_F16;
+                    auto values = [&](const uint4& q, float (&v)[8]) {
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
+                                                 : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+                            v[2 * e] = f.x; v[2 * e + 1] = f.y;
+                        }
+                    };
+                    const uint32_t limit = f16 ? 0x5C00u : 0x4380u;   // 256, by bit pattern
+                    uint32_t top = 0u;
+#pragma unroll 4
+                    for (int i = 0; i < CH; ++i) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(dst + sw128(wrow + RP * i + sub, ch & 7));
+                        top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+                    }
+                    const bool large = __any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > limit);
+                    if (U8 || !f16 || large) {
+                        // four rows a turn: converted where they lie, and their sums over the CH lanes of a row together: two steps that halve the rows a
+                        // lane carries, then those over what is left of the lanes (one row after the other it was four steps each, 5 - 9 k cycles)
+                        static_assert(CH % 4 == 0, "whole turns");
+#pragma unroll 1
+                        for (int b = 0; b < CH / 4; ++b) {
+                            uint4* at[4];
+                            uint4 w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                at[i] = reinterpret_cast<uint4*>(dst + sw128(wrow + RP * (4 * b + i) + sub, ch & 7));
+                                w[i] = *at[i];
+                            }
+                            if (!f16 || large) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    float v[8], mul = 1.f;
+                                    values(w[i], v);
+                                    if (large) {
+                                        float m = 0.f;
+#pragma unroll
+                                        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+#pragma unroll
+                                        for (int o = CH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                                        mul = prescale(m);
+                                        const float mine = __shfl_sync(0xffffffffu, mul, (lane % RP) * CH);   // row RP (4 b + i) + lane % RP
+                                        if (lane / RP == 4 * b + i) row.qs = qscale / mine;
+                                    }
+                                    w[i] = pack8(v, mul);
+                                    *at[i] = w[i];
+                                }
+                            }
+                            if constexpr (U8) {
+                                float t[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) t[i] = sum8(w[i]);
+                                const bool hi = (ch & (CH / 2)) != 0, hi2 = (ch & (CH / 4)) != 0;
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const float give = hi ? t[i] : t[i + 2], keep = hi ? t[i + 2] : t[i];
+                                    t[i] = keep + __shfl_xor_sync(0xffffffffu, give, CH / 2);
+                                }
+                                float s = (hi2 ? t[1] : t[0]) + __shfl_xor_sync(0xffffffffu, hi2 ? t[0] : t[1], CH / 4);
+#pragma unroll
+                                for (int o = CH / 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                                if ((ch & (CH / 4 - 1)) == b) qsum = s;
+                            }
+                        }
+                    }
+                }
+            } else {
+                sum_row = r;
+                float amax = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < CH; ++c) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+                    if (row.live) load_act_vec<8>(a.query, row.off * kD + 8 * c, a.g.act, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
+                }
+                const float mul = prescale(amax);
+                row.qs = qscale / mul;
+#pragma unroll 4
+                for (int c = 0; c < CH; ++c) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+                    if (row.live) load_act_vec<8>(a.query, row.off * kD + 8 * c, a.g.act, v);
+                    const uint4 w = pack8(v, mul);
+                    *reinterpret_cast<uint4*>(sq + (c / 8) * (kRows * 128) + sw128(r, c % 8)) = w;
+                    if constexpr (U8) qsum += sum8(w);
+                }
+            }
+            if constexpr (U8) {
+                const __half qh = f2h(qsum), ql = f2h(qsum - __half2float(qh));
+                const __half zero = __ushort_as_half(0);
+                *reinterpret_cast<uint4*>(sm.qx[X] + plain16(sum_row, 0)) = make_uint4(h2_bits(qh, qh), h2_bits(qh, ql), h2_bits(ql, zero), 0u);
+                *reinterpret_cast<uint4*>(sm.qx[X] + plain16(sum_row, 1)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            tc05::fence_proxy_async_smem();
+            warp_arrive(&sm.q_full[X]);
+        };
         int have = next_item();
         if (have < 0) goto done;
-        if (have) stage_q();
+        if (have) {
+            if constexpr (MK) {
+                stage_begin();
+                stage_end();
+            } else {
+                stage_q();
+            }
+        }
         while (have) {
             const int nt = it.nt[X], my_ctx = row.ctx;
             const float qs = row.qs;
@@ -651,7 +902,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             float m_run = -INFINITY;   // running maximum of q.k' (before the softmax scale)
             float l_own = 0.f;         // bf16 variant: the row's own sum of probabilities
             for (int j = 0; j < nt; ++j, ++n) {
-                const int col0 = tile_pos(it, j);
+                int col0;
+                if constexpr (MK) col0 = tile_pos(it, it.dup ? 2 * j + X : j);
+                else col0 = tile_pos(it, j);
                 if (!wait_warp(&sm.s_full[X], n & 1, 0)) goto done;
                 if ((warp & 3) == 0) PA_TRACE(X, 0, n);
                 tc05::fence_after_thread_sync();
@@ -664,7 +917,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
 #pragma unroll
                     for (int c = 0; c < 32; ++c) { sv[c] = __uint_as_float(s0[c]); sv[32 + c] = __uint_as_float(s1[c]); }
                 }
-                if constexpr (!U8) {
+                if constexpr (TwoMma) {
                     tc05::fence_before_thread_sync();
                     warp_arrive(&sm.s_read[X]);
                 }
@@ -686,8 +939,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     for (int c = 0; c < kKv; ++c) sv[c] = c < nvis ? sv[c] : -INFINITY;
                 }
                 float mx = -INFINITY;
+                if constexpr (MK && PA_X_CHAIN) {   // four chains: one of 32 links is as long as the exponentials
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < kKv; c += 2) mx = max3(mx, sv[c], sv[c + 1]);
+                    for (int c = 0; c < kKv; c += 2) m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], sv[c], sv[c + 1]);
+                    mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kKv; c += 2) mx = max3(mx, sv[c], sv[c + 1]);
+                }
                 float alpha = 1.f;
                 bool rescale = false;
                 if (j == 0) {
@@ -700,34 +960,51 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 if constexpr (BF) l_own *= alpha;
                 // P = 2^(qs * (s - m)) in f16 pairs: the exponent is rounded to f16 first, which costs
                 // at most 2^-12 of the exponent's magnitude in relative error of p
+                [[maybe_unused]] float2 l2 = make_float2(0.f, 0.f);
                 const float mq = MK && m_run == -INFINITY ? 0.f : m_run * qs;   // (nothing seen yet: every p is 0)
                 uint32_t pw[kKv / 2];
-                uint32_t pl[BF ? kKv / 2 : 1];   // bf16 variant: the low pieces, p = high + low up to 2^-17 p
+                uint32_t pl[PL ? kKv / 2 : 1];   // bf16 variant: the low pieces, p = high + low up to 2^-17 p
 #pragma unroll
                 for (int c = 0; c < kKv; c += 2) {
                     // the packed f16 exponential is good to 2^-9.9 relative: inside the u8 cache's error bound, not inside the
                     // f16 cache's, whose P goes through the f32 exponential and is rounded once
-                    if constexpr (U8) {
+                    if constexpr (MK) {   // the same, with the scaling and the row's sum two at a time
+                        const float2 x = fma_pair(sv[c], sv[c + 1], qs, -mq);
+                        if constexpr (U8) {
+                            pw[c >> 1] = ex2_h2(pack_h2(x.x, x.y));
+                        } else {
+                            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                            if constexpr (BF) l2 = add_pair(l2, p);
+                            pw[c >> 1] = BF ? pack_bf2(p.x, p.y) : pack_h2(p.x, p.y);
+                        }
+                    } else if constexpr (U8) {
                         pw[c >> 1] = ex2_h2(pack_h2(fmaf(sv[c], qs, -mq), fmaf(sv[c + 1], qs, -mq)));
                     } else if constexpr (BF) {
                         const float p0 = ex2(fmaf(sv[c], qs, -mq)), p1 = ex2(fmaf(sv[c + 1], qs, -mq));
                         l_own += p0 + p1;
                         const uint32_t hi = pack_bf2(p0, p1);
                         pw[c >> 1] = hi;
-                        pl[c >> 1] = pack_bf2(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+                        if constexpr (PL) pl[c >> 1] = pack_bf2(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
                     } else {
                         pw[c >> 1] = pack_h2(ex2(fmaf(sv[c], qs, -mq)), ex2(fmaf(sv[c + 1], qs, -mq)));
                     }
                 }
+                if constexpr (MK && BF) l_own += l2.x + l2.y;
                 // P.V of the previous tile of this half still reads the P tile and writes O
                 if ((warp & 3) == 0) PA_TRACE(X, 2, n);
                 if (n > 0) {
                     if (!wait_warp(&sm.o_done[X], (n - 1) & 1, 1)) goto done;
                     tc05::fence_after_thread_sync();
                 }
+                if constexpr (MK) {   // half A may still be reading the last item's results of half B
+                    if (joins_open) {
+                        if (!wait_warp(&sm.join_free, (joins - 1) & 1, 1)) goto done;
+                        joins_open = false;
+                    }
+                }
                 if ((warp & 3) == 0) PA_TRACE(X, 3, n);
                 if (rescale) {
-#pragma unroll
+#pragma unroll kRolled
                     for (int q4 = 0; q4 < kD / 32; ++q4) {
                         uint32_t t[32];
                         tc05::ld_32x32b_x32(tmem_o + 32 * q4, t);
@@ -747,7 +1024,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     tc05::wait_st();
                 }
                 tc05::st_32x32b_x32(tmem_p, pw);   // row r of the A operand: lane r, two tokens per column
-                if constexpr (BF) tc05::st_32x32b_x32(tmem_p + kKv / 2, pl);
+                if constexpr (PL) tc05::st_32x32b_x32(tmem_p + kKv / 2, pl);
                 tc05::wait_st();
                 tc05::fence_before_thread_sync();
                 warp_arrive(&sm.p_full[X]);
@@ -757,14 +1034,48 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             // first P, which starts a new O, comes after) ---------------------------------------------------
             const Row cur = row;
             int part = -1;
-            if constexpr (MK) part = it.part;
+            bool dup = false;
+            if constexpr (MK) { part = it.part; dup = it.dup && it.nt[1] > 0; }
             have = next_item();
             if (have < 0) goto done;
-            if (have) stage_q();
+            if (have) {
+                if constexpr (MK) stage_begin();
+                else stage_q();
+            }
             // ---- epilogue: out = (O - z) / l; z = the three zero-point columns, l = the all-ones column (u8 cache);
             // the f16 cache has no z and its l is the first column of the 16-column product
             if (!wait_warp(&sm.o_done[X], (n - 1) & 1, 2)) goto done;
             tc05::fence_after_thread_sync();
+            // masked: both halves have worked on these rows; half A takes fa of its own results and fb of half B's, which lie in the same lanes
+            float fa = 1.f, fb = 0.f, zb = 0.f, lb = 0.f;
+            if constexpr (MK) {
+                if (dup) {
+                    ++joins;
+                    if (X == 1) {
+                        reinterpret_cast<float2*>(sm.out_stage[warp])[lane] = make_float2(m_run * cur.qs, l_own);
+                        tc05::fence_before_thread_sync();
+                        warp_arrive(&sm.join_full);
+                        joins_open = true;
+                        if (have) stage_end();
+                        continue;
+                    }
+                    if (!wait_warp(&sm.join_full, (joins - 1) & 1, 2)) goto done;
+                    tc05::fence_after_thread_sync();
+                    const float2 other = reinterpret_cast<const float2*>(sm.out_stage[warp + 4])[lane];
+                    const float ma = m_run * cur.qs, top = fmaxf(ma, other.x);
+                    fa = ma == -INFINITY ? 0.f : ex2(ma - top);
+                    fb = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+                    m_run = top / cur.qs;
+                    lb = other.y;
+                    if constexpr (!BF) {
+                        uint32_t zr[16];
+                        tc05::ld_32x32b_x16(tmem_o + kNo + kD, zr);
+                        tc05::wait_ld();
+                        if constexpr (U8) zb = __uint_as_float(zr[0]) + __uint_as_float(zr[1]) + __uint_as_float(zr[2]);
+                        lb = __uint_as_float(zr[U8 ? 3 : 0]);
+                    }
+                }
+            }
             {
                 float z = 0.f, l_run = l_own;
                 if constexpr (!BF) {
@@ -774,6 +1085,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     if constexpr (U8) z = __uint_as_float(zr[0]) + __uint_as_float(zr[1]) + __uint_as_float(zr[2]);
                     l_run = __uint_as_float(zr[U8 ? 3 : 0]);
                 }
+                if constexpr (MK) {
+                    if (dup) { z = fa * z + fb * zb; l_run = fa * l_run + fb * lb; }
+                }
+                // columns of the row's results, of both halves where both have some
+                auto results = [&](int col, uint32_t (&t)[32]) {
+                    tc05::ld_32x32b_x32(tmem_o + col, t);
+                    tc05::wait_ld();
+                    if constexpr (MK) {
+                        if (dup) {
+                            uint32_t u[32];
+                            tc05::ld_32x32b_x32(tmem_o + kNo + col, u);
+                            tc05::wait_ld();
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) t[c] = __float_as_uint(fa * __uint_as_float(t[c]) + fb * __uint_as_float(u[c]));
+                        }
+                    }
+                };
                 const bool whole = !MK || part < 0;   // else a piece: unnormalised, to the scratch
                 const float inv = whole ? 1.f / l_run : 1.f;
                 // 128 bytes of every row at a time, turned around in shared memory so that eight lanes store one row's piece (a
@@ -782,7 +1110,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 const int own = cur.live ? (whole ? (int)cur.off : X * kRows + r) : -1;
                 uint8_t* const dst = whole ? (uint8_t*)a.output : (uint8_t*)(a.m.part_o + (long long)part * kPrefillItemRows * kD);
                 const int c8 = lane & 7;
-                bool finite = true;   // masked: a result that is not may come from what the row does not see
+                [[maybe_unused]] float odd = 0.f;   // masked: not-a-number once a result is not finite, which may come from what the row does not see
                 auto put = [&](int c, const uint4& w) { *reinterpret_cast<uint4*>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) = w; };
                 auto send = [&](int piece, int row_bytes) {   // the piece of every row of the warp
                     __syncwarp();
@@ -795,18 +1123,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     __syncwarp();
                 };
                 if (a.g.act == PA_DTYPE_F32 || !whole) {
-#pragma unroll
+#pragma unroll kRolled
                     for (int q4 = 0; q4 < kD / 32; ++q4) {
                         uint32_t t[32];
-                        tc05::ld_32x32b_x32(tmem_o + 32 * q4, t);
-                        tc05::wait_ld();
+                        results(32 * q4, t);
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             uint32_t w[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                w[e] = __float_as_uint((__uint_as_float(t[4 * c + e]) - z) * inv);
-                                if constexpr (MK) finite = finite && !not_finite(__uint_as_float(w[e]));
+                                if constexpr (MK) {
+                                    const float v = fmaf(__uint_as_float(t[4 * c + e]), inv, -z * inv);
+                                    odd = fmaf(v, 0.f, odd);
+                                    w[e] = __float_as_uint(v);
+                                } else {
+                                    w[e] = __float_as_uint((__uint_as_float(t[4 * c + e]) - z) * inv);
+                                }
                             }
                             put(c, make_uint4(w[0], w[1], w[2], w[3]));
                         }
@@ -814,21 +1146,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                     }
                 } else {
                     const bool f16 = a.g.act == PA_DTYPE_F16;
-#pragma unroll
+#pragma unroll kRolled
                     for (int q = 0; q < kD / 64; ++q) {
-#pragma unroll
+#pragma unroll kRolled
                         for (int h = 0; h < 2; ++h) {
                             uint32_t t[32];
-                            tc05::ld_32x32b_x32(tmem_o + 64 * q + 32 * h, t);
-                            tc05::wait_ld();
+                            results(64 * q + 32 * h, t);
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t w[4];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const float v0 = (__uint_as_float(t[8 * c + 2 * e]) - z) * inv, v1 = (__uint_as_float(t[8 * c + 2 * e + 1]) - z) * inv;
+                                    float v0, v1;
+                                    if constexpr (MK) {
+                                        v0 = fmaf(__uint_as_float(t[8 * c + 2 * e]), inv, -z * inv);
+                                        v1 = fmaf(__uint_as_float(t[8 * c + 2 * e + 1]), inv, -z * inv);
+                                        odd = fmaf(v0, 0.f, odd);
+                                        odd = fmaf(v1, 0.f, odd);
+                                    } else {
+                                        v0 = (__uint_as_float(t[8 * c + 2 * e]) - z) * inv;
+                                        v1 = (__uint_as_float(t[8 * c + 2 * e + 1]) - z) * inv;
+                                    }
                                     w[e] = f16 ? pack_h2(v0, v1) : pack_bf2(v0, v1);
-                                    if constexpr (MK) finite = finite && !not_finite(v0) && !not_finite(v1);
                                 }
                                 put(4 * h + c, make_uint4(w[0], w[1], w[2], w[3]));
                             }
@@ -836,7 +1175,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                         send(q, kD * 2);
                     }
                 }
-                if (MK && whole && cur.live && !finite) a.m.redo[atomicAdd(&a.plan->total_redo, 1)] = (int)cur.off;
+                if (MK && whole && cur.live && odd != 0.f) a.m.redo[atomicAdd(&a.plan->total_redo, 1)] = (int)cur.off;
                 if (MK && !whole) {
                     if (cur.live) a.m.part_ml[(long long)part * kPrefillItemRows + X * kRows + r] = make_float2(m_run * cur.qs, l_run);
                 } else if (cur.live && a.lse) {
@@ -844,12 +1183,122 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 }
             }
             tc05::fence_before_thread_sync();
+            if constexpr (MK) {
+                if (dup) warp_arrive(&sm.join_free);
+                if (have) stage_end();
+            }
         }
     } else if (warp < kWarpMma) {
         // ======================= converter: raw records -> f16 operand tiles =============================
         reg_dec<PA_TC_REG_CONV>();
         const int ctid = tid - kSoftmaxWarps * 32, cwarp = warp - kSoftmaxWarps;
-        if constexpr (U8) {
+        if constexpr (U8 && MK && PA_X_NEWCONV) {
+            // Masked: two warps for the keys and two for the values, so that neither's waits and fences hold up the other's (one behind the other, keys and
+            // values took 2900 cycles of a tile's 3600).  All loads of a batch of units come first, and the rare large scales (scale16) are decided once.
+            const bool values = cwarp >= kConvWarps / 2;
+            const int gt = ctid & 63;
+            constexpr int NB = 4;   // units of a batch
+            uint32_t t = 0;   // tiles so far, over all items
+            for (uint32_t ik = 0;; ++ik) {
+                It it;
+                const int item = fetch_item(ik, it);
+                if (item == -2) goto done;
+                if (item < 0) break;
+                const int ctx_hi = max(it.ctx_hi[0], it.ctx_hi[1]);
+                for (int j = 0; j < it.ntiles; ++j, ++t) {
+                    const int st = t & 1, pos0 = tile_pos(it, j);
+                    const uint32_t use = t >> 1;
+                    const uint8_t* const raw = values ? sm.raw_v[st] : sm.raw_k[st];
+                    if (!wait_warp(&sm.raw_full[st], use & 1, 0)) goto done;
+                    // every warp has the scales of all tokens (so that none waits for another); this thread sees to the zero-point of token gt
+                    uint2* const tok = sm.tok_scale[cwarp];
+                    __half zh = __ushort_as_half(0), zm = zh, zl = zh;
+                    bool ok = false, big = false;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int token = 32 * h + lane;
+                        const bool live = seen(it, ctx_hi, pos0 + token);
+                        const float* const par = reinterpret_cast<const float*>(raw + (token / BS) * Smem::RSTRIDE + BS * kD) + token % BS;
+                        const __half scale = f2h(live ? par[0] : 0.f);   // (a token that no row sees becomes zeros)
+                        const uint32_t s2 = h2_bits(scale, scale);
+                        tok[token] = make_uint2(s2, hmul2_bits(s2, 0xE400E400u));   // scale, -1024 * scale (exact)
+                        big |= !(fabsf(__half2float(scale)) < 32.f);
+                        if (token == gt) {
+                            const float z = live ? __half2float(scale) * par[BS] : 0.f;
+                            ok = live;
+                            split3(values ? z : -z, zh, zm, zl);
+                        }
+                    }
+                    const bool slow = __any_sync(0xffffffffu, big);
+                    const __half zero = __ushort_as_half(0);
+                    __syncwarp();
+                    if (!values) {
+                        if (use > 0 && !wait_warp(&sm.k_free[st], (use - 1) & 1, 1)) goto done;
+                        // K' = byte * f16(k scale): unit = 16 dims of one token
+                        *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 0)) = make_uint4(h2_bits(zh, zm), h2_bits(zl, zh), h2_bits(zm, zero), 0u);
+                        *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 1)) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+                        for (int u0 = gt; u0 < kKv * (kD / 16); u0 += 64 * NB) {
+                            uint4 lo4[NB], hi4[NB];
+                            uint2 sc[NB];
+#pragma unroll
+                            for (int i = 0; i < NB; ++i) {
+                                const int u = u0 + 64 * i, token = u / (kD / 16), seg = u % (kD / 16);
+                                sc[i] = tok[token];
+                                bytes16_to_h(*reinterpret_cast<const uint4*>(raw + (token / BS) * Smem::RSTRIDE + (token % BS) * kD + 16 * seg), lo4[i], hi4[i]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < NB; ++i) {
+                                const int u = u0 + 64 * i, token = u / (kD / 16), seg = u % (kD / 16);
+                                scale_pair(lo4[i], sc[i], slow);
+                                scale_pair(hi4[i], sc[i], slow);
+                                uint8_t* atom = sm.k[st] + (seg >> 2) * (kKv * 128);
+                                *reinterpret_cast<uint4*>(atom + sw128(token, (2 * seg) & 7)) = lo4[i];
+                                *reinterpret_cast<uint4*>(atom + sw128(token, (2 * seg + 1) & 7)) = hi4[i];
+                            }
+                        }
+                        tc05::fence_proxy_async_smem();
+                        warp_arrive(&sm.k_full[st]);
+                    } else {
+                        if (use > 0 && !wait_warp(&sm.v_free[st], (use - 1) & 1, 2)) goto done;
+                        // V'^T = byte * f16(v scale): unit = 16 tokens of one dim
+                        const int tg = gt & 3;
+                        uint2 tab[8];   // of two tokens: their scales, and -1024 times them
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint4 two = *reinterpret_cast<const uint4*>(&tok[16 * tg + 2 * k]);
+                            tab[k] = make_uint2(__byte_perm(two.x, two.z, 0x5410), __byte_perm(two.y, two.w, 0x5410));
+                        }
+                        constexpr int UPR = BS / 16;   // 16-token units per record
+                        const uint8_t* const col = raw + (tg / UPR) * Smem::RSTRIDE + 16 * (tg % UPR);
+#pragma unroll 1
+                        for (int d0 = gt >> 2; d0 < kD; d0 += 16 * NB) {
+                            uint4 lo4[NB], hi4[NB];
+#pragma unroll
+                            for (int i = 0; i < NB; ++i) bytes16_to_h(*reinterpret_cast<const uint4*>(col + (d0 + 16 * i) * BS), lo4[i], hi4[i]);
+#pragma unroll
+                            for (int i = 0; i < NB; ++i) {
+                                const int d = d0 + 16 * i;
+                                uint32_t w[8] = {lo4[i].x, lo4[i].y, lo4[i].z, lo4[i].w, hi4[i].x, hi4[i].y, hi4[i].z, hi4[i].w};
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE400E400u), tab[k].x) : hfma2_bits(w[k], tab[k].x, tab[k].y);
+                                *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg)) = make_uint4(w[0], w[1], w[2], w[3]);
+                                *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
+                        }
+                        const uint32_t off = (gt & 7) * 2;
+                        uint8_t* vt = sm.vt[st];
+                        *reinterpret_cast<__half*>(vt + sw128(kD + 0, gt >> 3) + off) = zh;
+                        *reinterpret_cast<__half*>(vt + sw128(kD + 1, gt >> 3) + off) = zm;
+                        *reinterpret_cast<__half*>(vt + sw128(kD + 2, gt >> 3) + off) = zl;
+                        *reinterpret_cast<__half*>(vt + sw128(kD + 3, gt >> 3) + off) = __ushort_as_half(ok ? (unsigned short)0x3C00u : (unsigned short)0u);
+                        tc05::fence_proxy_async_smem();
+                        warp_arrive(&sm.v_full[st]);
+                    }
+                    warp_arrive(&sm.raw_free[st]);   // (and the scales have been read)
+                }
+            }
+        } else if constexpr (U8) {
         uint32_t t = 0;   // tiles so far, over all items
         for (uint32_t ik = 0;; ++ik) {
             It it;
@@ -959,6 +1408,34 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             }
         }
         } else {
+            if constexpr (MK) {
+            // ---- 16-bit caches, masked: the loader's tensor copies bring the tiles; of those that no row sees as a whole, these warps clear the value rows
+            // that no row sees (0 times what is not a number is none), of blocks that were not brought too.  (Their keys' logits are not looked at.)
+            (void)cwarp;
+            constexpr int CH = kD / 8, TP = kConvWarps * 32 / CH, NU = kKv / TP;   // chunks of a row, tokens per pass, passes
+            const int ch = ctid % CH, trow = ctid / CH;
+            uint32_t t = 0;   // tiles so far
+            for (uint32_t ik = 0;; ++ik) {
+                It it;
+                const int item = fetch_item(ik, it);
+                if (item == -2) goto done;
+                if (item < 0) break;
+                const int ctx_hi = max(it.ctx_hi[0], it.ctx_hi[1]);
+                for (int j = 0; j < it.ntiles; ++j, ++t) {
+                    const int pos0 = tile_pos(it, j), st = t % NST;
+                    if (!wait_warp(&sm.v_land[st], (t / NST) & 1, 2)) goto done;   // (of every tile: a phase that is not waited for is mistaken for the one two on)
+                    if (whole_tile(it, ctx_hi, pos0)) continue;
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) {
+                        const int token = trow + TP * u;
+                        if (!seen(it, ctx_hi, pos0 + token))
+                            *reinterpret_cast<uint4*>(sm.vt[st] + (uint32_t)(ch >> 3) * (kKv * 128) + sw128(token, ch & 7)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    tc05::fence_proxy_async_smem();
+                    warp_arrive(&sm.v_full[st]);
+                }
+            }
+            } else {
             // ---- f16 cache: token rows -> operand tiles with cp.async; thread = 16-byte chunk `ch` of the rows trow + TP u.
             // The copies of tile t are in flight while tile t - 1 is handed over: K_t is issued, then K_(t-1) is
             // awaited, fenced for the tensor core's proxy and published, then the same for V.
@@ -1026,8 +1503,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 warp_arrive(&sm.v_full[(t - 1) % NST]);
             }
             if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
+            }
         }
-    } else if (warp == kWarpMma || (!U8 && warp == kWarpMma2)) {
+    } else if (warp == kWarpMma || (TwoMma && warp == kWarpMma2)) {
         // ======================= mma issue ================================================================
         // u8 cache: one warp serves both halves in turn, S of tile j + 1 of a half behind P of its tile j.  16-bit caches: one warp
         // per half, so that neither half's waits hold up the other's instructions, and S of tile j + 1 is issued as soon as
@@ -1082,13 +1560,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
 #pragma unroll
                     for (int kk = 1; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + 8 * kk, db0 + 2 * kk, idesc_o);
                 } else if constexpr (BF) {
-                    // high pieces of P, then the low pieces against the same value rows
+                    // high pieces of P, then the low pieces (where there are any) against the same value rows
                     if (acc) tc05::mma_ts<1>(d, pa, db0, idesc_o);
                     else tc05::mma_ts<0>(d, pa, db0, idesc_o);
 #pragma unroll
                     for (int kk = 1; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + 8 * kk, db0 + 128 * kk, idesc_o);
 #pragma unroll
-                    for (int kk = 0; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + kKv / 2 + 8 * kk, db0 + 128 * kk, idesc_o);
+                    for (int kk = 0; kk < (PL ? kKv / 16 : 0); ++kk) tc05::mma_ts<1>(d, pa + kKv / 2 + 8 * kk, db0 + 128 * kk, idesc_o);
                 } else {
                     // 16 tokens further along K = 16 rows of 128 bytes; the denominators go to the 16 columns after O
                     if (acc) { tc05::mma_ts<1>(d, pa, db0, idesc_o); tc05::mma_ts<1>(d + kD, pa, dones, idesc_l); }
@@ -1104,7 +1582,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                 __syncwarp();
             };
             uint32_t t = 0;   // tiles so far, over all items
-            if constexpr (U8) {
+            if constexpr (!TwoMma) {
                 uint32_t n[2] = {0, 0}, iq[2] = {0, 0};
                 for (uint32_t ik = 0;; ++ik) {
                     It it;
@@ -1158,24 +1636,37 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
             } else {
                 const int X = warp == kWarpMma ? 0 : 1;
                 uint32_t n = 0, iq = 0;   // tiles and items of this half
+                [[maybe_unused]] uint32_t cleared = 0;   // masked, 16-bit caches: bit s, the phase of v_full[s]
                 for (uint32_t ik = 0;; ++ik) {
                     It it;
                     const int item = fetch_item(ik, it);
                     if (item == -2) goto done;
                     if (item < 0) break;
                     const int nt = it.nt[X];
+                    [[maybe_unused]] const int ctx_hi = max(it.ctx_hi[0], it.ctx_hi[1]);
                     // first S of the item.  The S region is free: the half's softmax staged these rows after it had read the last S.
                     if (nt > 0) {
                         if (!wait_warp(&sm.q_full[X], iq & 1, 0)) goto done;
                         ++iq;
                     }
-                    for (int j = -1; j < it.ntiles; ++j) {
+                    // tiles of this half, and a tile's number among them; S runs ahead by one of the half's tiles
+                    auto uses = [&](int j) -> bool {
+                        if constexpr (MK) return it.uses(X, j);
+                        else return j < nt;
+                    };
+                    auto own = [&](int j) -> int {
+                        if constexpr (MK) return it.own(j);
+                        else return j;
+                    };
+                    int ahead = 1;
+                    if constexpr (MK) ahead = it.dup ? 2 : 1;
+                    for (int j = -ahead; j < it.ntiles; ++j) {
                         if (j >= 0) PA_TRACE(3 + 2 * X, 0, t + j);
-                        if (j + 1 < it.ntiles) {
-                            const int st1 = (t + j + 1) % NST;
-                            if (!wait_warp(&sm.k_full[st1], ((t + j + 1) / NST) & 1, 1)) goto done;
-                            if (j + 1 < nt) {
-                                if (j >= 0 && !wait_warp(&sm.s_read[X], (n + j) & 1, 2)) goto done;
+                        if (j + ahead < it.ntiles) {
+                            const int js = j + ahead, st1 = (t + js) % NST;
+                            if (!wait_warp(&sm.k_full[st1], ((t + js) / NST) & 1, 1)) goto done;
+                            if (uses(js)) {
+                                if (own(js) > 0 && !wait_warp(&sm.s_read[X], (n + own(js) - 1) & 1, 2)) goto done;
                                 tc05::fence_after_thread_sync();
                                 issue_s(X, st1);
                                 if (tc05::elect_one()) tc05::commit(&sm.k_free[st1]);
@@ -1187,13 +1678,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
                         }
                         if (j >= 0) {
                             const int st = (t + j) % NST;
-                            if (!wait_warp(&sm.v_full[st], ((t + j) / NST) & 1, 3)) goto done;
+                            if constexpr (!U8 && MK) {
+                                if (whole_tile(it, ctx_hi, tile_pos(it, j))) {
+                                    if (!wait_warp(&sm.v_land[st], ((t + j) / NST) & 1, 3)) goto done;
+                                } else {
+                                    if (!wait_warp(&sm.v_full[st], (cleared >> st) & 1u, 3)) goto done;
+                                    cleared ^= 1u << st;
+                                }
+                            } else {
+                                if (!wait_warp(&sm.v_full[st], ((t + j) / NST) & 1, 3)) goto done;
+                            }
                             PA_TRACE(3 + 2 * X, 3, t + j);
-                            if (j < nt) {
-                                if (!wait_warp(&sm.p_full[X], (n + j) & 1, 4)) goto done;
+                            if (uses(j)) {
+                                if (!wait_warp(&sm.p_full[X], (n + own(j)) & 1, 4)) goto done;
                                 PA_TRACE(3 + 2 * X, 4, t + j);
                                 tc05::fence_after_thread_sync();
-                                issue_pv(X, st, j > 0);
+                                issue_pv(X, st, own(j) > 0);
                                 if (tc05::elect_one()) tc05::commit(&sm.v_free[st]);
                                 __syncwarp();
                                 PA_TRACE(3 + 2 * X, 5, t + j);
@@ -1214,52 +1714,96 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(KernelArgs a) {
         if (lane == 0) {
             uint32_t t = 0;
             bool bad_index = false;
+            std::conditional_t<MK, MaskWalk, int> walk = make_walk<MK>(a);
             for (uint32_t ik = 0;; ++ik) {
                 const int slot = ik & (kItemSlots - 1);
                 if (ik >= kItemSlots && !wait(&sm.item_free[slot], ((ik / kItemSlots) - 1) & 1, 1)) goto done;
-                if constexpr (!U8) {
+                if constexpr (!U8 && !MK) {
                     // Nothing throttles this loader (it copies no tiles), and an item drawn early is an item another CTA cannot
                     // take: the next one is drawn when every role has started the previous one, which is still several tiles
                     // before the copy warps need it.
                     if (ik >= 1 && !wait(&sm.item_free[(ik - 1) & (kItemSlots - 1)], ((ik - 1) / kItemSlots) & 1, 1)) goto done;
                 }
-                int item = atomicAdd(&a.plan->next_pitem, 1);
-                if (item >= total_items) item = -1;
+                int item;
                 It it{};
-                if (item >= 0) {
-                    if constexpr (MK) it = locate_masked(a, item, G, Hkv);
-                    else it = locate_item(a, item, G, Hkv);
-                    sm.item_desc[slot] = it;
+                if constexpr (MK) {
+                    item = walk.template next<TwoMma>(a, G, it) ? 0 : -1;
+                } else {
+                    item = atomicAdd(&a.plan->next_pitem, 1);
+                    if (item >= total_items) item = -1;
+                    if (item >= 0) it = locate_item(a, item, G, Hkv);
                 }
+                if (item >= 0) sm.item_desc[slot] = it;
                 sm.item_ring[slot] = item;
                 mbar_arrive(&sm.item_full[slot]);
                 if (item < 0) break;
-                if constexpr (U8) {
                 const int ctx_hi = max(it.ctx_hi[0], it.ctx_hi[1]);
-                const uint8_t* kc = (const uint8_t*)a.key_cache + (long long)it.hk * a.g.head_bytes;
-                const uint8_t* vc = (const uint8_t*)a.value_cache + (long long)it.hk * a.g.head_bytes;
-                for (int j = 0; j < it.ntiles; ++j, ++t) {
-                    const int st = t & 1;
-                    const uint32_t use = t >> 1;
+                // block ids of an item's j-th tile, -1: no row sees any of the block
+                [[maybe_unused]] auto look_up = [&](int j, int (&blocks)[Smem::NREC]) {
                     const int pos0 = tile_pos(it, j);
-                    if (use > 0 && !wait(&sm.raw_free[st], (use - 1) & 1, 0)) goto done;
-                    PA_TRACE(4, 0, t);
-                    uint32_t bytes = 0;
-                    int blocks[Smem::NREC];
 #pragma unroll
                     for (int r = 0; r < Smem::NREC; ++r) {
                         const int bi = pos0 / BS + r;
-                        int blk = -1;
                         bool any = bi * BS < ctx_hi;
                         if constexpr (MK) any = any && (bi * BS < a.m.sinks || (bi + 1) * BS > it.lo);
-                        if (any) {
-                            blk = it.table[bi];
-                            if (blk < 0 || blk >= a.num_blocks) { blk = 0; bad_index = true; }
-                            bytes += 2 * Smem::REC;
-                        }
-                        blocks[r] = blk;
+                        blocks[r] = any ? it.table[bi] : -1;
+                        if (any && (blocks[r] < 0 || blocks[r] >= a.num_blocks)) { blocks[r] = 0; bad_index = true; }
                     }
+                };
+                if constexpr (!U8 && MK) {
+                    // tensor copies straight into the swizzled operand tiles; all stages under way
+                    int next[Smem::NREC];
+                    look_up(0, next);
+                    for (int j = 0; j < it.ntiles; ++j, ++t) {
+                        const int st = t % NST;
+                        const uint32_t use = t / NST;
+                        int blocks[Smem::NREC];
+                        uint32_t bytes = 0;
+#pragma unroll
+                        for (int r = 0; r < Smem::NREC; ++r) {
+                            blocks[r] = next[r];
+                            bytes += blocks[r] >= 0 ? BS * kD * 2 : 0;
+                        }
+                        if (j + 1 < it.ntiles) look_up(j + 1, next);
+                        auto bring = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+                            mbar_expect_tx(bar, bytes);
+#pragma unroll
+                            for (int r = 0; r < Smem::NREC; ++r)
+                                if (blocks[r] >= 0) {
+#pragma unroll
+                                    for (int c = 0; c < kD / 64; ++c) tma_3d(dst + c * (kKv * 128) + r * (BS * 128), map, 64 * c, 0, blocks[r] * Hkv + it.hk, bar);
+                                }
+                        };
+                        if (use > 0 && !wait(&sm.k_free[st], (use - 1) & 1, 0)) goto done;
+                        bring(sm.k[st], &a.m.map_k, &sm.k_full[st]);
+                        begun = t + 1;
+                        if (use > 0 && !wait(&sm.v_free[st], (use - 1) & 1, 0)) goto done;
+                        bring(sm.vt[st], &a.m.map_v, &sm.v_land[st]);
+                        begun_v = t + 1;
+                    }
+                }
+                if constexpr (U8) {
+                const uint8_t* kc = (const uint8_t*)a.key_cache + (long long)it.hk * a.g.head_bytes;
+                const uint8_t* vc = (const uint8_t*)a.value_cache + (long long)it.hk * a.g.head_bytes;
+                [[maybe_unused]] int next[Smem::NREC];   // masked: the next tile's, looked up before the wait for its stage
+                if constexpr (MK) look_up(0, next);
+                for (int j = 0; j < it.ntiles; ++j, ++t) {
+                    const int st = t & 1;
+                    const uint32_t use = t >> 1;
+                    int blocks[Smem::NREC];
+                    if constexpr (MK) {
+#pragma unroll
+                        for (int r = 0; r < Smem::NREC; ++r) blocks[r] = next[r];
+                        if (j + 1 < it.ntiles) look_up(j + 1, next);
+                    }
+                    if (use > 0 && !wait(&sm.raw_free[st], (use - 1) & 1, 0)) goto done;
+                    PA_TRACE(4, 0, t);
+                    if constexpr (!MK) look_up(j, blocks);
+                    uint32_t bytes = 0;
+#pragma unroll
+                    for (int r = 0; r < Smem::NREC; ++r) bytes += blocks[r] >= 0 ? 2 * Smem::REC : 0;
                     mbar_expect_tx(&sm.raw_full[st], bytes);
+                    if constexpr (MK) begun = t + 1;
 #pragma unroll
                     for (int r = 0; r < Smem::NREC; ++r)
                         if (blocks[r] >= 0) {
@@ -1287,6 +1831,20 @@ done:
         printf("prefill prof warp %d total %lld waits %lld %lld %lld %lld %lld\n", warp, clock64() - prof_begin, prof[0], prof[1], prof[2], prof[3], prof[4]);
 #endif
     if constexpr (!U8) cp_async_wait<0>();   // an aborted copy warp leaves no copy in flight
+    if constexpr (MK) {
+        cp_async_wait<0>();
+        // nor does the loader
+        if (warp == kWarpLoad && lane == 0 && sm.abort) {
+            for (uint32_t i = begun > NST ? begun - NST : 0; i < begun; ++i) {
+                if constexpr (U8) {
+                    mbar_wait_bounded(&sm.raw_full[i % NST], (i / NST) & 1);
+                } else {
+                    mbar_wait_bounded(&sm.k_full[i % NST], (i / NST) & 1);
+                    if (i < begun_v) mbar_wait_bounded(&sm.v_land[i % NST], (i / NST) & 1);
+                }
+            }
+        }
+    }
     tc05::fence_before_thread_sync();
     __syncthreads();
     if (warp == 0) tc05::tmem_dealloc(tmem, kTmemCols);
@@ -1304,6 +1862,7 @@ namespace {
 template <int BS, int CT, int D, bool MK>
 cudaError_t launch_tc_t(const KernelArgs& a, cudaStream_t stream, int grid) {
     const int bytes = (int)sizeof(PrefillSmem<BS, CT, D, MK>) + 1024;
+    static_assert(sizeof(PrefillSmem<BS, CT, D, MK>) + 1024 <= 232448, "227 KB a block");
     cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<BS, CT, D, MK>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     return launch_dependent(prefill_tc_kernel<BS, CT, D, MK>, dim3(grid), dim3(kThreads), bytes, stream, a);
