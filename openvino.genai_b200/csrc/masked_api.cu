@@ -56,6 +56,10 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 struct Scratch {
     size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, part_o, part_ml, total;
 };
+// Steps of single tokens go without a plan where a stream has few tiles (under a short window, or by its block table): the plan is a launch's chain in front
+// of a kernel that is not much longer.  Longer streams are better off in the plan's slices, which know how many tiles each has.
+constexpr int kDirectTiles = 64;
+
 Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     const pa::CacheGeom& g = h->g;
     const int G = g.Hq / g.Hkv, HK = g.Hkv * ((G + 15) / 16), RT = std::min(G, 16);
@@ -153,11 +157,11 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     k.part_o = (float*)(ws + s.decode_o);
     k.part_ml = (float*)(ws + s.decode_ml);
     k.rows_per_tile = std::min(G, 16);
-    // upper bound of the tiles of rows with one new token: all tiles of their block tables, or what their windows leave
-    long long tiles = (long long)a->num_block_indices * h->g.bs / 32 + a->num_sequences;
-    if (mask.sliding_window > 0)
-        tiles = std::min(tiles, (long long)a->num_sequences * (((long long)mask.sliding_window + 31) / 32 + ((long long)mask.sink_tokens + 31) / 32 + 1));
-    k.max_tiles = tiles * HK;
+    // upper bounds of the tiles of rows with one new token: all tiles of their block tables, or what their windows leave
+    const long long table_tiles = (long long)a->num_block_indices * h->g.bs / 32 + 1;
+    long long row_tiles = table_tiles;
+    if (mask.sliding_window > 0) row_tiles = std::min(row_tiles, ((long long)mask.sliding_window + 31) / 32 + ((long long)mask.sink_tokens + 31) / 32 + 1);
+    k.max_tiles = std::min(table_tiles + a->num_sequences, row_tiles * a->num_sequences) * HK;
     MaskParams& m = k.m;
     m.on = 1;
     m.window = mask.sliding_window;
@@ -174,9 +178,13 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     // As many tokens as sequences: single tokens, almost always, and no launches for chunks; what of them there is beside sequences without
     // tokens, the device finds out
     m.rows_in_decode = a->num_tokens > 1 && a->num_tokens == a->num_sequences;
+    if (a->num_tokens == a->num_sequences && row_tiles <= kDirectTiles && row_tiles * a->num_sequences * HK <= INT_MAX / 2) {
+        m.direct_tiles = (int)row_tiles;
+        k.release_early = 1;
+    }
     m.part_o = (float*)(ws + s.part_o);
     m.part_ml = (float2*)(ws + s.part_ml);
-    k.decode_all_workers = decode_launch_workers(k, h->sm_count);
+    if (m.direct_tiles == 0) k.decode_all_workers = decode_launch_workers(k, h->sm_count);
     int launches = 0;
     if (a->num_rotated_blocks > 0) { MASKED_CUDA(launch_rotate(k, stream)); ++launches; }
     MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;

@@ -1,7 +1,7 @@
 // Joins the pieces of lists that a masked step cut between CTAs (build_mask_items): a row's result is
 // sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over its pieces, M the largest m_i.  A lane has D / 32 neighbouring elements of a row, pieces are taken in
 // order, so that the result does not depend on who ended first.  Bound by the chain starts -> q tile -> pieces, so a block looks its list up once for 32
-// rows, and eight loads of a warp are under way: two pieces of four rows, or eight of one.  Rows whose result is not finite are computed again by themselves (masked_row): what they do not see may have been the cause.
+// rows, and eight or sixteen loads of a warp are under way: two pieces of four rows, or eight of two.  Rows whose result is not finite are computed again by themselves (masked_row): what they do not see may have been the cause.
 #include <type_traits>
 
 #include "masked.cuh"
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) masked_join_kernel(const __gr
                 }
             };
             if (all <= 2) join(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-            else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+            else join(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
         }
     }
     // rows of whole q tiles that are not finite: once more, by themselves

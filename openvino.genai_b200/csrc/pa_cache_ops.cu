@@ -472,6 +472,11 @@ __global__ void __launch_bounds__(256) write_kv_kernel(KernelArgs a) {
     int first_block = 0;
     if constexpr (PLAN) {
         if (blockIdx.x == 0) {
+            if (a.m.on && a.m.direct_tiles > 0) {   // no plan: the streams' counters only
+                const int G = a.g.Hq / a.g.Hkv, streams = a.num_sequences * a.g.Hkv * ((G + 15) / 16);
+                for (int i = threadIdx.x; i < streams; i += 256) a.stream_done[i] = 0;
+                return;
+            }
             build_decode_plan(a);
             return;
         }

@@ -20,7 +20,9 @@
 // reference maximum.  A stream cut by slice boundaries is merged by the warp whose partial
 // completes it (one atomic counter per stream, no waiting).
 // Rows under a sliding window (WIN; include/masked_b200.h): a stream's tiles are those that hold a position its row sees, the sinks' and then the
-// window's; the loader steps over the gap between them, and a stage's descriptor holds the bits of its visible tokens.
+// window's; the loader steps over the gap between them, and a stage's descriptor holds the bits of its visible tokens.  Steps of single tokens
+// under short windows go without a plan (DIRECT): every stream counts for a.m.direct_tiles tiles, the most that one can have, so that a worker finds its slice
+// by itself; and the launch overlaps the cache write, which it waits for only in front of the tile that holds the new token.
 // HBM-bound: 2*Hkv*(D+8) bytes per context token for the u8 cache.
 #include <algorithm>
 #include <atomic>
@@ -97,17 +99,86 @@ __device__ __forceinline__ void store_pair(void* out, long long idx, int act, fl
     else *reinterpret_cast<__nv_bfloat162*>((__nv_bfloat16*)out + idx) = __floats2bfloat162_rn(v0, v1);
 }
 
+// Without a plan: the slices of the sequence in which every stream counts for direct_tiles tiles.
+__host__ __device__ inline DecodeSlices direct_slices(const KernelArgs& a, int HK, int all_workers) {
+    const int total = a.num_sequences * HK * a.m.direct_tiles;
+    const int per = max((total + all_workers - 1) / all_workers, kDirectMinSlice);
+    return DecodeSlices{(total + per - 1) / per, per, total};
+}
+
+// Joins the partial results of a stream (slots first_slot .. of hcount rows each) into the output rows from `row` on; one warp.  (Inlined: as a function of
+// its own its call cost the loop more registers, and the step of one row 9 us.)
+template <int D>
+__device__ __forceinline__ void merge_stream(const KernelArgs& a, int first_slot, int nparts, int hcount, long long row) {
+    const int lane = threadIdx.x & 31;
+    // Four pieces of 16 bytes of a partial's rows a lane, four partials of them under way: the chain of loads is what a small step waits for (a
+    // lane for two columns of a row at a time, 17 partials took 11 us).
+    const int vecs = hcount * (D / 4);
+    for (int f0 = 0; f0 < vecs; f0 += 128) {
+        float m[4], l[4], o[4][4];
+        int at[4];
+        bool on[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            on[k] = f0 + 32 * k + lane < vecs;
+            at[k] = on[k] ? f0 + 32 * k + lane : 0;
+            m[k] = -INFINITY; l[k] = 0.f;
+            o[k][0] = 0.f; o[k][1] = 0.f; o[k][2] = 0.f; o[k][3] = 0.f;
+        }
+#pragma unroll 1
+        for (int j0 = 0; j0 < nparts; j0 += 4) {
+            float2 ml[4][4];
+            float4 v[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const long long slot = first_slot + min(j0 + u, nparts - 1);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    ml[u][k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + (slot * a.rows_per_tile + at[k] / (D / 4)) * 2));
+                    v[u][k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot * a.rows_per_tile * D + 4 * at[k]));
+                    if (j0 + u >= nparts) ml[u][k] = make_float2(-INFINITY, 0.f);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float top = fmaxf(fmaxf(m[k], fmaxf(ml[0][k].x, ml[1][k].x)), fmaxf(ml[2][k].x, ml[3][k].x));
+                const float keep = m[k] > -INFINITY ? fast_exp2(m[k] - top) : 0.f;
+                m[k] = top;
+                l[k] *= keep;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][e] *= keep;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (j0 + u >= nparts) continue;
+                    const float f = fast_exp2(ml[u][k].x - top);
+                    l[k] += f * ml[u][k].y;
+                    o[k][0] += f * v[u][k].x; o[k][1] += f * v[u][k].y; o[k][2] += f * v[u][k].z; o[k][3] += f * v[u][k].w;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (on[k]) {
+                const float inv = 1.f / l[k];
+                const long long out = (row + at[k] / (D / 4)) * D + 4 * (at[k] % (D / 4));
+                store_pair(a.output, out, a.g.act, o[k][0] * inv, o[k][1] * inv);
+                store_pair(a.output, out + 2, a.g.act, o[k][2] * inv, o[k][3] * inv);
+            }
+    }
+}
+
 #ifdef PA_DECODE_PROF
 __device__ unsigned long long g_decode_prof[8192 * 8];   // per worker: start, first tile ready, end (ns), tiles, cycles waiting for tiles, cycles in all, cycles in produce
 #endif
 
 // SC: the launch keeps the scaled logits of rows whose scores are wanted (a.score_raw is set); a
 // separate instantiation so that steps without a score output run the same code as before.
-template <int D, int BS, int CACHE, bool HI, bool SC, bool WIN>
+template <int D, int BS, int CACHE, bool HI, bool SC, int MASK>
 __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2) ? 2 : 3) decode_kernel(const __grid_constant__ KernelArgs a) {
     using Cfg = DecodeCfg<D, BS, CACHE>;
     constexpr bool U8 = Cfg::U8;
     constexpr bool BF16 = Cfg::BF16;
+    constexpr bool WIN = MASK != 0, DIRECT = MASK == 2;
     constexpr int NKK = D / 16;   // k-steps of Q.K^T
     constexpr int NDT = D / 8;    // n-tiles of P.V
     constexpr int ROWS = HI ? 2 : 1;
@@ -136,23 +207,28 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     const float sm_scale = a.scale != 0.f ? a.scale : rsqrtf((float)D);
     const bool q_pairs = (reinterpret_cast<uintptr_t>(a.query) & 7) == 0;   // a pair of elements is one aligned load
     bool bad_index = false;
-    // everything below reads what the launch before this one wrote (plan, start records, cache)
-    grid_wait();
+    // everything below reads what the launch before this one wrote (plan, start records, cache; without a plan the newest token of the cache alone)
+    bool waited = !DIRECT;
+    if (!DIRECT) grid_wait();
+    auto wait_once = [&] {
+        if (!waited) grid_wait();
+        waited = true;
+    };
 
     // ---- this worker's slice of the global tile sequence -----------------------------------------
-    const int all_workers = gridDim.x * kDecodeWarps;
+    const int all_workers = DIRECT ? a.m.direct_workers : gridDim.x * kDecodeWarps;
     const int wid = blockIdx.x * kDecodeWarps + warp;
     WorkerStart ws0;
     ws0.s = -1;
-    if (a.worker_start && a.decode_all_workers == all_workers) {   // one start record per worker
+    if (!DIRECT && a.worker_start && a.decode_all_workers == all_workers) {   // one start record per worker
         const int4 lo4 = __ldcg(reinterpret_cast<const int4*>(a.worker_start + wid));
         const int4 hi4 = __ldcg(reinterpret_cast<const int4*>(a.worker_start + wid) + 1);
         ws0 = WorkerStart{lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
     }
     int chunk_items = 0;   // chunks in a step that was not thought to hold any
-    if constexpr (WIN) chunk_items = a.m.rows_in_decode ? __ldcg(&a.plan->total_mitems) : 0;
-    const int total_tiles = ws0.s != -1 ? ws0.total_tiles : a.plan->total_tiles;   // all streams
-    const DecodeSlices sl = decode_slices(total_tiles, all_workers);
+    if constexpr (WIN && !DIRECT) chunk_items = a.m.rows_in_decode ? __ldcg(&a.plan->total_mitems) : 0;
+    const int total_tiles = DIRECT ? 0 : ws0.s != -1 ? ws0.total_tiles : a.plan->total_tiles;   // all streams
+    const DecodeSlices sl = DIRECT ? direct_slices(a, HK, all_workers) : decode_slices(total_tiles, all_workers);
     int g_tile = 0, g_end = 0;       // next global tile to load, end of the slice
 
     // ---- loader state (warp-uniform registers) -------------------------------------------------------
@@ -190,9 +266,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             r_gap = v.gap * kTile;
         }
         r_end = min(ctx - r_gap, (tile0 + ntile) * kTile);
-        const int s_begin = p0 * HK + r_hkp * r_tiles;             // global tile range of the stream
-        const int first_w = sl.worker_of(s_begin), last_w = sl.worker_of(s_begin + r_tiles - 1);
         const int stream = r_s * HK + r_hkp;
+        const int s_begin = DIRECT ? stream * a.m.direct_tiles : p0 * HK + r_hkp * r_tiles;   // global tile range of the stream
+        const int first_w = sl.worker_of(s_begin), last_w = sl.worker_of(s_begin + r_tiles - 1);
         ++r_seq;
         if (lane == 0) {
             // rows whose attention scores are wanted (window > 0) leave their scaled logits behind
@@ -214,7 +290,28 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         load_window(context_tok(r_tok) / BS);
     };
     // Moves the loader to its next run: the first tile of the next stream of the slice.  False when the slice is done.
+    bool chunks = false;   // without a plan: the slice begins streams of a sequence with several new tokens
     auto advance = [&]() -> bool {
+        if constexpr (DIRECT) {
+            const int V = a.m.direct_tiles;
+            while (g_tile < g_end) {
+                const int stream = g_tile / V, tile0 = g_tile % V, s = stream / HK;
+                SeqView sv;
+                const bool ok = seq_view(a, s, sv);
+                chunks |= sv.n > 1;
+                r_tiles = ok && sv.n == 1 ? vis_tiles<kTile>(sv.past + 1, window_lo(a.m, sv.past + 1), a.m.sinks).count : 0;
+                if (tile0 < r_tiles) {
+                    r_s = s; r_hkp = stream % HK;
+                    r_tb = sv.tb; r_nb = sv.nb;
+                    const int from = g_tile;
+                    start_run(tile0, 0, sv.past + 1, sv.t0);
+                    if (g_tile - from == r_tiles - tile0) g_tile = min(g_end, (stream + 1) * V);   // behind its last tile
+                    return true;
+                }
+                g_tile = min(g_end, (stream + 1) * V);
+            }
+            return false;
+        }
         if (g_tile >= g_end) return false;
         if (++r_hkp == HK) {
             r_hkp = 0;
@@ -231,7 +328,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     // The worker's own slice: from the record the plan step prepared, else by binary search in the prefix sums.
     g_tile = (int)sl.begin(wid);
     g_end = (int)sl.end(wid);
-    if (g_tile < g_end) {
+    if (DIRECT && wid >= sl.workers1) g_end = g_tile;
+    [[maybe_unused]] const int g_begin = g_tile;
+    if (!DIRECT && g_tile < g_end) {
         int p0, ctx, t0row;
         if (ws0.s >= 0) {
             r_s = ws0.s;
@@ -270,6 +369,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             if (lane == 0) descs[slot] = StageDesc{kEnd, 0, 0, 0};
             if constexpr (!U8) cp_async_commit();
             return;
+        }
+        // the tile with the new token, which the cache write puts there
+        if constexpr (DIRECT) {
+            if (r_tok + kTile >= r_tiles * kTile) wait_once();
         }
         uint8_t* st = ring + slot * Cfg::STAGE;
         const int hk = r_hkp / gtiles;
@@ -711,6 +814,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             }
             continue;
         }
+        if constexpr (DIRECT) wait_once();   // (which also clears the streams' counters)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const int hrow = g + 8 * r;
@@ -730,6 +834,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
         // ---- this partial completed the stream: merge all of its partials ---------------------------
         __threadfence();
         const int nparts = fin.nparts;
+        if constexpr (DIRECT) {
+            merge_stream<D>(a, fin.first_slot, nparts, hcount, (long long)t0 * a.g.Hq + hbase);
+            continue;
+        }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const int hrow = g + 8 * r;
@@ -776,7 +884,15 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     }
     if constexpr (!U8) cp_async_wait<0>();
     if (__any_sync(0xffffffffu, bad_index) && lane == 0) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
-    if constexpr (WIN) {
+    if constexpr (DIRECT) {
+        wait_once();   // (whoever follows waits for this kernel only)
+        if (chunks)   // chunks among them: the rows of a stream's first query head, one by one
+            for (int stream = (g_begin + a.m.direct_tiles - 1) / a.m.direct_tiles; stream * a.m.direct_tiles < g_end; ++stream) {
+                SeqView sv;
+                if (seq_view(a, stream / HK, sv) && sv.n > 1)
+                    for (int row = stream % HK; row < sv.n * a.g.Hq; row += HK) masked_row<D>(a, sv.t0 + row / a.g.Hq, row % a.g.Hq);
+            }
+    } else if constexpr (WIN) {
         if (chunk_items > 0)
             for (long long row = wid; row < (long long)a.num_tokens * a.g.Hq; row += all_workers) masked_row<D>(a, (int)(row / a.g.Hq), (int)(row % a.g.Hq));
     }
@@ -802,11 +918,14 @@ long long decode_ctas(const KernelArgs& a, int per_sm, int sm_count) {
     return std::max(1LL, std::min((long long)std::min(per_sm, kDecodeMaxCtasPerSm) * sm_count, cap));
 }
 
+int mask_of(const KernelArgs& a) { return !a.m.on ? 0 : a.m.direct_tiles > 0 ? 2 : 1; }
+
 template <int D, int BS, int CACHE>
-auto pick_kernel(bool hi, bool sc, bool masked) {
-    auto kern = hi ? (sc ? decode_kernel<D, BS, CACHE, true, true, false> : decode_kernel<D, BS, CACHE, true, false, false>)
-                   : (sc ? decode_kernel<D, BS, CACHE, false, true, false> : decode_kernel<D, BS, CACHE, false, false, false>);
-    if (masked) kern = hi ? decode_kernel<D, BS, CACHE, true, false, true> : decode_kernel<D, BS, CACHE, false, false, true>;
+auto pick_kernel(bool hi, bool sc, int mask) {
+    auto kern = hi ? (sc ? decode_kernel<D, BS, CACHE, true, true, 0> : decode_kernel<D, BS, CACHE, true, false, 0>)
+                   : (sc ? decode_kernel<D, BS, CACHE, false, true, 0> : decode_kernel<D, BS, CACHE, false, false, 0>);
+    if (mask == 1) kern = hi ? decode_kernel<D, BS, CACHE, true, false, 1> : decode_kernel<D, BS, CACHE, false, false, 1>;
+    if (mask == 2) kern = hi ? decode_kernel<D, BS, CACHE, true, false, 2> : decode_kernel<D, BS, CACHE, false, false, 2>;
     return kern;
 }
 
@@ -816,10 +935,10 @@ template <int D, int BS, int CACHE>
 int occupancy_t(const KernelArgs& a) {
     using Cfg = DecodeCfg<D, BS, CACHE>;
     constexpr int kMaxDevices = 64;
-    static std::atomic<int> cache[6][kMaxDevices];   // 0 = unknown, else per_sm + 1
+    static std::atomic<int> cache[8][kMaxDevices];   // 0 = unknown, else per_sm + 1
     const bool hi = a.g.Hq / a.g.Hkv > 8;
     const bool sc = a.score_raw != nullptr && a.score_aggregation_window != nullptr;
-    const int slot = (hi ? 3 : 0) + (a.m.on ? 2 : sc ? 1 : 0);
+    const int mask = mask_of(a), slot = (hi ? 4 : 0) + (mask ? 1 + mask : sc ? 1 : 0);
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const bool cached = dev >= 0 && dev < kMaxDevices;
@@ -827,7 +946,7 @@ int occupancy_t(const KernelArgs& a) {
         const int v = cache[slot][dev].load(std::memory_order_acquire);
         if (v > 0) return v - 1;
     }
-    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, a.m.on != 0);
+    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, mask_of(a));
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM) != cudaSuccess) return 0;
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kDecodeWarps * 32, Cfg::SMEM) != cudaSuccess) return 0;
@@ -841,13 +960,20 @@ cudaError_t launch_decode_t(const KernelArgs& a, cudaStream_t stream, int sm_cou
     const int G = a.g.Hq / a.g.Hkv;
     const bool hi = G > 8;
     const bool sc = a.score_raw != nullptr && a.score_aggregation_window != nullptr;
-    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, a.m.on != 0);
+    auto kern = pick_kernel<D, BS, CACHE>(hi, sc, mask_of(a));
     const int per_sm = occupancy_t<D, BS, CACHE>(a);
     if (per_sm < 1) return cudaErrorLaunchOutOfResources;
-    const long long ctas = decode_ctas(a, per_sm, sm_count);
+    long long ctas = decode_ctas(a, per_sm, sm_count);
+    KernelArgs direct;
+    if (mask_of(a) == 2) {
+        const int resident = std::min(per_sm, kDecodeMaxCtasPerSm) * sm_count * kDecodeWarps;
+        ctas = (direct_slices(a, a.g.Hkv * ((G + 15) / 16), resident).workers1 + kDecodeWarps - 1) / kDecodeWarps;
+        direct = a;
+        direct.m.direct_workers = resident;
+    }
     if (ev0) cudaEventRecord(ev0, stream);
     // (An event record in between, for the kernel timing, serialises as usual.)
-    const cudaError_t e = launch_dependent(kern, dim3((unsigned)ctas), dim3(kDecodeWarps * 32), Cfg::SMEM, stream, a);
+    const cudaError_t e = launch_dependent(kern, dim3((unsigned)ctas), dim3(kDecodeWarps * 32), Cfg::SMEM, stream, mask_of(a) == 2 ? direct : a);
     if (e != cudaSuccess) return e;
     if (ev1) cudaEventRecord(ev1, stream);
     ++*launches;

@@ -36,6 +36,7 @@ struct __align__(16) WorkerStart {
     int t0;           // row of the token in query / output
 };
 
+constexpr int kDirectMinSlice = 2;   // without a plan
 constexpr int kDecodeMinSlice = 4;   // a worker is given at least this many tiles
 constexpr int kDecodeSharedPhantom = 12;    // SM-shared decode: what one more stream in a CTA's slice costs, in tiles
 
@@ -99,6 +100,8 @@ struct MaskParams {
     long long* item_prefix;    // [q tiles + 1] tiles and phantoms in front of a q tile, of one kv head
     MaskStart* starts;         // [sm_count + 1]
     int* redo;                 // [num_tokens * Hq] rows (token * Hq + head) that are not finite and are computed again, one by one
+    int direct_tiles;          // a step of single tokens without a plan: most tiles that a stream can have; 0: with a plan
+    int direct_workers;        // and the workers among which they are cut (launch_decode fills it in)
     int rows_in_decode;        // the step has no launch for chunks: the decode kernel's warps see to those that it holds all the same
     float* part_o;             // [2 * sm_count][256][D] partial results: 2 w of CTA w's first list, if that began in front of it, 2 w + 1 of its last one
     float2* part_ml;           // [2 * sm_count][256] row maximum (base 2, scaled) and sum

@@ -166,17 +166,22 @@ class PagedAttentionExtension:
 
     def _whole(self, name: str, t, dtype: torch.dtype, shape: tuple) -> int:
         """The address of a contiguous device tensor of this type and shape."""
-        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != self._where or t.shape != shape or not t.is_contiguous():
-            self._refuse(name, t, f"contiguous {dtype} {list(shape)}")
-        return t.data_ptr()
+        try:
+            if t.dtype is dtype and t.shape == shape and t.get_device() == self.device and t.is_contiguous():
+                return t.data_ptr()
+        except (AttributeError, TypeError):
+            pass
+        self._refuse(name, t, f"contiguous {dtype} {list(shape)}")
 
     def _blocks(self, name: str, t) -> int:
         """Blocks of a cache tensor: contiguous, of any type, in the operator's layout."""
         if not self._cache_bytes:
             self._cache_bytes = self.cache_layout().key_block_bytes
-        if not isinstance(t, torch.Tensor) or t.device != self._where or not t.is_contiguous() or t.nbytes % self._cache_bytes:
-            self._refuse(name, t, f"a contiguous tensor of whole blocks of {self._cache_bytes} bytes")
-        return t.nbytes // self._cache_bytes
+        if isinstance(t, torch.Tensor) and t.get_device() == self.device and t.is_contiguous():
+            blocks, rest = divmod(t.numel() * t.element_size(), self._cache_bytes)
+            if not rest:
+                return blocks
+        self._refuse(name, t, f"a contiguous tensor of whole blocks of {self._cache_bytes} bytes")
 
     def _paged(self, inputs: dict) -> tuple:
         """Addresses of the paged metadata, number of sequences and of block indices."""
