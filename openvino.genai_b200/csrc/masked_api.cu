@@ -54,7 +54,7 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 
 // Scratch of a masked step.  No part falls where tokens, sequences or block indices grow, so the scratch of the largest step holds every smaller one.
 struct Scratch {
-    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, part_o, part_ml, total;
+    size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, cuts, part_o, part_ml, total;
 };
 // Steps of single tokens go without a plan where a stream has few tiles (under a short window, or by its block table): the plan is a launch's chain in front
 // of a kernel that is not much longer.  Longer streams are better off in the plan's slices, which know how many tiles each has.
@@ -81,6 +81,7 @@ Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     s.items = take(q_tiles * sizeof(pa::MaskItem));
     s.item_prefix = take((q_tiles + 1) * sizeof(long long));
     s.starts = take(((size_t)h->sm_count + 1) * sizeof(pa::MaskStart));
+    s.cuts = take((size_t)h->sm_count * sizeof(pa::MaskCut));
     s.part_o = take(pieces * pa::kPrefillItemRows * g.D * sizeof(float));
     s.part_ml = take(pieces * pa::kPrefillItemRows * sizeof(float2));
     s.total = off;
@@ -174,6 +175,7 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     m.items = (MaskItem*)(ws + s.items);
     m.item_prefix = (long long*)(ws + s.item_prefix);
     m.starts = (MaskStart*)(ws + s.starts);
+    m.cuts = (MaskCut*)(ws + s.cuts);
     m.redo = (int*)(ws + s.redo);
     // As many tokens as sequences: single tokens, almost always, and no launches for chunks; what of them there is beside sequences without
     // tokens, the device finds out

@@ -116,10 +116,29 @@ __device__ void build_mask_items(const KernelArgs& a, int total_p) {
     }
     __syncthreads();
     const bool cut = sh_longest > per + kMaskCut;
+    __shared__ int sh_cuts;
+    if (tid == 0) sh_cuts = 0;
     for (int w = tid; w <= ctas; w += 256) {
         long long unused;
         a.m.starts[w] = start_of(w, cut, unused);
     }
+    __syncthreads();
+    for (int w = 1 + tid; w < ctas; w += 256) {   // a list that CTA w is the first to take over in its middle
+        const MaskStart at = a.m.starts[w], before = a.m.starts[w - 1];
+        if (at.j == 0 || (before.q == at.q && before.hk == at.hk && before.j > 0)) continue;
+        const MaskItem it = a.m.items[at.q];
+        const QTile q = q_tile(a.m, it.past, it.n_new, G, it.row0, it.tree);
+        MaskCut c{it.t0, it.row0, min(kPrefillItemRows, it.n_new * G - it.row0), at.hk, w - 1, {1, 1}, 0};
+        for (int v = w; v < ctas; ++v) {
+            const MaskStart st = a.m.starts[v];
+            if (st.q != at.q || st.hk != at.hk || st.j == 0) break;
+            c.pieces[0] += st.j < q.cnt[0];
+            c.pieces[1] += st.j < q.cnt[1];
+        }
+        a.m.cuts[atomicAdd(&sh_cuts, 1)] = c;
+    }
+    __syncthreads();
+    if (tid == 0) a.plan->total_cuts = sh_cuts;
 }
 
 // Masked steps: ancestors and depths of one sequence's tree, one block of 256 threads, a token each.  Parents are in front of their children, so a

@@ -19,6 +19,7 @@ struct PlanHeader {
     int next_pitem;    // work counter of the prefill kernel: next (q tile, kv head) item to hand out
     int pitems_sorted; // 1: pitem_order lists the q tiles by decreasing context length
     int total_mitems;  // masked steps: q tiles
+    int total_cuts;    // masked steps: lists that are cut between CTAs
     int total_redo;    // masked steps: rows that are computed again
 };
 
@@ -84,8 +85,15 @@ struct __align__(16) MaskStart {
     int q, hk, j;
     int pad;
 };
+// A list that is cut between CTAs, whose pieces are joined: CTA w's last list, then the first ones of the CTAs behind it.
+struct __align__(16) MaskCut {
+    int t0, row0, rows, hk;    // of its q tile: first row of the sequence, first pair, pairs; kv head
+    int w;
+    int pieces[2];             // that hold tiles of each half's rows
+    int pad;
+};
 constexpr int kMaskPhantom = 4;   // what a q tile costs beside its tiles, in tiles: its rows' way in and out
-constexpr int kMaskLeast = 4;     // tiles that a CTA is given at least
+constexpr int kMaskLeast = 3;     // tiles that a CTA is given at least
 constexpr int kMaskCut = 14;      // what cutting lists between CTAs costs, in tiles
 constexpr int kMaskSnap = 2;      // a slice does not begin so near to either end of a q tile's list
 struct MaskParams {
@@ -99,6 +107,7 @@ struct MaskParams {
     MaskItem* items;
     long long* item_prefix;    // [q tiles + 1] tiles and phantoms in front of a q tile, of one kv head
     MaskStart* starts;         // [sm_count + 1]
+    MaskCut* cuts;             // [sm_count]
     int* redo;                 // [num_tokens * Hq] rows (token * Hq + head) that are not finite and are computed again, one by one
     int direct_tiles;          // a step of single tokens without a plan: most tiles that a stream can have; 0: with a plan
     int direct_workers;        // and the workers among which they are cut (launch_decode fills it in)
