@@ -10,8 +10,6 @@
  *   a tree of drafted tokens     position = past_len + depth in the tree; of the chunk only the row's ancestors and itself, by the same rule
  *                                with their own positions
  *
- * pa_b200_forward with sliding_window = W is the same call without sinks and without a tree.
- *
  * Blocks that no row of the step sees are neither looked up nor read: their entries of block_indices may hold anything, so that a cache
  * manager may give blocks back once the window has left them behind.  Positions that a row does not see take no part in it, whatever their bytes
  * are, not-a-number and infinities included.
@@ -48,7 +46,7 @@ typedef struct pa_mask_args {
 } pa_mask_args;
 
 /* The operator: every pointer in `args` and `mask` is device memory, query, output and the caches 16-byte aligned (PA_ERR_UNSUPPORTED
- * otherwise).  args->sliding_window is 0 or mask's.  No score output (PA_ERR_UNSUPPORTED): scores are those of causal rows.  Asynchronous on
+ * otherwise); args->sliding_window is 0, the mask has it.  No score output (PA_ERR_UNSUPPORTED): scores are those of causal rows.  Asynchronous on
  * the stream.  The handle's scratch grows when a call needs more; inside a stream capture such a call is PA_ERR_TOO_LARGE.  Graphs name the scratch
  * of their capture, which the handle keeps until it is destroyed; replays and calls of one handle stay ordered on one stream. */
 int pa_b200_forward_masked(pa_handle* h, const pa_forward_args* args, const pa_mask_args* mask);

@@ -117,7 +117,7 @@ typedef struct pa_forward_args {
     int32_t max_context_len;             /* max over sequences of past_len + new tokens */
 
     float scale;                         /* 0 => 1/sqrt(head_size) */
-    int32_t sliding_window;              /* must be 0 (PA_ERR_UNSUPPORTED otherwise) */
+    int32_t sliding_window;              /* must be 0 (PA_ERR_UNSUPPORTED otherwise): masked_b200.h has the steps with one */
     const float* alibi_slopes;           /* must be NULL */
 
     /* Eviction support (model_runner.hpp:838-848, 1483-1568).  All optional. */

@@ -111,7 +111,6 @@ int validate_masked(const pa_handle* h, const pa_forward_args* a, const pa_mask_
     if (rc != PA_OK) return rc;
     if (!m || m->struct_size != sizeof(pa_mask_args)) return fail(PA_ERR_INVALID_ARG, "pa_mask_args: NULL or struct_size mismatch");
     if (m->sliding_window < 0 || m->sink_tokens < 0) return fail(PA_ERR_INVALID_ARG, "negative sliding_window or sink_tokens");
-    if (a->sliding_window != 0 && a->sliding_window != m->sliding_window) return fail(PA_ERR_INVALID_ARG, "two different sliding windows");
     if (a->scores) return fail(PA_ERR_UNSUPPORTED, "a masked step has no score output");
     if (!(a->scale >= 0.f) || a->scale > 3.0e38f) return fail(PA_ERR_INVALID_ARG, "scale is negative or not finite");
     if (a->num_tokens == 0 || a->num_sequences == 0) return PA_OK;
@@ -207,11 +206,6 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     }
     h->launches += launches;
     return PA_OK;
-}
-
-int forward_windowed(pa_handle* h, const pa_forward_args* a, bool host) {
-    const pa_mask_args m{sizeof(pa_mask_args), a->sliding_window, 0, nullptr};
-    return host ? pa_b200_forward_masked_host(h, a, &m) : pa_b200_forward_masked(h, a, &m);
 }
 
 }  // namespace pa

@@ -131,7 +131,8 @@ int ensure_stage(pa_handle* h, size_t bytes) {
 int validate_args(const pa_handle* h, const pa_forward_args* a) {
     if (!h) return fail(PA_ERR_INVALID_ARG, "NULL handle");
     if (!a || a->struct_size != sizeof(pa_forward_args)) return fail(PA_ERR_INVALID_ARG, "pa_forward_args: NULL or struct_size mismatch");
-    if (a->sliding_window < 0) return fail(PA_ERR_INVALID_ARG, "negative sliding_window");
+    if (a->sliding_window != 0)
+        return fail(PA_ERR_UNSUPPORTED, "sliding_window is not supported by a causal step: pa_b200_forward_masked takes it, with its number of sink tokens");
     if (a->alibi_slopes != nullptr) return fail(PA_ERR_UNSUPPORTED, "alibi_slopes is not supported");
     if (a->num_tokens < 0 || a->num_sequences < 0 || a->num_blocks < 0 || a->num_block_indices < 0 || a->max_context_len < 0)
         return fail(PA_ERR_INVALID_ARG, "negative size");
@@ -333,7 +334,6 @@ int pa_b200_reserve(pa_handle* h, int32_t num_tokens, int32_t num_sequences, int
 int pa_b200_forward(pa_handle* h, const pa_forward_args* a) {
     int rc = validate_args(h, a);
     if (rc != PA_OK) return rc;
-    if (a->sliding_window > 0) return pa::forward_windowed(h, a, /*host=*/false);
     PA_CUDA(cudaSetDevice(h->device));
     cudaStream_t stream = a->stream ? (cudaStream_t)a->stream : h->stream;
     return run_forward(h, a, stream);
@@ -444,7 +444,6 @@ int pa_b200_get_kernel_timing(pa_handle* h, double* total_ms, int64_t* timed_lau
 int pa_b200_forward_host(pa_handle* h, const pa_forward_args* a) {
     int rc = validate_args(h, a);
     if (rc != PA_OK) return rc;
-    if (a->sliding_window > 0) return pa::forward_windowed(h, a, /*host=*/true);
     return pa::forward_host(h, a, nullptr);
 }
 

@@ -45,7 +45,6 @@ int validate_forward_args(const pa_handle* h, const pa_forward_args* a);
 // The host-tensor entry points; `mask` null: a causal step.
 int forward_host(pa_handle* h, const pa_forward_args* a, const pa_mask_args* mask);
 
-// masked_api.cu: a masked step of device tensors whose arguments have been checked, and pa_b200_forward's step with a sliding window.
+// masked_api.cu: a masked step of device tensors whose arguments have been checked.
 int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& mask, cudaStream_t stream);
-int forward_windowed(pa_handle* h, const pa_forward_args* a, bool host);
 }  // namespace pa

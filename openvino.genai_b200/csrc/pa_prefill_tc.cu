@@ -63,15 +63,6 @@ constexpr float kLazy = 4.f;   // log2 of the growth of a row maximum that force
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 
-#ifndef PA_X_TWO
-#define PA_X_TWO MK
-#endif
-#ifndef PA_X_NEWCONV
-#define PA_X_NEWCONV 1
-#endif
-#ifndef PA_X_CHAIN
-#define PA_X_CHAIN 1
-#endif
 constexpr int kSoftmaxWarps = 8, kConvWarps = 4;
 constexpr int kWarpMma = kSoftmaxWarps + kConvWarps, kWarpLoad = kWarpMma + 1, kWarpMma2 = kWarpMma + 2;   // the second mma warp: 16-bit caches
 constexpr int kThreads = 512;   // four warpgroups: softmax A, softmax B, converter / copy warps, {mma, loader, second mma (16-bit caches) or idle, idle}
@@ -339,7 +330,6 @@ struct MaskWalk {
         at = MaskStart{s.x, s.y, s.z, 0};
         end = MaskStart{e.x, e.y, e.z, 0};
     }
-    template <bool DUP>
     __device__ __forceinline__ bool next(const KernelArgs& a, int G, MaskedItem& it) {
         const bool last = at.q == end.q && at.hk == end.hk;
         if (at.q > end.q || (at.q == end.q && (at.hk > end.hk || (last && at.j >= end.j)))) return false;
@@ -356,7 +346,7 @@ struct MaskWalk {
         const QTile q = q_tile(a.m, it.past, it.n_new, G, it.row0, it.tree);
         it.v = q.v;
         it.lo = q.lo;
-        it.dup = DUP && q.cnt[1] == 0;
+        it.dup = q.cnt[1] == 0;
         it.ctx_hi[0] = q.ctx_hi[0];
         it.ctx_hi[1] = it.dup ? q.ctx_hi[0] : q.ctx_hi[1];
         it.nt[0] = it.dup ? (len + 1) / 2 : max(0, min(q.cnt[0], end_j) - at.j);
@@ -392,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
     // Masked: code that runs once an item stays in loops.  Straight through it is thousands of instructions that come from L2 every time: an epilogue
     // took 10 k cycles.
     constexpr int kRolled = MK ? 1 : 16;
-    constexpr bool TwoMma = !U8 || PA_X_TWO;     // a warp issues the products of each half
+    constexpr bool TwoMma = !U8 || MK;           // a warp issues the products of each half
     constexpr int kPCols = PL ? kKv : kKv / 2;   // tensor-memory columns of one half's P: f16, or bf16 high + low pieces
     constexpr int kFmt = BF ? 1 : 0;
     static_assert(!U8 || NST == 2, "the converter and the loader of the u8 variant index two stages");
@@ -417,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                 mbar_init(&sm.k_full[i], 1);
                 mbar_init(&sm.v_full[i], kConvWarps);
                 mbar_init(&sm.v_land[i], 1);
-            } else if constexpr (U8 && MK && PA_X_NEWCONV) {
+            } else if constexpr (U8 && MK) {
                 mbar_init(&sm.k_full[i], kConvWarps / 2);   // half of the converter's warps each
                 mbar_init(&sm.v_full[i], kConvWarps / 2);
             } else {
@@ -939,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                     for (int c = 0; c < kKv; ++c) sv[c] = c < nvis ? sv[c] : -INFINITY;
                 }
                 float mx = -INFINITY;
-                if constexpr (MK && PA_X_CHAIN) {   // four chains: one of 32 links is as long as the exponentials
+                if constexpr (MK) {   // four chains: one of 32 links is as long as the exponentials
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int c = 0; c < kKv; c += 2) m4[(c >> 1) & 3] = max3(m4[(c >> 1) & 3], sv[c], sv[c + 1]);
@@ -1192,7 +1182,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
         // ======================= converter: raw records -> f16 operand tiles =============================
         reg_dec<PA_TC_REG_CONV>();
         const int ctid = tid - kSoftmaxWarps * 32, cwarp = warp - kSoftmaxWarps;
-        if constexpr (U8 && MK && PA_X_NEWCONV) {
+        if constexpr (U8 && MK) {
             // Masked: two warps for the keys and two for the values, so that neither's waits and fences hold up the other's (one behind the other, keys and
             // values took 2900 cycles of a tile's 3600).  All loads of a batch of units come first, and the rare large scales (scale16) are decided once.
             const bool values = cwarp >= kConvWarps / 2;
@@ -1727,7 +1717,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                 int item;
                 It it{};
                 if constexpr (MK) {
-                    item = walk.template next<TwoMma>(a, G, it) ? 0 : -1;
+                    item = walk.next(a, G, it) ? 0 : -1;
                 } else {
                     item = atomicAdd(&a.plan->next_pitem, 1);
                     if (item >= total_items) item = -1;

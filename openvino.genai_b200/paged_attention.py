@@ -7,7 +7,7 @@ extension op would receive the same tensors in `evaluate(outputs, inputs)`
 those names and forwards to the C ABI: device tensors go to pa_b200_forward, host tensors to
 pa_b200_forward_host.  Errors raise GenaiB200Error where the reference raises ov::Exception.
 
-A step whose inputs name a `sliding_window` (with `sink_tokens`) or `tree_parents` goes to pa_b200_forward_masked
+A step whose inputs name `sink_tokens` (with `sliding_window`) or `tree_parents` goes to pa_b200_forward_masked
 (include/masked_b200.h): rows see a window of their context and its first few tokens, or the tree of drafts that they are part
 of.  `tree_accept` follows the sampled tokens down the trees behind such a step and moves what was accepted.
 """
@@ -135,14 +135,14 @@ class PagedAttentionExtension:
         """inputs / outputs are keyed by the reference's tensor names; `output` (and `scores`)
         must be preallocated by the caller, who owns every buffer.
 
-        Masks: `sliding_window` W > 0 leaves a row at position p the cached positions above p - W and, with `sink_tokens` S, those
-        below S; `tree_parents` (i32 [T], an index among the sequence's new tokens that is smaller than the token's own, -1: it follows
+        Masks: `sink_tokens` S with `sliding_window` W leaves a row at position p the cached positions above p - W and those below S (a window
+        without sinks has S = 0; without S `sliding_window` is refused, as it is of a causal step); `tree_parents` (i32 [T], an index among the sequence's new tokens that is smaller than the token's own, -1: it follows
         the last cached token, TREE_NONE at a sequence's first token: no tree) makes a sequence's new tokens a tree of drafts, whose rows
         see the cache, their ancestors and themselves, at position past_len + depth.  Blocks that no row sees are not looked up.  A step under
         a mask has no `scores`."""
-        window, sinks, parents = inputs.get("sliding_window") or 0, inputs.get("sink_tokens") or 0, inputs.get("tree_parents")
-        if window or sinks or parents is not None:
-            self._evaluate_masked(inputs, outputs, window, sinks, parents)
+        sinks, parents = inputs.get("sink_tokens"), inputs.get("tree_parents")
+        if sinks is not None or parents is not None:
+            self._evaluate_masked(inputs, outputs, inputs.get("sliding_window") or 0, sinks or 0, parents)
             return
         q = inputs["query"]
         host = isinstance(q, np.ndarray) or (isinstance(q, torch.Tensor) and not q.is_cuda)

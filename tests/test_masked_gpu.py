@@ -117,26 +117,21 @@ def test_large_queries_and_a_scale_of_ones_own():
 
 
 def test_a_window_of_the_whole_context_is_the_causal_step():
-    """pa_b200_forward by itself, with a window through its own argument, and through the masked call."""
+    """And the causal step by itself takes no window."""
     for cache in ("f16", "u8"):
         wide = H.Step([300, 40, 0], [1, 50, 20], cache=cache, window=1 << 30, seed=11)
         out, kc, vc, status = wide.run()
         assert status == 0
-        plain = H.Step([300, 40, 0], [1, 50, 20], cache=cache, seed=11)
-        ref, kc2, vc2, status = plain.run()
-        assert status == 0 and torch.equal(kc, kc2) and torch.equal(vc, vc2)
         wide.check(out)
-        plain.check(ref)
         op = wide.operator()
         x = wide.inputs(wide.packed["key"].clone(), wide.packed["value"].clone())
-        x.pop("sink_tokens"), x.pop("sliding_window")
         y = torch.zeros_like(out)
-        args = op.make_args(x["query"], x["key"], x["value"], y, x["key_cache"], x["value_cache"], x["past_lens"], x["subsequence_begins"], x["block_indices"],
-                            x["block_indices_begins"], None, 350, sliding_window=9)
-        op.forward_args(args)
+        with pytest.raises(H.pkg.GenaiB200Error, match="sink"):
+            op.evaluate({k: v for k, v in x.items() if k != "sink_tokens"}, {"output": y})
+        op.evaluate({k: v for k, v in x.items() if k not in ("sink_tokens", "sliding_window")}, {"output": y})
         torch.cuda.synchronize()
-        narrow = H.Step([300, 40, 0], [1, 50, 20], cache=cache, window=9, seed=11)
-        narrow.check(y)
+        wide.check(y)
+        assert torch.equal(x["key_cache"], kc) and torch.equal(x["value_cache"], vc)
 
 
 def test_host_tensors():
@@ -255,3 +250,64 @@ def test_chunks_beside_sequences_without_tokens(act, cache):
         past = [int(rng.integers(0, 90)) for _ in new]
         _whole(H.Step(past, new, act=act, cache=cache, window=20, sinks=2, seed=len(new)))
         _whole(H.Step(past, new, act=act, cache=cache, trees=[H.tree(rng, n) if n > 1 else None for n in new], seed=len(new)))
+
+
+def test_rows_behind_the_last_sequence_stay_as_they_were():
+    for new, trees in (([1, 1], None), ([1, 20], None), ([7, 3], [[-1, 0, 0, 1, 1, 2, 5], None])):
+        step = H.Step([50, 30, 0], new + [4], trees=trees + [None] if trees else None, window=16, seed=40)
+        op = step.operator()
+        for name in ("past_lens", "subsequence_begins", "block_indices_begins"):      # the third sequence is not told of
+            step.meta[name] = step.meta[name][:-1].contiguous()
+        out, kc, vc, status = step.run(op)
+        n = sum(new)
+        assert status in (0, 2)                 # tokens that no sequence owns may be reported
+        assert bool((out[n:] == 77).all())
+        step.check(out, rows=slice(0, n))
+
+
+@pytest.mark.parametrize("cache", ["f16", "u8"])
+def test_sequences_that_share_their_first_blocks(cache):
+    rng = np.random.default_rng(3)
+    for new, trees, window in (([1, 1, 1], None, 0), ([1, 1, 1], None, 50), ([12, 5, 1], [H.tree(rng, 12), H.tree(rng, 5), [-1]], 0), ([30, 40, 1], None, 70)):
+        step = H.Step([100, 100, 100], new, cache=cache, trees=trees, window=window, poison=False, seed=41)
+        shared = 96 // step.bs
+        for s in (1, 2):
+            a, b = int(step.first[s]), int(step.first[0])
+            step.table[a:a + shared] = step.table[b:b + shared]
+        step.meta["block_indices"] = torch.from_numpy(step.table.copy()).to(step.dev)
+        out, _, _, status = step.run()
+        assert status == 0
+        step.check(out)
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "u8")])
+def test_trees_of_one_token_in_a_step_without_a_window(act, cache):
+    past = [0, 5, 31, 32, 200, 1000, 1500]
+    _whole(H.Step(past, [1] * 7, act=act, cache=cache, trees=[[-1]] * 7, seed=42))
+    _whole(H.Step([4000, 100], [1, 1], act=act, cache=cache, trees=[[-1], None], seed=43))
+
+
+def test_blocks_of_zeros_and_rows_of_one_value():
+    """Keys that are all alike: every visible position has the same weight."""
+    for cache in ("f16", "u8"):
+        step = H.Step([77, 40], [1, 25], cache=cache, window=33, sinks=3, poison=False, seed=44)
+        for c in step.packed.values():
+            c.zero_()
+        step.key.zero_()
+        out, _, _, status = step.run()
+        assert status == 0
+        step.check(out)
+
+
+def test_a_step_of_nothing():
+    step = H.Step([10], [3], window=4, seed=45)
+    op = step.operator()
+    empty = {k: v[:0].contiguous() if k in ("query", "key", "value", "past_lens", "block_indices") else v for k, v in
+             step.inputs(step.packed["key"].clone(), step.packed["value"].clone()).items()}
+    empty["subsequence_begins"], empty["block_indices_begins"] = (torch.zeros(1, dtype=torch.int32, device=step.dev) for _ in range(2))
+    op.evaluate(empty, {"output": step.query[:0].clone()})
+    torch.cuda.synchronize()
+    assert op.device_status() == 0
+    idle = H.Step([10, 20], [0, 0], window=4, seed=46)
+    out, _, _, status = idle.run(op)
+    assert status == 0 and out.numel() == 0
