@@ -12,7 +12,8 @@
  *
  * Blocks that no row of the step sees are neither looked up nor read: their entries of block_indices may hold anything, so that a cache
  * manager may give blocks back once the window has left them behind.  Positions that a row does not see take no part in it, whatever their bytes
- * are, not-a-number and infinities included.
+ * are, not-a-number and infinities included: a row of a chunk whose result is not finite is computed again by a slow path, so that a step of which
+ * most rows rightly are not finite takes far longer than another.
  *
  * Conventions are those of pa_b200.h: plain C, status codes, the text of the last error of this thread from pa_b200_last_error(), a
  * device status word (PA_DEV_*) in place of faults.  The caller's current device is left as it was.
@@ -80,7 +81,7 @@ typedef struct pa_tree_accept_args {
     int32_t num_blocks;                  /* physical blocks in each cache tensor                                    */
     int32_t max_path;                    /* 1 .. PA_TREE_MAX_TOKENS: row length of `path`, the longest path taken   */
     int32_t num_layers;                  /* 0: nothing is moved                                                     */
-    void* const* key_caches;             /* [num_layers] host array of device pointers, 16-byte aligned             */
+    void* const* key_caches;             /* [num_layers] host array of device pointers, 16-byte aligned; no cache twice */
     void* const* value_caches;
     int32_t* path;                       /* out [num_sequences][max_path] accepted tokens, ascending; -1 behind them, and everywhere
                                           * for a sequence without a tree                                           */

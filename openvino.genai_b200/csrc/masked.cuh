@@ -152,7 +152,7 @@ static __device__ __noinline__ void masked_row(const KernelArgs& a, int t, int h
             }
             s = warp_sum(s);
             const float m_new = fmaxf(m, s);
-            const float f = m_new == -INFINITY ? 1.f : exp2f(m - m_new), p = m_new == -INFINITY ? 0.f : exp2f(s - m_new);
+            const float f = m_new == -INFINITY ? 1.f : exp2f(m - m_new), p = s == -INFINITY ? 0.f : exp2f(s - m_new);   // (an s that is not a number stays one)
             l = l * f + p;
 #pragma unroll
             for (int e = 0; e < PER; ++e) acc[e] = acc[e] * f + p * val[e];

@@ -2,7 +2,9 @@
 #include <algorithm>
 #include <climits>
 #include <cstring>
+#include <functional>
 #include <string>
+#include <vector>
 
 #include "pa_handle.h"
 #include "tensor_map.h"
@@ -264,6 +266,11 @@ int pa_b200_tree_accept(pa_handle* h, const pa_tree_accept_args* a) {
             if (!a->key_caches[i] || !a->value_caches[i]) return fail(PA_ERR_INVALID_ARG, "NULL cache pointer");
             if (!aligned(a->key_caches[i]) || !aligned(a->value_caches[i])) return fail(PA_ERR_UNSUPPORTED, "a cache is not 16-byte aligned");
         }
+        // a cache that is there twice would be moved by two blocks at once
+        std::vector<const void*> caches(a->key_caches, a->key_caches + a->num_layers);
+        caches.insert(caches.end(), a->value_caches, a->value_caches + a->num_layers);
+        std::sort(caches.begin(), caches.end(), std::less<>());
+        if (std::adjacent_find(caches.begin(), caches.end()) != caches.end()) return fail(PA_ERR_INVALID_ARG, "a cache is among the layers' twice");
         DeviceScope scope(h->device);
         MASKED_CUDA(scope.error);
         const pa::TreeAcceptArgs t{h->g, a->tree_parents, a->draft_tokens, a->sampled_tokens, a->past_lens, a->subsequence_begins, a->block_indices,

@@ -2,8 +2,8 @@
 // sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over its pieces, M the largest m_i.  A warp per row, a lane per D / 32 neighbouring elements, in the order of
 // the pieces, so that the result does not depend on who ended first.  Bound by the chain plan -> record -> pieces and by the kernel's own code, which every SM
 // has to fetch: this short loop over rows, dealt out one by one over all warps, takes 8 us for 864 rows of nine pieces, 15 us for 37,000 of two, where blocks of
-// 32 rows with their loads unrolled took 20 and 17.  Rows whose
-// result is not finite are computed again by themselves (masked_row): what they do not see may have been the cause.
+// 32 rows with their loads unrolled took 20 and 17.  Rows whose result is not finite are computed again by themselves (masked_row): what they do not
+// see may have been the cause.
 #include "masked.cuh"
 #include "pa_common.cuh"
 #include "pa_kernels.h"
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) masked_join_kernel(const _
                     const float2 w = __ldcg(reinterpret_cast<const float2*>(src));
                     v[i][0] = w.x; v[i][1] = w.y;
                 }
-                if (i0 + i >= pieces) ml[i].x = -INFINITY;
+                if (i0 + i >= pieces) ml[i] = make_float2(-INFINITY, 0.f);
             }
             float top = m;
 #pragma unroll
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) masked_join_kernel(const _
             for (int e = 0; e < PER; ++e) o[e] *= keep;
 #pragma unroll
             for (int i = 0; i < kJoinBatch; ++i) {
-                if (!(ml[i].x > -INFINITY)) continue;   // a piece of which the row sees nothing has no maximum and no weight
+                if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;   // a piece of which the row sees nothing (a sum that is not a number: it saw only such)
                 const float f = exp2f(ml[i].x - top);
                 l += f * ml[i].y;
 #pragma unroll

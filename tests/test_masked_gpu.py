@@ -311,3 +311,22 @@ def test_a_step_of_nothing():
     idle = H.Step([10, 20], [0, 0], window=4, seed=46)
     out, _, _, status = idle.run(op)
     assert status == 0 and out.numel() == 0
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "u8")])
+def test_keys_that_are_not_numbers_and_seen_reach_the_result(act, cache):
+    """Whichever piece of a cut list they fill: a piece with no other keys has no maximum, and still counts."""
+    past, trees = 64 * 30, [[-1, 0, 0, 1]]
+    whole = None
+    for first in range(0, 30, 2):
+        for tiles in (1, 3, 4):
+            step = H.Step([past], [4], hq=4, hkv=1, act=act, cache=cache, trees=trees, seed=3)
+            where = torch.zeros((step.pool, step.bs), dtype=torch.bool, device=step.dev)
+            for pos in range(64 * first, min(64 * (first + tiles), past)):
+                where[int(step.table[pos // step.bs]), pos % step.bs] = True
+            values = step.packed["value"].clone()
+            step.poison(where)
+            step.packed["value"] = values          # (of the keys alone)
+            whole = whole or step.operator()
+            out, *_, status = step.run(whole)
+            assert status == 0 and bool(out.isnan().all())

@@ -170,6 +170,9 @@ def test_refusals():
                    {"key_caches": [k.flatten()[:-16]]}, {"key_caches": [k.cpu()]}, {"past_lens": step.meta["past_lens"].long()}):
         with pytest.raises(H.pkg.GenaiB200Error):
             op.tree_accept({**good, **change}, out)
+    for twice in ({"key_caches": [k, k], "value_caches": [v, v.clone()]}, {"key_caches": [k], "value_caches": [k]}):
+        with pytest.raises(H.pkg.GenaiB200Error, match="twice"):
+            op.tree_accept({**good, **twice}, out)
     for change in ({"path": mk(1, 0)}, {"path": mk(1, 257)}, {"path": mk(2, 4)}, {"path": mk(4)}, {"num_accepted": mk(2)}, {"next_token": mk(1)}, {"new_past_lens": mk(2)}):
         with pytest.raises(H.pkg.GenaiB200Error):
             op.tree_accept(good, {**out, **change})
