@@ -122,7 +122,7 @@ struct PrefillSmem<BS, PA_DTYPE_U8, D, MK> {
     alignas(128) uint8_t raw_v[kStages][NREC * RSTRIDE];
     alignas(128) uint8_t out_stage[kSoftmaxWarps][32 * 128];   // 128 bytes of each of a warp's rows on their way to global memory
     alignas(16) uint2 v_tab[kConvWarps][kKv / 2];  // per converter warp: (scale, -1024 * scale) f16 pairs of two tokens
-    alignas(16) uint2 tok_scale[MK ? kConvWarps : 1][MK ? kKv : 1];   // masked, per converter warp: (scale, -1024 * scale) of a token, each as a pair of equal f16
+    alignas(16) uint2 tok_scale[MK ? kConvWarps : 1][MK ? kKv : 1];   // masked, per converter warp: (scale, -1152 * scale) of a token, each as a pair of equal f16
     alignas(8) uint64_t raw_full[kStages];   // loader -> converter (transaction bytes)
     alignas(8) uint64_t raw_free[kStages];   // converter -> loader
     alignas(8) uint64_t k_full[kStages];     // converter -> mma
@@ -274,11 +274,13 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
                  "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
 }
-// (1024 + byte) -> byte * scale for eight values of one scale; sc = (scale, -1024 * scale) as f16 pairs.  `slow`: the scale may be 32 or more (scale16).
+// (1024 + byte) -> (byte - 128) * scale for eight values of one scale, rounded once; sc = (scale, -1152 * scale) as f16 pairs.  `slow`: the scale may be 32
+// or more (scale16).  From the middle of the range a value loses a quarter of what it loses as byte * scale (masked u8 steps 1.0e-3 -> 6.6e-4 of the result in
+// all, f16 activations); what -1152 * scale loses in f16 is the same for every value of a token and goes with its zero-point.
 __device__ __forceinline__ void scale_pair(uint4& w4, uint2 sc, bool slow) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&w4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE400E400u), sc.x) : hfma2_bits(w[k], sc.x, sc.y);
+    for (int k = 0; k < 4; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE480E480u), sc.x) : hfma2_bits(w[k], sc.x, sc.y);
 }
 // One arrival for the whole warp, after every lane's preceding writes.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -958,15 +960,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                 for (int c = 0; c < kKv; c += 2) {
                     // the packed f16 exponential is good to 2^-9.9 relative: inside the u8 cache's error bound, not inside the
                     // f16 cache's, whose P goes through the f32 exponential and is rounded once
-                    if constexpr (MK) {   // the same, with the scaling and the row's sum two at a time
+                    if constexpr (MK) {   // of every cache, as for f16, with the scaling and the row's sum two at a time (u8 prompts 1027 us packed, 964 so)
                         const float2 x = fma_pair(sv[c], sv[c + 1], qs, -mq);
-                        if constexpr (U8) {
-                            pw[c >> 1] = ex2_h2(pack_h2(x.x, x.y));
-                        } else {
-                            const float2 p = make_float2(ex2(x.x), ex2(x.y));
-                            if constexpr (BF) l2 = add_pair(l2, p);
-                            pw[c >> 1] = BF ? pack_bf2(p.x, p.y) : pack_h2(p.x, p.y);
-                        }
+                        const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                        if constexpr (BF) l2 = add_pair(l2, p);
+                        pw[c >> 1] = BF ? pack_bf2(p.x, p.y) : pack_h2(p.x, p.y);
                     } else if constexpr (U8) {
                         pw[c >> 1] = ex2_h2(pack_h2(fmaf(sv[c], qs, -mq), fmaf(sv[c + 1], qs, -mq)));
                     } else if constexpr (BF) {
@@ -1202,7 +1200,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                     if (!wait_warp(&sm.raw_full[st], use & 1, 0)) goto done;
                     // every warp has the scales of all tokens (so that none waits for another); this thread sees to the zero-point of token gt
                     uint2* const tok = sm.tok_scale[cwarp];
-                    __half zh = __ushort_as_half(0), zm = zh, zl = zh;
+                    float scale_gt = 0.f, off_gt = 0.f, zero_gt = 0.f;   // of token gt: scale, the rounded -1152 * scale, zero-point
                     bool ok = false, big = false;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -1211,20 +1209,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                         const float* const par = reinterpret_cast<const float*>(raw + (token / BS) * Smem::RSTRIDE + BS * kD) + token % BS;
                         const __half scale = f2h(live ? par[0] : 0.f);   // (a token that no row sees becomes zeros)
                         const uint32_t s2 = h2_bits(scale, scale);
-                        tok[token] = make_uint2(s2, hmul2_bits(s2, 0xE400E400u));   // scale, -1024 * scale (exact)
+                        const uint32_t c2 = hmul2_bits(s2, 0xE480E480u);
+                        tok[token] = make_uint2(s2, c2);
                         big |= !(fabsf(__half2float(scale)) < 32.f);
                         if (token == gt) {
-                            const float z = live ? __half2float(scale) * par[BS] : 0.f;
                             ok = live;
-                            split3(values ? z : -z, zh, zm, zl);
+                            scale_gt = __half2float(scale);
+                            off_gt = __half2float(__ushort_as_half((unsigned short)(c2 & 0xffffu)));
+                            zero_gt = live ? par[BS] : 0.f;
                         }
                     }
                     const bool slow = __any_sync(0xffffffffu, big);
                     const __half zero = __ushort_as_half(0);
+                    // (byte - zp) * scale = operand - z: z = (zp - 128) * scale and what the offset was rounded by (scale * 1024 + offset is exact)
+                    const float z = fmaf(scale_gt, zero_gt, slow ? -128.f * scale_gt : fmaf(scale_gt, 1024.f, off_gt));
+                    __half zh, zm, zl;
+                    split3(values ? z : -z, zh, zm, zl);
                     __syncwarp();
                     if (!values) {
                         if (use > 0 && !wait_warp(&sm.k_free[st], (use - 1) & 1, 1)) goto done;
-                        // K' = byte * f16(k scale): unit = 16 dims of one token
+                        // K' = (byte - 128) * f16(k scale): unit = 16 dims of one token
                         *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 0)) = make_uint4(h2_bits(zh, zm), h2_bits(zl, zh), h2_bits(zm, zero), 0u);
                         *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 1)) = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
@@ -1251,9 +1255,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                         warp_arrive(&sm.k_full[st]);
                     } else {
                         if (use > 0 && !wait_warp(&sm.v_free[st], (use - 1) & 1, 2)) goto done;
-                        // V'^T = byte * f16(v scale): unit = 16 tokens of one dim
+                        // V'^T = (byte - 128) * f16(v scale): unit = 16 tokens of one dim
                         const int tg = gt & 3;
-                        uint2 tab[8];   // of two tokens: their scales, and -1024 times them
+                        uint2 tab[8];   // of two tokens: their scales, and -1152 times them
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const uint4 two = *reinterpret_cast<const uint4*>(&tok[16 * tg + 2 * k]);
@@ -1271,7 +1275,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                                 const int d = d0 + 16 * i;
                                 uint32_t w[8] = {lo4[i].x, lo4[i].y, lo4[i].z, lo4[i].w, hi4[i].x, hi4[i].y, hi4[i].z, hi4[i].w};
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE400E400u), tab[k].x) : hfma2_bits(w[k], tab[k].x, tab[k].y);
+                                for (int k = 0; k < 8; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE480E480u), tab[k].x) : hfma2_bits(w[k], tab[k].x, tab[k].y);
                                 *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg)) = make_uint4(w[0], w[1], w[2], w[3]);
                                 *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
                             }
