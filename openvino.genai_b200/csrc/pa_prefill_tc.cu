@@ -37,7 +37,8 @@
 // Masked steps (MK; include/masked_b200.h): a CTA has a slice of the q tiles' lists of context tiles (build_mask_items) and no counter; a tile of which a row
 // sees a part takes that part from a word of bits; tokens that no row of the item sees go in as zeros and their blocks are not looked up; a piece
 // leaves its rows' sums, maxima and unnormalised results to masked_join_kernel.  Few rows (one half's worth) are worked on by both halves, a tile each in
-// turn.  The u8 cache has a warp for each half's products here too, S of a tile ahead of the P.V before it.
+// turn.  The u8 cache has a warp for each half's products here too, S of a tile ahead of the P.V before it, and a pair of converter warps each for keys and
+// values; the 16-bit caches' operand tiles are the loader's tensor copies, and the four warps beside it clear value rows that no row of the item sees.
 // Tensor-bound for long contexts: 4 * Hq * D flops per (new token, context token) pair.
 #include <algorithm>
 #include <cstdio>
