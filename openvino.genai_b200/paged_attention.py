@@ -34,11 +34,16 @@ def _ptr(t) -> Optional[int]:
     return t.data_ptr()
 
 
+_nbytes = operator.attrgetter("nbytes")
+
+
 def _alike(tensors) -> bool:
-    """Whether all of them are contiguous tensors of one type, size and device."""
+    """Whether all of them are contiguous tensors of one size in bytes on one device."""
     T = torch.Tensor
-    return set(map(type, tensors)) <= {T} and all(map(T.is_contiguous, tensors)) and \
-        max(len(set(map(f, tensors))) for f in (T.get_device, T.numel, operator.attrgetter("dtype"))) <= 1
+    try:
+        return all(map(T.is_contiguous, tensors)) and len(set(map(T.get_device, tensors))) <= 1 and len(set(map(_nbytes, tensors))) <= 1
+    except TypeError:    # (not all of them are tensors)
+        return False
 
 
 class PagedAttentionExtension:
