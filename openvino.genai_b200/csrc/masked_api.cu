@@ -191,8 +191,8 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     int launches = 0;
     if (a->num_rotated_blocks > 0) { MASKED_CUDA(launch_rotate(k, stream)); ++launches; }
     MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;
-    // (the new tokens of a single sequence are its chunk: no row for the decode kernel, whose empty launch is 2 us of a tree's 30)
-    if (a->num_tokens == 1 || a->num_sequences > 1) MASKED_CUDA(launch_decode(k, stream, h->sm_count, &launches));
+    // (always: among the tokens that no sequence has, even a step of one sequence may hold a single token)
+    MASKED_CUDA(launch_decode(k, stream, h->sm_count, &launches));
     if (a->num_tokens > 1 && !m.rows_in_decode) {
         if (prefill_tc_supported(h->g)) {
             if (h->g.cache != PA_DTYPE_U8) {

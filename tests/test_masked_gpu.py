@@ -330,3 +330,42 @@ def test_keys_that_are_not_numbers_and_seen_reach_the_result(act, cache):
             whole = whole or step.operator()
             out, *_, status = step.run(whole)
             assert status == 0 and bool(out.isnan().all())
+
+
+@pytest.mark.parametrize("new", [[1], [3], [1, 1, 2], [0, 1]])
+def test_steps_padded_with_tokens_of_no_sequence(new):
+    """More rows than the sequences have, and as many rows as sequences though none has just one."""
+    step = H.Step([30 + 7 * i for i in range(len(new))], new, window=20, sinks=3, seed=len(new) + sum(new))
+    for rows in (step.T + 1, step.T + 4, len(new) + 3):
+        pad = rows - step.T
+        if pad <= 0:
+            continue
+        op, (kc, vc) = step.operator(), (step.packed["key"].clone(), step.packed["value"].clone())
+        given = step.inputs(kc, vc)
+        for name in ("query", "key", "value"):
+            given[name] = torch.cat([given[name], given[name].new_full((pad, given[name].shape[1]), float("nan"))])
+        out = torch.full((rows, step.hq * step.d), 77.0, dtype=torch.float16, device=step.dev)
+        op.evaluate(given, {"output": out})
+        torch.cuda.synchronize()
+        assert op.device_status() in (0, 2)     # tokens that no sequence owns may be reported
+        step.check(out[:step.T])
+        assert bool((out[step.T:] == 77).all())
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "f16"), ("f16", "u8"), ("f32", "bf16")])
+def test_begins_that_go_back_are_reported(act, cache):
+    """The same tokens given to several sequences: more q tiles than tokens make."""
+    past, n = [40] * 9, 300
+    step = H.Step(past, [n] + [0] * 8, hq=8, hkv=2, act=act, cache=cache, window=64, seed=50, spare_blocks=400)
+    op = step.operator()
+    good, blocks = dict(step.meta), (past[0] + n + step.bs - 1) // step.bs
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=step.dev)
+    step.meta["subsequence_begins"] = i32([0, n] * 5)          # 0 .. n, back, 0 .. n, back, ...
+    step.meta["block_indices"] = i32([(s * blocks + b) % step.pool for s in range(9) for b in range(blocks)])
+    step.meta["block_indices_begins"] = i32([s * blocks for s in range(10)])
+    out, *_, status = step.run(op)
+    assert status & 2
+    step.meta = good
+    out, *_, status = step.run(op)
+    assert status == 0
+    step.check(out)
