@@ -182,12 +182,13 @@ __device__ void build_decode_plan(const KernelArgs& a) {
     __shared__ int sh_run;
     __shared__ int sh_warp_p[8];
     __shared__ int sh_run_p;
+    __shared__ int sh_warp_end[8], sh_end;     // masked: behind the last token of the sequences so far
     constexpr int kPrefixCap = 2048;           // rows whose prefix sums are also kept in shared memory
     __shared__ int sh_prefix[kPrefixCap + 1];
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int B = a.num_sequences;
     const int G = a.g.Hq / a.g.Hkv, HK = a.g.Hkv * ((G + 15) / 16);
-    if (tid == 0) { sh_run = 0; sh_run_p = 0; }
+    if (tid == 0) { sh_run = 0; sh_run_p = 0; sh_end = 0; }
     __syncthreads();
     for (int base = 0; base < B; base += 256) {
         const int s = base + tid;
@@ -201,6 +202,26 @@ __device__ void build_decode_plan(const KernelArgs& a) {
                 atomicOr(a.status, PA_DEV_BAD_TREE);
                 np = 0;
             }
+        }
+        if (a.m.on) {
+            // a chunk whose tokens are another's too (begins that go back) is left out: the scratch holds as many q tiles and rows as tokens make
+            SeqView sv;
+            const bool ok = s < B && seq_view(a, s, sv);
+            int end = ok ? sv.t0 + sv.n : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) end = max(end, __shfl_up_sync(0xffffffffu, end, o));   // (lanes without a lower one get their own)
+            int before = __shfl_up_sync(0xffffffffu, end, 1);
+            if (lane == 0) before = 0;
+            if (lane == 31) sh_warp_end[wid] = end;
+            __syncthreads();
+            before = max(before, sh_end);
+            for (int w = 0; w < wid; ++w) before = max(before, sh_warp_end[w]);
+            if (np > 0 && sv.t0 < before) {
+                atomicOr(a.status, PA_DEV_BAD_BEGINS);
+                np = 0;
+            }
+            __syncthreads();
+            if (tid == 255) sh_end = max(before, end);
         }
         int v = n, vp = np;
 #pragma unroll
