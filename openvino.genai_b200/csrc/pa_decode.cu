@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     const float sm_scale = a.scale != 0.f ? a.scale : rsqrtf((float)D);
     const bool q_pairs = (reinterpret_cast<uintptr_t>(a.query) & 7) == 0;   // a pair of elements is one aligned load
     bool bad_index = false;
-    // everything below reads what the launch before this one wrote (plan, start records, cache; without a plan the newest token of the cache alone)
+    // everything below reads what the launch before this one wrote (plan, start records, cache; without a plan the cache alone)
     bool waited = !DIRECT;
     if (!DIRECT) grid_wait();
     auto wait_once = [&] {
@@ -370,10 +370,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             if constexpr (!U8) cp_async_commit();
             return;
         }
-        // the tile with the new token, which the cache write puts there
-        if constexpr (DIRECT) {
-            if (r_tok + kTile >= r_tiles * kTile) wait_once();
-        }
+        // The cache is read once the new tokens are written: a row may see those of other sequences over the same blocks.  (Only the tile with the row's own
+        // new token behind the wait is no faster: 16.5 and 28.7 us either way.)
+        if constexpr (DIRECT) wait_once();
         uint8_t* st = ring + slot * Cfg::STAGE;
         const int hk = r_hkp / gtiles;
         const uint8_t* kc = (const uint8_t*)a.key_cache + (long long)hk * a.g.head_bytes;

@@ -369,3 +369,57 @@ def test_begins_that_go_back_are_reported(act, cache):
     out, *_, status = step.run(op)
     assert status == 0
     step.check(out)
+
+
+@pytest.mark.parametrize("cache", ["f16", "u8"])
+def test_rotated_blocks_are_rotated_first(cache):
+    """Keys that the step rotates are rotated for its rows, as in a causal step."""
+    for new in ([1, 1, 1], [1, 30, 5]):
+        step = H.Step([200, 90, 140], new, cache=cache, window=1 << 30, sinks=2, seed=61)
+        op, dev = step.operator(), step.dev
+        angle = torch.rand(9, step.d // 2, device=dev)
+        blocks = torch.tensor([int(step.table[step.first[s] + b]) for s, b in ((0, 0), (0, 3), (1, 2), (2, 7))], dtype=torch.int32, device=dev)
+        extra = {"rotated_block_indices": blocks, "rotation_deltas": torch.tensor([[1], [7], [2], [5]], dtype=torch.int32, device=dev),
+                 "rotation_trig_lut": torch.cat([angle.cos(), angle.sin()], 1).contiguous()}
+        got = []
+        for masked in (True, False):
+            kc, vc = step.packed["key"].clone(), step.packed["value"].clone()
+            given = {**step.inputs(kc, vc), **extra}
+            if not masked:
+                del given["sliding_window"], given["sink_tokens"]
+            out = torch.zeros((step.T, step.hq * step.d), dtype=torch.float16, device=dev)
+            op.evaluate(given, {"output": out})
+            torch.cuda.synchronize()
+            assert op.device_status() == 0
+            got.append((out.double(), kc, vc))
+        assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2])
+        assert not torch.equal(got[0][1], step.cache_after()[0])
+        # each side is within the tolerance that a row has against the definition
+        tol = 2 * 4 * {"f16": 2e-3, "u8": 1e-2}[cache]
+        heads = lambda y: y.view(-1, step.hq, step.d)
+        assert bool((heads(got[0][0] - got[1][0]).norm(dim=-1) <= tol * heads(got[1][0]).norm(dim=-1)).all())
+
+
+@pytest.mark.parametrize("hq,d,bs", [(8, 64, 16), (8, 128, 32)])
+def test_rows_that_see_each_others_new_tokens(hq, d, bs):
+    """Single tokens given as sequences of their own over the same blocks: every new token is written before a row reads it."""
+    for last in (30, 31, 32, 63, 64):        # positions last .. last + 3, tiles of 32 end among them
+        rows = 4
+        one = H.Step([last], [rows], hq=hq, d=d, bs=bs, window=1 << 20, sinks=1, seed=70 + last)
+        op = one.operator()
+        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=one.dev)
+        blocks = one.meta["block_indices"].numel()
+        for window in (1 << 20, 50):
+            one.window, one.sinks = window, 1
+            one.sees = [one.seen(0)]
+            kc, vc = one.packed["key"].clone(), one.packed["value"].clone()
+            given = {**one.inputs(kc, vc), "sliding_window": window, "sink_tokens": 1, "past_lens": i32([last + i for i in range(rows)]),
+                     "subsequence_begins": i32(list(range(rows + 1))), "block_indices": one.meta["block_indices"].repeat(rows),
+                     "block_indices_begins": i32([i * blocks for i in range(rows + 1)])}
+            out = torch.zeros((rows, one.hq * one.d), dtype=torch.float16, device=one.dev)
+            for _ in range(20):
+                kc.copy_(one.packed["key"]); vc.copy_(one.packed["value"])
+                op.evaluate(given, {"output": out})
+                torch.cuda.synchronize()
+                assert op.device_status() == 0
+                one.check(out)
