@@ -102,13 +102,14 @@ __global__ void __launch_bounds__(kMoveThreads) tree_move_kernel(const __grid_co
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kMoveWarps = kMoveThreads / 32;
     static_assert(kMoveThreads == kTreeMax, "a thread per place of a path");
-    const int tb = a.block_indices_begins[s], count = a.num_accepted[s];
+    const int tb = a.block_indices_begins[s], pages = a.block_indices_begins[s + 1] - tb, count = a.num_accepted[s];
     const int from = tid < a.max_path ? a.path[(long long)s * a.max_path + tid] : -1;   // (-1 everywhere without a tree, and where the metadata are bad)
     const int past = a.past_lens[s] - (a.new_past_lens == a.past_lens ? count : 0);     // (the walk has written the new ones)
     int src = -1, dst = -1;
     if (from >= 0 && from != tid) {
         const int p0 = past + from, p1 = past + tid;
-        const int b0 = a.block_indices[tb + p0 / BS], b1 = a.block_indices[tb + p1 / BS];
+        const bool inside = past >= 0 && from < kTreeMax && p0 / BS < pages && p1 / BS < pages;   // (as the walk has checked, if its outputs are still its own)
+        const int b0 = inside ? a.block_indices[tb + p0 / BS] : -1, b1 = inside ? a.block_indices[tb + p1 / BS] : -1;
         if (b0 < 0 || b0 >= a.num_blocks || b1 < 0 || b1 >= a.num_blocks) {
             if (blockIdx.y == 0) atomicOr(a.status, PA_DEV_BAD_BLOCK_INDEX);
         } else {
