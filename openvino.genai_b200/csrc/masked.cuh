@@ -61,10 +61,16 @@ __device__ __forceinline__ RowMask row_mask(const KernelArgs& a, int t0, int pas
     const int t = t0 + tok;
     return RowMask{past, window_lo(a.m, past + __ldcg(a.m.tree_depth + t) + 1), a.m.tree_words + (long long)t * kTreeWords, past};
 }
-__device__ __forceinline__ uint32_t row_bits32(const KernelArgs& a, const RowMask& r, int pos0) {
-    uint32_t w = causal_bits32(pos0, r.ctx, r.lo, a.m.sinks);
+__host__ __device__ __forceinline__ uint32_t row_bits32(const MaskParams& m, const RowMask& r, int pos0) {
+    uint32_t w = causal_bits32(pos0, r.ctx, r.lo, m.sinks);
     if (r.words && pos0 + 32 > r.past) w |= tree_bits32(r.words, pos0 - r.past);
     return w;
+}
+// The tiles that one row of a chunk of n tokens goes through.  A tree's whole chunk is among them, however far the row's window has come: its tokens are seen by
+// their positions, and an ancestor whose position is below the sinks may lie anywhere in the chunk.
+template <int T>
+__host__ __device__ __forceinline__ VisTiles row_tiles(const MaskParams& m, const RowMask& r, int n) {
+    return r.words ? vis_tiles<T>(r.past + n, r.lo < r.past ? r.lo : r.past, m.sinks) : vis_tiles<T>(r.ctx, r.lo, m.sinks);
 }
 
 __device__ __forceinline__ bool has_tree(const KernelArgs& a, int t0, int n) { return a.m.parents && n > 0 && a.m.parents[t0] != kTreeNone; }
@@ -118,10 +124,10 @@ static __device__ __noinline__ void masked_row(const KernelArgs& a, int t, int h
         acc[i] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
-    const VisTiles v = vis_tiles<32>(tree ? sv.past + sv.n : rm.ctx, rm.lo, a.m.sinks);
+    const VisTiles v = row_tiles<32>(a.m, rm, sv.n);
     for (int i = 0; i < v.count; ++i) {
         const int pos0 = 32 * v.tile(i);
-        for (uint32_t w = row_bits32(a, rm, pos0); w; w &= w - 1) {
+        for (uint32_t w = row_bits32(a.m, rm, pos0); w; w &= w - 1) {
             const int pos = pos0 + __ffs(w) - 1;
             const int blk = a.block_indices[sv.tb + pos / bs];
             if (blk < 0 || blk >= a.num_blocks) {
