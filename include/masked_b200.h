@@ -87,8 +87,9 @@ typedef struct pa_tree_accept_args {
     void* const* value_caches;
     int32_t* path;                       /* out [num_sequences][max_path] accepted tokens, ascending; -1 behind them, and everywhere
                                           * for a sequence without a tree                                           */
-    int32_t* num_accepted;               /* out [num_sequences]; all tokens of a sequence without a tree; 0: the sequence has no tokens, or a
-                                          * tree or metadata that set the status word                               */
+    int32_t* num_accepted;               /* out [num_sequences]; all tokens of a sequence without a tree; 0: the sequence has no tokens, or metadata
+                                          * or a tree that set the status word: too many tokens, or any parent out of range (of which the attention
+                                          * makes a follower of the cache; here nothing of such a tree is accepted or moved) */
     int64_t* next_token;                 /* out [num_sequences] id sampled behind the last accepted token, -1: none */
     int32_t* new_past_lens;              /* out [num_sequences] past_len + num_accepted, or NULL; may be past_lens  */
     void* stream;                        /* cudaStream_t, NULL => the handle's stream */

@@ -33,15 +33,18 @@ __global__ void __launch_bounds__(kTreeMax) tree_walk_kernel(TreeAcceptArgs a) {
     SeqView v;
     accept_view(a, s, v, i == 0);
     const bool tree = v.n > 0 && a.parents[v.t0] != kTreeNone;
-    const bool walk = tree && v.n <= kTreeMax;
-    if (tree && !walk && i == 0) atomicOr(a.status, PA_DEV_BAD_TREE);
     int parent = -1;
     int64_t draft = 0;
-    if (walk && i < v.n) {
+    bool bad = tree && v.n > kTreeMax;
+    if (tree && !bad && i < v.n) {
         parent = a.parents[v.t0 + i];
         draft = a.draft[v.t0 + i];
-        if (parent < -1 || parent >= i) { atomicOr(a.status, PA_DEV_BAD_TREE); parent = -1; }
+        bad = parent < -1 || parent >= i;
     }
+    // one parent that is none: who knows what the drafts were judged by, so none of them is accepted and nothing is moved
+    bad = __syncthreads_or(bad) != 0;
+    if (bad && i == 0) atomicOr(a.status, PA_DEV_BAD_TREE);
+    const bool walk = tree && !bad;
     int32_t* path = a.path + (long long)s * a.max_path;
     int at = walk ? 0 : -1, count = 0;
     if (i == 0) sh_next[0] = kTreeMax;   // (turn 0's)

@@ -1,0 +1,29 @@
+"""Acceptance of drafted trees on the GPU: corrupt trees, and calls that are refused."""
+import numpy as np
+import pytest
+import torch
+
+from tests import masked_harness as H
+from tests.test_tree_accept_gpu import _run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("at,bad", [(0, 0), (0, 7), (2, 2), (3, 4), (4, 5), (5, 100), (1, -2), (5, -3), (3, -2147483648), (2, 2147483647)])
+def test_a_tree_with_a_bad_parent_is_not_walked(at, bad):
+    """On the path (tokens 0, 2, 3) or beside it: nothing of its sequence is accepted, the others' are."""
+    trees = [[-1, 0, 1], [-1, 0, 0, 2, 1, 1], [-1, 0]]
+    step = H.Step([20, 33, 40], [3, 6, 2], d=64, bs=16, trees=trees, poison=False, seed=1)
+    step.parents[3 + at] = bad
+    draft = np.array([1, 2, 3, 10, 11, 12, 13, 14, 15, 1, 2])
+    sampled = np.array([2, 3, 4, 12, 0, 13, 99, 0, 0, 2, 77])
+    for in_place in (False, True):
+        out, keys, values, before, status = _run(step, draft, sampled, 4, in_place=in_place)
+        assert status == H.M.PA_DEV_BAD_TREE
+        assert out["num_accepted"].tolist() == [3, 0, 2] and out["next_token"].tolist() == [4, -1, 77] and out["new_past_lens"].tolist() == [23, 33, 42]
+        assert out["path"].tolist() == [[0, 1, 2, -1], [-1] * 4, [0, 1, -1, -1]]
+        for i in range(2):
+            assert torch.equal(keys[i], before[i][0]) and torch.equal(values[i], before[i][1])
+    step.parents[3 + at] = trees[1][at]
+    out, _, _, _, status = _run(step, draft, sampled, 4)
+    assert status == 0 and out["num_accepted"].tolist() == [3, 3, 2] and out["next_token"].tolist() == [4, 99, 77]
