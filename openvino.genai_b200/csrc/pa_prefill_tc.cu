@@ -1208,7 +1208,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                         const int token = 32 * h + lane;
                         const bool live = seen(it, ctx_hi, pos0 + token);
                         const float* const par = reinterpret_cast<const float*>(raw + (token / BS) * Smem::RSTRIDE + BS * kD) + token % BS;
-                        const __half scale = f2h(live ? par[0] : 0.f);   // (a token that no row sees becomes zeros)
+                        __half scale = f2h(live ? par[0] : 0.f);   // (a token that no row sees becomes zeros)
+                        // -128 * scale leaves the f16 range from 512 on.  Of a key that would be a logit of -infinity, which hides the token as a mask does: not a
+                        // number instead, so that the rows that see it are computed again in 32 bits (masked_row).
+                        if (!(fabsf(__half2float(scale)) < 512.f)) scale = __ushort_as_half(0x7FFFu);
                         const uint32_t s2 = h2_bits(scale, scale);
                         const uint32_t c2 = hmul2_bits(s2, 0xE480E480u);
                         tok[token] = make_uint2(s2, c2);
