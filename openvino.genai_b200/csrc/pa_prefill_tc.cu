@@ -380,13 +380,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
     using It = typename ItemOf<MK>::type;
     constexpr bool U8 = CT == PA_DTYPE_U8, BF = CT == PA_DTYPE_BF16;
     constexpr int kD = D, kNo = Smem::NO, kTmemP = 2 * kKv + 2 * kNo, NST = Smem::NST;
-    constexpr bool PL = BF && !MK;               // P as two bf16 pieces.  (Masked steps: one, as in the decode kernel: P's 2^-9 beside the output's own, 2.3e-3 of the
-                                                 // result in all instead of 1.7e-3, for a third of the products)
     // Masked: code that runs once an item stays in loops.  Straight through it is thousands of instructions that come from L2 every time: an epilogue
     // took 10 k cycles.
     constexpr int kRolled = MK ? 1 : 16;
     constexpr bool TwoMma = !U8 || MK;           // a warp issues the products of each half
-    constexpr int kPCols = PL ? kKv : kKv / 2;   // tensor-memory columns of one half's P: f16, or bf16 high + low pieces
+    // tensor-memory columns of one half's P: f16, or bf16 high + low pieces.  (One bf16 piece leaves 2.3e-3 of the result in all where two leave the output's own
+    // 1.7e-3; it costs a third of the products: masked ragged prompts 369 | 310 us, long trees 292 | 268.)
+    constexpr int kPCols = BF ? kKv : kKv / 2;
     constexpr int kFmt = BF ? 1 : 0;
     static_assert(!U8 || NST == 2, "the converter and the loader of the u8 variant index two stages");
     static_assert(kTmemP + 2 * kPCols <= kTmemCols, "S, O and P of both halves fit the tensor memory");
@@ -956,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                 [[maybe_unused]] float2 l2 = make_float2(0.f, 0.f);
                 const float mq = MK && m_run == -INFINITY ? 0.f : m_run * qs;   // (nothing seen yet: every p is 0)
                 uint32_t pw[kKv / 2];
-                uint32_t pl[PL ? kKv / 2 : 1];   // bf16 variant: the low pieces, p = high + low up to 2^-17 p
+                uint32_t pl[BF ? kKv / 2 : 1];   // bf16 variant: the low pieces, p = high + low up to 2^-17 p
 #pragma unroll
                 for (int c = 0; c < kKv; c += 2) {
                     // the packed f16 exponential is good to 2^-9.9 relative: inside the u8 cache's error bound, not inside the
@@ -964,8 +964,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                     if constexpr (MK) {   // of every cache, as for f16, with the scaling and the row's sum two at a time (u8 prompts 1027 us packed, 964 so)
                         const float2 x = fma_pair(sv[c], sv[c + 1], qs, -mq);
                         const float2 p = make_float2(ex2(x.x), ex2(x.y));
-                        if constexpr (BF) l2 = add_pair(l2, p);
-                        pw[c >> 1] = BF ? pack_bf2(p.x, p.y) : pack_h2(p.x, p.y);
+                        if constexpr (BF) {
+                            l2 = add_pair(l2, p);
+                            const uint32_t hi = pack_bf2(p.x, p.y);
+                            pw[c >> 1] = hi;
+                            pl[c >> 1] = pack_bf2(p.x - __uint_as_float(hi << 16), p.y - __uint_as_float(hi & 0xffff0000u));
+                        } else {
+                            pw[c >> 1] = pack_h2(p.x, p.y);
+                        }
                     } else if constexpr (U8) {
                         pw[c >> 1] = ex2_h2(pack_h2(fmaf(sv[c], qs, -mq), fmaf(sv[c + 1], qs, -mq)));
                     } else if constexpr (BF) {
@@ -973,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                         l_own += p0 + p1;
                         const uint32_t hi = pack_bf2(p0, p1);
                         pw[c >> 1] = hi;
-                        if constexpr (PL) pl[c >> 1] = pack_bf2(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+                        pl[c >> 1] = pack_bf2(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
                     } else {
                         pw[c >> 1] = pack_h2(ex2(fmaf(sv[c], qs, -mq)), ex2(fmaf(sv[c + 1], qs, -mq)));
                     }
@@ -1013,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                     tc05::wait_st();
                 }
                 tc05::st_32x32b_x32(tmem_p, pw);   // row r of the A operand: lane r, two tokens per column
-                if constexpr (PL) tc05::st_32x32b_x32(tmem_p + kKv / 2, pl);
+                if constexpr (BF) tc05::st_32x32b_x32(tmem_p + kKv / 2, pl);
                 tc05::wait_st();
                 tc05::fence_before_thread_sync();
                 warp_arrive(&sm.p_full[X]);
@@ -1558,13 +1564,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
 #pragma unroll
                     for (int kk = 1; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + 8 * kk, db0 + 2 * kk, idesc_o);
                 } else if constexpr (BF) {
-                    // high pieces of P, then the low pieces (where there are any) against the same value rows
+                    // high pieces of P, then the low pieces against the same value rows
                     if (acc) tc05::mma_ts<1>(d, pa, db0, idesc_o);
                     else tc05::mma_ts<0>(d, pa, db0, idesc_o);
 #pragma unroll
                     for (int kk = 1; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + 8 * kk, db0 + 128 * kk, idesc_o);
 #pragma unroll
-                    for (int kk = 0; kk < (PL ? kKv / 16 : 0); ++kk) tc05::mma_ts<1>(d, pa + kKv / 2 + 8 * kk, db0 + 128 * kk, idesc_o);
+                    for (int kk = 0; kk < kKv / 16; ++kk) tc05::mma_ts<1>(d, pa + kKv / 2 + 8 * kk, db0 + 128 * kk, idesc_o);
                 } else {
                     // 16 tokens further along K = 16 rows of 128 bytes; the denominators go to the 16 columns after O
                     if (acc) { tc05::mma_ts<1>(d, pa, db0, idesc_o); tc05::mma_ts<1>(d + kD, pa, dones, idesc_l); }

@@ -1,0 +1,21 @@
+"""Masked attention on the GPU: how many bits of its numbers survive, where a looser tolerance would not tell."""
+import numpy as np
+import pytest
+import torch
+
+from tests import masked_harness as H
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 32)])
+def test_bf16_chunks_are_as_exact_as_a_causal_step(d, bs):
+    """The operator's tolerance for 16-bit caches, 2e-3 of the result as a whole.  The output's own rounding takes 1.7e-3 of it (a relative error that is spread
+    evenly over half a step of 2^-8 .. 2^-9 has a root mean square of 1.66e-3), so probabilities of 8 bits, another 1.6e-3 of the same kind, do not fit."""
+    rng = np.random.default_rng(1)
+    for past, new, trees, window in (([700, 90], [200, 64], None, 300), ([3000], [100], [H.tree(rng, 100)], 0), ([2, 40], [300, 77], None, 20)):
+        step = H.Step(past, new, d=d, bs=bs, act="bf16", cache="bf16", window=window, trees=trees, seed=window)
+        out, _, _, status = step.run()
+        ref, _ = step.reference()
+        err = ((out.double() - ref).norm() / ref.norm()).item()
+        assert status == 0 and err <= 2e-3, err
