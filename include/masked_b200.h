@@ -57,7 +57,9 @@ int pa_b200_forward_masked(pa_handle* h, const pa_forward_args* args, const pa_m
 /* The same for host tensors, as pa_b200_forward_host takes them (the caches stay device memory). */
 int pa_b200_forward_masked_host(pa_handle* h, const pa_forward_args* args, const pa_mask_args* mask);
 
-/* Grows the scratch for masked calls of up to so many tokens, sequences and block indices, which then do not allocate. */
+/* Grows the scratch for masked calls of up to so many tokens, sequences and block indices (which take none), which then do not allocate.  From two tokens on it holds
+ * what chunks take, 39 MB for the tensor cores' partial results at a head size of 128; a handle whose steps are all of single tokens does not take them
+ * by itself.  Layers of one geometry whose steps follow one another on one stream can share a handle. */
 int pa_b200_masked_reserve(pa_handle* h, int32_t num_tokens, int32_t num_sequences, int32_t num_block_indices);
 
 /* Judges trees of drafts and makes the accepted ones the cache's newest tokens.

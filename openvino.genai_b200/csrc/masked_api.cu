@@ -54,7 +54,7 @@ struct DeviceScope {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Scratch of a masked step.  No part falls where tokens, sequences or block indices grow, so the scratch of the largest step holds every smaller one.
+// Scratch of a masked step.  No part falls where tokens or sequences grow, so what is reserved for the largest step holds every smaller one.
 struct Scratch {
     size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, cuts, part_o, part_ml, total;
 };
@@ -62,7 +62,9 @@ struct Scratch {
 // of a kernel that is not much longer.  Longer streams are better off in the plan's slices, which know how many tiles each has.
 constexpr int kDirectTiles = 64;
 
-Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
+// The partial results of the tensor-core kernel's CTAs, by far the largest part (39 MB at a head size of 128), come last and are there where it is launched: not in
+// `rows_only`, a step of as many tokens as sequences.
+Scratch plan_scratch(const pa_handle* h, int tokens, int sequences, bool rows_only) {
     const pa::CacheGeom& g = h->g;
     const int G = g.Hq / g.Hkv, HK = g.Hkv * ((G + 15) / 16), RT = std::min(G, 16);
     Scratch s{};
@@ -84,8 +86,10 @@ Scratch plan_scratch(const pa_handle* h, int tokens, int sequences) {
     s.item_prefix = take((q_tiles + 1) * sizeof(long long));
     s.starts = take(((size_t)h->sm_count + 1) * sizeof(pa::MaskStart));
     s.cuts = take((size_t)h->sm_count * sizeof(pa::MaskCut));
-    s.part_o = take(pieces * pa::kPrefillItemRows * g.D * sizeof(float));
-    s.part_ml = take(pieces * pa::kPrefillItemRows * sizeof(float2));
+    if (!rows_only && tokens > 1 && pa::prefill_tc_supported(g)) {
+        s.part_o = take(pieces * pa::kPrefillItemRows * g.D * sizeof(float));
+        s.part_ml = take(pieces * pa::kPrefillItemRows * sizeof(float2));
+    }
     s.total = off;
     return s;
 }
@@ -131,7 +135,7 @@ namespace pa {
 
 int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& mask, cudaStream_t stream) {
     if (a->num_sequences == 0 || a->num_tokens == 0) return PA_OK;
-    const Scratch s = plan_scratch(h, a->num_tokens, a->num_sequences);
+    const Scratch s = plan_scratch(h, a->num_tokens, a->num_sequences, /*rows_only=*/a->num_tokens == a->num_sequences);
     const int rc = ensure_scratch(h, s.total, stream);
     if (rc != PA_OK) return rc;
     const int G = h->g.Hq / h->g.Hkv, HK = h->g.Hkv * ((G + 15) / 16);
@@ -185,8 +189,8 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
         m.direct_tiles = (int)row_tiles;
         k.release_early = 1;
     }
-    m.part_o = (float*)(ws + s.part_o);
-    m.part_ml = (float2*)(ws + s.part_ml);
+    m.part_o = s.part_o ? (float*)(ws + s.part_o) : nullptr;
+    m.part_ml = s.part_o ? (float2*)(ws + s.part_ml) : nullptr;
     if (m.direct_tiles == 0) k.decode_all_workers = decode_launch_workers(k, h->sm_count);
     int launches = 0;
     if (a->num_rotated_blocks > 0) { MASKED_CUDA(launch_rotate(k, stream)); ++launches; }
@@ -242,7 +246,7 @@ int pa_b200_masked_reserve(pa_handle* h, int32_t num_tokens, int32_t num_sequenc
         if (num_sequences > 65535) return fail(PA_ERR_TOO_LARGE, "more than 65535 sequences in one call");
         DeviceScope scope(h->device);
         MASKED_CUDA(scope.error);
-        return ensure_scratch(h, plan_scratch(h, num_tokens, num_sequences).total, nullptr);
+        return ensure_scratch(h, plan_scratch(h, num_tokens, num_sequences, /*rows_only=*/false).total, nullptr);
     });
 }
 
