@@ -147,7 +147,7 @@ class PagedAttentionExtension:
         a mask has no `scores`."""
         sinks, parents = inputs.get("sink_tokens"), inputs.get("tree_parents")
         if sinks is not None or parents is not None:
-            self._evaluate_masked(inputs, outputs, inputs.get("sliding_window") or 0, sinks or 0, parents)
+            self._evaluate_masked(inputs, outputs, self._count("sliding_window", inputs.get("sliding_window") or 0), self._count("sink_tokens", sinks or 0), parents)
             return
         q = inputs["query"]
         host = isinstance(q, np.ndarray) or (isinstance(q, torch.Tensor) and not q.is_cuda)
@@ -168,6 +168,15 @@ class PagedAttentionExtension:
     def _refuse(self, name: str, t, expected: str):
         what = f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise self._err(f"{name}: expected {expected} on {self._where}, got {what}")
+
+    def _count(self, name: str, n) -> int:
+        try:
+            n = operator.index(n)
+        except TypeError:
+            n = -1
+        if not 0 <= n < 1 << 31:
+            raise self._err(f"{name}: expected a whole number from 0 to 2^31 - 1")
+        return n
 
     def _whole(self, name: str, t, dtype: torch.dtype, shape: tuple) -> int:
         """The address of a contiguous device tensor of this type and shape."""
