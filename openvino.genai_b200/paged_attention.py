@@ -220,8 +220,9 @@ class PagedAttentionExtension:
         scale = inputs.get("scale")
         scale = 0.0 if scale is None else float(scale)
         if isinstance(query, np.ndarray) or (isinstance(query, torch.Tensor) and not query.is_cuda):
-            if parents is not None and (parents.shape != (query.shape[0],) or str(parents.dtype).split(".")[-1] != "int32" or getattr(parents, "is_cuda", False)):
-                raise self._err("tree_parents: expected host int32 of one entry per token")
+            if parents is not None and (parents.shape != (query.shape[0],) or str(parents.dtype).split(".")[-1] != "int32" or getattr(parents, "is_cuda", False) or
+                                        not (parents.flags.c_contiguous if isinstance(parents, np.ndarray) else parents.is_contiguous())):
+                raise self._err("tree_parents: expected contiguous host int32 of one entry per token")
             args = self.make_args(query, inputs["key"], inputs["value"], outputs["output"], key_cache, value_cache, inputs["past_lens"], inputs["subsequence_begins"],
                                   inputs["block_indices"], inputs["block_indices_begins"], scale, limit, None, None, inputs.get("rotated_block_indices"),
                                   inputs.get("rotation_deltas"), inputs.get("rotation_trig_lut"), inputs.get("stream"))
