@@ -85,7 +85,7 @@ typedef struct pa_tree_accept_args {
     int32_t num_blocks;                  /* physical blocks in each cache tensor                                    */
     int32_t max_path;                    /* 1 .. PA_TREE_MAX_TOKENS: row length of `path`, the longest path taken   */
     int32_t num_layers;                  /* 0: nothing is moved                                                     */
-    void* const* key_caches;             /* [num_layers] host array of device pointers, 16-byte aligned; no cache twice */
+    void* const* key_caches;             /* [num_layers] host array of device pointers, 16-byte aligned; no two overlap */
     void* const* value_caches;
     int32_t* path;                       /* out [num_sequences][max_path] accepted tokens, ascending; -1 behind them, and everywhere
                                           * for a sequence without a tree                                           */

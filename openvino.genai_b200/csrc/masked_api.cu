@@ -271,11 +271,13 @@ int pa_b200_tree_accept(pa_handle* h, const pa_tree_accept_args* a) {
             if (!a->key_caches[i] || !a->value_caches[i]) return fail(PA_ERR_INVALID_ARG, "NULL cache pointer");
             if (!aligned(a->key_caches[i]) || !aligned(a->value_caches[i])) return fail(PA_ERR_UNSUPPORTED, "a cache is not 16-byte aligned");
         }
-        // a cache that is there twice would be moved by two blocks at once
+        // bytes that two caches share would be moved by two blocks at once
         std::vector<const void*> caches(a->key_caches, a->key_caches + a->num_layers);
         caches.insert(caches.end(), a->value_caches, a->value_caches + a->num_layers);
         std::sort(caches.begin(), caches.end(), std::less<>());
-        if (std::adjacent_find(caches.begin(), caches.end()) != caches.end()) return fail(PA_ERR_INVALID_ARG, "a cache is among the layers' twice");
+        const uintptr_t bytes = (uintptr_t)a->num_blocks * (uintptr_t)h->g.block_bytes;
+        const auto shared = std::adjacent_find(caches.begin(), caches.end(), [&](const void* x, const void* y) { return (uintptr_t)y - (uintptr_t)x < bytes; });
+        if (shared != caches.end()) return fail(PA_ERR_INVALID_ARG, shared[0] == shared[1] ? "a cache is among the layers' twice" : "two of the layers' caches overlap");
         DeviceScope scope(h->device);
         MASKED_CUDA(scope.error);
         const pa::TreeAcceptArgs t{h->g, a->tree_parents, a->draft_tokens, a->sampled_tokens, a->past_lens, a->subsequence_begins, a->block_indices,

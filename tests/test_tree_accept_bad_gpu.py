@@ -27,3 +27,24 @@ def test_a_tree_with_a_bad_parent_is_not_walked(at, bad):
     step.parents[3 + at] = trees[1][at]
     out, _, _, _, status = _run(step, draft, sampled, 4)
     assert status == 0 and out["num_accepted"].tolist() == [3, 3, 2] and out["next_token"].tolist() == [4, 99, 77]
+
+
+def test_caches_that_overlap_are_refused():
+    """A layer's caches inside another's: each would be moved by blocks of its own, at once."""
+    step = H.Step([20], [4], d=64, bs=16, trees=[[-1, 0, 0, 1]], poison=False, seed=7)
+    op, dev = step.operator(), step.dev
+    ids = torch.zeros(4, dtype=torch.int64, device=dev)
+    n, block = step.packed["key"].numel(), step.packed["key"][0].numel()
+    mk = lambda *s, t=torch.int32: torch.full(s, 99, dtype=t, device=dev)
+    out = {"path": mk(1, 4), "num_accepted": mk(1), "next_token": mk(1, t=torch.int64)}
+    memory = torch.zeros(4 * n, dtype=torch.uint8, device=dev)
+    at = lambda offset: memory[offset:offset + n]
+    good = {**step.meta, "tree_parents": step.parents, "draft_tokens": ids, "sampled_tokens": ids}
+    for keys, values in (([at(0)], [at(block)]), ([at(n - block)], [at(0)]), ([at(0), at(2 * n)], [at(n), at(3 * n - block)]), ([at(0), at(16)], [at(2 * n), at(3 * n)])):
+        with pytest.raises(H.pkg.GenaiB200Error, match="overlap"):
+            op.tree_accept({**good, "key_caches": keys, "value_caches": values}, out)
+    torch.cuda.synchronize()
+    assert all(bool((x == 99).all()) for x in out.values())
+    op.tree_accept({**good, "key_caches": [at(0), at(2 * n)], "value_caches": [at(3 * n), at(n)]}, out)      # side by side
+    torch.cuda.synchronize()
+    assert int(out["num_accepted"][0]) >= 1
