@@ -261,7 +261,7 @@ class PagedAttentionExtension:
 
         inputs: tree_parents i32 [T] (as `evaluate` takes it), draft_tokens i64 [T] (the step's input ids; a sequence's first one is
         certain), sampled_tokens i64 [T] (what was sampled behind each of them), the paged metadata, and key_caches / value_caches: a
-        sequence of the layers' caches (may be left out: nothing is moved).  From an accepted token the path goes on to its
+        sequence of the layers' caches, or a tensor of them one behind the other (may be left out: nothing is moved).  From an accepted token the path goes on to its
         first child whose id was sampled behind it.
         outputs: path i32 [B, max_path] (accepted tokens, -1 behind them), num_accepted i32 [B], next_token i64 [B] (sampled behind
         the last accepted token), new_past_lens i32 [B] (optional, may be past_lens).  A sequence without a tree keeps all its tokens."""
@@ -269,7 +269,7 @@ class PagedAttentionExtension:
         parents, path = inputs["tree_parents"], outputs["path"]
         T = parents.shape[0] if isinstance(parents, torch.Tensor) and parents.dim() else 0
         meta, B, num_indices = self._paged(inputs)
-        keys, values = inputs.get("key_caches") or (), inputs.get("value_caches") or ()
+        keys, values = (() if inputs.get(name) is None else inputs[name] for name in ("key_caches", "value_caches"))
         if len(keys) != len(values):
             raise self._err("key_caches and value_caches differ in layers")
         caches = (*keys, *values)

@@ -48,3 +48,23 @@ def test_caches_that_overlap_are_refused():
     op.tree_accept({**good, "key_caches": [at(0), at(2 * n)], "value_caches": [at(3 * n), at(n)]}, out)      # side by side
     torch.cuda.synchronize()
     assert int(out["num_accepted"][0]) >= 1
+
+
+@pytest.mark.parametrize("cache", ["f16", "u8"])
+def test_caches_of_all_layers_in_one_tensor(cache):
+    """The same as the list of them."""
+    step = H.Step([20, 9], [4, 3], d=64, bs=16, cache=cache, trees=[[-1, 0, 0, 2], [-1, 0, 0]], poison=False, seed=8)
+    op, dev = step.operator(), step.dev
+    draft, sampled = (torch.tensor(x, dtype=torch.int64, device=dev) for x in ([1, 2, 3, 4, 5, 6, 7], [3, 0, 4, 9, 7, 0, 0]))
+    res = []
+    for stacked in (False, True):
+        keys, values = (torch.stack([step.packed[k].roll(i, 0) for i in range(5)]) for k in ("key", "value"))
+        mk = lambda *s, t=torch.int32: torch.full(s, 99, dtype=t, device=dev)
+        out = {"path": mk(2, 4), "num_accepted": mk(2), "next_token": mk(2, t=torch.int64)}
+        op.tree_accept({**step.meta, "tree_parents": step.parents, "draft_tokens": draft, "sampled_tokens": sampled, "key_caches": keys if stacked else list(keys),
+                        "value_caches": values if stacked else list(values)}, out)
+        torch.cuda.synchronize()
+        assert out["path"].tolist() == [[0, 2, 3, -1], [0, 2, -1, -1]]
+        res.append((keys, values))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+    assert not torch.equal(res[0][0], torch.stack([step.packed["key"].roll(i, 0) for i in range(5)]))
