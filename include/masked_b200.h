@@ -50,6 +50,8 @@ typedef struct pa_mask_args {
  * otherwise); args->sliding_window is 0, the mask has it.  No score output (PA_ERR_UNSUPPORTED): scores are those of causal rows.  Asynchronous on
  * the stream.  The handle's scratch grows when a call needs more; inside a stream capture such a call is PA_ERR_TOO_LARGE.  Graphs name the scratch
  * of their capture, which the handle keeps until it is destroyed; replays and calls of one handle stay ordered on one stream.
+ * pa_b200_last_prefill_kernel tells of masked steps too (row by row: PA_PREFILL_GENERIC; PA_PREFILL_NONE of as many tokens as sequences), the kernel
+ * timing of pa_b200.h of causal ones only.
  * Two kinds of chunks are served row by row, far from the tensor cores' pace: those over a bf16 cache under f16 or f32 activations, and those of a step with
  * exactly as many tokens as sequences (some of them without tokens), which is taken for one of single tokens. */
 int pa_b200_forward_masked(pa_handle* h, const pa_forward_args* args, const pa_mask_args* mask);

@@ -197,7 +197,9 @@ int forward_masked(pa_handle* h, const pa_forward_args* a, const pa_mask_args& m
     MASKED_CUDA(launch_write_kv(k, stream, /*with_plan=*/true)); ++launches;
     // (always: among the tokens that no sequence has, even a step of one sequence may hold a single token)
     MASKED_CUDA(launch_decode(k, stream, h->sm_count, &launches));
+    h->last_prefill_kernel = PA_PREFILL_NONE;
     if (a->num_tokens > 1 && !m.rows_in_decode) {
+        h->last_prefill_kernel = prefill_tc_supported(h->g) ? PA_PREFILL_TCGEN05 : PA_PREFILL_GENERIC;
         if (prefill_tc_supported(h->g)) {
             if (h->g.cache != PA_DTYPE_U8) {
                 const long long size[3] = {h->g.D, h->g.bs, (long long)a->num_blocks * h->g.Hkv}, stride[2] = {h->g.D, (long long)h->g.bs * h->g.D};
