@@ -66,6 +66,11 @@ __host__ __device__ __forceinline__ uint32_t row_bits32(const MaskParams& m, con
     if (r.words && pos0 + 32 > r.past) w |= tree_bits32(r.words, pos0 - r.past);
     return w;
 }
+// The same of a row of a chunk of n tokens, none behind it: the words of a token that two sequences claim may be the other one's, and positions behind the
+// chunk have no pages.
+__host__ __device__ __forceinline__ uint32_t row_bits32(const MaskParams& m, const RowMask& r, int n, int pos0) {
+    return row_bits32(m, r, pos0) & low_bits32(r.past + n - pos0);
+}
 // The tiles that one row of a chunk of n tokens goes through.  A tree's whole chunk is among them, however far the row's window has come: its tokens are seen by
 // their positions, and an ancestor whose position is below the sinks may lie anywhere in the chunk.
 template <int T>
@@ -127,7 +132,7 @@ static __device__ __noinline__ void masked_row(const KernelArgs& a, int t, int h
     const VisTiles v = row_tiles<32>(a.m, rm, sv.n);
     for (int i = 0; i < v.count; ++i) {
         const int pos0 = 32 * v.tile(i);
-        for (uint32_t w = row_bits32(a.m, rm, pos0); w; w &= w - 1) {
+        for (uint32_t w = row_bits32(a.m, rm, sv.n, pos0); w; w &= w - 1) {
             const int pos = pos0 + __ffs(w) - 1;
             const int blk = a.block_indices[sv.tb + pos / bs];
             if (blk < 0 || blk >= a.num_blocks) {

@@ -58,7 +58,7 @@ int main() {
                 const int t = v.tile(k);
                 if (t <= last) { std::printf("tiles out of order: past %d n %d row %d W %d S %d\n", past, n, i, W, S); return 1; }
                 last = t;
-                for (uint32_t w = pa::row_bits32(m, r, 32 * t); w; w &= w - 1) {
+                for (uint32_t w = pa::row_bits32(m, r, n, 32 * t); w; w &= w - 1) {
                     const int j = 32 * t + __builtin_ctz(w);
                     if (j >= past + n || !sees[j]) { std::printf("%s: past %d n %d row %d W %d S %d takes in %d\n", is_tree ? "tree" : "chunk", past, n, i, W, S, j); return 1; }
                     sees[j] = 0;
@@ -67,6 +67,20 @@ int main() {
             for (int j = 0; j < past + n; ++j)
                 if (sees[j]) { std::printf("%s: past %d n %d row %d W %d S %d misses %d\n", is_tree ? "tree" : "chunk", past, n, i, W, S, j); return 1; }
         }
+    }
+    // words of another sequence's: no position behind the row's own chunk
+    for (int round = 0; round < 20000; ++round) {
+        const int past = pick(200), n = 2 + pick(60);
+        pa::MaskParams m{};
+        m.window = pick(2) ? 1 + pick(50) : 0;
+        m.sinks = pick(300);
+        uint32_t words[pa::kTreeWords];
+        for (uint32_t& w : words) w = rng();
+        const pa::RowMask r{past, pa::window_lo(m, past + pick(256) + 1), words, past};
+        const pa::VisTiles v = pa::row_tiles<32>(m, r, n);
+        for (int k = 0; k < v.count; ++k)
+            for (uint32_t w = pa::row_bits32(m, r, n, 32 * v.tile(k)); w; w &= w - 1)
+                if (32 * v.tile(k) + __builtin_ctz(w) >= past + n) { std::printf("past %d n %d: a position behind the chunk\n", past, n); return 1; }
     }
     if (apart == 0) { std::printf("no row was drawn that sees a sink among its chunk\n"); return 1; }
     std::printf("ok\n");

@@ -90,3 +90,26 @@ def test_a_layer_behind_a_layer_on_one_handle_and_a_stream_of_its_own():
     assert op.device_status() == 0
     for s, out in zip(steps, outs):
         s.check(out)
+
+
+@pytest.mark.parametrize("act,cache", [("f16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f16", "u8")])
+def test_trees_that_claim_each_others_tokens_are_left_to_their_own_pages(act, cache):
+    """Begins that go back: a token is the seventh of one sequence's tree and the second of another's, whose block table ends with its own tokens."""
+    step = H.Step([20], [200], d=64, bs=16, act=act, cache=cache, trees=[list(range(-1, 199))], seed=9, spare_blocks=30)
+    op, dev = step.operator(), step.dev
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)
+    pages = (20 + 200 + 15) // 16
+    good = dict(step.meta)
+    step.meta["past_lens"], step.meta["subsequence_begins"] = i32([20, 0, 26]), i32([0, 200, 5, 11])          # (the second one's tokens are less than none)
+    step.meta["block_indices"] = torch.cat([good["block_indices"][:pages], good["block_indices"][:2]])
+    step.meta["block_indices_begins"] = i32([0, pages, pages, pages + 2])
+    step.parents[5:11] = i32([-1, 0, 1, 2, 3, 4])
+    for window in (0, 7):
+        step.window = window
+        out, _, _, status = step.run(op)
+        assert status & 0x2
+    step.window, step.meta = 0, good
+    step.parents = i32(list(range(-1, 199)))
+    out, _, _, status = step.run(op)
+    assert status == 0
+    step.check(out)
