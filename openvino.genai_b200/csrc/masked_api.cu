@@ -126,6 +126,9 @@ int validate_masked(const pa_handle* h, const pa_forward_args* a, const pa_mask_
     if ((long long)a->num_tokens * h->g.Hq > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 query rows in one call");
     if ((long long)a->num_blocks * h->g.Hkv > INT_MAX) return fail(PA_ERR_TOO_LARGE, "more than 2^31 blocks of heads in one cache");
     if ((long long)a->num_block_indices * h->g.bs > INT_MAX - 4096) return fail(PA_ERR_TOO_LARGE, "more than 2^31 tokens of context in one call");
+    const int G = h->g.Hq / h->g.Hkv;   // (the decode kernel numbers the tiles of all its streams)
+    if (((long long)a->num_block_indices * h->g.bs / 32 + a->num_sequences + 1) * h->g.Hkv * ((G + 15) / 16) > INT_MAX)
+        return fail(PA_ERR_TOO_LARGE, "more than 2^31 tiles of 32 tokens of all kv heads in one call");
     return PA_OK;
 }
 
