@@ -59,7 +59,16 @@ struct Scratch {
     size_t header, tile_prefix, ptile_prefix, worker_start, stream_done, decode_o, decode_ml, tree_words, tree_depth, redo, items, item_prefix, starts, cuts, part_o, part_ml, total;
 };
 // Steps of single tokens go without a plan where a stream has few tiles (under a short window, or by its block table): the plan is a launch's chain in front
-// of a kernel that is not much longer.  Longer streams are better off in the plan's slices, which know how many tiles each has.
+// of a kernel that is not much longer.  Longer streams are better off in the plan's slices, which know how many tiles each has.  us, with | without a plan, 8 kv
+// heads of 128, L2 flushed, contexts of 9001 (a window of 1984 makes 64 tiles):
+//   window          256        1000        1984        4000        8000
+//   1 row, bf16   26 | 17     30 | 23     32 | 26     54 | 44     65 | 38
+//   32, bf16      30 | 26     52 | 46     79 | 73    118 | 114   194 | 190
+//   128, bf16     60 | 56    122 | 119   198 | 196   351 | 351   650 | 656
+//   8, u8         28 | 22     32 | 28     36 | 40     54 | 48     69 | 65
+//   32, u8        32 | 28     48 | 42     63 | 60     91 | 89    140 | 140
+//   128, u8       52 | 50     93 | 93    138 | 145   228 | 243   396 | 429
+// The line lies where many rows over a u8 cache begin to lose; single rows would gain beyond it.
 constexpr int kDirectTiles = 64;
 
 // The partial results of the tensor-core kernel's CTAs, by far the largest part (39 MB at a head size of 128), come last and are there where it is launched: not in

@@ -22,7 +22,8 @@
 // Rows under a sliding window (WIN; include/masked_b200.h): a stream's tiles are those that hold a position its row sees, the sinks' and then the
 // window's; the loader steps over the gap between them, and a stage's descriptor holds the bits of its visible tokens.  Steps of single tokens
 // under short windows go without a plan (DIRECT): every stream counts for a.m.direct_tiles tiles, the most that one can have, so that a worker finds its slice
-// by itself; and the launch overlaps the cache write, which it waits for only in front of the tile that holds the new token.
+// by itself; and the launch overlaps the cache write with that search and with what it looks up of the metadata.  Before the first tile of the cache it waits for
+// the whole of the write: a row may see other sequences' new tokens in blocks that they share.
 // HBM-bound: 2*Hkv*(D+8) bytes per context token for the u8 cache.
 #include <algorithm>
 #include <atomic>
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             return;
         }
         // The cache is read once the new tokens are written: a row may see those of other sequences over the same blocks.  (Only the tile with the row's own
-        // new token behind the wait is no faster: 16.5 and 28.7 us either way.)
+        // new token behind the wait is no faster: 16.5 and 28.7 us either way.)  The write also clears the streams' counters.
         if constexpr (DIRECT) wait_once();
         uint8_t* st = ring + slot * Cfg::STAGE;
         const int hk = r_hkp / gtiles;
@@ -813,7 +814,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             }
             continue;
         }
-        if constexpr (DIRECT) wait_once();   // (which also clears the streams' counters)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const int hrow = g + 8 * r;

@@ -92,9 +92,17 @@ struct __align__(16) MaskCut {
     int pieces[2];             // that hold tiles of each half's rows
     int pad;
 };
-constexpr int kMaskPhantom = 4;   // what a q tile costs beside its tiles, in tiles: its rows' way in and out
-constexpr int kMaskLeast = 3;     // tiles that a CTA is given at least
-constexpr int kMaskCut = 14;      // what cutting lists between CTAs costs, in tiles
+// Rules of the slices (build_mask_items), in tiles of 64 tokens; us, 148 SMs, L2 flushed.
+// kMaskPhantom: what a q tile costs beside its tiles, its rows' way in and out.  0 | 4 | 12: a prompt of 1500 tokens 100 | 70 | 70, 32 trees (u8) 324 | 289 | 289, one
+// tree 47 | 43 | 49, 16 prompts of 130 139 | 133 | 143.
+constexpr int kMaskPhantom = 4;
+// kMaskLeast: tiles that a CTA is given at least.  1 | 3 | 8: one tree 43 | 43 | 47, a prompt of 300 tokens 38 | 41 | 49, three trees over 9000 66 | 68 | 68.
+constexpr int kMaskLeast = 3;
+// kMaskCut: by how much the longest slice has to pass the even one for lists to be cut.  48 drawn prompts, trees and mixed steps, cut | uncut: 9 tiles 88 | 78, 10
+// 102 | 94, 12 82 | 80, 13 55 | 59, 14 45 | 66, 15 41 | 47, 19 107 | 113, 25 51 | 82, 33 197 | 225, 51 180 | 223; up to 14 the uncut form won or was even in 9 of 15, above it the
+// cut one won in 32 of 33.  Steps of several long lists a CTA gain by the uncut form further on (nine ragged prompts, 15 - 18 tiles, 367 | 340; three u8 prompts,
+// 27 - 32 tiles, 965 | 889): their cuts fill the scratch with whole q tiles.
+constexpr int kMaskCut = 14;
 constexpr int kMaskSnap = 2;      // a slice does not begin so near to either end of a q tile's list
 struct MaskParams {
     int on;                    // 0: causal rows, nothing else below is read
