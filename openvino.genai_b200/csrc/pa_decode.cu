@@ -180,6 +180,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
     constexpr bool U8 = Cfg::U8;
     constexpr bool BF16 = Cfg::BF16;
     constexpr bool WIN = MASK != 0, DIRECT = MASK == 2;
+    // Rows under a window over a bf16 cache: P as a high and a low piece, 1.7e-3 of the result in all (the output's own rounding) where the high piece alone leaves 2.2e-3.
+    // Up to 8 heads have the low pieces in the rows of the fragment that are zero otherwise: the same products (64 rows, W 1000: 73 us either way; 16 heads a kv
+    // head take a second product, 40 | 42).
+    constexpr bool TWO = WIN && BF16;
     constexpr int NKK = D / 16;   // k-steps of Q.K^T
     constexpr int NDT = D / 8;    // n-tiles of P.V
     constexpr int ROWS = HI ? 2 : 1;
@@ -706,6 +710,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             }
         }
         uint32_t pa_frag[2][4];
+        [[maybe_unused]] uint32_t pa_low[2][4];   // TWO: what bf16 leaves of P, of up to 8 heads in the fragment's other rows
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             float lsum = 0.f, zsum = 0.f;
@@ -722,6 +727,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
                     zsum += (live(tk) ? __low2float(h) * vzp[j][0] : 0.f) + (live(tk + 1) ? __high2float(h) * vzp[j][1] : 0.f);
                 } else if constexpr (BF16) {
                     packed = pack_bf2(p0, p1);
+                    if constexpr (TWO) {
+                        const uint32_t low = pack_bf2(p0 - __uint_as_float(packed << 16), p1 - __uint_as_float(packed & 0xffff0000u));
+                        if constexpr (HI) pa_low[j >> 1][r + 2 * (j & 1)] = low;
+                        else pa_frag[j >> 1][1 + 2 * (j & 1)] = low;
+                    }
                 } else {
                     packed = pack_h2(p0, p1);
                 }
@@ -730,7 +740,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
             l_run[r] += lsum;
             z_run[r] += zsum;
         }
-        if constexpr (!HI) { pa_frag[0][1] = pa_frag[0][3] = pa_frag[1][1] = pa_frag[1][3] = 0u; }
+        if constexpr (!HI && !TWO) { pa_frag[0][1] = pa_frag[0][3] = pa_frag[1][1] = pa_frag[1][3] = 0u; }
 
         // ---- O += P.V -----------------------------------------------------------------------------
         if constexpr (U8) {
@@ -761,7 +771,14 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, (HI || PA_DECODE_STAGES > 2
                         float acc4[4];
                         acc4[0] = oacc[i][0]; acc4[1] = oacc[i][1];
                         if constexpr (HI) { acc4[2] = oacc[i][2]; acc4[3] = oacc[i][3]; }
-                        mma16816<BF16, HI>(acc4, pa_frag[kt], b[2 * e], b[2 * e + 1]);
+                        if constexpr (TWO && !HI) {
+                            acc4[2] = 0.f; acc4[3] = 0.f;
+                            mma16816<BF16, true>(acc4, pa_frag[kt], b[2 * e], b[2 * e + 1]);
+                            acc4[0] += acc4[2]; acc4[1] += acc4[3];
+                        } else {
+                            mma16816<BF16, HI>(acc4, pa_frag[kt], b[2 * e], b[2 * e + 1]);
+                            if constexpr (TWO) mma16816<BF16, HI>(acc4, pa_low[kt], b[2 * e], b[2 * e + 1]);
+                        }
                         oacc[i][0] = acc4[0]; oacc[i][1] = acc4[1];
                         if constexpr (HI) { oacc[i][2] = acc4[2]; oacc[i][3] = acc4[3]; }
                     }

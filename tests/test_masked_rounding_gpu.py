@@ -19,3 +19,15 @@ def test_bf16_chunks_are_as_exact_as_a_causal_step(d, bs):
         ref, _ = step.reference()
         err = ((out.double() - ref).norm() / ref.norm()).item()
         assert status == 0 and err <= 2e-3, err
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (24, 2)])
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 32)])
+def test_single_tokens_over_a_bf16_cache(d, bs, hq, hkv):
+    """The same tolerance, with a plan and without one, eight heads a kv head and more."""
+    for past, window in (([700, 1500, 90, 300] * 8, 1000), ([4000, 3000, 100, 7] * 8, 3500)):
+        step = H.Step(past, [1] * len(past), hq=hq, hkv=hkv, d=d, bs=bs, act="bf16", cache="bf16", window=window, sinks=4, seed=window)
+        out, _, _, status = step.run()
+        ref, _ = step.reference()
+        err = ((out.double() - ref).norm() / ref.norm()).item()
+        assert status == 0 and err <= 2e-3, err
