@@ -13,7 +13,7 @@
  * Blocks that no row of the step sees are neither looked up nor read: their entries of block_indices may hold anything, so that a cache
  * manager may give blocks back once the window has left them behind.  Positions that a row does not see take no part in it, whatever their bytes
  * are, not-a-number and infinities included: a row of a chunk whose result is not finite is computed again by a slow path, so that a step of which
- * most rows rightly are not finite takes far longer than another.  So are the rows of chunks that see a token of a u8 cache whose step is 512 or more.
+ * most rows rightly are not finite takes far longer than another.  So are the rows of chunks that see a token of a u8 cache whose step is 511 or more.
  *
  * Conventions are those of pa_b200.h: plain C, status codes, the text of the last error of this thread from pa_b200_last_error(), a
  * device status word (PA_DEV_*) in place of faults.  The caller's current device is left as it was.

@@ -123,7 +123,7 @@ struct PrefillSmem<BS, PA_DTYPE_U8, D, MK> {
     alignas(128) uint8_t raw_v[kStages][NREC * RSTRIDE];
     alignas(128) uint8_t out_stage[kSoftmaxWarps][32 * 128];   // 128 bytes of each of a warp's rows on their way to global memory
     alignas(16) uint2 v_tab[kConvWarps][kKv / 2];  // per converter warp: (scale, -1024 * scale) f16 pairs of two tokens
-    alignas(16) uint2 tok_scale[MK ? kConvWarps : 1][MK ? kKv : 1];   // masked, per converter warp: (scale, -1152 * scale) of a token, each as a pair of equal f16
+    alignas(16) uint2 tok_scale[MK ? kConvWarps : 1][MK ? kKv : 1];   // masked, per converter warp: a token's scale as the sum of two f16, each as a pair of equal ones
     alignas(8) uint64_t raw_full[kStages];   // loader -> converter (transaction bytes)
     alignas(8) uint64_t raw_free[kStages];   // converter -> loader
     alignas(8) uint64_t k_full[kStages];     // converter -> mma
@@ -275,13 +275,18 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
                  "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
 }
-// (1024 + byte) -> (byte - 128) * scale for eight values of one scale, rounded once; sc = (scale, -1152 * scale) as f16 pairs.  `slow`: the scale may be 32
-// or more (scale16).  From the middle of the range a value loses a quarter of what it loses as byte * scale (masked u8 steps 1.0e-3 -> 6.6e-4 of the result in
-// all, f16 activations); what -1152 * scale loses in f16 is the same for every value of a token and goes with its zero-point.
-__device__ __forceinline__ void scale_pair(uint4& w4, uint2 sc, bool slow) {
+// (1024 + byte) -> (byte - 128) * scale, two values; the scales' two f16 pieces of each.  byte - 128 is exact, and the small piece's product is rounded far below the
+// sum's own rounding: 2^-12 of a value in all, from the middle of the range.  With the scale rounded to one f16 (a multiply-add for three instructions) the result is
+// 6.7e-4 off in all under f16 activations, 4.3e-4 so (u8 prompts 982 | 997 us, trees 291 | 293); integers as operands and both scales in the softmax leave
+// 3.0e-4, the roundings of P and of the output, at 1070 - 1140 | 320 - 335.
+__device__ __forceinline__ uint32_t scale_two(uint32_t w, uint32_t high, uint32_t low) {
+    const uint32_t b = hadd2_bits(w, 0xE480E480u);
+    return hfma2_bits(b, high, hmul2_bits(b, low));
+}
+__device__ __forceinline__ void scale_eight(uint4& w4, uint2 sc) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&w4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE480E480u), sc.x) : hfma2_bits(w[k], sc.x, sc.y);
+    for (int k = 0; k < 4; ++k) w[k] = scale_two(w[k], sc.x, sc.y);
 }
 // One arrival for the whole warp, after every lane's preceding writes.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -1189,7 +1194,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
         const int ctid = tid - kSoftmaxWarps * 32, cwarp = warp - kSoftmaxWarps;
         if constexpr (U8 && MK) {
             // Masked: two warps for the keys and two for the values, so that neither's waits and fences hold up the other's (one behind the other, keys and
-            // values took 2900 cycles of a tile's 3600).  All loads of a batch of units come first, and the rare large scales (scale16) are decided once.
+            // values took 2900 cycles of a tile's 3600).  All loads of a batch of units come first.
             const bool values = cwarp >= kConvWarps / 2;
             const int gt = ctid & 63;
             constexpr int NB = 4;   // units of a batch
@@ -1207,38 +1212,32 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                     if (!wait_warp(&sm.raw_full[st], use & 1, 0)) goto done;
                     // every warp has the scales of all tokens (so that none waits for another); this thread sees to the zero-point of token gt
                     uint2* const tok = sm.tok_scale[cwarp];
-                    float scale_gt = 0.f, off_gt = 0.f, zero_gt = 0.f;   // of token gt: scale, the rounded -1152 * scale, zero-point
-                    bool ok = false, big = false;
+                    float z = 0.f;   // of token gt: (byte - zp) * scale = operand - z
+                    bool ok = false;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int token = 32 * h + lane;
                         const bool live = seen(it, ctx_hi, pos0 + token);
                         const float* const par = reinterpret_cast<const float*>(raw + (token / BS) * Smem::RSTRIDE + BS * kD) + token % BS;
-                        __half scale = f2h(live ? par[0] : 0.f);   // (a token that no row sees becomes zeros)
-                        // -128 * scale leaves the f16 range from 512 on.  Of a key that would be a logit of -infinity, which hides the token as a mask does: not a
+                        const float scale = live ? par[0] : 0.f;   // (a token that no row sees becomes zeros)
+                        __half high = f2h(scale);
+                        const __half low = f2h(scale - __half2float(high));
+                        // -128 * scale leaves the f16 range just behind 511.  Of a key that would be a logit of -infinity, which hides the token as a mask does: not a
                         // number instead, so that the rows that see it are computed again in 32 bits (masked_row).
-                        if (!(fabsf(__half2float(scale)) < 512.f)) scale = __ushort_as_half(0x7FFFu);
-                        const uint32_t s2 = h2_bits(scale, scale);
-                        const uint32_t c2 = hmul2_bits(s2, 0xE480E480u);
-                        tok[token] = make_uint2(s2, c2);
-                        big |= !(fabsf(__half2float(scale)) < 32.f);
+                        if (!(fabsf(scale) < 511.f)) high = __ushort_as_half(0x7FFFu);
+                        tok[token] = make_uint2(h2_bits(high, high), h2_bits(low, low));
                         if (token == gt) {
                             ok = live;
-                            scale_gt = __half2float(scale);
-                            off_gt = __half2float(__ushort_as_half((unsigned short)(c2 & 0xffffu)));
-                            zero_gt = live ? par[BS] : 0.f;
+                            z = live ? scale * (par[BS] - 128.f) : 0.f;
                         }
                     }
-                    const bool slow = __any_sync(0xffffffffu, big);
                     const __half zero = __ushort_as_half(0);
-                    // (byte - zp) * scale = operand - z: z = (zp - 128) * scale and what the offset was rounded by (scale * 1024 + offset is exact)
-                    const float z = fmaf(scale_gt, zero_gt, slow ? -128.f * scale_gt : fmaf(scale_gt, 1024.f, off_gt));
                     __half zh, zm, zl;
                     split3(values ? z : -z, zh, zm, zl);
                     __syncwarp();
                     if (!values) {
                         if (use > 0 && !wait_warp(&sm.k_free[st], (use - 1) & 1, 1)) goto done;
-                        // K' = (byte - 128) * f16(k scale): unit = 16 dims of one token
+                        // K' = (byte - 128) * k scale: unit = 16 dims of one token
                         *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 0)) = make_uint4(h2_bits(zh, zm), h2_bits(zl, zh), h2_bits(zm, zero), 0u);
                         *reinterpret_cast<uint4*>(sm.kx[st] + plain16(gt, 1)) = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
@@ -1254,8 +1253,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
 #pragma unroll
                             for (int i = 0; i < NB; ++i) {
                                 const int u = u0 + 64 * i, token = u / (kD / 16), seg = u % (kD / 16);
-                                scale_pair(lo4[i], sc[i], slow);
-                                scale_pair(hi4[i], sc[i], slow);
+                                scale_eight(lo4[i], sc[i]);
+                                scale_eight(hi4[i], sc[i]);
                                 uint8_t* atom = sm.k[st] + (seg >> 2) * (kKv * 128);
                                 *reinterpret_cast<uint4*>(atom + sw128(token, (2 * seg) & 7)) = lo4[i];
                                 *reinterpret_cast<uint4*>(atom + sw128(token, (2 * seg + 1) & 7)) = hi4[i];
@@ -1265,9 +1264,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                         warp_arrive(&sm.k_full[st]);
                     } else {
                         if (use > 0 && !wait_warp(&sm.v_free[st], (use - 1) & 1, 2)) goto done;
-                        // V'^T = (byte - 128) * f16(v scale): unit = 16 tokens of one dim
+                        // V'^T = (byte - 128) * v scale: unit = 16 tokens of one dim
                         const int tg = gt & 3;
-                        uint2 tab[8];   // of two tokens: their scales, and -1152 times them
+                        uint2 tab[8];   // of two tokens: their scales' two pieces
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const uint4 two = *reinterpret_cast<const uint4*>(&tok[16 * tg + 2 * k]);
@@ -1285,7 +1284,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const __grid_co
                                 const int d = d0 + 16 * i;
                                 uint32_t w[8] = {lo4[i].x, lo4[i].y, lo4[i].z, lo4[i].w, hi4[i].x, hi4[i].y, hi4[i].z, hi4[i].w};
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) w[k] = slow ? hmul2_bits(hadd2_bits(w[k], 0xE480E480u), tab[k].x) : hfma2_bits(w[k], tab[k].x, tab[k].y);
+                                for (int k = 0; k < 8; ++k) w[k] = scale_two(w[k], tab[k].x, tab[k].y);
                                 *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg)) = make_uint4(w[0], w[1], w[2], w[3]);
                                 *reinterpret_cast<uint4*>(sm.vt[st] + sw128(d, 2 * tg + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
                             }
