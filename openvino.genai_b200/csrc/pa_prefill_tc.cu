@@ -278,7 +278,7 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
 // (1024 + byte) -> (byte - 128) * scale, two values; the scales' two f16 pieces of each.  byte - 128 is exact, and the small piece's product is rounded far below the
 // sum's own rounding: 2^-12 of a value in all, from the middle of the range.  With the scale rounded to one f16 (a multiply-add for three instructions) the result is
 // 6.7e-4 off in all under f16 activations, 4.3e-4 so (u8 prompts 982 | 997 us, trees 291 | 293); integers as operands and both scales in the softmax leave
-// 3.0e-4, the roundings of P and of the output, at 1070 - 1140 | 320 - 335.
+// 3.0e-4, the roundings of P and of the output, at 1137 | 335.
 __device__ __forceinline__ uint32_t scale_two(uint32_t w, uint32_t high, uint32_t low) {
     const uint32_t b = hadd2_bits(w, 0xE480E480u);
     return hfma2_bits(b, high, hmul2_bits(b, low));
